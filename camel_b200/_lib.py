@@ -23,6 +23,8 @@ ADD, SUB, MUL, DIV, POW = range(5)
 LT, LE, GT, GE, EQ = range(5)
 # ct_activation
 ACT_NONE, ACT_RELU, ACT_SOFTMAX = 0, 1, 2
+# ct_gate
+GATE_SIGMOID, GATE_RELU, GATE_SILU, GATE_GELU = range(4)
 # ct_precision
 PREC_3XTF32, PREC_BF16 = 0, 1
 
@@ -100,6 +102,12 @@ PROTOTYPES = {
     "ct_matmul_packed_bands": (_int, [_vp, _vp, _int, C.POINTER(_i64), C.POINTER(_vp), _vp, C.POINTER(C.c_uint32)]),
     "ct_stream_wait_value": (_int, [_vp, C.c_uint32]),
     "ct_dense_packed": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp]),
+    "ct_layer_norm": (_int, [_vp, _vp, _vp, _i64, _i64, _dbl, _vp]),
+    "ct_layer_norm_grad": (_int, [_vp, _vp, _vp, _i64, _i64, _dbl, _vp, _vp, _vp]),
+    "ct_dense_gated": (_int, [_vp] * 5 + [_i64] * 3 + [_int, _vp, _vp, _vp]),
+    "ct_dense_gated_grad": (_int, [_vp] * 6 + [_i64] * 3 + [_int] + [_vp] * 5),
+    "ct_dense_cross_entropy": (_int, [_vp] * 4 + [_i64] * 3 + [_vp, _vp]),
+    "ct_dense_cross_entropy_grad": (_int, [_vp] * 6 + [_i64] * 3 + [_vp, _vp, _vp]),
     "ct_conv2d": (_int, [_vp, _vp, _vp] + [_i64] * 9 + [_int, _vp]),
     "ct_conv2d_maxpool2": (_int, [_vp, _vp, _vp] + [_i64] * 9 + [_int, _vp]),
     "ct_maxpool2d": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _vp]),

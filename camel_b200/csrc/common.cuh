@@ -173,6 +173,29 @@ class ProfScope {
     cudaEvent_t e0_, e1_;
 };
 
+// Device memory of one call, allocated and freed in the order of the stream that the call began on: calls on other streams and recorded
+// sequences have their own.
+class Scratch {
+  public:
+    Scratch() : stream_(stream()) {}
+    ~Scratch() {
+        if (ptr_)
+            cudaFreeAsync(ptr_, stream_);
+    }
+    Scratch(const Scratch &)            = delete;
+    Scratch &operator=(const Scratch &) = delete;
+    ct_status get(size_t bytes) {
+        CT_CUDA(cudaMallocAsync(&ptr_, bytes > 0 ? bytes : 1, stream_));
+        return CT_OK;
+    }
+    template <typename T> T *as(size_t offset = 0) const { return reinterpret_cast<T *>(static_cast<uint8_t *>(ptr_) + offset); }
+    explicit operator bool() const { return ptr_ != nullptr; }
+
+  private:
+    void *ptr_ = nullptr;
+    cudaStream_t stream_;
+};
+
 inline size_t dtype_size(int dt) { return dt == CT_F32 ? 4 : (dt == CT_I64 ? 8 : 1); }
 inline bool valid_dtype(int dt) { return dt == CT_F32 || dt == CT_I64 || dt == CT_BOOL; }
 

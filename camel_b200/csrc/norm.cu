@@ -1,0 +1,500 @@
+// Layer norm over the rows of a matrix, and its gradient.
+//
+//   mean = sum(x) / C,  var = sum((x - mean)^2) / C,  r = 1 / sqrt(var + eps),  h = (x - mean) r,  y = h gamma + beta
+//   g = dy gamma,  dx = r (g - mean(g) - h mean(g h)),  dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
+//
+// Both are bound by memory (8 and 12 bytes a value) if a row is read once, so a row stays in the registers of the threads that
+// share it from the load to the store: a warp for short rows, a block for longer ones, and only rows of more than 32768
+// values (16384 on the way back) are read again, from L2.
+//
+// Sums are float32, each of at most a few dozen values before it meets the others in a tree.  The mean is taken twice: the sums
+// of d = x - m and of d^2, about the first mean m, come from one exchange, and what d leaves of a mean corrects m and the
+// variance.  Rows whose mean is large beside their spread keep the digits that float32 has of x - mean.
+// The gradient takes them again from x, which it has in registers anyway, instead of reading them: one exchange more per row,
+// no statistics to keep.
+#include "common.cuh"
+
+#include <algorithm>
+
+namespace ct {
+namespace {
+
+// Values of a row that a thread of TPR holds, in groups of four: group j is columns 4 (j TPR + t) .. of aligned rows (VEC), and
+// of others columns (4 j + q) TPR + t, which neighbours read together at any alignment.
+template <int TPR, int V, bool VEC> struct Row {
+    __device__ static __forceinline__ int64_t column(int t, int j, int q) {
+        return VEC ? (int64_t)(j * TPR + t) * 4 + q : (int64_t)(j * 4 + q) * TPR + t;
+    }
+    __device__ static __forceinline__ void load(float (&v)[4 * V], const float *__restrict__ src, int64_t cols, int t) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (VEC) {
+                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (column(t, j, 0) < cols)
+                    f = *reinterpret_cast<const float4 *>(src + column(t, j, 0));
+                v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    v[4 * j + q] = column(t, j, q) < cols ? src[column(t, j, q)] : 0.0f;
+            }
+    }
+    __device__ static __forceinline__ void store(float *__restrict__ dst, const float (&v)[4 * V], int64_t cols, int t) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (VEC) {
+                if (column(t, j, 0) < cols)
+                    __stcs(reinterpret_cast<float4 *>(dst + column(t, j, 0)), make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (column(t, j, q) < cols)
+                        __stcs(dst + column(t, j, q), v[4 * j + q]);
+            }
+    }
+};
+
+// The sums of N values over the TPR threads of a row; all threads of the block call it.  Two calls in turn need words of their own: a
+// warp that is through the second call's barrier has seen every warp through the first.
+template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&s)[N], float (&words)[N][32]) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            s[i] = __fadd_rn(s[i], __shfl_xor_sync(0xffffffffu, s[i], o));
+    if (TPR > 32) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                words[i][warp] = s[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[i] = lane < TPR / 32 ? words[i][lane] : 0.0f;
+#pragma unroll
+            for (int o = TPR / 64; o; o >>= 1)
+                s[i] = __fadd_rn(s[i], __shfl_xor_sync(0xffffffffu, s[i], o));
+            if (TPR < 1024)
+                s[i] = __shfl_sync(0xffffffffu, s[i], 0);
+        }
+    }
+}
+
+// 1 / sqrt(var + eps) from the sums of d and d^2, and what d lacks of the mean.
+__device__ __forceinline__ float spread(float sum_d, float sum_dd, float inv_cols, float eps, float &rest) {
+    rest            = __fmul_rn(sum_d, inv_cols);
+    const float var = __fsub_rn(__fmul_rn(sum_dd, inv_cols), __fmul_rn(rest, rest));
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(var < 0.0f ? 0.0f : var, eps)));
+}
+
+template <int TPR> constexpr int kBlock = TPR < 256 ? 256 : TPR;
+
+template <int TPR, int V, bool VEC>
+__global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
+    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t rows, int64_t cols, float eps,
+    float *__restrict__ out) {
+    using R = Row<TPR, V, VEC>;
+    __shared__ float words1[1][32], words2[2][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t       = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR;
+    if (row >= rows) // whole warps
+        return;
+    const float inv_cols = __fdiv_rn(1.0f, (float)cols);
+    float v[4 * V];
+    R::load(v, x + row * cols, cols, t);
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i)
+        sum[0] = __fadd_rn(sum[0], v[i]);
+    row_sums<TPR>(sum, words1);
+    const float mean = __fmul_rn(sum[0], inv_cols);
+    float s[2]       = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float d = R::column(t, j, q) < cols ? __fsub_rn(v[4 * j + q], mean) : 0.0f;
+            v[4 * j + q]  = d;
+            s[0]          = __fadd_rn(s[0], d);
+            s[1]          = __fmaf_rn(d, d, s[1]);
+        }
+    row_sums<TPR>(s, words2);
+    float rest;
+    const float r = spread(s[0], s[1], inv_cols, eps, rest);
+    float g[4 * V], b[4 * V];
+    if (gamma)
+        R::load(g, gamma, cols, t);
+    if (beta)
+        R::load(b, beta, cols, t);
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) {
+        float y = __fmul_rn(__fsub_rn(v[i], rest), r);
+        if (gamma)
+            y = __fmul_rn(y, g[i]);
+        if (beta)
+            y = __fadd_rn(y, b[i]);
+        v[i] = y;
+    }
+    R::store(out + row * cols, v, cols, t);
+}
+
+// Rows of any length, a block to a row, which is read three times.
+__global__ void __launch_bounds__(1024) layer_norm_long_kernel(
+    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t cols, float eps, float *__restrict__ out) {
+    __shared__ float words1[1][32], words2[2][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const float *src     = x + (int64_t)blockIdx.x * cols;
+    const float inv_cols = __fdiv_rn(1.0f, (float)cols);
+    float sum[1]         = {0.0f};
+    for (int64_t c = threadIdx.x; c < cols; c += 1024)
+        sum[0] = __fadd_rn(sum[0], src[c]);
+    row_sums<1024>(sum, words1);
+    const float mean = __fmul_rn(sum[0], inv_cols);
+    float s[2]       = {0.0f, 0.0f};
+    for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+        const float d = __fsub_rn(src[c], mean);
+        s[0]          = __fadd_rn(s[0], d);
+        s[1]          = __fmaf_rn(d, d, s[1]);
+    }
+    row_sums<1024>(s, words2);
+    float rest;
+    const float r = spread(s[0], s[1], inv_cols, eps, rest);
+    for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+        float y = __fmul_rn(__fsub_rn(__fsub_rn(src[c], mean), rest), r);
+        if (gamma)
+            y = __fmul_rn(y, gamma[c]);
+        if (beta)
+            y = __fadd_rn(y, beta[c]);
+        out[(int64_t)blockIdx.x * cols + c] = y;
+    }
+}
+
+// The gradient.  A block walks rows; a thread has the same columns of each, and keeps their sums over the block's rows, which
+// go to partial[block][2][cols] (dgamma, dbeta) for norm_columns_kernel.
+template <int TPR, int V, bool VEC>
+__global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
+    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t rows, int64_t cols, float eps,
+    float *__restrict__ dx, float *__restrict__ partial) {
+    using R          = Row<TPR, V, VEC>;
+    constexpr int RPB = kBlock<TPR> / TPR;
+    __shared__ float words1[1][32], words2[4][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t          = threadIdx.x % TPR;
+    const float inv_cols = __fdiv_rn(1.0f, (float)cols);
+    float gm[4 * V], sum_g[4 * V], sum_b[4 * V];
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i)
+        gm[i] = 1.0f, sum_g[i] = sum_b[i] = 0.0f;
+    if (gamma)
+        R::load(gm, gamma, cols, t);
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < rows; row += (int64_t)gridDim.x * RPB) {
+        float v[4 * V], dy[4 * V];
+        R::load(v, x + row * cols, cols, t);
+        R::load(dy, dout + row * cols, cols, t);
+        float sum[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < 4 * V; ++i)
+            sum[0] = __fadd_rn(sum[0], v[i]);
+        row_sums<TPR>(sum, words1);
+        const float mean = __fmul_rn(sum[0], inv_cols);
+        float s[4]       = {0.0f, 0.0f, 0.0f, 0.0f}; // of d, d^2, g, g d
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i   = 4 * j + q;
+                const float d = R::column(t, j, q) < cols ? __fsub_rn(v[i], mean) : 0.0f;
+                const float g = __fmul_rn(dy[i], gm[i]);
+                v[i]          = d;
+                s[0]          = __fadd_rn(s[0], d);
+                s[1]          = __fmaf_rn(d, d, s[1]);
+                s[2]          = __fadd_rn(s[2], g);
+                s[3]          = __fmaf_rn(g, d, s[3]);
+            }
+        row_sums<TPR>(s, words2);
+        float rest;
+        const float r  = spread(s[0], s[1], inv_cols, eps, rest);
+        const float mg = __fmul_rn(s[2], inv_cols);                                                            // mean of g
+        const float mh = __fmul_rn(__fmul_rn(__fsub_rn(s[3], __fmul_rn(rest, s[2])), r), inv_cols); // mean of g h
+#pragma unroll
+        for (int i = 0; i < 4 * V; ++i) {
+            const float h = __fmul_rn(__fsub_rn(v[i], rest), r);
+            sum_g[i]      = __fmaf_rn(dy[i], h, sum_g[i]);
+            sum_b[i]      = __fadd_rn(sum_b[i], dy[i]);
+            v[i]          = __fmul_rn(r, __fsub_rn(__fsub_rn(__fmul_rn(dy[i], gm[i]), mg), __fmul_rn(h, mh)));
+        }
+        if (dx)
+            R::store(dx + row * cols, v, cols, t);
+    }
+    if (!partial)
+        return;
+    if (RPB > 1) { // the groups of the block, one after the other
+        extern __shared__ float sums[]; // [2][cols]
+        for (int group = 0; group < RPB; ++group) {
+            if ((int)threadIdx.x / TPR == group)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int64_t c = R::column(t, j, q);
+                        if (c < cols) {
+                            sums[c]        = group ? __fadd_rn(sums[c], sum_g[4 * j + q]) : sum_g[4 * j + q];
+                            sums[cols + c] = group ? __fadd_rn(sums[cols + c], sum_b[4 * j + q]) : sum_b[4 * j + q];
+                        }
+                    }
+            __syncthreads();
+        }
+        for (int64_t c = threadIdx.x; c < 2 * cols; c += kBlock<TPR>)
+            partial[(int64_t)blockIdx.x * 2 * cols + c] = sums[c];
+    } else {
+        R::store(partial + (int64_t)blockIdx.x * 2 * cols, sum_g, cols, t);
+        float *to = partial + ((int64_t)blockIdx.x * 2 + 1) * cols;
+        if (VEC) // cols is a multiple of four: aligned like the first half
+            R::store(to, sum_b, cols, t);
+        else
+            Row<TPR, V, false>::store(to, sum_b, cols, t);
+    }
+}
+
+// Longer rows: the statistics and dx, a block to a row, then the columns' sums from both matrices again.
+__global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(
+    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t cols, float eps, float *__restrict__ dx,
+    float2 *__restrict__ stats) {
+    __shared__ float words1[1][32], words2[4][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t row    = blockIdx.x;
+    const float *src     = x + row * cols, *dy = dout + row * cols;
+    const float inv_cols = __fdiv_rn(1.0f, (float)cols);
+    float sum[1]         = {0.0f};
+    for (int64_t c = threadIdx.x; c < cols; c += 1024)
+        sum[0] = __fadd_rn(sum[0], src[c]);
+    row_sums<1024>(sum, words1);
+    const float mean = __fmul_rn(sum[0], inv_cols);
+    float s[4]       = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+        const float d = __fsub_rn(src[c], mean), g = gamma ? __fmul_rn(dy[c], gamma[c]) : dy[c];
+        s[0] = __fadd_rn(s[0], d);
+        s[1] = __fmaf_rn(d, d, s[1]);
+        s[2] = __fadd_rn(s[2], g);
+        s[3] = __fmaf_rn(g, d, s[3]);
+    }
+    row_sums<1024>(s, words2);
+    float rest;
+    const float r  = spread(s[0], s[1], inv_cols, eps, rest);
+    const float mg = __fmul_rn(s[2], inv_cols);
+    const float mh = __fmul_rn(__fmul_rn(__fsub_rn(s[3], __fmul_rn(rest, s[2])), r), inv_cols);
+    if (stats && threadIdx.x == 0) // two numbers: their sum would be rounded to float32
+        stats[2 * row] = make_float2(mean, rest), stats[2 * row + 1] = make_float2(r, 0.0f);
+    if (dx)
+        for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+            const float g = gamma ? __fmul_rn(dy[c], gamma[c]) : dy[c];
+            const float h = __fmul_rn(__fsub_rn(__fsub_rn(src[c], mean), rest), r);
+            dx[row * cols + c] = __fmul_rn(r, __fsub_rn(__fsub_rn(g, mg), __fmul_rn(h, mh)));
+        }
+}
+
+__global__ void __launch_bounds__(256) layer_norm_grad_long_columns_kernel(
+    const float *__restrict__ x, const float *__restrict__ dout, const float2 *__restrict__ stats, int64_t rows, int64_t cols, int64_t rows_each,
+    float *__restrict__ partial) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols)
+        return;
+    const int64_t r1 = min(rows, ((int64_t)blockIdx.y + 1) * rows_each);
+    float sum_g = 0.0f, sum_b = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.y * rows_each; r < r1; ++r) {
+        const float2 m = stats[2 * r], q = stats[2 * r + 1];
+        const float dy = dout[r * cols + c];
+        sum_g = __fmaf_rn(dy, __fmul_rn(__fsub_rn(__fsub_rn(x[r * cols + c], m.x), m.y), q.x), sum_g);
+        sum_b = __fadd_rn(sum_b, dy);
+    }
+    partial[(int64_t)blockIdx.y * 2 * cols + c]        = sum_g;
+    partial[((int64_t)blockIdx.y * 2 + 1) * cols + c] = sum_b;
+}
+
+// out0[c] = sum over `parts` of partial[part][c], out1[c] of partial[part][cols + c]: 32 columns to a block, a warp takes every eighth part.
+__global__ void __launch_bounds__(256) norm_columns_kernel(
+    const float *__restrict__ partial, int parts, int64_t cols, float *__restrict__ out0, float *__restrict__ out1) {
+    __shared__ double sums[8][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    double s        = 0.0;
+    if (c < 2 * cols)
+#pragma unroll 8
+        for (int p = warp; p < parts; p += 8)
+            s += (double)partial[(int64_t)p * 2 * cols + c];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < 2 * cols) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w)
+            s += sums[w][lane];
+        float *out = c < cols ? out0 : out1;
+        if (out)
+            out[c < cols ? c : c - cols] = (float)s;
+    }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int TPR, int V>
+ct_status launch_norm(const float *x, const float *gamma, const float *beta, int64_t rows, int64_t cols, float eps, float *out, bool vec) {
+    constexpr int RPB   = kBlock<TPR> / TPR;
+    const dim3 grid((unsigned)((rows + RPB - 1) / RPB));
+    if (vec)
+        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, true>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out));
+    else
+        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, false>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out));
+    CT_LAUNCH_CHECK("layer_norm");
+    return CT_OK;
+}
+
+// How many blocks the gradient runs, each with a part of the columns' sums.
+template <int TPR, int V> int64_t grad_blocks(const DeviceState *st, int64_t rows) {
+    constexpr int RPB = kBlock<TPR> / TPR;
+    return std::min<int64_t>((rows + RPB - 1) / RPB, (int64_t)st->sm_count * (1024 / kBlock<TPR>));
+}
+
+template <int TPR, int V>
+ct_status launch_norm_grad(
+    const float *x, const float *gamma, const float *dout, int64_t rows, int64_t cols, float eps, float *dx, float *partial, int64_t blocks, bool vec) {
+    const size_t smem = kBlock<TPR> > TPR && partial ? (size_t)cols * 8 : 0;
+    if (vec)
+        CT_CUDA(launch_dependent(layer_norm_grad_kernel<TPR, V, true>, dim3((unsigned)blocks), dim3(kBlock<TPR>), smem, stream(), x, gamma, dout, rows,
+                                 cols, eps, dx, partial));
+    else
+        CT_CUDA(launch_dependent(layer_norm_grad_kernel<TPR, V, false>, dim3((unsigned)blocks), dim3(kBlock<TPR>), smem, stream(), x, gamma, dout, rows,
+                                 cols, eps, dx, partial));
+    CT_LAUNCH_CHECK("layer_norm_grad");
+    return CT_OK;
+}
+
+ct_status check_norm(const char *name, const void *x, const void *second, int64_t rows, int64_t cols, double eps) {
+    if (rows < 0 || cols < 0)
+        return fail(CT_ERR_INVALID, "%s: negative dimension", name);
+    if (!(eps >= 0.0))
+        return fail(CT_ERR_INVALID, "%s: eps must not be negative", name);
+    if (rows > 0x7fffffff || cols > 0x7fffffff)
+        return fail(CT_ERR_TOO_LARGE, "%s: dimension too large", name);
+    if (rows > 0 && cols > 0 && (!x || !second))
+        return fail(CT_ERR_INVALID, "%s: null pointer", name);
+    return CT_OK;
+}
+
+} // namespace
+} // namespace ct
+
+using namespace ct;
+
+extern "C" {
+
+ct_status ct_layer_norm(
+    const float *x, const float *gamma, const float *beta, int64_t rows, int64_t cols, double eps, float *out) {
+    OpLock op_lock;
+    DeviceState *st;
+    CT_TRY(current(&st));
+    CT_TRY(check_norm("layer_norm", x, out, rows, cols, eps));
+    if (rows == 0 || cols == 0)
+        return CT_OK;
+    ProfScope prof("layer_norm");
+    const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(out) && (!gamma || aligned16(gamma)) && (!beta || aligned16(beta));
+    const float e  = (float)eps;
+    const bool few = rows < st->sm_count * 4;
+    if (cols <= 256)
+        return launch_norm<32, 2>(x, gamma, beta, rows, cols, e, out, vec);
+    if (cols <= 1024)
+        return few ? launch_norm<256, 1>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<32, 8>(x, gamma, beta, rows, cols, e, out, vec);
+    if (cols <= 4096)
+        return few ? launch_norm<1024, 1>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<256, 4>(x, gamma, beta, rows, cols, e, out, vec);
+    if (cols <= 8192)
+        return few ? launch_norm<1024, 2>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<512, 4>(x, gamma, beta, rows, cols, e, out, vec);
+    if (cols <= 16384)
+        return launch_norm<1024, 4>(x, gamma, beta, rows, cols, e, out, vec);
+    if (cols <= 32768)
+        return launch_norm<1024, 8>(x, gamma, beta, rows, cols, e, out, vec);
+    CT_CUDA(launch_dependent(layer_norm_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out));
+    CT_LAUNCH_CHECK("layer_norm_long");
+    return CT_OK;
+}
+
+ct_status ct_layer_norm_grad(
+    const float *x, const float *gamma, const float *dout, int64_t rows, int64_t cols, double eps, float *dx, float *dgamma, float *dbeta) {
+    OpLock op_lock;
+    DeviceState *st;
+    CT_TRY(current(&st));
+    CT_TRY(check_norm("layer_norm_grad", x, dout, rows, cols, eps));
+    if (cols == 0)
+        return CT_OK;
+    if (rows == 0) { // sums of nothing
+        if (dgamma)
+            CT_CUDA(cudaMemsetAsync(dgamma, 0, (size_t)cols * 4, stream()));
+        if (dbeta)
+            CT_CUDA(cudaMemsetAsync(dbeta, 0, (size_t)cols * 4, stream()));
+        return CT_OK;
+    }
+    ProfScope prof("layer_norm_grad");
+    const float e   = (float)eps;
+    const bool sums = dgamma || dbeta;
+    Scratch scratch;
+    int64_t parts = 0;
+    if (cols <= 8192) {
+        const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(dout) && (!dx || aligned16(dx)) && (!gamma || aligned16(gamma));
+#define CT_NORM_GRAD(TPR, V)                                                                                                           \
+    do {                                                                                                                               \
+        parts = grad_blocks<TPR, V>(st, rows);                                                                                         \
+        if (sums)                                                                                                                      \
+            CT_TRY(scratch.get((size_t)parts * 8 * cols));                                                                             \
+        CT_TRY((launch_norm_grad<TPR, V>(x, gamma, dout, rows, cols, e, dx, sums ? scratch.as<float>() : nullptr, parts, vec)));          \
+    } while (0)
+        if (cols <= 256)
+            CT_NORM_GRAD(32, 2);
+        else if (cols <= 1024)
+            CT_NORM_GRAD(256, 1);
+        else if (cols <= 2048)
+            CT_NORM_GRAD(256, 2);
+        else if (cols <= 4096)
+            CT_NORM_GRAD(512, 2);
+        else
+            CT_NORM_GRAD(1024, 2);
+#undef CT_NORM_GRAD
+    } else {
+        const int64_t strips = (cols + 255) / 256;
+        const int64_t each   = std::max<int64_t>(8, (rows * strips + st->sm_count * 8 - 1) / (st->sm_count * 8));
+        parts                = (rows + each - 1) / each;
+        if (parts > 65535)
+            return fail(CT_ERR_TOO_LARGE, "layer_norm_grad: too many rows");
+        const size_t stats_bytes = ((size_t)rows * 16 + 255) & ~(size_t)255;
+        if (sums)
+            CT_TRY(scratch.get(stats_bytes + (size_t)parts * 8 * cols));
+        float2 *stats  = sums ? scratch.as<float2>() : nullptr;
+        float *partial = sums ? scratch.as<float>(stats_bytes) : nullptr;
+        CT_CUDA(launch_dependent(layer_norm_grad_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx, stats));
+        CT_LAUNCH_CHECK("layer_norm_grad_long");
+        if (sums) {
+            CT_CUDA(launch_dependent(layer_norm_grad_long_columns_kernel, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), x, dout,
+                                     static_cast<const float2 *>(stats), rows, cols, each, partial));
+            CT_LAUNCH_CHECK("layer_norm_grad_long_columns");
+            CT_CUDA(launch_dependent(norm_columns_kernel, dim3((unsigned)((2 * cols + 31) / 32)), dim3(256), 0, stream(),
+                                     static_cast<const float *>(partial), (int)parts, cols, dgamma, dbeta));
+            CT_LAUNCH_CHECK("norm_columns");
+        }
+        return CT_OK;
+    }
+    if (sums) {
+        CT_CUDA(launch_dependent(norm_columns_kernel, dim3((unsigned)((2 * cols + 31) / 32)), dim3(256), 0, stream(),
+                                 scratch.as<const float>(), (int)parts, cols, dgamma, dbeta));
+        CT_LAUNCH_CHECK("norm_columns");
+    }
+    return CT_OK;
+}
+
+} // extern "C"

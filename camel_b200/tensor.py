@@ -582,6 +582,125 @@ def flatten(x: Tensor) -> Tensor:
     return reshape(x, (x.shape[0], rest))
 
 
+# ---- layers of deeper networks and their gradients ------------------------------------------
+
+
+def _float_matrix(t: Tensor, name: str, rows: int | None = None, cols: int | None = None) -> None:
+    if not _is_tensor(t):
+        raise _invalid("Expected Tensor argument")
+    _require_float(t, name)
+    if t.rank != 2:
+        raise _invalid(f"{name} currently only supports rank-2 tensors")
+    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise _invalid(f"{name} dimension mismatch")
+
+
+def _float_values(t: Tensor | None, name: str, what: str, count: int):
+    """Device pointer of an optional vector of `count` floats."""
+    if t is None:
+        return None
+    if not _is_tensor(t) or t.dtype != L.F32 or t.numel != count:
+        raise _invalid(f"{name}: {what} must be a float tensor of {count} values")
+    return t.ptr
+
+
+def layer_norm(t: Tensor, gamma: Tensor | None = None, beta: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """(t - mean) / sqrt(var + eps) * gamma + beta over each row of a rank-2 tensor."""
+    _float_matrix(t, "layer_norm")
+    rows, cols = t.shape
+    out = Tensor(L.F32, t.shape)
+    check(lib.ct_layer_norm(t.ptr, _float_values(gamma, "layer_norm", "gamma", cols), _float_values(beta, "layer_norm", "beta", cols),
+                            rows, cols, float(eps), out.ptr))
+    return out
+
+
+def layer_norm_grad(x: Tensor, dout: Tensor, gamma: Tensor | None = None, eps: float = 1e-5):
+    """(dx, dgamma, dbeta) of layer_norm from its input and the gradient of its output."""
+    _float_matrix(x, "layer_norm_grad")
+    rows, cols = x.shape
+    _float_matrix(dout, "layer_norm_grad", rows, cols)
+    g = _float_values(gamma, "layer_norm_grad", "gamma", cols)
+    dx, dgamma, dbeta = Tensor(L.F32, x.shape), Tensor(L.F32, (cols,)), Tensor(L.F32, (cols,))
+    check(lib.ct_layer_norm_grad(x.ptr, g, dout.ptr, rows, cols, float(eps), dx.ptr, dgamma.ptr, dbeta.ptr))
+    return dx, dgamma, dbeta
+
+
+_GATE = {"sigmoid": L.GATE_SIGMOID, "relu": L.GATE_RELU, "silu": L.GATE_SILU, "gelu": L.GATE_GELU}
+
+
+def _gate_arg(name: str, gate: str) -> int:
+    if gate not in _GATE:
+        raise _invalid(f"{name}: unknown gate")
+    return _GATE[gate]
+
+
+def dense_gated(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Tensor | None = None, b_up: Tensor | None = None, gate: str = "silu",
+                keep: bool = False):
+    """gate(x @ w_gate + b_gate) * (x @ w_up + b_up) in one contraction; with keep also the two sums, which the gradient needs:
+    (out, gate_pre, up_pre)."""
+    _float_matrix(x, "dense_gated")
+    m, k = x.shape
+    _float_matrix(w_gate, "dense_gated", k)
+    n = w_gate.shape[1]
+    _float_matrix(w_up, "dense_gated", k, n)
+    kind = _gate_arg("dense_gated", gate)
+    bg, bu = _float_values(b_gate, "dense_gated", "b_gate", n), _float_values(b_up, "dense_gated", "b_up", n)
+    out = Tensor(L.F32, (m, n))
+    kept = (Tensor(L.F32, (m, n)), Tensor(L.F32, (m, n))) if keep else None
+    check(lib.ct_dense_gated(x.ptr, w_gate.ptr, bg, w_up.ptr, bu, m, k, n, kind, out.ptr, kept[0].ptr if kept else None,
+                             kept[1].ptr if kept else None))
+    return (out, *kept) if kept else out
+
+
+def dense_gated_grad(x: Tensor, w_gate: Tensor, w_up: Tensor, gate_pre: Tensor, up_pre: Tensor, dout: Tensor, gate: str = "silu",
+                     bias: bool = False):
+    """(dx, dw_gate, dw_up) of dense_gated from what it kept and the gradient of its output; with bias also db_gate and db_up."""
+    _float_matrix(x, "dense_gated_grad")
+    m, k = x.shape
+    _float_matrix(w_gate, "dense_gated_grad", k)
+    n = w_gate.shape[1]
+    _float_matrix(w_up, "dense_gated_grad", k, n)
+    for t in (gate_pre, up_pre, dout):
+        _float_matrix(t, "dense_gated_grad", m, n)
+    kind = _gate_arg("dense_gated_grad", gate)
+    dx, dwg, dwu = Tensor(L.F32, (m, k)), Tensor(L.F32, (k, n)), Tensor(L.F32, (k, n))
+    db = (Tensor(L.F32, (n,)), Tensor(L.F32, (n,))) if bias else ()
+    check(lib.ct_dense_gated_grad(x.ptr, w_gate.ptr, w_up.ptr, gate_pre.ptr, up_pre.ptr, dout.ptr, m, k, n, kind, dx.ptr, dwg.ptr, dwu.ptr,
+                                  db[0].ptr if bias else None, db[1].ptr if bias else None))
+    return (dx, dwg, dwu, *db)
+
+
+def _ce_args(name: str, x: Tensor, w: Tensor, targets: Tensor, b: Tensor | None):
+    _float_matrix(x, name)
+    m, k = x.shape
+    _float_matrix(w, name, k)
+    n = w.shape[1]
+    if not _is_tensor(targets) or targets.dtype != L.I64 or targets.shape != (m,):
+        raise _invalid(f"{name}: targets must be an int tensor with one class per row")
+    return m, k, n, _float_values(b, name, "bias", n)
+
+
+def dense_cross_entropy(x: Tensor, w: Tensor, targets: Tensor, b: Tensor | None = None):
+    """(loss, lse) of each row of the logits x @ w + b, which are not kept: lse = log(sum(exp(logits))), loss = lse - logits[target];
+    a target outside the classes (-1, say) marks a row without one, whose loss is 0."""
+    m, k, n, bias = _ce_args("dense_cross_entropy", x, w, targets, b)
+    loss, lse = Tensor(L.F32, (m,)), Tensor(L.F32, (m,))
+    check(lib.ct_dense_cross_entropy(x.ptr, w.ptr, bias, targets.ptr, m, k, n, loss.ptr, lse.ptr))
+    return loss, lse
+
+
+def dense_cross_entropy_grad(x: Tensor, w: Tensor, targets: Tensor, lse: Tensor, b: Tensor | None = None, dloss: Tensor | None = None):
+    """(dx, dw) of the sum of dense_cross_entropy's losses, weighted by dloss where it is given; with b also db."""
+    m, k, n, bias = _ce_args("dense_cross_entropy_grad", x, w, targets, b)
+    if lse is None:
+        raise _invalid("Expected Tensor argument")
+    plse, pd = _float_values(lse, "dense_cross_entropy_grad", "lse", m), _float_values(dloss, "dense_cross_entropy_grad", "dloss", m)
+    dx, dw = Tensor(L.F32, (m, k)), Tensor(L.F32, (k, n))
+    db = (Tensor(L.F32, (n,)),) if b is not None else ()
+    check(lib.ct_dense_cross_entropy_grad(x.ptr, w.ptr, bias, targets.ptr, plse, pd, m, k, n, dx.ptr, dw.ptr, db[0].ptr if db else None))
+    return (dx, dw, *db)
+
+
 class Graph:
     """Records the operator calls made inside `with Graph() as g:` and replays them with
     `g.launch()` (one CUDA-graph launch).  Tensors created inside the block and still referenced

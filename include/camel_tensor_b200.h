@@ -65,6 +65,14 @@ typedef enum ct_activation {
     CT_ACT_SOFTMAX = 2  /* row softmax of test/run/nn/mnist.cml:13-25 (dense only) */
 } ct_activation;
 
+/* What the gate of a gated dense layer goes through. */
+typedef enum ct_gate {
+    CT_GATE_SIGMOID = 0, /* 1 / (1 + exp(-x)) */
+    CT_GATE_RELU    = 1, /* x * (x > 0) */
+    CT_GATE_SILU    = 2, /* x / (1 + exp(-x)) */
+    CT_GATE_GELU    = 3  /* x * Phi(x), Phi the normal distribution function (not its tanh form) */
+} ct_gate;
+
 /* Arithmetic of the tensor-core contractions. */
 typedef enum ct_precision {
     CT_PREC_3XTF32 = 0, /* fp32 in, split into two terms of TF32's 11 significant bits, three MMAs, fp32
@@ -108,7 +116,8 @@ uint64_t ct_launch_count(void);
  * the launching stream.  ct_profile_read synchronises, sums and clears the records filed under
  * `kernel` ("gemm_tc", "gemm_prepass", "gemm_skinny", "gemm_splitk_reduce", "weights_pack",
  * "conv_prepass", "conv_small_c", "im2col", "elementwise", "reduce", "softmax", "transpose",
- * "concat", "maxpool"); NULL reads all. */
+ * "concat", "maxpool", "layer_norm", "layer_norm_grad", "dense_gated", "dense_gated_grad", "cross_entropy",
+ * "cross_entropy_grad"); NULL reads all. */
 ct_status ct_profile_enable(int on);
 ct_status ct_profile_read(const char *kernel, double *total_ms_host, uint64_t *launches_host);
 /* The tensor pipe's own ceiling, measured: every SM issues `mma_groups` x 4 tcgen05.mma of
@@ -337,6 +346,47 @@ ct_status ct_stream_wait_value(const uint32_t *addr_dev, uint32_t value);
 ct_status ct_dense_packed(
     const float *x_dev, const float *w_dev, const void *packed, const float *bias_dev, int64_t m,
     int64_t k, int64_t n, ct_activation act, float *out_dev, int64_t *argmax_dev);
+
+/* ---- layers of deeper networks and their gradients --------------------------------------
+ * The reference has none of these operators; the formulas stand with each.  Matrices are row-major float32 as everywhere.  An
+ * output must not overlap an input or another output, except where a function says so.  A gradient is that of a sum over everything
+ * weighted by the given gradient of the output; outputs that are null are not computed. */
+
+/* Layer norm of each row: out = (x - mean) / sqrt(var + eps) * gamma + beta, mean and var (the mean square deviation) over the
+ * row's `cols` values.  gamma and beta have one value per column; null: ones, zeros.  eps >= 0.  out may be x itself. */
+ct_status ct_layer_norm(
+    const float *x_dev, const float *gamma_dev, const float *beta_dev, int64_t rows, int64_t cols, double eps, float *out_dev);
+/* Its gradient from x and the gradient dout of its output: dx [rows][cols], dgamma and dbeta [cols], each may be null.  The
+ * statistics are computed again from x.  dx may be x or dout itself (up to 8192 columns; longer rows: not with dgamma or dbeta). */
+ct_status ct_layer_norm_grad(
+    const float *x_dev, const float *gamma_dev, const float *dout_dev, int64_t rows, int64_t cols, double eps, float *dx_dev,
+    float *dgamma_dev, float *dbeta_dev);
+
+/* Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), elementwise; x [m][k], both weights [k][n], both biases [n]
+ * or null.  gate_pre and up_pre [m][n] (null: not kept) receive the two sums themselves, which the gradient needs. */
+ct_status ct_dense_gated(
+    const float *x_dev, const float *w_gate_dev, const float *b_gate_dev, const float *w_up_dev, const float *b_up_dev, int64_t m,
+    int64_t k, int64_t n, ct_gate gate, float *out_dev, float *gate_pre_dev, float *up_pre_dev);
+/* Its gradient from what was kept and the gradient dout [m][n] of its output:
+ *   du = dout * gate(gate_pre), dg = dout * up_pre * gate'(gate_pre) (relu: 0 at 0),
+ *   dx = dg . w_gate^T + du . w_up^T, dw_gate = x^T . dg, dw_up = x^T . du, db_gate and db_up the columns' sums of dg and du. */
+ct_status ct_dense_gated_grad(
+    const float *x_dev, const float *w_gate_dev, const float *w_up_dev, const float *gate_pre_dev, const float *up_pre_dev,
+    const float *dout_dev, int64_t m, int64_t k, int64_t n, ct_gate gate, float *dx_dev, float *dw_gate_dev, float *dw_up_dev,
+    float *db_gate_dev, float *db_up_dev);
+
+/* Softmax cross entropy of the logits z = x . w + bias (x [m][k], w [k][n], bias [n] or null), which are not kept:
+ *   lse[i] = log(sum over j of exp(z[i][j])), loss[i] = lse[i] - z[i][targets[i]].
+ * A target outside 0 .. n-1 marks a row that has none (padding): its loss is 0.  loss or lse may be null; n >= 1. */
+ct_status ct_dense_cross_entropy(
+    const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, int64_t m, int64_t k, int64_t n,
+    float *loss_dev, float *lse_dev);
+/* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
+ *   d[i][j] = dloss[i] * (exp(z[i][j] - lse[i]) - (j == targets[i])), zero in rows without a target,
+ *   dx = d . w^T, dw = x^T . d, dbias the columns' sums of d.  The logits are computed again, in pieces. */
+ct_status ct_dense_cross_entropy_grad(
+    const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, const float *lse_dev,
+    const float *dloss_dev, int64_t m, int64_t k, int64_t n, float *dx_dev, float *dw_dev, float *dbias_dev);
 
 /* conv2d, NCHW input [n,c,h,w], OIHW weights [k_out,c,kh,kw], zero padding, then + bias and
  * activation (NONE or RELU).  No reference counterpart (the reference has no conv operator);
