@@ -1,9 +1,16 @@
 // Softmax cross entropy of a dense layer's logits, and its gradient, without keeping the logits.
 //
 //   lse = log(sum exp z), loss = lse - z[target];  d = dloss (exp(z - lse) - [target]),  dx = d . w^T, dw = x^T . d, dbias = column sums of d
-#include "common.cuh"
-
-#include <algorithm>
+//
+// Forward: a product whose tiles are not stored (fused_product.cuh).  A thread of the epilogue has a row and half of the tile's columns in
+// registers; it leaves their maximum, the sum of exponentials about it and, where it meets the target, that logit.  ce_join_kernel adds
+// up a row's parts: 16 bytes for 256 logits.
+// Gradient: the same product again, whose epilogue turns the logits into d / dloss = exp(z - lse) - [target], in [-1, 1], as planes of float16
+// pairs under one scale.  A piece of the vocabulary at a time they are the left operand of dx += d . w^T as they lie (rows weighted by
+// dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
+// A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
+// Up to 32 classes, and under the reduced precision, the logits of a piece of the rows are computed by the library's products.
+#include "fused_product.cuh"
 
 namespace ct {
 namespace {
@@ -62,6 +69,259 @@ __global__ void __launch_bounds__(256) ce_slopes_kernel(
     }
 }
 
+// ---- logits that stay in the epilogue ----
+
+__device__ __forceinline__ float exp2_fast(float x) { // 2^x, to 2^-22 of itself; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.44269504f;
+
+// acc becomes the logits of the lane's row; columns past the last are -inf.  NC columns from col.
+template <int NC>
+__device__ __forceinline__ void logits_of(const fused::Product &p, const float *bias, float *acc, float rs, int64_t col) {
+    const bool all = col + NC <= p.n;
+#pragma unroll
+    for (int j = 0; j < NC / 4; ++j) {
+        const float4 s = fused::scales4(p.col_scale, col + 4 * j);
+        acc[4 * j] = __fmul_rn(acc[4 * j], fused::weight(rs, s.x)), acc[4 * j + 1] = __fmul_rn(acc[4 * j + 1], fused::weight(rs, s.y));
+        acc[4 * j + 2] = __fmul_rn(acc[4 * j + 2], fused::weight(rs, s.z)), acc[4 * j + 3] = __fmul_rn(acc[4 * j + 3], fused::weight(rs, s.w));
+    }
+    if (bias)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            acc[j] = __fadd_rn(acc[j], col + j < p.n ? __ldg(bias + col + j) : 0.0f);
+    if (!all)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            acc[j] = col + j < p.n ? acc[j] : -INFINITY;
+}
+
+struct SumExp {
+    static constexpr bool kTwin = false;
+    struct Params {
+        const float *bias;
+        const int64_t *targets;
+        float2 *part; // [2 tiles_n][m]: maximum, sum
+        float *at_target;
+    };
+    template <int COLS>
+    __device__ static __forceinline__ void store(
+        const fused::Product &p, const Params &e, float (&z)[COLS], int64_t row0, int lane, int64_t col0, int, int slot, uint8_t *) {
+        const int64_t row = row0 + lane;
+        const bool mine   = row < p.m;
+        logits_of<COLS>(p, e.bias, z, mine ? __ldg(p.row_scale + row) : 0.0f, col0);
+        const int64_t t = mine ? e.targets[row] : -1, at = t >= 0 ? t - col0 : -1;
+        if (__any_sync(0xffffffffu, at >= 0 && at < COLS)) { // one in n / COLS tiles for each row
+            float found = 0.0f;
+#pragma unroll
+            for (int j = 0; j < COLS; ++j)
+                found = at == j ? z[j] : found;
+            if (at >= 0 && at < COLS && col0 + at < p.n)
+                e.at_target[row] = found;
+        }
+        float top[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+        for (int j = 4; j < COLS; ++j)
+            top[j & 3] = fmaxf(top[j & 3], z[j]);
+        const float mx   = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float sum[4]     = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+            sum[j & 3] = __fadd_rn(sum[j & 3], exp2_fast(__fmul_rn(__fsub_rn(z[j], base), kLog2e)));
+        if (mine)
+            e.part[(int64_t)slot * p.m + row] = make_float2(mx, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+    }
+};
+
+// A row's parts: 32 rows to a block, a warp takes every eighth part.
+__global__ void __launch_bounds__(256) ce_join_kernel(
+    const float2 *__restrict__ part, int slots, const float *__restrict__ at_target, const int64_t *__restrict__ targets, int64_t m, int64_t n,
+    float *__restrict__ loss, float *__restrict__ lse, const uint32_t *__restrict__ flags) {
+    __shared__ float2 words[8][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the parts were not computed
+        return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+    auto join = [](float2 a, float2 b) {
+        const float top  = fmaxf(a.x, b.x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float x    = __fmul_rn(a.y, exp2_fast(__fmul_rn(__fsub_rn(a.x, base), kLog2e))), y = __fmul_rn(b.y, exp2_fast(__fmul_rn(__fsub_rn(b.x, base), kLog2e)));
+        return make_float2(top, __fadd_rn(a.x == -INFINITY ? a.y : x, b.x == -INFINITY ? b.y : y)); // nothing but -inf: a sum of 0, or NaN
+    };
+    float2 v = make_float2(-INFINITY, 0.0f);
+    if (row < m)
+        for (int s = warp; s < slots; s += 8)
+            v = join(v, part[(int64_t)s * m + row]);
+    words[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && row < m) {
+        for (int w = 1; w < 8; ++w)
+            v = join(v, words[w][lane]);
+        const float l   = __fadd_rn(v.x == -INFINITY && v.y == v.y ? 0.0f : v.x, logf(v.y));
+        const int64_t t = targets[row];
+        if (lse)
+            lse[row] = l;
+        if (loss)
+            loss[row] = t >= 0 && t < n ? __fsub_rn(l, at_target[row]) : 0.0f;
+    }
+}
+
+ct_status ce_fused(
+    DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, int64_t m, int64_t k, int64_t n, float *loss, float *lse) {
+    using namespace fused;
+    const int64_t lk = padded(k), ln = padded(n);
+    const bool pair     = m > 128 && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
+    const int64_t slots = pair ? (n + 255) / 256 * 2 : (n + 127) / 128 * 2;
+    Parts parts;
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
+                 wm = parts.take((size_t)scales(ln) * 4), pp = parts.take((size_t)(slots * m) * 8), tp = parts.take((size_t)m * 4);
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, ln, ln);
+    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
+    CT_TRY(split_cols(st, w, nullptr, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    Product p{};
+    p.m = m, p.n = n, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
+    SumExp::Params e{bias, targets, s.as<float2>(pp), s.as<float>(tp)};
+    CT_TRY(pair ? (launch<SumExp, 256, 2, false, true>(st, px, pw, p, e, 1, "cross_entropy"))
+                : (launch<SumExp, 128, 1, false, true>(st, px, pw, p, e, 1, "cross_entropy")));
+    CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((m + 31) / 32)), dim3(256), 0, stream(), (const float2 *)e.part, (int)slots,
+                             (const float *)e.at_target, targets, m, n, loss, lse, (const uint32_t *)st->flags_dev));
+    CT_LAUNCH_CHECK("ce_join");
+    return CT_OK;
+}
+
+// ---- the gradient ----
+
+constexpr float kSlopeScale = 16384.0f; // 2^14: d / dloss is at most 1
+
+// Logits to the planes of (exp(z - lse) - [target]) 2^14.
+struct Slopes {
+    static constexpr bool kTwin = false;
+    struct Params {
+        const float *bias, *lse;
+        const int64_t *targets;
+        int64_t first, classes; // of the piece's columns
+        __half *hi, *lo;
+        int64_t ld;
+    };
+    template <int COLS>
+    __device__ static __forceinline__ void store(
+        const fused::Product &p, const Params &e, float (&z)[COLS], int64_t row0, int lane, int64_t col0, int, int, uint8_t *stage) {
+        const int64_t row  = row0 + lane;
+        const bool mine    = row < p.m;
+        const float rs     = mine ? __ldg(p.row_scale + row) : 0.0f, l = mine ? __ldg(e.lse + row) : 0.0f;
+        const int64_t t    = mine ? e.targets[row] : -1;
+        const bool has     = t >= 0 && t < e.classes;
+        const int64_t at   = has ? t - e.first - col0 : -1;
+        const int64_t left = p.m - row0;
+        const int rows     = left < 0 ? 0 : (left < 32 ? (int)left : 32);
+        if (rows == 0)
+            return;
+#pragma unroll
+        for (int g = 0; g < COLS / 32; ++g) {
+            const int64_t col = col0 + g * 32;
+            if (col >= p.n)
+                break;
+            float *d = z + g * 32;
+            logits_of<32>(p, e.bias, d, rs, col);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float v = exp2_fast(__fmul_rn(__fsub_rn(d[j], l), kLog2e));
+                d[j]          = has ? __fmul_rn(at == g * 32 + j ? __fsub_rn(v, 1.0f) : v, kSlopeScale) : 0.0f;
+            }
+            // rows of 128 bytes, hi terms and lo terms: 16-byte slots XOR-swizzled by row
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                __half2 hi[4], lo[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    fused::split2(d[8 * j + 2 * q], d[8 * j + 2 * q + 1], hi[q], lo[q]);
+                *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4))       = *reinterpret_cast<uint4 *>(hi);
+                *reinterpret_cast<uint4 *>(stage + lane * 128 + (((j + 4) ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4 *>(lo);
+            }
+            __syncwarp();
+            const int sub = lane & 7, rr = lane >> 3;
+            __half *to = (sub < 4 ? e.hi : e.lo) + (row0 + rr) * e.ld + col + (sub & 3) * 8;
+            if (col + (sub & 3) * 8 < p.n) // to the end of the slot, which ld covers
+#pragma unroll
+                for (int it = 0; it < 8; ++it) {
+                    const int r = it * 4 + rr;
+                    if (r < rows)
+                        *reinterpret_cast<uint4 *>(to + (int64_t)it * 4 * e.ld) = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((sub ^ (r & 7)) << 4));
+                }
+            __syncwarp();
+        }
+    }
+};
+
+// What the rows of d are weighted with behind the planes: dloss / 2^14, zero for rows without a target.
+__global__ void __launch_bounds__(256) ce_weights_kernel(
+    const float *__restrict__ dloss, const int64_t *__restrict__ targets, int64_t m, int64_t n, float *__restrict__ weight) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < m)
+        weight[i] = targets[i] >= 0 && targets[i] < n ? __fmul_rn(dloss ? dloss[i] : 1.0f, 1.0f / kSlopeScale) : 0.0f;
+}
+
+ct_status ce_grad_fused(
+    DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
+    int64_t n, float *dx, float *dw, float *dbias) {
+    using namespace fused;
+    const int64_t lk = padded(k), ln = padded(n);
+    // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
+    const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
+    const int64_t count = (n + most - 1) / most;
+    const int64_t piece = std::min<int64_t>(n, ((n + count - 1) / count + 255) / 256 * 256), ld = padded(piece);
+    Parts parts;
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
+                 wm = parts.take((size_t)scales(ln) * 4), dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
+    const size_t vp = dx ? parts.planes(k, ln) : 0, vi = dx ? parts.take((size_t)scales(k) * 4) : 0;
+    const size_t yp = dw ? parts.planes(m, lk) : 0, yi = dw ? parts.take((size_t)scales(lk) * 4) : 0, ym = dw ? parts.take((size_t)scales(lk) * 4) : 0;
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, ln, ln), pv = planes_at(s, vp, k, ln, ln), py = planes_at(s, yp, m, lk, lk);
+    float *weight = s.as<float>(rw);
+    CT_CUDA(launch_dependent(ce_weights_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream(), dloss, targets, m, n, weight));
+    CT_LAUNCH_CHECK("ce_weights");
+    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
+    CT_TRY(split_cols(st, w, nullptr, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    if (dx)
+        CT_TRY(split_rows(w, nullptr, k, n, pv, s.as<float>(vi)));
+    if (dw)
+        CT_TRY(split_cols(st, x, nullptr, weight, m, k, py, s.as<uint32_t>(ym), s.as<float>(yi)));
+    for (int64_t c = 0; c < n; c += piece) {
+        const int64_t cols = std::min(piece, n - c);
+        const Planes pd    = planes_at(s, dp, m, cols, ld);
+        Product p{};
+        p.m = m, p.n = cols, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi) + c;
+        Slopes::Params e{bias ? bias + c : nullptr, lse, targets, c, n, pd.hi, pd.lo, ld};
+        const Planes right = columns_of(pw, c, cols);
+        const bool pair    = m > 128 && (m + 255) / 256 * ((cols + 255) / 256) * 4 >= st->sm_count;
+        CT_TRY(pair ? (launch<Slopes, 256, 2, false, true>(st, px, right, p, e, 1, "cross_entropy_grad"))
+                    : (launch<Slopes, 128, 1, false, true>(st, px, right, p, e, 1, "cross_entropy_grad")));
+        if (dx) {
+            Result r{dx};
+            r.cols = r.stride = k, r.add = c > 0;
+            CT_TRY(product(st, pd, false, columns_of(pv, c, cols), false, m, k, weight, s.as<float>(vi), r));
+        }
+        if (dw) {
+            Result r{dw + c};
+            r.cols = cols, r.stride = n;
+            CT_TRY(product(st, py, true, pd, true, k, cols, s.as<float>(yi), nullptr, r));
+        }
+        if (dbias)
+            CT_TRY(column_sums(st, pd, weight, dbias + c));
+    }
+    return CT_OK;
+}
+
 ct_status check_ce(const char *name, const void *x, const void *w, const void *targets, int64_t m, int64_t k, int64_t n) {
     if (m < 0 || k < 0 || n < 0)
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
@@ -93,12 +353,18 @@ ct_status ct_dense_cross_entropy(
     if (m == 0)
         return CT_OK;
     ProfScope prof("cross_entropy");
+    const bool fused_form = n > 32 && k > 0 && ct_get_precision() == CT_PREC_3XTF32;
+    if (fused_form && m > fused::kFewRows)
+        return ce_fused(st, x, w, bias, targets, m, k, n, loss, lse);
     const int64_t piece = rows_at_once(m, n);
     Scratch logits;
     CT_TRY(logits.get((size_t)(piece * n) * 4));
     for (int64_t r = 0; r < m; r += piece) {
         const int64_t rows = std::min(piece, m - r);
-        CT_TRY(ct_dense(x + r * k, w, bias, rows, k, n, CT_ACT_NONE, logits.as<float>(), nullptr));
+        if (fused_form)
+            CT_TRY(fused::few_rows(st, x + r * k, w, bias, nullptr, nullptr, rows, k, n, 0, logits.as<float>(), nullptr, nullptr));
+        else
+            CT_TRY(ct_dense(x + r * k, w, bias, rows, k, n, CT_ACT_NONE, logits.as<float>(), nullptr));
         CT_CUDA(launch_dependent(ce_rows_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), logits.as<const float>(), targets + r, n,
                                  loss ? loss + r : nullptr, lse ? lse + r : nullptr));
         CT_LAUNCH_CHECK("ce_rows");
@@ -123,6 +389,8 @@ ct_status ct_dense_cross_entropy_grad(
         return CT_OK;
     }
     ProfScope prof("cross_entropy_grad");
+    if (n > 32 && k > 0 && ct_get_precision() == CT_PREC_3XTF32)
+        return ce_grad_fused(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     const int64_t piece = rows_at_once(m, n);
     Scratch logits, turned, sums;
     CT_TRY(logits.get((size_t)(piece * n) * 4));

@@ -1,0 +1,365 @@
+// Operand planes of the fused products (fused_product.cuh), and the product that is simply stored.
+//
+// The pre-passes are bound by memory: 4 bytes read and 4 written a value.  A scale per row is found and used while the row is in
+// registers; a scale per column needs the whole column first, so the matrix is read twice, the second time from L2 where it fits.
+#include "fused_product.cuh"
+
+namespace ct {
+namespace fused {
+namespace {
+
+// Two matrices side by side, the second from column ld on; zeros between cols and ld.
+struct Source {
+    const float *in, *in2;
+    int64_t rows, cols, ld;
+    int vec; // rows of both are whole and aligned float4
+    __device__ __forceinline__ float4 quad(int64_t r, int64_t c) const {
+        const float *src = in;
+        if (c >= ld)
+            src = in2, c -= ld;
+        src += r * cols + c;
+        if (vec && c + 3 < cols)
+            return *reinterpret_cast<const float4 *>(src);
+        float4 q;
+        q.x = c < cols ? src[0] : 0.0f;
+        q.y = c + 1 < cols ? src[1] : 0.0f;
+        q.z = c + 2 < cols ? src[2] : 0.0f;
+        q.w = c + 3 < cols ? src[3] : 0.0f;
+        return q;
+    }
+};
+
+__device__ __forceinline__ uint32_t quad_bits(const float4 &q) {
+    return max(max(finite_bits(q.x), finite_bits(q.y)), max(finite_bits(q.z), finite_bits(q.w)));
+}
+__device__ __forceinline__ void put_quad(const Planes &to, int64_t at, float a, float b, float c, float d) {
+    __half2 hi[2], lo[2];
+    split2(a, b, hi[0], lo[0]);
+    split2(c, d, hi[1], lo[1]);
+    *reinterpret_cast<uint2 *>(to.hi + at) = *reinterpret_cast<uint2 *>(hi);
+    *reinterpret_cast<uint2 *>(to.lo + at) = *reinterpret_cast<uint2 *>(lo);
+}
+
+// TPR threads to a row, which they hold in V float4 each if it is that short.
+template <int TPR, int V>
+__global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64_t width, const Planes to, float *__restrict__ inverse) {
+    __shared__ uint32_t words[8];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t       = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (row >= src.rows) // whole warps, or the whole block
+        return;
+    const bool fits = width <= TPR * V * 4;
+    float4 v[V];
+    uint32_t mx = 0;
+    if (fits) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t c = (int64_t)(j * TPR + t) * 4;
+            v[j]            = c < width ? src.quad(row, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            mx = max(mx, quad_bits(v[j]));
+    } else {
+        for (int64_t c = t * 4; c < width; c += TPR * 4)
+            mx = max(mx, quad_bits(src.quad(row, c)));
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (TPR > 32) {
+        if ((threadIdx.x & 31) == 0)
+            words[threadIdx.x >> 5] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            mx = max(mx, words[w]);
+    }
+    const float s = line_scale(mx);
+    if (fits) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t c = (int64_t)(j * TPR + t) * 4;
+            if (c < width)
+                put_quad(to, row * to.ld + c, v[j].x * s, v[j].y * s, v[j].z * s, v[j].w * s);
+        }
+    } else {
+        for (int64_t c = t * 4; c < width; c += TPR * 4) {
+            const float4 q = src.quad(row, c);
+            put_quad(to, row * to.ld + c, q.x * s, q.y * s, q.z * s, q.w * s);
+        }
+    }
+    if (t == 0)
+        inverse[row] = line_inverse(mx);
+}
+
+__device__ __forceinline__ float4 factored(float4 q, const float *row_factor, int64_t r) {
+    if (row_factor) {
+        const float f = row_factor[r]; // a row of factor zero takes no part, whatever it holds
+        q = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
+    }
+    return q;
+}
+
+// Largest finite magnitude of each column into col_max (zeroed before): a lane has four columns, the block's warps the rows in turn.
+__global__ void __launch_bounds__(256) col_max_kernel(
+    const Source src, int64_t width, const float *__restrict__ row_factor, int64_t rows_each, uint32_t *__restrict__ col_max) {
+    __shared__ uint32_t max_s[8][128];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 128 + lane * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_each, r1 = min(src.rows, r0 + rows_each);
+    uint32_t mx[4] = {0, 0, 0, 0};
+    if (c < width)
+#pragma unroll 8
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            const float4 q = factored(src.quad(r, c), row_factor, r);
+            mx[0] = max(mx[0], finite_bits(q.x)), mx[1] = max(mx[1], finite_bits(q.y));
+            mx[2] = max(mx[2], finite_bits(q.z)), mx[3] = max(mx[3], finite_bits(q.w));
+        }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        max_s[warp][lane * 4 + q] = mx[q];
+    __syncthreads();
+    const int64_t mine = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && mine < width) {
+        uint32_t all = max_s[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 8; ++w)
+            all = max(all, max_s[w][threadIdx.x]);
+        if (all)
+            atomicMax(col_max + mine, all); // the same whatever the order
+    }
+}
+
+__global__ void __launch_bounds__(256) split_cols_kernel(
+    const Source src, int64_t width, const float *__restrict__ row_factor, int64_t rows_each, const uint32_t *__restrict__ col_max, const Planes to,
+    float *__restrict__ inverse) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 128 + lane * 4;
+    if (c >= width)
+        return;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_each, r1 = min(src.rows, r0 + rows_each);
+    const uint4 mx = *reinterpret_cast<const uint4 *>(col_max + c);
+    const float s0 = line_scale(mx.x), s1 = line_scale(mx.y), s2 = line_scale(mx.z), s3 = line_scale(mx.w);
+    if (blockIdx.y == 0 && warp == 0)
+        *reinterpret_cast<float4 *>(inverse + c) = make_float4(line_inverse(mx.x), line_inverse(mx.y), line_inverse(mx.z), line_inverse(mx.w));
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+        const float4 q = factored(src.quad(r, c), row_factor, r);
+        put_quad(to, r * to.ld + c, q.x * s0, q.y * s1, q.z * s2, q.w * s3);
+    }
+}
+
+// out = the slices' sums, in order (and what out held); columns from `second` on to out2.
+__global__ void __launch_bounds__(256) join_slices_kernel(
+    const float *__restrict__ partial, int slices, int64_t m, int64_t n, float *__restrict__ out, float *__restrict__ out2, int64_t out_cols,
+    int64_t stride, int64_t second, int add, const uint32_t *__restrict__ flags) {
+    griddep_wait();
+    griddep_launch_dependents();
+    if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the slices were not computed
+        return;
+    const int64_t total = m * n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / n;
+        int64_t c       = i - r * n;
+        float *to       = out;
+        if (out2 && c >= second)
+            to = out2, c -= second;
+        if (c >= out_cols)
+            continue;
+        to += r * stride + c;
+        float v = partial[i];
+#pragma unroll 4
+        for (int z = 1; z < slices; ++z)
+            v = __fadd_rn(v, partial[(int64_t)z * total + i]);
+        *to = add ? __fadd_rn(*to, v) : v;
+    }
+}
+
+Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols) {
+    const bool vec = (cols & 3) == 0 && (reinterpret_cast<uintptr_t>(in) & 15u) == 0 && (reinterpret_cast<uintptr_t>(in2) & 15u) == 0;
+    return Source{in, in2, rows, cols, padded(cols), vec ? 1 : 0};
+}
+
+template <int BN, int CG>
+ct_status launch_store(
+    DeviceState *st, const Planes &a, bool a_mn, const Planes &b, bool b_mn, const Product &p, const Store::Params &e, int splits) {
+    if (a_mn)
+        return b_mn ? launch<Store, BN, CG, true, true>(st, a, b, p, e, splits, "fused_product")
+                    : launch<Store, BN, CG, true, false>(st, a, b, p, e, splits, "fused_product");
+    return b_mn ? launch<Store, BN, CG, false, true>(st, a, b, p, e, splits, "fused_product")
+                : launch<Store, BN, CG, false, false>(st, a, b, p, e, splits, "fused_product");
+}
+
+} // namespace
+
+ct_status split_rows(const float *in, const float *in2, int64_t rows, int64_t cols, const Planes &to, float *inverse) {
+    const Source src    = source_of(in, in2, rows, cols);
+    const int64_t width = in2 ? 2 * src.ld : src.ld;
+#define CT_SPLIT_ROWS(TPR, V)                                                                                                                \
+    CT_CUDA(launch_dependent(split_rows_kernel<TPR, V>, dim3((unsigned)((rows + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, stream(), src, \
+                             width, to, inverse))
+    if (width <= 256)
+        CT_SPLIT_ROWS(32, 2);
+    else if (width <= 1024)
+        CT_SPLIT_ROWS(32, 8);
+    else if (width <= 4096)
+        CT_SPLIT_ROWS(256, 4);
+    else
+        CT_SPLIT_ROWS(256, 8);
+#undef CT_SPLIT_ROWS
+    CT_LAUNCH_CHECK("split_rows");
+    return CT_OK;
+}
+
+ct_status split_cols(
+    DeviceState *st, const float *in, const float *in2, const float *row_factor, int64_t rows, int64_t cols, const Planes &to, uint32_t *col_max,
+    float *inverse) {
+    const Source src     = source_of(in, in2, rows, cols);
+    const int64_t width  = in2 ? 2 * src.ld : src.ld;
+    const int64_t strips = (width + 127) / 128;
+    // a few blocks to an SM, of at least 32 rows
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((rows + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t each   = (rows + slices - 1) / slices;
+    const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, (rows + each - 1) / each));
+    CT_CUDA(cudaMemsetAsync(col_max, 0, (size_t)width * 4, stream()));
+    CT_CUDA(launch_dependent(col_max_kernel, grid, dim3(256), 0, stream(), src, width, row_factor, each, col_max));
+    CT_LAUNCH_CHECK("col_max");
+    CT_CUDA(launch_dependent(split_cols_kernel, grid, dim3(256), 0, stream(), src, width, row_factor, each, (const uint32_t *)col_max, to, inverse));
+    CT_LAUNCH_CHECK("split_cols");
+    return CT_OK;
+}
+
+ct_status product(
+    DeviceState *st, const Planes &a, bool a_mn, const Planes &b, bool b_mn, int64_t m, int64_t n, const float *row_scale, const float *col_scale,
+    const Result &to) {
+    const int64_t stages = ((a_mn ? a.rows : a.cols) + 63) / 64;
+    // Tile and slices by what they take, in microseconds: a stage of a pair's 256 x 256 tile ~ 0.95, of a single CTA's 128 x 128 ~ 0.6;
+    // filling and draining a tile as much as four stages; the slices' sums written, read and a launch.
+    bool pair = false;
+    int splits = 1;
+    double best = 1e300;
+    for (int kind = 0; kind < 2; ++kind) {
+        const int64_t side = kind ? 256 : 128, units = kind ? st->sm_count / 2 : st->sm_count;
+        const int64_t tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
+        for (int s = 1; s <= 32 && (s == 1 || stages >= 4 * s); ++s) {
+            const double waves = (double)((tiles * s + units - 1) / units);
+            const double cost  = waves * (double)((stages + s - 1) / s + 4) * (kind ? 0.95 : 0.6) + (s > 1 ? 3.0 + (double)(m * n) * (s + 1) * 4 / 5e6 : 0.0);
+            if (cost < best)
+                best = cost, pair = kind != 0, splits = s;
+        }
+    }
+    if (splits > 1) { // no empty slice
+        const int64_t each = (stages + splits - 1) / splits;
+        splits             = (int)((stages + each - 1) / each);
+    }
+    Product p{};
+    p.m = m, p.n = n, p.row_scale = row_scale, p.col_scale = col_scale;
+    auto whole = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
+    Store::Params e{};
+    e.out = to.out, e.out2 = to.out2, e.n = to.cols, e.stride = to.stride, e.second = to.second, e.add = to.add ? 1 : 0;
+    e.vec = (to.stride & 3) == 0 && whole(to.out) && whole(to.out2) ? 1 : 0;
+    Scratch partial;
+    if (splits > 1) {
+        CT_TRY(partial.get((size_t)splits * m * n * 4));
+        e.out = partial.as<float>(), e.out2 = nullptr, e.n = e.stride = n, e.second = 0, e.slice = m * n, e.add = 0;
+        e.vec = (n & 3) == 0 ? 1 : 0;
+    }
+    CT_TRY(pair ? (launch_store<256, 2>(st, a, a_mn, b, b_mn, p, e, splits)) : (launch_store<128, 1>(st, a, a_mn, b, b_mn, p, e, splits)));
+    if (splits > 1) {
+        const int64_t blocks = std::min<int64_t>((m * n + 255) / 256, (int64_t)st->sm_count * 16);
+        CT_CUDA(launch_dependent(join_slices_kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), partial.as<const float>(), splits, m, n, to.out,
+                                 to.out2, to.cols, to.stride, to.second, to.add ? 1 : 0, (const uint32_t *)st->flags_dev));
+        CT_LAUNCH_CHECK("join_slices");
+    }
+    return CT_OK;
+}
+
+namespace {
+
+// Sums of eight columns to a lane (16 bytes of each plane) over the block's rows, a row to each warp in turn.
+__global__ void __launch_bounds__(256) plane_sums_kernel(
+    const Planes x, const float *__restrict__ row_weight, int64_t rows_each, double *__restrict__ partial) {
+    __shared__ float sums[8][256];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c  = (int64_t)blockIdx.x * 256 + lane * 8, cols = x.cols;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_each, r1 = min(x.rows, r0 + rows_each);
+    float s[8] = {};
+    if (c < cols)
+#pragma unroll 4
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            const float w = row_weight[r];
+            const uint4 h = *reinterpret_cast<const uint4 *>(x.hi + r * x.ld + c), l = *reinterpret_cast<const uint4 *>(x.lo + r * x.ld + c);
+            const __half2 *hi = reinterpret_cast<const __half2 *>(&h), *lo = reinterpret_cast<const __half2 *>(&l);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                s[2 * q]     = __fmaf_rn(w, __fmaf_rn(__low2float(lo[q]), kLoInv, __low2float(hi[q])), s[2 * q]);
+                s[2 * q + 1] = __fmaf_rn(w, __fmaf_rn(__high2float(lo[q]), kLoInv, __high2float(hi[q])), s[2 * q + 1]);
+            }
+        }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        sums[warp][lane * 8 + q] = s[q];
+    __syncthreads();
+    const int64_t mine = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (mine < cols) {
+        double all = 0.0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            all += (double)sums[w][threadIdx.x];
+        partial[(int64_t)blockIdx.y * cols + mine] = all;
+    }
+}
+// 32 columns to a block, a warp takes every eighth part.
+__global__ void __launch_bounds__(256) join_columns_kernel(
+    const double *__restrict__ partial, int64_t parts, int64_t n, int64_t width, float *__restrict__ first, float *__restrict__ second) {
+    __shared__ double sums[8][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    double s = 0.0;
+    if (c < width)
+#pragma unroll 4
+        for (int64_t p = warp; p < parts; p += 8)
+            s += partial[p * width + c];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < width) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w)
+            s += sums[w][lane];
+        float *out = c < n ? first : second;
+        if (out)
+            out[c < n ? c : c - n] = (float)s;
+    }
+}
+
+} // namespace
+
+ct_status join_columns(const double *partial, int64_t parts, int64_t n, bool two, float *first, float *second) {
+    const int64_t width = two ? 2 * n : n;
+    CT_CUDA(launch_dependent(join_columns_kernel, dim3((unsigned)((width + 31) / 32)), dim3(256), 0, stream(), partial, parts, n, width, first, second));
+    CT_LAUNCH_CHECK("join_columns");
+    return CT_OK;
+}
+
+ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight, float *out) {
+    const int64_t strips = (x.cols + 255) / 256;
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((x.rows + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t each = (x.rows + slices - 1) / slices, parts = (x.rows + each - 1) / each;
+    Scratch partial;
+    CT_TRY(partial.get((size_t)(parts * x.cols) * 8));
+    CT_CUDA(launch_dependent(plane_sums_kernel, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), x, row_weight, each, partial.as<double>()));
+    CT_LAUNCH_CHECK("plane_sums");
+    return join_columns(partial.as<const double>(), parts, x.cols, false, out, nullptr);
+}
+
+} // namespace fused
+} // namespace ct

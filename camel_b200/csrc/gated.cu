@@ -1,5 +1,12 @@
 // Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), and its gradient.
-#include "common.cuh"
+//
+// Forward: one product whose tiles have the same columns of both weight matrices (fused_product.cuh); a thread of the epilogue
+// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu.
+// Gradient: gated_slopes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
+// dx = d . [w_gate | w_up]^T as they lie, and the right operand of dw = x'^T . d with their rows as k, x' being x with the rows' scales
+// taken back.  So d is written once, 8 bytes for each of its values' pairs of terms, and read in place.
+// The reduced precision runs the library's products one after the other.
+#include "fused_product.cuh"
 #include "gate.cuh"
 
 #include <algorithm>
@@ -32,6 +39,297 @@ __global__ void __launch_bounds__(256) gated_slopes_kernel(
     }
 }
 
+// ---- one product with the gate behind it ----
+
+template <int GATE> struct GateEpilogue {
+    static constexpr bool kTwin = true;
+    struct Params {
+        const float *b_gate, *b_up;
+        float *out, *gate_pre, *up_pre;
+        int vec;
+    };
+    template <int COLS>
+    __device__ static __forceinline__ void store(
+        const fused::Product &p, const Params &e, float (&acc)[COLS], int64_t row0, int lane, int64_t col0, int, int, uint8_t *stage) {
+        const int64_t left = p.m - row0;
+        const int rows     = left < 0 ? 0 : (left < 32 ? (int)left : 32);
+        if (rows == 0)
+            return;
+        const float rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
+#pragma unroll
+        for (int g = 0; g < COLS / 64; ++g) {
+            const int64_t col = col0 + g * 32;
+            if (col >= p.n)
+                break;
+            const int cols = (int)(p.n - col < 32 ? p.n - col : 32);
+            float *a = acc + g * 32, *b = acc + COLS / 2 + g * 32;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float4 s = fused::scales4(p.col_scale, col + 4 * j), t = fused::scales4(p.col_scale, p.twin_offset + col + 4 * j);
+                a[4 * j] = __fmul_rn(a[4 * j], fused::weight(rs, s.x)), a[4 * j + 1] = __fmul_rn(a[4 * j + 1], fused::weight(rs, s.y));
+                a[4 * j + 2] = __fmul_rn(a[4 * j + 2], fused::weight(rs, s.z)), a[4 * j + 3] = __fmul_rn(a[4 * j + 3], fused::weight(rs, s.w));
+                b[4 * j] = __fmul_rn(b[4 * j], fused::weight(rs, t.x)), b[4 * j + 1] = __fmul_rn(b[4 * j + 1], fused::weight(rs, t.y));
+                b[4 * j + 2] = __fmul_rn(b[4 * j + 2], fused::weight(rs, t.z)), b[4 * j + 3] = __fmul_rn(b[4 * j + 3], fused::weight(rs, t.w));
+            }
+            if (e.b_gate)
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    a[j] = __fadd_rn(a[j], j < cols ? __ldg(e.b_gate + col + j) : 0.0f);
+            if (e.b_up)
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    b[j] = __fadd_rn(b[j], j < cols ? __ldg(e.b_up + col + j) : 0.0f);
+            const int64_t at = row0 * p.n + col;
+            if (e.gate_pre)
+                fused::store_block<false>(e.gate_pre + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return a[j]; });
+            if (e.up_pre)
+                fused::store_block<false>(e.up_pre + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return b[j]; });
+            fused::store_block<false>(
+                e.out + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return __fmul_rn(gate_value<GATE>(a[j]), b[j]); });
+        }
+    }
+};
+
+bool whole(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+ct_status gated_fused(
+    DeviceState *st, const float *x, const float *w_gate, const float *b_gate, const float *w_up, const float *b_up, int64_t m, int64_t k, int64_t n,
+    int gate, float *out, float *gate_pre, float *up_pre) {
+    using namespace fused;
+    const int64_t lk = padded(k), ln = padded(n);
+    Parts parts;
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, 2 * ln), wi = parts.take((size_t)scales(2 * ln) * 4),
+                 wm = parts.take((size_t)scales(2 * ln) * 4);
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, 2 * ln, 2 * ln);
+    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
+    CT_TRY(split_cols(st, w_gate, w_up, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    Product p{};
+    p.m = m, p.n = n, p.twin_offset = (int)ln, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
+    return with_gate(gate, [&](auto G) -> ct_status {
+        using E = GateEpilogue<G.value>;
+        typename E::Params e{b_gate, b_up, out, gate_pre, up_pre, (n & 3) == 0 && whole(out) && whole(gate_pre) && whole(up_pre) ? 1 : 0};
+        // pairs where their tiles fill at least half of the machine
+        const int64_t tiles = (m + 255) / 256 * ((n + 127) / 128);
+        return m > 128 && tiles * 4 >= st->sm_count ? launch<E, 256, 2, false, true>(st, px, pw, p, e, 1, "dense_gated")
+                                                    : launch<E, 128, 1, false, true>(st, px, pw, p, e, 1, "dense_gated");
+    });
+}
+
+// ---- the gradient's left operand ----
+
+// d = [dg | du] of a row, its largest magnitude, and its planes: TPR threads to a row, which hold V groups of four columns of both; longer
+// rows are computed twice.  inverse[row] is zero for a row of zeros: such a row must not widen the range of x' (gated_grad_fused).
+template <int GATE, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kernel(
+    const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, const fused::Planes to,
+    float *__restrict__ inverse) {
+    __shared__ uint32_t words[32];
+    griddep_wait();
+    griddep_launch_dependents();
+    constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR, ld = to.ld / 2;
+    if (row >= rows) // whole warps, or the whole block
+        return;
+    auto load = [&](const float *src, int64_t c) {
+        src += row * n + c;
+        if (vec && c + 3 < n)
+            return __ldcs(reinterpret_cast<const float4 *>(src));
+        float4 q;
+        q.x = c < n ? src[0] : 0.0f, q.y = c + 1 < n ? src[1] : 0.0f;
+        q.z = c + 2 < n ? src[2] : 0.0f, q.w = c + 3 < n ? src[3] : 0.0f;
+        return q;
+    };
+    auto slopes = [&](int64_t c, float4 &dg, float4 &du) {
+        const float4 a = load(g, c), b = load(u, c), d = load(dout, c);
+        auto one = [](float a, float b, float d, float &dg, float &du) {
+            float value, slope;
+            gate_slope<GATE>(a, value, slope);
+            dg = __fmul_rn(__fmul_rn(d, b), slope), du = __fmul_rn(d, value);
+        };
+        one(a.x, b.x, d.x, dg.x, du.x), one(a.y, b.y, d.y, dg.y, du.y), one(a.z, b.z, d.z, dg.z, du.z), one(a.w, b.w, d.w, dg.w, du.w);
+    };
+    auto bits = [](const float4 &q) {
+        return max(max(fused::finite_bits(q.x), fused::finite_bits(q.y)), max(fused::finite_bits(q.z), fused::finite_bits(q.w)));
+    };
+    const bool fits = ld <= TPR * V * 4;
+    float4 dg[V], du[V];
+    uint32_t mx = 0;
+    if (fits) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t c = (int64_t)(j * TPR + t) * 4;
+            dg[j] = du[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c < n)
+                slopes(c, dg[j], du[j]);
+            mx = max(mx, max(bits(dg[j]), bits(du[j])));
+        }
+    } else {
+        for (int64_t c = t * 4; c < n; c += TPR * 4) {
+            slopes(c, dg[0], du[0]);
+            mx = max(mx, max(bits(dg[0]), bits(du[0])));
+        }
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (TPR > 32) {
+        if ((threadIdx.x & 31) == 0)
+            words[threadIdx.x >> 5] = mx;
+        __syncthreads();
+        mx = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < TPR / 32 ? words[threadIdx.x & 31] : 0u);
+    }
+    const float s = fused::line_scale(mx);
+    auto put      = [&](int64_t c, const float4 &q) {
+        __half2 hi[2], lo[2];
+        fused::split2(q.x * s, q.y * s, hi[0], lo[0]);
+        fused::split2(q.z * s, q.w * s, hi[1], lo[1]);
+        *reinterpret_cast<uint2 *>(to.hi + row * to.ld + c) = *reinterpret_cast<uint2 *>(hi);
+        *reinterpret_cast<uint2 *>(to.lo + row * to.ld + c) = *reinterpret_cast<uint2 *>(lo);
+    };
+    if (fits) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t c = (int64_t)(j * TPR + t) * 4;
+            if (c < ld)
+                put(c, dg[j]), put(ld + c, du[j]);
+        }
+    } else {
+        for (int64_t c = t * 4; c < ld; c += TPR * 4) {
+            dg[0] = du[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c < n)
+                slopes(c, dg[0], du[0]);
+            put(c, dg[0]), put(ld + c, du[0]);
+        }
+    }
+    if (t == 0)
+        inverse[row] = mx ? fused::line_inverse(mx) : 0.0f;
+}
+
+// The columns' sums of dg and du, from the values themselves: what the planes hold of a value depends on the rest of its row.  A lane has
+// four columns, a warp every eighth row of the block's; partial[block][2][n] are added up by join_columns.
+template <int GATE>
+__global__ void __launch_bounds__(256) gated_bias_kernel(
+    const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, int64_t rows_each,
+    double *__restrict__ partial) {
+    __shared__ float sums[8][2][128];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c  = (int64_t)blockIdx.x * 128 + lane * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_each, r1 = min(rows, r0 + rows_each);
+    float sg[4] = {}, su[4] = {};
+    auto load = [&](const float *src, int64_t r) {
+        src += r * n + c;
+        if (vec && c + 3 < n)
+            return *reinterpret_cast<const float4 *>(src);
+        float4 q;
+        q.x = c < n ? src[0] : 0.0f, q.y = c + 1 < n ? src[1] : 0.0f;
+        q.z = c + 2 < n ? src[2] : 0.0f, q.w = c + 3 < n ? src[3] : 0.0f;
+        return q;
+    };
+    if (c < n)
+#pragma unroll 4
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            const float4 a = load(g, r), b = load(u, r), d = load(dout, r);
+            auto one = [&](float a, float b, float d, int q) {
+                float value, slope;
+                gate_slope<GATE>(a, value, slope);
+                sg[q] = __fmaf_rn(__fmul_rn(d, b), slope, sg[q]);
+                su[q] = __fmaf_rn(d, value, su[q]);
+            };
+            one(a.x, b.x, d.x, 0), one(a.y, b.y, d.y, 1), one(a.z, b.z, d.z, 2), one(a.w, b.w, d.w, 3);
+        }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        sums[warp][0][lane * 4 + q] = sg[q], sums[warp][1][lane * 4 + q] = su[q];
+    __syncthreads();
+    const int which = threadIdx.x >> 7, at = threadIdx.x & 127;
+    const int64_t mine = (int64_t)blockIdx.x * 128 + at;
+    if (mine < n) {
+        double all = 0.0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            all += (double)sums[w][which][at];
+        partial[((int64_t)blockIdx.y * 2 + which) * n + mine] = all;
+    }
+}
+
+ct_status gated_bias(
+    DeviceState *st, const float *g, const float *u, const float *dout, int64_t m, int64_t n, int gate, int vec, float *db_gate, float *db_up) {
+    const int64_t strips = (n + 127) / 128;
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((m + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t each = (m + slices - 1) / slices, parts = (m + each - 1) / each;
+    Scratch partial;
+    CT_TRY(partial.get((size_t)(parts * 2 * n) * 8));
+    CT_TRY(with_gate(gate, [&](auto G) -> ct_status {
+        CT_CUDA(launch_dependent(gated_bias_kernel<G.value>, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), g, u, dout, m, n, vec, each,
+                                 partial.as<double>()));
+        CT_LAUNCH_CHECK("gated_bias");
+        return CT_OK;
+    }));
+    return fused::join_columns(partial.as<const double>(), parts, n, true, db_gate, db_up);
+}
+
+template <int GATE, int TPR, int V>
+ct_status launch_slopes_of(
+    const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V>, dim3((unsigned)((m + RPB - 1) / RPB)), dim3(TPR * RPB), 0, stream(), g, u, dout, m,
+                             n, vec, to, inverse));
+    CT_LAUNCH_CHECK("gated_slopes");
+    return CT_OK;
+}
+template <int GATE>
+ct_status launch_slopes(const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse) {
+    if (n <= 256)
+        return launch_slopes_of<GATE, 32, 2>(g, u, dout, m, n, vec, to, inverse);
+    if (n <= 1024)
+        return launch_slopes_of<GATE, 256, 1>(g, u, dout, m, n, vec, to, inverse);
+    if (n <= 4096)
+        return launch_slopes_of<GATE, 512, 2>(g, u, dout, m, n, vec, to, inverse);
+    return launch_slopes_of<GATE, 512, 4>(g, u, dout, m, n, vec, to, inverse);
+}
+
+ct_status gated_grad_fused(
+    DeviceState *st, const float *x, const float *w_gate, const float *w_up, const float *gate_pre, const float *up_pre, const float *dout, int64_t m,
+    int64_t k, int64_t n, int gate, float *dx, float *dw_gate, float *dw_up, float *db_gate, float *db_up) {
+    using namespace fused;
+    const int64_t lk = padded(k), ln = padded(n);
+    const bool weights = (dw_gate || dw_up) && k > 0, back = dx && k > 0;
+    Parts parts;
+    const size_t dp = parts.planes(m, 2 * ln), di = parts.take((size_t)m * 4);
+    const size_t wp = back ? parts.planes(k, 2 * ln) : 0, wi = back ? parts.take((size_t)scales(k) * 4) : 0;
+    const size_t xp = weights ? parts.planes(m, lk) : 0, xi = weights ? parts.take((size_t)scales(lk) * 4) : 0,
+                 xm = weights ? parts.take((size_t)scales(lk) * 4) : 0;
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes pd = planes_at(s, dp, m, 2 * ln, 2 * ln);
+    const int vec   = (n & 3) == 0 && whole(gate_pre) && whole(up_pre) && whole(dout) ? 1 : 0;
+    CT_TRY(with_gate(gate, [&](auto G) { return launch_slopes<G.value>(gate_pre, up_pre, dout, m, n, vec, pd, s.as<float>(di)); }));
+    if (db_gate || db_up)
+        CT_TRY(gated_bias(st, gate_pre, up_pre, dout, m, n, gate, vec, db_gate, db_up));
+    if (back) {
+        const Planes pw = planes_at(s, wp, k, 2 * ln, 2 * ln);
+        CT_TRY(split_rows(w_gate, w_up, k, n, pw, s.as<float>(wi)));
+        Result r{dx};
+        r.cols = r.stride = k;
+        CT_TRY(product(st, pd, false, pw, false, m, k, s.as<float>(di), s.as<float>(wi), r));
+    }
+    if (weights) {
+        const Planes px = planes_at(s, xp, m, lk, lk);
+        CT_TRY(split_cols(st, x, nullptr, s.as<float>(di), m, k, px, s.as<uint32_t>(xm), s.as<float>(xi)));
+        Result r{dw_gate};
+        r.cols = r.stride = n;
+        if (dw_gate && dw_up)
+            r.out2 = dw_up, r.second = ln;
+        const Planes right = dw_gate && dw_up ? pd : columns_of(pd, dw_gate ? 0 : ln, n);
+        r.out              = dw_gate ? dw_gate : dw_up;
+        CT_TRY(product(st, px, true, right, true, k, dw_gate && dw_up ? 2 * ln : n, s.as<float>(xi), nullptr, r));
+    }
+    return CT_OK;
+}
+
 unsigned grid_of(const DeviceState *st, int64_t count) {
     return (unsigned)std::min<int64_t>((count + 255) / 256, (int64_t)st->sm_count * 16);
 }
@@ -62,7 +360,14 @@ ct_status ct_dense_gated(
         return CT_OK;
     if (!out || (k > 0 && (!x || !w_gate || !w_up)))
         return fail(CT_ERR_INVALID, "dense_gated: null pointer");
+    if (m > 0x7fffffff || k > 0x7fffffff || n > 0x3fffffff)
+        return fail(CT_ERR_TOO_LARGE, "dense_gated: dimension too large");
     ProfScope prof("dense_gated");
+    if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
+        if (m <= fused::kFewRows)
+            return fused::few_rows(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
+        return gated_fused(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
+    }
     const int64_t count = m * n;
     Scratch scratch;
     float *g = gate_pre, *u = up_pre;
@@ -104,6 +409,10 @@ ct_status ct_dense_gated_grad(
         CT_CUDA(clear(db_up, n));
         return CT_OK;
     }
+    if (m > 0x7fffffff || k > 0x7fffffff || n > 0x3fffffff)
+        return fail(CT_ERR_TOO_LARGE, "dense_gated_grad: dimension too large");
+    if (ct_get_precision() == CT_PREC_3XTF32)
+        return gated_grad_fused(st, x, w_gate, w_up, gate_pre, up_pre, dout, m, k, n, gate, dx, dw_gate, dw_up, db_gate, db_up);
     const int64_t count = m * n;
     Scratch slopes;
     CT_TRY(slopes.get((size_t)count * 8));
