@@ -58,7 +58,7 @@ template <int TPR, int V, bool VEC> struct Row {
 // warp that is through the second call's barrier has seen every warp through the first.
 template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&s)[N], float (&words)[N][32]) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1)
 #pragma unroll
         for (int i = 0; i < N; ++i)
             s[i] = __fadd_rn(s[i], __shfl_xor_sync(0xffffffffu, s[i], o));
@@ -88,7 +88,7 @@ __device__ __forceinline__ float spread(float sum_d, float sum_dd, float inv_col
     return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(var < 0.0f ? 0.0f : var, eps)));
 }
 
-template <int TPR> constexpr int kBlock = TPR < 256 ? 256 : TPR;
+template <int TPR> constexpr int kBlock = TPR <= 32 ? 256 : TPR; // several rows, or one
 
 template <int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
@@ -100,11 +100,12 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
     griddep_launch_dependents();
     const int t       = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR;
-    if (row >= rows) // whole warps
+    const int64_t mine = row < rows ? cols : 0; // a warp's last rows may not be there
+    if (TPR == 32 && row >= rows)
         return;
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
     float v[4 * V];
-    R::load(v, x + row * cols, cols, t);
+    R::load(v, x + row * cols, mine, t);
     float sum[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < 4 * V; ++i)
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
             y = __fadd_rn(y, b[i]);
         v[i] = y;
     }
-    R::store(out + row * cols, v, cols, t);
+    R::store(out + row * cols, v, mine, t);
 }
 
 // Rows of any length, a block to a row, which is read three times.
@@ -173,29 +174,113 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(
     }
 }
 
-// The gradient.  A block walks rows; a thread has the same columns of each, and keeps their sums over the block's rows, which
-// go to partial[block][2][cols] (dgamma, dbeta) for norm_columns_kernel.
+// A row on its way to shared memory, column c at slot + 4 c: aligned rows 16 bytes at a time, each thread what it will read (only its own
+// copies are waited for); other rows of an aligned matrix as the 16-byte pieces that they touch, from slot - 4 skew on, where skew is the row's
+// distance from a 16-byte boundary; else value by value, which is four times the instructions (60000 x 785: 161 us).
+template <int TPR, int V, bool VEC>
+__device__ __forceinline__ void row_copy(uint32_t slot, const float *__restrict__ src, int64_t cols, int skew, bool pieces, int t) {
+    using R = Row<TPR, V, VEC>;
+    if (VEC) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t c = R::column(t, j, 0);
+            const int bytes = c < cols ? 16 : 0; // none: zeros, and nothing is read
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + (int)c * 4), "l"(src + (bytes ? c : 0)), "r"(bytes) : "memory");
+        }
+    } else if (pieces) {
+        const int end = skew + (int)cols;
+        for (int c = 4 * t; c < end; c += 4 * TPR) {
+            const int bytes = end - c < 4 ? (end - c) * 4 : 16; // not past the last row's end
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + (c - skew) * 4), "l"(src + (c - skew)), "r"(bytes) : "memory");
+        }
+    } else {
+        for (int c = t; c < (int)cols; c += TPR)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot + c * 4), "l"(src + c) : "memory");
+    }
+}
+// A thread's values of it; columns that the row does not have are zero (VEC: in the slot as well).
+template <int TPR, int V, bool VEC> __device__ __forceinline__ void row_read(float (&v)[4 * V], const float *slot, int64_t cols, int t) {
+    using R = Row<TPR, V, VEC>;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (VEC) {
+            const float4 f = *reinterpret_cast<const float4 *>(slot + R::column(t, j, 0));
+            v[4 * j] = f.x, v[4 * j + 1] = f.y, v[4 * j + 2] = f.z, v[4 * j + 3] = f.w;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                v[4 * j + q] = R::column(t, j, q) < cols ? slot[R::column(t, j, q)] : 0.0f;
+        }
+}
+template <int TPR> __device__ __forceinline__ void row_sync() {
+    if (TPR <= 32)
+        __syncwarp();
+    else
+        __syncthreads();
+}
+
+// The gradient.  A block (of one row at a time, or a row per warp) walks rows; a thread has the same columns of each, and keeps their sums
+// over its rows, which go to partial[block][2][cols] (dgamma, dbeta) for norm_columns_kernel.  Between a row's loads and its stores stand two
+// exchanges, so the next two rows are on their way meanwhile: with the loads of a row issued when it was its turn, 16384 x 4096 took 177 us
+// and 60000 x 785 208.
+constexpr int kAhead = 3; // rows in shared memory, the one at work among them
+// Values of a slot: a row, with what lies before and behind it in its 16-byte pieces.  Slots begin on 128-byte boundaries: 16 bytes off, 2048
+// aligned columns took 165 us for 140.
+template <int TPR, int V, bool VEC> constexpr int kSlot = 4 * V * TPR + (VEC ? 0 : 32);
+template <int TPR, int V, bool VEC> constexpr int kGradSmem = (kAhead * 2 * kSlot<TPR, V, VEC> * (kBlock<TPR> / TPR) + 4 * V * TPR) * 4;
 template <int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t rows, int64_t cols, float eps,
-    float *__restrict__ dx, float *__restrict__ partial) {
-    using R          = Row<TPR, V, VEC>;
-    constexpr int RPB = kBlock<TPR> / TPR;
+    float *__restrict__ dx, float *__restrict__ partial, int pieces) {
+    using R               = Row<TPR, V, VEC>;
+    constexpr int THREADS = kBlock<TPR>, RPB = THREADS / TPR, SLOT = kSlot<TPR, V, VEC>;
+    extern __shared__ __align__(128) float smem[];
     __shared__ float words1[1][32], words2[4][32];
     griddep_wait();
     griddep_launch_dependents();
-    const int t          = threadIdx.x % TPR;
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    float *ring    = smem + group * kAhead * 2 * SLOT; // [row][x, dout], column 0 up to three values behind the beginning
+    float *gamma_s = smem + RPB * kAhead * 2 * SLOT;
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    const int64_t step = (int64_t)gridDim.x * RPB, row0 = (int64_t)blockIdx.x * RPB + group;
+    auto skew_of = [&](int64_t row) { return VEC || !pieces ? 0 : (int)((row * cols) & 3); };
+    auto fetch   = [&](int64_t row, int at) {
+        if (row < rows) {
+            const int skew = skew_of(row);
+            row_copy<TPR, V, VEC>(ring_at + (at * 2 * SLOT + skew) * 4, x + row * cols, cols, skew, pieces != 0, t);
+            row_copy<TPR, V, VEC>(ring_at + ((at * 2 + 1) * SLOT + skew) * 4, dout + row * cols, cols, skew, pieces != 0, t);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+        fetch(row0 + i * step, i);
+    for (int c = threadIdx.x; c < 4 * V * TPR; c += THREADS)
+        gamma_s[c] = c < cols ? (gamma ? gamma[c] : 1.0f) : 0.0f;
+    __syncthreads();
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
-    float gm[4 * V], sum_g[4 * V], sum_b[4 * V];
+    float sum_g[4 * V], sum_b[4 * V];
 #pragma unroll
     for (int i = 0; i < 4 * V; ++i)
-        gm[i] = 1.0f, sum_g[i] = sum_b[i] = 0.0f;
-    if (gamma)
-        R::load(gm, gamma, cols, t);
-    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < rows; row += (int64_t)gridDim.x * RPB) {
+        sum_g[i] = sum_b[i] = 0.0f;
+    int at = 0;
+    const int64_t warp_row = TPR < 32 ? (int64_t)blockIdx.x * RPB + (threadIdx.x >> 5) * (32 / (TPR < 32 ? TPR : 32)) : row0; // the warp's first
+    for (int64_t row = row0; row - row0 + warp_row < rows; row += step) { // whole warps, or the whole block
+        if (!VEC && TPR <= 32)
+            __syncwarp(); // the slot's last row has been read (a block's exchanges come behind its reads)
+        fetch(row + (kAhead - 1) * step, at == 0 ? kAhead - 1 : at - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        if (!VEC)
+            row_sync<TPR>(); // the others' copies
         float v[4 * V], dy[4 * V];
-        R::load(v, x + row * cols, cols, t);
-        R::load(dy, dout + row * cols, cols, t);
+        row_read<TPR, V, VEC>(v, ring + at * 2 * SLOT + skew_of(row), cols, t);
+        row_read<TPR, V, VEC>(dy, ring + (at * 2 + 1) * SLOT + skew_of(row), cols, t);
+        const bool here = TPR >= 32 || row < rows; // a warp's last rows may not be: what their slots hold is not used
+        if (!here)
+#pragma unroll
+            for (int i = 0; i < 4 * V; ++i)
+                v[i] = dy[i] = 0.0f;
+        at = at == kAhead - 1 ? 0 : at + 1;
         float sum[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < 4 * V; ++i)
@@ -203,18 +288,20 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
         row_sums<TPR>(sum, words1);
         const float mean = __fmul_rn(sum[0], inv_cols);
         float s[4]       = {0.0f, 0.0f, 0.0f, 0.0f}; // of d, d^2, g, g d
+        float g[4 * V];
+        row_read<TPR, V, VEC>(g, gamma_s, cols, t);
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int i   = 4 * j + q;
                 const float d = R::column(t, j, q) < cols ? __fsub_rn(v[i], mean) : 0.0f;
-                const float g = __fmul_rn(dy[i], gm[i]);
+                g[i]          = __fmul_rn(dy[i], g[i]);
                 v[i]          = d;
                 s[0]          = __fadd_rn(s[0], d);
                 s[1]          = __fmaf_rn(d, d, s[1]);
-                s[2]          = __fadd_rn(s[2], g);
-                s[3]          = __fmaf_rn(g, d, s[3]);
+                s[2]          = __fadd_rn(s[2], g[i]);
+                s[3]          = __fmaf_rn(g[i], d, s[3]);
             }
         row_sums<TPR>(s, words2);
         float rest;
@@ -223,41 +310,36 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
         const float mh = __fmul_rn(__fmul_rn(__fsub_rn(s[3], __fmul_rn(rest, s[2])), r), inv_cols); // mean of g h
 #pragma unroll
         for (int i = 0; i < 4 * V; ++i) {
-            const float h = __fmul_rn(__fsub_rn(v[i], rest), r);
+            const float h = here ? __fmul_rn(__fsub_rn(v[i], rest), r) : 0.0f;
             sum_g[i]      = __fmaf_rn(dy[i], h, sum_g[i]);
             sum_b[i]      = __fadd_rn(sum_b[i], dy[i]);
-            v[i]          = __fmul_rn(r, __fsub_rn(__fsub_rn(__fmul_rn(dy[i], gm[i]), mg), __fmul_rn(h, mh)));
+            v[i]          = __fmul_rn(r, __fsub_rn(__fsub_rn(g[i], mg), __fmul_rn(h, mh)));
         }
-        if (dx)
+        if (dx && here)
             R::store(dx + row * cols, v, cols, t);
     }
     if (!partial)
         return;
-    if (RPB > 1) { // the groups of the block, one after the other
-        extern __shared__ float sums[]; // [2][cols]
-        for (int group = 0; group < RPB; ++group) {
-            if ((int)threadIdx.x / TPR == group)
+    float *mine = partial + (int64_t)blockIdx.x * 2 * cols;
+    if (RPB > 1) { // the warps' sums, one after the other
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads(); // no row is at work any more
+        float *sums = smem; // [2][4 V TPR]
+        for (int who = 0; who < RPB; ++who) {
+            if (group == who)
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int64_t c = R::column(t, j, q);
-                        if (c < cols) {
-                            sums[c]        = group ? __fadd_rn(sums[c], sum_g[4 * j + q]) : sum_g[4 * j + q];
-                            sums[cols + c] = group ? __fadd_rn(sums[cols + c], sum_b[4 * j + q]) : sum_b[4 * j + q];
-                        }
-                    }
+                for (int i = 0; i < 4 * V; ++i) {
+                    const int64_t c = R::column(t, i >> 2, i & 3);
+                    sums[c]               = who ? __fadd_rn(sums[c], sum_g[i]) : sum_g[i];
+                    sums[4 * V * TPR + c] = who ? __fadd_rn(sums[4 * V * TPR + c], sum_b[i]) : sum_b[i];
+                }
             __syncthreads();
         }
-        for (int64_t c = threadIdx.x; c < 2 * cols; c += kBlock<TPR>)
-            partial[(int64_t)blockIdx.x * 2 * cols + c] = sums[c];
+        for (int64_t c = threadIdx.x; c < cols; c += THREADS)
+            mine[c] = sums[c], mine[cols + c] = sums[4 * V * TPR + c];
     } else {
-        R::store(partial + (int64_t)blockIdx.x * 2 * cols, sum_g, cols, t);
-        float *to = partial + ((int64_t)blockIdx.x * 2 + 1) * cols;
-        if (VEC) // cols is a multiple of four: aligned like the first half
-            R::store(to, sum_b, cols, t);
-        else
-            Row<TPR, V, false>::store(to, sum_b, cols, t);
+        R::store(mine, sum_g, cols, t);
+        R::store(mine + cols, sum_b, cols, t); // VEC: cols is a multiple of four, aligned like the first half
     }
 }
 
@@ -358,22 +440,24 @@ ct_status launch_norm(const float *x, const float *gamma, const float *beta, int
     return CT_OK;
 }
 
-// How many blocks the gradient runs, each with a part of the columns' sums.
-template <int TPR, int V> int64_t grad_blocks(const DeviceState *st, int64_t rows) {
-    constexpr int RPB = kBlock<TPR> / TPR;
-    return std::min<int64_t>((rows + RPB - 1) / RPB, (int64_t)st->sm_count * (1024 / kBlock<TPR>));
-}
-
-template <int TPR, int V>
+template <int TPR, int V, bool VEC>
 ct_status launch_norm_grad(
-    const float *x, const float *gamma, const float *dout, int64_t rows, int64_t cols, float eps, float *dx, float *partial, int64_t blocks, bool vec) {
-    const size_t smem = kBlock<TPR> > TPR && partial ? (size_t)cols * 8 : 0;
-    if (vec)
-        CT_CUDA(launch_dependent(layer_norm_grad_kernel<TPR, V, true>, dim3((unsigned)blocks), dim3(kBlock<TPR>), smem, stream(), x, gamma, dout, rows,
-                                 cols, eps, dx, partial));
-    else
-        CT_CUDA(launch_dependent(layer_norm_grad_kernel<TPR, V, false>, dim3((unsigned)blocks), dim3(kBlock<TPR>), smem, stream(), x, gamma, dout, rows,
-                                 cols, eps, dx, partial));
+    const DeviceState *st, const float *x, const float *gamma, const float *dout, int64_t rows, int64_t cols, float eps, float *dx, bool sums, Scratch &partial,
+    int64_t *blocks) {
+    constexpr int SMEM = kGradSmem<TPR, V, VEC>, RPB = kBlock<TPR> / TPR;
+    auto kernel        = layer_norm_grad_kernel<TPR, V, VEC>;
+    static int resident[16] = {}; // blocks to an SM, per device; under the entry points' lock
+    int &fit                = resident[st->device & 15];
+    if (fit == 0) {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        CT_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, kBlock<TPR>, SMEM));
+        fit = std::max(fit, 1);
+    }
+    *blocks = std::min<int64_t>((rows + RPB - 1) / RPB, (int64_t)st->sm_count * fit);
+    if (sums)
+        CT_TRY(partial.get((size_t)*blocks * 8 * cols));
+    CT_CUDA(launch_dependent(kernel, dim3((unsigned)*blocks), dim3(kBlock<TPR>), SMEM, stream(), x, gamma, dout, rows, cols, eps, dx,
+                             sums ? partial.as<float>() : nullptr, aligned16(x) && aligned16(dout) ? 1 : 0));
     CT_LAUNCH_CHECK("layer_norm_grad");
     return CT_OK;
 }
@@ -409,14 +493,36 @@ ct_status ct_layer_norm(
     const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(out) && (!gamma || aligned16(gamma)) && (!beta || aligned16(beta));
     const float e  = (float)eps;
     const bool few = rows < st->sm_count * 4;
+#define CT_NORM(TPR, V) launch_norm<TPR, V>(x, gamma, beta, rows, cols, e, out, vec)
+    if (cols <= 32)
+        return CT_NORM(8, 1);
+    if (cols <= 64)
+        return CT_NORM(8, 2);
+    if (cols <= 128)
+        return CT_NORM(16, 2);
     if (cols <= 256)
-        return launch_norm<32, 2>(x, gamma, beta, rows, cols, e, out, vec);
+        return CT_NORM(32, 2);
+    if (few && cols <= 1024) // a row spread over more threads is there sooner
+        return CT_NORM(256, 1);
+    if (cols <= 512)
+        return CT_NORM(32, 4);
+    if (cols <= 768)
+        return CT_NORM(32, 6);
+    if (cols <= 896)
+        return CT_NORM(32, 7);
     if (cols <= 1024)
-        return few ? launch_norm<256, 1>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<32, 8>(x, gamma, beta, rows, cols, e, out, vec);
+        return CT_NORM(32, 8);
+    if (few && cols <= 4096)
+        return CT_NORM(1024, 1);
+    if (cols <= 2048)
+        return CT_NORM(128, 4);
     if (cols <= 4096)
-        return few ? launch_norm<1024, 1>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<256, 4>(x, gamma, beta, rows, cols, e, out, vec);
+        return vec ? CT_NORM(256, 4) : CT_NORM(128, 8);
+    if (few && cols <= 8192)
+        return CT_NORM(1024, 2);
     if (cols <= 8192)
-        return few ? launch_norm<1024, 2>(x, gamma, beta, rows, cols, e, out, vec) : launch_norm<512, 4>(x, gamma, beta, rows, cols, e, out, vec);
+        return CT_NORM(256, 8);
+#undef CT_NORM
     if (cols <= 16384)
         return launch_norm<1024, 4>(x, gamma, beta, rows, cols, e, out, vec);
     if (cols <= 32768)
@@ -448,23 +554,33 @@ ct_status ct_layer_norm_grad(
     int64_t parts = 0;
     if (cols <= 8192) {
         const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(dout) && (!dx || aligned16(dx)) && (!gamma || aligned16(gamma));
-#define CT_NORM_GRAD(TPR, V)                                                                                                           \
-    do {                                                                                                                               \
-        parts = grad_blocks<TPR, V>(st, rows);                                                                                         \
-        if (sums)                                                                                                                      \
-            CT_TRY(scratch.get((size_t)parts * 8 * cols));                                                                             \
-        CT_TRY((launch_norm_grad<TPR, V>(x, gamma, dout, rows, cols, e, dx, sums ? scratch.as<float>() : nullptr, parts, vec)));          \
-    } while (0)
-        if (cols <= 256)
+#define CT_NORM_GRAD(TPR, V)                                                                                                      \
+    CT_TRY(vec ? (launch_norm_grad<TPR, V, true>(st, x, gamma, dout, rows, cols, e, dx, sums, scratch, &parts))                  \
+               : (launch_norm_grad<TPR, V, false>(st, x, gamma, dout, rows, cols, e, dx, sums, scratch, &parts)))
+        if (cols <= 32)
+            CT_NORM_GRAD(8, 1);
+        else if (cols <= 64)
+            CT_NORM_GRAD(8, 2);
+        else if (cols <= 128)
+            CT_NORM_GRAD(16, 2);
+        else if (cols <= 256)
             CT_NORM_GRAD(32, 2);
+        else if (cols <= 512)
+            CT_NORM_GRAD(32, 4);
+        else if (cols <= 768 && rows >= st->sm_count * 8)
+            CT_NORM_GRAD(32, 6);
+        else if (cols <= 896 && rows >= st->sm_count * 8)
+            CT_NORM_GRAD(32, 7);
+        else if (cols <= 1024 && rows >= st->sm_count * 8)
+            CT_NORM_GRAD(32, 8);
         else if (cols <= 1024)
             CT_NORM_GRAD(256, 1);
         else if (cols <= 2048)
             CT_NORM_GRAD(256, 2);
         else if (cols <= 4096)
-            CT_NORM_GRAD(512, 2);
+            CT_NORM_GRAD(256, 4);
         else
-            CT_NORM_GRAD(1024, 2);
+            CT_NORM_GRAD(512, 4);
 #undef CT_NORM_GRAD
     } else {
         const int64_t strips = (cols + 255) / 256;
