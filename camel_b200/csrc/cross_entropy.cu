@@ -136,17 +136,17 @@ struct SumExp {
     }
 };
 
-// A row's parts: 32 rows to a block, a warp takes every eighth part.
+// A row's parts: eight rows to a block, a lane group of eight takes every 32nd part (with 32 rows to a block 64 rows of 500 parts took 23 us).
 __global__ void __launch_bounds__(256) ce_join_kernel(
     const float2 *__restrict__ part, int slots, const float *__restrict__ at_target, const int64_t *__restrict__ targets, int64_t m, int64_t n,
     float *__restrict__ loss, float *__restrict__ lse, const uint32_t *__restrict__ flags) {
-    __shared__ float2 words[8][32];
+    __shared__ float2 words[32][8];
     griddep_wait();
     griddep_launch_dependents();
     if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the parts were not computed
         return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+    const int at = threadIdx.x & 7, group = threadIdx.x >> 3;
+    const int64_t row = (int64_t)blockIdx.x * 8 + at;
     auto join = [](float2 a, float2 b) {
         const float top  = fmaxf(a.x, b.x);
         const float base = top == -INFINITY ? 0.0f : top;
@@ -155,13 +155,14 @@ __global__ void __launch_bounds__(256) ce_join_kernel(
     };
     float2 v = make_float2(-INFINITY, 0.0f);
     if (row < m)
-        for (int s = warp; s < slots; s += 8)
+#pragma unroll 4
+        for (int s = group; s < slots; s += 32)
             v = join(v, part[(int64_t)s * m + row]);
-    words[warp][lane] = v;
+    words[group][at] = v;
     __syncthreads();
-    if (warp == 0 && row < m) {
-        for (int w = 1; w < 8; ++w)
-            v = join(v, words[w][lane]);
+    if (group == 0 && row < m) {
+        for (int w = 1; w < 32; ++w)
+            v = join(v, words[w][at]);
         const float l   = __fadd_rn(v.x == -INFINITY && v.y == v.y ? 0.0f : v.x, logf(v.y));
         const int64_t t = targets[row];
         if (lse)
@@ -190,7 +191,7 @@ ct_status ce_fused(
     SumExp::Params e{bias, targets, s.as<float2>(pp), s.as<float>(tp)};
     CT_TRY(pair ? (launch<SumExp, 256, 2, false, true>(st, px, pw, p, e, 1, "cross_entropy"))
                 : (launch<SumExp, 128, 1, false, true>(st, px, pw, p, e, 1, "cross_entropy")));
-    CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((m + 31) / 32)), dim3(256), 0, stream(), (const float2 *)e.part, (int)slots,
+    CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((m + 7) / 8)), dim3(256), 0, stream(), (const float2 *)e.part, (int)slots,
                              (const float *)e.at_target, targets, m, n, loss, lse, (const uint32_t *)st->flags_dev));
     CT_LAUNCH_CHECK("ce_join");
     return CT_OK;
@@ -322,6 +323,134 @@ ct_status ce_grad_fused(
     return CT_OK;
 }
 
+// ---- few classes: logits of up to kFewClasses columns, as the library's few-column products give them ----
+
+constexpr int kFewClasses = 32;
+
+// A thread per row.
+__global__ void __launch_bounds__(256) ce_few_kernel(
+    const float *__restrict__ z, const int64_t *__restrict__ targets, int64_t m, int n, float *__restrict__ loss, float *__restrict__ lse) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= m)
+        return;
+    const float *src = z + row * n;
+    float top = -INFINITY, sum = 0.0f;
+    for (int c = 0; c < n; ++c)
+        top = fmaxf(top, src[c]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (int c = 0; c < n; ++c)
+        sum = __fadd_rn(sum, expf(__fsub_rn(src[c], base))); // a NaN shows here
+    const float l   = __fadd_rn(base, logf(sum));
+    const int64_t t = targets[row];
+    if (lse)
+        lse[row] = l;
+    if (loss)
+        loss[row] = t >= 0 && t < n ? __fsub_rn(l, src[t]) : 0.0f;
+}
+
+// d in the place of the logits, and the columns' sums over the block's 256 rows (partial may be null).
+__global__ void __launch_bounds__(256) ce_few_slopes_kernel(
+    float *__restrict__ z, const int64_t *__restrict__ targets, const float *__restrict__ lse, const float *__restrict__ dloss, int64_t m, int n,
+    double *__restrict__ partial) {
+    __shared__ float tile[256 * (kFewClasses + 1)];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t row0 = (int64_t)blockIdx.x * 256;
+    const int rows = (int)(m - row0 < 256 ? m - row0 : 256), pitch = n | 1;
+    for (int i = threadIdx.x; i < rows * n; i += 256)
+        tile[i / n * pitch + i % n] = z[row0 * n + i];
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        const int64_t row = row0 + threadIdx.x, t = targets[row];
+        const bool has = t >= 0 && t < n;
+        const float l = lse[row], by = dloss ? dloss[row] : 1.0f;
+        float *mine = tile + threadIdx.x * pitch;
+        for (int c = 0; c < n; ++c) {
+            const float p = expf(__fsub_rn(mine[c], l));
+            mine[c]       = has ? __fmul_rn(by, c == t ? __fsub_rn(p, 1.0f) : p) : 0.0f;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * n; i += 256)
+        z[row0 * n + i] = tile[i / n * pitch + i % n];
+    if (partial)
+        for (int c = threadIdx.x >> 5; c < n; c += 8) {
+            float s = 0.0f;
+            for (int r = threadIdx.x & 31; r < rows; r += 32)
+                s = __fadd_rn(s, tile[r * pitch + c]);
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+                s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, o));
+            if ((threadIdx.x & 31) == 0)
+                partial[(int64_t)blockIdx.x * n + c] = (double)s;
+        }
+}
+
+// dx[i][c] = sum over j of d[i][j] w[c][j]: a thread has a column of dx and its weights in registers, d's rows come from shared memory.  Bound
+// by the store of dx; as a product through planes, whose k is a tenth of a stage, 60000 x 10 x 785 took 180 us.
+template <int N>
+__global__ void __launch_bounds__(256) ce_few_back_kernel(
+    const float *__restrict__ d, const float *__restrict__ w, int64_t m, int64_t k, int n, float *__restrict__ dx) {
+    constexpr int R = 64;
+    __shared__ __align__(16) float tile[R][N];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x;
+    float mine[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        mine[j] = c < k && j < n ? w[c * n + j] : 0.0f;
+    for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < m; row0 += (int64_t)gridDim.x * R) {
+        const int rows = (int)(m - row0 < R ? m - row0 : R);
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * N; i += 256)
+            tile[i / N][i % N] = i % N < n ? d[(row0 + i / N) * n + i % N] : 0.0f;
+        __syncthreads();
+        if (c < k)
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(&tile[r][j]);
+                    s = __fmaf_rn(q.x, mine[j], s), s = __fmaf_rn(q.y, mine[j + 1], s), s = __fmaf_rn(q.z, mine[j + 2], s), s = __fmaf_rn(q.w, mine[j + 3], s);
+                }
+                __stcs(dx + (row0 + r) * k + c, s);
+            }
+    }
+}
+
+ct_status ce_few_grad(
+    DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
+    int64_t n, float *dx, float *dw, float *dbias) {
+    const int64_t blocks = (m + 255) / 256;
+    fused::Parts parts;
+    const size_t zp = parts.take((size_t)(m * n) * 4), pp = parts.take(dbias ? (size_t)(blocks * n) * 8 : 0);
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    float *d = s.as<float>(zp);
+    CT_TRY(ct_dense(x, w, bias, m, k, n, CT_ACT_NONE, d, nullptr));
+    CT_CUDA(launch_dependent(ce_few_slopes_kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), d, targets, lse, dloss, m, (int)n,
+                             dbias ? s.as<double>(pp) : nullptr));
+    CT_LAUNCH_CHECK("ce_few_slopes");
+    if (dbias)
+        CT_TRY(fused::join_columns(s.as<const double>(pp), blocks, n, false, dbias, nullptr));
+    if (dw && k > 0)
+        CT_TRY(ct_matmul_tn(x, d, k, m, n, dw));
+    if (dx && k > 0) {
+        const int64_t strips = (k + 255) / 256;
+        if (strips > 65535)
+            return fail(CT_ERR_TOO_LARGE, "dense_cross_entropy_grad: too many columns");
+        const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 8 / strips)), (unsigned)strips);
+        auto back = n <= 4 ? ce_few_back_kernel<4> : n <= 8 ? ce_few_back_kernel<8> : n <= 12 ? ce_few_back_kernel<12> : n <= 16 ? ce_few_back_kernel<16> : n <= 24 ? ce_few_back_kernel<24> : ce_few_back_kernel<32>;
+        CT_CUDA(launch_dependent(back, grid, dim3(256), 0, stream(), (const float *)d, w, m, k, (int)n, dx));
+        CT_LAUNCH_CHECK("ce_few_back");
+    }
+    return CT_OK;
+}
+
 ct_status check_ce(const char *name, const void *x, const void *w, const void *targets, int64_t m, int64_t k, int64_t n) {
     if (m < 0 || k < 0 || n < 0)
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
@@ -353,12 +482,19 @@ ct_status ct_dense_cross_entropy(
     if (m == 0)
         return CT_OK;
     ProfScope prof("cross_entropy");
-    const bool fused_form = n > 32 && k > 0 && ct_get_precision() == CT_PREC_3XTF32;
+    const bool fused_form = n > kFewClasses && k > 0 && ct_get_precision() == CT_PREC_3XTF32;
     if (fused_form && m > fused::kFewRows)
         return ce_fused(st, x, w, bias, targets, m, k, n, loss, lse);
-    const int64_t piece = rows_at_once(m, n);
+    const int64_t piece = n <= kFewClasses ? m : rows_at_once(m, n);
     Scratch logits;
     CT_TRY(logits.get((size_t)(piece * n) * 4));
+    if (n <= kFewClasses) {
+        CT_TRY(ct_dense(x, w, bias, m, k, n, CT_ACT_NONE, logits.as<float>(), nullptr));
+        CT_CUDA(launch_dependent(ce_few_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream(), logits.as<const float>(), targets, m, (int)n,
+                                 loss, lse));
+        CT_LAUNCH_CHECK("ce_few");
+        return CT_OK;
+    }
     for (int64_t r = 0; r < m; r += piece) {
         const int64_t rows = std::min(piece, m - r);
         if (fused_form)
@@ -389,8 +525,10 @@ ct_status ct_dense_cross_entropy_grad(
         return CT_OK;
     }
     ProfScope prof("cross_entropy_grad");
-    if (n > 32 && k > 0 && ct_get_precision() == CT_PREC_3XTF32)
+    if (n > kFewClasses && k > 0 && ct_get_precision() == CT_PREC_3XTF32)
         return ce_grad_fused(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+    if (n <= kFewClasses)
+        return ce_few_grad(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     const int64_t piece = rows_at_once(m, n);
     Scratch logits, turned, sums;
     CT_TRY(logits.get((size_t)(piece * n) * 4));

@@ -24,7 +24,7 @@ struct FewParams {
 
 // GATE < 0: no gate; column c of half 1 is column 64 + c of the strip.
 template <int M, int GATE>
-__global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(256, M == 1 ? 4 : M == 4 ? 3 : 2) few_rows_kernel(const __grid_constant__ FewParams p) {
     __shared__ float xs[M][kPart];
     __shared__ __align__(16) float sums[8][M][128]; // [0]: the CTA's, read by the cluster
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = lane >> 4;
@@ -40,16 +40,10 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ F
         acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0.0f;
     const float *w = p.w[GATE < 0 ? 0 : half];
     for (int64_t from = k0; from < k1; from += kPart) {
-        const int count = (int)min((int64_t)kPart, k1 - from);
-        __syncthreads(); // the last part's have been read
-        for (int i = threadIdx.x; i < M * kPart; i += 256) {
-            const int r = i / kPart, c = i % kPart;
-            xs[r][c] = r < p.m && c < count ? p.x[(int64_t)r * p.k + from + c] : 0.0f;
-        }
-        __syncthreads();
+        const int count  = (int)min((int64_t)kPart, k1 - from);
         const float *src = w + from * p.n + col;
-        constexpr int U = M <= 4 ? 16 : 8; // loads in flight
-        for (int i0 = warp; i0 < count; i0 += 8 * U) {
+        constexpr int U  = 8; // loads in flight
+        for (int i0 = warp; i0 < (count + 63) / 64 * 64; i0 += 8 * U) {
             float4 v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -65,6 +59,14 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ F
                         v[u].z = col + 2 < p.n ? __ldcs(at + 2) : 0.0f, v[u].w = col + 3 < p.n ? __ldcs(at + 3) : 0.0f;
                     }
                 }
+            }
+            if (i0 == warp) { // x behind the first weights
+                __syncthreads(); // the last part's has been read
+                for (int i = threadIdx.x; i < M * count; i += 256) {
+                    const int r = i / count, c = i % count;
+                    xs[r][c] = r < p.m ? p.x[(int64_t)r * p.k + from + c] : 0.0f;
+                }
+                __syncthreads();
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
