@@ -2,9 +2,9 @@
 //
 //   lse = log(sum exp z), loss = lse - z[target];  d = dloss (exp(z - lse) - [target]),  dx = d . w^T, dw = x^T . d, dbias = column sums of d
 //
-// Forward: a product whose tiles are not stored (fused_product.cuh).  A thread of the epilogue has a row and half of the tile's columns in
+// Forward: a product whose tiles are not stored (fused_product.cuh).  A thread of the epilogue has a row and a quarter of the tile's columns in
 // registers; it leaves their maximum, the sum of exponentials about it and, where it meets the target, that logit.  ce_join_kernel adds
-// up a row's parts: 16 bytes for 256 logits.
+// up a row's parts: 32 bytes for 256 logits.
 // Gradient: the same product again, whose epilogue turns the logits into d / dloss = exp(z - lse) - [target], in [-1, 1], as planes of float16
 // pairs under one scale.  A piece of the vocabulary at a time they are the left operand of dx += d . w^T as they lie (rows weighted by
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
@@ -103,7 +103,7 @@ struct SumExp {
     struct Params {
         const float *bias;
         const int64_t *targets;
-        float2 *part; // [2 tiles_n][m]: maximum, sum
+        float2 *part; // [4 tiles_n][m]: maximum, sum
         float *at_target;
     };
     template <int COLS>
@@ -177,7 +177,7 @@ ct_status ce_fused(
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
     const bool pair     = m > 128 && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
-    const int64_t slots = pair ? (n + 255) / 256 * 2 : (n + 127) / 128 * 2;
+    const int64_t slots = pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
     const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
                  wm = parts.take((size_t)scales(ln) * 4), pp = parts.take((size_t)(slots * m) * 8), tp = parts.take((size_t)m * 4);
@@ -225,36 +225,36 @@ struct Slopes {
         if (rows == 0)
             return;
 #pragma unroll
-        for (int g = 0; g < COLS / 32; ++g) {
-            const int64_t col = col0 + g * 32;
+        for (int g = 0; g < COLS / 16; ++g) {
+            const int64_t col = col0 + g * 16;
             if (col >= p.n)
                 break;
-            float *d = z + g * 32;
-            logits_of<32>(p, e.bias, d, rs, col);
+            float *d = z + g * 16;
+            logits_of<16>(p, e.bias, d, rs, col);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < 16; ++j) {
                 const float v = exp2_fast(__fmul_rn(__fsub_rn(d[j], l), kLog2e));
-                d[j]          = has ? __fmul_rn(at == g * 32 + j ? __fsub_rn(v, 1.0f) : v, kSlopeScale) : 0.0f;
+                d[j]          = has ? __fmul_rn(at == g * 16 + j ? __fsub_rn(v, 1.0f) : v, kSlopeScale) : 0.0f;
             }
-            // rows of 128 bytes, hi terms and lo terms: 16-byte slots XOR-swizzled by row
+            // rows of 64 bytes, hi terms and lo terms: 16-byte slots XOR-swizzled by row
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 __half2 hi[4], lo[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     fused::split2(d[8 * j + 2 * q], d[8 * j + 2 * q + 1], hi[q], lo[q]);
-                *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4))       = *reinterpret_cast<uint4 *>(hi);
-                *reinterpret_cast<uint4 *>(stage + lane * 128 + (((j + 4) ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4 *>(lo);
+                *reinterpret_cast<uint4 *>(stage + fused::stage_slot(lane, j))     = *reinterpret_cast<uint4 *>(hi);
+                *reinterpret_cast<uint4 *>(stage + fused::stage_slot(lane, j + 2)) = *reinterpret_cast<uint4 *>(lo);
             }
             __syncwarp();
-            const int sub = lane & 7, rr = lane >> 3;
-            __half *to = (sub < 4 ? e.hi : e.lo) + (row0 + rr) * e.ld + col + (sub & 3) * 8;
-            if (col + (sub & 3) * 8 < p.n) // to the end of the slot, which ld covers
+            const int sub = lane & 3, rr = lane >> 2;
+            __half *to = (sub < 2 ? e.hi : e.lo) + (row0 + rr) * e.ld + col + (sub & 1) * 8;
+            if (col + (sub & 1) * 8 < p.n) // to the end of the slot, which ld covers
 #pragma unroll
-                for (int it = 0; it < 8; ++it) {
-                    const int r = it * 4 + rr;
+                for (int it = 0; it < 4; ++it) {
+                    const int r = it * 8 + rr;
                     if (r < rows)
-                        *reinterpret_cast<uint4 *>(to + (int64_t)it * 4 * e.ld) = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((sub ^ (r & 7)) << 4));
+                        *reinterpret_cast<uint4 *>(to + (int64_t)it * 8 * e.ld) = *reinterpret_cast<const uint4 *>(stage + fused::stage_slot(r, sub));
                 }
             __syncwarp();
         }

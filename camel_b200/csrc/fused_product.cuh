@@ -16,7 +16,8 @@
 // columns of 64 values of k in 8 KB, the next 64 columns behind them.
 //
 // Structure as gemm_half.cu: pairs of CTAs (cta_group::2) with tiles of 256 x 256, or single CTAs with 128 x 128 and two sets of
-// accumulators; TMA warp, issuing warp, eight epilogue warps; a lane has a row and its registers columns.  All waits are bounded.
+// accumulators; TMA warp, issuing warp, sixteen epilogue warps; a lane has a row and its registers a quarter of the tile's columns.  What
+// an epilogue does has the next tile's first 256 values of k to hide behind, some 8000 clocks.  All waits are bounded.
 #pragma once
 
 #include "common.cuh"
@@ -80,13 +81,13 @@ struct Product {
 };
 
 constexpr int kRows     = 128; // accumulator rows of a CTA
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kThreads  = 64 + 32 * kEpiWarps;
 constexpr int kTile     = 128 * 128;  // bytes of one plane of one operand in a stage
 constexpr int kStage    = 4 * kTile;
 constexpr int kStages   = 3;
 constexpr int kChunk    = 4; // stages per drain of the leading accumulator
-constexpr int kSmem     = kStages * kStage + kEpiWarps * 4096 + 1024;
+constexpr int kSmem     = kStages * kStage + kEpiWarps * 2048 + 1024;
 
 #ifdef __CUDACC__
 
@@ -110,13 +111,13 @@ __device__ __forceinline__ void tile_of(const Product &p, int tile, int &tm, int
 }
 
 // EPI: kTwin - the tile's columns are half of one matrix and half of another, and a thread has the same columns of both;
-// Params; store(p, e, acc, row0, lane, col0, z, stage): acc holds unscaled sums of row row0 + lane, columns col0 .. (twin: COLS / 2
-// columns from col0 of the first matrix, then those of the second); stage is the warp's 4 KB.
+// Params; store(p, e, acc, row0, lane, col0, z, part, stage): acc holds unscaled sums of row row0 + lane, columns col0 .. (twin: COLS / 2
+// columns from col0 of the first matrix, then those of the second), the part-th quarter of the tile's; stage is the warp's 2 KB.
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ typename EPI::Params e) {
     static_assert(BN / CG == 128, "128 columns of B to a CTA");
-    constexpr int SETS = 512 / (2 * BN), COLS = BN / 2;
+    constexpr int SETS = 512 / (2 * BN), COLS = BN / 4;
     const int rank   = CG == 2 ? (int)cluster_rank() : 0;
     const int first  = (int)blockIdx.x / CG;
     const int stride = (int)gridDim.x / CG;
@@ -321,8 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ===== epilogue =====
         const int quarter = warp & 3;       // TMEM lanes this warp may read: 32 * quarter ..
-        const int half    = (warp - 2) >> 2; // which half of the tile's columns
-        uint8_t *stage = smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStage + (warp - 2) * 4096;
+        const int part    = (warp - 2) >> 2; // which quarter of the tile's columns
+        uint8_t *stage = smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStage + (warp - 2) * 2048;
         uint32_t full_phase = 0;
         int i               = 0;
         for (int tile = first; tile < p.total; tile += stride, ++i) {
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float acc[COLS];
             const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(set * 2 * BN);
             auto column = [&](int c) { // of the accumulator, of acc[c]
-                return !EPI::kTwin ? half * COLS + c : (c < COLS / 2 ? half * (COLS / 2) + c : BN / 2 + half * (COLS / 2) + c - COLS / 2);
+                return !EPI::kTwin ? part * COLS + c : (c < COLS / 2 ? part * (COLS / 2) + c : BN / 2 + part * (COLS / 2) + c - COLS / 2);
             };
             bool ok    = true;
             auto await = [&](int which) {
@@ -382,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok)
                 break;
             const int64_t row0 = (int64_t)(tm * CG + rank) * kRows + quarter * 32;
-            const int64_t col0 = EPI::kTwin ? (int64_t)tn * (BN / 2) + half * (COLS / 2) : (int64_t)tn * BN + half * COLS;
-            EPI::template store<COLS>(p, e, acc, row0, lane, col0, tz, tn * 2 + half, stage);
+            const int64_t col0 = EPI::kTwin ? (int64_t)tn * (BN / 2) + part * (COLS / 2) : (int64_t)tn * BN + part * COLS;
+            EPI::template store<COLS>(p, e, acc, row0, lane, col0, tz, tn * 4 + part, stage);
         }
     }
 
@@ -408,21 +409,23 @@ __device__ __forceinline__ float4 scales4(const float *scale, int64_t col) {
     return scale ? __ldg(reinterpret_cast<const float4 *>(scale + col)) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
 }
 
-// 32 x 32 values of a warp, lane = row, to row-major memory through the warp's 4 KB: float4 slots XOR-swizzled by row, written as
-// runs of 128 bytes per row.  value(j): column j of the lane's row.  dst: row 0, column 0 of the block; `cols` of them exist.
+// 32 rows x 16 columns of a warp, lane = row, to row-major memory through the warp's 2 KB: float4 slots XOR-swizzled by row, written
+// as runs of 64 bytes per row.  value(j): column j of the lane's row.  dst: row 0, column 0 of the block; `cols` of them exist, from `skip` on.
+__device__ __forceinline__ uint32_t stage_slot(int row, int slot) { return (uint32_t)(row * 64 + ((slot ^ (row >> 1 & 3)) << 4)); }
 template <bool ADD, typename F>
-__device__ __forceinline__ void store_block(float *dst, int64_t stride, int rows, int cols, bool vec, uint8_t *stage, int lane, F &&value) {
+__device__ __forceinline__ void store_block(
+    float *dst, int64_t stride, int rows, int skip, int cols, bool vec, uint8_t *stage, int lane, F &&value) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<float4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(value(4 * j), value(4 * j + 1), value(4 * j + 2), value(4 * j + 3));
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4 *>(stage + stage_slot(lane, j)) = make_float4(value(4 * j), value(4 * j + 1), value(4 * j + 2), value(4 * j + 3));
     __syncwarp();
-    if (vec && cols == 32) {
-        const int sub = lane & 7, rr = lane >> 3;
+    if (vec && cols == 16 && skip == 0) {
+        const int sub = lane & 3, rr = lane >> 2;
         float *to = dst + rr * stride + sub * 4;
 #pragma unroll
-        for (int it = 0; it < 8; ++it, to += 4 * stride) {
-            const int r = it * 4 + rr;
-            float4 v    = *reinterpret_cast<const float4 *>(stage + r * 128 + ((sub ^ (r & 7)) << 4));
+        for (int it = 0; it < 4; ++it, to += 8 * stride) {
+            const int r = it * 8 + rr;
+            float4 v    = *reinterpret_cast<const float4 *>(stage + stage_slot(r, sub));
             if (r < rows) {
                 if (ADD) {
                     const float4 o = *reinterpret_cast<const float4 *>(to);
@@ -432,11 +435,12 @@ __device__ __forceinline__ void store_block(float *dst, int64_t stride, int rows
             }
         }
     } else {
-        float *to = dst + lane; // a column per lane
+        const int c = lane & 15; // a column per lane, two rows at a time
+        float *to   = dst + (int64_t)(lane >> 4) * stride + c;
 #pragma unroll 4
-        for (int r = 0; r < rows; ++r, to += stride) {
-            const float v = *reinterpret_cast<const float *>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-            if (lane < cols)
+        for (int r = lane >> 4; r < rows; r += 2, to += 2 * stride) {
+            const float v = *reinterpret_cast<const float *>(stage + stage_slot(r, c >> 2) + (c & 3) * 4);
+            if (c >= skip && c < cols)
                 *to = ADD ? __fadd_rn(*to, v) : v;
         }
     }
@@ -462,42 +466,32 @@ struct Store {
             return;
         const float rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
 #pragma unroll
-        for (int g = 0; g < COLS / 32; ++g) {
-            const int64_t col = col0 + g * 32;
+        for (int g = 0; g < COLS / 16; ++g) {
+            const int64_t col = col0 + g * 16;
             if (col >= p.n)
                 break;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const float4 c = scales4(p.col_scale, col + 4 * j);
-                float *a       = acc + g * 32 + 4 * j;
+                float *a       = acc + g * 16 + 4 * j;
                 a[0] = __fmul_rn(a[0], weight(rs, c.x)), a[1] = __fmul_rn(a[1], weight(rs, c.y));
                 a[2] = __fmul_rn(a[2], weight(rs, c.z)), a[3] = __fmul_rn(a[3], weight(rs, c.w));
             }
-            auto value     = [&](int j) { return acc[g * 32 + j]; };
+            auto value = [&](int j) { return acc[g * 16 + j]; };
+            // of the first matrix (or the only one), of the second, or of both where the block straddles its beginning
             const bool sec = e.out2 && col >= e.second;
-            // of the first matrix (or the only one), and of the second one's beginning where the block straddles it
-            float *base        = (sec ? e.out2 : e.out) + (int64_t)z * e.slice + row0 * e.stride;
-            const int64_t at   = sec ? col - e.second : col;
-            const int64_t many = e.n - at;
+            float *base    = (sec ? e.out2 : e.out) + (int64_t)z * e.slice + row0 * e.stride;
+            const int64_t at = sec ? col - e.second : col, many = e.n - at;
             if (many > 0) {
                 if (e.add)
-                    store_block<true>(base + at, e.stride, rows, many < 32 ? (int)many : 32, e.vec != 0, stage, lane, value);
+                    store_block<true>(base + at, e.stride, rows, 0, many < 16 ? (int)many : 16, e.vec != 0, stage, lane, value);
                 else
-                    store_block<false>(base + at, e.stride, rows, many < 32 ? (int)many : 32, e.vec != 0, stage, lane, value);
+                    store_block<false>(base + at, e.stride, rows, 0, many < 16 ? (int)many : 16, e.vec != 0, stage, lane, value);
             }
-            if (e.out2 && !sec && col + 32 > e.second) {
+            if (e.out2 && !sec && col + 16 > e.second) {
                 const int skip = (int)(e.second - col);
-                float *to      = e.out2 + (int64_t)z * e.slice + row0 * e.stride - skip;
-                const int cols = e.n < 32 - skip ? (int)e.n + skip : 32;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<float4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                        make_float4(value(4 * j), value(4 * j + 1), value(4 * j + 2), value(4 * j + 3));
-                __syncwarp();
-                for (int r = 0; r < rows; ++r)
-                    if (lane >= skip && lane < cols)
-                        to[(int64_t)r * e.stride + lane] = *reinterpret_cast<const float *>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                __syncwarp();
+                store_block<false>(e.out2 + (int64_t)z * e.slice + row0 * e.stride - skip, e.stride, rows, skip, e.n < 16 - skip ? (int)e.n + skip : 16,
+                                   false, stage, lane, value);
             }
         }
     }

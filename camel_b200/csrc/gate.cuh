@@ -8,13 +8,22 @@
 namespace ct {
 
 // Both sides of the logistic function with their full relative precision: 1 - sigmoid(g) is sigmoid(-g), not a difference.
+// exp(-|g|) = 2^t (1 + r ln 2), t the rounded -|g| log2(e) and r what it lacks, to 2^-22 of itself; 1 / (1 + e), of a number from 1 to 2, by
+// a reciprocal and a Newton step.  No branches: in the epilogue of a product the division's and expf's cost a tile as much as half of its MMAs.
 __device__ __forceinline__ void sigmoids(float g, float &s, float &other) {
-    const float e = expf(-fabsf(g));
-    const float a = __fdiv_rn(1.0f, __fadd_rn(1.0f, e)), b = __fmul_rn(e, a);
+    const float kLog2e = 1.44269502162933349609375f, kLog2eRest = 1.925963033500011079e-8f;
+    float x, e, a;
+    asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(x) : "f"(fabsf(g))); // 104, where exp(-x) is no float any more
+    const float t = __fmul_rn(-x, kLog2e);
+    const float r = __fmaf_rn(-x, kLog2eRest, __fmaf_rn(-x, kLog2e, -t));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e             = __fmaf_rn(__fmul_rn(e, r), 0.693147182464599609375f, e);
+    const float d = __fadd_rn(1.0f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(d));
+    a             = __fmaf_rn(a, __fmaf_rn(-d, a, 1.0f), a);
+    const float b = __fmul_rn(e, a);
     s     = g >= 0.0f ? a : b;
     other = g >= 0.0f ? b : a;
-    if (g != g)
-        s = other = g;
 }
 
 template <int GATE> __device__ __forceinline__ float gate_value(float g) {

@@ -57,14 +57,14 @@ template <int GATE> struct GateEpilogue {
             return;
         const float rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
 #pragma unroll
-        for (int g = 0; g < COLS / 64; ++g) {
-            const int64_t col = col0 + g * 32;
+        for (int g = 0; g < COLS / 32; ++g) {
+            const int64_t col = col0 + g * 16;
             if (col >= p.n)
                 break;
-            const int cols = (int)(p.n - col < 32 ? p.n - col : 32);
-            float *a = acc + g * 32, *b = acc + COLS / 2 + g * 32;
+            const int cols = (int)(p.n - col < 16 ? p.n - col : 16);
+            float *a = acc + g * 16, *b = acc + COLS / 2 + g * 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const float4 s = fused::scales4(p.col_scale, col + 4 * j), t = fused::scales4(p.col_scale, p.twin_offset + col + 4 * j);
                 a[4 * j] = __fmul_rn(a[4 * j], fused::weight(rs, s.x)), a[4 * j + 1] = __fmul_rn(a[4 * j + 1], fused::weight(rs, s.y));
                 a[4 * j + 2] = __fmul_rn(a[4 * j + 2], fused::weight(rs, s.z)), a[4 * j + 3] = __fmul_rn(a[4 * j + 3], fused::weight(rs, s.w));
@@ -73,19 +73,19 @@ template <int GATE> struct GateEpilogue {
             }
             if (e.b_gate)
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
+                for (int j = 0; j < 16; ++j)
                     a[j] = __fadd_rn(a[j], j < cols ? __ldg(e.b_gate + col + j) : 0.0f);
             if (e.b_up)
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
+                for (int j = 0; j < 16; ++j)
                     b[j] = __fadd_rn(b[j], j < cols ? __ldg(e.b_up + col + j) : 0.0f);
             const int64_t at = row0 * p.n + col;
             if (e.gate_pre)
-                fused::store_block<false>(e.gate_pre + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return a[j]; });
+                fused::store_block<false>(e.gate_pre + at, p.n, rows, 0, cols, e.vec != 0, stage, lane, [&](int j) { return a[j]; });
             if (e.up_pre)
-                fused::store_block<false>(e.up_pre + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return b[j]; });
+                fused::store_block<false>(e.up_pre + at, p.n, rows, 0, cols, e.vec != 0, stage, lane, [&](int j) { return b[j]; });
             fused::store_block<false>(
-                e.out + at, p.n, rows, cols, e.vec != 0, stage, lane, [&](int j) { return __fmul_rn(gate_value<GATE>(a[j]), b[j]); });
+                e.out + at, p.n, rows, 0, cols, e.vec != 0, stage, lane, [&](int j) { return __fmul_rn(gate_value<GATE>(a[j]), b[j]); });
         }
     }
 };
