@@ -180,12 +180,12 @@ ct_status ce_fused(
     const int64_t slots = pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
     const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
-                 wm = parts.take((size_t)scales(ln) * 4), pp = parts.take((size_t)(slots * m) * 8), tp = parts.take((size_t)m * 4);
+                 pp = parts.take((size_t)(slots * m) * 8), tp = parts.take((size_t)m * 4);
     Scratch s;
     CT_TRY(s.get(parts.bytes));
     const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, ln, ln);
-    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
-    CT_TRY(split_cols(st, w, nullptr, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    const Split operands[2] = {{w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)}, {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
+    CT_TRY(split(st, operands, 2));
     Product p{};
     p.m = m, p.n = n, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
     SumExp::Params e{bias, targets, s.as<float2>(pp), s.as<float>(tp)};
@@ -282,21 +282,22 @@ ct_status ce_grad_fused(
     const int64_t piece = std::min<int64_t>(n, ((n + count - 1) / count + 255) / 256 * 256), ld = padded(piece);
     Parts parts;
     const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
-                 wm = parts.take((size_t)scales(ln) * 4), dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
+                 dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
     const size_t vp = dx ? parts.planes(k, ln) : 0, vi = dx ? parts.take((size_t)scales(k) * 4) : 0;
-    const size_t yp = dw ? parts.planes(m, lk) : 0, yi = dw ? parts.take((size_t)scales(lk) * 4) : 0, ym = dw ? parts.take((size_t)scales(lk) * 4) : 0;
+    const size_t yp = dw ? parts.planes(m, lk) : 0, yi = dw ? parts.take((size_t)scales(lk) * 4) : 0;
     Scratch s;
     CT_TRY(s.get(parts.bytes));
     const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, ln, ln), pv = planes_at(s, vp, k, ln, ln), py = planes_at(s, yp, m, lk, lk);
     float *weight = s.as<float>(rw);
     CT_CUDA(launch_dependent(ce_weights_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream(), dloss, targets, m, n, weight));
     CT_LAUNCH_CHECK("ce_weights");
-    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
-    CT_TRY(split_cols(st, w, nullptr, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    Split operands[4] = {{w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)}, {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
+    int operand_count = 2;
     if (dx)
-        CT_TRY(split_rows(w, nullptr, k, n, pv, s.as<float>(vi)));
+        operands[operand_count++] = {w, nullptr, k, n, false, nullptr, pv, s.as<float>(vi)};
     if (dw)
-        CT_TRY(split_cols(st, x, nullptr, weight, m, k, py, s.as<uint32_t>(ym), s.as<float>(yi)));
+        operands[operand_count++] = {x, nullptr, m, k, true, weight, py, s.as<float>(yi)};
+    CT_TRY(split(st, operands, operand_count));
     for (int64_t c = 0; c < n; c += piece) {
         const int64_t cols = std::min(piece, n - c);
         const Planes pd    = planes_at(s, dp, m, cols, ld);

@@ -1,7 +1,8 @@
 // Operand planes of the fused products (fused_product.cuh), and the product that is simply stored.
 //
-// The pre-passes are bound by memory: 4 bytes read and 4 written a value.  A scale per row is found and used while the row is in
-// registers; a scale per column needs the whole column first, so the matrix is read twice, the second time from L2 where it fits.
+// The pre-passes are bound by memory: 4 bytes read and 4 written a value.  A scale is found and used while its line is in registers: rows of up to
+// 8192 values, a warp or a block to each, and columns of up to 2048, a block to 16 (8) of them.  Longer lines are read twice, the second
+// time from L2 where that holds them.  All operands of a product whose columns are short are split in one launch.
 #include "fused_product.cuh"
 
 namespace ct {
@@ -13,6 +14,8 @@ struct Source {
     const float *in, *in2;
     int64_t rows, cols, ld;
     int vec; // rows of both are whole and aligned float4
+    // Columns c .. c + 3, c a multiple of four.  Rows that are not aligned take a load for each: as aligned pieces, with what a lane lacks shuffled over
+    // from the next one, columns of 1024 x 32003 took 160 us for 85, the selects and shuffles outweighing the loads.
     __device__ __forceinline__ float4 quad(int64_t r, int64_t c) const {
         const float *src = in;
         if (c >= ld)
@@ -40,14 +43,19 @@ __device__ __forceinline__ void put_quad(const Planes &to, int64_t at, float a, 
     *reinterpret_cast<uint2 *>(to.lo + at) = *reinterpret_cast<uint2 *>(lo);
 }
 
+__device__ __forceinline__ float4 factored(float4 q, const float *row_factor, int64_t r) {
+    if (row_factor) {
+        const float f = row_factor[r]; // a row of factor zero takes no part, whatever it holds
+        q = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
+    }
+    return q;
+}
+
 // TPR threads to a row, which they hold in V float4 each if it is that short.
 template <int TPR, int V>
-__global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64_t width, const Planes to, float *__restrict__ inverse) {
-    __shared__ uint32_t words[8];
-    griddep_wait();
-    griddep_launch_dependents();
+__device__ __forceinline__ void split_rows(const Source &src, int64_t width, const Planes &to, float *inverse, int64_t block, uint32_t (&words)[8]) {
     const int t       = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int64_t row = block * (256 / TPR) + threadIdx.x / TPR;
     if (row >= src.rows) // whole warps, or the whole block
         return;
     const bool fits = width <= TPR * V * 4;
@@ -63,6 +71,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64
         for (int j = 0; j < V; ++j)
             mx = max(mx, quad_bits(v[j]));
     } else {
+#pragma unroll 8
         for (int64_t c = t * 4; c < width; c += TPR * 4)
             mx = max(mx, quad_bits(src.quad(row, c)));
     }
@@ -84,6 +93,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64
                 put_quad(to, row * to.ld + c, v[j].x * s, v[j].y * s, v[j].z * s, v[j].w * s);
         }
     } else {
+#pragma unroll 8
         for (int64_t c = t * 4; c < width; c += TPR * 4) {
             const float4 q = src.quad(row, c);
             put_quad(to, row * to.ld + c, q.x * s, q.y * s, q.z * s, q.w * s);
@@ -93,12 +103,99 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64
         inverse[row] = line_inverse(mx);
 }
 
-__device__ __forceinline__ float4 factored(float4 q, const float *row_factor, int64_t r) {
-    if (row_factor) {
-        const float f = row_factor[r]; // a row of factor zero takes no part, whatever it holds
-        q = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
+// 4 L columns to the block, L lanes to a row; at most kShort rows of 256 / L to a thread.
+constexpr int kShort = 16;
+constexpr int64_t kFewValues = 1 << 22;
+template <int L>
+__device__ __forceinline__ void split_short_cols(
+    const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int64_t block, uint32_t (&words)[8][16]) {
+    constexpr int RP = 256 / L;
+    const int t = threadIdx.x, quad = t % L;
+    const int64_t c = block * (4 * L) + quad * 4;
+    float4 v[kShort];
+    uint32_t mx[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kShort; ++i) {
+        const int64_t r = i * RP + t / L;
+        v[i]            = r < src.rows && c < width ? src.quad(r, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    return q;
+#pragma unroll
+    for (int i = 0; i < kShort; ++i) {
+        const int64_t r = i * RP + t / L;
+        if (row_factor && r < src.rows)
+            v[i] = factored(v[i], row_factor, r);
+        mx[0] = max(mx[0], finite_bits(v[i].x)), mx[1] = max(mx[1], finite_bits(v[i].y));
+        mx[2] = max(mx[2], finite_bits(v[i].z)), mx[3] = max(mx[3], finite_bits(v[i].w));
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int o = 16; o >= L; o >>= 1)
+            mx[q] = max(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], o));
+    if ((t & 31) < L)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            words[t >> 5][quad * 4 + q] = mx[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        mx[q] = words[0][quad * 4 + q];
+#pragma unroll
+        for (int w = 1; w < 8; ++w)
+            mx[q] = max(mx[q], words[w][quad * 4 + q]);
+    }
+    if (c >= width)
+        return;
+    const float s0 = line_scale(mx[0]), s1 = line_scale(mx[1]), s2 = line_scale(mx[2]), s3 = line_scale(mx[3]);
+#pragma unroll
+    for (int i = 0; i < kShort; ++i) {
+        const int64_t r = i * RP + t / L;
+        if (r < src.rows)
+            put_quad(to, r * to.ld + c, v[i].x * s0, v[i].y * s1, v[i].z * s2, v[i].w * s3);
+    }
+    if (t < L)
+        *reinterpret_cast<float4 *>(inverse + c) = make_float4(line_inverse(mx[0]), line_inverse(mx[1]), line_inverse(mx[2]), line_inverse(mx[3]));
+}
+
+// Up to four matrices, each with its range of blocks.
+enum Form : int { kRowsWarp, kRowsBlock, kCols16, kCols8 };
+struct SplitJobs {
+    struct Job {
+        Source src;
+        int64_t width;
+        const float *row_factor;
+        Planes to;
+        float *inverse;
+        int form;
+        int64_t first; // block
+    } job[6];
+    int count;
+};
+template <bool ROWS> // rows among them
+__global__ void __launch_bounds__(256, 2) split_jobs_kernel(const __grid_constant__ SplitJobs jobs) {
+    __shared__ uint32_t words[8], many[8][16];
+    griddep_wait();
+    griddep_launch_dependents();
+    int j = 0;
+    while (j + 1 < jobs.count && (int64_t)blockIdx.x >= jobs.job[j + 1].first)
+        ++j;
+    const SplitJobs::Job &x = jobs.job[j];
+    const int64_t block     = blockIdx.x - x.first;
+    if (ROWS && x.form == kRowsWarp)
+        split_rows<32, 8>(x.src, x.width, x.to, x.inverse, block, words);
+    else if (ROWS && x.form == kRowsBlock)
+        split_rows<256, 8>(x.src, x.width, x.to, x.inverse, block, words);
+    else if (x.form == kCols16)
+        split_short_cols<4>(x.src, x.width, x.row_factor, x.to, x.inverse, block, many);
+    else
+        split_short_cols<2>(x.src, x.width, x.row_factor, x.to, x.inverse, block, many);
+}
+template <int TPR, int V>
+__global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64_t width, const Planes to, float *__restrict__ inverse) {
+    __shared__ uint32_t words[8];
+    griddep_wait();
+    griddep_launch_dependents();
+    split_rows<TPR, V>(src, width, to, inverse, blockIdx.x, words);
 }
 
 // Largest finite magnitude of each column into col_max (zeroed before): a lane has four columns, the block's warps the rows in turn.
@@ -222,40 +319,84 @@ ct_status launch_store(
 
 } // namespace
 
-ct_status split_rows(const float *in, const float *in2, int64_t rows, int64_t cols, const Planes &to, float *inverse) {
-    const Source src    = source_of(in, in2, rows, cols);
-    const int64_t width = in2 ? 2 * src.ld : src.ld;
-#define CT_SPLIT_ROWS(TPR, V)                                                                                                                \
-    CT_CUDA(launch_dependent(split_rows_kernel<TPR, V>, dim3((unsigned)((rows + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, stream(), src, \
-                             width, to, inverse))
-    if (width <= 256)
-        CT_SPLIT_ROWS(32, 2);
-    else if (width <= 1024)
-        CT_SPLIT_ROWS(32, 8);
-    else if (width <= 4096)
-        CT_SPLIT_ROWS(256, 4);
-    else
-        CT_SPLIT_ROWS(256, 8);
-#undef CT_SPLIT_ROWS
-    CT_LAUNCH_CHECK("split_rows");
+// Long columns: their maxima, then the planes.
+static ct_status split_long_cols(DeviceState *st, const Split &x) {
+    const Source src     = source_of(x.in, x.in2, x.rows, x.cols);
+    const int64_t width  = x.in2 ? 2 * src.ld : src.ld;
+    const int64_t strips = (width + 127) / 128;
+    // a few blocks to an SM, of at least 32 rows
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((x.rows + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t each   = (x.rows + slices - 1) / slices;
+    const dim3 grid((unsigned)strips, (unsigned)((x.rows + each - 1) / each));
+    Scratch words;
+    CT_TRY(words.get((size_t)width * 4));
+    uint32_t *col_max = words.as<uint32_t>();
+    CT_CUDA(cudaMemsetAsync(col_max, 0, (size_t)width * 4, stream()));
+    CT_CUDA(launch_dependent(col_max_kernel, grid, dim3(256), 0, stream(), src, width, x.row_factor, each, col_max));
+    CT_LAUNCH_CHECK("col_max");
+    CT_CUDA(launch_dependent(split_cols_kernel, grid, dim3(256), 0, stream(), src, width, x.row_factor, each, (const uint32_t *)col_max, x.to, x.inverse));
+    CT_LAUNCH_CHECK("split_cols");
     return CT_OK;
 }
 
-ct_status split_cols(
-    DeviceState *st, const float *in, const float *in2, const float *row_factor, int64_t rows, int64_t cols, const Planes &to, uint32_t *col_max,
-    float *inverse) {
-    const Source src     = source_of(in, in2, rows, cols);
-    const int64_t width  = in2 ? 2 * src.ld : src.ld;
-    const int64_t strips = (width + 127) / 128;
-    // a few blocks to an SM, of at least 32 rows
-    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((rows + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
-    const int64_t each   = (rows + slices - 1) / slices;
-    const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, (rows + each - 1) / each));
-    CT_CUDA(cudaMemsetAsync(col_max, 0, (size_t)width * 4, stream()));
-    CT_CUDA(launch_dependent(col_max_kernel, grid, dim3(256), 0, stream(), src, width, row_factor, each, col_max));
-    CT_LAUNCH_CHECK("col_max");
-    CT_CUDA(launch_dependent(split_cols_kernel, grid, dim3(256), 0, stream(), src, width, row_factor, each, (const uint32_t *)col_max, to, inverse));
-    CT_LAUNCH_CHECK("split_cols");
+ct_status split(DeviceState *st, const Split *what, int count) {
+    // One launch of all forms while there is little to do, and it is the launches that count; else rows and columns apart.
+    SplitJobs rows{}, cols{};
+    int64_t row_blocks = 0, col_blocks = 0, values = 0;
+    auto add = [&](SplitJobs &jobs, int64_t &blocks, const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int form) {
+        jobs.job[jobs.count++] = SplitJobs::Job{src, width, row_factor, to, inverse, form, blocks};
+        blocks += form == kRowsWarp ? (src.rows + 7) / 8 : form == kRowsBlock ? src.rows : form == kCols16 ? (width + 15) / 16 : (width + 7) / 8;
+        values += src.rows * width;
+    };
+    for (int i = 0; i < count; ++i) {
+        const Split &x   = what[i];
+        const Source src = source_of(x.in, x.in2, x.rows, x.cols);
+        if (!x.by_column) {
+            const int64_t width = x.in2 ? 2 * src.ld : src.ld;
+            add(rows, row_blocks, src, width, nullptr, x.to, x.inverse, width <= 1024 ? kRowsWarp : kRowsBlock);
+        } else if (x.rows <= kShort * 64 || (x.rows <= kShort * 128 && x.rows * src.ld <= kFewValues)) {
+            const int form = x.rows <= kShort * 64 ? kCols16 : kCols8;
+            add(cols, col_blocks, source_of(x.in, nullptr, x.rows, x.cols), src.ld, x.row_factor, x.to, x.inverse, form);
+            if (x.in2)
+                add(cols, col_blocks, source_of(x.in2, nullptr, x.rows, x.cols), src.ld, x.row_factor, columns_of(x.to, src.ld, src.ld), x.inverse + src.ld, form);
+        } else {
+            CT_TRY(split_long_cols(st, x));
+        }
+    }
+    if (row_blocks + col_blocks > 0x7fffffff)
+        return fail(CT_ERR_TOO_LARGE, "split: too many rows");
+    if (row_blocks > 0 && col_blocks > 0 && values <= kFewValues) {
+        for (int i = 0; i < rows.count; ++i)
+            cols.job[cols.count] = rows.job[i], cols.job[cols.count++].first += col_blocks;
+        CT_CUDA(launch_dependent(split_jobs_kernel<true>, dim3((unsigned)(row_blocks + col_blocks)), dim3(256), 0, stream(), cols));
+        CT_LAUNCH_CHECK("split_jobs");
+        return CT_OK;
+    }
+    if (col_blocks > 0) {
+        CT_CUDA(launch_dependent(split_jobs_kernel<false>, dim3((unsigned)col_blocks), dim3(256), 0, stream(), cols));
+        CT_LAUNCH_CHECK("split_jobs");
+    }
+    for (int i = 0; i < rows.count; ++i) {
+        const SplitJobs::Job &x = rows.job[i];
+        auto run = [&](auto kernel, int per_block) {
+            return launch_dependent(kernel, dim3((unsigned)((x.src.rows + per_block - 1) / per_block)), dim3(256), 0, stream(), x.src, x.width, x.to, x.inverse);
+        };
+        if (x.width <= 256)
+            CT_CUDA(run(split_rows_kernel<32, 2>, 8));
+        else if (x.width <= 512)
+            CT_CUDA(run(split_rows_kernel<32, 4>, 8));
+        else if (x.width <= 1024)
+            CT_CUDA(run(split_rows_kernel<32, 8>, 8));
+        else if (x.width <= 2048)
+            CT_CUDA(run(split_rows_kernel<256, 2>, 1));
+        else if (x.width <= 4096)
+            CT_CUDA(run(split_rows_kernel<256, 4>, 1));
+        else if (x.width <= 8192)
+            CT_CUDA(run(split_rows_kernel<256, 8>, 1));
+        else
+            CT_CUDA(run(split_rows_kernel<256, 16>, 1));
+        CT_LAUNCH_CHECK("split_rows");
+    }
     return CT_OK;
 }
 

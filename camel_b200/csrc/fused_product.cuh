@@ -563,13 +563,17 @@ inline Planes columns_of(Planes p, int64_t from, int64_t cols) {
     return p;
 }
 
-// Planes of in [rows][cols] (and of in2, of the same shape, whose columns follow those of in at column ld: planes of 2 ld columns), with a
-// scale per row over all of them; inverse[rows].
-ct_status split_rows(const float *in, const float *in2, int64_t rows, int64_t cols, const Planes &to, float *inverse);
-// The same with a scale per column; row_factor (may be null): in[r][c] * row_factor[r] is what is split.  col_max: scales(to.cols) words
-// of scratch; inverse[to.cols].
-ct_status split_cols(
-    DeviceState *st, const float *in, const float *in2, const float *row_factor, int64_t rows, int64_t cols, const Planes &to, uint32_t *col_max, float *inverse);
+// What planes are made of, some matrices in one launch.
+struct Split {
+    const float *in, *in2; // in2 (may be null): a matrix of the same shape whose columns follow those of in at column padded(cols) of the planes
+    int64_t rows, cols;
+    bool by_column;        // a scale per column, else per row (over both matrices)
+    const float *row_factor; // by_column, may be null: row r is taken times row_factor[r], and as zeros where that is zero
+    Planes to;
+    float *inverse;        // [rows], or scales(columns of the planes)
+};
+ct_status split(DeviceState *st, const Split *what, int count);
+
 // out = a . b, [m][n] with rows `stride` apart; k sliced where there are few tiles, with partial sums in scratch of the call.  With out2 the
 // columns from `second` on are a matrix of its own (both have `cols` columns).  add: to what out holds.
 struct Result {

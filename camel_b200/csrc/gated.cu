@@ -98,13 +98,12 @@ ct_status gated_fused(
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
     Parts parts;
-    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, 2 * ln), wi = parts.take((size_t)scales(2 * ln) * 4),
-                 wm = parts.take((size_t)scales(2 * ln) * 4);
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, 2 * ln), wi = parts.take((size_t)scales(2 * ln) * 4);
     Scratch s;
     CT_TRY(s.get(parts.bytes));
     const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, 2 * ln, 2 * ln);
-    CT_TRY(split_rows(x, nullptr, m, k, px, s.as<float>(xi)));
-    CT_TRY(split_cols(st, w_gate, w_up, nullptr, k, n, pw, s.as<uint32_t>(wm), s.as<float>(wi)));
+    const Split operands[2] = {{w_gate, w_up, k, n, true, nullptr, pw, s.as<float>(wi)}, {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
+    CT_TRY(split(st, operands, 2));
     Product p{};
     p.m = m, p.n = n, p.twin_offset = (int)ln, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
     return with_gate(gate, [&](auto G) -> ct_status {
@@ -300,8 +299,7 @@ ct_status gated_grad_fused(
     Parts parts;
     const size_t dp = parts.planes(m, 2 * ln), di = parts.take((size_t)m * 4);
     const size_t wp = back ? parts.planes(k, 2 * ln) : 0, wi = back ? parts.take((size_t)scales(k) * 4) : 0;
-    const size_t xp = weights ? parts.planes(m, lk) : 0, xi = weights ? parts.take((size_t)scales(lk) * 4) : 0,
-                 xm = weights ? parts.take((size_t)scales(lk) * 4) : 0;
+    const size_t xp = weights ? parts.planes(m, lk) : 0, xi = weights ? parts.take((size_t)scales(lk) * 4) : 0;
     Scratch s;
     CT_TRY(s.get(parts.bytes));
     const Planes pd = planes_at(s, dp, m, 2 * ln, 2 * ln);
@@ -309,16 +307,20 @@ ct_status gated_grad_fused(
     CT_TRY(with_gate(gate, [&](auto G) { return launch_slopes<G.value>(gate_pre, up_pre, dout, m, n, vec, pd, s.as<float>(di)); }));
     if (db_gate || db_up)
         CT_TRY(gated_bias(st, gate_pre, up_pre, dout, m, n, gate, vec, db_gate, db_up));
+    const Planes pw = planes_at(s, wp, k, 2 * ln, 2 * ln), px = planes_at(s, xp, m, lk, lk);
+    Split operands[2];
+    int count = 0;
+    if (back)
+        operands[count++] = {w_gate, w_up, k, n, false, nullptr, pw, s.as<float>(wi)};
+    if (weights)
+        operands[count++] = {x, nullptr, m, k, true, s.as<float>(di), px, s.as<float>(xi)};
+    CT_TRY(split(st, operands, count));
     if (back) {
-        const Planes pw = planes_at(s, wp, k, 2 * ln, 2 * ln);
-        CT_TRY(split_rows(w_gate, w_up, k, n, pw, s.as<float>(wi)));
         Result r{dx};
         r.cols = r.stride = k;
         CT_TRY(product(st, pd, false, pw, false, m, k, s.as<float>(di), s.as<float>(wi), r));
     }
     if (weights) {
-        const Planes px = planes_at(s, xp, m, lk, lk);
-        CT_TRY(split_cols(st, x, nullptr, s.as<float>(di), m, k, px, s.as<uint32_t>(xm), s.as<float>(xi)));
         Result r{dw_gate};
         r.cols = r.stride = n;
         if (dw_gate && dw_up)
