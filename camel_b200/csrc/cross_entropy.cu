@@ -10,7 +10,7 @@
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
 // A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
 // Up to 32 classes, and under the reduced precision, the logits of a piece of the rows are computed by the library's products.
-#include "fused_product.cuh"
+#include "stream_product.cuh"
 
 namespace ct {
 namespace {
@@ -172,27 +172,92 @@ __global__ void __launch_bounds__(256) ce_join_kernel(
     }
 }
 
+// 17 to 128 rows: a thread of a tile has a row's logits at every S-th column, and keeps maximum and sum across the CTA's tiles.
+struct SumExpStream {
+    static constexpr bool kTwin = false;
+    struct Params {
+        const float *bias;
+        const int64_t *targets;
+        float2 *part; // [S grid][rows]
+        float *at_target;
+        int64_t rows; // of all launches
+    };
+    struct State {
+        float top, sum;
+    };
+    __device__ static __forceinline__ void init(State &s) { s.top = -INFINITY, s.sum = 0.0f; }
+    template <int NT>
+    __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &s, const float *z, int64_t c0, int cols, int t) {
+        constexpr int S = 128 / NT;
+        const int r = t % NT, first = t / NT;
+        if (r >= p.m)
+            return;
+        const float rs   = p.row_scale[r] * fused::kStreamUp;
+        const float *row = z + r * fused::kStreamPitch;
+        auto logit       = [&](int c) {
+            const float v = __fmul_rn(row[c], rs);
+            return e.bias ? __fadd_rn(v, __ldg(e.bias + c0 + c)) : v;
+        };
+        float top = s.top;
+#pragma unroll 8
+        for (int c = first; c < cols; c += S)
+            top = fmaxf(top, logit(c));
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum[4]     = {s.top == -INFINITY ? s.sum : __fmul_rn(s.sum, exp2_fast(__fmul_rn(__fsub_rn(s.top, base), kLog2e))), 0.0f, 0.0f, 0.0f};
+        int c = first;
+        for (; c + 3 * S < cols; c += 4 * S)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                sum[q] = __fadd_rn(sum[q], exp2_fast(__fmul_rn(__fsub_rn(logit(c + q * S), base), kLog2e)));
+        for (; c < cols; c += S)
+            sum[0] = __fadd_rn(sum[0], exp2_fast(__fmul_rn(__fsub_rn(logit(c), base), kLog2e)));
+        s.top = top, s.sum = __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3]));
+        const int64_t at = e.targets[r] >= 0 ? e.targets[r] - c0 : -1;
+        if (at >= 0 && at < cols && (int)at % S == first)
+            e.at_target[r] = logit((int)at);
+    }
+    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &p, const Params &e, State &s, int t) {
+        constexpr int S = 128 / NT;
+        if (t % NT < p.m)
+            e.part[((int64_t)blockIdx.x * S + t / NT) * e.rows + t % NT] = make_float2(s.top, s.sum);
+    }
+};
+
 ct_status ce_fused(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, int64_t m, int64_t k, int64_t n, float *loss, float *lse) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    const bool pair     = m > 128 && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
-    const int64_t slots = pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
+    const bool few = m <= kStreamRows, pair = !few && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
+    int per;
+    const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) * stream_shares(m) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
-    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = few ? 0 : parts.planes(k, ln),
+                 wi = few ? 0 : parts.take((size_t)scales(ln) * 4),
                  pp = parts.take((size_t)(slots * m) * 8), tp = parts.take((size_t)m * 4);
     Scratch s;
     CT_TRY(s.get(parts.bytes));
     const Planes px = planes_at(s, xp, m, lk, lk), pw = planes_at(s, wp, k, ln, ln);
-    const Split operands[2] = {{w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)}, {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
-    CT_TRY(split(st, operands, 2));
-    Product p{};
-    p.m = m, p.n = n, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
-    SumExp::Params e{bias, targets, s.as<float2>(pp), s.as<float>(tp)};
-    CT_TRY(pair ? (launch<SumExp, 256, 2, false, true>(st, px, pw, p, e, 1, "cross_entropy"))
-                : (launch<SumExp, 128, 1, false, true>(st, px, pw, p, e, 1, "cross_entropy")));
-    CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((m + 7) / 8)), dim3(256), 0, stream(), (const float2 *)e.part, (int)slots,
-                             (const float *)e.at_target, targets, m, n, loss, lse, (const uint32_t *)st->flags_dev));
+    const Split operands[2] = {{x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}, {w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)}};
+    CT_TRY(split(st, operands, few ? 1 : 2));
+    float2 *part     = s.as<float2>(pp);
+    float *at_target = s.as<float>(tp);
+    if (few) {
+        Stream p{};
+        p.w = w, p.k = k, p.n = p.ld = n, p.row_scale = s.as<float>(xi);
+        const SumExpStream::Params e{bias, targets, part, at_target, m};
+        CT_TRY(launch_stream<SumExpStream>(st, px, p, e, "cross_entropy", [](SumExpStream::Params f, int64_t r) {
+            f.targets += r, f.part += r, f.at_target += r;
+            return f;
+        }));
+    } else {
+        Product p{};
+        p.m = m, p.n = n, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi);
+        const SumExp::Params e{bias, targets, part, at_target};
+        CT_TRY(pair ? (launch<SumExp, 256, 2, false, true>(st, px, pw, p, e, 1, "cross_entropy"))
+                    : (launch<SumExp, 128, 1, false, true>(st, px, pw, p, e, 1, "cross_entropy")));
+    }
+    CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((m + 7) / 8)), dim3(256), 0, stream(), (const float2 *)part, (int)slots,
+                             (const float *)at_target, targets, m, n, loss, lse, (const uint32_t *)st->flags_dev));
     CT_LAUNCH_CHECK("ce_join");
     return CT_OK;
 }
@@ -261,6 +326,40 @@ struct Slopes {
     }
 };
 
+// 17 to 128 rows: a warp has a row of a tile at a time, a lane four of its columns.
+struct SlopesStream {
+    static constexpr bool kTwin = false;
+    using Params = Slopes::Params;
+    struct State {};
+    __device__ static __forceinline__ void init(State &) {}
+    template <int NT>
+    __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &, const float *z, int64_t c0, int cols, int t) {
+        const int c = (t & 31) * 4;
+        if (c >= cols)
+            return;
+        for (int r = t >> 5; r < p.m; r += 4) {
+            const float rs   = p.row_scale[r] * fused::kStreamUp, l = e.lse[r];
+            const int64_t tg = e.targets[r], at = tg - e.first - c0;
+            const bool has   = tg >= 0 && tg < e.classes;
+            float d[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v = __fmul_rn(z[r * fused::kStreamPitch + c + q], rs);
+                if (e.bias && c + q < cols)
+                    v = __fadd_rn(v, __ldg(e.bias + c0 + c + q));
+                v    = exp2_fast(__fmul_rn(__fsub_rn(v, l), kLog2e));
+                d[q] = has && c + q < cols ? __fmul_rn(at == c + q ? __fsub_rn(v, 1.0f) : v, kSlopeScale) : 0.0f;
+            }
+            __half2 hi[2], lo[2];
+            fused::split2(d[0], d[1], hi[0], lo[0]);
+            fused::split2(d[2], d[3], hi[1], lo[1]);
+            *reinterpret_cast<uint2 *>(e.hi + r * e.ld + c0 + c) = *reinterpret_cast<uint2 *>(hi); // ld covers it
+            *reinterpret_cast<uint2 *>(e.lo + r * e.ld + c0 + c) = *reinterpret_cast<uint2 *>(lo);
+        }
+    }
+    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, int) {}
+};
+
 // What the rows of d are weighted with behind the planes: dloss / 2^14, zero for rows without a target.
 __global__ void __launch_bounds__(256) ce_weights_kernel(
     const float *__restrict__ dloss, const int64_t *__restrict__ targets, int64_t m, int64_t n, float *__restrict__ weight) {
@@ -276,13 +375,14 @@ ct_status ce_grad_fused(
     int64_t n, float *dx, float *dw, float *dbias) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
+    const bool few = m <= kStreamRows;
     // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
     const int64_t count = (n + most - 1) / most;
     const int64_t piece = std::min<int64_t>(n, ((n + count - 1) / count + 255) / 256 * 256), ld = padded(piece);
     Parts parts;
-    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = parts.planes(k, ln), wi = parts.take((size_t)scales(ln) * 4),
-                 dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = few ? 0 : parts.planes(k, ln),
+                 wi = few ? 0 : parts.take((size_t)scales(ln) * 4), dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
     const size_t vp = dx ? parts.planes(k, ln) : 0, vi = dx ? parts.take((size_t)scales(k) * 4) : 0;
     const size_t yp = dw ? parts.planes(m, lk) : 0, yi = dw ? parts.take((size_t)scales(lk) * 4) : 0;
     Scratch s;
@@ -291,8 +391,10 @@ ct_status ce_grad_fused(
     float *weight = s.as<float>(rw);
     CT_CUDA(launch_dependent(ce_weights_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream(), dloss, targets, m, n, weight));
     CT_LAUNCH_CHECK("ce_weights");
-    Split operands[4] = {{w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)}, {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
-    int operand_count = 2;
+    Split operands[4] = {{x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)}};
+    int operand_count = 1;
+    if (!few)
+        operands[operand_count++] = {w, nullptr, k, n, true, nullptr, pw, s.as<float>(wi)};
     if (dx)
         operands[operand_count++] = {w, nullptr, k, n, false, nullptr, pv, s.as<float>(vi)};
     if (dw)
@@ -301,13 +403,22 @@ ct_status ce_grad_fused(
     for (int64_t c = 0; c < n; c += piece) {
         const int64_t cols = std::min(piece, n - c);
         const Planes pd    = planes_at(s, dp, m, cols, ld);
-        Product p{};
-        p.m = m, p.n = cols, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi) + c;
-        Slopes::Params e{bias ? bias + c : nullptr, lse, targets, c, n, pd.hi, pd.lo, ld};
-        const Planes right = columns_of(pw, c, cols);
-        const bool pair    = m > 128 && (m + 255) / 256 * ((cols + 255) / 256) * 4 >= st->sm_count;
-        CT_TRY(pair ? (launch<Slopes, 256, 2, false, true>(st, px, right, p, e, 1, "cross_entropy_grad"))
-                    : (launch<Slopes, 128, 1, false, true>(st, px, right, p, e, 1, "cross_entropy_grad")));
+        const Slopes::Params e{bias ? bias + c : nullptr, lse, targets, c, n, pd.hi, pd.lo, ld};
+        if (few) {
+            Stream p{};
+            p.w = w + c, p.k = k, p.n = cols, p.ld = n, p.row_scale = s.as<float>(xi);
+            CT_TRY(launch_stream<SlopesStream>(st, px, p, e, "cross_entropy_grad", [](Slopes::Params f, int64_t r) {
+                f.lse += r, f.targets += r, f.hi += r * f.ld, f.lo += r * f.ld;
+                return f;
+            }));
+        } else {
+            Product p{};
+            p.m = m, p.n = cols, p.row_scale = s.as<float>(xi), p.col_scale = s.as<float>(wi) + c;
+            const Planes right = columns_of(pw, c, cols);
+            const bool pair    = (m + 255) / 256 * ((cols + 255) / 256) * 4 >= st->sm_count;
+            CT_TRY(pair ? (launch<Slopes, 256, 2, false, true>(st, px, right, p, e, 1, "cross_entropy_grad"))
+                        : (launch<Slopes, 128, 1, false, true>(st, px, right, p, e, 1, "cross_entropy_grad")));
+        }
         if (dx) {
             Result r{dx};
             r.cols = r.stride = k, r.add = c > 0;

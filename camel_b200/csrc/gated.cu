@@ -1,12 +1,13 @@
 // Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), and its gradient.
 //
 // Forward: one product whose tiles have the same columns of both weight matrices (fused_product.cuh); a thread of the epilogue
-// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu.
+// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu; up to
+// 128: stream_product.cuh.
 // Gradient: gated_slopes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
 // dx = d . [w_gate | w_up]^T as they lie, and the right operand of dw = x'^T . d with their rows as k, x' being x with the rows' scales
 // taken back.  So d is written once, 8 bytes for each of its values' pairs of terms, and read in place.
 // The reduced precision runs the library's products one after the other.
-#include "fused_product.cuh"
+#include "stream_product.cuh"
 #include "gate.cuh"
 
 #include <algorithm>
@@ -89,6 +90,64 @@ template <int GATE> struct GateEpilogue {
         }
     }
 };
+
+// 17 to 128 rows: a warp has a row of a tile's results at a time.
+template <int GATE> struct GateStream {
+    static constexpr bool kTwin = true;
+    struct Params {
+        const float *b_gate, *b_up;
+        float *out, *gate_pre, *up_pre;
+    };
+    struct State {};
+    __device__ static __forceinline__ void init(State &) {}
+    template <int NT>
+    __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &, const float *z, int64_t c0, int cols, int t) {
+        const int lane = t & 31;
+        for (int r = t >> 5; r < p.m; r += 4) {
+            const float rs = p.row_scale[r] * fused::kStreamUp;
+#pragma unroll
+            for (int c = lane; c < 64; c += 32)
+                if (c < cols) {
+                    float g = __fmul_rn(z[r * fused::kStreamPitch + c], rs), u = __fmul_rn(z[r * fused::kStreamPitch + 64 + c], rs);
+                    const int64_t at = r * p.n + c0 + c;
+                    if (e.b_gate)
+                        g = __fadd_rn(g, __ldg(e.b_gate + c0 + c));
+                    if (e.b_up)
+                        u = __fadd_rn(u, __ldg(e.b_up + c0 + c));
+                    if (e.gate_pre)
+                        e.gate_pre[at] = g;
+                    if (e.up_pre)
+                        e.up_pre[at] = u;
+                    e.out[at] = __fmul_rn(gate_value<GATE>(g), u);
+                }
+        }
+    }
+    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, int) {}
+};
+
+ct_status gated_stream(
+    DeviceState *st, const float *x, const float *w_gate, const float *b_gate, const float *w_up, const float *b_up, int64_t m, int64_t k, int64_t n,
+    int gate, float *out, float *gate_pre, float *up_pre) {
+    using namespace fused;
+    const int64_t lk = padded(k);
+    Parts parts;
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4);
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes px     = planes_at(s, xp, m, lk, lk);
+    const Split operand = {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)};
+    CT_TRY(split(st, &operand, 1));
+    Stream p{};
+    p.w = w_gate, p.w2 = w_up, p.k = k, p.n = p.ld = n, p.row_scale = s.as<float>(xi);
+    return with_gate(gate, [&](auto G) -> ct_status {
+        using E = GateStream<G.value>;
+        const typename E::Params e{b_gate, b_up, out, gate_pre, up_pre};
+        return launch_stream<E>(st, px, p, e, "dense_gated", [&](typename E::Params f, int64_t r) {
+            f.out += r * n, f.gate_pre = f.gate_pre ? f.gate_pre + r * n : nullptr, f.up_pre = f.up_pre ? f.up_pre + r * n : nullptr;
+            return f;
+        });
+    });
+}
 
 bool whole(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -368,6 +427,8 @@ ct_status ct_dense_gated(
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
         if (m <= fused::kFewRows)
             return fused::few_rows(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
+        if (m <= fused::kStreamRows)
+            return gated_stream(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
         return gated_fused(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
     }
     const int64_t count = m * n;
