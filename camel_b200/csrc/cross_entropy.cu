@@ -136,6 +136,14 @@ struct SumExp {
     }
 };
 
+// (maximum, sum of exponentials about it) of two sets of logits.
+__device__ __forceinline__ float2 join_parts(float2 a, float2 b) {
+    const float top  = fmaxf(a.x, b.x);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float x    = __fmul_rn(a.y, exp2_fast(__fmul_rn(__fsub_rn(a.x, base), kLog2e))), y = __fmul_rn(b.y, exp2_fast(__fmul_rn(__fsub_rn(b.x, base), kLog2e)));
+    return make_float2(top, __fadd_rn(a.x == -INFINITY ? a.y : x, b.x == -INFINITY ? b.y : y)); // nothing but -inf: a sum of 0, or NaN
+}
+
 // A row's parts: eight rows to a block, a lane group of eight takes every 32nd part (with 32 rows to a block 64 rows of 500 parts took 23 us).
 __global__ void __launch_bounds__(256) ce_join_kernel(
     const float2 *__restrict__ part, int slots, const float *__restrict__ at_target, const int64_t *__restrict__ targets, int64_t m, int64_t n,
@@ -147,22 +155,16 @@ __global__ void __launch_bounds__(256) ce_join_kernel(
         return;
     const int at = threadIdx.x & 7, group = threadIdx.x >> 3;
     const int64_t row = (int64_t)blockIdx.x * 8 + at;
-    auto join = [](float2 a, float2 b) {
-        const float top  = fmaxf(a.x, b.x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        const float x    = __fmul_rn(a.y, exp2_fast(__fmul_rn(__fsub_rn(a.x, base), kLog2e))), y = __fmul_rn(b.y, exp2_fast(__fmul_rn(__fsub_rn(b.x, base), kLog2e)));
-        return make_float2(top, __fadd_rn(a.x == -INFINITY ? a.y : x, b.x == -INFINITY ? b.y : y)); // nothing but -inf: a sum of 0, or NaN
-    };
     float2 v = make_float2(-INFINITY, 0.0f);
     if (row < m)
 #pragma unroll 4
         for (int s = group; s < slots; s += 32)
-            v = join(v, part[(int64_t)s * m + row]);
+            v = join_parts(v, part[(int64_t)s * m + row]);
     words[group][at] = v;
     __syncthreads();
     if (group == 0 && row < m) {
         for (int w = 1; w < 32; ++w)
-            v = join(v, words[w][at]);
+            v = join_parts(v, words[w][at]);
         const float l   = __fadd_rn(v.x == -INFINITY && v.y == v.y ? 0.0f : v.x, logf(v.y));
         const int64_t t = targets[row];
         if (lse)
@@ -172,54 +174,70 @@ __global__ void __launch_bounds__(256) ce_join_kernel(
     }
 }
 
-// 17 to 128 rows: a thread of a tile has a row's logits at every S-th column, and keeps maximum and sum across the CTA's tiles.
+// 17 to 128 rows: a thread has every sixteenth of a row's logits, and keeps maximum and sum across the CTA's tiles.
 struct SumExpStream {
-    static constexpr bool kTwin = false;
+    static constexpr bool kTwin  = false;
+    static constexpr int kShares = fused::kStreamDrain * 32 / fused::kStreamPass;
     struct Params {
         const float *bias;
         const int64_t *targets;
-        float2 *part; // [S grid][rows]
+        float2 *part; // [grid][rows]
         float *at_target;
         int64_t rows; // of all launches
     };
     struct State {
-        float top, sum;
+        float2 v[4]; // maximum, sum; of row t % 16 of each pass
     };
-    __device__ static __forceinline__ void init(State &s) { s.top = -INFINITY, s.sum = 0.0f; }
-    template <int NT>
+    __device__ static __forceinline__ void init(State &s) { s.v[0] = s.v[1] = s.v[2] = s.v[3] = make_float2(-INFINITY, 0.0f); }
+    template <int Q>
     __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &s, const float *z, int64_t c0, int cols, int t) {
-        constexpr int S = 128 / NT;
-        const int r = t % NT, first = t / NT;
+        constexpr int S = kShares, N = 128 / S;
+        const int r = 16 * Q + (t & 15), first = t >> 4;
         if (r >= p.m)
             return;
         const float rs   = p.row_scale[r] * fused::kStreamUp;
-        const float *row = z + r * fused::kStreamPitch;
-        auto logit       = [&](int c) {
-            const float v = __fmul_rn(row[c], rs);
-            return e.bias ? __fadd_rn(v, __ldg(e.bias + c0 + c)) : v;
-        };
-        float top = s.top;
-#pragma unroll 8
-        for (int c = first; c < cols; c += S)
-            top = fmaxf(top, logit(c));
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum[4]     = {s.top == -INFINITY ? s.sum : __fmul_rn(s.sum, exp2_fast(__fmul_rn(__fsub_rn(s.top, base), kLog2e))), 0.0f, 0.0f, 0.0f};
-        int c = first;
-        for (; c + 3 * S < cols; c += 4 * S)
+        const float *row = z + (t & 15) * fused::kStreamPitch + first;
+        float v[N];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                sum[q] = __fadd_rn(sum[q], exp2_fast(__fmul_rn(__fsub_rn(logit(c + q * S), base), kLog2e)));
-        for (; c < cols; c += S)
-            sum[0] = __fadd_rn(sum[0], exp2_fast(__fmul_rn(__fsub_rn(logit(c), base), kLog2e)));
-        s.top = top, s.sum = __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3]));
+        for (int i = 0; i < N; ++i) {
+            const int c = first + i * S;
+            v[i]        = __fmul_rn(row[i * S], rs);
+            if (e.bias && c < cols)
+                v[i] = __fadd_rn(v[i], __ldg(e.bias + c0 + c));
+            v[i] = c < cols ? v[i] : -INFINITY;
+        }
+        float top = s.v[Q].x;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            top = fmaxf(top, v[i]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum        = s.v[Q].x == -INFINITY ? s.v[Q].y : __fmul_rn(s.v[Q].y, exp2_fast(__fmul_rn(__fsub_rn(s.v[Q].x, base), kLog2e)));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            sum = __fadd_rn(sum, exp2_fast(__fmul_rn(__fsub_rn(v[i], base), kLog2e)));
+        s.v[Q]           = make_float2(top, sum);
         const int64_t at = e.targets[r] >= 0 ? e.targets[r] - c0 : -1;
         if (at >= 0 && at < cols && (int)at % S == first)
-            e.at_target[r] = logit((int)at);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((int)at / S == i)
+                    e.at_target[r] = v[i];
     }
-    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &p, const Params &e, State &s, int t) {
-        constexpr int S = 128 / NT;
-        if (t % NT < p.m)
-            e.part[((int64_t)blockIdx.x * S + t / NT) * e.rows + t % NT] = make_float2(s.top, s.sum);
+    // The shares of each row, in order.
+    __device__ static __forceinline__ void finish(const fused::Stream &p, const Params &e, State &s, float *z, int t) {
+        float2 *words = reinterpret_cast<float2 *>(z); // [share][16]
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            fused::stream_epilogue_sync();
+            words[t] = s.v[q];
+            fused::stream_epilogue_sync();
+            if (t < 16 && 16 * q + t < p.m) {
+                float2 v = words[t];
+                for (int i = 1; i < kShares; ++i)
+                    v = join_parts(v, words[i * 16 + t]);
+                e.part[(int64_t)blockIdx.x * e.rows + 16 * q + t] = v;
+            }
+        }
     }
 };
 
@@ -229,7 +247,7 @@ ct_status ce_fused(
     const int64_t lk = padded(k), ln = padded(n);
     const bool few = m <= kStreamRows, pair = !few && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
     int per;
-    const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) * stream_shares(m) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
+    const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
     const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), wp = few ? 0 : parts.planes(k, ln),
                  wi = few ? 0 : parts.take((size_t)scales(ln) * 4),
@@ -332,19 +350,20 @@ struct SlopesStream {
     using Params = Slopes::Params;
     struct State {};
     __device__ static __forceinline__ void init(State &) {}
-    template <int NT>
+    template <int Q>
     __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &, const float *z, int64_t c0, int cols, int t) {
-        const int c = (t & 31) * 4;
+        const int c = (t & 31) * 4, rows = p.m - 16 * Q < 16 ? p.m - 16 * Q : 16;
         if (c >= cols)
             return;
-        for (int r = t >> 5; r < p.m; r += 4) {
+        for (int i = t >> 5; i < rows; i += fused::kStreamDrain) {
+            const int r      = 16 * Q + i;
             const float rs   = p.row_scale[r] * fused::kStreamUp, l = e.lse[r];
             const int64_t tg = e.targets[r], at = tg - e.first - c0;
             const bool has   = tg >= 0 && tg < e.classes;
             float d[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float v = __fmul_rn(z[r * fused::kStreamPitch + c + q], rs);
+                float v = __fmul_rn(z[i * fused::kStreamPitch + c + q], rs);
                 if (e.bias && c + q < cols)
                     v = __fadd_rn(v, __ldg(e.bias + c0 + c + q));
                 v    = exp2_fast(__fmul_rn(__fsub_rn(v, l), kLog2e));
@@ -357,7 +376,7 @@ struct SlopesStream {
             *reinterpret_cast<uint2 *>(e.lo + r * e.ld + c0 + c) = *reinterpret_cast<uint2 *>(lo);
         }
     }
-    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, int) {}
+    __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, float *, int) {}
 };
 
 // What the rows of d are weighted with behind the planes: dloss / 2^14, zero for rows without a target.

@@ -100,15 +100,16 @@ template <int GATE> struct GateStream {
     };
     struct State {};
     __device__ static __forceinline__ void init(State &) {}
-    template <int NT>
+    template <int Q>
     __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &, const float *z, int64_t c0, int cols, int t) {
-        const int lane = t & 31;
-        for (int r = t >> 5; r < p.m; r += 4) {
+        const int lane = t & 31, rows = p.m - 16 * Q < 16 ? p.m - 16 * Q : 16;
+        for (int i = t >> 5; i < rows; i += fused::kStreamDrain) {
+            const int r    = 16 * Q + i;
             const float rs = p.row_scale[r] * fused::kStreamUp;
 #pragma unroll
             for (int c = lane; c < 64; c += 32)
                 if (c < cols) {
-                    float g = __fmul_rn(z[r * fused::kStreamPitch + c], rs), u = __fmul_rn(z[r * fused::kStreamPitch + 64 + c], rs);
+                    float g = __fmul_rn(z[i * fused::kStreamPitch + c], rs), u = __fmul_rn(z[i * fused::kStreamPitch + 64 + c], rs);
                     const int64_t at = r * p.n + c0 + c;
                     if (e.b_gate)
                         g = __fadd_rn(g, __ldg(e.b_gate + c0 + c));
@@ -122,7 +123,7 @@ template <int GATE> struct GateStream {
                 }
         }
     }
-    template <int NT> __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, int) {}
+    __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, float *, int) {}
 };
 
 ct_status gated_stream(
