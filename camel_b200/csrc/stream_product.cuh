@@ -11,6 +11,7 @@
 // Epilogue: the tile's sums go to shared memory as [row of x][column], 16 rows at a time; the draining warps do with them what EPI says.
 #pragma once
 
+#include "fastmath.cuh"
 #include "fused_product.cuh"
 
 #include <type_traits>
@@ -53,14 +54,18 @@ constexpr float kStreamDown = 1.0f / 16384.0f, kStreamUp = 16384.0f;
 
 #ifdef __CUDACC__
 
-// mbar_wait for waits of a few hundred clocks: the clock that bounds a wait is not read before some tries have failed.
-__device__ __forceinline__ bool stream_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i)
-        if (mbar_try_wait(bar, parity))
-            return true;
-    return mbar_wait(bar, parity, abort_flag);
-}
+// A bounded wait that leaves the issue slots to others: the hardware suspends the thread until the phase completes.
+__device__ __forceinline__ bool stream_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) { return mbar_wait_patient(bar, parity, abort_flag); }
+
+// Where a role stands in a ring of N: the place, and the parity of its phase.
+template <int N> struct Ring {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N)
+            at = 0, phase ^= 1u;
+    }
+};
 
 // EPI: kTwin; Params; State (of a draining thread, across the CTA's tiles); tile<Q>(p, e, state, z, c0, cols, t): rows 16 Q .. of x,
 // z[(row - 16 Q) * kStreamPitch + c] the sums over 2^14, but for the row's scale, of the tile's columns c0 + c < c0 + cols (twin: the second
@@ -126,11 +131,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         // ===== x =====
         if (elect_one()) {
             int issued = 0;
-            for (int s = 0, kb = 0; s < total; ++s) {
-                const int slot = s % kStreamX;
-                if (!stream_wait(smem_u32(&bar_x_empty[slot]), (uint32_t)(s / kStreamX + 1) & 1u, abort_flag))
+            Ring<kStreamX> ring;
+            for (int s = 0, kb = 0; s < total; ++s, ring.next()) {
+                if (!stream_wait(smem_u32(&bar_x_empty[ring.at]), ring.phase ^ 1u, abort_flag))
                     break;
-                const uint32_t full = smem_u32(&bar_x[slot]), dst = smem_base + kStreamSlots * SLOT + slot * kStreamXBytes<NT>;
+                const uint32_t full = smem_u32(&bar_x[ring.at]), dst = smem_base + kStreamSlots * SLOT + ring.at * kStreamXBytes<NT>;
                 mbar_expect_tx(full, kStreamXBytes<NT>);
                 tma_load_2d(dst, &maps.x_hi, full, kb * 64, 0);
                 tma_load_2d(dst + NT * 128, &maps.x_lo, full, kb * 64, 0);
@@ -150,11 +155,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         if (elect_one()) {
             constexpr uint32_t idesc = make_idesc(0u, 128, NT) | 1u << 15; // the weights are MN-major
             bool ok = true;
-            for (int s = 0; s < total && ok; ++s) {
-                const int slot = s % kStreamSlots, set = s % kStreamSets, from = s % kStreamX;
-                ok = stream_wait(smem_u32(&bar_full[slot]), (uint32_t)(s / kStreamSlots) & 1u, abort_flag) &&
-                     stream_wait(smem_u32(&bar_x[from]), (uint32_t)(s / kStreamX) & 1u, abort_flag) &&
-                     stream_wait(smem_u32(&bar_acc_empty[set]), (uint32_t)(s / kStreamSets + 1) & 1u, abort_flag);
+            Ring<kStreamSlots> planes;
+            Ring<kStreamX> xs;
+            Ring<kStreamSets> sets;
+            for (int s = 0; s < total && ok; ++s, planes.next(), xs.next(), sets.next()) {
+                const int slot = planes.at, set = sets.at, from = xs.at;
+                ok = stream_wait(smem_u32(&bar_full[slot]), planes.phase, abort_flag) && stream_wait(smem_u32(&bar_x[from]), xs.phase, abort_flag) &&
+                     stream_wait(smem_u32(&bar_acc_empty[set]), sets.phase ^ 1u, abort_flag);
                 if (!ok)
                     break;
                 tc_fence_after_sync();
@@ -189,21 +196,23 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         typename EPI::State state;
         EPI::init(state);
         bool ok = true;
-        for (int tile = 0, s = 0; tile < tiles; ++tile) { // all warps take all tiles' barriers, also after a failed wait
+        Ring<kStreamSets> sets;
+        Ring<8> scales;
+        for (int tile = 0; tile < tiles; ++tile) { // all warps take all tiles' barriers, also after a failed wait
             float acc[OWN];
 #pragma unroll
             for (int j = 0; j < OWN; ++j)
                 acc[j] = 0.0f;
 #pragma unroll 1
-            for (int kb = 0; kb < p.stages; ++kb, ++s) {
-                const int set = s % kStreamSets;
+            for (int kb = 0; kb < p.stages; ++kb, sets.next(), scales.next()) {
+                const int set = sets.at;
                 if (ok)
-                    ok = __all_sync(0xffffffffu, stream_wait(smem_u32(&bar_acc_full[set]), (uint32_t)(s / kStreamSets) & 1u, abort_flag) &&
-                                                     stream_wait(smem_u32(&bar_scale[s & 7]), (uint32_t)(s >> 3) & 1u, abort_flag)) != 0;
+                    ok = __all_sync(0xffffffffu, stream_wait(smem_u32(&bar_acc_full[set]), sets.phase, abort_flag) &&
+                                                     stream_wait(smem_u32(&bar_scale[scales.at]), scales.phase, abort_flag)) != 0;
                 if (!ok)
                     continue;
                 tc_fence_after_sync();
-                const float by = __fmul_rn(pow2(exponent_s[s & 7][row]), kStreamDown * kStreamDown);
+                const float by = __fmul_rn(pow2(exponent_s[scales.at][row]), kStreamDown * kStreamDown);
                 const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + set * 128 + which * OWN;
 #pragma unroll
                 for (int g = 0; g < OWN / 8; ++g) {
@@ -212,8 +221,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     tmem_ld_32x8(at + 64 + g * 8, b);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        acc[g * 8 + j] = __fmaf_rn(__fmaf_rn(__uint_as_float(b[j]), kLoInv, __uint_as_float(a[j])), by, acc[g * 8 + j]);
+                    for (int j = 0; j < 8; j += 2) {
+                        const f32x2 m = pack2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), c = pack2(__uint_as_float(b[j]), __uint_as_float(b[j + 1]));
+                        unpack2(fma2(fma2(c, dup2(0x3A000000u), m), pack2(by, by), pack2(acc[g * 8 + j], acc[g * 8 + j + 1])), acc[g * 8 + j], acc[g * 8 + j + 1]); // 2^-11
+                    }
                 }
                 tc_fence_before_sync();
                 __syncwarp();
@@ -251,15 +262,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const float *matrix = EPI::kTwin && h ? p.w2 : p.w, *matrix17 = EPI::kTwin && h17 ? p.w2 : p.w;
         const int64_t values = (p.k - 1) * p.ld + p.n, step = kStreamFetch * p.ld;
         bool ok = true;
-        for (int tile = 0, s = 0; tile < tiles && ok; ++tile) {
+        Ring<kStreamRaw> ring;
+        for (int tile = 0; tile < tiles && ok; ++tile) {
             const int64_t col0 = begin + (int64_t)tile * TILE, col = col0 + (EPI::kTwin ? 0 : 64 * h);
             int64_t at         = (((int64_t)who * p.ld + col) & ~(int64_t)3) + q; // the thread's first piece in its matrix
             const int64_t own  = (int64_t)r17 * p.ld + col0 + (EPI::kTwin ? 0 : 64 * h17);
             int64_t at17       = (own & ~(int64_t)3) + 64;
             const bool here = col + q - 3 < end, need17 = !p.whole && (own & 3) != 0;
-            for (int kb = 0; kb < p.stages; ++kb, ++s, at += 64 * p.ld, at17 += 64 * p.ld) {
-                const int slot = s % kStreamRaw, row = kb * 64 + who;
-                ok = stream_wait(smem_u32(&bar_raw_empty[slot]), (uint32_t)(s / kStreamRaw + 1) & 1u, abort_flag);
+            for (int kb = 0; kb < p.stages; ++kb, at += 64 * p.ld, at17 += 64 * p.ld, ring.next()) {
+                const int slot = ring.at, row = kb * 64 + who;
+                ok = stream_wait(smem_u32(&bar_raw_empty[slot]), ring.phase ^ 1u, abort_flag);
                 if (!ok)
                     break;
                 const uint32_t to = smem_u32(smem) + kStreamSlots * SLOT + kStreamX * kStreamXBytes<NT> + slot * kStreamRawBytes;
@@ -313,9 +325,15 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const int chunk  = (local & 63) >> 3, ld3 = p.pieces ? (int)(p.ld & 3) : 0;
         int kb = group < p.stages ? group : 0;
         int tile_col = (int)(begin & 3) + (EPI::kTwin ? 0 : local & 64) + (group < p.stages ? 0 : TILE); // of the half that this warp converts, but for multiples of four
-        for (int s = group; s < total; s += 2) {
-            const int slot = s % kStreamSlots, from_slot = s % kStreamRaw;
-            if (!__all_sync(0xffffffffu, stream_wait(smem_u32(&bar_raw[from_slot]), (uint32_t)(s / kStreamRaw) & 1u, abort_flag)))
+        static_assert(kStreamSlots == 2, "a group has a slot of its own");
+        Ring<kStreamRaw> ring;
+        Ring<8> scales;
+        if (group)
+            ring.next(), scales.next();
+        uint32_t empty_phase = 1u;
+        for (int s = group; s < total; s += 2, ring.next(), ring.next(), scales.next(), scales.next(), empty_phase ^= 1u) {
+            const int slot = group, from_slot = ring.at;
+            if (!__all_sync(0xffffffffu, stream_wait(smem_u32(&bar_raw[from_slot]), ring.phase, abort_flag)))
                 break;
             const float *from = raw + from_slot * (kStreamRawBytes / 4);
             float2 x[16];
@@ -360,27 +378,35 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o)), m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
             }
             const float s0 = line_scale(__float_as_uint(m0)), s1 = line_scale(__float_as_uint(m1));
-            if (!__all_sync(0xffffffffu, stream_wait(smem_u32(&bar_empty[slot]), (uint32_t)(s / kStreamSlots + 1) & 1u, abort_flag)))
+            if (!__all_sync(0xffffffffu, stream_wait(smem_u32(&bar_empty[slot]), empty_phase, abort_flag)))
                 break;
             uint8_t *plane = smem + slot * SLOT + (local >> 6) * 8192 + (local & 7) * 2 + 2 * g * 128;
+            const f32x2 by = pack2(s0, s1), by_lo = pack2(s0 * kLoScale, s1 * kLoScale);
             uint8_t *to[2] = {plane + ((chunk ^ (2 * g)) << 4), plane + 128 + ((chunk ^ (2 * g + 1)) << 4)};
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float a = x[i].x * s0, b = x[i].y * s1;
-                __half2 hi = __floats2half2_rn(a, b);
-                __half2 lo = __floats2half2_rn(__fmul_rn(__fsub_rn(a, __low2float(hi)), kLoScale), __fmul_rn(__fsub_rn(b, __high2float(hi)), kLoScale));
-                if (!finite)
+                // both columns at once: hi of v s, lo of v s 2^11 - hi 2^11, which is exact
+                const f32x2 v = pack2(x[i].x, x[i].y);
+                float a, b;
+                unpack2(mul2(v, by), a, b);
+                __half2 hi = __floats2half2_rn(a, b), lo;
+                if (finite) {
+                    float c, d;
+                    unpack2(fma2(pack2(__low2float(hi), __high2float(hi)), dup2(0xC5000000u), mul2(v, by_lo)), c, d); // - 2048
+                    lo = __floats2half2_rn(c, d);
+                } else {
                     split2(a, b, hi, lo);
+                }
                 *reinterpret_cast<__half2 *>(to[i & 1] + (i >> 1) * 1024)         = hi;
                 *reinterpret_cast<__half2 *>(to[i & 1] + kTile + (i >> 1) * 1024) = lo;
             }
             if (g == 0)
-                *reinterpret_cast<char2 *>(&exponent_s[s & 7][local]) =
+                *reinterpret_cast<char2 *>(&exponent_s[scales.at][local]) =
                     make_char2((signed char)line_exponent(__float_as_uint(m0)), (signed char)line_exponent(__float_as_uint(m1)));
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // written here, read by the tensor core
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&bar_scale[s & 7]));
+                mbar_arrive(smem_u32(&bar_scale[scales.at]));
                 mbar_arrive(smem_u32(&bar_full[slot]));
             }
         }
