@@ -105,7 +105,7 @@ __device__ __forceinline__ void split_rows(const Source &src, int64_t width, con
 
 // 4 L columns to the block, L lanes to a row; at most kShort rows of 256 / L to a thread.
 constexpr int kShort = 16;
-constexpr int64_t kFewValues = 1 << 22;
+constexpr int64_t kFewValues = 1 << 20;
 template <int L>
 __device__ __forceinline__ void split_short_cols(
     const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int64_t block, uint32_t (&words)[8][16]) {
@@ -171,24 +171,87 @@ struct SplitJobs {
     } job[6];
     int count;
 };
-template <bool ROWS> // rows among them
-__global__ void __launch_bounds__(256, 2) split_jobs_kernel(const __grid_constant__ SplitJobs jobs) {
-    __shared__ uint32_t words[8], many[8][16];
+__global__ void __launch_bounds__(256, 2) split_short_cols_kernel(const __grid_constant__ SplitJobs jobs) {
+    __shared__ uint32_t many[8][16];
     griddep_wait();
     griddep_launch_dependents();
     int j = 0;
     while (j + 1 < jobs.count && (int64_t)blockIdx.x >= jobs.job[j + 1].first)
         ++j;
     const SplitJobs::Job &x = jobs.job[j];
-    const int64_t block     = blockIdx.x - x.first;
-    if (ROWS && x.form == kRowsWarp)
-        split_rows<32, 8>(x.src, x.width, x.to, x.inverse, block, words);
-    else if (ROWS && x.form == kRowsBlock)
-        split_rows<256, 8>(x.src, x.width, x.to, x.inverse, block, words);
-    else if (x.form == kCols16)
-        split_short_cols<4>(x.src, x.width, x.row_factor, x.to, x.inverse, block, many);
+    if (x.form == kCols16)
+        split_short_cols<4>(x.src, x.width, x.row_factor, x.to, x.inverse, blockIdx.x - x.first, many);
     else
-        split_short_cols<2>(x.src, x.width, x.row_factor, x.to, x.inverse, block, many);
+        split_short_cols<2>(x.src, x.width, x.row_factor, x.to, x.inverse, blockIdx.x - x.first, many);
+}
+
+// All of a small product's operands: a warp to a row, a block to 16 columns, read twice (the second time from L1).  In registers as above
+// they are read once, but the code is ten times as long, and fetching it is what a launch of a few blocks then waits for (5 against 20 us
+// with cold caches).
+__global__ void __launch_bounds__(256) split_small_kernel(const __grid_constant__ SplitJobs jobs) {
+    __shared__ uint32_t many[8][16];
+    griddep_wait();
+    griddep_launch_dependents();
+    int j = 0;
+    while (j + 1 < jobs.count && (int64_t)blockIdx.x >= jobs.job[j + 1].first)
+        ++j;
+    const SplitJobs::Job &x = jobs.job[j];
+    const Source &src       = x.src;
+    const int64_t block     = blockIdx.x - x.first;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (x.form == kRowsWarp) {
+        const int64_t row = block * 8 + warp;
+        if (row >= src.rows)
+            return;
+        uint32_t mx = 0;
+#pragma unroll 4
+        for (int64_t c = lane * 4; c < x.width; c += 128)
+            mx = max(mx, quad_bits(src.quad(row, c)));
+        mx            = __reduce_max_sync(0xffffffffu, mx);
+        const float s = line_scale(mx);
+#pragma unroll 4
+        for (int64_t c = lane * 4; c < x.width; c += 128) {
+            const float4 q = src.quad(row, c);
+            put_quad(x.to, row * x.to.ld + c, q.x * s, q.y * s, q.z * s, q.w * s);
+        }
+        if (lane == 0)
+            x.inverse[row] = line_inverse(mx);
+    } else {
+        const int t = threadIdx.x, quad = t & 3;
+        const int64_t c = block * 16 + quad * 4;
+        uint32_t mx[4] = {0, 0, 0, 0};
+        if (c < x.width)
+#pragma unroll 4
+            for (int64_t r = t >> 2; r < src.rows; r += 64) {
+                const float4 q = factored(src.quad(r, c), x.row_factor, r);
+                mx[0] = max(mx[0], finite_bits(q.x)), mx[1] = max(mx[1], finite_bits(q.y));
+                mx[2] = max(mx[2], finite_bits(q.z)), mx[3] = max(mx[3], finite_bits(q.w));
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int o = 16; o >= 4; o >>= 1)
+                mx[q] = max(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], o));
+            if (lane < 4)
+                many[warp][quad * 4 + q] = mx[q];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                mx[q] = max(mx[q], many[w][quad * 4 + q]);
+        if (c >= x.width)
+            return;
+        const float s0 = line_scale(mx[0]), s1 = line_scale(mx[1]), s2 = line_scale(mx[2]), s3 = line_scale(mx[3]);
+#pragma unroll 4
+        for (int64_t r = t >> 2; r < src.rows; r += 64) {
+            const float4 q = factored(src.quad(r, c), x.row_factor, r);
+            put_quad(x.to, r * x.to.ld + c, q.x * s0, q.y * s1, q.z * s2, q.w * s3);
+        }
+        if (t < 4)
+            *reinterpret_cast<float4 *>(x.inverse + c) = make_float4(line_inverse(mx[0]), line_inverse(mx[1]), line_inverse(mx[2]), line_inverse(mx[3]));
+    }
 }
 template <int TPR, int V>
 __global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64_t width, const Planes to, float *__restrict__ inverse) {
@@ -208,16 +271,36 @@ __global__ void __launch_bounds__(256) col_max_kernel(
     const int64_t c = (int64_t)blockIdx.x * 128 + lane * 4;
     const int64_t r0 = (int64_t)blockIdx.y * rows_each, r1 = min(src.rows, r0 + rows_each);
     uint32_t mx[4] = {0, 0, 0, 0};
-    if (c < width)
+    if (!src.vec) { // the order is all the same to a maximum: neighbours
+        const float *in[4];
+        bool here[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int64_t at = (int64_t)blockIdx.x * 128 + lane + 32 * i;
+            in[i]      = at >= src.ld ? src.in2 : src.in;
+            at -= at >= src.ld ? src.ld : 0;
+            here[i] = in[i] && at < src.cols;
+            in[i] += at;
+        }
+#pragma unroll 8
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            float4 q = make_float4(here[0] ? in[0][r * src.cols] : 0.0f, here[1] ? in[1][r * src.cols] : 0.0f, here[2] ? in[2][r * src.cols] : 0.0f,
+                                   here[3] ? in[3][r * src.cols] : 0.0f);
+            q = factored(q, row_factor, r);
+            mx[0] = max(mx[0], finite_bits(q.x)), mx[1] = max(mx[1], finite_bits(q.y));
+            mx[2] = max(mx[2], finite_bits(q.z)), mx[3] = max(mx[3], finite_bits(q.w));
+        }
+    } else if (c < width) {
 #pragma unroll 8
         for (int64_t r = r0 + warp; r < r1; r += 8) {
             const float4 q = factored(src.quad(r, c), row_factor, r);
             mx[0] = max(mx[0], finite_bits(q.x)), mx[1] = max(mx[1], finite_bits(q.y));
             mx[2] = max(mx[2], finite_bits(q.z)), mx[3] = max(mx[3], finite_bits(q.w));
         }
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-        max_s[warp][lane * 4 + q] = mx[q];
+        max_s[warp][src.vec ? lane * 4 + q : lane + 32 * q] = mx[q];
     __syncthreads();
     const int64_t mine = (int64_t)blockIdx.x * 128 + threadIdx.x;
     if (threadIdx.x < 128 && mine < width) {
@@ -251,8 +334,8 @@ __global__ void __launch_bounds__(256) split_cols_kernel(
     }
 }
 
-// out = the slices' sums, in order (and what out held); columns from `second` on to out2.  A block per row and 1024 columns, V values
-// to a thread: with a division for each value and one value to a thread 8192 x 2048 of two slices took 66 us, so 3 TB/s.
+// out = the slices' sums, in order (and what out held); columns from `second` on to out2.  V values to a thread: with a division for each
+// value and one value to a thread 8192 x 2048 of two slices took 66 us, so 29.
 template <int V>
 __global__ void __launch_bounds__(256) join_slices_kernel(
     const float *__restrict__ partial, int slices, int64_t m, int64_t n, float *__restrict__ out, float *__restrict__ out2, int64_t out_cols,
@@ -261,45 +344,38 @@ __global__ void __launch_bounds__(256) join_slices_kernel(
     griddep_launch_dependents();
     if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the slices were not computed
         return;
-    const int64_t total = m * n;
-    for (int64_t r = blockIdx.y; r < m; r += gridDim.y)
-        for (int u = 0; u < 4 / V; ++u) {
-            int64_t c = (int64_t)blockIdx.x * 1024 + (u * 256 + threadIdx.x) * V;
-            if (c >= n)
-                break;
-            const float *src = partial + r * n + c;
-            __align__(16) float v[V];
+    const int64_t total = m * n, c0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    if (c0 >= n)
+        return;
+    for (int64_t r = blockIdx.y; r < m; r += gridDim.y) {
+        const float *src = partial + r * n + c0;
+        float4 s         = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int z = 0; z < slices; ++z) {
             if (V == 4) {
-                float4 s = __ldcs(reinterpret_cast<const float4 *>(src));
-#pragma unroll 4
-                for (int z = 1; z < slices; ++z) {
-                    const float4 q = __ldcs(reinterpret_cast<const float4 *>(src + z * total));
-                    s = make_float4(__fadd_rn(s.x, q.x), __fadd_rn(s.y, q.y), __fadd_rn(s.z, q.z), __fadd_rn(s.w, q.w));
-                }
-                *reinterpret_cast<float4 *>(v) = s;
+                const float4 q = __ldcs(reinterpret_cast<const float4 *>(src + z * total));
+                s = make_float4(__fadd_rn(s.x, q.x), __fadd_rn(s.y, q.y), __fadd_rn(s.z, q.z), __fadd_rn(s.w, q.w));
             } else {
-                v[0] = __ldcs(src);
-#pragma unroll 4
-                for (int z = 1; z < slices; ++z)
-                    v[0] = __fadd_rn(v[0], __ldcs(src + z * total));
-            }
-            float *to = out;
-            if (out2 && c >= second)
-                to = out2, c -= second;
-            if (c >= out_cols)
-                continue;
-            to += r * stride + c;
-            if (V == 4) {
-                float4 s = *reinterpret_cast<const float4 *>(v);
-                if (add) {
-                    const float4 o = *reinterpret_cast<const float4 *>(to);
-                    s = make_float4(__fadd_rn(o.x, s.x), __fadd_rn(o.y, s.y), __fadd_rn(o.z, s.z), __fadd_rn(o.w, s.w));
-                }
-                *reinterpret_cast<float4 *>(to) = s;
-            } else {
-                *to = add ? __fadd_rn(*to, v[0]) : v[0];
+                s.x = __fadd_rn(s.x, __ldcs(src + z * total));
             }
         }
+        int64_t c = c0;
+        float *to = out;
+        if (out2 && c >= second)
+            to = out2, c -= second;
+        if (c >= out_cols)
+            continue;
+        to += r * stride + c;
+        if (V == 4) {
+            if (add) {
+                const float4 o = *reinterpret_cast<const float4 *>(to);
+                s = make_float4(__fadd_rn(o.x, s.x), __fadd_rn(o.y, s.y), __fadd_rn(o.z, s.z), __fadd_rn(o.w, s.w));
+            }
+            *reinterpret_cast<float4 *>(to) = s;
+        } else {
+            *to = add ? __fadd_rn(*to, s.x) : s.x;
+        }
+    }
 }
 
 Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols) {
@@ -340,41 +416,59 @@ static ct_status split_long_cols(DeviceState *st, const Split &x) {
 }
 
 ct_status split(DeviceState *st, const Split *what, int count) {
-    // One launch of all forms while there is little to do, and it is the launches that count; else rows and columns apart.
-    SplitJobs rows{}, cols{};
-    int64_t row_blocks = 0, col_blocks = 0, values = 0;
-    auto add = [&](SplitJobs &jobs, int64_t &blocks, const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int form) {
-        jobs.job[jobs.count++] = SplitJobs::Job{src, width, row_factor, to, inverse, form, blocks};
-        blocks += form == kRowsWarp ? (src.rows + 7) / 8 : form == kRowsBlock ? src.rows : form == kCols16 ? (width + 15) / 16 : (width + 7) / 8;
-        values += src.rows * width;
+    auto blocks_of = [](int form, int64_t rows, int64_t width) {
+        return form == kRowsWarp ? (rows + 7) / 8 : form == kRowsBlock ? rows : form == kCols16 ? (width + 15) / 16 : (width + 7) / 8;
     };
+    auto add = [&](SplitJobs &jobs, int64_t &blocks, const Split &x, const float *in, const float *in2, int64_t at, int form) {
+        const Source src    = source_of(in, in2, x.rows, x.cols);
+        const int64_t width = in2 ? 2 * src.ld : src.ld;
+        Planes to           = x.to;
+        to.hi += at, to.lo += at;
+        jobs.job[jobs.count++] = SplitJobs::Job{src, width, x.row_factor, to, x.by_column ? x.inverse + at : x.inverse, form, blocks};
+        blocks += blocks_of(form, x.rows, width);
+    };
+    // a column job to each matrix, since its columns are its own
+    auto add_cols = [&](SplitJobs &jobs, int64_t &blocks, const Split &x, int form) {
+        add(jobs, blocks, x, x.in, nullptr, 0, form);
+        if (x.in2)
+            add(jobs, blocks, x, x.in2, nullptr, padded(x.cols), form);
+    };
+    // One launch while there is little to do, and it is the launches that count.
+    int64_t values = 0, longest = 0;
     for (int i = 0; i < count; ++i) {
-        const Split &x   = what[i];
-        const Source src = source_of(x.in, x.in2, x.rows, x.cols);
-        if (!x.by_column) {
-            const int64_t width = x.in2 ? 2 * src.ld : src.ld;
-            add(rows, row_blocks, src, width, nullptr, x.to, x.inverse, width <= 1024 ? kRowsWarp : kRowsBlock);
-        } else if (x.rows <= kShort * 64 || (x.rows <= kShort * 128 && x.rows * src.ld <= kFewValues)) {
-            const int form = x.rows <= kShort * 64 ? kCols16 : kCols8;
-            add(cols, col_blocks, source_of(x.in, nullptr, x.rows, x.cols), src.ld, x.row_factor, x.to, x.inverse, form);
-            if (x.in2)
-                add(cols, col_blocks, source_of(x.in2, nullptr, x.rows, x.cols), src.ld, x.row_factor, columns_of(x.to, src.ld, src.ld), x.inverse + src.ld, form);
-        } else {
-            CT_TRY(split_long_cols(st, x));
-        }
+        values += what[i].rows * what[i].cols * (what[i].in2 ? 2 : 1);
+        longest = std::max(longest, what[i].by_column ? what[i].rows : what[i].cols);
     }
-    if (row_blocks + col_blocks > 0x7fffffff)
-        return fail(CT_ERR_TOO_LARGE, "split: too many rows");
-    if (row_blocks > 0 && col_blocks > 0 && values <= kFewValues) {
-        for (int i = 0; i < rows.count; ++i)
-            cols.job[cols.count] = rows.job[i], cols.job[cols.count++].first += col_blocks;
-        CT_CUDA(launch_dependent(split_jobs_kernel<true>, dim3((unsigned)(row_blocks + col_blocks)), dim3(256), 0, stream(), cols));
-        CT_LAUNCH_CHECK("split_jobs");
+    if (values <= kFewValues && longest <= 4096) {
+        SplitJobs jobs{};
+        int64_t blocks = 0;
+        for (int i = 0; i < count; ++i)
+            if (what[i].by_column)
+                add_cols(jobs, blocks, what[i], kCols16);
+            else
+                add(jobs, blocks, what[i], what[i].in, what[i].in2, 0, kRowsWarp);
+        if (blocks > 0) {
+            CT_CUDA(launch_dependent(split_small_kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), jobs));
+            CT_LAUNCH_CHECK("split_small");
+        }
         return CT_OK;
     }
+    SplitJobs rows{}, cols{};
+    int64_t row_blocks = 0, col_blocks = 0;
+    for (int i = 0; i < count; ++i) {
+        const Split &x = what[i];
+        if (!x.by_column)
+            add(rows, row_blocks, x, x.in, x.in2, 0, kRowsBlock);
+        else if (x.rows <= kShort * 64 || (x.rows <= kShort * 128 && x.rows * x.cols <= 4 * kFewValues))
+            add_cols(cols, col_blocks, x, x.rows <= kShort * 64 ? kCols16 : kCols8);
+        else
+            CT_TRY(split_long_cols(st, x));
+    }
+    if (row_blocks > 0x7fffffff || col_blocks > 0x7fffffff)
+        return fail(CT_ERR_TOO_LARGE, "split: too many rows");
     if (col_blocks > 0) {
-        CT_CUDA(launch_dependent(split_jobs_kernel<false>, dim3((unsigned)col_blocks), dim3(256), 0, stream(), cols));
-        CT_LAUNCH_CHECK("split_jobs");
+        CT_CUDA(launch_dependent(split_short_cols_kernel, dim3((unsigned)col_blocks), dim3(256), 0, stream(), cols));
+        CT_LAUNCH_CHECK("split_short_cols");
     }
     for (int i = 0; i < rows.count; ++i) {
         const SplitJobs::Job &x = rows.job[i];
@@ -414,7 +508,7 @@ ct_status product(
         const int64_t tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
         for (int s = 1; s <= 32 && (s == 1 || stages >= 4 * s); ++s) {
             const double waves = (double)((tiles * s + units - 1) / units);
-            const double cost  = waves * (double)((stages + s - 1) / s + 4) * (kind ? 0.95 : 0.6) + (s > 1 ? 3.0 + (double)(m * n) * (s + 1) * 4 / 5e6 : 0.0);
+            const double cost  = waves * (double)((stages + s - 1) / s + 4) * (kind ? 0.95 : 0.6) + (s > 1 ? 3.0 + 0.1 * s + (double)(m * n) * (s + 1) * 4 / 5e6 : 0.0);
             if (cost < best)
                 best = cost, pair = kind != 0, splits = s;
         }
@@ -438,7 +532,7 @@ ct_status product(
     CT_TRY(pair ? (launch_store<256, 2>(st, a, a_mn, b, b_mn, p, e, splits)) : (launch_store<128, 1>(st, a, a_mn, b, b_mn, p, e, splits)));
     if (splits > 1) {
         const bool quads = (n & 3) == 0 && (to.cols & 3) == 0 && (to.stride & 3) == 0 && whole(to.out) && whole(to.out2); // second is a multiple of eight
-        const int64_t strips = (n + 1023) / 1024;
+        const int64_t strips = quads ? (n + 1023) / 1024 : (n + 255) / 256;
         const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(m, 65535), (int64_t)st->sm_count * 16 / strips)));
         CT_CUDA(launch_dependent(quads ? join_slices_kernel<4> : join_slices_kernel<1>, grid, dim3(256), 0, stream(), partial.as<const float>(), splits, m,
                                  n, to.out, to.out2, to.cols, to.stride, to.second, to.add ? 1 : 0, (const uint32_t *)st->flags_dev));

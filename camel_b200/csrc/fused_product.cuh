@@ -8,9 +8,10 @@
 // alone: |error| <= 2^-22 sum |a||b| + 2^-49 max|a| max|b| k, and the additions'.  Scales take any exponent.
 //
 // The tensor core truncates at every addition, always towards zero, which shows in sums of one sign as a bias: the leading
-// accumulator is drained into registers every 256 values of k (16 additions) and summed there with rounding.  The drain has the
-// next stage's cross products to hide behind; with 1024 values 8192 x 2048 x 11008 was 2.5e-6 off (2-norm against 64 bits).
-//
+// accumulator is drained into registers every 128 values of k (8 additions) and summed there with rounding.  The drain has the
+// next stage's cross products to hide behind, and every 256 values 8192 x 2048 x 11008 takes as long; with 1024 it was 2.5e-6 off (2-norm against
+// 64 bits).
+
 // Planes are row-major [rows][ld] float16, ld a multiple of eight.  An operand's rows may be its outer index (K-major) or its k
 // (MN-major): the same planes of d serve d . w^T and x^T . d, and the weights [k][n] are never transposed.  MN-major stages hold 64
 // columns of 64 values of k in 8 KB, the next 64 columns behind them.
@@ -75,6 +76,7 @@ struct Product {
     int stages;       // of 64 values of k
     int stages_split; // > 0: k is cut in slices of that many stages, slice z stores its own result
     int tiles_m, tiles_n, group_m, total;
+    int chunk_first; // stages until a tile's first drain
     int twin_offset; // twin epilogues: column of the planes of B where the second matrix begins
     const float *row_scale, *col_scale; // null: the columns' are one
     uint32_t *flags;
@@ -86,7 +88,8 @@ constexpr int kThreads  = 64 + 32 * kEpiWarps;
 constexpr int kTile     = 128 * 128;  // bytes of one plane of one operand in a stage
 constexpr int kStage    = 4 * kTile;
 constexpr int kStages   = 3;
-constexpr int kChunk    = 4; // stages per drain of the leading accumulator
+// Stages per drain of the leading accumulator: two, and four in the first of a tile that has another tile's epilogue to wait for.
+constexpr int kChunk = 2, kChunkFirst = 4;
 constexpr int kSmem     = kStages * kStage + kEpiWarps * 2048 + 1024;
 
 #ifdef __CUDACC__
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 k_range(tz, from, count);
                 const int set         = SETS == 1 ? 0 : (i & (SETS - 1));
                 const uint32_t d_main = tmem_base + (uint32_t)(set * 2 * BN), d_cross = d_main + BN;
-                int in_chunk = 0;
+                int in_chunk = 0, chunk = p.chunk_first;
                 for (int kb = 0; kb < count; ++kb) {
                     if (!mbar_wait(smem_u32(&bar_full[s]), phase, abort_flag)) {
                         ok = false;
@@ -303,9 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     commit(smem_u32(&bar_empty[s])); // stage reusable once these MMAs retire
                     if (++s == kStages)
                         s = 0, phase ^= 1u;
-                    if (++in_chunk == kChunk || last) {
+                    if (++in_chunk == chunk || last) {
                         commit(smem_u32(&bar_acc_full[set * 2]));
-                        in_chunk = 0;
+                        in_chunk = 0, chunk = kChunk;
                     }
                     if (last)
                         commit(smem_u32(&bar_acc_full[set * 2 + 1]));
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_of(p, tile, tm, tn, tz);
             k_range(tz, from, count);
             const int set    = SETS == 1 ? 0 : (i & (SETS - 1));
-            const int chunks = (count + kChunk - 1) / kChunk;
+            const int chunks = count == 0 ? 0 : count <= p.chunk_first ? 1 : 1 + (count - p.chunk_first + kChunk - 1) / kChunk;
             float acc[COLS];
             const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(set * 2 * BN);
             auto column = [&](int c) { // of the accumulator, of acc[c]
@@ -531,6 +534,7 @@ ct_status launch(DeviceState *st, const Planes &a, const Planes &b, Product p, c
         attr_set_dev[st->device & 15] = true;
     }
     const int64_t units = st->sm_count / CG;
+    p.chunk_first       = tiles <= units ? kChunk : kChunkFirst;
     CT_CUDA(launch_dependent_cluster(kernel, CG, dim3((unsigned)(std::min(tiles, units) * CG)), dim3(kThreads), (size_t)kSmem, stream(), maps, p, e));
     CT_LAUNCH_CHECK(name);
     return CT_OK;

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kern
 template <int GATE>
 __global__ void __launch_bounds__(256) gated_bias_kernel(
     const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, int64_t rows_each,
-    double *__restrict__ partial) {
+    double *__restrict__ partial, float *__restrict__ db_gate, float *__restrict__ db_up) {
     __shared__ float sums[8][2][128];
     griddep_wait();
     griddep_launch_dependents();
@@ -310,7 +310,11 @@ __global__ void __launch_bounds__(256) gated_bias_kernel(
 #pragma unroll
         for (int w = 0; w < 8; ++w)
             all += (double)sums[w][which][at];
-        partial[((int64_t)blockIdx.y * 2 + which) * n + mine] = all;
+        float *to = which ? db_up : db_gate;
+        if (partial)
+            partial[((int64_t)blockIdx.y * 2 + which) * n + mine] = all;
+        else if (to)
+            to[mine] = (float)all;
     }
 }
 
@@ -319,14 +323,17 @@ ct_status gated_bias(
     const int64_t strips = (n + 127) / 128;
     const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((m + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
     const int64_t each = (m + slices - 1) / slices, parts = (m + each - 1) / each;
-    Scratch partial;
-    CT_TRY(partial.get((size_t)(parts * 2 * n) * 8));
+    Scratch partial; // of one part there is nothing to add up
+    if (parts > 1)
+        CT_TRY(partial.get((size_t)(parts * 2 * n) * 8));
     CT_TRY(with_gate(gate, [&](auto G) -> ct_status {
         CT_CUDA(launch_dependent(gated_bias_kernel<G.value>, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), g, u, dout, m, n, vec, each,
-                                 partial.as<double>()));
+                                 parts > 1 ? partial.as<double>() : nullptr, db_gate, db_up));
         CT_LAUNCH_CHECK("gated_bias");
         return CT_OK;
     }));
+    if (parts == 1)
+        return CT_OK;
     return fused::join_columns(partial.as<const double>(), parts, n, true, db_gate, db_up);
 }
 
