@@ -519,8 +519,8 @@ __global__ void __launch_bounds__(256) ce_few_slopes_kernel(
         }
 }
 
-// dx[i][c] = sum over j of d[i][j] w[c][j]: a thread has a column of dx and its weights in registers, d's rows come from shared memory.  Bound
-// by the store of dx; as a product through planes, whose k is a tenth of a stage, 60000 x 10 x 785 took 180 us.
+// dx[i][c] = sum over j of d[i][j] w[c][j]: a thread has two columns of dx and their weights in registers, d's rows come from shared memory.
+// Bound by the store of dx; as a product through planes, whose k is a tenth of a stage, 60000 x 10 x 785 took 180 us.
 template <int N>
 __global__ void __launch_bounds__(256) ce_few_back_kernel(
     const float *__restrict__ d, const float *__restrict__ w, int64_t m, int64_t k, int n, float *__restrict__ dx) {
@@ -528,27 +528,30 @@ __global__ void __launch_bounds__(256) ce_few_back_kernel(
     __shared__ __align__(16) float tile[R][N];
     griddep_wait();
     griddep_launch_dependents();
-    const int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x;
-    float mine[N];
+    const int64_t c0 = (int64_t)blockIdx.y * 2 * blockDim.x + threadIdx.x, c1 = c0 + blockDim.x;
+    float w0[N], w1[N];
 #pragma unroll
     for (int j = 0; j < N; ++j)
-        mine[j] = c < k && j < n ? w[c * n + j] : 0.0f;
+        w0[j] = c0 < k && j < n ? w[c0 * n + j] : 0.0f, w1[j] = c1 < k && j < n ? w[c1 * n + j] : 0.0f;
     for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < m; row0 += (int64_t)gridDim.x * R) {
         const int rows = (int)(m - row0 < R ? m - row0 : R);
         __syncthreads();
-        for (int i = threadIdx.x; i < rows * N; i += 256)
+        for (int i = threadIdx.x; i < rows * N; i += blockDim.x)
             tile[i / N][i % N] = i % N < n ? d[(row0 + i / N) * n + i % N] : 0.0f;
         __syncthreads();
-        if (c < k)
+        if (c0 < k)
 #pragma unroll 4
             for (int r = 0; r < rows; ++r) {
-                float s = 0.0f;
+                float a = 0.0f, b = 0.0f;
 #pragma unroll
                 for (int j = 0; j < N; j += 4) {
                     const float4 q = *reinterpret_cast<const float4 *>(&tile[r][j]);
-                    s = __fmaf_rn(q.x, mine[j], s), s = __fmaf_rn(q.y, mine[j + 1], s), s = __fmaf_rn(q.z, mine[j + 2], s), s = __fmaf_rn(q.w, mine[j + 3], s);
+                    a = __fmaf_rn(q.x, w0[j], a), a = __fmaf_rn(q.y, w0[j + 1], a), a = __fmaf_rn(q.z, w0[j + 2], a), a = __fmaf_rn(q.w, w0[j + 3], a);
+                    b = __fmaf_rn(q.x, w1[j], b), b = __fmaf_rn(q.y, w1[j + 1], b), b = __fmaf_rn(q.z, w1[j + 2], b), b = __fmaf_rn(q.w, w1[j + 3], b);
                 }
-                __stcs(dx + (row0 + r) * k + c, s);
+                dx[(row0 + r) * k + c0] = a;
+                if (c1 < k)
+                    dx[(row0 + r) * k + c1] = b;
             }
     }
 }
@@ -578,12 +581,13 @@ ct_status ce_few_grad(
     if (dw && k > 0)
         CT_TRY(ct_matmul_tn(x, d, k, m, n, dw));
     if (dx && k > 0) {
-        const int64_t strips = (k + 255) / 256;
+        const int64_t strips = (k + 511) / 512; // of as many columns each, two to a thread
         if (strips > 65535)
             return fail(CT_ERR_TOO_LARGE, "dense_cross_entropy_grad: too many columns");
         const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 8 / strips)), (unsigned)strips);
         auto back = n <= 4 ? ce_few_back_kernel<4> : n <= 8 ? ce_few_back_kernel<8> : n <= 12 ? ce_few_back_kernel<12> : n <= 16 ? ce_few_back_kernel<16> : n <= 24 ? ce_few_back_kernel<24> : ce_few_back_kernel<32>;
-        CT_CUDA(launch_dependent(back, grid, dim3(256), 0, stream(), (const float *)d, w, m, k, (int)n, dx));
+        const unsigned threads = (unsigned)(((k + 2 * strips - 1) / (2 * strips) + 31) / 32 * 32);
+        CT_CUDA(launch_dependent(back, grid, dim3(threads), 0, stream(), (const float *)d, w, m, k, (int)n, dx));
         CT_LAUNCH_CHECK("ce_few_back");
     }
     return CT_OK;

@@ -578,36 +578,36 @@ __global__ void __launch_bounds__(256) plane_sums_kernel(
         partial[(int64_t)blockIdx.y * cols + mine] = all;
     }
 }
-// 32 columns to a block, a warp takes every eighth part.
-__global__ void __launch_bounds__(256) join_columns_kernel(
+// 32 columns to a block, a warp takes every 32nd part.
+__global__ void __launch_bounds__(1024) join_columns_kernel(
     const double *__restrict__ partial, int64_t parts, int64_t n, int64_t width, float *__restrict__ first, float *__restrict__ second) {
-    __shared__ double sums[8][32];
+    __shared__ double sums[32][33];
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     double s = 0.0;
     if (c < width)
-#pragma unroll 4
-        for (int64_t p = warp; p < parts; p += 8)
+#pragma unroll 8
+        for (int64_t p = warp; p < parts; p += 32)
             s += partial[p * width + c];
     sums[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < width) {
+    s = sums[lane][warp]; // column `warp` of the block, part `lane`
 #pragma unroll
-        for (int w = 1; w < 8; ++w)
-            s += sums[w][lane];
-        float *out = c < n ? first : second;
-        if (out)
-            out[c < n ? c : c - n] = (float)s;
-    }
+    for (int o = 16; o; o >>= 1)
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + warp;
+    float *out         = mine < n ? first : second;
+    if (lane == 0 && mine < width && out)
+        out[mine < n ? mine : mine - n] = (float)s;
 }
 
 } // namespace
 
 ct_status join_columns(const double *partial, int64_t parts, int64_t n, bool two, float *first, float *second) {
     const int64_t width = two ? 2 * n : n;
-    CT_CUDA(launch_dependent(join_columns_kernel, dim3((unsigned)((width + 31) / 32)), dim3(256), 0, stream(), partial, parts, n, width, first, second));
+    CT_CUDA(launch_dependent(join_columns_kernel, dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, stream(), partial, parts, n, width, first, second));
     CT_LAUNCH_CHECK("join_columns");
     return CT_OK;
 }

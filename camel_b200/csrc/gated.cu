@@ -180,19 +180,20 @@ ct_status gated_fused(
 
 // d = [dg | du] of a row, its largest magnitude, and its planes: TPR threads to a row, which hold V groups of four columns of both; longer
 // rows are computed twice.  inverse[row] is zero for a row of zeros: such a row must not widen the range of x' (gated_grad_fused).
-template <int GATE, int TPR, int V>
+// BIAS: a thread also sums its columns over the rows that it has, in float32, into partial[which of the grid's rows at a time][2][n] - of the
+// values themselves, since what the planes hold of a value depends on the rest of its row.  By a kernel that computes the slopes again
+// 1537 x 2050 took 17 us more.
+template <int GATE, int TPR, int V, bool BIAS>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kernel(
     const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, const fused::Planes to,
-    float *__restrict__ inverse) {
-    __shared__ uint32_t words[32];
+    float *__restrict__ inverse, double *__restrict__ partial) {
+    __shared__ uint32_t words[2][32];
     griddep_wait();
     griddep_launch_dependents();
     constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR, ld = to.ld / 2;
-    if (row >= rows) // whole warps, or the whole block
-        return;
-    auto load = [&](const float *src, int64_t c) {
+    const int64_t row0 = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR, ld = to.ld / 2;
+    auto load = [&](const float *src, int64_t row, int64_t c) {
         src += row * n + c;
         if (vec && c + 3 < n)
             return __ldcs(reinterpret_cast<const float4 *>(src));
@@ -201,8 +202,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kern
         q.z = c + 2 < n ? src[2] : 0.0f, q.w = c + 3 < n ? src[3] : 0.0f;
         return q;
     };
-    auto slopes = [&](int64_t c, float4 &dg, float4 &du) {
-        const float4 a = load(g, c), b = load(u, c), d = load(dout, c);
+    auto slopes = [&](int64_t row, int64_t c, float4 &dg, float4 &du) {
+        const float4 a = load(g, row, c), b = load(u, row, c), d = load(dout, row, c);
         auto one = [](float a, float b, float d, float &dg, float &du) {
             float value, slope;
             gate_slope<GATE>(a, value, slope);
@@ -214,59 +215,79 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kern
         return max(max(fused::finite_bits(q.x), fused::finite_bits(q.y)), max(fused::finite_bits(q.z), fused::finite_bits(q.w)));
     };
     const bool fits = ld <= TPR * V * 4;
-    float4 dg[V], du[V];
-    uint32_t mx = 0;
-    if (fits) {
+    float sum_g[BIAS ? 4 * V : 1] = {}, sum_u[BIAS ? 4 * V : 1] = {};
+    int turn = 0;
+    for (int64_t row = row0; row < rows; row += (int64_t)gridDim.x * RPB, turn ^= 1) { // whole warps, or the whole block
+        float4 dg[V], du[V];
+        uint32_t mx = 0;
+        if (fits) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int64_t c = (int64_t)(j * TPR + t) * 4;
-            dg[j] = du[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (c < n)
-                slopes(c, dg[j], du[j]);
-            mx = max(mx, max(bits(dg[j]), bits(du[j])));
+            for (int j = 0; j < V; ++j) {
+                const int64_t c = (int64_t)(j * TPR + t) * 4;
+                dg[j] = du[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (c < n)
+                    slopes(row, c, dg[j], du[j]);
+                mx = max(mx, max(bits(dg[j]), bits(du[j])));
+                if (BIAS) {
+                    sum_g[4 * j] = __fadd_rn(sum_g[4 * j], dg[j].x), sum_g[4 * j + 1] = __fadd_rn(sum_g[4 * j + 1], dg[j].y);
+                    sum_g[4 * j + 2] = __fadd_rn(sum_g[4 * j + 2], dg[j].z), sum_g[4 * j + 3] = __fadd_rn(sum_g[4 * j + 3], dg[j].w);
+                    sum_u[4 * j] = __fadd_rn(sum_u[4 * j], du[j].x), sum_u[4 * j + 1] = __fadd_rn(sum_u[4 * j + 1], du[j].y);
+                    sum_u[4 * j + 2] = __fadd_rn(sum_u[4 * j + 2], du[j].z), sum_u[4 * j + 3] = __fadd_rn(sum_u[4 * j + 3], du[j].w);
+                }
+            }
+        } else {
+            for (int64_t c = t * 4; c < n; c += TPR * 4) {
+                slopes(row, c, dg[0], du[0]);
+                mx = max(mx, max(bits(dg[0]), bits(du[0])));
+            }
         }
-    } else {
-        for (int64_t c = t * 4; c < n; c += TPR * 4) {
-            slopes(c, dg[0], du[0]);
-            mx = max(mx, max(bits(dg[0]), bits(du[0])));
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (TPR > 32) {
+            if ((threadIdx.x & 31) == 0)
+                words[turn][threadIdx.x >> 5] = mx;
+            __syncthreads();
+            mx = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < TPR / 32 ? words[turn][threadIdx.x & 31] : 0u);
         }
-    }
-    mx = __reduce_max_sync(0xffffffffu, mx);
-    if (TPR > 32) {
-        if ((threadIdx.x & 31) == 0)
-            words[threadIdx.x >> 5] = mx;
-        __syncthreads();
-        mx = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < TPR / 32 ? words[threadIdx.x & 31] : 0u);
-    }
-    const float s = fused::line_scale(mx);
-    auto put      = [&](int64_t c, const float4 &q) {
-        __half2 hi[2], lo[2];
-        fused::split2(q.x * s, q.y * s, hi[0], lo[0]);
-        fused::split2(q.z * s, q.w * s, hi[1], lo[1]);
-        *reinterpret_cast<uint2 *>(to.hi + row * to.ld + c) = *reinterpret_cast<uint2 *>(hi);
-        *reinterpret_cast<uint2 *>(to.lo + row * to.ld + c) = *reinterpret_cast<uint2 *>(lo);
-    };
-    if (fits) {
+        const float s = fused::line_scale(mx);
+        auto put      = [&](int64_t c, const float4 &q) {
+            __half2 hi[2], lo[2];
+            fused::split2(q.x * s, q.y * s, hi[0], lo[0]);
+            fused::split2(q.z * s, q.w * s, hi[1], lo[1]);
+            *reinterpret_cast<uint2 *>(to.hi + row * to.ld + c) = *reinterpret_cast<uint2 *>(hi);
+            *reinterpret_cast<uint2 *>(to.lo + row * to.ld + c) = *reinterpret_cast<uint2 *>(lo);
+        };
+        if (fits) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int64_t c = (int64_t)(j * TPR + t) * 4;
-            if (c < ld)
-                put(c, dg[j]), put(ld + c, du[j]);
+            for (int j = 0; j < V; ++j) {
+                const int64_t c = (int64_t)(j * TPR + t) * 4;
+                if (c < ld)
+                    put(c, dg[j]), put(ld + c, du[j]);
+            }
+        } else {
+            for (int64_t c = t * 4; c < ld; c += TPR * 4) {
+                dg[0] = du[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (c < n)
+                    slopes(row, c, dg[0], du[0]);
+                put(c, dg[0]), put(ld + c, du[0]);
+            }
         }
-    } else {
-        for (int64_t c = t * 4; c < ld; c += TPR * 4) {
-            dg[0] = du[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (c < n)
-                slopes(c, dg[0], du[0]);
-            put(c, dg[0]), put(ld + c, du[0]);
-        }
+        if (t == 0)
+            inverse[row] = mx ? fused::line_inverse(mx) : 0.0f;
     }
-    if (t == 0)
-        inverse[row] = mx ? fused::line_inverse(mx) : 0.0f;
+    if (BIAS) {
+        double *mine = partial + row0 * 2 * n; // row0 counts the rows that the grid has at a time
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t c = (int64_t)(j * TPR + t) * 4 + q;
+                if (c < n)
+                    mine[c] = (double)sum_g[4 * j + q], mine[n + c] = (double)sum_u[4 * j + q];
+            }
+    }
 }
 
-// The columns' sums of dg and du, from the values themselves: what the planes hold of a value depends on the rest of its row.  A lane has
-// four columns, a warp every eighth row of the block's; partial[block][2][n] are added up by join_columns.
+// The columns' sums of dg and du where rows are too long for the kernel above to keep theirs.  A lane has four columns, a warp every eighth row of the block's; partial[block][2][n] are added up by join_columns.
 template <int GATE>
 __global__ void __launch_bounds__(256) gated_bias_kernel(
     const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, int64_t rows_each,
@@ -337,24 +358,45 @@ ct_status gated_bias(
     return fused::join_columns(partial.as<const double>(), parts, n, true, db_gate, db_up);
 }
 
+constexpr int64_t kSlopesFit = 512 * 4 * 4; // columns
+
 template <int GATE, int TPR, int V>
 ct_status launch_slopes_of(
-    const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse) {
+    const DeviceState *st, const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse,
+    float *db_gate, float *db_up) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-    CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V>, dim3((unsigned)((m + RPB - 1) / RPB)), dim3(TPR * RPB), 0, stream(), g, u, dout, m,
-                             n, vec, to, inverse));
+    int64_t blocks    = (m + RPB - 1) / RPB;
+    if (!db_gate && !db_up) {
+        CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V, false>, dim3((unsigned)blocks), dim3(TPR * RPB), 0, stream(), g, u, dout, m, n, vec,
+                                 to, inverse, (double *)nullptr));
+        CT_LAUNCH_CHECK("gated_slopes");
+        return CT_OK;
+    }
+    blocks = std::min<int64_t>(blocks, (int64_t)st->sm_count * (TPR <= 256 ? 4 : 2));
+    Scratch partial;
+    CT_TRY(partial.get((size_t)(blocks * RPB * 2 * n) * 8));
+    CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V, true>, dim3((unsigned)blocks), dim3(TPR * RPB), 0, stream(), g, u, dout, m, n, vec, to,
+                             inverse, partial.as<double>()));
     CT_LAUNCH_CHECK("gated_slopes");
-    return CT_OK;
+    return fused::join_columns(partial.as<const double>(), blocks * RPB, n, true, db_gate, db_up);
 }
 template <int GATE>
-ct_status launch_slopes(const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse) {
+ct_status launch_slopes(
+    const DeviceState *st, const float *g, const float *u, const float *dout, int64_t m, int64_t n, int vec, const fused::Planes &to, float *inverse,
+    float *db_gate, float *db_up) {
+    if (n <= 128)
+        return launch_slopes_of<GATE, 32, 1>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
     if (n <= 256)
-        return launch_slopes_of<GATE, 32, 2>(g, u, dout, m, n, vec, to, inverse);
+        return launch_slopes_of<GATE, 32, 2>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
     if (n <= 1024)
-        return launch_slopes_of<GATE, 256, 1>(g, u, dout, m, n, vec, to, inverse);
+        return launch_slopes_of<GATE, 256, 1>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
+    if (n <= 2048)
+        return launch_slopes_of<GATE, 256, 2>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
     if (n <= 4096)
-        return launch_slopes_of<GATE, 512, 2>(g, u, dout, m, n, vec, to, inverse);
-    return launch_slopes_of<GATE, 512, 4>(g, u, dout, m, n, vec, to, inverse);
+        return launch_slopes_of<GATE, 512, 2>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
+    if (n <= 6144)
+        return launch_slopes_of<GATE, 512, 3>(st, g, u, dout, m, n, vec, to, inverse, db_gate, db_up);
+    return launch_slopes_of<GATE, 512, 4>(st, g, u, dout, m, n, vec, to, inverse, n <= kSlopesFit ? db_gate : nullptr, n <= kSlopesFit ? db_up : nullptr);
 }
 
 ct_status gated_grad_fused(
@@ -371,8 +413,8 @@ ct_status gated_grad_fused(
     CT_TRY(s.get(parts.bytes));
     const Planes pd = planes_at(s, dp, m, 2 * ln, 2 * ln);
     const int vec   = (n & 3) == 0 && whole(gate_pre) && whole(up_pre) && whole(dout) ? 1 : 0;
-    CT_TRY(with_gate(gate, [&](auto G) { return launch_slopes<G.value>(gate_pre, up_pre, dout, m, n, vec, pd, s.as<float>(di)); }));
-    if (db_gate || db_up)
+    CT_TRY(with_gate(gate, [&](auto G) { return launch_slopes<G.value>(st, gate_pre, up_pre, dout, m, n, vec, pd, s.as<float>(di), db_gate, db_up); }));
+    if (n > kSlopesFit && (db_gate || db_up))
         CT_TRY(gated_bias(st, gate_pre, up_pre, dout, m, n, gate, vec, db_gate, db_up));
     const Planes pw = planes_at(s, wp, k, 2 * ln, 2 * ln), px = planes_at(s, xp, m, lk, lk);
     Split operands[2];
