@@ -10,6 +10,7 @@
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
 // A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
 // Up to 32 classes, and under the reduced precision, the logits of a piece of the rows are computed by the library's products.
+#include "fastmath.cuh"
 #include "stream_product.cuh"
 
 namespace ct {
@@ -563,9 +564,239 @@ ct_status few_logits(DeviceState *st, const float *x, const float *w, const floa
     return ct_dense(x, w, bias, m, k, n, CT_ACT_NONE, z, nullptr);
 }
 
+// The whole gradient of up to 16 classes and 1024 columns of x in one reading of x, float32: 16 rows of x in shared memory at a time, the
+// next ones on their way.  Logits: a warp has four rows and a quarter of the columns of each 128, and its 4 N sums meet by halves; d: a
+// thread to each; then a thread has two columns of dx, dw and w in registers and walks the rows.
+// Bound by issue, some 1000 instructions a row (two values an FMA); as five kernels, each with its own reading of x or of d, 60000 x 785 x 10 took
+// 212 us.  dw's sums are chains of a CTA's rows (m / 148), joined in 64 bits.
+constexpr int kOneRows = 16, kOneThreads = 512, kOneColumns = 2 * kOneThreads;
+
+template <int N> constexpr int one_words(int64_t k, int ring) { // of shared memory: rows of x, w, parts of the logits, d
+    return ring * kOneRows * (int)k + (int)k * N + 4 * kOneRows * N + kOneRows * N;
+}
+
+// v[0 .. COUNT) summed over the warp, halves of the values to halves of the lanes: lane l ends up with the COUNT / 16 values from
+// (l >> 1) * COUNT / 16 on.
+template <int COUNT> __device__ __forceinline__ void sum_by_halves(float (&v)[COUNT]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+        const int half = COUNT >> (step + 1), o = 16 >> step;
+        const bool up  = lane & o;
+#pragma unroll
+        for (int i = 0; i < COUNT / 2; ++i)
+            if (i < half) {
+                const float keep = up ? v[i + half] : v[i], give = up ? v[i] : v[i + half];
+                v[i]             = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, o));
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < COUNT / 16; ++i)
+        v[i] = __fadd_rn(v[i], __shfl_xor_sync(0xffffffffu, v[i], 1));
+}
+
+template <int N, int RING>
+__global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
+    const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ bias, const int64_t *__restrict__ targets,
+    const float *__restrict__ lse, const float *__restrict__ dloss, int64_t m, int k, int n, float *__restrict__ dx, double *__restrict__ partial) {
+    extern __shared__ __align__(16) float smem[];
+    __shared__ int has_s[kOneRows]; // a row without a target takes no part, whatever x holds there
+    float *xs = smem, *parts = xs + RING * kOneRows * k, *ds = parts + 4 * kOneRows * N, *ws = ds + kOneRows * N;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t tiles = (m + kOneRows - 1) / kOneRows;
+    auto fetch = [&](int64_t tile, int at) {
+        if (tile < tiles) {
+            const int64_t left = (m - tile * kOneRows < kOneRows ? m - tile * kOneRows : kOneRows) * k; // values; the rows are one piece
+            const float *src   = x + tile * kOneRows * k;
+            const uint32_t to  = ptx::smem_u32(xs + at * kOneRows * k);
+            for (int64_t i = 4 * t; i < left; i += 4 * kOneThreads)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (uint32_t)i * 4), "l"(src + i), "r"(left - i < 4 ? (int)(left - i) * 4 : 16)
+                             : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < RING; ++i)
+        fetch(blockIdx.x + (int64_t)i * gridDim.x, i);
+    for (int i = t; i < k * N; i += kOneThreads)
+        ws[i] = i % N < n ? w[(i / N) * n + i % N] : 0.0f;
+    f32x2 wc[2][N / 2], sum[2][N / 2]; // of columns t and t + 512
+    float sum_b = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            const int c = t + q * kOneThreads;
+            wc[q][j]    = pack2(c < k && 2 * j < n ? w[(int64_t)c * n + 2 * j] : 0.0f, c < k && 2 * j + 1 < n ? w[(int64_t)c * n + 2 * j + 1] : 0.0f);
+            sum[q][j]   = 0;
+        }
+    const int group = warp & 3, quarter = warp >> 2;
+    int at = 0;
+    int64_t before = -1; // the tile whose place is free
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+        __syncthreads();
+        const float *rows_at = xs + at * kOneRows * k;
+        const int rows       = (int)(m - tile * kOneRows < kOneRows ? m - tile * kOneRows : kOneRows);
+        // what d needs of this thread's row is on its way meanwhile
+        const int64_t row = tile * kOneRows + t / N;
+        const bool slope  = t < kOneRows * N && t / N < rows && t % N < n;
+        const int64_t target = slope ? __ldg(targets + row) : -1;
+        const float l = slope ? __ldg(lse + row) : 0.0f, by = slope && dloss ? __ldg(dloss + row) : 1.0f, add = slope && bias ? __ldg(bias + t % N) : 0.0f;
+        { // the logits' parts
+            f32x2 acc[4][N / 2];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j)
+                    acc[r][j] = 0;
+            const float *mine = rows_at + group * 4 * k;
+#pragma unroll 2
+            for (int c = quarter * 32 + lane; c < k; c += 128) {
+                f32x2 wv[N / 2];
+#pragma unroll
+                for (int j = 0; j < N / 4; ++j) {
+                    const float4 q = *reinterpret_cast<const float4 *>(ws + c * N + 4 * j);
+                    wv[2 * j] = pack2(q.x, q.y), wv[2 * j + 1] = pack2(q.z, q.w);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float v = mine[r * k + c];
+#pragma unroll
+                    for (int j = 0; j < N / 2; ++j)
+                        acc[r][j] = fma2(pack2(v, v), wv[j], acc[r][j]);
+                }
+            }
+            float v[4 * N];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j)
+                    unpack2(acc[r][j], v[r * N + 2 * j], v[r * N + 2 * j + 1]);
+            sum_by_halves<4 * N>(v);
+            if (!(lane & 1))
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i)
+                    parts[(quarter * kOneRows + group * 4) * N + (lane >> 1) * (N / 4) + i] = v[i];
+        }
+        __syncthreads();
+        if (before >= 0) // all are through with the tile before
+            fetch(before + (int64_t)RING * gridDim.x, at == 0 ? RING - 1 : at - 1);
+        before = tile;
+        if (t < kOneRows * N) {
+            const int j = t % N;
+            float d     = 0.0f;
+            if (slope) {
+                float z = parts[t];
+#pragma unroll
+                for (int q = 1; q < 4; ++q)
+                    z = __fadd_rn(z, parts[q * kOneRows * N + t]);
+                if (bias)
+                    z = __fadd_rn(z, add);
+                const float p  = expf(__fsub_rn(z, l));
+                const bool has = target >= 0 && target < n;
+                if (j == 0)
+                    has_s[t / N] = has;
+                if (has)
+                    d = __fmul_rn(by, j == target ? __fsub_rn(p, 1.0f) : p);
+            }
+            ds[t] = d;
+        }
+        __syncthreads();
+        if (t < N)
+            for (int r = 0; r < rows; ++r)
+                sum_b = __fadd_rn(sum_b, ds[r * N + t]);
+        const bool here[2] = {t < k, t + kOneThreads < k};
+        if (here[0])
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const bool has = has_s[r] != 0;
+                f32x2 d[N / 2];
+#pragma unroll
+                for (int j = 0; j < N / 4; ++j) {
+                    const float4 q = *reinterpret_cast<const float4 *>(ds + r * N + 4 * j);
+                    d[2 * j] = pack2(q.x, q.y), d[2 * j + 1] = pack2(q.z, q.w);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (here[q]) {
+                        const int c   = t + q * kOneThreads;
+                        const float v = has ? rows_at[r * k + c] : 0.0f;
+                        f32x2 back    = 0;
+#pragma unroll
+                        for (int j = 0; j < N / 2; ++j) {
+                            sum[q][j] = fma2(pack2(v, v), d[j], sum[q][j]);
+                            back      = fma2(d[j], wc[q][j], back);
+                        }
+                        float a, b;
+                        unpack2(back, a, b);
+                        if (dx)
+                            dx[(tile * kOneRows + r) * k + c] = __fadd_rn(a, b);
+                    }
+            }
+        at = at == RING - 1 ? 0 : at + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!partial)
+        return;
+    double *to = partial + (int64_t)blockIdx.x * ((int64_t)k * n + n);
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            const int c = t + q * kOneThreads;
+            float a, b;
+            unpack2(sum[q][j], a, b);
+            if (c < k && 2 * j < n)
+                to[(int64_t)c * n + 2 * j] = (double)a;
+            if (c < k && 2 * j + 1 < n)
+                to[(int64_t)c * n + 2 * j + 1] = (double)b;
+        }
+    if (t < n)
+        to[(int64_t)k * n + t] = (double)sum_b;
+}
+
+bool ce_one_applicable(const float *x, int64_t k, int64_t n) {
+    return n <= 16 && k > 0 && k <= kOneColumns && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+}
+
+template <int N, int RING>
+ct_status launch_ce_one(
+    const DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m,
+    int64_t k, int64_t n, float *dx, float *dw, float *dbias) {
+    const int smem = one_words<N>(k, RING) * 4;
+    auto kernel    = ce_one_kernel<N, RING>;
+    static bool attr_set_dev[16] = {};
+    if (!attr_set_dev[st->device & 15]) {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+        attr_set_dev[st->device & 15] = true;
+    }
+    const int64_t grid = std::min<int64_t>((m + kOneRows - 1) / kOneRows, st->sm_count), width = k * n + n;
+    Scratch partial;
+    if (dw || dbias)
+        CT_TRY(partial.get((size_t)(grid * width) * 8));
+    CT_CUDA(launch_dependent(kernel, dim3((unsigned)grid), dim3(kOneThreads), (size_t)smem, stream(), x, w, bias, targets, lse, dloss, m, (int)k, (int)n, dx,
+                             dw || dbias ? partial.as<double>() : nullptr));
+    CT_LAUNCH_CHECK("ce_one");
+    return dw || dbias ? fused::join_columns(partial.as<const double>(), grid, k * n, width, dw, dbias) : CT_OK;
+}
+template <int N>
+ct_status launch_ce_one_ring(
+    const DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m,
+    int64_t k, int64_t n, float *dx, float *dw, float *dbias) {
+    return one_words<N>(k, 3) * 4 <= 224 * 1024 ? launch_ce_one<N, 3>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias)
+                                                : launch_ce_one<N, 2>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+}
+
 ct_status ce_few_grad(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
     int64_t n, float *dx, float *dw, float *dbias) {
+    if (ce_one_applicable(x, k, n)) {
+        auto run = n <= 4 ? launch_ce_one_ring<4> : n <= 8 ? launch_ce_one_ring<8> : n <= 12 ? launch_ce_one_ring<12> : launch_ce_one_ring<16>;
+        return run(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+    }
     const int64_t blocks = (m + 255) / 256;
     fused::Parts parts;
     const size_t zp = parts.take((size_t)(m * n) * 4), pp = parts.take(dbias ? (size_t)(blocks * n) * 8 : 0);
@@ -577,7 +808,7 @@ ct_status ce_few_grad(
                              dbias ? s.as<double>(pp) : nullptr));
     CT_LAUNCH_CHECK("ce_few_slopes");
     if (dbias)
-        CT_TRY(fused::join_columns(s.as<const double>(pp), blocks, n, false, dbias, nullptr));
+        CT_TRY(fused::join_columns(s.as<const double>(pp), blocks, n, n, dbias, nullptr));
     if (dw && k > 0)
         CT_TRY(ct_matmul_tn(x, d, k, m, n, dw));
     if (dx && k > 0) {

@@ -605,8 +605,7 @@ __global__ void __launch_bounds__(1024) join_columns_kernel(
 
 } // namespace
 
-ct_status join_columns(const double *partial, int64_t parts, int64_t n, bool two, float *first, float *second) {
-    const int64_t width = two ? 2 * n : n;
+ct_status join_columns(const double *partial, int64_t parts, int64_t n, int64_t width, float *first, float *second) {
     CT_CUDA(launch_dependent(join_columns_kernel, dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, stream(), partial, parts, n, width, first, second));
     CT_LAUNCH_CHECK("join_columns");
     return CT_OK;
@@ -620,7 +619,7 @@ ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight,
     CT_TRY(partial.get((size_t)(parts * x.cols) * 8));
     CT_CUDA(launch_dependent(plane_sums_kernel, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), x, row_weight, each, partial.as<double>()));
     CT_LAUNCH_CHECK("plane_sums");
-    return join_columns(partial.as<const double>(), parts, x.cols, false, out, nullptr);
+    return join_columns(partial.as<const double>(), parts, x.cols, x.cols, out, nullptr);
 }
 
 } // namespace fused

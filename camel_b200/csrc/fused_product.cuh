@@ -590,8 +590,8 @@ ct_status product(
     const Result &to);
 // out[c] = sum over the rows of row_weight[r] * planes[r][c].
 ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight, float *out);
-// first[c] = sum over parts of partial[part][c], and where there are two second[c] of partial[part][n + c]; either may be null.
-ct_status join_columns(const double *partial, int64_t parts, int64_t n, bool two, float *first, float *second);
+// first[c] = sum over parts of partial[part][c] for c < n, second[c] of partial[part][n + c] for n + c < width; either may be null.
+ct_status join_columns(const double *partial, int64_t parts, int64_t n, int64_t width, float *first, float *second);
 
 // out[m][n] = x . w + bias for at most kFewRows rows, or gate(x . w + bias) * (x . w_up + b_up) (w_up non-null), float32 on the CUDA cores.
 constexpr int64_t kFewRows = 16;

@@ -355,7 +355,7 @@ ct_status gated_bias(
     }));
     if (parts == 1)
         return CT_OK;
-    return fused::join_columns(partial.as<const double>(), parts, n, true, db_gate, db_up);
+    return fused::join_columns(partial.as<const double>(), parts, n, 2 * n, db_gate, db_up);
 }
 
 constexpr int64_t kSlopesFit = 512 * 4 * 4; // columns
@@ -378,7 +378,7 @@ ct_status launch_slopes_of(
     CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V, true>, dim3((unsigned)blocks), dim3(TPR * RPB), 0, stream(), g, u, dout, m, n, vec, to,
                              inverse, partial.as<double>()));
     CT_LAUNCH_CHECK("gated_slopes");
-    return fused::join_columns(partial.as<const double>(), blocks * RPB, n, true, db_gate, db_up);
+    return fused::join_columns(partial.as<const double>(), blocks * RPB, n, 2 * n, db_gate, db_up);
 }
 template <int GATE>
 ct_status launch_slopes(
