@@ -829,7 +829,7 @@ ct_status check_ce(const char *name, const void *x, const void *w, const void *t
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
     if (n == 0 && m > 0)
         return fail(CT_ERR_INVALID, "%s: no classes", name);
-    if (m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
+    if (m > fused::kMostSize || n > fused::kMostSize || k > fused::kMostSize)
         return fail(CT_ERR_TOO_LARGE, "%s: dimension too large", name);
     if (m > 0 && (!targets || (k > 0 && (!x || !w))))
         return fail(CT_ERR_INVALID, "%s: null pointer", name);

@@ -59,6 +59,9 @@ __device__ __forceinline__ void split2(float a, float b, __half2 &hi, __half2 &l
 __device__ __forceinline__ float weight(float row, float col) { return fminf(__fmul_rn(row, col), 1.7014118346e38f); }
 #endif
 
+// Sizes that tile coordinates of 32 bits hold, two matrices side by side and what is rounded up included.
+constexpr int64_t kMostSize = 1 << 29;
+
 // Planes of a matrix [rows][cols], and where one factor per row or column stands (the caller knows which).
 struct Planes {
     __half *hi = nullptr, *lo = nullptr;

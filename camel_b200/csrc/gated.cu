@@ -471,7 +471,7 @@ ct_status ct_dense_gated(
         return CT_OK;
     if (!out || (k > 0 && (!x || !w_gate || !w_up)))
         return fail(CT_ERR_INVALID, "dense_gated: null pointer");
-    if (m > 0x7fffffff || k > 0x7fffffff || n > 0x3fffffff)
+    if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
         return fail(CT_ERR_TOO_LARGE, "dense_gated: dimension too large");
     ProfScope prof("dense_gated");
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
@@ -522,7 +522,7 @@ ct_status ct_dense_gated_grad(
         CT_CUDA(clear(db_up, n));
         return CT_OK;
     }
-    if (m > 0x7fffffff || k > 0x7fffffff || n > 0x3fffffff)
+    if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
         return fail(CT_ERR_TOO_LARGE, "dense_gated_grad: dimension too large");
     if (ct_get_precision() == CT_PREC_3XTF32)
         return gated_grad_fused(st, x, w_gate, w_up, gate_pre, up_pre, dout, m, k, n, gate, dx, dw_gate, dw_up, db_gate, db_up);
