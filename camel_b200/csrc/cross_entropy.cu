@@ -9,7 +9,8 @@
 // pairs under one scale.  A piece of the vocabulary at a time they are the left operand of dx += d . w^T as they lie (rows weighted by
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
 // A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
-// Up to 32 classes, and under the reduced precision, the logits of a piece of the rows are computed by the library's products.
+// Few classes (kFewClasses) take kernels of their own, whose logits are memory's smallest part; under the reduced precision the logits of a
+// piece of the rows are written, by the library's products.
 #include "fastmath.cuh"
 #include "stream_product.cuh"
 
@@ -55,6 +56,17 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(
             lse[blockIdx.x] = l;
         if (loss)
             loss[blockIdx.x] = t >= 0 && t < n ? __fsub_rn(l, row[t]) : 0.0f;
+    }
+}
+
+// x without the rows that have no target: 0 x anything of theirs is no term of dw.
+__global__ void __launch_bounds__(256) ce_rows_with_target_kernel(
+    const float *__restrict__ x, const int64_t *__restrict__ targets, int64_t count, int64_t k, int64_t n, float *__restrict__ out) {
+    griddep_wait();
+    griddep_launch_dependents();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = targets[i / k];
+        out[i]          = t >= 0 && t < n ? x[i] : 0.0f;
     }
 }
 
@@ -457,7 +469,9 @@ ct_status ce_grad_fused(
 
 // ---- few classes: logits of up to kFewClasses columns, as the library's few-column products give them ----
 
-constexpr int kFewClasses = 32;
+// From 17 classes on the tiles of 128 win, empty as most of them is: gradient of 60000 x 785 x 17 494 us against 1626 (the library's products
+// of more than 16 columns read x in many strips), of 2000 x 256 x 20 54 against 50.  At 10 classes the kernels below take 170 us, tiles as much as at 17.
+constexpr int kFewClasses = 16;
 
 // A thread per row.
 __global__ void __launch_bounds__(256) ce_few_kernel(
@@ -520,44 +534,78 @@ __global__ void __launch_bounds__(256) ce_few_slopes_kernel(
         }
 }
 
-// dx[i][c] = sum over j of d[i][j] w[c][j]: a thread has two columns of dx and their weights in registers, d's rows come from shared memory.
-// Bound by the store of dx; as a product through planes, whose k is a tenth of a stage, 60000 x 10 x 785 took 180 us.
+// dx = d . w^T and the parts of dw = x^T . d in one reading of x and d: a thread has a column of x, its weights and its sums in registers, 64
+// rows of d come from shared memory at a time.  Blocks are strips x parts; a part has every parts-th 64 rows.  A row without a target takes
+// no part, whatever x holds there.  Bound by issue, n FMAs of two values to a value of x.  Sums are chains of a part's rows, joined in 64 bits.
 template <int N>
 __global__ void __launch_bounds__(256) ce_few_back_kernel(
-    const float *__restrict__ d, const float *__restrict__ w, int64_t m, int64_t k, int n, float *__restrict__ dx) {
+    const float *__restrict__ d, const float *__restrict__ x, const float *__restrict__ w, const int64_t *__restrict__ targets, int64_t m, int64_t k, int n,
+    int64_t strips, int64_t parts, float *__restrict__ dx, double *__restrict__ partial) {
     constexpr int R = 64;
     __shared__ __align__(16) float tile[R][N];
+    __shared__ int has_s[R];
     griddep_wait();
     griddep_launch_dependents();
-    const int64_t c0 = (int64_t)blockIdx.y * 2 * blockDim.x + threadIdx.x, c1 = c0 + blockDim.x;
-    float w0[N], w1[N];
+    const int64_t part = blockIdx.x / strips, c = (blockIdx.x - part * strips) * 256 + threadIdx.x;
+    f32x2 wc[N / 2], sum[N / 2];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-        w0[j] = c0 < k && j < n ? w[c0 * n + j] : 0.0f, w1[j] = c1 < k && j < n ? w[c1 * n + j] : 0.0f;
-    for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < m; row0 += (int64_t)gridDim.x * R) {
+    for (int j = 0; j < N / 2; ++j) {
+        wc[j]  = pack2(c < k && 2 * j < n ? w[c * n + 2 * j] : 0.0f, c < k && 2 * j + 1 < n ? w[c * n + 2 * j + 1] : 0.0f);
+        sum[j] = 0;
+    }
+    for (int64_t row0 = part * R; row0 < m; row0 += parts * R) {
         const int rows = (int)(m - row0 < R ? m - row0 : R);
         __syncthreads();
-        for (int i = threadIdx.x; i < rows * N; i += blockDim.x)
+        for (int i = threadIdx.x; i < rows * N; i += 256)
             tile[i / N][i % N] = i % N < n ? d[(row0 + i / N) * n + i % N] : 0.0f;
+        if ((int)threadIdx.x < rows) {
+            const int64_t t   = targets[row0 + threadIdx.x];
+            has_s[threadIdx.x] = t >= 0 && t < n;
+        }
         __syncthreads();
-        if (c0 < k)
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                float a = 0.0f, b = 0.0f;
+        if (c >= k)
+            continue;
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            float v[8];
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(&tile[r][j]);
-                    a = __fmaf_rn(q.x, w0[j], a), a = __fmaf_rn(q.y, w0[j + 1], a), a = __fmaf_rn(q.z, w0[j + 2], a), a = __fmaf_rn(q.w, w0[j + 3], a);
-                    b = __fmaf_rn(q.x, w1[j], b), b = __fmaf_rn(q.y, w1[j + 1], b), b = __fmaf_rn(q.z, w1[j + 2], b), b = __fmaf_rn(q.w, w1[j + 3], b);
+            for (int i = 0; i < 8; ++i)
+                v[i] = partial && r0 + i < rows && has_s[r0 + i] ? x[(row0 + r0 + i) * k + c] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (r0 + i >= rows)
+                    break;
+                f32x2 back = 0, e[N / 2];
+#pragma unroll
+                for (int j = 0; j < N / 4; ++j) {
+                    const float4 q = *reinterpret_cast<const float4 *>(&tile[r0 + i][4 * j]);
+                    e[2 * j] = pack2(q.x, q.y), e[2 * j + 1] = pack2(q.z, q.w);
                 }
-                dx[(row0 + r) * k + c0] = a;
-                if (c1 < k)
-                    dx[(row0 + r) * k + c1] = b;
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    sum[j] = fma2(pack2(v[i], v[i]), e[j], sum[j]);
+                    back   = fma2(e[j], wc[j], back);
+                }
+                if (dx) {
+                    float a, b;
+                    unpack2(back, a, b);
+                    dx[(row0 + r0 + i) * k + c] = __fadd_rn(a, b);
+                }
             }
+        }
     }
+    if (partial && c < k)
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            float a, b;
+            unpack2(sum[j], a, b);
+            if (2 * j < n)
+                partial[(part * k + c) * n + 2 * j] = (double)a;
+            if (2 * j + 1 < n)
+                partial[(part * k + c) * n + 2 * j + 1] = (double)b;
+        }
 }
 
-// The logits of few classes: of few rows by few_rows, whose cluster shares k (5 x 429 x 31 took 28 us as the library's few-column product).
+// The logits of few classes: of few rows by few_rows, whose cluster shares k.
 ct_status few_logits(DeviceState *st, const float *x, const float *w, const float *bias, int64_t m, int64_t k, int64_t n, float *z) {
     if (m <= fused::kFewRows && k > 0 && ct_get_precision() == CT_PREC_3XTF32)
         return fused::few_rows(st, x, w, bias, nullptr, nullptr, m, k, n, 0, z, nullptr, nullptr);
@@ -567,8 +615,8 @@ ct_status few_logits(DeviceState *st, const float *x, const float *w, const floa
 // The whole gradient of up to 16 classes and 1024 columns of x in one reading of x, float32: 16 rows of x in shared memory at a time, the
 // next ones on their way.  Logits: a warp has four rows and a quarter of the columns of each 128, and its 4 N sums meet by halves; d: a
 // thread to each; then a thread has two columns of dx, dw and w in registers and walks the rows.
-// Bound by issue, some 1000 instructions a row (two values an FMA); as five kernels, each with its own reading of x or of d, 60000 x 785 x 10 took
-// 212 us.  dw's sums are chains of a CTA's rows (m / 148), joined in 64 bits.
+// Bound by issue, some 1000 instructions a row (two values an FMA): 60000 x 785 x 10 takes 170 us, at the copy rate it would be 58; as five
+// kernels, each with its own reading of x or of d, it took 212.  dw's sums are chains of a CTA's rows (m / 148), joined in 64 bits.
 constexpr int kOneRows = 16, kOneThreads = 512, kOneColumns = 2 * kOneThreads;
 
 template <int N> constexpr int one_words(int64_t k, int ring) { // of shared memory: rows of x, w, parts of the logits, d
@@ -758,8 +806,8 @@ __global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
         to[(int64_t)k * n + t] = (double)sum_b;
 }
 
-bool ce_one_applicable(const float *x, int64_t k, int64_t n) {
-    return n <= 16 && k > 0 && k <= kOneColumns && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+bool ce_one_applicable(const float *x, int64_t k) { // n <= kFewClasses
+    return k > 0 && k <= kOneColumns && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
 }
 
 template <int N, int RING>
@@ -793,7 +841,7 @@ ct_status launch_ce_one_ring(
 ct_status ce_few_grad(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
     int64_t n, float *dx, float *dw, float *dbias) {
-    if (ce_one_applicable(x, k, n)) {
+    if (ce_one_applicable(x, k)) {
         auto run = n <= 4 ? launch_ce_one_ring<4> : n <= 8 ? launch_ce_one_ring<8> : n <= 12 ? launch_ce_one_ring<12> : launch_ce_one_ring<16>;
         return run(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     }
@@ -809,17 +857,17 @@ ct_status ce_few_grad(
     CT_LAUNCH_CHECK("ce_few_slopes");
     if (dbias)
         CT_TRY(fused::join_columns(s.as<const double>(pp), blocks, n, n, dbias, nullptr));
-    if (dw && k > 0)
-        CT_TRY(ct_matmul_tn(x, d, k, m, n, dw));
-    if (dx && k > 0) {
-        const int64_t strips = (k + 511) / 512; // of as many columns each, two to a thread
-        if (strips > 65535)
-            return fail(CT_ERR_TOO_LARGE, "dense_cross_entropy_grad: too many columns");
-        const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 8 / strips)), (unsigned)strips);
-        auto back = n <= 4 ? ce_few_back_kernel<4> : n <= 8 ? ce_few_back_kernel<8> : n <= 12 ? ce_few_back_kernel<12> : n <= 16 ? ce_few_back_kernel<16> : n <= 24 ? ce_few_back_kernel<24> : ce_few_back_kernel<32>;
-        const unsigned threads = (unsigned)(((k + 2 * strips - 1) / (2 * strips) + 31) / 32 * 32);
-        CT_CUDA(launch_dependent(back, grid, dim3(threads), 0, stream(), (const float *)d, w, m, k, (int)n, dx));
+    if ((dw || dx) && k > 0) {
+        const int64_t strips = (k + 255) / 256, parts = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 4 / strips));
+        Scratch sums;
+        if (dw)
+            CT_TRY(sums.get((size_t)(parts * k * n) * 8));
+        auto back = n <= 4 ? ce_few_back_kernel<4> : n <= 8 ? ce_few_back_kernel<8> : n <= 12 ? ce_few_back_kernel<12> : ce_few_back_kernel<16>;
+        CT_CUDA(launch_dependent(back, dim3((unsigned)(strips * parts)), dim3(256), 0, stream(), (const float *)d, x, w, targets, m, k, (int)n, strips,
+                                 parts, dx, dw ? sums.as<double>() : nullptr));
         CT_LAUNCH_CHECK("ce_few_back");
+        if (dw)
+            CT_TRY(fused::join_columns(sums.as<const double>(), parts, k * n, k * n, dw, nullptr));
     }
     return CT_OK;
 }
@@ -903,13 +951,15 @@ ct_status ct_dense_cross_entropy_grad(
     if (n <= kFewClasses)
         return ce_few_grad(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     const int64_t piece = rows_at_once(m, n);
-    Scratch logits, turned, sums;
+    Scratch logits, turned, sums, kept;
     CT_TRY(logits.get((size_t)(piece * n) * 4));
     float *d = logits.as<float>();
     if (dx && k > 0) {
         CT_TRY(turned.get((size_t)(k * n) * 4));
         CT_TRY(ct_transpose(CT_F32, w, k, n, turned.as<float>()));
     }
+    if (dw && k > 0)
+        CT_TRY(kept.get((size_t)(piece * k) * 4));
     if (piece < m)
         CT_TRY(sums.get((size_t)(k * n + n) * 4));
     for (int64_t r = 0; r < m; r += piece) {
@@ -922,7 +972,10 @@ ct_status ct_dense_cross_entropy_grad(
         if (dx && k > 0)
             CT_TRY(ct_matmul(CT_F32, d, CT_F32, turned.as<float>(), rows, n, k, dx + r * k));
         if (dw && k > 0) {
-            CT_TRY(ct_matmul_tn(x + r * k, d, k, rows, n, r ? sums.as<float>() : dw));
+            CT_CUDA(launch_dependent(ce_rows_with_target_kernel, dim3((unsigned)std::min<int64_t>((rows * k + 255) / 256, (int64_t)st->sm_count * 16)),
+                                     dim3(256), 0, stream(), x + r * k, targets + r, rows * k, k, n, kept.as<float>()));
+            CT_LAUNCH_CHECK("ce_rows_with_target");
+            CT_TRY(ct_matmul_tn(kept.as<const float>(), d, k, rows, n, r ? sums.as<float>() : dw));
             if (r)
                 CT_TRY(ct_binary(CT_ADD, CT_F32, dw, CT_F32, sums.as<float>(), (uint64_t)(k * n), dw));
         }

@@ -350,7 +350,12 @@ ct_status ct_dense_packed(
 /* ---- layers of deeper networks and their gradients --------------------------------------
  * The reference has none of these operators; the formulas stand with each.  Matrices are row-major float32 as everywhere.  An
  * output must not overlap an input or another output, except where a function says so.  A gradient is that of a sum over everything
- * weighted by the given gradient of the output; outputs that are null are not computed. */
+ * weighted by the given gradient of the output; outputs that are null are not computed.  Dimensions go up to 2^29.
+ *
+ * Products of more than 16 rows hold each operand as pairs of float16 under one power of two per row (or per column, where rows are summed
+ * over): to 2^-23 of a value down to 2^-27 of its line's largest, to 2^-50 of that largest below.  The error of a sum is at most 2^-22 of
+ * its products' sizes and 2^-49 of its length times the two lines' largest, and the additions'.  Under CT_PREC_BF16 the products are
+ * those of ct_dense. */
 
 /* Layer norm of each row: out = (x - mean) / sqrt(var + eps) * gamma + beta, mean and var (the mean square deviation) over the
  * row's `cols` values.  gamma and beta have one value per column; null: ones, zeros.  eps >= 0.  out may be x itself. */
@@ -377,13 +382,16 @@ ct_status ct_dense_gated_grad(
 
 /* Softmax cross entropy of the logits z = x . w + bias (x [m][k], w [k][n], bias [n] or null), which are not kept:
  *   lse[i] = log(sum over j of exp(z[i][j])), loss[i] = lse[i] - z[i][targets[i]].
- * A target outside 0 .. n-1 marks a row that has none (padding): its loss is 0.  loss or lse may be null; n >= 1. */
+ * A target outside 0 .. n-1 marks a row that has none (padding): its loss is 0, whatever x holds there.  loss or lse may be null;
+ * n >= 1. */
 ct_status ct_dense_cross_entropy(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, int64_t m, int64_t k, int64_t n,
     float *loss_dev, float *lse_dev);
-/* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
+/* Its gradient, with lse as the forward call left it (exp(z - lse) up to 4 is represented) and the gradient dloss [m] of the losses
+ * (null: ones):
  *   d[i][j] = dloss[i] * (exp(z[i][j] - lse[i]) - (j == targets[i])), zero in rows without a target,
- *   dx = d . w^T, dw = x^T . d, dbias the columns' sums of d.  The logits are computed again, in pieces. */
+ *   dx = d . w^T, dw = x^T . d, dbias the columns' sums of d.  The logits are computed again, in pieces.  A row without a target takes
+ * no part in the sums, whatever x and dloss hold there. */
 ct_status ct_dense_cross_entropy_grad(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, const float *lse_dev,
     const float *dloss_dev, int64_t m, int64_t k, int64_t n, float *dx_dev, float *dw_dev, float *dbias_dev);

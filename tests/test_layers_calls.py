@@ -214,8 +214,17 @@ def test_memory_that_holds_anything():
 
 
 @gpu
-@pytest.mark.parametrize("m,k,n", [(300, 64, 200), (60, 64, 200), (8, 64, 200), (300, 64, 10)])
-def test_padding_rows_may_hold_nan(m, k, n):
+@pytest.mark.parametrize("precision", ["3xtf32", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(300, 64, 200), (60, 64, 200), (8, 64, 200), (300, 64, 10), (300, 64, 24), (300, 1100, 10), (9, 64, 32)])
+def test_padding_rows_may_hold_nan(m, k, n, precision):
+    L.check(L.lib.ct_set_precision(L.PREC_BF16 if precision == "bf16" else L.PREC_3XTF32))
+    try:
+        padding_rows(m, k, n)
+    finally:
+        L.check(L.lib.ct_set_precision(L.PREC_3XTF32))
+
+
+def padding_rows(m, k, n):
     """Rows without a target: whatever x holds there, their loss is 0 and they have no part in the gradients."""
     x, w, b, t = ce_inputs(m, k, n, 28)
     t[:] = np.random.default_rng(0).integers(0, n, m)
