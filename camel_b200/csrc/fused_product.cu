@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(256, 2) split_short_cols_kernel(const __grid_c
 }
 
 // All of a small product's operands: a warp to a row, a block to 16 columns, read twice (the second time from L1).  In registers as above
-// they are read once, but the code is ten times as long, and fetching it is what a launch of a few blocks then waits for (5 against 20 us
-// with cold caches).
+// they are read once, but the code is ten times as long, and fetching it is what a launch of a few blocks then waits for (8 to 10 against
+// 18 to 24 us with cold caches).
 __global__ void __launch_bounds__(256) split_small_kernel(const __grid_constant__ SplitJobs jobs) {
     __shared__ uint32_t many[8][16];
     griddep_wait();

@@ -1,9 +1,8 @@
 // Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), and its gradient.
 //
 // Forward: one product whose tiles have the same columns of both weight matrices (fused_product.cuh); a thread of the epilogue
-// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu; up to
-// 128: stream_product.cuh.
-// Gradient: gated_slopes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
+// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu; up to 128: stream_product.cuh.
+// Gradient: gated_slope_planes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
 // dx = d . [w_gate | w_up]^T as they lie, and the right operand of dw = x'^T . d with their rows as k, x' being x with the rows' scales
 // taken back.  So d is written once, 8 bytes for each of its values' pairs of terms, and read in place.
 // The reduced precision runs the library's products one after the other.
@@ -287,7 +286,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) gated_slope_planes_kern
     }
 }
 
-// The columns' sums of dg and du where rows are too long for the kernel above to keep theirs.  A lane has four columns, a warp every eighth row of the block's; partial[block][2][n] are added up by join_columns.
+// The columns' sums of dg and du where rows are too long for the kernel above to keep theirs (kSlopesFit).  A lane has four columns, a warp
+// every eighth row of the block's; partial[block][2][n] are added up by join_columns.
 template <int GATE>
 __global__ void __launch_bounds__(256) gated_bias_kernel(
     const float *__restrict__ g, const float *__restrict__ u, const float *__restrict__ dout, int64_t rows, int64_t n, int vec, int64_t rows_each,

@@ -1,11 +1,13 @@
 // Products of 17 to 128 rows: the weights are streamed through the tensor cores as they lie, float32, and read once.
 //
 // With so few rows a product is as long as it takes to read the weights, and writing their planes and reading them again is three times that
-// (64 x 1024 x 32003: 76 us of pre-pass, 33 of product).  So four warps fetch the weights, 64 values of k of 128 columns a stage (cp.async in the
-// 16-byte pieces that they lie in), and two groups of eight, which take stages in turn, split them under a scale per column and stage, and write the planes to shared memory.  The weights' columns are the rows of the accumulator
-// (128 lanes), the rows of x its columns (32 or 64; more rows go by 64, a launch each), so that a scale belongs to a lane and a stage: eight warps drain every stage and add it up
-// in registers under its scale.  x comes as planes (K-major, a scale per row) by TMA.
-// What bounds it is HBM; per stage the MMAs take 12 x 54 clocks (64 rows) of the 1400 in which its 32 KB arrive.
+// (64 x 1024 x 32003: 76 us of pre-pass, 33 of product; here 63 in all).  So four warps fetch the weights, 64 values of k of 128 columns a stage
+// (cp.async in the 16-byte pieces that they lie in), and two groups of eight, which take stages in turn, split them under a scale per
+// column and stage, and write the planes to shared memory.  The weights' columns are the rows of the accumulator (128 lanes), the rows
+// of x its columns (32 or 64; more rows go by 64, a launch each), so that a scale belongs to a lane and a stage: eight warps drain every
+// stage and add it up in registers under its scale.  x comes as planes (K-major, a scale per row) by TMA.
+// What bounds it: HBM would bring a stage's 32 KB in 1400 clocks, the MMAs take 12 x 54 of them (64 rows); splitting, scaling and draining
+// keep the issue slots 62 % busy and a stage takes some 2000.  64 x 1024 x 128000 takes 147 us, 3.6 TB/s.
 // A CTA has a range of columns, a multiple of 16, so that all CTAs have as much to read.
 //
 // Epilogue: the tile's sums go to shared memory as [row of x][column], 16 rows at a time; the draining warps do with them what EPI says.
