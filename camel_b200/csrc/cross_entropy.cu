@@ -9,9 +9,11 @@
 // pairs under one scale.  A piece of the vocabulary at a time they are the left operand of dx += d . w^T as they lie (rows weighted by
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
 // A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
+// Up to 16 rows have their logits written, and take few_rows.cu and few_rows_grad.cuh.
 // Few classes (kFewClasses) take kernels of their own, whose logits are memory's smallest part; under the reduced precision the logits of a
 // piece of the rows are written, by the library's products.
 #include "fastmath.cuh"
+#include "few_rows_grad.cuh"
 #include "stream_product.cuh"
 
 namespace ct {
@@ -623,26 +625,6 @@ template <int N> constexpr int one_words(int64_t k, int ring) { // of shared mem
     return ring * kOneRows * (int)k + (int)k * N + 4 * kOneRows * N + kOneRows * N;
 }
 
-// v[0 .. COUNT) summed over the warp, halves of the values to halves of the lanes: lane l ends up with the COUNT / 16 values from
-// (l >> 1) * COUNT / 16 on.
-template <int COUNT> __device__ __forceinline__ void sum_by_halves(float (&v)[COUNT]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-        const int half = COUNT >> (step + 1), o = 16 >> step;
-        const bool up  = lane & o;
-#pragma unroll
-        for (int i = 0; i < COUNT / 2; ++i)
-            if (i < half) {
-                const float keep = up ? v[i + half] : v[i], give = up ? v[i] : v[i + half];
-                v[i]             = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, o));
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < COUNT / 16; ++i)
-        v[i] = __fadd_rn(v[i], __shfl_xor_sync(0xffffffffu, v[i], 1));
-}
-
 template <int N, int RING>
 __global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
     const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ bias, const int64_t *__restrict__ targets,
@@ -723,7 +705,7 @@ __global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j)
                     unpack2(acc[r][j], v[r * N + 2 * j], v[r * N + 2 * j + 1]);
-            sum_by_halves<4 * N>(v);
+            fused::sum_by_halves<4 * N>(v);
             if (!(lane & 1))
 #pragma unroll
                 for (int i = 0; i < N / 4; ++i)
@@ -872,6 +854,71 @@ ct_status ce_few_grad(
     return CT_OK;
 }
 
+// Few rows: their logits are written.
+struct LogitsStream {
+    static constexpr bool kTwin = false;
+    struct Params {
+        const float *bias;
+        float *out;
+    };
+    struct State {};
+    __device__ static __forceinline__ void init(State &) {}
+    template <int Q>
+    __device__ static __forceinline__ void tile(const fused::Stream &p, const Params &e, State &, const float *z, int64_t c0, int cols, int t) {
+        const int lane = t & 31, rows = p.m - 16 * Q < 16 ? p.m - 16 * Q : 16;
+        for (int i = t >> 5; i < rows; i += fused::kStreamDrain) {
+            const int r    = 16 * Q + i;
+            const float rs = p.row_scale[r] * fused::kStreamUp;
+#pragma unroll
+            for (int c = lane; c < 128; c += 32)
+                if (c < cols) {
+                    const float v = __fmul_rn(z[i * fused::kStreamPitch + c], rs);
+                    e.out[r * p.n + c0 + c] = e.bias ? __fadd_rn(v, __ldg(e.bias + c0 + c)) : v;
+                }
+        }
+    }
+    __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, float *, int) {}
+};
+ct_status few_rows_logits(DeviceState *st, const float *x, const float *w, const float *bias, int64_t m, int64_t k, int64_t n, float *z) {
+    using namespace fused;
+    if (takes_few_rows(m, n))
+        return few_rows(st, x, w, bias, nullptr, nullptr, m, k, n, 0, z, nullptr, nullptr);
+    const int64_t lk = padded(k);
+    Parts parts;
+    const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4);
+    Scratch s;
+    CT_TRY(s.get(parts.bytes));
+    const Planes px     = planes_at(s, xp, m, lk, lk);
+    const Split operand = {x, nullptr, m, k, false, nullptr, px, s.as<float>(xi)};
+    CT_TRY(split(st, &operand, 1));
+    Stream p{};
+    p.w = w, p.k = k, p.n = p.ld = n, p.row_scale = s.as<float>(xi);
+    return launch_stream<LogitsStream>(st, px, p, LogitsStream::Params{bias, z}, "cross_entropy_grad", [](LogitsStream::Params f, int64_t) { return f; });
+}
+
+// Few rows: d of the logits.
+struct FewSlopes {
+    static constexpr int kMatrices = 1;
+    const float *z, *lse, *dloss;
+    const int64_t *targets;
+    int64_t n;
+    __device__ __forceinline__ bool has(int r) const { return targets[r] >= 0 && targets[r] < n; }
+    __device__ __forceinline__ float at(int, int r, int64_t c) const {
+        const float v = expf(__fsub_rn(z[r * n + c], lse[r]));
+        return __fmul_rn(dloss ? dloss[r] : 1.0f, c == targets[r] ? __fsub_rn(v, 1.0f) : v);
+    }
+};
+ct_status ce_few_rows_grad(
+    DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
+    int64_t n, float *dx, float *dw, float *dbias) {
+    Scratch logits;
+    CT_TRY(logits.get((size_t)(m * n) * 4));
+    CT_TRY(few_rows_logits(st, x, w, bias, m, k, n, logits.as<float>()));
+    fused::FewGrad p{};
+    p.x = x, p.w[0] = w, p.dw[0] = dw, p.db[0] = dbias, p.dx = dx, p.k = k, p.n = n, p.m = (int)m;
+    return fused::few_rows_grad(st, p, FewSlopes{logits.as<const float>(), lse, dloss, targets, n});
+}
+
 ct_status check_ce(const char *name, const void *x, const void *w, const void *targets, int64_t m, int64_t k, int64_t n) {
     if (m < 0 || k < 0 || n < 0)
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
@@ -904,7 +951,7 @@ ct_status ct_dense_cross_entropy(
         return CT_OK;
     ProfScope prof("cross_entropy");
     const bool fused_form = n > kFewClasses && k > 0 && ct_get_precision() == CT_PREC_3XTF32;
-    if (fused_form && m > fused::kFewRows)
+    if (fused_form && !fused::takes_few_rows(m, n))
         return ce_fused(st, x, w, bias, targets, m, k, n, loss, lse);
     const int64_t piece = n <= kFewClasses ? m : rows_at_once(m, n);
     Scratch logits;
@@ -946,6 +993,8 @@ ct_status ct_dense_cross_entropy_grad(
         return CT_OK;
     }
     ProfScope prof("cross_entropy_grad");
+    if (m <= fused::kFewRows && m * n <= (int64_t)1 << 28 && k > 0 && ct_get_precision() == CT_PREC_3XTF32 && (dx || dw || dbias))
+        return ce_few_rows_grad(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     if (n > kFewClasses && k > 0 && ct_get_precision() == CT_PREC_3XTF32)
         return ce_grad_fused(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     if (n <= kFewClasses)

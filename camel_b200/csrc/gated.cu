@@ -1,13 +1,14 @@
 // Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), and its gradient.
 //
 // Forward: one product whose tiles have the same columns of both weight matrices (fused_product.cuh); a thread of the epilogue
-// has both sums of an output and stores what the layer gives.  Up to 16 rows: few_rows.cu; up to 128: stream_product.cuh.
+// has both sums of an output and stores what the layer gives.  Up to 8 or 16 rows (takes_few_rows): few_rows.cu; up to 128: stream_product.cuh.
 // Gradient: gated_slope_planes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
 // dx = d . [w_gate | w_up]^T as they lie, and the right operand of dw = x'^T . d with their rows as k, x' being x with the rows' scales
 // taken back.  So d is written once, 8 bytes for each of its values' pairs of terms, and read in place.
-// The reduced precision runs the library's products one after the other.
-#include "stream_product.cuh"
+// Up to 16 rows: few_rows_grad.cuh.  The reduced precision runs the library's products one after the other.
+#include "few_rows_grad.cuh"
 #include "gate.cuh"
+#include "stream_product.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -441,6 +442,20 @@ ct_status gated_grad_fused(
     return CT_OK;
 }
 
+// Few rows: dg or du of what was kept.
+template <int GATE> struct FewGateSlopes {
+    static constexpr int kMatrices = 2;
+    const float *g, *u, *dout;
+    int64_t n;
+    __device__ __forceinline__ bool has(int) const { return true; }
+    __device__ __forceinline__ float at(int which, int r, int64_t c) const {
+        const int64_t i = r * n + c;
+        float value, slope;
+        gate_slope<GATE>(g[i], value, slope);
+        return which ? __fmul_rn(dout[i], value) : __fmul_rn(__fmul_rn(dout[i], u[i]), slope);
+    }
+};
+
 unsigned grid_of(const DeviceState *st, int64_t count) {
     return (unsigned)std::min<int64_t>((count + 255) / 256, (int64_t)st->sm_count * 16);
 }
@@ -475,7 +490,7 @@ ct_status ct_dense_gated(
         return fail(CT_ERR_TOO_LARGE, "dense_gated: dimension too large");
     ProfScope prof("dense_gated");
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
-        if (m <= fused::kFewRows)
+        if (fused::takes_few_rows(m, 2 * n))
             return fused::few_rows(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
         if (m <= fused::kStreamRows)
             return gated_stream(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
@@ -524,6 +539,12 @@ ct_status ct_dense_gated_grad(
     }
     if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
         return fail(CT_ERR_TOO_LARGE, "dense_gated_grad: dimension too large");
+    if (ct_get_precision() == CT_PREC_3XTF32 && m <= fused::kFewRows && k > 0 && (dx || dw_gate || dw_up || db_gate || db_up)) {
+        fused::FewGrad p{};
+        p.x = x, p.w[0] = w_gate, p.w[1] = w_up, p.dw[0] = dw_gate, p.dw[1] = dw_up, p.db[0] = db_gate, p.db[1] = db_up;
+        p.dx = dx, p.k = k, p.n = n, p.m = (int)m;
+        return with_gate(gate, [&](auto G) { return fused::few_rows_grad(st, p, FewGateSlopes<G.value>{gate_pre, up_pre, dout, n}); });
+    }
     if (ct_get_precision() == CT_PREC_3XTF32)
         return gated_grad_fused(st, x, w_gate, w_up, gate_pre, up_pre, dout, m, k, n, gate, dx, dw_gate, dw_up, db_gate, db_up);
     const int64_t count = m * n;

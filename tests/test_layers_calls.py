@@ -127,6 +127,21 @@ def test_dense_gated_grad_of_many_rows(m, k, n):
 
 
 @gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 16])
+@pytest.mark.parametrize("k,n", [(1, 7), (97, 1300), (300, 3100), (41, 1024)])
+def test_few_rows(m, k, n):
+    """Blocks of 1024 columns and parts of the weights' rows; and 9 to 16 rows of wide layers, whose logits are streamed."""
+    x, wg, wu, bg, bu = gated_inputs(m, k, n, 29)
+    check_gated(x, wg, wu, bg, bu, "gelu")
+    g, u, dout = (np.random.default_rng(i).normal(0, 1, (m, n)).astype(np.float32) for i in range(3))
+    check_gated_grad(x, wg, wu, g, u, dout, "gelu")
+    for classes in (n + 20, 2 * n + 100):
+        x, w, b, t = ce_inputs(m, k, classes, 29)
+        check_ce(x, w, b, t)
+        check_ce_grad(x, w, b, t, np.random.default_rng(3).uniform(0.5, 1, m).astype(np.float32))
+
+
+@gpu
 def test_dense_gated_wide_rows():
     """Rows of d that no block holds (n beyond 8192)."""
     m, k, n = 12, 24, 8300
