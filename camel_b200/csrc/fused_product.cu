@@ -2,7 +2,7 @@
 //
 // The pre-passes are bound by memory: 4 bytes read and 4 written a value.  A scale is found and used while its line is in registers: rows of up to
 // 8192 values, a warp or a block to each, and columns of up to 2048, a block to 16 (8) of them.  Longer lines are read twice, the second
-// time from L2 where that holds them.  All operands of a product whose columns are short are split in one launch.
+// time from L2 where that holds them; rows of up to 65536 by clusters, once.  All operands of a product whose columns are short are split in one launch.
 #include "fused_product.cuh"
 
 namespace ct {
@@ -261,6 +261,53 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const Source src, int64
     split_rows<TPR, V>(src, width, to, inverse, blockIdx.x, words);
 }
 
+// Longer rows, a cluster of CTAs to each, 8192 values to a CTA.  Read twice, as rows beyond that are, 1024 x 50257 took 183 us: all rows are under
+// way at once, and L2 does not hold them.
+constexpr int kLongQuads = 8;
+__global__ void __launch_bounds__(256) split_long_rows_kernel(
+    const Source src, int64_t width, int ranks, int64_t each, const Planes to, float *__restrict__ inverse) {
+    __shared__ uint32_t words[8], most;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t = threadIdx.x, rank = (int)(blockIdx.x % ranks);
+    const int64_t row = blockIdx.x / ranks, first = rank * each, last = min(width, first + each);
+    float4 v[kLongQuads];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int j = 0; j < kLongQuads; ++j) {
+        const int64_t c = first + (int64_t)(j * 256 + t) * 4;
+        v[j]            = c < last ? src.quad(row, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < kLongQuads; ++j)
+        mx = max(mx, quad_bits(v[j]));
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if ((t & 31) == 0)
+        words[t >> 5] = mx;
+    __syncthreads();
+    if (t == 0) {
+        for (int w = 0; w < 8; ++w)
+            mx = max(mx, words[w]);
+        most = mx;
+    }
+    ptx::cluster_sync();
+    for (int q = 0; q < ranks; ++q) {
+        uint32_t other;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(other) : "r"(ptx::mapa(ptx::smem_u32(&most), (uint32_t)q)) : "memory");
+        mx = max(mx, other);
+    }
+    const float s = line_scale(mx);
+#pragma unroll
+    for (int j = 0; j < kLongQuads; ++j) {
+        const int64_t c = first + (int64_t)(j * 256 + t) * 4;
+        if (c < last)
+            put_quad(to, row * to.ld + c, v[j].x * s, v[j].y * s, v[j].z * s, v[j].w * s);
+    }
+    if (t == 0 && rank == 0)
+        inverse[row] = line_inverse(mx);
+    ptx::cluster_sync(); // a CTA's word stays until the others have read it
+}
+
 // Largest finite magnitude of each column into col_max (zeroed before): a lane has four columns, the block's warps the rows in turn.
 __global__ void __launch_bounds__(256) col_max_kernel(
     const Source src, int64_t width, const float *__restrict__ row_factor, int64_t rows_each, uint32_t *__restrict__ col_max) {
@@ -487,7 +534,12 @@ ct_status split(DeviceState *st, const Split *what, int count) {
             CT_CUDA(run(split_rows_kernel<256, 4>, 1));
         else if (x.width <= 8192)
             CT_CUDA(run(split_rows_kernel<256, 8>, 1));
-        else
+        else if (x.width <= 8 * kLongQuads * 1024) {
+            const int ranks    = x.width <= 2 * kLongQuads * 1024 ? 2 : x.width <= 4 * kLongQuads * 1024 ? 4 : 8;
+            const int64_t each = (x.width + 4 * ranks - 1) / (4 * ranks) * 4;
+            CT_CUDA(launch_dependent_cluster(split_long_rows_kernel, ranks, dim3((unsigned)(x.src.rows * ranks)), dim3(256), 0, stream(), x.src, x.width, ranks, each,
+                                             x.to, x.inverse));
+        } else
             CT_CUDA(run(split_rows_kernel<256, 16>, 1));
         CT_LAUNCH_CHECK("split_rows");
     }

@@ -192,7 +192,7 @@ def big_ce(m, k, n):
 
 
 @gpu
-@pytest.mark.parametrize("m,k,n", [(4100, 40, 33001), (128, 17, 1048600), (2000, 64, 70000)])
+@pytest.mark.parametrize("m,k,n", [(4100, 40, 33001), (128, 17, 1048600), (2000, 64, 70000), (150, 40, 12001), (150, 41, 20004)])
 def test_cross_entropy_vocabulary_in_pieces(m, k, n):
     big_ce(m, k, n)
 
