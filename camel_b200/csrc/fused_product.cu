@@ -11,12 +11,21 @@ namespace {
 
 // Two matrices side by side, the second from column ld on; zeros between cols and ld.
 struct Source {
-    const float *in, *in2;
+    const float *in, *in2, *col_factor;
     int64_t rows, cols, ld;
     int vec; // rows of both are whole and aligned float4
+    __device__ __forceinline__ float4 quad(int64_t r, int64_t c) const {
+        float4 q = plain_quad(r, c);
+        if (col_factor) { // of columns that there are
+            const float4 f = *reinterpret_cast<const float4 *>(col_factor + c);
+            q.x = q.x != 0.0f ? q.x * f.x : 0.0f, q.y = q.y != 0.0f ? q.y * f.y : 0.0f;
+            q.z = q.z != 0.0f ? q.z * f.z : 0.0f, q.w = q.w != 0.0f ? q.w * f.w : 0.0f;
+        }
+        return q;
+    }
     // Columns c .. c + 3, c a multiple of four.  Rows that are not aligned take a load for each: as aligned pieces, with what a lane lacks shuffled over
     // from the next one, columns of 1024 x 32003 took 160 us for 85, the selects and shuffles outweighing the loads.
-    __device__ __forceinline__ float4 quad(int64_t r, int64_t c) const {
+    __device__ __forceinline__ float4 plain_quad(int64_t r, int64_t c) const {
         const float *src = in;
         if (c >= ld)
             src = in2, c -= ld;
@@ -425,9 +434,9 @@ __global__ void __launch_bounds__(256) join_slices_kernel(
     }
 }
 
-Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols) {
+Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols, const float *col_factor = nullptr) {
     const bool vec = (cols & 3) == 0 && (reinterpret_cast<uintptr_t>(in) & 15u) == 0 && (reinterpret_cast<uintptr_t>(in2) & 15u) == 0;
-    return Source{in, in2, rows, cols, padded(cols), vec ? 1 : 0};
+    return Source{in, in2, col_factor, rows, cols, padded(cols), vec ? 1 : 0};
 }
 
 template <int BN, int CG>
@@ -467,7 +476,7 @@ ct_status split(DeviceState *st, const Split *what, int count) {
         return form == kRowsWarp ? (rows + 7) / 8 : form == kRowsBlock ? rows : form == kCols16 ? (width + 15) / 16 : (width + 7) / 8;
     };
     auto add = [&](SplitJobs &jobs, int64_t &blocks, const Split &x, const float *in, const float *in2, int64_t at, int form) {
-        const Source src    = source_of(in, in2, x.rows, x.cols);
+        const Source src    = source_of(in, in2, x.rows, x.cols, x.col_factor);
         const int64_t width = in2 ? 2 * src.ld : src.ld;
         Planes to           = x.to;
         to.hi += at, to.lo += at;

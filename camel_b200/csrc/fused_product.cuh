@@ -38,8 +38,8 @@ constexpr float kLoScale = 2048.0f, kLoInv = 1.0f / 2048.0f;
 
 // From the largest finite magnitude of a line: the factor that brings it to [2^14, 2^15), and its inverse; both normal numbers.
 __host__ __device__ __forceinline__ int line_exponent(uint32_t max_bits) {
-    const int e = max_bits == 0 ? 14 : (int)(max_bits >> 23) - 127;
-    return e < -100 ? -100 : e;
+    const int e = (int)(max_bits >> 23) - 127;
+    return e < -100 ? -100 : e; // a line of zeros: its factor widens no other line's range
 }
 #ifdef __CUDACC__
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -578,6 +578,7 @@ struct Split {
     const float *row_factor; // by_column, may be null: row r is taken times row_factor[r], and as zeros where that is zero
     Planes to;
     float *inverse;        // [rows], or scales(columns of the planes)
+    const float *col_factor = nullptr; // else, may be null: column c is taken times col_factor[c] (a multiple of four of them)
 };
 ct_status split(DeviceState *st, const Split *what, int count);
 

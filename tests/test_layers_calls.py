@@ -198,6 +198,18 @@ def test_cross_entropy_vocabulary_in_pieces(m, k, n):
 
 
 @gpu
+def test_weights_whose_rows_and_columns_differ_in_size():
+    """Rows of the weights 2^-30 .. 2^30 against columns of x the other way, a row of zeros, columns 2^-30 below the others."""
+    for m, k, n in ((200, 60, 20000), (200, 60, 300)):
+        x, w, b, t = ce_inputs(m, k, n, 30)
+        e = np.random.default_rng(1).integers(-30, 31, k)
+        x, w = np.ldexp(x, e).astype(np.float32), np.ldexp(w, -e[:, None]).astype(np.float32)
+        w[7] = 0.0
+        w[:, ::9] *= np.float32(2.0 ** -30)
+        check_ce_grad(x, w, b, t, np.ones(m, np.float32))
+
+
+@gpu
 def test_memory_that_holds_anything():
     """Scratch comes from a pool of freed tensors: what they held does not show."""
     cx, cw, cb, ct = ce_inputs(150, 75, 333, 26)
