@@ -1,7 +1,7 @@
 // Operand planes of the fused products (fused_product.cuh), and the product that is simply stored.
 //
 // The pre-passes are bound by memory: 4 bytes read and 4 written a value.  A scale is found and used while its line is in registers: rows of up to
-// 8192 values, a warp or a block to each, and columns of up to 2048, a block to 16 (8) of them.  Longer lines are read twice, the second
+// 8192 values, a warp or a block to each, and columns of up to 1024, a block to 16 of them.  Longer lines are read twice, the second
 // time from L2 where that holds them; rows of up to 65536 by clusters, once.  All operands of a product whose columns are short are split in one launch.
 #include "fused_product.cuh"
 
@@ -112,13 +112,12 @@ __device__ __forceinline__ void split_rows(const Source &src, int64_t width, con
         inverse[row] = line_inverse(mx);
 }
 
-// 4 L columns to the block, L lanes to a row; at most kShort rows of 256 / L to a thread.
+// 16 columns to the block, four lanes to a row; at most kShort rows of 64 to a thread.
 constexpr int kShort = 16;
 constexpr int64_t kFewValues = 1 << 20;
-template <int L>
 __device__ __forceinline__ void split_short_cols(
     const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int64_t block, uint32_t (&words)[8][16]) {
-    constexpr int RP = 256 / L;
+    constexpr int L = 4, RP = 256 / L;
     const int t = threadIdx.x, quad = t % L;
     const int64_t c = block * (4 * L) + quad * 4;
     float4 v[kShort];
@@ -167,7 +166,7 @@ __device__ __forceinline__ void split_short_cols(
 }
 
 // Up to four matrices, each with its range of blocks.
-enum Form : int { kRowsWarp, kRowsBlock, kCols16, kCols8 };
+enum Form : int { kRowsWarp, kRowsBlock, kCols16, kCols4 };
 struct SplitJobs {
     struct Job {
         Source src;
@@ -188,13 +187,11 @@ __global__ void __launch_bounds__(256, 2) split_short_cols_kernel(const __grid_c
     while (j + 1 < jobs.count && (int64_t)blockIdx.x >= jobs.job[j + 1].first)
         ++j;
     const SplitJobs::Job &x = jobs.job[j];
-    if (x.form == kCols16)
-        split_short_cols<4>(x.src, x.width, x.row_factor, x.to, x.inverse, blockIdx.x - x.first, many);
-    else
-        split_short_cols<2>(x.src, x.width, x.row_factor, x.to, x.inverse, blockIdx.x - x.first, many);
+    split_short_cols(x.src, x.width, x.row_factor, x.to, x.inverse, blockIdx.x - x.first, many);
 }
 
-// All of a small product's operands: a warp to a row, a block to 16 columns, read twice (the second time from L1).  In registers as above
+// All of a small product's operands: a warp to a row, a block to 16 columns (4 of more than 256 rows, whose turns would take longer than the
+// launch: 1569 x 247 23 us), read twice (the second time from L1).  In registers as above
 // they are read once, but the code is ten times as long, and fetching it is what a launch of a few blocks then waits for (8 to 10 against
 // 18 to 24 us with cold caches).
 __global__ void __launch_bounds__(256) split_small_kernel(const __grid_constant__ SplitJobs jobs) {
@@ -226,22 +223,21 @@ __global__ void __launch_bounds__(256) split_small_kernel(const __grid_constant_
         if (lane == 0)
             x.inverse[row] = line_inverse(mx);
     } else {
-        const int t = threadIdx.x, quad = t & 3;
-        const int64_t c = block * 16 + quad * 4;
+        const int t = threadIdx.x, lanes = x.form == kCols16 ? 4 : 1, quad = t & (lanes - 1), step = 256 / lanes, first = t / lanes;
+        const int64_t c = (block * lanes + quad) * 4;
         uint32_t mx[4] = {0, 0, 0, 0};
         if (c < x.width)
 #pragma unroll 4
-            for (int64_t r = t >> 2; r < src.rows; r += 64) {
+            for (int64_t r = first; r < src.rows; r += step) {
                 const float4 q = factored(src.quad(r, c), x.row_factor, r);
                 mx[0] = max(mx[0], finite_bits(q.x)), mx[1] = max(mx[1], finite_bits(q.y));
                 mx[2] = max(mx[2], finite_bits(q.z)), mx[3] = max(mx[3], finite_bits(q.w));
             }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-#pragma unroll
-            for (int o = 16; o >= 4; o >>= 1)
+            for (int o = 16; o >= lanes; o >>= 1)
                 mx[q] = max(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], o));
-            if (lane < 4)
+            if (lane < lanes)
                 many[warp][quad * 4 + q] = mx[q];
         }
         __syncthreads();
@@ -254,11 +250,11 @@ __global__ void __launch_bounds__(256) split_small_kernel(const __grid_constant_
             return;
         const float s0 = line_scale(mx[0]), s1 = line_scale(mx[1]), s2 = line_scale(mx[2]), s3 = line_scale(mx[3]);
 #pragma unroll 4
-        for (int64_t r = t >> 2; r < src.rows; r += 64) {
+        for (int64_t r = first; r < src.rows; r += step) {
             const float4 q = factored(src.quad(r, c), x.row_factor, r);
             put_quad(x.to, r * x.to.ld + c, q.x * s0, q.y * s1, q.z * s2, q.w * s3);
         }
-        if (t < 4)
+        if (t < lanes)
             *reinterpret_cast<float4 *>(x.inverse + c) = make_float4(line_inverse(mx[0]), line_inverse(mx[1]), line_inverse(mx[2]), line_inverse(mx[3]));
     }
 }
@@ -390,46 +386,44 @@ __global__ void __launch_bounds__(256) split_cols_kernel(
     }
 }
 
-// out = the slices' sums, in order (and what out held); columns from `second` on to out2.  V values to a thread: with a division for each
-// value and one value to a thread 8192 x 2048 of two slices took 66 us, so 29.
-template <int V>
+// out = the slices' sums, in order (and what out held); columns from `second` (a multiple of eight) on to out2.  The slices' rows are whole float4,
+// what out's may not be: with a division for each value and one value to a thread 8192 x 2048 of two slices took 66 us, so 29.
 __global__ void __launch_bounds__(256) join_slices_kernel(
-    const float *__restrict__ partial, int slices, int64_t m, int64_t n, float *__restrict__ out, float *__restrict__ out2, int64_t out_cols,
-    int64_t stride, int64_t second, int add, const uint32_t *__restrict__ flags) {
+    const float *__restrict__ partial, int slices, int64_t m, int64_t n, int64_t pitch, float *__restrict__ out, float *__restrict__ out2,
+    int64_t out_cols, int64_t stride, int64_t second, int shift, int vec, int add, const uint32_t *__restrict__ flags) {
     griddep_wait();
     griddep_launch_dependents();
     if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the slices were not computed
         return;
-    const int64_t total = m * n, c0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    const int64_t total = m * pitch, c0 = (((int64_t)blockIdx.x << shift) + (threadIdx.x & ((1 << shift) - 1))) * 4;
     if (c0 >= n)
         return;
-    for (int64_t r = blockIdx.y; r < m; r += gridDim.y) {
-        const float *src = partial + r * n + c0;
+    const int rows = 256 >> shift; // at a time
+    for (int64_t r = (int64_t)blockIdx.y * rows + (threadIdx.x >> shift); r < m; r += (int64_t)gridDim.y * rows) {
+        const float *src = partial + r * pitch + c0;
         float4 s         = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
         for (int z = 0; z < slices; ++z) {
-            if (V == 4) {
-                const float4 q = __ldcs(reinterpret_cast<const float4 *>(src + z * total));
-                s = make_float4(__fadd_rn(s.x, q.x), __fadd_rn(s.y, q.y), __fadd_rn(s.z, q.z), __fadd_rn(s.w, q.w));
-            } else {
-                s.x = __fadd_rn(s.x, __ldcs(src + z * total));
-            }
+            const float4 q = __ldcs(reinterpret_cast<const float4 *>(src + z * total));
+            s = make_float4(__fadd_rn(s.x, q.x), __fadd_rn(s.y, q.y), __fadd_rn(s.z, q.z), __fadd_rn(s.w, q.w));
         }
         int64_t c = c0;
         float *to = out;
         if (out2 && c >= second)
             to = out2, c -= second;
-        if (c >= out_cols)
-            continue;
         to += r * stride + c;
-        if (V == 4) {
+        if (vec && c + 3 < out_cols) {
             if (add) {
                 const float4 o = *reinterpret_cast<const float4 *>(to);
                 s = make_float4(__fadd_rn(o.x, s.x), __fadd_rn(o.y, s.y), __fadd_rn(o.z, s.z), __fadd_rn(o.w, s.w));
             }
             *reinterpret_cast<float4 *>(to) = s;
         } else {
-            *to = add ? __fadd_rn(*to, s.x) : s.x;
+            const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < out_cols)
+                    to[q] = add ? __fadd_rn(to[q], v[q]) : v[q];
         }
     }
 }
@@ -473,7 +467,7 @@ static ct_status split_long_cols(DeviceState *st, const Split &x) {
 
 ct_status split(DeviceState *st, const Split *what, int count) {
     auto blocks_of = [](int form, int64_t rows, int64_t width) {
-        return form == kRowsWarp ? (rows + 7) / 8 : form == kRowsBlock ? rows : form == kCols16 ? (width + 15) / 16 : (width + 7) / 8;
+        return form == kRowsWarp ? (rows + 7) / 8 : form == kRowsBlock ? rows : form == kCols16 ? (width + 15) / 16 : (width + 3) / 4;
     };
     auto add = [&](SplitJobs &jobs, int64_t &blocks, const Split &x, const float *in, const float *in2, int64_t at, int form) {
         const Source src    = source_of(in, in2, x.rows, x.cols, x.col_factor);
@@ -500,7 +494,7 @@ ct_status split(DeviceState *st, const Split *what, int count) {
         int64_t blocks = 0;
         for (int i = 0; i < count; ++i)
             if (what[i].by_column)
-                add_cols(jobs, blocks, what[i], kCols16);
+                add_cols(jobs, blocks, what[i], what[i].rows > 256 ? kCols4 : kCols16);
             else
                 add(jobs, blocks, what[i], what[i].in, what[i].in2, 0, kRowsWarp);
         if (blocks > 0) {
@@ -515,8 +509,8 @@ ct_status split(DeviceState *st, const Split *what, int count) {
         const Split &x = what[i];
         if (!x.by_column)
             add(rows, row_blocks, x, x.in, x.in2, 0, kRowsBlock);
-        else if (x.rows <= kShort * 64 || (x.rows <= kShort * 128 && x.rows * x.cols <= 4 * kFewValues))
-            add_cols(cols, col_blocks, x, x.rows <= kShort * 64 ? kCols16 : kCols8);
+        else if (x.rows <= kShort * 64)
+            add_cols(cols, col_blocks, x, kCols16);
         else
             CT_TRY(split_long_cols(st, x));
     }
@@ -584,19 +578,23 @@ ct_status product(
     Store::Params e{};
     e.out = to.out, e.out2 = to.out2, e.n = to.cols, e.stride = to.stride, e.second = to.second, e.add = to.add ? 1 : 0;
     e.vec = (to.stride & 3) == 0 && whole(to.out) && whole(to.out2) ? 1 : 0;
+    const int64_t pitch = (n + 3) / 4 * 4;
     Scratch partial;
     if (splits > 1) {
-        CT_TRY(partial.get((size_t)splits * m * n * 4));
-        e.out = partial.as<float>(), e.out2 = nullptr, e.n = e.stride = n, e.second = 0, e.slice = m * n, e.add = 0;
-        e.vec = (n & 3) == 0 ? 1 : 0;
+        CT_TRY(partial.get((size_t)splits * m * pitch * 4));
+        e.out = partial.as<float>(), e.out2 = nullptr, e.n = e.stride = pitch, e.second = 0, e.slice = m * pitch, e.add = 0;
+        e.vec = 1;
     }
     CT_TRY(pair ? (launch_store<256, 2>(st, a, a_mn, b, b_mn, p, e, splits)) : (launch_store<128, 1>(st, a, a_mn, b, b_mn, p, e, splits)));
     if (splits > 1) {
-        const bool quads = (n & 3) == 0 && (to.cols & 3) == 0 && (to.stride & 3) == 0 && whole(to.out) && whole(to.out2); // second is a multiple of eight
-        const int64_t strips = quads ? (n + 1023) / 1024 : (n + 255) / 256;
-        const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(m, 65535), (int64_t)st->sm_count * 16 / strips)));
-        CT_CUDA(launch_dependent(quads ? join_slices_kernel<4> : join_slices_kernel<1>, grid, dim3(256), 0, stream(), partial.as<const float>(), splits, m,
-                                 n, to.out, to.out2, to.cols, to.stride, to.second, to.add ? 1 : 0, (const uint32_t *)st->flags_dev));
+        const int vec = (to.stride & 3) == 0 && whole(to.out) && whole(to.out2) ? 1 : 0;
+        int shift = 3; // threads to a row, up to the block's 256
+        while (shift < 8 && (4 << shift) < n)
+            ++shift;
+        const int64_t strips = (n + (4 << shift) - 1) / (4 << shift), turns = (m + (256 >> shift) - 1) / (256 >> shift);
+        const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(turns, 65535), (int64_t)st->sm_count * 16 / strips)));
+        CT_CUDA(launch_dependent(join_slices_kernel, grid, dim3(256), 0, stream(), partial.as<const float>(), splits, m, n, pitch, to.out, to.out2, to.cols,
+                                 to.stride, to.second, shift, vec, to.add ? 1 : 0, (const uint32_t *)st->flags_dev));
         CT_LAUNCH_CHECK("join_slices");
     }
     return CT_OK;
