@@ -412,8 +412,8 @@ ct_status ce_grad_fused(
     const bool few = m <= kStreamRows;
     // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
-    const int64_t count = (n + most - 1) / most;
-    const int64_t piece = std::min<int64_t>(n, ((n + count - 1) / count + 255) / 256 * 256), ld = padded(piece);
+    const int64_t pieces = (n + most - 1) / most;
+    const int64_t piece = std::min<int64_t>(n, ((n + pieces - 1) / pieces + 255) / 256 * 256), ld = padded(piece);
     Parts parts;
     // The weights' planes for dx have a scale per row; with those folded into x they are the logits' as well, which saves a pre-pass over the
     // weights (1000 x 512 x 50257: 639 us, so 575) and keeps what features of different sizes meet.
@@ -461,16 +461,20 @@ ct_status ce_grad_fused(
             CT_TRY(pair ? (launch<Slopes, 256, 2, false, true>(st, px, right, p, e, 1, "cross_entropy_grad"))
                         : (launch<Slopes, 128, 1, false, true>(st, px, right, p, e, 1, "cross_entropy_grad")));
         }
+        Wanted wanted[2];
+        int count = 0;
         if (dx) {
             Result r{dx};
             r.cols = r.stride = k, r.add = c > 0;
-            CT_TRY(product(st, pd, false, columns_of(pw, c, cols), false, m, k, weight, s.as<float>(wi), r));
+            wanted[count++] = {pd, columns_of(pw, c, cols), false, m, k, weight, s.as<float>(wi), r};
         }
         if (dw) {
             Result r{dw + c};
             r.cols = cols, r.stride = n;
-            CT_TRY(product(st, py, true, pd, true, k, cols, s.as<float>(yi), nullptr, r));
+            wanted[count++] = {py, pd, true, k, cols, s.as<float>(yi), nullptr, r};
         }
+        if (count)
+            CT_TRY(products(st, wanted, count));
         if (dbias)
             CT_TRY(column_sums(st, pd, weight, dbias + c));
     }

@@ -388,32 +388,45 @@ __global__ void __launch_bounds__(256) split_cols_kernel(
 
 // out = the slices' sums, in order (and what out held); columns from `second` (a multiple of eight) on to out2.  The slices' rows are whole float4,
 // what out's may not be: with a division for each value and one value to a thread 8192 x 2048 of two slices took 66 us, so 29.
-__global__ void __launch_bounds__(256) join_slices_kernel(
-    const float *__restrict__ partial, int slices, int64_t m, int64_t n, int64_t pitch, float *__restrict__ out, float *__restrict__ out2,
-    int64_t out_cols, int64_t stride, int64_t second, int shift, int vec, int add, const uint32_t *__restrict__ flags) {
+struct Joins {
+    struct Job {
+        const float *partial;
+        int slices, shift; // 2^shift threads to a row
+        int64_t m, n, pitch, strips, first; // blocks: strips to each turn of the rows; the first block
+        float *out, *out2;
+        int64_t cols, stride, second;
+        int vec, add;
+    } job[2];
+    int64_t blocks; // of both
+    int count;
+};
+__global__ void __launch_bounds__(256) join_slices_kernel(const __grid_constant__ Joins joins, const uint32_t *__restrict__ flags) {
     griddep_wait();
     griddep_launch_dependents();
     if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0) // the slices were not computed
         return;
-    const int64_t total = m * pitch, c0 = (((int64_t)blockIdx.x << shift) + (threadIdx.x & ((1 << shift) - 1))) * 4;
-    if (c0 >= n)
+    const int which     = joins.count > 1 && (int64_t)blockIdx.x >= joins.job[1].first ? 1 : 0;
+    const Joins::Job &x = joins.job[which];
+    const int64_t block = blockIdx.x - x.first, turns = ((which + 1 < joins.count ? joins.job[1].first : joins.blocks) - x.first) / x.strips;
+    const int64_t total = x.m * x.pitch, c0 = ((block % x.strips << x.shift) + (threadIdx.x & ((1 << x.shift) - 1))) * 4;
+    if (c0 >= x.n)
         return;
-    const int rows = 256 >> shift; // at a time
-    for (int64_t r = (int64_t)blockIdx.y * rows + (threadIdx.x >> shift); r < m; r += (int64_t)gridDim.y * rows) {
-        const float *src = partial + r * pitch + c0;
+    const int rows = 256 >> x.shift; // at a time
+    for (int64_t r = block / x.strips * rows + (threadIdx.x >> x.shift); r < x.m; r += turns * rows) {
+        const float *src = x.partial + r * x.pitch + c0;
         float4 s         = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-        for (int z = 0; z < slices; ++z) {
+        for (int z = 0; z < x.slices; ++z) {
             const float4 q = __ldcs(reinterpret_cast<const float4 *>(src + z * total));
             s = make_float4(__fadd_rn(s.x, q.x), __fadd_rn(s.y, q.y), __fadd_rn(s.z, q.z), __fadd_rn(s.w, q.w));
         }
         int64_t c = c0;
-        float *to = out;
-        if (out2 && c >= second)
-            to = out2, c -= second;
-        to += r * stride + c;
-        if (vec && c + 3 < out_cols) {
-            if (add) {
+        float *to = x.out;
+        if (x.out2 && c >= x.second)
+            to = x.out2, c -= x.second;
+        to += r * x.stride + c;
+        if (x.vec && c + 3 < x.cols) {
+            if (x.add) {
                 const float4 o = *reinterpret_cast<const float4 *>(to);
                 s = make_float4(__fadd_rn(o.x, s.x), __fadd_rn(o.y, s.y), __fadd_rn(o.z, s.z), __fadd_rn(o.w, s.w));
             }
@@ -422,8 +435,8 @@ __global__ void __launch_bounds__(256) join_slices_kernel(
             const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (c + q < out_cols)
-                    to[q] = add ? __fadd_rn(to[q], v[q]) : v[q];
+                if (c + q < x.cols)
+                    to[q] = x.add ? __fadd_rn(to[q], v[q]) : v[q];
         }
     }
 }
@@ -433,14 +446,14 @@ Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols, 
     return Source{in, in2, col_factor, rows, cols, padded(cols), vec ? 1 : 0};
 }
 
-template <int BN, int CG>
-ct_status launch_store(
-    DeviceState *st, const Planes &a, bool a_mn, const Planes &b, bool b_mn, const Product &p, const Store::Params &e, int splits) {
-    if (a_mn)
-        return b_mn ? launch<Store, BN, CG, true, true>(st, a, b, p, e, splits, "fused_product")
-                    : launch<Store, BN, CG, true, false>(st, a, b, p, e, splits, "fused_product");
-    return b_mn ? launch<Store, BN, CG, false, true>(st, a, b, p, e, splits, "fused_product")
-                : launch<Store, BN, CG, false, false>(st, a, b, p, e, splits, "fused_product");
+// Two small products side by side: the K-major one has the first blocks.
+__global__ void __launch_bounds__(kThreads, 1) two_products_kernel(
+    const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Store::Params e, const __grid_constant__ Maps maps_mn,
+    const __grid_constant__ Product p_mn, const __grid_constant__ Store::Params e_mn) {
+    if ((int)blockIdx.x < p.total)
+        product_body<Store, 128, 1, false, false>(maps, p, e, (int)blockIdx.x, p.total);
+    else
+        product_body<Store, 128, 1, true, true>(maps_mn, p_mn, e_mn, (int)blockIdx.x - p.total, p_mn.total);
 }
 
 } // namespace
@@ -549,53 +562,127 @@ ct_status split(DeviceState *st, const Split *what, int count) {
     return CT_OK;
 }
 
-ct_status product(
-    DeviceState *st, const Planes &a, bool a_mn, const Planes &b, bool b_mn, int64_t m, int64_t n, const float *row_scale, const float *col_scale,
-    const Result &to) {
-    const int64_t stages = ((a_mn ? a.rows : a.cols) + 63) / 64;
-    // Tile and slices by what they take, in microseconds: a stage of a pair's 256 x 256 tile ~ 0.95, of a single CTA's 128 x 128 ~ 0.6;
-    // filling and draining a tile as much as four stages; the slices' sums written, read and a launch.
-    bool pair = false;
+namespace {
+
+// Tile and slices of a product by what they take, in microseconds: a stage of a pair's 256 x 256 tile ~ 0.95, of a single CTA's 128 x 128 ~ 0.6;
+// filling and draining a tile as much as four stages; the slices' sums written, read and a launch.
+struct Plan {
+    int64_t stages;
+    bool pair  = false;
     int splits = 1;
-    double best = 1e300;
+    double cost = 1e300;
+};
+int64_t stages_of(const Wanted &x) { return ((x.mn ? x.a.rows : x.a.cols) + 63) / 64; }
+int64_t tiles_of(const Wanted &x, int64_t side) { return ((x.m + side - 1) / side) * ((x.n + side - 1) / side); }
+double cost_of(const Wanted &x, int splits, int64_t waves, bool pair) {
+    return (double)waves * (double)((stages_of(x) + splits - 1) / splits + 4) * (pair ? 0.95 : 0.6);
+}
+double join_cost(const Wanted &x, int splits) { return splits > 1 ? 3.0 + 0.1 * splits + (double)(x.m * x.n) * (splits + 1) * 4 / 5e6 : 0.0; }
+bool may_split(const Wanted &x, int splits) { return splits == 1 || stages_of(x) >= 4 * splits; }
+int whole_slices(const Wanted &x, int splits) { // no empty slice
+    const int64_t stages = stages_of(x), each = (stages + splits - 1) / splits;
+    return splits > 1 ? (int)((stages + each - 1) / each) : 1;
+}
+Plan plan_of(const DeviceState *st, const Wanted &x) {
+    Plan best;
     for (int kind = 0; kind < 2; ++kind) {
-        const int64_t side = kind ? 256 : 128, units = kind ? st->sm_count / 2 : st->sm_count;
-        const int64_t tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
-        for (int s = 1; s <= 32 && (s == 1 || stages >= 4 * s); ++s) {
-            const double waves = (double)((tiles * s + units - 1) / units);
-            const double cost  = waves * (double)((stages + s - 1) / s + 4) * (kind ? 0.95 : 0.6) + (s > 1 ? 3.0 + 0.1 * s + (double)(m * n) * (s + 1) * 4 / 5e6 : 0.0);
-            if (cost < best)
-                best = cost, pair = kind != 0, splits = s;
+        const int64_t units = kind ? st->sm_count / 2 : st->sm_count, tiles = tiles_of(x, kind ? 256 : 128);
+        for (int s = 1; s <= 32 && may_split(x, s); ++s) {
+            const double cost = cost_of(x, s, (tiles * s + units - 1) / units, kind != 0) + join_cost(x, s);
+            if (cost < best.cost)
+                best.cost = cost, best.pair = kind != 0, best.splits = s;
         }
     }
-    if (splits > 1) { // no empty slice
-        const int64_t each = (stages + splits - 1) / splits;
-        splits             = (int)((stages + each - 1) / each);
+    best.splits = whole_slices(x, best.splits);
+    return best;
+}
+// Both at once, in one wave of single CTAs, and their joins: gated gradient of 404 x 322 x 177 30 us one after the other, so 19, of
+// 1315 x 118 x 773 41 and 32.
+bool plan_both(const DeviceState *st, const Wanted (&x)[2], Plan (&plan)[2]) {
+    const int64_t tiles[2] = {tiles_of(x[0], 128), tiles_of(x[1], 128)};
+    double best            = plan[0].cost + plan[1].cost + 3.0; // a launch
+    bool both              = false;
+    for (int s = 1; s <= 32 && may_split(x[0], s); ++s) {
+        int t = (int)std::min<int64_t>(32, (st->sm_count - tiles[0] * s) / tiles[1]);
+        while (t > 1 && !may_split(x[1], t))
+            --t;
+        if (t < 1)
+            break;
+        const double cost = std::max(cost_of(x[0], s, 1, false), cost_of(x[1], t, 1, false)) + std::max(join_cost(x[0], s), join_cost(x[1], t));
+        if (cost < best)
+            best = cost, both = true, plan[0].splits = s, plan[1].splits = t;
     }
-    Product p{};
-    p.m = m, p.n = n, p.row_scale = row_scale, p.col_scale = col_scale;
-    auto whole = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-    Store::Params e{};
-    e.out = to.out, e.out2 = to.out2, e.n = to.cols, e.stride = to.stride, e.second = to.second, e.add = to.add ? 1 : 0;
-    e.vec = (to.stride & 3) == 0 && whole(to.out) && whole(to.out2) ? 1 : 0;
-    const int64_t pitch = (n + 3) / 4 * 4;
-    Scratch partial;
-    if (splits > 1) {
-        CT_TRY(partial.get((size_t)splits * m * pitch * 4));
-        e.out = partial.as<float>(), e.out2 = nullptr, e.n = e.stride = pitch, e.second = 0, e.slice = m * pitch, e.add = 0;
-        e.vec = 1;
+    if (both)
+        for (int i = 0; i < 2; ++i)
+            plan[i].pair = false, plan[i].splits = whole_slices(x[i], plan[i].splits);
+    return both;
+}
+
+bool whole(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+} // namespace
+
+ct_status products(DeviceState *st, const Wanted *what, int count) {
+    const char *name = "fused_product";
+    Plan plan[2]     = {plan_of(st, what[0]), {}};
+    bool both        = false;
+    if (count == 2) {
+        const Wanted pair[2] = {what[0], what[1]};
+        plan[1]              = plan_of(st, what[1]);
+        both                 = plan_both(st, pair, plan);
     }
-    CT_TRY(pair ? (launch_store<256, 2>(st, a, a_mn, b, b_mn, p, e, splits)) : (launch_store<128, 1>(st, a, a_mn, b, b_mn, p, e, splits)));
-    if (splits > 1) {
+    Scratch partial[2];
+    Product p[2]{};
+    Store::Params e[2]{};
+    Joins joins{};
+    auto join = [&]() -> ct_status {
+        if (joins.count) {
+            CT_CUDA(launch_dependent(join_slices_kernel, dim3((unsigned)joins.blocks), dim3(256), 0, stream(), joins, (const uint32_t *)st->flags_dev));
+            CT_LAUNCH_CHECK("join_slices");
+        }
+        joins = Joins{};
+        return CT_OK;
+    };
+    for (int i = 0; i < count; ++i) {
+        const Wanted &x  = what[i];
+        const Result &to = x.to;
+        p[i].m = x.m, p[i].n = x.n, p[i].row_scale = x.row_scale, p[i].col_scale = x.col_scale;
         const int vec = (to.stride & 3) == 0 && whole(to.out) && whole(to.out2) ? 1 : 0;
-        int shift = 3; // threads to a row, up to the block's 256
-        while (shift < 8 && (4 << shift) < n)
-            ++shift;
-        const int64_t strips = (n + (4 << shift) - 1) / (4 << shift), turns = (m + (256 >> shift) - 1) / (256 >> shift);
-        const dim3 grid((unsigned)strips, (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(turns, 65535), (int64_t)st->sm_count * 16 / strips)));
-        CT_CUDA(launch_dependent(join_slices_kernel, grid, dim3(256), 0, stream(), partial.as<const float>(), splits, m, n, pitch, to.out, to.out2, to.cols,
-                                 to.stride, to.second, shift, vec, to.add ? 1 : 0, (const uint32_t *)st->flags_dev));
-        CT_LAUNCH_CHECK("join_slices");
+        e[i].out = to.out, e[i].out2 = to.out2, e[i].n = to.cols, e[i].stride = to.stride, e[i].second = to.second, e[i].add = to.add ? 1 : 0;
+        e[i].vec = vec;
+        if (plan[i].splits > 1) {
+            const int64_t pitch = (x.n + 3) / 4 * 4;
+            CT_TRY(partial[i].get((size_t)plan[i].splits * x.m * pitch * 4));
+            e[i].out = partial[i].as<float>(), e[i].out2 = nullptr, e[i].n = e[i].stride = pitch, e[i].second = 0, e[i].slice = x.m * pitch, e[i].add = 0;
+            e[i].vec = 1;
+            int shift = 3;
+            while (shift < 8 && (4 << shift) < x.n)
+                ++shift;
+            const int64_t strips = (x.n + (4 << shift) - 1) / (4 << shift), turns = (x.m + (256 >> shift) - 1) / (256 >> shift);
+            joins.job[joins.count++] = Joins::Job{partial[i].as<const float>(), plan[i].splits, shift, x.m, x.n, pitch, strips, joins.blocks, to.out,
+                                                  to.out2, to.cols, to.stride, to.second, vec, to.add ? 1 : 0};
+            joins.blocks += strips * std::max<int64_t>(1, std::min<int64_t>(turns, (int64_t)st->sm_count * 16 / strips));
+        }
+        if (both)
+            continue;
+        if (x.mn)
+            CT_TRY(plan[i].pair ? (launch<Store, 256, 2, true, true>(st, x.a, x.b, p[i], e[i], plan[i].splits, name))
+                                : (launch<Store, 128, 1, true, true>(st, x.a, x.b, p[i], e[i], plan[i].splits, name)));
+        else
+            CT_TRY(plan[i].pair ? (launch<Store, 256, 2, false, false>(st, x.a, x.b, p[i], e[i], plan[i].splits, name))
+                                : (launch<Store, 128, 1, false, false>(st, x.a, x.b, p[i], e[i], plan[i].splits, name)));
+        CT_TRY(join()); // while the slices are in L2
+    }
+    if (both) {
+        Maps maps[2];
+        CT_TRY((prepare<Store, 128, 1, false, false>(st, what[0].a, what[0].b, plan[0].splits, maps[0], p[0], name)));
+        CT_TRY((prepare<Store, 128, 1, true, true>(st, what[1].a, what[1].b, plan[1].splits, maps[1], p[1], name)));
+        static bool set_dev[16] = {};
+        CT_TRY(allow_shared(st, two_products_kernel, set_dev));
+        CT_CUDA(launch_dependent(two_products_kernel, dim3((unsigned)(p[0].total + p[1].total)), dim3(kThreads), (size_t)kSmem, stream(), maps[0], p[0], e[0],
+                                 maps[1], p[1], e[1]));
+        CT_LAUNCH_CHECK(name);
+        CT_TRY(join());
     }
     return CT_OK;
 }

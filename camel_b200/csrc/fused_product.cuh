@@ -119,14 +119,14 @@ __device__ __forceinline__ void tile_of(const Product &p, int tile, int &tm, int
 // EPI: kTwin - the tile's columns are half of one matrix and half of another, and a thread has the same columns of both;
 // Params; store(p, e, acc, row0, lane, col0, z, part, stage): acc holds unscaled sums of row row0 + lane, columns col0 .. (twin: COLS / 2
 // columns from col0 of the first matrix, then those of the second), the part-th quarter of the tile's; stage is the warp's 2 KB.
+// block of `blocks`: which CTA of the product's this one is.
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(kThreads, 1)
-    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ typename EPI::Params e) {
+__device__ __forceinline__ void product_body(const Maps &maps, const Product &p, const typename EPI::Params &e, int block, int blocks) {
     static_assert(BN / CG == 128, "128 columns of B to a CTA");
     constexpr int SETS = 512 / (2 * BN), COLS = BN / 4;
     const int rank   = CG == 2 ? (int)cluster_rank() : 0;
-    const int first  = (int)blockIdx.x / CG;
-    const int stride = (int)gridDim.x / CG;
+    const int first  = block / CG;
+    const int stride = blocks / CG;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[kStages], bar_empty[kStages];
     __shared__ uint64_t bar_acc_full[2 * SETS], bar_acc_empty[2 * SETS]; // [set * 2 + which]: 0 leading accumulator, 1 cross products
@@ -409,6 +409,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && !failed && *abort_flag)
         atomicExch(p.flags + FLAG_TIMEOUT, 1u + (uint32_t)blockIdx.x);
 }
+template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ typename EPI::Params e) {
+    product_body<EPI, BN, CG, A_MN, B_MN>(maps, p, e, (int)blockIdx.x, (int)gridDim.x);
+}
 
 // The inverse scales of columns col0 + 4 j .. + 3: one address for the warp.  Arrays of scales reach to the end of the last tile.
 __device__ __forceinline__ float4 scales4(const float *scale, int64_t col) {
@@ -509,11 +514,10 @@ inline ct_status operand_map(CUtensorMap *map, const __half *base, const Planes 
     return encode_tiled_map_f16(map, base, 2, dims, strides, box, 128);
 }
 
-// Launches the product of prepared planes; a.rows (K-major) or a.cols (MN-major) is m, b's likewise n (twin: of one matrix); k the
-// other index of both.  `splits` slices of k.
+// The product of prepared planes; a.rows (K-major) or a.cols (MN-major) is m, b's likewise n (twin: of one matrix); k the other index of
+// both.  `splits` slices of k.
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
-ct_status launch(DeviceState *st, const Planes &a, const Planes &b, Product p, const typename EPI::Params &e, int splits, const char *name) {
-    Maps maps;
+ct_status prepare(DeviceState *st, const Planes &a, const Planes &b, int splits, Maps &maps, Product &p, const char *name) {
     CT_TRY(operand_map(&maps.a_hi, a.hi, a, A_MN));
     CT_TRY(operand_map(&maps.a_lo, a.lo, a, A_MN));
     CT_TRY(operand_map(&maps.b_hi, b.hi, b, B_MN));
@@ -529,16 +533,26 @@ ct_status launch(DeviceState *st, const Planes &a, const Planes &b, Product p, c
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * splits;
     if (tiles > 0x3fffffff)
         return fail(CT_ERR_TOO_LARGE, "%s: too many tiles", name);
-    p.total = (int)tiles;
-    auto kernel = product_kernel<EPI, BN, CG, A_MN, B_MN>;
-    static bool attr_set_dev[16] = {}; // the attribute belongs to a device's context
-    if (!attr_set_dev[st->device & 15]) {
+    p.total       = (int)tiles;
+    p.chunk_first = tiles <= st->sm_count / CG ? kChunk : kChunkFirst;
+    return CT_OK;
+}
+template <typename K> ct_status allow_shared(const DeviceState *st, K kernel, bool (&set_dev)[16]) { // the attribute belongs to a device's context
+    if (!set_dev[st->device & 15]) {
         CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        attr_set_dev[st->device & 15] = true;
+        set_dev[st->device & 15] = true;
     }
-    const int64_t units = st->sm_count / CG;
-    p.chunk_first       = tiles <= units ? kChunk : kChunkFirst;
-    CT_CUDA(launch_dependent_cluster(kernel, CG, dim3((unsigned)(std::min(tiles, units) * CG)), dim3(kThreads), (size_t)kSmem, stream(), maps, p, e));
+    return CT_OK;
+}
+template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
+ct_status launch(DeviceState *st, const Planes &a, const Planes &b, Product p, const typename EPI::Params &e, int splits, const char *name) {
+    Maps maps;
+    CT_TRY((prepare<EPI, BN, CG, A_MN, B_MN>(st, a, b, splits, maps, p, name)));
+    auto kernel = product_kernel<EPI, BN, CG, A_MN, B_MN>;
+    static bool set_dev[16] = {};
+    CT_TRY(allow_shared(st, kernel, set_dev));
+    const int units = st->sm_count / CG;
+    CT_CUDA(launch_dependent_cluster(kernel, CG, dim3((unsigned)(std::min(p.total, units) * CG)), dim3(kThreads), (size_t)kSmem, stream(), maps, p, e));
     CT_LAUNCH_CHECK(name);
     return CT_OK;
 }
@@ -589,9 +603,16 @@ struct Result {
     int64_t cols, stride, second = 0;
     bool add = false;
 };
-ct_status product(
-    DeviceState *st, const Planes &a, bool a_mn, const Planes &b, bool b_mn, int64_t m, int64_t n, const float *row_scale, const float *col_scale,
-    const Result &to);
+// A product to be: a [m][k] and b [n][k] K-major, or both MN-major.
+struct Wanted {
+    Planes a, b;
+    bool mn;
+    int64_t m, n;
+    const float *row_scale, *col_scale;
+    Result to;
+};
+// One, or a K-major and an MN-major one.
+ct_status products(DeviceState *st, const Wanted *what, int count);
 // out[c] = sum over the rows of row_weight[r] * planes[r][c].
 ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight, float *out);
 // first[c] = sum over parts of partial[part][c] for c < n, second[c] of partial[part][n + c] for n + c < width; either may be null.

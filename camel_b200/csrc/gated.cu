@@ -425,21 +425,22 @@ ct_status gated_grad_fused(
     if (weights)
         operands[count++] = {x, nullptr, m, k, true, s.as<float>(di), px, s.as<float>(xi)};
     CT_TRY(split(st, operands, count));
+    Wanted wanted[2];
+    count = 0;
     if (back) {
         Result r{dx};
         r.cols = r.stride = k;
-        CT_TRY(product(st, pd, false, pw, false, m, k, s.as<float>(di), s.as<float>(wi), r));
+        wanted[count++] = {pd, pw, false, m, k, s.as<float>(di), s.as<float>(wi), r};
     }
     if (weights) {
-        Result r{dw_gate};
+        Result r{dw_gate ? dw_gate : dw_up};
         r.cols = r.stride = n;
         if (dw_gate && dw_up)
             r.out2 = dw_up, r.second = ln;
         const Planes right = dw_gate && dw_up ? pd : columns_of(pd, dw_gate ? 0 : ln, n);
-        r.out              = dw_gate ? dw_gate : dw_up;
-        CT_TRY(product(st, px, true, right, true, k, dw_gate && dw_up ? 2 * ln : n, s.as<float>(xi), nullptr, r));
+        wanted[count++]    = {px, right, true, k, dw_gate && dw_up ? 2 * ln : n, s.as<float>(xi), nullptr, r};
     }
-    return CT_OK;
+    return count ? products(st, wanted, count) : CT_OK;
 }
 
 // Few rows: dg or du of what was kept.
