@@ -626,34 +626,38 @@ ct_status few_logits(DeviceState *st, const float *x, const float *w, const floa
     return ct_dense(x, w, bias, m, k, n, CT_ACT_NONE, z, nullptr);
 }
 
-// The whole gradient of up to 16 classes and 1024 columns of x in one reading of x, float32: 16 rows of x in shared memory at a time, the
-// next ones on their way.  Logits: a warp has four rows and a quarter of the columns of each 128, and its 4 N sums meet by halves; d: a
-// thread to each; then a thread has two columns of dx, dw and w in registers and walks the rows.
-// Bound by issue, some 1000 instructions a row (two values an FMA): 60000 x 785 x 10 takes 170 us, at the copy rate it would be 58; as five
-// kernels, each with its own reading of x or of d, it took 212.  dw's sums are chains of a CTA's rows (m / 148), joined in 64 bits.
-constexpr int kOneRows = 16, kOneThreads = 512, kOneColumns = 2 * kOneThreads;
+// The whole gradient of up to 16 classes and 1024 columns of x in one reading of x, float32: a row of x for each warp of the block (8 or 16) in
+// shared memory at a time, the next ones on their way.  Logits: a warp has four rows and a quarter of the columns of each 128, and its 4 N sums
+// meet by halves; d: a thread to each; then half of the warps have the columns of dw as sums in registers, the other half those of w, for
+// dx, and walk the rows.
+// Bound by issue (half of the slots are busy, the FMAs of two values take a third) and by the phases' barriers.  60000 x 785 x 10: at the copy rate
+// 58 us; as five kernels, each with its own reading of x or of d, 212; with columns of both w and dw in every thread 173; so 160.  dw's sums are
+// chains of a block's rows, joined in 64 bits.
+constexpr int kOneColumns = 1024;
+// Between the rows of w in shared memory: an odd number of float4, so that eight of them lie in different banks (16 classes: 364 us at 16).
+template <int P> constexpr int kOnePitch = (P / 4 | 1) * 4;
+// Of shared memory: rows of x, parts of the logits, d, w.
+constexpr int64_t one_words(int64_t k, int rows, int pitch, int ring) { return ring * rows * k + 4 * rows * pitch + rows * pitch + k * ((pitch / 4 | 1) * 4); }
 
-template <int N> constexpr int one_words(int64_t k, int ring) { // of shared memory: rows of x, w, parts of the logits, d
-    return ring * kOneRows * (int)k + (int)k * N + 4 * kOneRows * N + kOneRows * N;
-}
-
-template <int N, int RING>
-__global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
+template <int N, int RING, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) ce_one_kernel(
     const float *__restrict__ x, const float *__restrict__ w, const float *__restrict__ bias, const int64_t *__restrict__ targets,
     const float *__restrict__ lse, const float *__restrict__ dloss, int64_t m, int k, int n, float *__restrict__ dx, double *__restrict__ partial) {
+    constexpr int ROWS = THREADS / 32, HALF = THREADS / 2, SLOTS = kOneColumns / HALF, P = (N + 3) / 4 * 4, PW = kOnePitch<P>, GROUPS = ROWS / 4;
+    constexpr int AT_ONCE = (SLOTS + 4) * N <= 100 ? 4 : 2; // rows whose logits a warp sums up at once: what the registers hold
     extern __shared__ __align__(16) float smem[];
-    __shared__ int has_s[kOneRows]; // a row without a target takes no part, whatever x holds there
-    float *xs = smem, *parts = xs + RING * kOneRows * k, *ds = parts + 4 * kOneRows * N, *ws = ds + kOneRows * N;
+    __shared__ int has_s[ROWS]; // a row without a target takes no part, whatever x holds there
+    float *xs = smem, *parts = xs + RING * ROWS * k, *ds = parts + 4 * ROWS * P, *ws = ds + ROWS * P;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     griddep_wait();
     griddep_launch_dependents();
-    const int64_t tiles = (m + kOneRows - 1) / kOneRows;
+    const int64_t tiles = (m + ROWS - 1) / ROWS;
     auto fetch = [&](int64_t tile, int at) {
         if (tile < tiles) {
-            const int64_t left = (m - tile * kOneRows < kOneRows ? m - tile * kOneRows : kOneRows) * k; // values; the rows are one piece
-            const float *src   = x + tile * kOneRows * k;
-            const uint32_t to  = ptx::smem_u32(xs + at * kOneRows * k);
-            for (int64_t i = 4 * t; i < left; i += 4 * kOneThreads)
+            const int64_t left = (m - tile * ROWS < ROWS ? m - tile * ROWS : ROWS) * k; // values; the rows are one piece
+            const float *src   = x + tile * ROWS * k;
+            const uint32_t to  = ptx::smem_u32(xs + at * ROWS * k);
+            for (int64_t i = 4 * t; i < left; i += 4 * THREADS)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (uint32_t)i * 4), "l"(src + i), "r"(left - i < 4 ? (int)(left - i) * 4 : 16)
                              : "memory");
         }
@@ -662,181 +666,221 @@ __global__ void __launch_bounds__(kOneThreads, 1) ce_one_kernel(
 #pragma unroll
     for (int i = 0; i < RING; ++i)
         fetch(blockIdx.x + (int64_t)i * gridDim.x, i);
-    for (int i = t; i < k * N; i += kOneThreads)
-        ws[i] = i % N < n ? w[(i / N) * n + i % N] : 0.0f;
-    f32x2 wc[2][N / 2], sum[2][N / 2]; // of columns t and t + 512
+    for (int i = t; i < k * PW; i += THREADS)
+        ws[i] = i % PW < n ? w[(i / PW) * n + i % PW] : 0.0f;
+    const bool back = t >= HALF; // dx, else dw
+    const int mine  = t & (HALF - 1), turns = mine - lane >= k ? 0 : (k - (mine - lane) + HALF - 1) / HALF; // the warp's
+    f32x2 reg[SLOTS][N / 2]; // of columns mine + HALF i: w, or sums
     float sum_b = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int i = 0; i < SLOTS; ++i)
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) {
-            const int c = t + q * kOneThreads;
-            wc[q][j]    = pack2(c < k && 2 * j < n ? w[(int64_t)c * n + 2 * j] : 0.0f, c < k && 2 * j + 1 < n ? w[(int64_t)c * n + 2 * j + 1] : 0.0f);
-            sum[q][j]   = 0;
+            const int c = mine + i * HALF;
+            reg[i][j]   = back ? pack2(c < k && 2 * j < n ? w[(int64_t)c * n + 2 * j] : 0.0f, c < k && 2 * j + 1 < n ? w[(int64_t)c * n + 2 * j + 1] : 0.0f)
+                               : (f32x2)0;
         }
-    const int group = warp & 3, quarter = warp >> 2;
+    const int group = warp % GROUPS, quarter = warp / GROUPS;
     int at = 0;
-    int64_t before = -1; // the tile whose place is free
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
         __syncthreads();
-        const float *rows_at = xs + at * kOneRows * k;
-        const int rows       = (int)(m - tile * kOneRows < kOneRows ? m - tile * kOneRows : kOneRows);
+        const float *rows_at = xs + at * ROWS * k;
+        const int rows       = (int)(m - tile * ROWS < ROWS ? m - tile * ROWS : ROWS);
         // what d needs of this thread's row is on its way meanwhile
-        const int64_t row = tile * kOneRows + t / N;
-        const bool slope  = t < kOneRows * N && t / N < rows && t % N < n;
+        const int64_t row = tile * ROWS + t / P;
+        const bool slope  = t < ROWS * P && t / P < rows && t % P < n;
         const int64_t target = slope ? __ldg(targets + row) : -1;
-        const float l = slope ? __ldg(lse + row) : 0.0f, by = slope && dloss ? __ldg(dloss + row) : 1.0f, add = slope && bias ? __ldg(bias + t % N) : 0.0f;
-        { // the logits' parts
-            f32x2 acc[4][N / 2];
+        const float l = slope ? __ldg(lse + row) : 0.0f, by = slope && dloss ? __ldg(dloss + row) : 1.0f, add = slope && bias ? __ldg(bias + t % P) : 0.0f;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 4; r0 += AT_ONCE) { // the logits' parts
+            f32x2 acc[AT_ONCE][N / 2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < AT_ONCE; ++r)
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j)
                     acc[r][j] = 0;
-            const float *mine = rows_at + group * 4 * k;
+            const float *from = rows_at + (group * 4 + r0) * k;
 #pragma unroll 2
             for (int c = quarter * 32 + lane; c < k; c += 128) {
-                f32x2 wv[N / 2];
+                f32x2 wv[P / 2];
 #pragma unroll
-                for (int j = 0; j < N / 4; ++j) {
-                    const float4 q = *reinterpret_cast<const float4 *>(ws + c * N + 4 * j);
+                for (int j = 0; j < P / 4; ++j) {
+                    const float4 q = *reinterpret_cast<const float4 *>(ws + c * PW + 4 * j);
                     wv[2 * j] = pack2(q.x, q.y), wv[2 * j + 1] = pack2(q.z, q.w);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float v = mine[r * k + c];
+                for (int r = 0; r < AT_ONCE; ++r) {
+                    const float v = from[r * k + c];
 #pragma unroll
                     for (int j = 0; j < N / 2; ++j)
                         acc[r][j] = fma2(pack2(v, v), wv[j], acc[r][j]);
                 }
             }
-            float v[4 * N];
+            constexpr int COUNT = (AT_ONCE * P + 15) / 16 * 16;
+            float v[COUNT] = {};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < AT_ONCE; ++r)
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j)
-                    unpack2(acc[r][j], v[r * N + 2 * j], v[r * N + 2 * j + 1]);
-            fused::sum_by_halves<4 * N>(v);
+                    unpack2(acc[r][j], v[r * P + 2 * j], v[r * P + 2 * j + 1]);
+            fused::sum_by_halves<COUNT>(v);
             if (!(lane & 1))
 #pragma unroll
-                for (int i = 0; i < N / 4; ++i)
-                    parts[(quarter * kOneRows + group * 4) * N + (lane >> 1) * (N / 4) + i] = v[i];
+                for (int i = 0; i < COUNT / 16; ++i) {
+                    const int which = (lane >> 1) * (COUNT / 16) + i;
+                    if (which < AT_ONCE * P)
+                        parts[(quarter * ROWS + group * 4 + r0) * P + which] = v[i];
+                }
         }
         __syncthreads();
-        if (before >= 0) // all are through with the tile before
-            fetch(before + (int64_t)RING * gridDim.x, at == 0 ? RING - 1 : at - 1);
-        before = tile;
-        if (t < kOneRows * N) {
-            const int j = t % N;
+        if (t < ROWS * P) {
+            const int j = t % P;
             float d     = 0.0f;
             if (slope) {
                 float z = parts[t];
 #pragma unroll
                 for (int q = 1; q < 4; ++q)
-                    z = __fadd_rn(z, parts[q * kOneRows * N + t]);
+                    z = __fadd_rn(z, parts[q * ROWS * P + t]);
                 if (bias)
                     z = __fadd_rn(z, add);
                 const float p  = expf(__fsub_rn(z, l));
                 const bool has = target >= 0 && target < n;
                 if (j == 0)
-                    has_s[t / N] = has;
+                    has_s[t / P] = has;
                 if (has)
                     d = __fmul_rn(by, j == target ? __fsub_rn(p, 1.0f) : p);
             }
             ds[t] = d;
         }
         __syncthreads();
-        if (t < N)
+        if (t >= THREADS - 32 && lane < N) // a warp that has no more columns than another
             for (int r = 0; r < rows; ++r)
-                sum_b = __fadd_rn(sum_b, ds[r * N + t]);
-        const bool here[2] = {t < k, t + kOneThreads < k};
-        if (here[0])
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const bool has = has_s[r] != 0;
-                f32x2 d[N / 2];
+                sum_b = __fadd_rn(sum_b, ds[r * P + lane]);
+        auto row_of = [&](int r, f32x2 (&d)[P / 2]) {
 #pragma unroll
-                for (int j = 0; j < N / 4; ++j) {
-                    const float4 q = *reinterpret_cast<const float4 *>(ds + r * N + 4 * j);
-                    d[2 * j] = pack2(q.x, q.y), d[2 * j + 1] = pack2(q.z, q.w);
-                }
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    if (here[q]) {
-                        const int c   = t + q * kOneThreads;
-                        const float v = has ? rows_at[r * k + c] : 0.0f;
-                        f32x2 back    = 0;
-#pragma unroll
-                        for (int j = 0; j < N / 2; ++j) {
-                            sum[q][j] = fma2(pack2(v, v), d[j], sum[q][j]);
-                            back      = fma2(d[j], wc[q][j], back);
-                        }
-                        float a, b;
-                        unpack2(back, a, b);
-                        if (dx)
-                            dx[(tile * kOneRows + r) * k + c] = __fadd_rn(a, b);
-                    }
+            for (int j = 0; j < P / 4; ++j) {
+                const float4 q = *reinterpret_cast<const float4 *>(ds + r * P + 4 * j);
+                d[2 * j] = pack2(q.x, q.y), d[2 * j + 1] = pack2(q.z, q.w);
             }
+        };
+        if (!back) {
+#pragma unroll 2
+            for (int r = 0; r < rows; ++r) {
+                if (!has_s[r])
+                    continue;
+                f32x2 d[P / 2];
+                row_of(r, d);
+                const float *from = rows_at + r * k + mine; // beyond the last column: within shared memory, and of no use
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    if (i >= turns)
+                        break;
+                    const float v = from[i * HALF];
+#pragma unroll
+                    for (int j = 0; j < N / 2; ++j)
+                        reg[i][j] = fma2(pack2(v, v), d[j], reg[i][j]);
+                }
+            }
+        } else if (dx) {
+#pragma unroll 2
+            for (int r = 0; r < rows; ++r) {
+                f32x2 d[P / 2];
+                row_of(r, d);
+                float *to = dx + (tile * ROWS + r) * k + mine;
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    if (i >= turns)
+                        break;
+                    f32x2 sum = 0;
+#pragma unroll
+                    for (int j = 0; j < N / 2; ++j)
+                        sum = fma2(d[j], reg[i][j], sum);
+                    float a, b;
+                    unpack2(sum, a, b);
+                    if (mine + i * HALF < k)
+                        to[i * HALF] = __fadd_rn(a, b);
+                }
+            }
+        }
+        __syncthreads(); // all are through with the rows
+        fetch(tile + (int64_t)RING * gridDim.x, at);
         at = at == RING - 1 ? 0 : at + 1;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!partial)
         return;
     double *to = partial + (int64_t)blockIdx.x * ((int64_t)k * n + n);
+    if (!back) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+        for (int i = 0; i < SLOTS; ++i)
 #pragma unroll
-        for (int j = 0; j < N / 2; ++j) {
-            const int c = t + q * kOneThreads;
-            float a, b;
-            unpack2(sum[q][j], a, b);
-            if (c < k && 2 * j < n)
-                to[(int64_t)c * n + 2 * j] = (double)a;
-            if (c < k && 2 * j + 1 < n)
-                to[(int64_t)c * n + 2 * j + 1] = (double)b;
-        }
-    if (t < n)
-        to[(int64_t)k * n + t] = (double)sum_b;
+            for (int j = 0; j < N / 2; ++j) {
+                const int c = mine + i * HALF;
+                float a, b;
+                unpack2(reg[i][j], a, b);
+                if (c < k && 2 * j < n)
+                    to[(int64_t)c * n + 2 * j] = (double)a;
+                if (c < k && 2 * j + 1 < n)
+                    to[(int64_t)c * n + 2 * j + 1] = (double)b;
+            }
+    }
+    if (t >= THREADS - 32 && lane < n)
+        to[(int64_t)k * n + lane] = (double)sum_b;
 }
 
 bool ce_one_applicable(const float *x, int64_t k) { // n <= kFewClasses
     return k > 0 && k <= kOneColumns && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
 }
 
-template <int N, int RING>
+template <int N, int RING, int THREADS>
 ct_status launch_ce_one(
     const DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m,
     int64_t k, int64_t n, float *dx, float *dw, float *dbias) {
-    const int smem = one_words<N>(k, RING) * 4;
-    auto kernel    = ce_one_kernel<N, RING>;
+    constexpr int ROWS = THREADS / 32;
+    const size_t smem  = (size_t)one_words(k, ROWS, (N + 3) / 4 * 4, RING) * 4;
+    auto kernel        = ce_one_kernel<N, RING, THREADS>;
     static bool attr_set_dev[16] = {};
     if (!attr_set_dev[st->device & 15]) {
         CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
         attr_set_dev[st->device & 15] = true;
     }
-    const int64_t grid = std::min<int64_t>((m + kOneRows - 1) / kOneRows, st->sm_count), width = k * n + n;
+    const int64_t grid = std::min<int64_t>((m + ROWS - 1) / ROWS, (int64_t)st->sm_count * (512 / THREADS)), width = k * n + n;
     Scratch partial;
     if (dw || dbias)
         CT_TRY(partial.get((size_t)(grid * width) * 8));
-    CT_CUDA(launch_dependent(kernel, dim3((unsigned)grid), dim3(kOneThreads), (size_t)smem, stream(), x, w, bias, targets, lse, dloss, m, (int)k, (int)n, dx,
+    CT_CUDA(launch_dependent(kernel, dim3((unsigned)grid), dim3(THREADS), smem, stream(), x, w, bias, targets, lse, dloss, m, (int)k, (int)n, dx,
                              dw || dbias ? partial.as<double>() : nullptr));
     CT_LAUNCH_CHECK("ce_one");
     return dw || dbias ? fused::join_columns(partial.as<const double>(), grid, k * n, width, dw, dbias) : CT_OK;
 }
+// Two blocks of eight warps to an SM, whose phases overlap, where both fit: up to 8 classes, whose columns then fit the registers, in shared memory
+// with two or three tiles of x, and enough rows to pay for as many blocks' beginnings (60000 x 785 x 8: 150 us with one, 135; 1000 x 785 x 10: 17
+// with one, 25).  Else one of sixteen (60000 x 785 x 10: 160, as two 185).
 template <int N>
-ct_status launch_ce_one_ring(
+ct_status launch_ce_one_of(
     const DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m,
     int64_t k, int64_t n, float *dx, float *dw, float *dbias) {
-    return one_words<N>(k, 3) * 4 <= 224 * 1024 ? launch_ce_one<N, 3>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias)
-                                                : launch_ce_one<N, 2>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+    constexpr int64_t P = (N + 3) / 4 * 4, half = 112 * 1024 / 4;
+    if constexpr (N <= 8) {
+        const bool many = m >= (int64_t)st->sm_count * 64;
+        if (many && one_words(k, 8, P, 3) <= half)
+            return launch_ce_one<N, 3, 256>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+        if (many && one_words(k, 8, P, 2) <= half)
+            return launch_ce_one<N, 2, 256>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+    }
+    if constexpr (one_words(kOneColumns, 16, P, 3) > 2 * half) {
+        if (one_words(k, 16, P, 3) > 2 * half)
+            return launch_ce_one<N, 2, 512>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
+    }
+    return launch_ce_one<N, 3, 512>(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
 }
 
 ct_status ce_few_grad(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m, int64_t k,
     int64_t n, float *dx, float *dw, float *dbias) {
     if (ce_one_applicable(x, k)) {
-        auto run = n <= 4 ? launch_ce_one_ring<4> : n <= 8 ? launch_ce_one_ring<8> : n <= 12 ? launch_ce_one_ring<12> : launch_ce_one_ring<16>;
+        auto run = n <= 4 ? launch_ce_one_of<4> : n <= 8 ? launch_ce_one_of<8> : n <= 10 ? launch_ce_one_of<10> : n <= 12 ? launch_ce_one_of<12> : launch_ce_one_of<16>;
         return run(st, x, w, bias, targets, lse, dloss, m, k, n, dx, dw, dbias);
     }
     const int64_t blocks = (m + 255) / 256;

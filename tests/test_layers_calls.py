@@ -198,6 +198,15 @@ def test_cross_entropy_vocabulary_in_pieces(m, k, n):
 
 
 @gpu
+@pytest.mark.parametrize("m,k,n", [(30, 1024, 16), (9600, 1024, 4), (9500, 700, 3), (9500, 1000, 8), (40, 1024, 8), (200, 33, 15), (2500, 511, 12), (300, 1, 2)])
+def test_few_classes(m, k, n):
+    """Blocks of eight and of sixteen warps, two and three tiles on their way."""
+    x, w, b, t = ce_inputs(m, k, n, 34)
+    check_ce(x, w, b, t)
+    check_ce_grad(x, w, b, t, np.random.default_rng(4).uniform(0.5, 1, m).astype(np.float32))
+
+
+@gpu
 def test_weights_whose_rows_and_columns_differ_in_size():
     """Rows of the weights 2^-30 .. 2^30 against columns of x the other way, a row of zeros, columns 2^-30 below the others."""
     for m, k, n in ((200, 60, 20000), (200, 60, 300)):
