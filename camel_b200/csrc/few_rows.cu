@@ -138,7 +138,7 @@ template <int M, int GATE> ct_status launch_few(DeviceState *st, FewParams &p) {
     constexpr int WIDE   = GATE < 0 ? 128 : 64;
     const int64_t strips = (p.n + WIDE - 1) / WIDE;
     p.parts              = 1;
-    while (p.parts < 8 && strips * p.parts * 2 <= (int64_t)st->sm_count * 4 && p.k >= p.parts * 2 * 64)
+    while (p.parts < 8 && strips * p.parts * 2 <= (int64_t)st->sm_count * (M == 1 ? 4 : M == 4 ? 3 : 2) && p.k >= p.parts * 2 * 64) // in one wave
         p.parts *= 2;
     CT_CUDA(launch_dependent_cluster(few_rows_kernel<M, GATE>, p.parts, dim3((unsigned)(strips * p.parts)), dim3(256), 0, stream(), p));
     CT_LAUNCH_CHECK("few_rows");
