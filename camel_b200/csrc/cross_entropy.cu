@@ -61,6 +61,54 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(
     }
 }
 
+// Long rows: the parts that ce_join_kernel adds up, 4096 logits to a block, read once.  By one block to a row 4 x 64 x 64000 took 30 us, so 11,
+// 1 x 1024 x 131072 121 and 82.
+constexpr int kPartLogits = 4096;
+__global__ void __launch_bounds__(256) ce_parts_kernel(
+    const float *__restrict__ z, const int64_t *__restrict__ targets, int64_t rows, int64_t n, float2 *__restrict__ part, float *__restrict__ at_target) {
+    __shared__ float top_s[8], sum_s[8];
+    griddep_wait();
+    griddep_launch_dependents();
+    const float *row = z + (int64_t)blockIdx.y * n;
+    const int64_t c0 = (int64_t)blockIdx.x * kPartLogits;
+    float v[kPartLogits / 256], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPartLogits / 256; ++i) {
+        const int64_t c = c0 + i * 256 + threadIdx.x;
+        v[i]            = c < n ? row[c] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < kPartLogits / 256; ++i)
+        top = fmaxf(top, v[i]); // a NaN shows in the sum
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0)
+        top_s[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < 8; ++w)
+        top = fmaxf(top, top_s[w]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int i = 0; i < kPartLogits / 256; ++i)
+        sum = __fadd_rn(sum, expf(__fsub_rn(v[i], base)));
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+    if ((threadIdx.x & 31) == 0)
+        sum_s[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = 0.0f;
+        for (int w = 0; w < 8; ++w)
+            sum = __fadd_rn(sum, sum_s[w]);
+        part[(int64_t)blockIdx.x * rows + blockIdx.y] = make_float2(top, sum);
+        const int64_t t = targets[blockIdx.y];
+        if (t >= c0 && t < n && t < c0 + kPartLogits)
+            at_target[blockIdx.y] = row[t];
+    }
+}
+
 // x without the rows that have no target: 0 x anything of theirs is no term of dw.
 __global__ void __launch_bounds__(256) ce_rows_with_target_kernel(
     const float *__restrict__ x, const int64_t *__restrict__ targets, int64_t count, int64_t k, int64_t n, float *__restrict__ out) {
@@ -1010,8 +1058,11 @@ ct_status ct_dense_cross_entropy(
     if (fused_form && !fused::takes_few_rows(m, n))
         return ce_fused(st, x, w, bias, targets, m, k, n, loss, lse);
     const int64_t piece = n <= kFewClasses ? m : rows_at_once(m, n);
-    Scratch logits;
+    const int64_t slots = (n + kPartLogits - 1) / kPartLogits;
+    Scratch logits, parts;
     CT_TRY(logits.get((size_t)(piece * n) * 4));
+    if (slots > 2)
+        CT_TRY(parts.get((size_t)(slots * piece) * 8 + (size_t)piece * 4));
     if (n <= kFewClasses) {
         CT_TRY(few_logits(st, x, w, bias, m, k, n, logits.as<float>()));
         CT_CUDA(launch_dependent(ce_few_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream(), logits.as<const float>(), targets, m, (int)n,
@@ -1025,6 +1076,18 @@ ct_status ct_dense_cross_entropy(
             CT_TRY(fused::few_rows(st, x + r * k, w, bias, nullptr, nullptr, rows, k, n, 0, logits.as<float>(), nullptr, nullptr));
         else
             CT_TRY(ct_dense(x + r * k, w, bias, rows, k, n, CT_ACT_NONE, logits.as<float>(), nullptr));
+        if (slots > 2) {
+            float2 *part     = parts.as<float2>();
+            float *at_target = parts.as<float>((size_t)(slots * piece) * 8);
+            CT_CUDA(launch_dependent(ce_parts_kernel, dim3((unsigned)slots, (unsigned)rows), dim3(256), 0, stream(), logits.as<const float>(), targets + r, rows,
+                                     n, part, at_target));
+            CT_LAUNCH_CHECK("ce_parts");
+            CT_CUDA(launch_dependent(ce_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream(), (const float2 *)part, (int)slots,
+                                     (const float *)at_target, targets + r, rows, n, loss ? loss + r : nullptr, lse ? lse + r : nullptr,
+                                     (const uint32_t *)st->flags_dev));
+            CT_LAUNCH_CHECK("ce_join");
+            continue;
+        }
         CT_CUDA(launch_dependent(ce_rows_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), logits.as<const float>(), targets + r, n,
                                  loss ? loss + r : nullptr, lse ? lse + r : nullptr));
         CT_LAUNCH_CHECK("ce_rows");

@@ -620,7 +620,7 @@ ct_status join_columns(const double *partial, int64_t parts, int64_t n, int64_t 
 
 // Whether a product of m rows and that many columns (of both matrices) is few_rows': its passes have eight rows, the second of which reads
 // the weights from L2 where they fit, while the streamed product has some 15 us of its own: 16 x 1024 x 2000 20 us against 29, x 8000 37
-// against 29, x 32000 102 against 48, 9 x 64 x 64000 37 against 16; two matrices 16 x 1024 x 2048 18 against 25, x 4096 32 against 25.
+// against 29, x 32000 94 against 48; two matrices 16 x 1024 x 2048 18 against 25, x 4096 32 against 25.
 inline bool takes_few_rows(int64_t m, int64_t columns) { return m <= 8 || (m <= 16 && columns < 6144); }
 // out[m][n] = x . w + bias for at most kFewRows rows, or gate(x . w + bias) * (x . w_up + b_up) (w_up non-null), float32 on the CUDA cores.
 constexpr int64_t kFewRows = 16;

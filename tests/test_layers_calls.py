@@ -207,6 +207,26 @@ def test_few_classes(m, k, n):
 
 
 @gpu
+@pytest.mark.parametrize("n", [8193, 12288, 20001])
+def test_long_rows_of_logits(n):
+    """Masked stretches as long as a part, a row that is masked but for its target, a NaN, rows without a target."""
+    x, w, b, t = ce_inputs(6, 24, n, 35)
+    t[:] = [0, n - 1, 4095, 4096, -1, n]
+    b[4097:8192] = -np.inf
+    check_ce(x, w, b, t)
+    only = np.full(n, -np.inf, np.float32)
+    only[4096] = 0.5
+    loss, lse = T.dense_cross_entropy(dev(x), dev(w), dev(np.full(6, 4096)), dev(only))
+    z = x.astype(np.float64) @ w[:, 4096].astype(np.float64) + 0.5
+    assert np.abs(lse.numpy() - z).max() <= 1e-5 and np.abs(loss.numpy()).max() <= 1e-6
+    x[2, 3] = np.nan
+    loss, lse = T.dense_cross_entropy(dev(x), dev(w), dev(t), dev(b))
+    assert np.isnan(lse.numpy()).tolist() == [False, False, True, False, False, False] and np.isnan(loss.numpy()[2])
+    lse = T.dense_cross_entropy(dev(x), dev(w), dev(t), dev(np.full(n, -np.inf, np.float32)))[1].numpy()
+    assert np.isneginf(lse[[0, 1, 3, 4, 5]]).all() and np.isnan(lse[2])
+
+
+@gpu
 def test_weights_whose_rows_and_columns_differ_in_size():
     """Rows of the weights 2^-30 .. 2^30 against columns of x the other way, a row of zeros, columns 2^-30 below the others."""
     for m, k, n in ((200, 60, 20000), (200, 60, 300)):
