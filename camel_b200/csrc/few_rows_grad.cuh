@@ -3,10 +3,10 @@
 //   dx = d . w^T (of two matrices the sum over both), dw = x^T . d, db = column sums of d
 //
 // Bound by reading the weights and writing their gradient, once each: a block has 1024 columns and a part of the rows of a matrix, a lane four
-// columns (32 apart: any alignment is whole lines), whose d stay in registers while the rows go by.  A row's value of dw is a few products in
+// columns (32 apart: any alignment is whole lines), whose d stay in registers while the rows go by, the next ones on their way.  A row's value of dw is a few products in
 // the lane; its parts of dx are summed over the lane's columns, by halves over the warp, in shared memory over the block, and in 64 bits over
 // the blocks beside it (join_columns).  d itself comes from what D computes it of, again in each part.
-// As operand planes and tiles, which mostly hold nothing, 1 x 975 x 37218 with the logits took 317 us, so 115; 16 x 1024 x 32000 250, so 173.
+// As operand planes and tiles, which mostly hold nothing, 1 x 975 x 37218 with the logits took 317 us, so 102; 16 x 1024 x 32000 250, so 172.
 #pragma once
 
 #include "fastmath.cuh"
@@ -22,7 +22,7 @@ struct FewGrad {
     int64_t k, n, each;        // each: rows of a part, a multiple of 8
     int m, strips, parts;
 };
-constexpr int kFewGradColumns = 1024, kFewGradRows = 32; // of a block; rows of w whose x and sums are in shared memory at a time
+constexpr int kFewGradColumns = 1024; // of a block
 
 #ifdef __CUDACC__
 
@@ -49,29 +49,44 @@ template <int COUNT> __device__ __forceinline__ void sum_by_halves(float (&v)[CO
 // D: kMatrices; has(r): whether row r takes part (else at is 0 and x is not looked at); at(which, r, c).  M: rows, rounded up.
 template <class D, int M>
 __global__ void __launch_bounds__(256, M == 4 ? 3 : 2) few_grad_kernel(const __grid_constant__ FewGrad p, const __grid_constant__ D d) {
-    constexpr int KK = M == 16 ? 2 : 4; // rows of w at a time
+    constexpr int KK = M == 16 ? 2 : 4, ROWS = 512 / M; // rows of w at a time; whose x and sums are in shared memory at a time
     extern __shared__ __align__(16) float few_smem[];
-    __shared__ __align__(16) float xs[kFewGradRows][M];
-    __shared__ float sums[8][kFewGradRows * M];
+    __shared__ __align__(16) float xs[ROWS][M];
+    __shared__ float sums[8][ROWS * M];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int strip = (int)(blockIdx.x % p.strips), part = (int)(blockIdx.x / p.strips % p.parts), which = (int)(blockIdx.x / p.strips / p.parts);
     const int64_t c0 = (int64_t)strip * kFewGradColumns, k0 = part * p.each, k1 = min(p.k, k0 + p.each);
     const int wide = (int)min((int64_t)kFewGradColumns, p.n - c0);
     griddep_wait();
     griddep_launch_dependents();
-    const bool active = warp * 128 < wide;
-    for (int i = t; i < M * kFewGradColumns; i += 256) { // one copy of the code, however many values
-        const int r = i / kFewGradColumns, c = i % kFewGradColumns;
-        few_smem[i] = r < p.m && c < wide && d.has(r) ? d.at(which, r, c0 + c) : 0.0f;
-    }
-    __syncthreads();
-    f32x2 dd[M / 2][4]; // of rows 2 j and 2 j + 1
+    const bool active = warp * 128 < wide, back = p.dx != nullptr;
+    const float *w = p.w[which];
+    float *dw      = p.dw[which];
     int64_t col[4];
     bool here[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int c = warp * 128 + q * 32 + lane;
         col[q] = c0 + c, here[q] = c < wide;
+    }
+    float v[KK][4], next[KK][4];
+    auto load = [&](int64_t row, float (&to)[KK][4]) {
+#pragma unroll
+        for (int i = 0; i < KK; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                to[i][q] = back && here[q] && row + i < k1 ? __ldcs(w + (row + i) * p.n + col[q]) : 0.0f;
+    };
+    load(k0, next); // d is computed meanwhile
+    for (int i = t; i < M * kFewGradColumns; i += 256) { // one copy of the code, however many values
+        const int r = i / kFewGradColumns, c = i % kFewGradColumns;
+        few_smem[i] = r < p.m && c < wide && d.has(r) ? d.at(which, r, c0 + c) : 0.0f;
+    }
+    __syncthreads();
+    f32x2 dd[M / 2][4]; // of rows 2 j and 2 j + 1
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int c = warp * 128 + q * 32 + lane;
 #pragma unroll
         for (int j = 0; j < M / 2; ++j)
             dd[j][q] = pack2(few_smem[2 * j * kFewGradColumns + c], few_smem[(2 * j + 1) * kFewGradColumns + c]);
@@ -86,23 +101,11 @@ __global__ void __launch_bounds__(256, M == 4 ? 3 : 2) few_grad_kernel(const __g
             p.db[which][col[q]] = s;
         }
     }
-    const float *w = p.w[which];
-    float *dw      = p.dw[which];
-    const bool back = p.dx != nullptr;
-    for (int64_t from = k0; from < k1; from += kFewGradRows) {
-        const int rows = (int)min((int64_t)kFewGradRows, k1 - from);
-        float v[KK][4], next[KK][4];
-        auto load = [&](int r0, float (&to)[KK][4]) {
-#pragma unroll
-            for (int i = 0; i < KK; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    to[i][q] = back && here[q] && r0 + i < rows ? __ldcs(w + (from + r0 + i) * p.n + col[q]) : 0.0f;
-        };
-        load(0, next);
+    for (int64_t from = k0; from < k1; from += ROWS) {
+        const int rows = (int)min((int64_t)ROWS, k1 - from);
         __syncthreads(); // the rows before these are through
-        for (int i = t; i < kFewGradRows * M; i += 256) {
-            const int r = i / kFewGradRows, kk = i % kFewGradRows;
+        for (int i = t; i < ROWS * M; i += 256) {
+            const int r = i / ROWS, kk = i % ROWS;
             xs[kk][r] = r < p.m && kk < rows && dw && d.has(r) ? p.x[r * p.k + from + kk] : 0.0f;
         }
         __syncthreads();
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(256, M == 4 ? 3 : 2) few_grad_kernel(const __g
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         v[i][q] = next[i][q];
-                load(r0 + KK, next);
+                load(from + r0 + KK, next);
                 if (dw)
 #pragma unroll
                     for (int i = 0; i < KK; ++i) {
@@ -154,8 +157,8 @@ __global__ void __launch_bounds__(256, M == 4 ? 3 : 2) few_grad_kernel(const __g
             }
         __syncthreads();
         if (back)
-            for (int i = t; i < kFewGradRows * M; i += 256) {
-                const int kk = i % kFewGradRows, r = i / kFewGradRows;
+            for (int i = t; i < ROWS * M; i += 256) {
+                const int kk = i % ROWS, r = i / ROWS;
                 if (kk >= rows || r >= p.m)
                     continue;
                 float s = sums[0][kk * M + r];
