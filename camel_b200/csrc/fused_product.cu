@@ -446,14 +446,13 @@ Source source_of(const float *in, const float *in2, int64_t rows, int64_t cols, 
     return Source{in, in2, col_factor, rows, cols, padded(cols), vec ? 1 : 0};
 }
 
-// Two small products side by side: the K-major one has the first blocks.
+// A K-major and an MN-major product over the same machine.
 __global__ void __launch_bounds__(kThreads, 1) two_products_kernel(
     const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ Store::Params e, const __grid_constant__ Maps maps_mn,
-    const __grid_constant__ Product p_mn, const __grid_constant__ Store::Params e_mn) {
-    if ((int)blockIdx.x < p.total)
-        product_body<Store, 128, 1, false, false>(maps, p, e, (int)blockIdx.x, p.total);
-    else
-        product_body<Store, 128, 1, true, true>(maps_mn, p_mn, e_mn, (int)blockIdx.x - p.total, p_mn.total);
+    const __grid_constant__ Product p_mn, const __grid_constant__ Store::Params e_mn, int longer, int turns) {
+    product_body<Store, 128, 1, false, false>(
+        maps, p, e, maps_mn, p_mn, e_mn,
+        TilesOfTwo{(int)blockIdx.x, (int)gridDim.x, longer, longer ? p_mn.total : p.total, longer ? p.total : p_mn.total, turns});
 }
 
 } // namespace
@@ -596,26 +595,42 @@ Plan plan_of(const DeviceState *st, const Wanted &x) {
     best.splits = whole_slices(x, best.splits);
     return best;
 }
-// Both at once, in one wave of single CTAs, and their joins: gated gradient of 404 x 322 x 177 30 us one after the other, so 19, of
-// 1315 x 118 x 773 41 and 32.
-bool plan_both(const DeviceState *st, const Wanted (&x)[2], Plan (&plan)[2]) {
-    const int64_t tiles[2] = {tiles_of(x[0], 128), tiles_of(x[1], 128)};
-    double best            = plan[0].cost + plan[1].cost + 3.0; // a launch
-    bool both              = false;
-    for (int s = 1; s <= 32 && may_split(x[0], s); ++s) {
-        int t = (int)std::min<int64_t>(32, (st->sm_count - tiles[0] * s) / tiles[1]);
-        while (t > 1 && !may_split(x[1], t))
-            --t;
-        if (t < 1)
-            break;
-        const double cost = std::max(cost_of(x[0], s, 1, false), cost_of(x[1], t, 1, false)) + std::max(join_cost(x[0], s), join_cost(x[1], t));
-        if (cost < best)
-            best = cost, both = true, plan[0].splits = s, plan[1].splits = t;
-    }
-    if (both)
+// Both at once, on single CTAs, and their joins at once: TilesOfTwo, where the longer tiles are no more than the CTAs.  Gated gradient of
+// 404 x 322 x 177 30 us one after the other, so 19, of 1315 x 118 x 773 41 and 32, of 1537 x 771 x 2050 120 and 103.
+struct Shared {
+    bool use   = false;
+    int longer = 0, turns = 0;
+};
+Shared plan_both(const DeviceState *st, const Wanted *x, Plan *plan) {
+    constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+    const int64_t units = st->sm_count;
+    double best         = plan[0].cost + plan[1].cost + 3.0; // a launch
+    Shared how;
+    for (int s : kSplits)
+        for (int t : kSplits) {
+            if (!may_split(x[0], s) || !may_split(x[1], t))
+                break;
+            const int splits[2]     = {s, t};
+            const int64_t tiles[2]  = {tiles_of(x[0], 128) * s, tiles_of(x[1], 128) * t};
+            const double of_tile[2] = {cost_of(x[0], s, 1, false), cost_of(x[1], t, 1, false)};
+            const int longer        = of_tile[0] >= of_tile[1] ? 0 : 1;
+            const int64_t spare = units - tiles[longer], others = tiles[1 - longer];
+            const double lt = of_tile[longer], ot = of_tile[1 - longer], join = std::max(join_cost(x[0], s), join_cost(x[1], t));
+            if (spare < 0 || others > 0x3fffffff)
+                continue;
+            for (int turns = (int)(lt / ot); turns <= (int)(lt / ot) + 1; ++turns) {
+                const int64_t first = spare > 0 ? std::min<int64_t>(turns, (others + spare - 1) / spare) : 0, left = std::max<int64_t>(0, others - turns * spare);
+                const double cost = std::max(lt, (double)first * ot) + (double)((left + units - 1) / units) * ot + join;
+                if (cost < best) {
+                    best = cost, how.use = true, how.longer = longer, how.turns = turns;
+                    plan[0].splits = splits[0], plan[1].splits = splits[1], plan[0].pair = plan[1].pair = false;
+                }
+            }
+        }
+    if (how.use)
         for (int i = 0; i < 2; ++i)
-            plan[i].pair = false, plan[i].splits = whole_slices(x[i], plan[i].splits);
-    return both;
+            plan[i].splits = whole_slices(x[i], plan[i].splits);
+    return how;
 }
 
 bool whole(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
@@ -625,11 +640,10 @@ bool whole(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; 
 ct_status products(DeviceState *st, const Wanted *what, int count) {
     const char *name = "fused_product";
     Plan plan[2]     = {plan_of(st, what[0]), {}};
-    bool both        = false;
+    Shared both;
     if (count == 2) {
-        const Wanted pair[2] = {what[0], what[1]};
-        plan[1]              = plan_of(st, what[1]);
-        both                 = plan_both(st, pair, plan);
+        plan[1] = plan_of(st, what[1]);
+        both    = plan_both(st, what, plan);
     }
     Scratch partial[2];
     Product p[2]{};
@@ -663,7 +677,7 @@ ct_status products(DeviceState *st, const Wanted *what, int count) {
                                                   to.out2, to.cols, to.stride, to.second, vec, to.add ? 1 : 0};
             joins.blocks += strips * std::max<int64_t>(1, std::min<int64_t>(turns, (int64_t)st->sm_count * 16 / strips));
         }
-        if (both)
+        if (both.use)
             continue;
         if (x.mn)
             CT_TRY(plan[i].pair ? (launch<Store, 256, 2, true, true>(st, x.a, x.b, p[i], e[i], plan[i].splits, name))
@@ -673,14 +687,16 @@ ct_status products(DeviceState *st, const Wanted *what, int count) {
                                 : (launch<Store, 128, 1, false, false>(st, x.a, x.b, p[i], e[i], plan[i].splits, name)));
         CT_TRY(join()); // while the slices are in L2
     }
-    if (both) {
+    if (both.use) {
         Maps maps[2];
         CT_TRY((prepare<Store, 128, 1, false, false>(st, what[0].a, what[0].b, plan[0].splits, maps[0], p[0], name)));
         CT_TRY((prepare<Store, 128, 1, true, true>(st, what[1].a, what[1].b, plan[1].splits, maps[1], p[1], name)));
         static bool set_dev[16] = {};
         CT_TRY(allow_shared(st, two_products_kernel, set_dev));
-        CT_CUDA(launch_dependent(two_products_kernel, dim3((unsigned)(p[0].total + p[1].total)), dim3(kThreads), (size_t)kSmem, stream(), maps[0], p[0], e[0],
-                                 maps[1], p[1], e[1]));
+        const int grid = (int)std::min<int64_t>((int64_t)p[0].total + p[1].total, st->sm_count);
+        p[0].chunk_first = p[1].chunk_first = p[0].total + p[1].total <= grid ? kChunk : kChunkFirst;
+        CT_CUDA(launch_dependent(two_products_kernel, dim3((unsigned)grid), dim3(kThreads), (size_t)kSmem, stream(), maps[0], p[0], e[0], maps[1], p[1], e[1],
+                                 both.longer, both.turns));
         CT_LAUNCH_CHECK(name);
         CT_TRY(join());
     }

@@ -101,7 +101,7 @@ constexpr int kSmem     = kStages * kStage + kEpiWarps * 2048 + 1024;
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-template <bool MN> __device__ __forceinline__ uint64_t desc(uint32_t addr) { return MN ? desc_mn(addr) : smem_desc_k<128>(addr); }
+__device__ __forceinline__ uint64_t desc(bool mn, uint32_t addr) { return mn ? desc_mn(addr) : smem_desc_k<128>(addr); }
 
 __device__ __forceinline__ void tile_of(const Product &p, int tile, int &tm, int &tn, int &tz) {
     // groups of row tiles sweep the column tiles, so that CTAs running together share operands in L2
@@ -119,14 +119,41 @@ __device__ __forceinline__ void tile_of(const Product &p, int tile, int &tm, int
 // EPI: kTwin - the tile's columns are half of one matrix and half of another, and a thread has the same columns of both;
 // Params; store(p, e, acc, row0, lane, col0, z, part, stage): acc holds unscaled sums of row row0 + lane, columns col0 .. (twin: COLS / 2
 // columns from col0 of the first matrix, then those of the second), the part-th quarter of the tile's; stage is the warp's 2 KB.
-// block of `blocks`: which CTA of the product's this one is.
-template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
-__device__ __forceinline__ void product_body(const Maps &maps, const Product &p, const typename EPI::Params &e, int block, int blocks) {
+// Tiles is which tiles of which products this CTA has: kTwo; Tiles::at(i, job, tile), the i-th, or false.  Of two products the first (A_MN, B_MN
+// false) is K-major and the second MN-major.
+struct TilesOfOne {
+    static constexpr bool kTwo = false;
+    int first, stride, total;
+    __device__ __forceinline__ bool at(int i, int &job, int &tile) const {
+        job = 0, tile = first + i * stride;
+        return tile < total;
+    }
+};
+// A tile of the product whose tiles take longer to each of the first CTAs; the others begin with `turns` tiles of the other one each, and then all
+// share what is left of it, those others first.
+struct TilesOfTwo {
+    static constexpr bool kTwo = true;
+    int block, blocks, longer, long_total, other_total, turns;
+    __device__ __forceinline__ bool at(int i, int &job, int &tile) const {
+        const int spare = blocks - long_total;
+        job = longer, tile = block;
+        if (i == 0 && block < long_total)
+            return true;
+        job = 1 - longer;
+        if (block < long_total)
+            tile = turns * spare + (i - 1) * blocks + block + spare;
+        else
+            tile = i < turns ? i * spare + block - long_total : turns * spare + (i - turns) * blocks + block - long_total;
+        return tile < other_total;
+    }
+};
+template <class EPI, int BN, int CG, bool A_MN, bool B_MN, class Tiles>
+__device__ __forceinline__ void product_body(
+    const Maps &maps0, const Product &p0, const typename EPI::Params &e0, const Maps &maps1, const Product &p1, const typename EPI::Params &e1, const Tiles &tiles) {
     static_assert(BN / CG == 128, "128 columns of B to a CTA");
+    static_assert(!Tiles::kTwo || (CG == 1 && !A_MN && !B_MN), "two products");
     constexpr int SETS = 512 / (2 * BN), COLS = BN / 4;
-    const int rank   = CG == 2 ? (int)cluster_rank() : 0;
-    const int first  = block / CG;
-    const int stride = blocks / CG;
+    const int rank = CG == 2 ? (int)cluster_rank() : 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[kStages], bar_empty[kStages];
     __shared__ uint64_t bar_acc_full[2 * SETS], bar_acc_empty[2 * SETS]; // [set * 2 + which]: 0 leading accumulator, 1 cross products
@@ -137,7 +164,7 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     griddep_launch_dependents();
     if (threadIdx.x == 0)
-        abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
+        abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p0.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -150,10 +177,10 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
         }
         mbar_init(smem_u32(&bar_done), 1);
         mbar_fence_init();
-        prefetch_tensormap(&maps.a_hi);
-        prefetch_tensormap(&maps.a_lo);
-        prefetch_tensormap(&maps.b_hi);
-        prefetch_tensormap(&maps.b_lo);
+        prefetch_tensormap(&maps0.a_hi);
+        prefetch_tensormap(&maps0.a_lo);
+        prefetch_tensormap(&maps0.b_hi);
+        prefetch_tensormap(&maps0.b_lo);
     }
     if (warp == 1) {
         if (CG == 2) {
@@ -174,7 +201,7 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
     __syncthreads(); // every thread has read abort_flag_s before a role may raise it
     griddep_wait();
     auto stage_addr = [&](int s) { return smem_base + (uint32_t)s * kStage; };
-    auto k_range    = [&](int tz, int &from, int &count) {
+    auto k_range    = [&](const Product &p, int tz, int &from, int &count) {
         from           = p.stages_split > 0 ? tz * p.stages_split : 0;
         const int left = p.stages > from ? p.stages - from : 0;
         count          = p.stages_split > 0 && left > p.stages_split ? p.stages_split : left;
@@ -187,10 +214,13 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
             int s = 0, issued = 0;
             uint32_t phase = 1;
             bool ok        = true;
-            for (int tile = first; tile < p.total && ok; tile += stride) {
+            for (int i = 0, job, tile; ok && tiles.at(i, job, tile); ++i) {
+                const bool two      = Tiles::kTwo && job == 1, a_mn = A_MN || two, b_mn = B_MN || two;
+                const Product &p = two ? p1 : p0;
+                const Maps &maps = two ? maps1 : maps0;
                 int tm, tn, tz, from, count;
                 tile_of(p, tile, tm, tn, tz);
-                k_range(tz, from, count);
+                k_range(p, tz, from, count);
                 const int32_t a_row = (tm * CG + rank) * kRows;
                 // the two blocks of 64 columns of B; a K-major operand's are one box
                 const int32_t b_first  = !EPI::kTwin ? tn * BN + rank * 128 : (CG == 2 ? rank * p.twin_offset + tn * 128 : tn * 64);
@@ -214,7 +244,7 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                     const uint32_t dst = stage_addr(s);
                     const int32_t k0   = (from + kb) * 64;
                     auto load_a = [&](uint32_t to, const CUtensorMap *map) {
-                        if (A_MN) {
+                        if (a_mn) {
                             load(to, map, a_row, k0);
                             load(to + 8192, map, a_row + 64, k0);
                         } else {
@@ -222,7 +252,7 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                         }
                     };
                     auto load_b = [&](uint32_t to, const CUtensorMap *map) {
-                        if (B_MN) {
+                        if (b_mn) {
                             load(to, map, b_first, k0);
                             load(to + 8192, map, b_second, k0);
                         } else {
@@ -250,12 +280,11 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
     } else if (warp == 1) {
         // ===== MMA issuer (the leader's, for the pair) =====
         if (elect_one() && rank == 0) {
-            constexpr uint32_t idesc = make_idesc(0u, kRows * CG, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
-            constexpr int A_STEP = A_MN ? 128 : 2, B_STEP = B_MN ? 128 : 2; // descriptor units of 16 bytes per 16 values of k
-            int s = 0, i = 0;
+            constexpr uint32_t kIdesc = make_idesc(0u, kRows * CG, BN);
+            int s = 0;
             uint32_t phase = 0, empty_phase = (1u << (2 * SETS)) - 1u; // bit per accumulator: parity to wait for
             bool ok  = true;
-            auto mma = [&](uint32_t d, uint64_t da, uint64_t db, uint32_t accumulate) {
+            auto mma = [&](uint32_t idesc, uint32_t d, uint64_t da, uint64_t db, uint32_t accumulate) {
                 if (CG == 2)
                     mma_f16_pair(d, da, db, idesc, accumulate);
                 else
@@ -273,10 +302,14 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                 tc_fence_after_sync();
                 return got;
             };
-            for (int tile = first; tile < p.total && ok; tile += stride, ++i) {
+            for (int i = 0, job, tile; ok && tiles.at(i, job, tile); ++i) {
+                const bool two = Tiles::kTwo && job == 1, a_mn = A_MN || two, b_mn = B_MN || two;
+                const Product &p     = two ? p1 : p0;
+                const uint32_t idesc = kIdesc | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+                const int a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2; // descriptor units of 16 bytes per 16 values of k
                 int tm, tn, tz, from, count;
                 tile_of(p, tile, tm, tn, tz);
-                k_range(tz, from, count);
+                k_range(p, tz, from, count);
                 const int set         = SETS == 1 ? 0 : (i & (SETS - 1));
                 const uint32_t d_main = tmem_base + (uint32_t)(set * 2 * BN), d_cross = d_main + BN;
                 int in_chunk = 0, chunk = p.chunk_first;
@@ -287,8 +320,8 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                     }
                     tc_fence_after_sync();
                     const uint32_t at    = stage_addr(s);
-                    const uint64_t a_hi = desc<A_MN>(at), a_lo = desc<A_MN>(at + kTile);
-                    const uint64_t b_hi = desc<B_MN>(at + 2 * kTile), b_lo = desc<B_MN>(at + 3 * kTile);
+                    const uint64_t a_hi = desc(a_mn, at), a_lo = desc(a_mn, at + kTile);
+                    const uint64_t b_hi = desc(b_mn, at + 2 * kTile), b_lo = desc(b_mn, at + 3 * kTile);
                     const bool last = kb + 1 == count;
                     if (kb == 0 && !wait_empty(set * 2 + 1)) {
                         ok = false;
@@ -296,8 +329,8 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                     }
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        mma(d_cross, a_lo + A_STEP * kk, b_hi + B_STEP * kk, kb == 0 && kk == 0 ? 0u : 1u);
-                        mma(d_cross, a_hi + A_STEP * kk, b_lo + B_STEP * kk, 1u);
+                        mma(idesc, d_cross, a_lo + a_step * kk, b_hi + b_step * kk, kb == 0 && kk == 0 ? 0u : 1u);
+                        mma(idesc, d_cross, a_hi + a_step * kk, b_lo + b_step * kk, 1u);
                     }
                     if (in_chunk == 0 && !wait_empty(set * 2)) {
                         ok = false;
@@ -305,7 +338,7 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
                     }
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        mma(d_main, a_hi + A_STEP * kk, b_hi + B_STEP * kk, in_chunk == 0 && kk == 0 ? 0u : 1u);
+                        mma(idesc, d_main, a_hi + a_step * kk, b_hi + b_step * kk, in_chunk == 0 && kk == 0 ? 0u : 1u);
                     commit(smem_u32(&bar_empty[s])); // stage reusable once these MMAs retire
                     if (++s == kStages)
                         s = 0, phase ^= 1u;
@@ -331,11 +364,13 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
         const int part    = (warp - 2) >> 2; // which quarter of the tile's columns
         uint8_t *stage = smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStage + (warp - 2) * 2048;
         uint32_t full_phase = 0;
-        int i               = 0;
-        for (int tile = first; tile < p.total; tile += stride, ++i) {
+        for (int i = 0, job, tile; tiles.at(i, job, tile); ++i) {
+            const bool two                 = Tiles::kTwo && job == 1;
+            const Product &p               = two ? p1 : p0;
+            const typename EPI::Params &e = two ? e1 : e0;
             int tm, tn, tz, from, count;
             tile_of(p, tile, tm, tn, tz);
-            k_range(tz, from, count);
+            k_range(p, tz, from, count);
             const int set    = SETS == 1 ? 0 : (i & (SETS - 1));
             const int chunks = count == 0 ? 0 : count <= p.chunk_first ? 1 : 1 + (count - p.chunk_first + kChunk - 1) / kChunk;
             float acc[COLS];
@@ -407,12 +442,12 @@ __device__ __forceinline__ void product_body(const Maps &maps, const Product &p,
             tmem_dealloc(tmem_base, 512);
     }
     if (threadIdx.x == 0 && !failed && *abort_flag)
-        atomicExch(p.flags + FLAG_TIMEOUT, 1u + (uint32_t)blockIdx.x);
+        atomicExch(p0.flags + FLAG_TIMEOUT, 1u + (uint32_t)blockIdx.x);
 }
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ typename EPI::Params e) {
-    product_body<EPI, BN, CG, A_MN, B_MN>(maps, p, e, (int)blockIdx.x, (int)gridDim.x);
+    product_body<EPI, BN, CG, A_MN, B_MN>(maps, p, e, maps, p, e, TilesOfOne{(int)blockIdx.x / CG, (int)gridDim.x / CG, p.total});
 }
 
 // The inverse scales of columns col0 + 4 j .. + 3: one address for the warp.  Arrays of scales reach to the end of the last tile.
