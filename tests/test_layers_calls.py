@@ -142,6 +142,23 @@ def test_few_rows(m, k, n):
 
 
 @gpu
+@pytest.mark.parametrize("gate", ["sigmoid", "silu", "gelu"])
+def test_gates_keep_their_small_values(gate):
+    """Relative to the value, also where it is 1e-30: 2^-22 of the approximate exponential and ten roundings more, 14 in all."""
+    g = np.concatenate([np.linspace(-12, 12, 4001), -np.geomspace(1e-6, 12, 4000)]).astype(np.float32)
+    one = np.ones((1, 16), np.float32)
+    out, pre, _ = T.dense_gated(dev(g[:, None]), dev(one), dev(0 * one), None, dev(np.ones(16, np.float32)), gate=gate, keep=True)
+    assert (np.abs(pre.numpy() - g[:, None]) <= 2.0 ** -22 * np.abs(g[:, None])).all()
+    x = pre.numpy()[:, 0].astype(np.float64)  # what the gate was given
+    if gate == "gelu":
+        want = x * 0.5 * np.array([math.erfc(-v / math.sqrt(2)) for v in x])
+    else:
+        s = np.where(x >= 0, 1 / (1 + np.exp(-np.abs(x))), np.exp(-np.abs(x)) / (1 + np.exp(-np.abs(x))))
+        want = s if gate == "sigmoid" else x * s
+    within(out.numpy(), np.repeat(want[:, None], 16, 1), np.repeat(14 * U * np.abs(want)[:, None], 16, 1), gate)
+
+
+@gpu
 def test_dense_gated_wide_rows():
     """Rows of d that no block holds (n beyond 8192)."""
     m, k, n = 12, 24, 8300
