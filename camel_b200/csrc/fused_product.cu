@@ -555,7 +555,7 @@ ct_status split(DeviceState *st, const Split *what, int count) {
             CT_CUDA(launch_dependent_cluster(split_long_rows_kernel, ranks, dim3((unsigned)(x.src.rows * ranks)), dim3(256), 0, stream(), x.src, x.width, ranks, each,
                                              x.to, x.inverse));
         } else
-            CT_CUDA(run(split_rows_kernel<256, 16>, 1));
+            CT_CUDA(run(split_rows_kernel<256, 8>, 1)); // read twice
         CT_LAUNCH_CHECK("split_rows");
     }
     return CT_OK;

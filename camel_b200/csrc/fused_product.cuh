@@ -119,32 +119,32 @@ __device__ __forceinline__ void tile_of(const Product &p, int tile, int &tm, int
 // EPI: kTwin - the tile's columns are half of one matrix and half of another, and a thread has the same columns of both;
 // Params; store(p, e, acc, row0, lane, col0, z, part, stage): acc holds unscaled sums of row row0 + lane, columns col0 .. (twin: COLS / 2
 // columns from col0 of the first matrix, then those of the second), the part-th quarter of the tile's; stage is the warp's 2 KB.
-// Tiles is which tiles of which products this CTA has: kTwo; Tiles::at(i, job, tile), the i-th, or false.  Of two products the first (A_MN, B_MN
+// Tiles is which tiles of which products this CTA has: start, is there one, the next (the i-th).  kTwo: of two products the first (A_MN, B_MN
 // false) is K-major and the second MN-major.
 struct TilesOfOne {
     static constexpr bool kTwo = false;
-    int first, stride, total;
-    __device__ __forceinline__ bool at(int i, int &job, int &tile) const {
-        job = 0, tile = first + i * stride;
-        return tile < total;
-    }
+    int first, stride;
+    __device__ __forceinline__ void start(int &job, int &tile) const { job = 0, tile = first; }
+    __device__ __forceinline__ bool has(const Product &p, int, int tile) const { return tile < p.total; }
+    __device__ __forceinline__ void next(int, int &, int &tile) const { tile += stride; }
 };
 // A tile of the product whose tiles take longer to each of the first CTAs; the others begin with `turns` tiles of the other one each, and then all
 // share what is left of it, those others first.
 struct TilesOfTwo {
     static constexpr bool kTwo = true;
     int block, blocks, longer, long_total, other_total, turns;
-    __device__ __forceinline__ bool at(int i, int &job, int &tile) const {
+    __device__ __forceinline__ void start(int &job, int &tile) const {
+        job  = block < long_total ? longer : 1 - longer;
+        tile = block < long_total ? block : block - long_total;
+    }
+    __device__ __forceinline__ bool has(const Product &, int job, int tile) const { return job == longer || tile < other_total; }
+    __device__ __forceinline__ void next(int i, int &job, int &tile) const {
         const int spare = blocks - long_total;
-        job = longer, tile = block;
-        if (i == 0 && block < long_total)
-            return true;
         job = 1 - longer;
         if (block < long_total)
             tile = turns * spare + (i - 1) * blocks + block + spare;
         else
             tile = i < turns ? i * spare + block - long_total : turns * spare + (i - turns) * blocks + block - long_total;
-        return tile < other_total;
     }
 };
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN, class Tiles>
@@ -214,8 +214,9 @@ __device__ __forceinline__ void product_body(
             int s = 0, issued = 0;
             uint32_t phase = 1;
             bool ok        = true;
-            for (int i = 0, job, tile; ok && tiles.at(i, job, tile); ++i) {
-                const bool two      = Tiles::kTwo && job == 1, a_mn = A_MN || two, b_mn = B_MN || two;
+            int job, tile, i = 0;
+            for (tiles.start(job, tile); tiles.has(p0, job, tile) && ok; tiles.next(++i, job, tile)) {
+                const bool two   = Tiles::kTwo && job == 1, a_mn = A_MN || two, b_mn = B_MN || two;
                 const Product &p = two ? p1 : p0;
                 const Maps &maps = two ? maps1 : maps0;
                 int tm, tn, tz, from, count;
@@ -302,7 +303,8 @@ __device__ __forceinline__ void product_body(
                 tc_fence_after_sync();
                 return got;
             };
-            for (int i = 0, job, tile; ok && tiles.at(i, job, tile); ++i) {
+            int job, tile, i = 0;
+            for (tiles.start(job, tile); tiles.has(p0, job, tile) && ok; tiles.next(++i, job, tile)) {
                 const bool two = Tiles::kTwo && job == 1, a_mn = A_MN || two, b_mn = B_MN || two;
                 const Product &p     = two ? p1 : p0;
                 const uint32_t idesc = kIdesc | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
@@ -364,7 +366,8 @@ __device__ __forceinline__ void product_body(
         const int part    = (warp - 2) >> 2; // which quarter of the tile's columns
         uint8_t *stage = smem_raw + (smem_base - smem_u32(smem_raw)) + kStages * kStage + (warp - 2) * 2048;
         uint32_t full_phase = 0;
-        for (int i = 0, job, tile; tiles.at(i, job, tile); ++i) {
+        int job, tile, i = 0;
+        for (tiles.start(job, tile); tiles.has(p0, job, tile); tiles.next(++i, job, tile)) {
             const bool two                 = Tiles::kTwo && job == 1;
             const Product &p               = two ? p1 : p0;
             const typename EPI::Params &e = two ? e1 : e0;
@@ -447,7 +450,7 @@ __device__ __forceinline__ void product_body(
 template <class EPI, int BN, int CG, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, const __grid_constant__ typename EPI::Params e) {
-    product_body<EPI, BN, CG, A_MN, B_MN>(maps, p, e, maps, p, e, TilesOfOne{(int)blockIdx.x / CG, (int)gridDim.x / CG, p.total});
+    product_body<EPI, BN, CG, A_MN, B_MN>(maps, p, e, maps, p, e, TilesOfOne{(int)blockIdx.x / CG, (int)gridDim.x / CG});
 }
 
 // The inverse scales of columns col0 + 4 j .. + 3: one address for the warp.  Arrays of scales reach to the end of the last tile.
