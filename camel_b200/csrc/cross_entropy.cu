@@ -442,14 +442,14 @@ struct SlopesStream {
     __device__ static __forceinline__ void finish(const fused::Stream &, const Params &, State &, float *, int) {}
 };
 
-// What the rows of d are weighted with behind the planes: dloss / 2^14, zero for rows without a target.
+// What the rows of d are weighted with behind the planes: dloss / 2^14 (never -0), and -0 for rows without a target, which take no part.
 __global__ void __launch_bounds__(256) ce_weights_kernel(
     const float *__restrict__ dloss, const int64_t *__restrict__ targets, int64_t m, int64_t n, float *__restrict__ weight) {
     griddep_wait();
     griddep_launch_dependents();
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < m)
-        weight[i] = targets[i] >= 0 && targets[i] < n ? __fmul_rn(dloss ? dloss[i] : 1.0f, 1.0f / kSlopeScale) : 0.0f;
+        weight[i] = targets[i] >= 0 && targets[i] < n ? __fadd_rn(__fmul_rn(dloss ? dloss[i] : 1.0f, 1.0f / kSlopeScale), 0.0f) : __uint_as_float(fused::kNoPart);
 }
 
 ct_status ce_grad_fused(

@@ -54,8 +54,8 @@ __device__ __forceinline__ void put_quad(const Planes &to, int64_t at, float a, 
 
 __device__ __forceinline__ float4 factored(float4 q, const float *row_factor, int64_t r) {
     if (row_factor) {
-        const float f = row_factor[r]; // a row of factor zero takes no part, whatever it holds
-        q = f == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
+        const float f = row_factor[r];
+        q = __float_as_uint(f) == kNoPart ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(q.x * f, q.y * f, q.z * f, q.w * f);
     }
     return q;
 }

@@ -513,7 +513,7 @@ struct Store {
         const int rows     = left < 0 ? 0 : (left < 32 ? (int)left : 32);
         if (rows == 0)
             return;
-        const float rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.0f;
+        const float rs = lane < rows ? __fadd_rn(__ldg(p.row_scale + row0 + lane), 0.0f) : 0.0f; // kNoPart: a row of +0
 #pragma unroll
         for (int g = 0; g < COLS / 16; ++g) {
             const int64_t col = col0 + g * 16;
@@ -622,12 +622,15 @@ inline Planes columns_of(Planes p, int64_t from, int64_t cols) {
     return p;
 }
 
+// The factor of a row that takes no part, whatever it holds: -0.  Under a factor of 0 what is no number stays (0 x NaN is a term of a sum).
+constexpr uint32_t kNoPart = 0x80000000u;
+
 // What planes are made of, some matrices in one launch.
 struct Split {
     const float *in, *in2; // in2 (may be null): a matrix of the same shape whose columns follow those of in at column padded(cols) of the planes
     int64_t rows, cols;
     bool by_column;        // a scale per column, else per row (over both matrices)
-    const float *row_factor; // by_column, may be null: row r is taken times row_factor[r], and as zeros where that is zero
+    const float *row_factor; // by_column, may be null: row r is taken times row_factor[r], and as zeros where that is kNoPart
     Planes to;
     float *inverse;        // [rows], or scales(columns of the planes)
     const float *col_factor = nullptr; // else, may be null: column c is taken times col_factor[c] (a multiple of four of them)

@@ -179,7 +179,8 @@ ct_status gated_fused(
 // ---- the gradient's left operand ----
 
 // d = [dg | du] of a row, its largest magnitude, and its planes: TPR threads to a row, which hold V groups of four columns of both; longer
-// rows are computed twice.  inverse[row] is zero for a row of zeros: such a row must not widen the range of x' (gated_grad_fused).
+// rows are computed twice.  inverse[row] is zero for a row of zeros: such a row must not widen the range of x' (gated_grad_fused), where only
+// what is no number is left of it.
 // BIAS: a thread also sums its columns over the rows that it has, in float32, into partial[which of the grid's rows at a time][2][n] - of the
 // values themselves, since what the planes hold of a value depends on the rest of its row.  By a kernel that computes the slopes again
 // 1537 x 2050 took 17 us more.

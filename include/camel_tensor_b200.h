@@ -354,8 +354,8 @@ ct_status ct_dense_packed(
  *
  * Products of more than 16 rows hold each operand as pairs of float16 under one power of two per row (or per column, where rows are summed
  * over): to 2^-23 of a value down to 2^-27 of its line's largest, to 2^-50 of that largest below.  The error of a sum is at most 2^-22 of
- * its products' sizes and 2^-49 of its length times the two lines' largest, and the additions'.  Under CT_PREC_BF16 the products are
- * those of ct_dense. */
+ * its products' sizes and 2^-49 of its length times the two lines' largest, and the additions'.  A sum that meets an infinity of an
+ * operand is infinite or NaN (infinity times a low term of zero).  Under CT_PREC_BF16 the products are those of ct_dense. */
 
 /* Layer norm of each row: out = (x - mean) / sqrt(var + eps) * gamma + beta, mean and var (the mean square deviation) over the
  * row's `cols` values.  gamma and beta have one value per column; null: ones, zeros.  eps >= 0.  out may be x itself. */

@@ -1,0 +1,53 @@
+"""Layer norm, the gated dense layer and the cross entropy of a dense layer: what holds whatever the number of rows, and the kernels
+that only sizes beyond those of test_layers reach.  Definitions in 64 bits and bounds as there; tighter ones are derived here.
+"""
+import numpy as np
+import pytest
+
+import camel_b200._lib as L
+from camel_b200 import tensor as T
+from test_layers import ce_inputs, dev, gated_inputs
+
+gpu = pytest.mark.gpu
+
+
+# ---- values that are no numbers -------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["3xtf32", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(5, 40, 70), (16, 40, 70), (40, 40, 70), (200, 40, 70), (200, 40, 300), (1500, 33, 70)])
+def test_gated_rows_of_zero_gradient_count(m, k, n, precision):
+    """0 x NaN is a term of dw like any other, with any number of rows: x that is no number shows in its row of dw, and only there."""
+    x, wg, wu, _, _ = gated_inputs(m, k, n, 51)
+    g, u, dout = (np.random.default_rng(i).normal(0, 1, (m, n)).astype(np.float32) for i in range(3))
+    dout[3] = 0.0
+    x[3, 7], x[3, 9] = np.nan, np.inf
+    L.check(L.lib.ct_set_precision(L.PREC_BF16 if precision == "bf16" else L.PREC_3XTF32))
+    try:
+        dx, dwg, dwu = (a.numpy() for a in T.dense_gated_grad(*[dev(a) for a in (x, wg, wu, g, u, dout)]))
+    finally:
+        L.check(L.lib.ct_set_precision(L.PREC_3XTF32))
+    assert not dx[3].any() and np.isfinite(dx).all()
+    rest = [c for c in range(k) if c not in (7, 9)]
+    for dw in (dwg, dwu):
+        assert np.isnan(dw[[7, 9]]).all() and np.isfinite(dw[rest]).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(5, 40, 70), (40, 40, 70), (200, 40, 70), (200, 40, 24), (200, 40, 10), (200, 1100, 10)])
+def test_cross_entropy_rows_of_zero_weight_count(m, k, n):
+    """A row with a target and dloss = 0, where x holds a NaN: so are its logits, and 0 x NaN is a term of all sums over rows.  Without a
+    target it is none."""
+    x, w, b, t = ce_inputs(m, k, n, 52)
+    t = np.abs(t) % n
+    lse = T.dense_cross_entropy(dev(x), dev(w), dev(t), dev(b))[1]
+    x[3, 7] = np.nan
+    dloss = np.ones(m, np.float32)
+    dloss[3] = 0.0
+    dx, dw, db = (a.numpy() for a in T.dense_cross_entropy_grad(dev(x), dev(w), dev(t), lse, dev(b), dev(dloss)))
+    rest = [r for r in range(m) if r != 3]
+    assert np.isnan(dx[3]).all() and np.isfinite(dx[rest]).all() and np.isnan(dw).all() and np.isnan(db).all()
+    t[3] = -1
+    dx, dw, db = (a.numpy() for a in T.dense_cross_entropy_grad(dev(x), dev(w), dev(t), lse, dev(b), dev(dloss)))
+    assert not dx[3].any() and not np.signbit(dx[3]).any() and np.isfinite(dx).all() and np.isfinite(dw).all() and np.isfinite(db).all()
