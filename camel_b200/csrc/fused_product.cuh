@@ -55,8 +55,12 @@ __device__ __forceinline__ void split2(float a, float b, __half2 &hi, __half2 &l
     const float da = __fmul_rn(__fsub_rn(a, __low2float(hi)), kLoScale), db = __fmul_rn(__fsub_rn(b, __high2float(hi)), kLoScale);
     lo = __floats2half2_rn(fabsf(a) < INFINITY ? da : 0.0f, fabsf(b) < INFINITY ? db : 0.0f);
 }
-// The weight of an accumulated value: the product of two inverse scales, kept finite so that a sum of zero stays zero.
-__device__ __forceinline__ float weight(float row, float col) { return fminf(__fmul_rn(row, col), 1.7014118346e38f); }
+// The weight of an accumulated value: the product of two inverse scales, kept finite (2^127) so that a sum of zero stays zero; NaN stays.
+__device__ __forceinline__ float weight(float row, float col) {
+    float w;
+    asm("min.NaN.f32 %0, %1, 0f7F000000;" : "=f"(w) : "f"(__fmul_rn(row, col)));
+    return w;
+}
 #endif
 
 // Sizes that tile coordinates of 32 bits hold, two matrices side by side and what is rounded up included.
@@ -513,7 +517,9 @@ struct Store {
         const int rows     = left < 0 ? 0 : (left < 32 ? (int)left : 32);
         if (rows == 0)
             return;
-        const float rs = lane < rows ? __fadd_rn(__ldg(p.row_scale + row0 + lane), 0.0f) : 0.0f; // kNoPart: a row of +0
+        // kNoPart: a row of +0.  Other than scales, a row's weight may be infinite: its sums, of terms of both signs, are then NaN.
+        float rs = lane < rows ? __fadd_rn(__ldg(p.row_scale + row0 + lane), 0.0f) : 0.0f;
+        rs       = fabsf(rs) < INFINITY ? rs : NAN;
 #pragma unroll
         for (int g = 0; g < COLS / 16; ++g) {
             const int64_t col = col0 + g * 16;

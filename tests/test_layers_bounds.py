@@ -51,3 +51,21 @@ def test_cross_entropy_rows_of_zero_weight_count(m, k, n):
     t[3] = -1
     dx, dw, db = (a.numpy() for a in T.dense_cross_entropy_grad(dev(x), dev(w), dev(t), lse, dev(b), dev(dloss)))
     assert not dx[3].any() and not np.signbit(dx[3]).any() and np.isfinite(dx).all() and np.isfinite(dw).all() and np.isfinite(db).all()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("m,k,n", [(5, 40, 70), (40, 40, 70), (200, 40, 70), (200, 40, 10), (1500, 33, 300)])
+def test_cross_entropy_weights_that_are_no_numbers(m, k, n, bad):
+    """dloss that is NaN or infinite shows in its row of dx, also where the weights are zero, and in all of dw and db; other rows keep theirs."""
+    x, w, b, t = ce_inputs(m, k, n, 53)
+    t = np.abs(t) % n
+    w[5] = 0.0
+    lse = T.dense_cross_entropy(dev(x), dev(w), dev(t), dev(b))[1]
+    dloss = np.ones(m, np.float32)
+    clean = [a.numpy() for a in T.dense_cross_entropy_grad(dev(x), dev(w), dev(t), lse, dev(b), dev(dloss))]
+    dloss[3] = bad
+    dx, dw, db = (a.numpy() for a in T.dense_cross_entropy_grad(dev(x), dev(w), dev(t), lse, dev(b), dev(dloss)))
+    rest = [r for r in range(m) if r != 3]
+    assert (np.isnan(dx[3]).all() if np.isnan(bad) else not np.isfinite(dx[3]).any()) and not np.isfinite(dw).any() and not np.isfinite(db).any()
+    assert np.abs(dx[rest] - clean[0][rest]).max() <= 1e-6 * np.abs(clean[0]).max()
