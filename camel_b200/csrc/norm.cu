@@ -593,8 +593,14 @@ ct_status ct_layer_norm_grad(
             CT_TRY(scratch.get(stats_bytes + (size_t)parts * 8 * cols));
         float2 *stats  = sums ? scratch.as<float2>() : nullptr;
         float *partial = sums ? scratch.as<float>(stats_bytes) : nullptr;
-        CT_CUDA(launch_dependent(layer_norm_grad_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx, stats));
-        CT_LAUNCH_CHECK("layer_norm_grad_long");
+        auto rows_pass = [&](float *dx_to, float2 *stats_to) -> ct_status {
+            CT_CUDA(launch_dependent(layer_norm_grad_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx_to, stats_to));
+            CT_LAUNCH_CHECK("layer_norm_grad_long");
+            return CT_OK;
+        };
+        // dx in the place of x or dout, which the columns' sums read: it is written behind them, by a second pass
+        const bool behind = sums && (dx == x || dx == dout);
+        CT_TRY(rows_pass(behind ? nullptr : dx, stats));
         if (sums) {
             CT_CUDA(launch_dependent(layer_norm_grad_long_columns_kernel, dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, stream(), x, dout,
                                      static_cast<const float2 *>(stats), rows, cols, each, partial));
@@ -603,6 +609,8 @@ ct_status ct_layer_norm_grad(
                                      static_cast<const float *>(partial), (int)parts, cols, dgamma, dbeta));
             CT_LAUNCH_CHECK("norm_columns");
         }
+        if (behind)
+            CT_TRY(rows_pass(dx, nullptr));
         return CT_OK;
     }
     if (sums) {

@@ -362,7 +362,7 @@ ct_status ct_dense_packed(
 ct_status ct_layer_norm(
     const float *x_dev, const float *gamma_dev, const float *beta_dev, int64_t rows, int64_t cols, double eps, float *out_dev);
 /* Its gradient from x and the gradient dout of its output: dx [rows][cols], dgamma and dbeta [cols], each may be null.  The
- * statistics are computed again from x.  dx may be x or dout itself (up to 8192 columns; longer rows: not with dgamma or dbeta). */
+ * statistics are computed again from x.  dx may be x or dout itself. */
 ct_status ct_layer_norm_grad(
     const float *x_dev, const float *gamma_dev, const float *dout_dev, int64_t rows, int64_t cols, double eps, float *dx_dev,
     float *dgamma_dev, float *dbeta_dev);

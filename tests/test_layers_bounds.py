@@ -6,7 +6,7 @@ import pytest
 
 import camel_b200._lib as L
 from camel_b200 import tensor as T
-from test_layers import ce_inputs, dev, gated_inputs
+from test_layers import ce_inputs, dev, gated_inputs, norm_inputs
 
 gpu = pytest.mark.gpu
 
@@ -69,3 +69,21 @@ def test_cross_entropy_weights_that_are_no_numbers(m, k, n, bad):
     rest = [r for r in range(m) if r != 3]
     assert (np.isnan(dx[3]).all() if np.isnan(bad) else not np.isfinite(dx[3]).any()) and not np.isfinite(dw).any() and not np.isfinite(db).any()
     assert np.abs(dx[rest] - clean[0][rest]).max() <= 1e-6 * np.abs(clean[0]).max()
+
+
+# ---- layer norm -----------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(70, 785), (300, 4096), (3, 8193), (300, 8193), (40, 12345)])
+@pytest.mark.parametrize("over", ["x", "dout"])
+def test_layer_norm_grad_over_an_input(rows, cols, over):
+    """dx in the place of x or of dout, with the columns' sums of both: the same bytes as beside them."""
+    x, gamma, _, dy = norm_inputs(rows, cols, 54)
+    want = [a.numpy() for a in T.layer_norm_grad(dev(x), dev(dy), dev(gamma))]
+    tx, td, g = dev(x), dev(dy), dev(gamma)
+    to = tx if over == "x" else td
+    dg, db = T.zeros([cols]), T.zeros([cols])
+    L.check(L.lib.ct_layer_norm_grad(tx.ptr, g.ptr, td.ptr, rows, cols, 1e-5, to.ptr, dg.ptr, db.ptr))
+    for a, b in zip((to, dg, db), want):
+        assert a.numpy().tobytes() == b.tobytes()
