@@ -4,12 +4,13 @@
 //   g = dy gamma,  dx = r (g - mean(g) - h mean(g h)),  dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
 //
 // Both are bound by memory (8 and 12 bytes a value) if a row is read once, so a row stays in the registers of the threads that
-// share it from the load to the store: a warp for short rows, a block for longer ones, and only rows of more than 32768
-// values (16384 on the way back) are read again, from L2.
+// share it from the load to the store: a warp for short rows, a block for longer ones.  Only rows of more than 32768 values (8192 on the
+// way back) are read again, three times in all and four.
 //
-// Sums are float32, each of at most a few dozen values before it meets the others in a tree.  The mean is taken twice: the sums
-// of d = x - m and of d^2, about the first mean m, come from one exchange, and what d leaves of a mean corrects m and the
-// variance.  Rows whose mean is large beside their spread keep the digits that float32 has of x - mean.
+// Sums along a row are float32, of at most 64 values before they meet in a tree (beyond 65536 columns: in 64 bits first).  Sums over rows are
+// float32 over at most kChainRows rows of a thread (kChainRowsLong above 8192 columns) and the up to 32 rows that a block has at a time, then 64 bits.  The
+// mean is taken twice: the sums of d = x - m and of d^2, about the first mean m, come from one exchange, and what d leaves of a mean corrects
+// m and the variance.  Rows whose mean is large beside their spread keep the digits that float32 has of x - mean.
 // The gradient takes them again from x, which it has in registers anyway, instead of reading them: one exchange more per row,
 // no statistics to keep.
 #include "common.cuh"
@@ -81,6 +82,36 @@ template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&s)[N]
     }
 }
 
+// The sums of N float32 terms over a thread's columns first, first + 1024, ...: add(c, s) puts the terms of column c into s.  CHAINED: they meet
+// 64 bits every 64 columns; 1000 x 100000 takes 307 us so, 291 in one chain, 1 x 100000 45 and 43.
+constexpr int64_t kChainColumns = 64 * 1024; // of a row, where one chain has 64 values
+template <bool CHAINED, int N, typename F> __device__ __forceinline__ void column_sums(float (&sums)[N], int64_t first, int64_t last, F &&add) {
+    float s[N] = {};
+    int64_t c  = first;
+    if (CHAINED) {
+        double all[N] = {};
+        while (last - c > kChainColumns) {
+#pragma unroll 8
+            for (int q = 0; q < 64; ++q, c += 1024)
+                add(c, s);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                all[j] += (double)s[j], s[j] = 0.0f;
+        }
+        for (; c < last; c += 1024)
+            add(c, s);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            s[j] = (float)(all[j] + (double)s[j]);
+    } else {
+        for (; c < last; c += 1024)
+            add(c, s);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        sums[j] = s[j];
+}
+
 // 1 / sqrt(var + eps) from the sums of d and d^2, and what d lacks of the mean.
 __device__ __forceinline__ float spread(float sum_d, float sum_dd, float inv_cols, float eps, float &rest) {
     rest            = __fmul_rn(sum_d, inv_cols);
@@ -143,6 +174,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
 }
 
 // Rows of any length, a block to a row, which is read three times.
+template <bool CHAINED>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t cols, float eps, float *__restrict__ out) {
     __shared__ float words1[1][32], words2[2][32];
@@ -150,17 +182,16 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(
     griddep_launch_dependents();
     const float *src     = x + (int64_t)blockIdx.x * cols;
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
-    float sum[1]         = {0.0f};
-    for (int64_t c = threadIdx.x; c < cols; c += 1024)
-        sum[0] = __fadd_rn(sum[0], src[c]);
+    float sum[1];
+    column_sums<CHAINED>(sum, threadIdx.x, cols, [&](int64_t c, float (&s)[1]) { s[0] = __fadd_rn(s[0], src[c]); });
     row_sums<1024>(sum, words1);
     const float mean = __fmul_rn(sum[0], inv_cols);
-    float s[2]       = {0.0f, 0.0f};
-    for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+    float s[2];
+    column_sums<CHAINED>(s, threadIdx.x, cols, [&](int64_t c, float (&s)[2]) {
         const float d = __fsub_rn(src[c], mean);
         s[0]          = __fadd_rn(s[0], d);
         s[1]          = __fmaf_rn(d, d, s[1]);
-    }
+    });
     row_sums<1024>(s, words2);
     float rest;
     const float r = spread(s[0], s[1], inv_cols, eps, rest);
@@ -224,6 +255,8 @@ template <int TPR> __device__ __forceinline__ void row_sync() {
 // exchanges, so the next two rows are on their way meanwhile: with the loads of a row issued when it was its turn, 16384 x 4096 took 177 us
 // and 60000 x 785 208.
 constexpr int kAhead = 3; // rows in shared memory, the one at work among them
+// Rows of a thread whose sums are one float32 chain: with more rows there are more blocks, as many turns of the machine as it takes.
+constexpr int64_t kChainRows = 256, kChainRowsLong = 64; // up to 8192 columns, and beyond
 // Values of a slot: a row, with what lies before and behind it in its 16-byte pieces.  Slots begin on 128-byte boundaries: 16 bytes off, 2048
 // aligned columns took 165 us for 140.
 template <int TPR, int V, bool VEC> constexpr int kSlot = 4 * V * TPR + (VEC ? 0 : 32);
@@ -344,6 +377,7 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
 }
 
 // Longer rows: the statistics and dx, a block to a row, then the columns' sums from both matrices again.
+template <bool CHAINED>
 __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t cols, float eps, float *__restrict__ dx,
     float2 *__restrict__ stats) {
@@ -353,19 +387,18 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(
     const int64_t row    = blockIdx.x;
     const float *src     = x + row * cols, *dy = dout + row * cols;
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
-    float sum[1]         = {0.0f};
-    for (int64_t c = threadIdx.x; c < cols; c += 1024)
-        sum[0] = __fadd_rn(sum[0], src[c]);
+    float sum[1];
+    column_sums<CHAINED>(sum, threadIdx.x, cols, [&](int64_t c, float (&s)[1]) { s[0] = __fadd_rn(s[0], src[c]); });
     row_sums<1024>(sum, words1);
     const float mean = __fmul_rn(sum[0], inv_cols);
-    float s[4]       = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t c = threadIdx.x; c < cols; c += 1024) {
+    float s[4];
+    column_sums<CHAINED>(s, threadIdx.x, cols, [&](int64_t c, float (&s)[4]) {
         const float d = __fsub_rn(src[c], mean), g = gamma ? __fmul_rn(dy[c], gamma[c]) : dy[c];
         s[0] = __fadd_rn(s[0], d);
         s[1] = __fmaf_rn(d, d, s[1]);
         s[2] = __fadd_rn(s[2], g);
         s[3] = __fmaf_rn(g, d, s[3]);
-    }
+    });
     row_sums<1024>(s, words2);
     float rest;
     const float r  = spread(s[0], s[1], inv_cols, eps, rest);
@@ -453,7 +486,8 @@ ct_status launch_norm_grad(
         CT_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, kBlock<TPR>, SMEM));
         fit = std::max(fit, 1);
     }
-    *blocks = std::min<int64_t>((rows + RPB - 1) / RPB, (int64_t)st->sm_count * fit);
+    const int64_t turns = (rows + RPB - 1) / RPB, at_once = (int64_t)st->sm_count * fit;
+    *blocks = std::min(turns, at_once * ((turns + at_once * kChainRows - 1) / (at_once * kChainRows)));
     if (sums)
         CT_TRY(partial.get((size_t)*blocks * 8 * cols));
     CT_CUDA(launch_dependent(kernel, dim3((unsigned)*blocks), dim3(kBlock<TPR>), SMEM, stream(), x, gamma, dout, rows, cols, eps, dx,
@@ -527,7 +561,8 @@ ct_status ct_layer_norm(
         return launch_norm<1024, 4>(x, gamma, beta, rows, cols, e, out, vec);
     if (cols <= 32768)
         return launch_norm<1024, 8>(x, gamma, beta, rows, cols, e, out, vec);
-    CT_CUDA(launch_dependent(layer_norm_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out));
+    auto kernel = cols <= kChainColumns ? layer_norm_long_kernel<false> : layer_norm_long_kernel<true>;
+    CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out));
     CT_LAUNCH_CHECK("layer_norm_long");
     return CT_OK;
 }
@@ -584,17 +619,18 @@ ct_status ct_layer_norm_grad(
 #undef CT_NORM_GRAD
     } else {
         const int64_t strips = (cols + 255) / 256;
-        const int64_t each   = std::max<int64_t>(8, (rows * strips + st->sm_count * 8 - 1) / (st->sm_count * 8));
-        parts                = (rows + each - 1) / each;
-        if (parts > 65535)
-            return fail(CT_ERR_TOO_LARGE, "layer_norm_grad: too many rows");
+        // parts for eight blocks to an SM, of 8 rows at least and kChainRowsLong at most, or as many as a grid has
+        const int64_t fill = (rows * strips + st->sm_count * 8 - 1) / (st->sm_count * 8);
+        const int64_t each = std::max(std::min(std::max<int64_t>(8, fill), kChainRowsLong), (rows + 65534) / 65535);
+        parts              = (rows + each - 1) / each;
         const size_t stats_bytes = ((size_t)rows * 16 + 255) & ~(size_t)255;
         if (sums)
             CT_TRY(scratch.get(stats_bytes + (size_t)parts * 8 * cols));
         float2 *stats  = sums ? scratch.as<float2>() : nullptr;
         float *partial = sums ? scratch.as<float>(stats_bytes) : nullptr;
         auto rows_pass = [&](float *dx_to, float2 *stats_to) -> ct_status {
-            CT_CUDA(launch_dependent(layer_norm_grad_long_kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx_to, stats_to));
+            auto kernel = cols <= kChainColumns ? layer_norm_grad_long_kernel<false> : layer_norm_grad_long_kernel<true>;
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx_to, stats_to));
             CT_LAUNCH_CHECK("layer_norm_grad_long");
             return CT_OK;
         };

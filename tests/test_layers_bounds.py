@@ -6,7 +6,7 @@ import pytest
 
 import camel_b200._lib as L
 from camel_b200 import tensor as T
-from test_layers import ce_inputs, dev, gated_inputs, norm_inputs
+from test_layers import U, ce_inputs, dev, gated_inputs, norm_inputs
 
 gpu = pytest.mark.gpu
 
@@ -87,3 +87,55 @@ def test_layer_norm_grad_over_an_input(rows, cols, over):
     L.check(L.lib.ct_layer_norm_grad(tx.ptr, g.ptr, td.ptr, rows, cols, 1e-5, to.ptr, dg.ptr, db.ptr))
     for a, b in zip((to, dg, db), want):
         assert a.numpy().tobytes() == b.tobytes()
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,chain", [(1 << 26, 4, 256), (600000, 96, 256), (40000, 8193, 64), (300000, 8200, 64)])
+def test_layer_norm_grad_sums_of_many_rows(rows, cols, chain):
+    """Float32 sums of at most `chain` rows (up to 32 of them again), then 64 bits: beside ones, values that are half of a rounding each
+    are lost to a sum that goes on."""
+    import torch
+
+    if rows * cols > 1 << 30:
+        rows = (1 << 30) // cols
+    x = torch.randn(rows, cols, device="cuda")
+    dy = torch.full((rows, cols), 2.0 ** -25, device="cuda")
+    if cols <= 8192:
+        dy[:40000] = 1.0  # the first rows of all blocks
+    else:
+        dy[::max(8, -(-rows * -(-cols // 256) // 1184))] = 1.0  # of all parts
+    dg, db = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    torch.cuda.synchronize()
+    L.check(L.lib.ct_layer_norm_grad(x.data_ptr(), None, dy.data_ptr(), rows, cols, 1e-5, None, dg.data_ptr(), db.data_ptr()))
+    T.check_async()
+    want = torch.stack([part.double().sum(0) for part in dy.split(1 << 20)]).sum(0)
+    assert ((db.double() - want).abs() <= (chain + 32) * U * want).all()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1 << 17, (1 << 25) + 3])
+def test_layer_norm_of_very_long_rows(cols):
+    """Sums of at most 64 values, then 64 bits, then a tree of ten: squares of one size do not stop to count."""
+    import torch
+
+    x = torch.full((2, cols), 0.3, device="cuda")
+    x[:, ::2] = -0.3
+    x[1, 5] = 1000.0
+    dy = torch.randn(2, cols, device="cuda")
+    out, dx = torch.empty_like(x), torch.empty_like(x)
+    torch.cuda.synchronize()
+    L.check(L.lib.ct_layer_norm(x.data_ptr(), None, None, 2, cols, 1e-5, out.data_ptr()))
+    L.check(L.lib.ct_layer_norm_grad(x.data_ptr(), None, dy.data_ptr(), 2, cols, 1e-5, dx.data_ptr(), None, None))
+    T.check_async()
+    d, g = x.double(), dy.double()
+    d -= d.mean(1, keepdim=True)
+    r = 1 / (d.square().mean(1, keepdim=True) + float(np.float32(1e-5))).sqrt()
+    h = d * r
+    depth = 64 + 12
+    off_h = U * ((depth / 2 + 10) * h.abs() + (depth + 2) * d.abs().mean(1, keepdim=True) * r)
+    assert ((out.double() - h).abs() <= off_h).all()
+    mean_g, mean_gh = g.mean(1, keepdim=True), (g * h).mean(1, keepdim=True)
+    want = r * (g - mean_g - h * mean_gh)
+    mixed = (g.abs() * (h.abs() + 1)).mean(1, keepdim=True)
+    off = r * U * ((depth + 16) * (g.abs() + g.abs().mean(1, keepdim=True)) + 3 * (depth + 16) * (h.abs() + 1) * mixed)
+    assert ((dx.double() - want).abs() <= off).all()
