@@ -1,12 +1,15 @@
 """Layer norm, the gated dense layer and the cross entropy of a dense layer: what holds whatever the number of rows, and the kernels
 that only sizes beyond those of test_layers reach.  Definitions in 64 bits and bounds as there; tighter ones are derived here.
 """
+import math
+
 import numpy as np
 import pytest
 
 import camel_b200._lib as L
 from camel_b200 import tensor as T
-from test_layers import U, ce_inputs, dev, gated_inputs, norm_inputs
+from test_layers import (GATES, U, ce64, ce_inputs, check_gated, check_gated_grad, dev, gate64, gated_grad64, gated_inputs, norm_bounds, norm_grad64,
+                         norm_grad_bounds, norm_inputs, within)
 
 gpu = pytest.mark.gpu
 
@@ -139,3 +142,93 @@ def test_layer_norm_of_very_long_rows(cols):
     mixed = (g.abs() * (h.abs() + 1)).mean(1, keepdim=True)
     off = r * U * ((depth + 16) * (g.abs() + g.abs().mean(1, keepdim=True)) + 3 * (depth + 16) * (h.abs() + 1) * mixed)
     assert ((dx.double() - want).abs() <= off).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [600, 640])
+@pytest.mark.parametrize("cols", [300, 400, 512, 700, 850, 1024, 1500, 2048, 2050, 3001, 4092, 5000, 8192])
+def test_layer_norm_of_many_rows(rows, cols):
+    """From four rows to an SM on a row has fewer threads."""
+    x, gamma, beta, _ = norm_inputs(rows, cols, 55)
+    y, _, _, _, off = norm_bounds(x, gamma, beta, 1e-5)
+    within(T.layer_norm(dev(x), dev(gamma), dev(beta)).numpy(), y, off, "y")
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(300, 8193), (1000, 12345), (130, 40003), (1300, 500), (1300, 760), (1300, 890), (1300, 1000), (700, 7000)])
+def test_layer_norm_grad_in_parts(rows, cols):
+    """Rows above 8192 columns whose sums come from several parts; the forms of 1184 rows and more."""
+    x, gamma, _, dy = norm_inputs(rows, cols, 56)
+    want, off = norm_grad64(x, dy, gamma, 1e-5), norm_grad_bounds(x, dy, gamma, 1e-5, blocks=rows / 64)
+    for name, a, b, c in zip(("dx", "dgamma", "dbeta"), T.layer_norm_grad(dev(x), dev(dy), dev(gamma)), want, off):
+        within(a.numpy(), b, c, name)
+
+
+# ---- gated dense layer: the kernels of larger sizes --------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("m,k,n", [(1300, 130, 1100), (2100, 70, 523), (1281, 64, 1024), (5000, 33, 258)])
+def test_dense_gated_on_pairs(m, k, n, gate):
+    """Tiles of CTA pairs, each CTA of which has the columns of one matrix; ragged edges, with and without the sums kept."""
+    x, wg, wu, bg, bu = gated_inputs(m, k, n, 57)
+    check_gated(x, wg, wu, bg, bu, gate, keep=True)
+    check_gated(x, wg, wu, None, bu, gate, keep=False)
+
+
+@gpu
+@pytest.mark.parametrize("n", [130, 260, 1030, 1500, 2050, 4100, 5504, 8192, 8300, 12290])
+@pytest.mark.parametrize("m", [40, 700])
+def test_dense_gated_grad_of_wide_layers(m, n):
+    """Every form of the planes of d, rows that no block holds among them; without biases the other gradients have the same bytes."""
+    k = 24
+    x, wg, wu, _, _ = gated_inputs(m, k, n, 58)
+    g, u, dout = (np.random.default_rng(i).normal(0, 1, (m, n)).astype(np.float32) for i in range(3))
+    got = check_gated_grad(x, wg, wu, g, u, dout, "silu")
+    alone = T.dense_gated_grad(*[dev(a) for a in (x, wg, wu, g, u, dout)], gate="silu")
+    assert [a.numpy().tobytes() for a in alone] == [a.numpy().tobytes() for a in got[:3]]
+
+
+@gpu
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("m", [8, 40, 200])
+def test_slopes_at_the_ends(m, gate):
+    """Where the exponential is 0 or its argument overflows, value and slope are their limits."""
+    ends = np.array([-3e38, -1e30, -200.0, 200.0, 1e30, 3e38], np.float32)
+    limit = {"sigmoid": (0, 1, 0, 0), "relu": (0, None, 0, 1), "silu": (0, None, 0, 1), "gelu": (0, None, 0, 1)}[gate]  # value and slope, below and above
+    g = np.tile(ends, (m, 4))
+    n = g.shape[1]
+    one, x, w = np.ones((m, n), np.float32), np.zeros((m, 8), np.float32), np.zeros((8, n), np.float32)
+    _, _, _, dbg, dbu = (a.numpy() for a in T.dense_gated_grad(*[dev(a) for a in (x, w, w, g, one, one)], gate=gate, bias=True))
+    below, above = ends < 0, ends > 0
+    for i in range(4):
+        part = slice(6 * i, 6 * i + 6)
+        assert (dbu[part][below] == m * limit[0]).all()
+        assert (dbg[part][below] == m * limit[2]).all() and (dbg[part][above] == m * limit[3]).all()
+        if limit[1] is not None:
+            assert (dbu[part][above] == m * limit[1]).all()
+
+
+# ---- cross entropy ----------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("m", [2, 20, 200])
+def test_cross_entropy_of_very_many_classes(m):
+    """Sums of exponentials, of one size but for the target's: chains of at most 256 float32 terms."""
+    import torch
+
+    n = (1 << 24) + 40
+    x, w = torch.ones(m, 1, device="cuda"), torch.full((1, n), -1.2, device="cuda")
+    w[0, 7] = 0.0
+    t = torch.full((m,), 7, device="cuda")
+    loss, lse = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    torch.cuda.synchronize()
+    p = lambda a: a.data_ptr()  # noqa: E731
+    L.check(L.lib.ct_dense_cross_entropy(p(x), p(w), None, p(t), m, 1, n, p(loss), p(lse)))
+    T.check_async()
+    want = np.log1p((n - 1) * np.exp(-np.float64(np.float32(1.2))))
+    # a chain and the tree, exp and its argument, the logit of 1.2, the logarithm and the last addition
+    off = U * (256 + 32 + 12) + 2 * U * 1.2 + 3 * U * want
+    assert np.abs(lse.double().cpu().numpy() - want).max() <= off
