@@ -8,7 +8,8 @@
 // Gradient: the same product again, whose epilogue turns the logits into d / dloss = exp(z - lse) - [target], in [-1, 1], as planes of float16
 // pairs under one scale.  A piece of the vocabulary at a time they are the left operand of dx += d . w^T as they lie (rows weighted by
 // dloss at the end), and the right operand of dw = x'^T . d with their rows as k, x' being x with dloss in its rows.
-// A pair holds d to 2^-22 of itself, and to 2^-51 of 1.
+// A pair holds d / dloss to 2^-23 of itself down to 2^-28, and to 2^-50 below: one scale for all, since a row's largest, 1 - p[target], is known
+// only behind its last tile, and rows meet columns of any size in dw.
 // Up to 16 rows have their logits written, and take few_rows.cu and few_rows_grad.cuh.
 // Few classes (kFewClasses) take kernels of their own, whose logits are memory's smallest part; under the reduced precision the logits of a
 // piece of the rows are written, by the library's products.
@@ -134,7 +135,9 @@ __global__ void __launch_bounds__(256) ce_slopes_kernel(
 
 // ---- logits that stay in the epilogue ----
 
-__device__ __forceinline__ float exp2_fast(float x) { // 2^x, to 2^-22 of itself; 0 below 2^-126
+// 2^x, to 2^-22 of itself; 0 below 2^-126.  Its argument is a rounded product with a rounded constant: three roundings of |z - lse| in all, about as
+// many as the logit has of its own, so they are not taken back.
+__device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
@@ -345,7 +348,7 @@ ct_status ce_fused(
 
 // ---- the gradient ----
 
-constexpr float kSlopeScale = 16384.0f; // 2^14: d / dloss is at most 1
+constexpr float kSlopeScale = 16384.0f; // 2^14: d / dloss is at most 1, and representable up to 3.99
 
 // Logits to the planes of (exp(z - lse) - [target]) 2^14.
 struct Slopes {

@@ -5,7 +5,8 @@
 // the largest magnitude of its line to [2^14, 2^15).  Three MMAs of kind::f16 per 16 values of k: lo.hi and hi.lo into an accumulator of
 // cross products (weight 2^-11), hi.hi into the leading one.  Here a pair holds what it can of every value - to 2^-23 of itself down to 2^-27 of
 // its line's largest, below that to 2^-50 of the largest - and nothing is listed apart, so that a line's bits depend on that line
-// alone: |error| <= 2^-22 sum |a||b| + 2^-49 max|a| max|b| k, and the additions'.  Scales take any exponent.
+// alone: |error| <= 2^-21 sum |a||b| (2^-23 of each value, 2^-22 the lo.lo left out) + 2^-48 max|a| max|b| k, and the additions'.  Scales take
+// any exponent.
 //
 // The tensor core truncates at every addition, always towards zero, which shows in sums of one sign as a bias: the leading
 // accumulator is drained into registers every 128 values of k (8 additions) and summed there with rounding.  The drain has the

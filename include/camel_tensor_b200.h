@@ -353,9 +353,11 @@ ct_status ct_dense_packed(
  * weighted by the given gradient of the output; outputs that are null are not computed.  Dimensions go up to 2^29.
  *
  * Products of more than 16 rows hold each operand as pairs of float16 under one power of two per row (or per column, where rows are summed
- * over): to 2^-23 of a value down to 2^-27 of its line's largest, to 2^-50 of that largest below.  The error of a sum is at most 2^-22 of
- * its products' sizes and 2^-49 of its length times the two lines' largest, and the additions'.  A sum that meets an infinity of an
- * operand is infinite or NaN (infinity times a low term of zero).  Under CT_PREC_BF16 the products are those of ct_dense. */
+ * over): to 2^-23 of a value down to 2^-27 of its line's largest, to 2^-50 of that largest below; the product of two low terms is left out.
+ * The error of a sum is at most 2^-21 of its products' sizes and 2^-48 of its length times the two lines' largest, and the additions' (by
+ * 16 terms to 2^-23, by 128 to 2^-24, in float32).  Unlike ct_dense's, lines of a wider range are not computed another way.  A sum
+ * that meets an infinity of an operand is infinite or NaN (infinity times a low term of zero).  Under CT_PREC_BF16 the products
+ * are those of ct_dense. */
 
 /* Layer norm of each row: out = (x - mean) / sqrt(var + eps) * gamma + beta, mean and var (the mean square deviation) over the
  * row's `cols` values.  gamma and beta have one value per column; null: ones, zeros.  eps >= 0.  out may be x itself. */
@@ -387,11 +389,12 @@ ct_status ct_dense_gated_grad(
 ct_status ct_dense_cross_entropy(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, int64_t m, int64_t k, int64_t n,
     float *loss_dev, float *lse_dev);
-/* Its gradient, with lse as the forward call left it (exp(z - lse) up to 4 is represented) and the gradient dloss [m] of the losses
- * (null: ones):
+/* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
  *   d[i][j] = dloss[i] * (exp(z[i][j] - lse[i]) - (j == targets[i])), zero in rows without a target,
  *   dx = d . w^T, dw = x^T . d, dbias the columns' sums of d.  The logits are computed again, in pieces.  A row without a target takes
- * no part in the sums, whatever x and dloss hold there. */
+ * no part in the sums, whatever x and dloss hold there.
+ * Of more than 16 rows and 16 classes d / dloss is held as pairs under one scale for all: to 2^-23 of itself down to 2^-28, below that to
+ * 2^-50 (a class of probability 2^-40 in every row has 2^-10 of its column of dw and of dbias); exp(z - lse) up to 3.99 is represented. */
 ct_status ct_dense_cross_entropy_grad(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, const float *lse_dev,
     const float *dloss_dev, int64_t m, int64_t k, int64_t n, float *dx_dev, float *dw_dev, float *dbias_dev);
