@@ -4,7 +4,7 @@
 //   g = dy gamma,  dx = r (g - mean(g) - h mean(g h)),  dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
 //
 // Both are bound by memory (8 and 12 bytes a value) if a row is read once, so a row stays in the registers of the threads that
-// share it from the load to the store: a warp for short rows, a block for longer ones.  Only rows of more than 32768 values (8192 on the
+// share it from the load to the store: a warp for short rows, a block for longer ones.  Only rows of more than 16384 values (8192 on the
 // way back) are read again, three times in all and four.
 //
 // Sums along a row are float32, of at most 64 values before they meet in a tree (beyond 65536 columns: in 64 bits first).  Sums over rows are
@@ -526,7 +526,14 @@ ct_status ct_layer_norm(
     ProfScope prof("layer_norm");
     const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(out) && (!gamma || aligned16(gamma)) && (!beta || aligned16(beta));
     const float e  = (float)eps;
-    const bool few = rows < st->sm_count * 4;
+    // Threads to a row and float4 to a thread, measured (us; 200 calls in line, or many rows with L2 flushed):
+    //   512 columns: a warp 1.7, 256 threads 1.9 (1 row), 2.1 and 2.3 (500), 18 and 37 (16384)
+    //   1024: a warp 2.9, 256 threads 2.0 (16 rows), 3.0 and 2.5 (500), 31 and 41 (16384); 768: 2.6 and 2.0 (16 rows), 2.8 and 2.4 (500)
+    //   785: 7 float4 88, 8 94 (60000 rows); 896: 84 and 86; 640: 6 float4 59, 7 75
+    //   2048: 128 threads 2.0, 256 2.1, 1024 2.4 (1 row), 2.9, 3.0, 6.1 (500), 49, 53, 155 (16384)
+    //   4095: 128 threads 57, 256 68, 1024 107 (8000 rows); 4096: 2.4, 2.4, 2.6 (1 row), 51, 52, 88 (8000)
+    //   8192: 256 threads 3.1, 512 3.1, 1024 3.4 (1 row), 7.5, 7.7, 9.7 (500), 58, 59, 66 (4000)
+    //   16384: in registers 8, read three times 12 (50 rows), 105 and 104 (3000); 24576: 16 and 14 (50), 125 and 84 (1500)
 #define CT_NORM(TPR, V) launch_norm<TPR, V>(x, gamma, beta, rows, cols, e, out, vec)
     if (cols <= 32)
         return CT_NORM(8, 1);
@@ -536,31 +543,25 @@ ct_status ct_layer_norm(
         return CT_NORM(16, 2);
     if (cols <= 256)
         return CT_NORM(32, 2);
-    if (few && cols <= 1024) // a row spread over more threads is there sooner
-        return CT_NORM(256, 1);
     if (cols <= 512)
         return CT_NORM(32, 4);
+    if (cols <= 1024 && rows < st->sm_count * 4)
+        return CT_NORM(256, 1);
     if (cols <= 768)
         return CT_NORM(32, 6);
     if (cols <= 896)
         return CT_NORM(32, 7);
     if (cols <= 1024)
         return CT_NORM(32, 8);
-    if (few && cols <= 4096)
-        return CT_NORM(1024, 1);
     if (cols <= 2048)
         return CT_NORM(128, 4);
     if (cols <= 4096)
-        return vec ? CT_NORM(256, 4) : CT_NORM(128, 8);
-    if (few && cols <= 8192)
-        return CT_NORM(1024, 2);
+        return CT_NORM(128, 8);
     if (cols <= 8192)
         return CT_NORM(256, 8);
-#undef CT_NORM
     if (cols <= 16384)
-        return launch_norm<1024, 4>(x, gamma, beta, rows, cols, e, out, vec);
-    if (cols <= 32768)
-        return launch_norm<1024, 8>(x, gamma, beta, rows, cols, e, out, vec);
+        return CT_NORM(1024, 4);
+#undef CT_NORM
     auto kernel = cols <= kChainColumns ? layer_norm_long_kernel<false> : layer_norm_long_kernel<true>;
     CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out));
     CT_LAUNCH_CHECK("layer_norm_long");
@@ -589,6 +590,9 @@ ct_status ct_layer_norm_grad(
     int64_t parts = 0;
     if (cols <= 8192) {
         const bool vec = (cols & 3) == 0 && aligned16(x) && aligned16(dout) && (!dx || aligned16(dx)) && (!gamma || aligned16(gamma));
+        // measured (us, L2 flushed): 512 columns a warp 31, 256 threads 62 (16384 rows), 17 and 21 (1000), 15 and 15 (300); 1024: 51 and 64 (16384
+        // rows), 22 and 24 (1300), 19 and 17 (300); 785: 7 float4 to a lane 127, 8 138 (60000 rows), 896: 125 and 123; 640: 6 88, 7 97; 2048: 256
+        // threads 86, 512 113 (16384 rows); 4096: 256 threads 80, 512 88 (8000 rows); 8192: 512 threads 88, 1024 92 (4000 rows)
 #define CT_NORM_GRAD(TPR, V)                                                                                                      \
     CT_TRY(vec ? (launch_norm_grad<TPR, V, true>(st, x, gamma, dout, rows, cols, e, dx, sums, scratch, &parts))                  \
                : (launch_norm_grad<TPR, V, false>(st, x, gamma, dout, rows, cols, e, dx, sums, scratch, &parts)))
