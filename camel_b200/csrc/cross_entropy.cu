@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(
     }
 }
 
-// 17 to 128 rows: a thread has every sixteenth of a row's logits, and keeps maximum and sum across the CTA's tiles.
+// Streamed: a thread has every sixteenth of a row's logits, and keeps maximum and sum across the CTA's tiles.
 struct SumExpStream {
     static constexpr bool kTwin  = false;
     static constexpr int kShares = fused::kStreamDrain * 32 / fused::kStreamPass;
@@ -311,7 +311,7 @@ ct_status ce_fused(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, int64_t m, int64_t k, int64_t n, float *loss, float *lse) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    const bool few = m <= kStreamRows, pair = !few && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
+    const bool few = takes_stream(m, n), pair = !few && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
     int per;
     const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
@@ -410,7 +410,7 @@ struct Slopes {
     }
 };
 
-// 17 to 128 rows: a warp has a row of a tile at a time, a lane four of its columns.
+// Streamed (without dx): a warp has a row of a tile at a time, a lane four of its columns.
 struct SlopesStream {
     static constexpr bool kTwin = false;
     using Params = Slopes::Params;
@@ -460,7 +460,9 @@ ct_status ce_grad_fused(
     int64_t n, float *dx, float *dw, float *dbias) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    const bool few = m <= kStreamRows;
+    // dx needs the weights' planes in any case, and with them tiles are sooner (20 x 1024 x 8192 78 us, streamed 89; 64 x 32000 both 222; 20 x 32000 215
+    // and 209); without it 64 x 32000 takes 127 streamed, 186 by tiles.
+    const bool few = !dx && takes_stream(m, n);
     // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
     const int64_t pieces = (n + most - 1) / most;
@@ -469,7 +471,7 @@ ct_status ce_grad_fused(
     // The weights' planes for dx have a scale per row; with those folded into x they are the logits' as well, which saves a pre-pass over the
     // weights (1000 x 512 x 50257: 639 us, so 575) and keeps what features of different sizes meet.
     const size_t xp = parts.planes(m, lk), xi = parts.take((size_t)m * 4), dp = parts.planes(m, ld), rw = parts.take((size_t)m * 4);
-    const bool weights = dx || !few;
+    const bool weights = !few;
     const size_t wp = weights ? parts.planes(k, ln) : 0, wi = weights ? parts.take((size_t)scales(k) * 4) : 0;
     const size_t yp = dw ? parts.planes(m, lk) : 0, yi = dw ? parts.take((size_t)scales(lk) * 4) : 0;
     Scratch s;

@@ -1,7 +1,7 @@
 // Gated dense layer: out = gate(x . w_gate + b_gate) * (x . w_up + b_up), and its gradient.
 //
 // Forward: one product whose tiles have the same columns of both weight matrices (fused_product.cuh); a thread of the epilogue
-// has both sums of an output and stores what the layer gives.  Up to 8 or 16 rows (takes_few_rows): few_rows.cu; up to 128: stream_product.cuh.
+// has both sums of an output and stores what the layer gives.  Up to 8 or 16 rows (takes_few_rows): few_rows.cu; up to 128: stream_product.cuh (takes_stream).
 // Gradient: gated_slope_planes_kernel turns dout and what was kept into the planes of d = [dg | du], scaled by row; they are the left operand of
 // dx = d . [w_gate | w_up]^T as they lie, and the right operand of dw = x'^T . d with their rows as k, x' being x with the rows' scales
 // taken back.  So d is written once, 8 bytes for each of its values' pairs of terms, and read in place.
@@ -91,7 +91,7 @@ template <int GATE> struct GateEpilogue {
     }
 };
 
-// 17 to 128 rows: a warp has a row of a tile's results at a time.
+// Streamed: a warp has a row of a tile's results at a time.
 template <int GATE> struct GateStream {
     static constexpr bool kTwin = true;
     struct Params {
@@ -494,7 +494,7 @@ ct_status ct_dense_gated(
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
         if (fused::takes_few_rows(m, 2 * n))
             return fused::few_rows(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
-        if (m <= fused::kStreamRows)
+        if (fused::takes_stream(m, 2 * n))
             return gated_stream(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
         return gated_fused(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
     }

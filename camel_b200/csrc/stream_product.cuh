@@ -1,4 +1,4 @@
-// Products of 17 to 128 rows: the weights are streamed through the tensor cores as they lie, float32, and read once.
+// Products of 17 to 128 rows (takes_stream): the weights are streamed through the tensor cores as they lie, float32, and read once for 64 rows.
 //
 // With so few rows a product is as long as it takes to read the weights, and writing their planes and reading them again is three times that
 // (64 x 1024 x 32003: 76 us of pre-pass, 33 of product; here 63 in all).  So four warps fetch the weights, 64 values of k of 128 columns a stage
@@ -21,7 +21,12 @@
 namespace ct {
 namespace fused {
 
-constexpr int64_t kStreamRows = 128; // at most, 64 a launch
+// Whether a product of more than 16 rows is streamed, `columns` those of both matrices: a CTA has an even share of them, of at least 16, and tiles of
+// 128 are the emptier the fewer there are; of more than 64 rows the weights are read twice.  Streamed, and by tiles of planes (us, k = 1024, cross entropy):
+// 64 rows x 1000 39 and 35, x 4096 39 and 37, x 8192 41 and 45, x 32000 63 and 129; 128 rows x 8192 68 and 47, x 16384 72 and 78, x 32000 111 and
+// 130; gated, two matrices of n: 64 x 1000 35 and 33, x 2048 35 and 33 (k = 4096 92 and 118), x 8192 39 and 62; 128 x 8192 68 and 62 (k = 2048 105
+// and 182), x 16384 115 and 111, x 32000 189 and 199.
+inline bool takes_stream(int64_t m, int64_t columns) { return m <= 64 ? columns >= 4096 : m <= 128 && columns >= 16384; }
 constexpr int kStreamSlots   = 2;
 // Warps: of a stage fetched by the warps that convert it all did the same at the same time, and a stage of 64 x 1024 x 128000 took 3350 clocks.
 constexpr int kStreamDrain = 8, kStreamFetch = 4, kStreamConvert = 8; // kStreamConvert: of a group
@@ -456,7 +461,7 @@ ct_status launch_stream_of(DeviceState *st, const Planes &x, Stream p, const typ
     CT_LAUNCH_CHECK(name);
     return CT_OK;
 }
-// Rows of x as planes [m][k], m <= kStreamRows.  rows_from(e, r): the parameters for the rows from r on.
+// Rows of x as planes [m][k], 64 a launch.  rows_from(e, r): the parameters for the rows from r on.
 template <class EPI, typename F>
 ct_status launch_stream(DeviceState *st, const Planes &x, Stream p, const typename EPI::Params &e, const char *name, F &&rows_from) {
     const float *row_scale = p.row_scale;
