@@ -311,7 +311,7 @@ ct_status ce_fused(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, int64_t m, int64_t k, int64_t n, float *loss, float *lse) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    const bool few = takes_stream(m, n), pair = !few && (m + 255) / 256 * ((n + 255) / 256) * 4 >= st->sm_count;
+    const bool few = takes_stream(m, n), pair = !few && takes_pairs(st, m, n);
     int per;
     const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
@@ -460,8 +460,8 @@ ct_status ce_grad_fused(
     int64_t n, float *dx, float *dw, float *dbias) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    // dx needs the weights' planes in any case, and with them tiles are sooner (20 x 1024 x 8192 78 us, streamed 89; 64 x 32000 both 222; 20 x 32000 215
-    // and 209); without it 64 x 32000 takes 127 streamed, 186 by tiles.
+    // dx needs the weights' planes in any case, and with them tiles are sooner (20 x 1024 x 8192 78 us, streamed 89; 40 x 32000 205
+    // and 219); without it 64 x 32000 takes 127 streamed, 186 by tiles.
     const bool few = !dx && takes_stream(m, n);
     // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
@@ -510,7 +510,7 @@ ct_status ce_grad_fused(
             Product p{};
             p.m = m, p.n = cols, p.row_scale = s.as<float>(xi);
             const Planes right = columns_of(pw, c, cols);
-            const bool pair    = (m + 255) / 256 * ((cols + 255) / 256) * 4 >= st->sm_count;
+            const bool pair    = takes_pairs(st, m, cols);
             CT_TRY(pair ? (launch<Slopes, 256, 2, false, true>(st, px, right, p, e, 1, "cross_entropy_grad"))
                         : (launch<Slopes, 128, 1, false, true>(st, px, right, p, e, 1, "cross_entropy_grad")));
         }

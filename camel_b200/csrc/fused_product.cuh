@@ -602,6 +602,12 @@ ct_status launch(DeviceState *st, const Planes &a, const Planes &b, Product p, c
     return CT_OK;
 }
 
+// Pairs of CTAs with tiles of 256 x 256 (of both matrices, twin), or single ones with 128 x 128: pairs from where those are more than the machine
+// has at a time and there are rows for both.  Single and pairs (us, k = 1024; cross entropy): 300 x 4736 (111 single tiles) 40 and 51, 512 x 4096 (128) 39 and 49, 768 x
+// 3200 (150) 47 and 49, 512 x 8192 (256) 62 and 60, 1024 x 8192 84 and 81; gated 512 x 2048 (128) 37 and 47, 512 x 4096 58 and 58, 2048 x 5504 158 and 151;
+// 128 x 32000, gradient, 215 and 232.
+inline bool takes_pairs(const DeviceState *st, int64_t m, int64_t columns) { return m > 128 && (m + 127) / 128 * ((columns + 127) / 128) > st->sm_count; }
+
 #endif // __CUDACC__
 
 // ---- fused_product.cu ----------------------------------------------------------------------------

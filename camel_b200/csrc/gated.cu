@@ -169,9 +169,7 @@ ct_status gated_fused(
     return with_gate(gate, [&](auto G) -> ct_status {
         using E = GateEpilogue<G.value>;
         typename E::Params e{b_gate, b_up, out, gate_pre, up_pre, (n & 3) == 0 && whole(out) && whole(gate_pre) && whole(up_pre) ? 1 : 0};
-        // pairs where their tiles fill at least half of the machine
-        const int64_t tiles = (m + 255) / 256 * ((n + 127) / 128);
-        return m > 128 && tiles * 4 >= st->sm_count ? launch<E, 256, 2, false, true>(st, px, pw, p, e, 1, "dense_gated")
+        return takes_pairs(st, m, 2 * n) ? launch<E, 256, 2, false, true>(st, px, pw, p, e, 1, "dense_gated")
                                                     : launch<E, 128, 1, false, true>(st, px, pw, p, e, 1, "dense_gated");
     });
 }
