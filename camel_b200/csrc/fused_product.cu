@@ -114,6 +114,8 @@ __device__ __forceinline__ void split_rows(const Source &src, int64_t width, con
 
 // 16 columns to the block, four lanes to a row; at most kShort rows of 64 to a thread.
 constexpr int kShort = 16;
+// Values that split_small_kernel takes: gated 1024 x 1024 x 500 (2.1 M) 32 us so, 33 by two launches, 1500 x 600 x 300 (1.3 M) 27 and 29, 1024 x 1024 x
+// 1000 (3.1 M) 39 and 36, but both products' operands of a gradient of 2^21 21 and 14.
 constexpr int64_t kFewValues = 1 << 20;
 __device__ __forceinline__ void split_short_cols(
     const Source &src, int64_t width, const float *row_factor, const Planes &to, float *inverse, int64_t block, uint32_t (&words)[8][16]) {
