@@ -196,6 +196,13 @@ class Scratch {
     cudaStream_t stream_;
 };
 
+// Blocks of a kernel whose blocks walk `turns` of something and keep float32 sums: `at_once` (what the machine holds) or fewer, and where a block had more
+// than `chain` turns, that many times more.
+inline int64_t blocks_for(int64_t turns, int64_t at_once, int64_t chain) {
+    const int64_t waves = (turns + at_once * chain - 1) / (at_once * chain), blocks = at_once * waves;
+    return turns < blocks ? turns : blocks;
+}
+
 inline size_t dtype_size(int dt) { return dt == CT_F32 ? 4 : (dt == CT_I64 ? 8 : 1); }
 inline bool valid_dtype(int dt) { return dt == CT_F32 || dt == CT_I64 || dt == CT_BOOL; }
 

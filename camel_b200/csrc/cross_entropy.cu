@@ -539,6 +539,8 @@ ct_status ce_grad_fused(
 // From 17 classes on the tiles of 128 win, empty as most of them is: gradient of 60000 x 785 x 17 494 us against 1626 (the library's products
 // of more than 16 columns read x in many strips), of 2000 x 256 x 20 54 against 50.  At 10 classes the kernels below take 170 us, tiles as much as at 17.
 constexpr int kFewClasses = 16;
+// Rows of a block whose sums are one float32 chain, at most (60000 rows: 400).
+constexpr int64_t kChainFew = 1024;
 
 // A thread per row.
 __global__ void __launch_bounds__(256) ce_few_kernel(
@@ -603,7 +605,7 @@ __global__ void __launch_bounds__(256) ce_few_slopes_kernel(
 
 // dx = d . w^T and the parts of dw = x^T . d in one reading of x and d: a thread has a column of x, its weights and its sums in registers, 64
 // rows of d come from shared memory at a time.  Blocks are strips x parts; a part has every parts-th 64 rows.  A row without a target takes
-// no part, whatever x holds there.  Bound by issue, n FMAs of two values to a value of x.  Sums are chains of a part's rows, joined in 64 bits.
+// no part, whatever x holds there.  Bound by issue, n FMAs of two values to a value of x.  Sums are chains of a part's rows, kChainFew at most, joined in 64 bits.
 template <int N>
 __global__ void __launch_bounds__(256) ce_few_back_kernel(
     const float *__restrict__ d, const float *__restrict__ x, const float *__restrict__ w, const int64_t *__restrict__ targets, int64_t m, int64_t k, int n,
@@ -898,7 +900,7 @@ ct_status launch_ce_one(
         CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
         attr_set_dev[st->device & 15] = true;
     }
-    const int64_t grid = std::min<int64_t>((m + ROWS - 1) / ROWS, (int64_t)st->sm_count * (512 / THREADS)), width = k * n + n;
+    const int64_t grid = blocks_for((m + ROWS - 1) / ROWS, (int64_t)st->sm_count * (512 / THREADS), kChainFew / ROWS), width = k * n + n;
     Scratch partial;
     if (dw || dbias)
         CT_TRY(partial.get((size_t)(grid * width) * 8));
@@ -949,7 +951,7 @@ ct_status ce_few_grad(
     if (dbias)
         CT_TRY(fused::join_columns(s.as<const double>(pp), blocks, n, n, dbias, nullptr));
     if ((dw || dx) && k > 0) {
-        const int64_t strips = (k + 255) / 256, parts = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 4 / strips));
+        const int64_t strips = (k + 255) / 256, parts = std::max((m + kChainFew - 1) / kChainFew, std::min<int64_t>((m + 63) / 64, (int64_t)st->sm_count * 4 / strips));
         Scratch sums;
         if (dw)
             CT_TRY(sums.get((size_t)(parts * k * n) * 8));

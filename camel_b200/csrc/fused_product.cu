@@ -777,7 +777,7 @@ ct_status join_columns(const double *partial, int64_t parts, int64_t n, int64_t 
 
 ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight, float *out) {
     const int64_t strips = (x.cols + 255) / 256;
-    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((x.rows + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t slices = row_slices(st, x.rows, strips);
     const int64_t each = (x.rows + slices - 1) / slices, parts = (x.rows + each - 1) / each;
     Scratch partial;
     CT_TRY(partial.get((size_t)(parts * x.cols) * 8));

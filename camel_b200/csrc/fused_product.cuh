@@ -667,6 +667,12 @@ struct Wanted {
 };
 // One, or a K-major and an MN-major one.
 ct_status products(DeviceState *st, const Wanted *what, int count);
+// Slices of rows for sums over columns, a row to each of eight warps in turn: as many as six blocks to an SM, of 32 rows at least, and of 2048 at most
+// (chains of 256) while a grid has that many.
+inline int64_t row_slices(const DeviceState *st, int64_t rows, int64_t strips) {
+    const int64_t fill = std::min<int64_t>((rows + 31) / 32, (int64_t)st->sm_count * 6 / strips), least = std::max<int64_t>(1, (rows + 2047) / 2048);
+    return std::min<int64_t>(std::max(fill, least), 65535);
+}
 // out[c] = sum over the rows of row_weight[r] * planes[r][c].
 ct_status column_sums(DeviceState *st, const Planes &x, const float *row_weight, float *out);
 // first[c] = sum over parts of partial[part][c] for c < n, second[c] of partial[part][n + c] for n + c < width; either may be null.

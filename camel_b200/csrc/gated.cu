@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(256) gated_bias_kernel(
 ct_status gated_bias(
     DeviceState *st, const float *g, const float *u, const float *dout, int64_t m, int64_t n, int gate, int vec, float *db_gate, float *db_up) {
     const int64_t strips = (n + 127) / 128;
-    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((m + 31) / 32, 65535), (int64_t)st->sm_count * 6 / strips));
+    const int64_t slices = fused::row_slices(st, m, strips);
     const int64_t each = (m + slices - 1) / slices, parts = (m + each - 1) / each;
     Scratch partial; // of one part there is nothing to add up
     if (parts > 1)
@@ -372,7 +372,7 @@ ct_status launch_slopes_of(
         CT_LAUNCH_CHECK("gated_slopes");
         return CT_OK;
     }
-    blocks = std::min<int64_t>(blocks, (int64_t)st->sm_count * (TPR <= 256 ? 4 : 2));
+    blocks = blocks_for(blocks, (int64_t)st->sm_count * (TPR <= 256 ? 4 : 2), 256); // rows of a thread's sums
     Scratch partial;
     CT_TRY(partial.get((size_t)(blocks * RPB * 2 * n) * 8));
     CT_CUDA(launch_dependent(gated_slope_planes_kernel<GATE, TPR, V, true>, dim3((unsigned)blocks), dim3(TPR * RPB), 0, stream(), g, u, dout, m, n, vec, to,

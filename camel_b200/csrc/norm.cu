@@ -486,8 +486,7 @@ ct_status launch_norm_grad(
         CT_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, kBlock<TPR>, SMEM));
         fit = std::max(fit, 1);
     }
-    const int64_t turns = (rows + RPB - 1) / RPB, at_once = (int64_t)st->sm_count * fit;
-    *blocks = std::min(turns, at_once * ((turns + at_once * kChainRows - 1) / (at_once * kChainRows)));
+    *blocks = blocks_for((rows + RPB - 1) / RPB, (int64_t)st->sm_count * fit, kChainRows);
     if (sums)
         CT_TRY(partial.get((size_t)*blocks * 8 * cols));
     CT_CUDA(launch_dependent(kernel, dim3((unsigned)*blocks), dim3(kBlock<TPR>), SMEM, stream(), x, gamma, dout, rows, cols, eps, dx,

@@ -232,3 +232,59 @@ def test_cross_entropy_of_very_many_classes(m):
     # a chain and the tree, exp and its argument, the logit of 1.2, the logarithm and the last addition
     off = U * (256 + 32 + 12) + 2 * U * 1.2 + 3 * U * want
     assert np.abs(lse.double().cpu().numpy() - want).max() <= off
+
+
+# ---- sums over many rows --------------------------------------------------------------------------
+
+
+def first_of_chains(m, pick):
+    """Values that are half of a rounding beside one, and a one where a chain of sums begins: what follows it is lost to a chain that goes on."""
+    import torch
+
+    r = torch.arange(m, device="cuda")
+    return torch.where(pick(r), 1.0, 2.0 ** -25)
+
+
+@gpu
+@pytest.mark.parametrize("m,n,pick", [(1 << 22, 250, lambda r: r < 4736), (1 << 20, 1000, lambda r: r < 592), (1 << 20, 2050, lambda r: r < 296),
+                                      (1 << 17, 8200, lambda r: r % 10083 < 8)])
+def test_gated_bias_gradients_of_many_rows(m, n, pick):
+    """Float32 chains of at most 256 rows, which meet in 64 bits."""
+    import torch
+
+    k = 8
+    x, w = torch.zeros(m, k, device="cuda"), torch.zeros(k, n, device="cuda")
+    one = torch.ones(m, n, device="cuda")
+    rows = first_of_chains(m, pick)
+    dout = rows[:, None].expand(m, n).contiguous()
+    db = torch.empty(2, n, device="cuda")
+    torch.cuda.synchronize()
+    p = lambda a: a.data_ptr()  # noqa: E731
+    L.check(L.lib.ct_dense_gated_grad(p(x), p(w), p(w), p(one), p(one), p(dout), m, k, n, L.GATE_RELU, None, None, None, p(db[0]), p(db[1])))
+    T.check_async()
+    want = rows.double().sum().item()
+    assert ((db.double() - want).abs() <= (256 + 32) * U * want).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,chain,pick", [(1 << 23, 8, 32, 256, lambda r: r % 9447 < 8), (1 << 21, 16, 8, 1024, lambda r: (r % 8 == 0) & (r < 2368)),
+                                              (1 << 21, 16, 12, 1024, lambda r: (r % 16 == 0) & (r < 2368)),
+                                              (1 << 20, 1100, 8, 1024, lambda r: (r % 64 == 0) & (r < 118 * 64))])
+def test_cross_entropy_gradients_of_many_rows(m, k, n, chain, pick):
+    """db, and dw over few classes: float32 chains of at most `chain` rows."""
+    import torch
+
+    x, w, b = torch.ones(m, k, device="cuda"), torch.zeros(k, n, device="cuda"), torch.zeros(n, device="cuda")
+    t = torch.zeros(m, device="cuda", dtype=torch.int64)
+    lse = torch.full((m,), float(np.log(n)), device="cuda")
+    dloss = first_of_chains(m, pick)
+    dw, db = torch.empty_like(w), torch.empty_like(b)
+    torch.cuda.synchronize()
+    p = lambda a: a.data_ptr()  # noqa: E731
+    L.check(L.lib.ct_dense_cross_entropy_grad(p(x), p(w), p(b), p(t), p(lse), p(dloss), m, k, n, None, p(dw), p(db)))
+    T.check_async()
+    want = dloss.double().sum().item() / n
+    off = (chain + 32) * U + 2.0 ** -20  # and a probability: its exponent's rounding and its pair
+    assert ((db[1:].double() - want).abs() <= off * want).all()
+    if n <= 16:
+        assert ((dw[:, 1:].double() - want).abs() <= off * want).all()
