@@ -189,7 +189,6 @@ class Scratch {
         return CT_OK;
     }
     template <typename T> T *as(size_t offset = 0) const { return reinterpret_cast<T *>(static_cast<uint8_t *>(ptr_) + offset); }
-    explicit operator bool() const { return ptr_ != nullptr; }
 
   private:
     void *ptr_ = nullptr;

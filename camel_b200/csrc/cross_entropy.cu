@@ -911,7 +911,8 @@ ct_status launch_ce_one(
 }
 // Two blocks of eight warps to an SM, whose phases overlap, where both fit: up to 8 classes, whose columns then fit the registers, in shared memory
 // with two or three tiles of x, and enough rows to pay for as many blocks' beginnings (60000 x 785 x 8: 150 us with one, 135; 1000 x 785 x 10: 17
-// with one, 25).  Else one of sixteen (60000 x 785 x 10: 160, as two 185).
+// with one, 25).  Else one of sixteen (60000 x 785 x 10: 160, as two 185).  N is classes rounded up; nine and ten have a form of their own,
+// with a sixth fewer FMAs than that of twelve: 60000 x 785 x 10 166 so and 181, x 1024 x 10 189 and 203.
 template <int N>
 ct_status launch_ce_one_of(
     const DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, const float *lse, const float *dloss, int64_t m,

@@ -168,7 +168,7 @@ __device__ __forceinline__ void split_short_cols(
 }
 
 // Up to four matrices, each with its range of blocks.
-enum Form : int { kRowsWarp, kRowsBlock, kCols16, kCols4 };
+enum Form : int { kRowsWarp, kCols16, kCols4 };
 struct SplitJobs {
     struct Job {
         Source src;
@@ -481,7 +481,7 @@ static ct_status split_long_cols(DeviceState *st, const Split &x) {
 
 ct_status split(DeviceState *st, const Split *what, int count) {
     auto blocks_of = [](int form, int64_t rows, int64_t width) {
-        return form == kRowsWarp ? (rows + 7) / 8 : form == kRowsBlock ? rows : form == kCols16 ? (width + 15) / 16 : (width + 3) / 4;
+        return form == kRowsWarp ? (rows + 7) / 8 : form == kCols16 ? (width + 15) / 16 : (width + 3) / 4;
     };
     auto add = [&](SplitJobs &jobs, int64_t &blocks, const Split &x, const float *in, const float *in2, int64_t at, int form) {
         const Source src    = source_of(in, in2, x.rows, x.cols, x.col_factor);
@@ -517,44 +517,46 @@ ct_status split(DeviceState *st, const Split *what, int count) {
         }
         return CT_OK;
     }
-    SplitJobs rows{}, cols{};
-    int64_t row_blocks = 0, col_blocks = 0;
+    SplitJobs cols{};
+    int64_t col_blocks = 0;
     for (int i = 0; i < count; ++i) {
         const Split &x = what[i];
         if (!x.by_column)
-            add(rows, row_blocks, x, x.in, x.in2, 0, kRowsBlock);
-        else if (x.rows <= kShort * 64)
+            continue;
+        if (x.rows <= kShort * 64)
             add_cols(cols, col_blocks, x, kCols16);
         else
             CT_TRY(split_long_cols(st, x));
     }
-    if (row_blocks > 0x7fffffff || col_blocks > 0x7fffffff)
-        return fail(CT_ERR_TOO_LARGE, "split: too many rows");
-    if (col_blocks > 0) {
+    if (col_blocks > 0) { // of 16 columns each: a grid holds kMostSize of two matrices
         CT_CUDA(launch_dependent(split_short_cols_kernel, dim3((unsigned)col_blocks), dim3(256), 0, stream(), cols));
         CT_LAUNCH_CHECK("split_short_cols");
     }
-    for (int i = 0; i < rows.count; ++i) {
-        const SplitJobs::Job &x = rows.job[i];
+    for (int i = 0; i < count; ++i) {
+        const Split &x = what[i];
+        if (x.by_column)
+            continue;
+        const Source src    = source_of(x.in, x.in2, x.rows, x.cols, x.col_factor);
+        const int64_t width = x.in2 ? 2 * src.ld : src.ld;
         auto run = [&](auto kernel, int per_block) {
-            return launch_dependent(kernel, dim3((unsigned)((x.src.rows + per_block - 1) / per_block)), dim3(256), 0, stream(), x.src, x.width, x.to, x.inverse);
+            return launch_dependent(kernel, dim3((unsigned)((x.rows + per_block - 1) / per_block)), dim3(256), 0, stream(), src, width, x.to, x.inverse);
         };
-        if (x.width <= 256)
+        if (width <= 256)
             CT_CUDA(run(split_rows_kernel<32, 2>, 8));
-        else if (x.width <= 512)
+        else if (width <= 512)
             CT_CUDA(run(split_rows_kernel<32, 4>, 8));
-        else if (x.width <= 1024)
+        else if (width <= 1024)
             CT_CUDA(run(split_rows_kernel<32, 8>, 8));
-        else if (x.width <= 2048)
+        else if (width <= 2048)
             CT_CUDA(run(split_rows_kernel<256, 2>, 1));
-        else if (x.width <= 4096)
+        else if (width <= 4096)
             CT_CUDA(run(split_rows_kernel<256, 4>, 1));
-        else if (x.width <= 8192)
+        else if (width <= 8192)
             CT_CUDA(run(split_rows_kernel<256, 8>, 1));
-        else if (x.width <= 8 * kLongQuads * 1024) {
-            const int ranks    = x.width <= 2 * kLongQuads * 1024 ? 2 : x.width <= 4 * kLongQuads * 1024 ? 4 : 8;
-            const int64_t each = (x.width + 4 * ranks - 1) / (4 * ranks) * 4;
-            CT_CUDA(launch_dependent_cluster(split_long_rows_kernel, ranks, dim3((unsigned)(x.src.rows * ranks)), dim3(256), 0, stream(), x.src, x.width, ranks, each,
+        else if (width <= 8 * kLongQuads * 1024) {
+            const int ranks    = width <= 2 * kLongQuads * 1024 ? 2 : width <= 4 * kLongQuads * 1024 ? 4 : 8;
+            const int64_t each = (width + 4 * ranks - 1) / (4 * ranks) * 4;
+            CT_CUDA(launch_dependent_cluster(split_long_rows_kernel, ranks, dim3((unsigned)(x.rows * ranks)), dim3(256), 0, stream(), src, width, ranks, each,
                                              x.to, x.inverse));
         } else
             CT_CUDA(run(split_rows_kernel<256, 8>, 1)); // read twice
@@ -568,7 +570,6 @@ namespace {
 // Tile and slices of a product by what they take, in microseconds: a stage of a pair's 256 x 256 tile ~ 0.95, of a single CTA's 128 x 128 ~ 0.6;
 // filling and draining a tile as much as four stages; the slices' sums written, read and a launch.
 struct Plan {
-    int64_t stages;
     bool pair  = false;
     int splits = 1;
     double cost = 1e300;

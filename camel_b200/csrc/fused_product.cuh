@@ -71,7 +71,6 @@ constexpr int64_t kMostSize = 1 << 29;
 struct Planes {
     __half *hi = nullptr, *lo = nullptr;
     int64_t rows = 0, cols = 0, ld = 0;
-    int64_t plane() const { return rows * ld; } // values of one plane
 };
 inline int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 
