@@ -468,6 +468,8 @@ ct_status check_gated(const char *name, int64_t m, int64_t k, int64_t n, int gat
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
     if (!valid_gate(gate))
         return fail(CT_ERR_INVALID, "%s: unknown gate", name);
+    if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
+        return fail(CT_ERR_TOO_LARGE, "%s: dimension too large", name);
     return CT_OK;
 }
 
@@ -489,8 +491,6 @@ ct_status ct_dense_gated(
         return CT_OK;
     if (!out || (k > 0 && (!x || !w_gate || !w_up)))
         return fail(CT_ERR_INVALID, "dense_gated: null pointer");
-    if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
-        return fail(CT_ERR_TOO_LARGE, "dense_gated: dimension too large");
     ProfScope prof("dense_gated");
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
         if (fused::takes_few_rows(m, 2 * n))
@@ -540,8 +540,6 @@ ct_status ct_dense_gated_grad(
         CT_CUDA(clear(db_up, n));
         return CT_OK;
     }
-    if (m > fused::kMostSize || k > fused::kMostSize || n > fused::kMostSize)
-        return fail(CT_ERR_TOO_LARGE, "dense_gated_grad: dimension too large");
     if (ct_get_precision() == CT_PREC_3XTF32 && m <= fused::kFewRows && k > 0 && (dx || dw_gate || dw_up || db_gate || db_up)) {
         fused::FewGrad p{};
         p.x = x, p.w[0] = w_gate, p.w[1] = w_up, p.dw[0] = dw_gate, p.dw[1] = dw_up, p.db[0] = db_gate, p.db[1] = db_up;

@@ -500,7 +500,7 @@ ct_status check_norm(const char *name, const void *x, const void *second, int64_
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
     if (!(eps >= 0.0))
         return fail(CT_ERR_INVALID, "%s: eps must not be negative", name);
-    if (rows > 0x7fffffff || cols > 0x7fffffff)
+    if (rows > 1 << 29 || cols > 1 << 29)
         return fail(CT_ERR_TOO_LARGE, "%s: dimension too large", name);
     if (rows > 0 && cols > 0 && (!x || !second))
         return fail(CT_ERR_INVALID, "%s: null pointer", name);

@@ -288,3 +288,13 @@ def test_cross_entropy_gradients_of_many_rows(m, k, n, chain, pick):
     assert ((db[1:].double() - want).abs() <= off * want).all()
     if n <= 16:
         assert ((dw[:, 1:].double() - want).abs() <= off * want).all()
+
+
+@gpu
+def test_dimensions_that_are_too_large_are_refused_also_where_there_is_nothing_to_do():
+    big, z = (1 << 29) + 1, None
+    for rc in (L.lib.ct_dense_gated(z, z, z, z, z, 0, big, 4, 0, z, z, z), L.lib.ct_dense_gated_grad(z, z, z, z, z, z, 0, 1 << 33, 1 << 31, 0, z, z, z, z, z),
+               L.lib.ct_dense_gated_grad(z, z, z, z, z, z, 4, big, 0, 0, z, z, z, z, z), L.lib.ct_layer_norm(z, z, z, 0, big, 1e-5, z),
+               L.lib.ct_layer_norm(z, z, z, big, 0, 1e-5, z), L.lib.ct_layer_norm_grad(z, z, z, 0, big, 1e-5, z, z, z),
+               L.lib.ct_dense_cross_entropy(z, z, z, z, 0, big, 4, z, z), L.lib.ct_dense_cross_entropy_grad(z, z, z, z, z, z, 0, 4, big, z, z, z)):
+        assert rc == L.ERR_TOO_LARGE, L.lib.ct_last_error()
