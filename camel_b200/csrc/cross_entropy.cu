@@ -463,7 +463,7 @@ ct_status ce_grad_fused(
     // dx needs the weights' planes in any case, and with them tiles are sooner (20 x 1024 x 8192 78 us, streamed 89; 40 x 32000 205
     // and 219); without it 64 x 32000 takes 127 streamed, 186 by tiles.
     const bool few = !dx && takes_stream(m, n);
-    // Pieces of the vocabulary: planes of d of up to 512 MB, alike in size and whole tiles.
+    // Pieces of the vocabulary: planes of d of up to 512 MB (more only above 2^19 rows, of 256 classes), alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
     const int64_t pieces = (n + most - 1) / most;
     const int64_t piece = std::min<int64_t>(n, ((n + pieces - 1) / pieces + 255) / 256 * 256), ld = padded(piece);

@@ -7,13 +7,14 @@
 
 namespace ct {
 
-// Both sides of the logistic function with their full relative precision: 1 - sigmoid(g) is sigmoid(-g), not a difference.
+// Both sides of the logistic function with their full relative precision: 1 - sigmoid(g) is sigmoid(-g), not a difference; the smaller one is 0
+// below 2^-126 (|g| beyond 87.3).
 // exp(-|g|) = 2^t (1 + r ln 2), t the rounded -|g| log2(e) and r what it lacks, to 2^-22 of itself; 1 / (1 + e), of a number from 1 to 2, by
 // a reciprocal and a Newton step.  No branches: in the epilogue of a product the division's and expf's cost a tile as much as half of its MMAs.
 __device__ __forceinline__ void sigmoids(float g, float &s, float &other) {
     const float kLog2e = 1.44269502162933349609375f, kLog2eRest = 1.925963033500011079e-8f;
     float x, e, a;
-    asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(x) : "f"(fabsf(g))); // 104, where exp(-x) is no float any more
+    asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(x) : "f"(fabsf(g))); // 104: e is 0 from 87.3 on, and stays it
     const float t = __fmul_rn(-x, kLog2e);
     const float r = __fmaf_rn(-x, kLog2eRest, __fmaf_rn(-x, kLog2e, -t));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
