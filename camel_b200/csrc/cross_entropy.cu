@@ -311,7 +311,7 @@ ct_status ce_fused(
     DeviceState *st, const float *x, const float *w, const float *bias, const int64_t *targets, int64_t m, int64_t k, int64_t n, float *loss, float *lse) {
     using namespace fused;
     const int64_t lk = padded(k), ln = padded(n);
-    const bool few = takes_stream(m, n), pair = !few && takes_pairs(st, m, n);
+    const bool few = takes_stream(m, k, n), pair = !few && takes_pairs(st, m, n);
     int per;
     const int64_t slots = few ? (int64_t)stream_grid(st, n, &per) : pair ? (n + 255) / 256 * 4 : (n + 127) / 128 * 4;
     Parts parts;
@@ -462,7 +462,7 @@ ct_status ce_grad_fused(
     const int64_t lk = padded(k), ln = padded(n);
     // dx needs the weights' planes in any case, and with them tiles are sooner (20 x 1024 x 8192 78 us, streamed 89; 40 x 32000 205
     // and 219); without it 64 x 32000 takes 127 streamed, 186 by tiles.
-    const bool few = !dx && takes_stream(m, n);
+    const bool few = !dx && takes_stream(m, k, n);
     // Pieces of the vocabulary: planes of d of up to 512 MB (more only above 2^19 rows, of 256 classes), alike in size and whole tiles.
     const int64_t most = std::max<int64_t>(256, (int64_t)(1u << 27) / m / 256 * 256);
     const int64_t pieces = (n + most - 1) / most;

@@ -495,7 +495,7 @@ ct_status ct_dense_gated(
     if (ct_get_precision() == CT_PREC_3XTF32 && k > 0) {
         if (fused::takes_few_rows(m, 2 * n))
             return fused::few_rows(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
-        if (fused::takes_stream(m, 2 * n))
+        if (fused::takes_stream(m, k, 2 * n))
             return gated_stream(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
         return gated_fused(st, x, w_gate, b_gate, w_up, b_up, m, k, n, gate, out, gate_pre, up_pre);
     }

@@ -22,11 +22,21 @@ namespace ct {
 namespace fused {
 
 // Whether a product of more than 16 rows is streamed, `columns` those of both matrices: a CTA has an even share of them, of at least 16, and tiles of
-// 128 are the emptier the fewer there are; of more than 64 rows the weights are read twice.  Streamed, and by tiles of planes (us, k = 1024, cross entropy):
-// 64 rows x 1000 39 and 35, x 4096 39 and 37, x 8192 41 and 45, x 32000 63 and 129; 128 rows x 8192 68 and 47, x 16384 72 and 78, x 32000 111 and
-// 130; gated, two matrices of n: 64 x 1000 35 and 33, x 2048 35 and 33 (k = 4096 92 and 118), x 8192 39 and 62; 128 x 8192 68 and 62 (k = 2048 105
-// and 182), x 16384 115 and 111, x 32000 189 and 199.
-inline bool takes_stream(int64_t m, int64_t columns) { return m <= 64 ? columns >= 4096 : m <= 128 && columns >= 16384; }
+// 128 are the emptier the fewer there are, while a pre-pass takes as long as there are weights; of more than 64 rows they are read twice.
+// Streamed, and by tiles of planes (us; cross entropy over n classes, gated of two matrices of n; the first three lines without flushing L2):
+//   17 rows, k = 128: gated x 300 8.7 and 10.2, x 2000 9.1 and 12.0; cross entropy x 1000 12.0 and 12.8; k = 1024: gated x 300 24 and 22, x 1000 25 and
+//     25, x 2000 25 and 26; cross entropy x 1000 28 and 25, x 2000 29 and 26, x 4000 29 and 28; k = 4096: x 1000 82 and 67, x 4000 83 and 116
+//   64 rows, k = 128: gated x 1000 11.7 and 11.0, x 2000 12.0 and 12.1; k = 1024: x 1000 28 and 26, x 2000 29 and 26, x 4000 29 and 33; k = 4096: x 1000
+//     83 and 73, x 2000 83 and 116; cross entropy k = 1024: x 2000 33 and 26, x 4000 33 and 28; k = 4096: x 2000 88 and 73, x 4000 89 and 118
+//   64 rows, k = 1024: cross entropy x 8192 41 and 45, x 32000 63 and 129; 128 rows: x 8192 68 and 47, x 16384 72 and 78, x 32000 111 and 130; gated
+//     x 8192 68 and 62 (k = 2048 105 and 182), x 16384 115 and 111, x 32000 189 and 199
+inline bool takes_stream(int64_t m, int64_t k, int64_t columns) {
+    if (m <= 32)
+        return k <= 384 || columns >= 2048; // k = 300: gated x 1000 13 and 14, cross entropy x 1000 17 and 15
+    if (m <= 64)
+        return columns >= (k < 2048 ? 4096 : 3000);
+    return m <= 128 && columns >= 16384;
+}
 constexpr int kStreamSlots   = 2;
 // Warps: of a stage fetched by the warps that convert it all did the same at the same time, and a stage of 64 x 1024 x 128000 took 3350 clocks.
 constexpr int kStreamDrain = 8, kStreamFetch = 4, kStreamConvert = 8; // kStreamConvert: of a group

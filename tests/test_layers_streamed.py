@@ -1,4 +1,5 @@
-"""Products of 17 to 128 rows whose weights are streamed: from 4096 columns of weights (16384 above 64 rows), at any address."""
+"""Products of 17 to 128 rows whose weights are streamed: few values of k or 2048 columns of weights, 4096 above 32 rows (3000 of many values), 16384
+above 64; at any address."""
 import numpy as np
 import pytest
 
@@ -9,8 +10,8 @@ from test_layers_calls import Buffer
 from test_layers_precision import ce_grad_at_bounds, f64, most, SMALL, SUM, U, within
 
 gpu = pytest.mark.gpu
-GATED = [(17, 70, 2049), (20, 1, 2048), (33, 65, 2050), (64, 130, 2115), (40, 200, 3001), (65, 64, 8200), (100, 65, 8193), (128, 33, 8192)]
-CE = [(17, 1, 4096), (30, 130, 4100), (64, 65, 5003), (33, 300, 4601), (65, 40, 16384), (100, 96, 16401), (128, 63, 17002)]
+GATED = [(17, 70, 2049), (20, 1, 2048), (17, 256, 5), (32, 100, 33), (31, 300, 1024), (40, 2100, 1501), (33, 65, 2050), (64, 130, 2115), (40, 200, 3001), (65, 64, 8200), (100, 65, 8193), (128, 33, 8192)]
+CE = [(17, 1, 4096), (32, 256, 17), (25, 130, 129), (20, 1000, 2050), (50, 2048, 3001), (30, 130, 4100), (64, 65, 5003), (33, 300, 4601), (65, 40, 16384), (100, 96, 16401), (128, 63, 17002)]
 
 
 @gpu
