@@ -384,8 +384,8 @@ ct_status ct_dense_gated_grad(
 
 /* Softmax cross entropy of the logits z = x . w + bias (x [m][k], w [k][n], bias [n] or null), which are not kept:
  *   lse[i] = log(sum over j of exp(z[i][j])), loss[i] = lse[i] - z[i][targets[i]].
- * A target outside 0 .. n-1 marks a row that has none (padding): its loss is 0, whatever x holds there.  loss or lse may be null;
- * n >= 1. */
+ * A target outside 0 .. n-1 marks a row that has none (padding): its loss is 0, whatever x holds there.  A logit of -infinity takes its
+ * class out (of nothing else lse is -infinity); one that is NaN or +infinity makes lse NaN.  loss or lse may be null; n >= 1. */
 ct_status ct_dense_cross_entropy(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, int64_t m, int64_t k, int64_t n,
     float *loss_dev, float *lse_dev);

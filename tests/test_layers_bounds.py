@@ -298,3 +298,74 @@ def test_dimensions_that_are_too_large_are_refused_also_where_there_is_nothing_t
                L.lib.ct_layer_norm(z, z, z, big, 0, 1e-5, z), L.lib.ct_layer_norm_grad(z, z, z, 0, big, 1e-5, z, z, z),
                L.lib.ct_dense_cross_entropy(z, z, z, z, 0, big, 4, z, z), L.lib.ct_dense_cross_entropy_grad(z, z, z, z, z, z, 0, 4, big, z, z, z)):
         assert rc == L.ERR_TOO_LARGE, L.lib.ct_last_error()
+
+
+# ---- outputs that are not asked for, logits that are no numbers --------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(5, 40), (300, 200), (1300, 785), (300, 1024), (70, 3001), (40, 8193)])
+def test_layer_norm_gradients_alone(rows, cols):
+    x, gamma, _, dy = norm_inputs(rows, cols, 81)
+    tx, td, g = dev(x), dev(dy), dev(gamma)
+    want = [a.numpy().tobytes() for a in T.layer_norm_grad(tx, td, g)]
+    for mask in range(1, 8):
+        outs = [T.zeros([rows, cols]), T.zeros([cols]), T.zeros([cols])]
+        p = [o.ptr if mask >> i & 1 else None for i, o in enumerate(outs)]
+        L.check(L.lib.ct_layer_norm_grad(tx.ptr, g.ptr, td.ptr, rows, cols, 1e-5, *p))
+        for i, o in enumerate(outs):
+            assert o.numpy().tobytes() == want[i] if mask >> i & 1 else not o.numpy().any()
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(1, 40, 70), (16, 40, 70), (20, 40, 70), (40, 40, 2100), (200, 40, 70), (1300, 40, 1100)])
+def test_dense_gated_keeps_what_is_asked_for(m, k, n):
+    t = [dev(a) for a in gated_inputs(m, k, n, 82)]
+    want = [a.numpy().tobytes() for a in T.dense_gated(*t, keep=True)]
+    for mask in range(4):
+        out, kept = T.zeros([m, n]), [T.zeros([m, n]), T.zeros([m, n])]
+        p = [o.ptr if mask >> i & 1 else None for i, o in enumerate(kept)]
+        L.check(L.lib.ct_dense_gated(t[0].ptr, t[1].ptr, t[3].ptr, t[2].ptr, t[4].ptr, m, k, n, L.GATE_SILU, out.ptr, *p))
+        T.check_async()
+        assert out.numpy().tobytes() == want[0]
+        for i, o in enumerate(kept):
+            assert o.numpy().tobytes() == want[1 + i] if mask >> i & 1 else not o.numpy().any()
+
+
+CE_FORMS = [(1, 40, 70), (4, 40, 9000), (16, 40, 8), (20, 40, 70), (40, 40, 300), (64, 40, 4200), (200, 40, 300), (200, 40, 10), (1300, 40, 2100)]
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", CE_FORMS)
+def test_cross_entropy_outputs_alone(m, k, n):
+    x, w, b, t = (dev(a) for a in ce_inputs(m, k, n, 83))
+    loss, lse = (a.numpy().tobytes() for a in T.dense_cross_entropy(x, w, t, b))
+    one, other = T.zeros([m]), T.zeros([m])
+    L.check(L.lib.ct_dense_cross_entropy(x.ptr, w.ptr, b.ptr, t.ptr, m, k, n, one.ptr, None))
+    L.check(L.lib.ct_dense_cross_entropy(x.ptr, w.ptr, b.ptr, t.ptr, m, k, n, None, other.ptr))
+    L.check(L.lib.ct_dense_cross_entropy(x.ptr, w.ptr, b.ptr, t.ptr, m, k, n, None, None))
+    T.check_async()
+    assert one.numpy().tobytes() == loss and other.numpy().tobytes() == lse
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["3xtf32", "bf16"])
+@pytest.mark.parametrize("m,k,n", CE_FORMS)
+def test_logits_that_are_no_numbers(m, k, n, precision):
+    """Biases of -infinity take classes out, all of them: lse -infinity; one of +infinity or NaN makes it NaN.  With any number of rows."""
+    x, w, b, t = ce_inputs(m, k, n, 84)
+    t[:] = n - 1
+    L.check(L.lib.ct_set_precision(L.PREC_BF16 if precision == "bf16" else L.PREC_3XTF32))
+    try:
+        lse = lambda c: T.dense_cross_entropy(dev(x), dev(w), dev(t), dev(c))[1].numpy()  # noqa: E731
+        assert np.isneginf(lse(np.full(n, -np.inf, np.float32))).all()
+        only = np.full(n, -np.inf, np.float32)
+        only[n // 2] = 1.0
+        want = x.astype(np.float64) @ w[:, n // 2].astype(np.float64) + 1.0
+        assert np.abs(lse(only) - want).max() <= 0.2  # bfloat16: 2^-7 of sum |x||w|
+        for bad in (np.inf, np.nan):
+            c = b.copy()
+            c[n // 3] = bad
+            assert np.isnan(lse(c)).all()
+    finally:
+        L.check(L.lib.ct_set_precision(L.PREC_3XTF32))
