@@ -112,9 +112,11 @@ ct_status report_timeout(DeviceState *st, const char *what);
 // returns once the predecessor grid has completed and its writes are visible), so only its set-up
 // (barrier initialisation, TMEM allocation, descriptor prefetch, index arithmetic) overlaps.  A
 // kernel lets its successor start early with griddep_launch_dependents(); without that call the
-// successor starts when the grid ends, as usual.  A kernel of a few microseconds calls it behind its own wait: before it,
-// the successor of its successor would come up while its predecessor still runs, and take the slots that are free then instead
-// of spreading over the SMs (a training step of 5493 x 279 x 16 47 us, and 39 so).  CAMEL_TENSOR_NO_PDL=1 turns the attribute off.
+// successor starts when the grid ends, as usual.  That call comes behind the kernel's own wait, never before it: an SM's first-level cache
+// is emptied when a grid is launched, not when its wait returns.  With the call before the wait, the successor of the successor is launched
+// while this kernel's predecessor still runs, and finds in that cache what the predecessor reads from then on, also where this kernel has
+// written it anew (product, transpose into its operand, product again: up to 190 of 200 wrong).  It would also take the slots that are free then
+// instead of spreading over the SMs (a training step of 5493 x 279 x 16 47 us, and 39 so).  CAMEL_TENSOR_NO_PDL=1 turns the attribute off.
 // While per-kernel event brackets are on (ct_profile_enable) kernels are launched the ordinary way,
 // so that a bracket times one kernel alone and not its overlap with the neighbours.
 bool profiling_enabled();

@@ -66,9 +66,9 @@ __global__ void __launch_bounds__(256, V == kPatchRegs ? 4 : 0) im2col_half_kern
     HalfExceptions *__restrict__ exceptions) {
     extern __shared__ int2 where[]; // element kk: offset from the patch's origin in its image, r << 16 | s
     __half *p_hi = static_cast<__half *>(plane_hi), *p_lo = static_cast<__half *>(plane_lo);
-    griddep_launch_dependents();
     if (WIDE) {
         griddep_wait();
+        griddep_launch_dependents();
         if (!half_wide(exceptions, exceptions))
             return;
     }
@@ -77,8 +77,10 @@ __global__ void __launch_bounds__(256, V == kPatchRegs ? 4 : 0) im2col_half_kern
         where[kk] = kk < kdim ? make_int2((ic * h + r) * w + s, (r << 16) | s) : make_int2(0, 0x7fff7fff);
     }
     __syncthreads();
-    if (!WIDE)
+    if (!WIDE) {
         griddep_wait();
+        griddep_launch_dependents();
+    }
     const int lane = threadIdx.x & 31, pix = ho * wo;
     for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
         const int img = (int)(row / pix), p = (int)(row - (int64_t)img * pix);

@@ -193,7 +193,6 @@ __global__ void __launch_bounds__(kH_Threads, 1) conv_halo_stream_kernel(
     const int lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1); // in the cluster of two
 
-    griddep_launch_dependents();
     const uint32_t smem_base  = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t halo_stage = 2u * (uint32_t)p.halo_plane_bytes;
     const uint32_t slot_base  = smem_base + (uint32_t)p.halo_stages * halo_stage;
@@ -224,6 +223,7 @@ __global__ void __launch_bounds__(kH_Threads, 1) conv_halo_stream_kernel(
         tmem_relinquish_pair();
     }
     griddep_wait(); // the planes, the scales and what the caller's earlier kernels wrote
+    griddep_launch_dependents();
     if (threadIdx.x == 0)
         abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
     tc_fence_before_sync();
@@ -585,8 +585,8 @@ __global__ void __launch_bounds__(256) conv_range_kernel(
     const float *__restrict__ w, int c, int taps, int c_pad, int ko, const __grid_constant__ FilterPlanes f, const float *__restrict__ x,
     int64_t count, int slices, int vec_ok, uint2 *__restrict__ ranges) {
     __shared__ uint2 part[8];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const bool filter = (int64_t)blockIdx.x < ko;
     const int64_t o   = filter ? blockIdx.x : (blockIdx.x - ko) / slices;
     const int slice   = filter ? 0 : (int)(blockIdx.x - ko - o * slices);
@@ -677,8 +677,8 @@ __global__ void __launch_bounds__(256, 3) conv_planes_kernel(
     const float *__restrict__ filter_scale, int ko, uint8_t *__restrict__ slots, float *__restrict__ image_scale) {
     __shared__ uint4 stage_s[8][128];
     __shared__ float scale_s;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int img  = (int)(gridDim.y - 1 - blockIdx.y);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int item = (int)blockIdx.x * 8 + warp, hw = g.h * g.w;

@@ -750,8 +750,8 @@ template <bool RAW, int CG>
 __global__ void __launch_bounds__(kCP_Threads, 1) conv_pairs_kernel(
     const __grid_constant__ CUtensorMap map_x_hi, const __grid_constant__ CUtensorMap map_x_lo,
     const __grid_constant__ ConvPairParams p, const int total_tiles) {
-    griddep_launch_dependents(); // the tf32 form, which allocates no tensor memory before this kernel ends
     griddep_wait();
+    griddep_launch_dependents(); // the tf32 form, which allocates no tensor memory before this kernel ends
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[kCP_MaxStages], bar_empty[kCP_MaxStages];
     __shared__ uint64_t bar_raw_full, bar_raw_empty;

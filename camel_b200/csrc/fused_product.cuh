@@ -166,7 +166,6 @@ __device__ __forceinline__ void product_body(
     __shared__ int abort_flag_s;
     volatile int *abort_flag = &abort_flag_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    griddep_launch_dependents();
     if (threadIdx.x == 0)
         abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p0.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -204,6 +203,7 @@ __device__ __forceinline__ void product_body(
     const bool failed        = abort_flag_s != 0; // an earlier launch failed: no work
     __syncthreads(); // every thread has read abort_flag_s before a role may raise it
     griddep_wait();
+    griddep_launch_dependents();
     auto stage_addr = [&](int s) { return smem_base + (uint32_t)s * kStage; };
     auto k_range    = [&](const Product &p, int tz, int &from, int &count) {
         from           = p.stages_split > 0 ? tz * p.stages_split : 0;

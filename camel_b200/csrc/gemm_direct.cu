@@ -75,7 +75,6 @@ __global__ void __launch_bounds__(kGD_Threads, 1) gemm_direct_kernel(const __gri
     uint8_t *smem            = smem_raw + (smem_base - smem_u32(smem_raw));
     uint2(*ranges)[128]      = reinterpret_cast<uint2(*)[128]>(smem + kGD_Ranges);
 
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         wide_s = 0;
         mbar_init(smem_u32(&bar), 1);
@@ -91,6 +90,7 @@ __global__ void __launch_bounds__(kGD_Threads, 1) gemm_direct_kernel(const __gri
     const int ksteps = (kn + 15) >> 4;
     cluster_arrive(); // this CTA runs: the others may write to its shared memory
     griddep_wait();
+    griddep_launch_dependents();
     if (threadIdx.x == 0)
         abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
 

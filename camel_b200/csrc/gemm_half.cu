@@ -316,7 +316,6 @@ __global__ void __launch_bounds__(kHThreads, 1)
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    griddep_launch_dependents();
     if (threadIdx.x == 0)
         abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
 
@@ -361,6 +360,7 @@ __global__ void __launch_bounds__(kHThreads, 1)
     // everything above is set-up that does not depend on earlier kernels; the planes, the words and the
     // output may
     griddep_wait();
+    griddep_launch_dependents();
     if (LEFT && *reinterpret_cast<volatile uint32_t *>(p.only_if) == 0u) {
         __syncthreads();
         if (slices > 1)
@@ -1064,8 +1064,8 @@ template <int TPR, int V>
 __global__ void __launch_bounds__(256) half_rows_kernel(
     const float *__restrict__ in, int64_t rows, int64_t k, int64_t kp, const HalfPlanes p, int vec_ok,
     uint32_t *__restrict__ zero, int64_t zero_count) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < zero_count; i += (int64_t)gridDim.x * 256)
         zero[i] = 0u; // scales and column maxima of the right operand, accumulated by the next kernels
     half_rows<TPR, V>((int64_t)blockIdx.x, in, rows, k, kp, p, vec_ok);
@@ -1075,8 +1075,8 @@ __global__ void __launch_bounds__(256) half_rows_kernel(
 __global__ void __launch_bounds__(256) half_rows_left_kernel(
     const float *__restrict__ in, int64_t rows, int64_t k, int64_t kp, const HalfPlanes p, int vec_ok,
     const uint32_t *__restrict__ only_if) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     if (*reinterpret_cast<const volatile uint32_t *>(only_if) == 0u)
         return;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -1090,8 +1090,8 @@ __global__ void __launch_bounds__(256) half_rows_left_kernel(
 __global__ void __launch_bounds__(256) half_col_max_kernel(
     const float *__restrict__ in, int64_t k, int64_t n, int64_t rows_per_block, int vec_ok, uint32_t *__restrict__ col_max) {
     __shared__ uint32_t max_s[8][128];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t n0 = (int64_t)blockIdx.x * 128;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(k, r0 + rows_per_block);
@@ -1133,8 +1133,8 @@ __global__ void __launch_bounds__(256) half_col_max_kernel(
 __global__ void __launch_bounds__(256) half_cols_kernel(
     const float *__restrict__ in, int64_t k, int64_t n, int64_t kp, const HalfPlanes p, int vec_ok, const uint32_t *__restrict__ col_max) {
     __shared__ float tile[64][65];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t n0 = (int64_t)blockIdx.x * 64, k0 = (int64_t)blockIdx.y * 64;
     transpose_load(tile, in, k, n, k0, n0, vec_ok);
     __syncthreads();
@@ -1260,8 +1260,8 @@ __device__ __forceinline__ void half_cols_short(
 __global__ void __launch_bounds__(256) half_cols_short_kernel(
     const float *__restrict__ in, int64_t k, int64_t n, int64_t kp, const HalfPlanes p) {
     extern __shared__ float tile_short[];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     half_cols_short(tile_short, (int)blockIdx.x, in, k, n, kp, p);
 }
 
@@ -1272,8 +1272,8 @@ __global__ void __launch_bounds__(256) half_both_kernel(
     const float *__restrict__ a, int64_t m, int a_vec_ok, const HalfPlanes pa, int row_blocks,
     const float *__restrict__ b, int64_t n, const HalfPlanes pb, int64_t k, int64_t kp) {
     extern __shared__ float tile_short[];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     if ((int)blockIdx.x < row_blocks)
         half_rows<32, V>((int64_t)blockIdx.x, a, m, k, kp, pa, a_vec_ok);
     else
@@ -1294,8 +1294,8 @@ __global__ void __launch_bounds__(256) wide_planes_kernel(
     const HalfExceptions *__restrict__ ea, const HalfExceptions *__restrict__ eb, const WideOperand a, const WideOperand b,
     int64_t k, int64_t kp) {
     __shared__ float tile[64][65];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     if (!half_wide(ea, eb))
         return;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -1364,8 +1364,8 @@ __global__ void __launch_bounds__(256) widen_planes_kernel(
 __global__ void __launch_bounds__(256) half_splitk_reduce_kernel(
     const float *__restrict__ partial, int splits, int64_t total, int64_t n, const float *__restrict__ bias,
     int act, float *__restrict__ out, const uint32_t *__restrict__ flags) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     // the slices were not computed if an earlier failure is on record
     if (*reinterpret_cast<const volatile uint32_t *>(flags + FLAG_TIMEOUT) != 0)
         return;

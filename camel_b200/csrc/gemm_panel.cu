@@ -69,7 +69,6 @@ __global__ void __launch_bounds__(kGP_Threads, 1) gemm_panel_kernel(
     const uint32_t smem_base = smem_u32(smem_raw);
     uint8_t *smem            = smem_raw;
 
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&bar_a_full[b]), kGP_Workers);
@@ -89,6 +88,7 @@ __global__ void __launch_bounds__(kGP_Threads, 1) gemm_panel_kernel(
         listed_s     = 0;
     }
     griddep_wait();
+    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         // whether an earlier launch failed (no work, but the cluster's CTAs stay together), or B is not for this kernel
         const bool b_bad  = half_wide(p.exceptions_b, p.exceptions_b);

@@ -417,8 +417,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 1) gemm_few_columns_kernel(
     extern __shared__ __align__(16) double w_few[]; // [k rounded up to 32][S], then the warps' rings [D][R][32] floats
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int steps = (k + 31) >> 5;
-    griddep_launch_dependents();
     griddep_wait(); // activations (and possibly weights) come from the previous kernel
+    griddep_launch_dependents();
     // the walk of a warp: tiles of R rows, 32 values of k a step; the fetch runs D - 1 steps ahead of it, across tiles
     const int64_t tiles = (m + R - 1) / R, first = (int64_t)blockIdx.x + (int64_t)warp * gridDim.x;
     const int64_t stride = (int64_t)gridDim.x * kFewWarps;
@@ -571,8 +571,8 @@ __global__ void __launch_bounds__(32 * kTallWarps, 1) gemm_tall_kernel(
     extern __shared__ __align__(16) double2 w_tall[]; // [steps][units], then the warps' rings [D][R][kTallRow] floats
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int steps = (k + 31) >> 5;
-    griddep_launch_dependents();
     griddep_wait(); // activations (and possibly weights) come from the previous kernel
+    griddep_launch_dependents();
     const int64_t tiles = (m + R - 1) / R, first = (int64_t)blockIdx.x + (int64_t)warp * gridDim.x;
     const int64_t stride = (int64_t)gridDim.x * kTallWarps;
     float *ring = reinterpret_cast<float *>(w_tall + (size_t)steps * C::kUnits) + warp * kTallRing * kTallRow;
@@ -746,8 +746,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) gemm_few_rows_kernel(
     int act, float *__restrict__ out, int64_t *__restrict__ argmax) {
     __shared__ double part[kFewWarps][R][NE];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t row0 = (int64_t)blockIdx.x * R;
     const int rows     = m - row0 < R ? (int)(m - row0) : R;
     double acc[R][NE];

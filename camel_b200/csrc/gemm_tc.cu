@@ -147,8 +147,8 @@ template <int MODE>
 __global__ void __launch_bounds__(256) split_rows_vec_kernel(
     const float *__restrict__ in, int64_t rows, int64_t k, int64_t kp, void *__restrict__ p_hi,
     void *__restrict__ p_lo, int in_vec_ok) {
-    griddep_launch_dependents();
     griddep_wait(); // the input may be the previous kernel's output, the planes its operands
+    griddep_launch_dependents();
     const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (c >= kp)
         return;
@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(256) split_transpose_bf_kernel(
     const float *__restrict__ in, int64_t k, int64_t n, int64_t kp, __nv_bfloat16 *__restrict__ plane, int vec_ok,
     int64_t in_batch_stride, int64_t out_batch_stride) {
     __shared__ float tile[64][65];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t n0 = (int64_t)blockIdx.x * 64, k0 = (int64_t)blockIdx.y * 64;
     // blockIdx.z walks a batch of [k][n] matrices (conv: one [c][h*w] image each)
     in += (int64_t)blockIdx.z * in_batch_stride;
@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(256) split_transpose_kernel(
     const float *__restrict__ in, int64_t k, int64_t n, int64_t kp, void *__restrict__ p_hi,
     void *__restrict__ p_lo, int64_t in_batch_stride, int64_t out_batch_stride) {
     __shared__ float tile[32][33];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     int tx     = threadIdx.x & 31;
     int ty     = threadIdx.x >> 5;
     int64_t n0 = (int64_t)blockIdx.x * 32;
@@ -324,7 +324,6 @@ __global__ void __launch_bounds__(Cfg<BN, MODE, RB>::kThreads, 1) gemm_tc_kernel
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    griddep_launch_dependents();
 
     // If an earlier CTA of this launch already timed out, do not start: the launch has failed
     // and the remaining CTAs should drain at once instead of each waiting out its own budget.
@@ -403,6 +402,7 @@ __global__ void __launch_bounds__(Cfg<BN, MODE, RB>::kThreads, 1) gemm_tc_kernel
     // everything above is set-up that does not depend on earlier kernels; the operands and the
     // output may
     griddep_wait();
+    griddep_launch_dependents();
 
     // split-K (kb_per_split > 0): the leading block index selects a slice of the k-blocks instead
     // of a batch entry; every slice writes its own partial output, summed by a second kernel

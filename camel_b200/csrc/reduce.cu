@@ -49,8 +49,8 @@ template <typename T> __device__ __forceinline__ double block_sum_double(double 
 // Pass 1: every block strides over the input and leaves one float64 partial.
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) sum_partial_kernel(const T *in, uint64_t n, double *partials) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     double acc      = 0.0;
     uint64_t stride = (uint64_t)gridDim.x * kSumThreads;
     uint64_t i      = (uint64_t)blockIdx.x * kSumThreads + threadIdx.x;
@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(kSumThreads) sum_partial_kernel(const T *in, u
 // float32 specialisation of pass 1: 128-bit loads, four independent accumulators.
 __global__ void __launch_bounds__(kSumThreads)
     sum_partial_f32x4_kernel(const float4 *in, uint64_t nvec, double *partials) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
     uint64_t stride = (uint64_t)gridDim.x * kSumThreads;
     uint64_t i      = (uint64_t)blockIdx.x * kSumThreads + threadIdx.x;
@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(kSumThreads)
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads)
     sum_final_kernel(const double *partials, int count, const T *tail, uint64_t tail_n, double *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     double acc = 0.0;
     for (int i = threadIdx.x; i < count; i += kSumThreads)
         acc += partials[i];
@@ -232,8 +232,8 @@ template <> __device__ __forceinline__ void acc_store<RED_ARGMAX, int64_t>(int64
 // axis = 1: one warp per row (cols <= 2048) - lanes stride over the columns.
 template <int KIND, typename T, typename OT>
 __global__ void __launch_bounds__(256) reduce_rows_warp_kernel(const T *in, int64_t rows, int64_t cols, OT *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows)
         return;
@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(256) reduce_rows_warp_kernel(const T *in, int6
 // axis = 1, wide rows: one block per row.
 template <int KIND, typename T, typename OT>
 __global__ void __launch_bounds__(256) reduce_rows_block_kernel(const T *in, int64_t rows, int64_t cols, OT *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ double sv[8];
     __shared__ long long si[8];
     int64_t row = blockIdx.x;
@@ -277,8 +277,8 @@ __global__ void __launch_bounds__(256) reduce_rows_block_kernel(const T *in, int
 // 128-byte reads per warp), then merge through shared memory in a fixed order.
 template <int KIND, typename T, typename OT>
 __global__ void __launch_bounds__(256) reduce_cols_kernel(const T *in, int64_t rows, int64_t cols, OT *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ double sv[8][33];
     __shared__ long long si[8][33];
     int tx      = threadIdx.x & 31;
@@ -383,8 +383,8 @@ template <int KIND, typename OT> __device__ __forceinline__ void best_store(OT *
 template <int KIND, typename OT, int RPT>
 __global__ void __launch_bounds__(256) reduce_rows_narrow_f32_kernel(
     const float *__restrict__ in, int64_t rows, int cols, OT *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     extern __shared__ float stage[];
     constexpr int kRows = 256 * RPT;
     const int64_t row0  = (int64_t)blockIdx.x * kRows;
@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(256) reduce_rows_narrow_f32_kernel(
 template <int KIND, typename OT>
 __global__ void __launch_bounds__(256) reduce_rows_direct_f32_kernel(
     const float *__restrict__ in, int64_t rows, int cols, OT *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (row >= rows)
         return;
@@ -463,8 +463,8 @@ __global__ void __launch_bounds__(256) reduce_rows_direct_f32_kernel(
 template <int KIND, typename OT, int GROUP>
 __global__ void __launch_bounds__(256) reduce_rows_f32_kernel(
     const float *__restrict__ in, int64_t rows, int64_t cols, OT *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     constexpr int kGroupsPerBlock = 256 / GROUP;
     __shared__ double s_sum[8];
     __shared__ float s_v[8];
@@ -549,8 +549,8 @@ template <int KIND>
 __global__ void __launch_bounds__(256) reduce_cols_f32_kernel(
     const float *__restrict__ in, int64_t rows, int64_t cols, int64_t rows_per_slice, double *__restrict__ psum,
     float *__restrict__ pv, int64_t *__restrict__ pidx) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ double s_sum[8][129];
     __shared__ float s_v[8][129];
     __shared__ long long s_i[8][129];
@@ -602,8 +602,8 @@ template <int KIND, typename OT>
 __global__ void __launch_bounds__(256) reduce_cols_finish_f32_kernel(
     const float *__restrict__ in, int64_t cols, int slices, const double *__restrict__ psum,
     const float *__restrict__ pv, const int64_t *__restrict__ pidx, OT *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= cols)
         return;
@@ -711,8 +711,8 @@ ct_status reduce_axis(int dt, const void *in, int64_t rows, int64_t cols, int64_
 
 template <int PER_LANE, int THREADS>
 __global__ void __launch_bounds__(THREADS) softmax_rows_kernel(const float *in, int64_t rows, int64_t cols, float *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     constexpr int WARPS         = THREADS / 32;
     constexpr bool kWarpPerRow  = PER_LANE <= 32 && THREADS == 256 && false;
     (void)kWarpPerRow;
@@ -782,8 +782,8 @@ __global__ void __launch_bounds__(THREADS) softmax_rows_kernel(const float *in, 
 template <int V4, int THREADS, int MIN_BLOCKS = 2>
 __global__ void __launch_bounds__(THREADS, MIN_BLOCKS)
     softmax_rows_wide_kernel(const float *__restrict__ in, int64_t rows, int64_t cols, float *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     constexpr int WARPS = THREADS / 32;
     __shared__ float s_max[WARPS];
     __shared__ double s_sum[WARPS];
@@ -871,8 +871,8 @@ __global__ void __launch_bounds__(THREADS, MIN_BLOCKS)
 // Several short rows per block: one warp per row, row kept in registers.
 template <int PER_LANE>
 __global__ void __launch_bounds__(256) softmax_rows_warp_kernel(const float *in, int64_t rows, int64_t cols, float *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows)
         return;
@@ -916,8 +916,8 @@ __global__ void __launch_bounds__(256) softmax_rows_warp_kernel(const float *in,
 
 // Rows too long for registers: three passes over global memory, one block per row.
 __global__ void __launch_bounds__(256) softmax_rows_stream_kernel(const float *in, int64_t rows, int64_t cols, float *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ float s_max[8];
     __shared__ double s_sum[8];
     int64_t row    = blockIdx.x;
@@ -960,8 +960,8 @@ __global__ void __launch_bounds__(256) softmax_rows_stream_kernel(const float *i
 
 template <typename T>
 __global__ void __launch_bounds__(256) transpose_kernel(const T *in, int64_t rows, int64_t cols, T *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ T tile[32][33];
     int tx      = threadIdx.x & 31;
     int ty      = threadIdx.x >> 5;
@@ -987,8 +987,8 @@ __global__ void __launch_bounds__(256) transpose_kernel(const T *in, int64_t row
 // element-wise kernel above).
 __global__ void __launch_bounds__(256) transpose_f32x4_kernel(
     const float *__restrict__ in, int64_t rows, int64_t cols, float *__restrict__ out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     __shared__ float tile[64][65];
     const int q      = threadIdx.x & 15;  // which group of four along the contiguous direction
     const int lane_r = threadIdx.x >> 4;  // 0..15
@@ -1018,8 +1018,8 @@ __global__ void __launch_bounds__(256) transpose_f32x4_kernel(
 template <typename U>
 __global__ void __launch_bounds__(256) concat_kernel(
     const U *lhs, const U *rhs, uint64_t outer, uint64_t lhs_len, uint64_t rhs_len, U *out) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     uint64_t row_len = lhs_len + rhs_len;
     uint64_t total   = outer * row_len;
     uint64_t stride  = (uint64_t)gridDim.x * 256;

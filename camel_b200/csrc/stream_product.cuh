@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     __shared__ __align__(2) int8_t exponent_s[8][128]; // of a stage's columns' largest magnitudes; a converting warp is at most six stages ahead of the draining ones
     volatile int *abort_flag = &abort_flag_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    griddep_launch_dependents();
     if (threadIdx.x == 0)
         abort_flag_s = *reinterpret_cast<volatile uint32_t *>(p.flags + FLAG_TIMEOUT) != 0 ? 1 : 0;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -140,6 +139,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const bool failed        = abort_flag_s != 0;
     __syncthreads(); // every thread has read abort_flag_s before a role may raise it
     griddep_wait();
+    griddep_launch_dependents();
     const int64_t begin = (int64_t)blockIdx.x * p.per, end = min(p.n, begin + p.per);
     const int tiles = (int)((end - begin + TILE - 1) / TILE), total = tiles * p.stages; // stages numbered across tiles
 
