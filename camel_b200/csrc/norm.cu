@@ -121,14 +121,18 @@ __device__ __forceinline__ float spread(float sum_d, float sum_dd, float inv_col
 
 template <int TPR> constexpr int kBlock = TPR <= 32 ? 256 : TPR; // several rows, or one
 
+// early: whether the next kernel may be launched meanwhile.  Not in place: a block's loads bring what lies beside its rows into the SM's first-level
+// cache, which the next kernel would find there as it was.
+
 template <int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t rows, int64_t cols, float eps,
-    float *__restrict__ out) {
+    float *__restrict__ out, int early) {
     using R = Row<TPR, V, VEC>;
     __shared__ float words1[1][32], words2[2][32];
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int t       = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kBlock<TPR> / TPR) + threadIdx.x / TPR;
     const int64_t mine = row < rows ? cols : 0; // a warp's last rows may not be there
@@ -176,10 +180,12 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_kernel(
 // Rows of any length, a block to a row, which is read three times.
 template <bool CHAINED>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(
-    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t cols, float eps, float *__restrict__ out) {
+    const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta, int64_t cols, float eps, float *__restrict__ out,
+    int early) {
     __shared__ float words1[1][32], words2[2][32];
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const float *src     = x + (int64_t)blockIdx.x * cols;
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
     float sum[1];
@@ -264,13 +270,14 @@ template <int TPR, int V, bool VEC> constexpr int kGradSmem = (kAhead * 2 * kSlo
 template <int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t rows, int64_t cols, float eps,
-    float *__restrict__ dx, float *__restrict__ partial, int pieces) {
+    float *__restrict__ dx, float *__restrict__ partial, int pieces, int early) {
     using R               = Row<TPR, V, VEC>;
     constexpr int THREADS = kBlock<TPR>, RPB = THREADS / TPR, SLOT = kSlot<TPR, V, VEC>;
     extern __shared__ __align__(128) float smem[];
     __shared__ float words1[1][32], words2[4][32];
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     float *ring    = smem + group * kAhead * 2 * SLOT; // [row][x, dout], column 0 up to three values behind the beginning
     float *gamma_s = smem + RPB * kAhead * 2 * SLOT;
@@ -380,10 +387,11 @@ __global__ void __launch_bounds__(kBlock<TPR>) layer_norm_grad_kernel(
 template <bool CHAINED>
 __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(
     const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ dout, int64_t cols, float eps, float *__restrict__ dx,
-    float2 *__restrict__ stats) {
+    float2 *__restrict__ stats, int early) {
     __shared__ float words1[1][32], words2[4][32];
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int64_t row    = blockIdx.x;
     const float *src     = x + row * cols, *dy = dout + row * cols;
     const float inv_cols = __fdiv_rn(1.0f, (float)cols);
@@ -466,9 +474,9 @@ ct_status launch_norm(const float *x, const float *gamma, const float *beta, int
     constexpr int RPB   = kBlock<TPR> / TPR;
     const dim3 grid((unsigned)((rows + RPB - 1) / RPB));
     if (vec)
-        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, true>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out));
+        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, true>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out, out != x));
     else
-        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, false>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out));
+        CT_CUDA(launch_dependent(layer_norm_kernel<TPR, V, false>, grid, dim3(kBlock<TPR>), 0, stream(), x, gamma, beta, rows, cols, eps, out, out != x));
     CT_LAUNCH_CHECK("layer_norm");
     return CT_OK;
 }
@@ -490,7 +498,7 @@ ct_status launch_norm_grad(
     if (sums)
         CT_TRY(partial.get((size_t)*blocks * 8 * cols));
     CT_CUDA(launch_dependent(kernel, dim3((unsigned)*blocks), dim3(kBlock<TPR>), SMEM, stream(), x, gamma, dout, rows, cols, eps, dx,
-                             sums ? partial.as<float>() : nullptr, aligned16(x) && aligned16(dout) ? 1 : 0));
+                             sums ? partial.as<float>() : nullptr, aligned16(x) && aligned16(dout) ? 1 : 0, dx != x && dx != dout));
     CT_LAUNCH_CHECK("layer_norm_grad");
     return CT_OK;
 }
@@ -562,7 +570,7 @@ ct_status ct_layer_norm(
         return CT_NORM(1024, 4);
 #undef CT_NORM
     auto kernel = cols <= kChainColumns ? layer_norm_long_kernel<false> : layer_norm_long_kernel<true>;
-    CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out));
+    CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, beta, cols, e, out, out != x));
     CT_LAUNCH_CHECK("layer_norm_long");
     return CT_OK;
 }
@@ -633,7 +641,7 @@ ct_status ct_layer_norm_grad(
         float *partial = sums ? scratch.as<float>(stats_bytes) : nullptr;
         auto rows_pass = [&](float *dx_to, float2 *stats_to) -> ct_status {
             auto kernel = cols <= kChainColumns ? layer_norm_grad_long_kernel<false> : layer_norm_grad_long_kernel<true>;
-            CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx_to, stats_to));
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)rows), dim3(1024), 0, stream(), x, gamma, dout, cols, e, dx_to, stats_to, dx_to != x && dx_to != dout));
             CT_LAUNCH_CHECK("layer_norm_grad_long");
             return CT_OK;
         };
