@@ -93,3 +93,96 @@ def test_operator_on_rewritten_inputs(name, m, k, n, precision):
         assert [run(False) == want for _ in range(10)] == [True] * 10
     finally:
         L.check(L.lib.ct_set_precision(L.PREC_3XTF32))
+
+
+# ---- sequences of operators over a few buffers ---------------------------------------------------------
+
+QUARTER = 1 << 18  # values; a buffer has four, an operator's operands are different quarters of different buffers
+
+
+def size(rng, most):
+    return max(1, int(round(np.exp(rng.uniform(0, np.log(most))))))
+
+
+def dimensions(rng):
+    while True:
+        m, k, n = size(rng, 3000), size(rng, 900), rng.integers(1, 18) if rng.uniform() < 0.3 else size(rng, 900)
+        if max(m * k, k * n, m * n) <= QUARTER:
+            return int(m), int(k), int(n)
+
+
+def any_call(rng, buffers, targets):
+    """One operator with operands and outputs in the buffers, no output over an operand except where operators allow it."""
+    i, j, l, o = rng.permutation(len(buffers))[:4]
+    m, k, n = dimensions(rng)
+    at = lambda b, quarter=0: buffers[b].ptr + quarter * QUARTER * 4  # noqa: E731
+    x, w, v, out = at(i), at(j, 1), at(l, 2), [at(o, q) for q in range(4)]
+    act, p, f = int(rng.integers(0, 3)), L.lib, L.F32
+    return [
+        lambda: p.ct_transpose(f, x, k, n, out[0]),
+        lambda: p.ct_matmul(f, x, f, w, m, k, n, out[0]),
+        lambda: p.ct_matmul_tn(x, w, k, m, n, out[0]),
+        lambda: p.ct_dense(x, w, v, m, k, n, act, out[0], None),
+        lambda: p.ct_sum_axis(f, x, m, k, act & 1, out[0]),
+        lambda: p.ct_binary(L.ADD, f, x, f, w, m * k, out[0]),
+        lambda: p.ct_binary(L.ADD, f, x, f, w, m * k, x),
+        lambda: p.ct_relu(x, m * k, out[0]),
+        lambda: p.ct_softmax_rows(x, m, k, out[0]),
+        lambda: p.ct_scaled_sub(x, w, 0.1, m * k, out[0]),
+        lambda: p.ct_fill(f, 0.25, m, out[0]),
+        lambda: p.ct_layer_norm(x, w, None, m, k, 1e-5, out[0]),
+        lambda: p.ct_layer_norm(x, None, None, m, k, 1e-5, x),
+        lambda: p.ct_layer_norm_grad(x, w, v, m, k, 1e-5, out[0], out[1], out[2]),
+        lambda: p.ct_dense_gated(x, w, None, v, None, m, k, n, L.GATE_SILU, out[0], out[1], out[2]),
+        lambda: p.ct_dense_gated_grad(x, w, v, at(i, 3), at(j, 3), at(l, 3), m, k, n, L.GATE_SILU, *out, out[3] + 4 * n),
+        lambda: p.ct_dense_cross_entropy(x, w, None, targets.ptr, m, k, n, out[0], out[1]),
+        lambda: p.ct_dense_cross_entropy_grad(x, w, None, targets.ptr, v, None, m, k, n, out[0], out[1], out[2]),
+    ][int(rng.integers(0, 18))]
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["3xtf32", "bf16"])
+@pytest.mark.parametrize("seed", range(4))
+def test_sequences_without_pauses(seed, precision):
+    """Sequences of up to 14 operators leave the same bytes in all buffers as with a pause behind each, and recorded and replayed, too."""
+    rng = np.random.default_rng(seed)
+    first = [T.from_numpy(rng.normal(0, 0.3, 4 * QUARTER).astype(np.float32)) for _ in range(5)]
+    buffers, kept = [T.zeros([4 * QUARTER]) for _ in first], [T.zeros([4 * QUARTER]) for _ in first]
+    targets = T.from_numpy(rng.integers(-1, 300, 4096))
+
+    def copy(to, source):
+        for a, b in zip(to, source):
+            L.check(L.lib.ct_d2d(a.ptr, b.ptr, a.nbytes))
+        T.sync()
+
+    def same():
+        equal = [T.Tensor(L.BOOL, (2 * QUARTER,)) for _ in buffers]
+        for e, a, b in zip(equal, buffers, kept):  # two values as an int64: NaN equals itself
+            L.check(L.lib.ct_compare(L.EQ, L.I64, a.ptr, L.I64, b.ptr, 2 * QUARTER, e.ptr))
+        return all(e.numpy().all() for e in equal)
+
+    L.check(L.lib.ct_set_precision(L.PREC_BF16 if precision == "bf16" else L.PREC_3XTF32))
+    try:
+        for number in range(200):
+            calls = [any_call(rng, buffers, targets) for _ in range(int(rng.integers(3, 15)))]
+            copy(buffers, first)
+            for call in calls:
+                L.check(call())
+                T.sync()
+            copy(kept, buffers)
+            for again in range(3):
+                copy(buffers, first)
+                for call in calls:
+                    L.check(call())
+                T.check_async()
+                assert same(), (number, again)
+            with T.Graph() as graph:
+                for call in calls:
+                    L.check(call())
+            copy(buffers, first)
+            graph.launch()
+            T.check_async()
+            assert same(), (number, "recorded")
+            del graph  # not while the next one records
+    finally:
+        L.check(L.lib.ct_set_precision(L.PREC_3XTF32))
