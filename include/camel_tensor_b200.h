@@ -20,6 +20,9 @@
  *  - Kernels are enqueued on the stream set by ct_set_stream (default: the legacy default
  *    stream).  Functions that return a host value, or that must report a data-dependent
  *    error, synchronise that stream before returning; the others do not.
+ *  - Products, convolutions and sums use workspaces that the device has once: their calls (and
+ *    recordings of them) on different streams must not run at the same time, except where a
+ *    function says that they may.
  *  - There is no CPU fallback: without a usable CUDA device every compute entry point
  *    returns CT_ERR_NO_DEVICE.
  *  - The selected device belongs to the process, not to the calling thread: every entry point
@@ -356,8 +359,10 @@ ct_status ct_dense_packed(
  * over): to 2^-23 of a value down to 2^-27 of its line's largest, to 2^-50 of that largest below; the product of two low terms is left out.
  * The error of a sum is at most 2^-21 of its products' sizes and 2^-48 of its length times the two lines' largest, and the additions' (by
  * 16 terms to 2^-23, by 128 to 2^-24, in float32).  Unlike ct_dense's, lines of a wider range are not computed another way.  A sum
- * that meets an infinity of an operand is infinite or NaN (infinity times a low term of zero).  Under CT_PREC_BF16 the products
- * are those of ct_dense. */
+ * that meets an infinity of an operand is infinite or NaN (infinity times a low term of zero).
+ *
+ * Scratch memory belongs to a call: calls and recordings of these functions on different streams may run at the same time.  Not so
+ * under CT_PREC_BF16, where the products are those of ct_dense, with its workspaces. */
 
 /* Layer norm of each row: out = (x - mean) / sqrt(var + eps) * gamma + beta, mean and var (the mean square deviation) over the
  * row's `cols` values.  gamma and beta have one value per column; null: ones, zeros.  eps >= 0.  out may be x itself. */
