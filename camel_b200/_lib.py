@@ -108,6 +108,12 @@ PROTOTYPES = {
     "ct_dense_gated_grad": (_int, [_vp] * 6 + [_i64] * 3 + [_int] + [_vp] * 5),
     "ct_dense_cross_entropy": (_int, [_vp] * 4 + [_i64] * 3 + [_vp, _vp]),
     "ct_dense_cross_entropy_grad": (_int, [_vp] * 6 + [_i64] * 3 + [_vp, _vp, _vp]),
+    "ct_embedding": (_int, [_vp, _vp] + [_i64] * 3 + [_dbl, _vp]),
+    "ct_embedding_grad": (_int, [_vp, _vp] + [_i64] * 3 + [_dbl, _vp]),
+    "ct_gated_scan": (_int, [_vp] * 4 + [_i64] * 3 + [_vp, _vp]),
+    "ct_gated_scan_grad": (_int, [_vp] * 7 + [_i64] * 3 + [_vp] * 3),
+    "ct_distill": (_int, [_vp] * 3 + [_i64] * 3 + [_dbl, _vp, _vp]),
+    "ct_distill_grad": (_int, [_vp] * 5 + [_i64] * 3 + [_dbl, _vp]),
     "ct_conv2d": (_int, [_vp, _vp, _vp] + [_i64] * 9 + [_int, _vp]),
     "ct_conv2d_maxpool2": (_int, [_vp, _vp, _vp] + [_i64] * 9 + [_int, _vp]),
     "ct_maxpool2d": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _vp]),

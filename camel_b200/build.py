@@ -19,7 +19,8 @@ OBJ_DIR = ROOT / "build"
 LIB = ROOT / "libcamel_tensor_b200.so"
 
 SOURCES = ["runtime.cu", "elementwise.cu", "reduce.cu", "gemm_simt.cu", "gemm_tc.cu", "gemm_half.cu", "gemm_direct.cu", "gemm_panel.cu", "contract.cu",
-           "graph.cu", "peak.cu", "conv_tmem.cu", "conv_halo.cu", "norm.cu", "fused_product.cu", "few_rows.cu", "gated.cu", "cross_entropy.cu"]
+           "graph.cu", "peak.cu", "conv_tmem.cu", "conv_halo.cu", "norm.cu", "fused_product.cu", "few_rows.cu", "gated.cu", "cross_entropy.cu",
+           "embedding.cu", "gated_scan.cu", "distill.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

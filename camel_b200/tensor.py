@@ -701,6 +701,114 @@ def dense_cross_entropy_grad(x: Tensor, w: Tensor, targets: Tensor, lse: Tensor,
     return (dx, dw, *db)
 
 
+# ---- networks over sequences of tokens ------------------------------------------------------
+
+
+def _int_values(t: Tensor | None, name: str, what: str, shape: tuple):
+    """Device pointer of an int tensor of a shape."""
+    if not _is_tensor(t) or t.dtype != L.I64 or t.shape != shape:
+        raise _invalid(f"{name}: {what} must be an int tensor of shape {list(shape)}")
+    return t.ptr
+
+
+def embedding(table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
+    """Rows ids of table, times scale: [*ids.shape, k]; an id outside the table (-1, say) is padding, whose row is zeros."""
+    _float_matrix(table, "embedding")
+    if not _is_tensor(ids):
+        raise _invalid("Expected Tensor argument")
+    pids = _int_values(ids, "embedding", "ids", ids.shape)
+    n, k = table.shape
+    out = Tensor(L.F32, (*ids.shape, k))
+    check(lib.ct_embedding(table.ptr, pids, ids.numel, n, k, float(scale), out.ptr))
+    return out
+
+
+def embedding_grad(ids: Tensor, dout: Tensor, rows: int, scale: float = 1.0) -> Tensor:
+    """The gradient [rows, k] of embedding's table from that of its output; the same bytes at every call."""
+    if not _is_tensor(ids) or not _is_tensor(dout):
+        raise _invalid("Expected Tensor argument")
+    pids = _int_values(ids, "embedding_grad", "ids", ids.shape)
+    _require_float(dout, "embedding_grad")
+    if dout.rank != ids.rank + 1 or dout.shape[:-1] != ids.shape:
+        raise _invalid("embedding_grad dimension mismatch")
+    if rows < 0:
+        raise _invalid("embedding_grad: negative dimension")
+    k = dout.shape[-1]
+    dtable = Tensor(L.F32, (rows, k))
+    check(lib.ct_embedding_grad(pids, dout.ptr, ids.numel, rows, k, float(scale), dtable.ptr))
+    return dtable
+
+
+def _scan_args(name: str, gate: Tensor, others: tuple, lengths: Tensor | None):
+    for t in (gate, *others):
+        if not _is_tensor(t):
+            raise _invalid("Expected Tensor argument")
+        _require_float(t, name)
+        if t.rank != 3:
+            raise _invalid(f"{name} currently only supports rank-3 tensors [batch, steps, channels]")
+        if t.shape != gate.shape:
+            raise _invalid(f"{name} dimension mismatch")
+    b, t, c = gate.shape
+    return b, t, c, None if lengths is None else _int_values(lengths, name, "lengths", (b,))
+
+
+def _state_arg(state: Tensor | None, name: str, what: str, b: int, c: int):
+    if state is not None and (not _is_tensor(state) or state.dtype != L.F32 or state.shape != (b, c)):
+        raise _invalid(f"{name}: {what} must be a float tensor of shape {[b, c]}")
+    return None if state is None else state.ptr
+
+
+def gated_scan(gate: Tensor, value: Tensor, state: Tensor | None = None, lengths: Tensor | None = None):
+    """(out, state) of h[t] = a h[t-1] + (1 - a) value[t], a = sigmoid(gate[t]), along the steps of each sequence [batch, steps, channels];
+    the state after the last step goes into the next call.  Steps from lengths[b] on are padding."""
+    b, t, c, plen = _scan_args("gated_scan", gate, (value,), lengths)
+    p0 = _state_arg(state, "gated_scan", "state", b, c)
+    out, last = Tensor(L.F32, gate.shape), Tensor(L.F32, (b, c))
+    check(lib.ct_gated_scan(gate.ptr, value.ptr, p0, plen, b, t, c, out.ptr, last.ptr))
+    return out, last
+
+
+def gated_scan_grad(gate: Tensor, value: Tensor, out: Tensor, dout: Tensor, state: Tensor | None = None, lengths: Tensor | None = None,
+                    dstate: Tensor | None = None):
+    """(dgate, dvalue) of gated_scan from its output and the gradients of its output and, where it is given, of its last state; with state also
+    that of the state it began with."""
+    b, t, c, plen = _scan_args("gated_scan_grad", gate, (value, out, dout), lengths)
+    p0, pd = _state_arg(state, "gated_scan_grad", "state", b, c), _state_arg(dstate, "gated_scan_grad", "dstate", b, c)
+    dgate, dvalue = Tensor(L.F32, gate.shape), Tensor(L.F32, gate.shape)
+    dfirst = (Tensor(L.F32, (b, c)),) if state is not None else ()
+    check(lib.ct_gated_scan_grad(gate.ptr, value.ptr, p0, plen, out.ptr, dout.ptr, pd, b, t, c, dgate.ptr, dvalue.ptr,
+                                 dfirst[0].ptr if dfirst else None))
+    return (dgate, dvalue, *dfirst)
+
+
+def _distill_args(name: str, logits: Tensor, ids: Tensor, teacher: Tensor):
+    _float_matrix(logits, name)
+    m, n = logits.shape
+    _float_matrix(teacher, name, m)
+    top = teacher.shape[1]
+    return m, n, top, _int_values(ids, name, "ids", (m, top))
+
+
+def distill(logits: Tensor, ids: Tensor, teacher: Tensor, temperature: float = 1.0):
+    """(loss, lse) of each row: T^2 times the divergence of softmax(logits / T) from softmax(teacher / T) over the row's entries, the classes ids with
+    the logits teacher of a larger network; an id outside the classes is no entry, and a row without entries has loss 0."""
+    m, n, top, pids = _distill_args("distill", logits, ids, teacher)
+    loss, lse = Tensor(L.F32, (m,)), Tensor(L.F32, (m,))
+    check(lib.ct_distill(logits.ptr, pids, teacher.ptr, m, n, top, float(temperature), loss.ptr, lse.ptr))
+    return loss, lse
+
+
+def distill_grad(logits: Tensor, ids: Tensor, teacher: Tensor, lse: Tensor, temperature: float = 1.0, dloss: Tensor | None = None) -> Tensor:
+    """The gradient of the sum of distill's losses, weighted by dloss where it is given."""
+    m, n, top, pids = _distill_args("distill_grad", logits, ids, teacher)
+    if lse is None:
+        raise _invalid("Expected Tensor argument")
+    plse, pd = _float_values(lse, "distill_grad", "lse", m), _float_values(dloss, "distill_grad", "dloss", m)
+    out = Tensor(L.F32, (m, n))
+    check(lib.ct_distill_grad(logits.ptr, pids, teacher.ptr, plse, pd, m, n, top, float(temperature), out.ptr))
+    return out
+
+
 class Graph:
     """Records the operator calls made inside `with Graph() as g:` and replays them with
     `g.launch()` (one CUDA-graph launch).  Tensors created inside the block and still referenced

@@ -404,6 +404,57 @@ ct_status ct_dense_cross_entropy_grad(
     const float *x_dev, const float *w_dev, const float *bias_dev, const int64_t *targets_dev, const float *lse_dev,
     const float *dloss_dev, int64_t m, int64_t k, int64_t n, float *dx_dev, float *dw_dev, float *dbias_dev);
 
+/* ---- networks over sequences of tokens -----------------------------------------------------
+ * What such a network has around its dense layers: the way in, what carries along a sequence, and the loss of one that learns from a larger
+ * one's answers.  As above: dense row-major float32, outputs that overlap nothing else except where a function says so, gradients weighted by
+ * the given one, dimensions up to 2^29, scratch memory that belongs to the call.  These use no workspace in any precision: calls and recordings of them on
+ * different streams may run at the same time. */
+
+/* Embedding lookup: out[i] = scale * table[ids[i]], table [n][k], ids [m] int64, out [m][k].  An id outside 0 .. n-1 is padding: its row of out
+ * is zeros.  scale is rounded to float32 and must be finite there; it multiplies in float32. */
+ct_status ct_embedding(
+    const float *table_dev, const int64_t *ids_dev, int64_t m, int64_t n, int64_t k, double scale, float *out_dev);
+/* The gradient of its table from the gradient dout [m][k] of its output: dtable[v] = scale * (sum of dout[i] over the i with ids[i] = v), every row
+ * of dtable [n][k] written, zeros where no id is.  Rows of padding take no part, whatever dout holds there.  Sums are in 64 bits, in an order
+ * that the ids alone decide, and rounded once: the same call gives the same bytes. */
+ct_status ct_embedding_grad(
+    const int64_t *ids_dev, const float *dout_dev, int64_t m, int64_t n, int64_t k, double scale, float *dtable_dev);
+
+/* Gated scan, a linear recurrence along the steps of each sequence: with a = sigmoid(gate),
+ *   h[t] = a[t] * h[t-1] + (1 - a[t]) * value[t],   h[-1] = state0
+ * gate, value and out [batch][steps][channels], out[t] = h[t]; state0 and state [batch][channels], state the last h; lengths [batch] int64.
+ * state0 null: zeros.  lengths null: all sequences have all steps; else steps from lengths[b] on (0 below, `steps` above) are padding: out is zero
+ * there and state that of the last step before, whatever gate and value hold.  out or state may be null, and state may be state0 itself: with
+ * steps = 1 a call moves the states of a batch that is being answered by one token.
+ * The error of h is a few roundings of the largest |value| and |state0| so far, however long a gate near 1 remembers (a and 1 - a each have their own
+ * digits, and states are carried between pieces of the steps in 64 bits; the smaller of the two is 0 below 2^-126, beyond gates of 87).  A state that is infinite or NaN leaves such values behind it. */
+ct_status ct_gated_scan(
+    const float *gate_dev, const float *value_dev, const float *state0_dev, const int64_t *lengths_dev, int64_t batch, int64_t steps, int64_t channels,
+    float *out_dev, float *state_dev);
+/* Its gradient, with out as the forward call left it, dout [batch][steps][channels] and dstate [batch][channels] (null: zeros), the gradients of out and
+ * state:  g[t] = dout[t] + a[t+1] * g[t+1], the last step's with dstate,
+ *   dvalue = (1 - a) * g,  dgate[t] = a * (1 - a) * g * (h[t-1] - value[t]),  dstate0 = a[0] * g[0] (of no steps dstate).
+ * Zeros at padding, whatever dout holds there.  Each output may be null; dstate0 may be dstate. */
+ct_status ct_gated_scan_grad(
+    const float *gate_dev, const float *value_dev, const float *state0_dev, const int64_t *lengths_dev, const float *out_dev, const float *dout_dev,
+    const float *dstate_dev, int64_t batch, int64_t steps, int64_t channels, float *dgate_dev, float *dvalue_dev, float *dstate0_dev);
+
+/* Distillation from a teacher's top logits.  Row i of logits [m][n] is the student's z; its entries are the classes ids[i][..] (int64, [m][top], in any order)
+ * with the teacher's logits teacher[i][..].  With p = softmax(teacher / T) over the row's entries and q = softmax(z / T) over its classes
+ *   loss[i] = T^2 * (sum over entries of p * (log p - log q[class])),   lse[i] = log(sum over classes of exp(z / T))
+ * An id outside 0 .. n-1 is no entry (a row may have fewer than top); a row without entries is padding: its loss is 0, whatever its logits hold.  Entries of
+ * the same class count each.  An entry of weight 0 (teacher -infinity) adds nothing; otherwise infinities and NaN as for ct_dense_cross_entropy.  T is the
+ * temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null. */
+ct_status ct_distill(
+    const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, int64_t m, int64_t n, int64_t top, double temperature, float *loss_dev,
+    float *lse_dev);
+/* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
+ *   dlogits[i][c] = dloss[i] * T * (exp(z[c] / T - lse[i]) - (sum of p over the row's entries of class c)), zeros in rows without entries.
+ * dlogits may be logits itself. */
+ct_status ct_distill_grad(
+    const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, const float *lse_dev, const float *dloss_dev, int64_t m, int64_t n,
+    int64_t top, double temperature, float *dlogits_dev);
+
 /* conv2d, NCHW input [n,c,h,w], OIHW weights [k_out,c,kh,kw], zero padding, then + bias and
  * activation (NONE or RELU).  No reference counterpart (the reference has no conv operator);
  * arithmetic follows the reference's style: one accumulation per output over (c,kh,kw). */
