@@ -9,8 +9,10 @@
 // that out for its steps, takes what the pieces before its own do to the state of the tile's beginning, and then goes through its steps.  The next tile's values are
 // on their way meanwhile.  The gradient is the same along the reversed axis, of c[t] = a[t] g[t] = a[t] (dout[t] + c[t+1]).
 //
-// Of a gate only the smaller of a and 1 - a is kept, with all its digits (the sign tells which): a state moves from h towards value by 1 - a, or from
-// value towards h by a.  Held as a float32, an `a` near 1 would be off by 2^-25, which a state that remembers 1 / (1 - a) steps adds up.
+// Of a gate both a and 1 - a are taken with all their digits (sigmoids): a product of `a`s, each off by 2^-25 of 1, would be off by what 1 - a loses
+// of its digits, and a state that remembers 1 / (1 - a) steps would add that up.  A lane's steps therefore do to a state h what is a product A and
+// what they add, b, and their 1 - A is summed up by itself, S' = a S + (1 - a).  A is 1 - S in 64 bits, or, from where S has more than 1/2, the
+// product, which is then small and has its digits.  Between pieces states are in 64 bits.
 #include "common.cuh"
 #include "gate.cuh"
 #include "tc_ptx.cuh"
@@ -22,73 +24,95 @@ namespace {
 
 using namespace ptx;
 
-// The smaller of a and 1 - a: 1 - a as it is, a with its sign bit set.
-__device__ __forceinline__ float smaller_side(float gate) {
-    float a, rest;
-    sigmoids(gate, a, rest);
-    return gate >= 0.0f ? rest : -a;
-}
-__device__ __forceinline__ bool keeps(float side) { return __float_as_int(side) >= 0; } // a >= 1/2
-// a h + (1 - a) v
-__device__ __forceinline__ float move(float side, float h, float v) {
-    const float from = keeps(side) ? h : v, to = keeps(side) ? v : h;
-    return __fmaf_rn(fabsf(side), __fsub_rn(to, from), from);
-}
-// a x
-__device__ __forceinline__ float times_a(float side, float x) { return keeps(side) ? __fmaf_rn(-side, x, x) : __fmul_rn(-side, x); }
-__device__ __forceinline__ float one_minus_a(float side) { return keeps(side) ? side : __fadd_rn(1.0f, side); }
-
-// What a piece of a chain does to the state before it: a h + b, a held like a gate's.
+// What steps do to the state before them: a h + b.
 struct Piece {
-    float side, b;
+    float a = 1.0f, lost = 0.0f, b = 0.0f; // lost: 1 - a
+    __device__ __forceinline__ void step(float ga, float rest, float add) {
+        b    = __fmaf_rn(ga, b, add);
+        lost = __fmaf_rn(ga, lost, rest);
+        a    = __fmul_rn(ga, a);
+    }
+    __device__ __forceinline__ double2 joined() const { return make_double2(lost <= 0.5f ? 1.0 - (double)lost : (double)a, (double)b); }
 };
-__device__ __forceinline__ double apply(Piece p, double h) {
-    const double a = keeps(p.side) ? 1.0 - (double)p.side : -(double)p.side;
-    return fma(a, h, (double)p.b);
-}
+
+constexpr int kMostBlocks = 8; // of a cluster
 
 // The state before each warp's steps, from what all pieces of the tile do; `state` goes on to the tile's end.  Pieces lie in the order of warps, and
-// of the cluster's blocks.  One call after the other alternates between two places (turn), so that a fast warp does not write over what a slow one reads.
+// of the cluster's blocks.  One tile after the other alternates between two places, so that a fast warp does not write over what a slow one reads.
+// Blocks send what their pieces do to one another by st.async, whose arrival a barrier counts: a cluster-wide barrier would wait until the last
+// tile's stores to global memory are done.
 template <int W> struct Exchange {
-    Piece pieces[2][W][32];
-    double2 blocks[2][16][32]; // (a, b) of the cluster's blocks
+    double2 pieces[2][W][32];
+    double2 blocks[2][kMostBlocks][32];
+    uint64_t arrived[2];
+    int gave_up;
 };
+__device__ __forceinline__ void send(uint32_t at, uint32_t barrier, double2 p) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(at), "d"(p.x), "d"(p.y), "r"(barrier)
+                 : "memory");
+}
 template <int W>
-__device__ __forceinline__ double exchange(Exchange<W> &e, int turn, Piece mine, double &state, int warp, int lane, int blocks, uint32_t rank) {
-    e.pieces[turn][warp][lane] = mine;
+__device__ __forceinline__ double exchange(Exchange<W> &e, int tile, Piece mine, double &state, int warp, int lane, int blocks, uint32_t rank) {
+    const int turn             = tile & 1;
+    e.pieces[turn][warp][lane] = mine.joined();
     __syncthreads();
     double before = state;
-    if (blocks > 1) {
-        if (warp == 0) {
-            double a = 1.0, b = 0.0;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const Piece p = e.pieces[turn][w][lane];
-                b             = apply(p, b);
-                a *= keeps(p.side) ? 1.0 - (double)p.side : -(double)p.side;
-            }
-            const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(&e.blocks[turn][rank][lane]));
-            for (int r = 0; r < blocks; ++r)
-                asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(mapa(at, r)), "d"(a), "d"(b) : "memory");
-        }
-        cluster_sync();
-        for (int r = 0; r < blocks; ++r) {
-            const double2 p = e.blocks[turn][r][lane];
-            before          = r == (int)rank ? state : before;
-            state           = fma(p.x, state, p.y);
-        }
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-            if (w < warp)
-                before = apply(e.pieces[turn][w][lane], before);
-    } else {
+    if (blocks == 1) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            before = w == warp ? state : before;
-            state  = apply(e.pieces[turn][w][lane], state);
+            before          = w == warp ? state : before;
+            const double2 p = e.pieces[turn][w][lane];
+            state           = fma(p.x, state, p.y);
         }
+        return before;
     }
-    return before;
+    // what the warps before this one do, and the last warp's with it: the block's
+    double a = 1.0, b = 0.0;
+    const int upto = warp == W - 1 ? W : warp;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        if (w < upto) {
+            const double2 p = e.pieces[turn][w][lane];
+            if (w == W - 1) {
+                const uint32_t at  = static_cast<uint32_t>(__cvta_generic_to_shared(&e.blocks[turn][rank][lane]));
+                const uint32_t bar = static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[turn]));
+                const double2 all  = make_double2(a * p.x, fma(p.x, b, p.y));
+                if (lane == 0)
+                    mbar_expect_tx(bar, blocks * 512);
+                for (int r = 0; r < blocks; ++r)
+                    send(mapa(at, r), mapa(bar, r), all);
+            } else {
+                b = fma(p.x, b, p.y);
+                a *= p.x;
+            }
+        }
+    // a wait that has run out is reported by the kernel's end; until then the block goes on, for the others' sake
+    if (!*(volatile int *)&e.gave_up)
+        mbar_wait<kClusterWritten>(static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[turn])), (tile >> 1) & 1, &e.gave_up);
+    for (int r = 0; r < blocks; ++r) {
+        const double2 p = e.blocks[turn][r][lane];
+        before          = r == (int)rank ? state : before;
+        state           = fma(p.x, state, p.y);
+    }
+    return fma(a, before, b);
+}
+template <int W> __device__ __forceinline__ void exchange_begin(Exchange<W> &e, int blocks) {
+    if (blocks == 1)
+        return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i)
+            mbar_init(static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[i])), 1);
+        e.gave_up = 0;
+        mbar_fence_init();
+    }
+    cluster_sync();
+}
+template <int W> __device__ __forceinline__ void exchange_end(Exchange<W> &e, int blocks, uint32_t *flags) {
+    if (blocks == 1)
+        return;
+    cluster_sync(); // nothing is on its way to a block that has ended
+    if (threadIdx.x == 0 && e.gave_up)
+        atomicMax(&flags[FLAG_TIMEOUT], 1u + blockIdx.x);
 }
 
 struct Chain {
@@ -100,10 +124,10 @@ struct Chain {
 __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t steps, int64_t channels, const int64_t *__restrict__ lengths) {
     Chain c;
     c.here          = index < chains;
-    c.index         = index;
-    const int64_t b = index / channels;
-    c.first         = b * steps * channels + (index - b * channels);
-    c.steps         = steps;
+    c.index         = c.here ? index : 0;
+    const int64_t b = c.index / channels;
+    c.first         = b * steps * channels + (c.index - b * channels);
+    c.steps         = c.here ? steps : 0;
     if (c.here && lengths) {
         const int64_t length = lengths[b];
         c.steps              = length < 0 ? 0 : (length < steps ? length : steps);
@@ -111,78 +135,84 @@ __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t
     return c;
 }
 
-// W warps to a block; the blocks of a cluster have the same 32 chains.
-template <int W, int S>
-__global__ void __launch_bounds__(W * 32) gated_scan_kernel(
+// W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
+template <int W, int S, int FIT>
+__global__ void __launch_bounds__(W * 32, FIT) gated_scan_kernel(
     const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths, int64_t chains,
-    int64_t steps, int64_t channels, int blocks, float *__restrict__ out, float *state_out) {
+    int64_t steps, int channels, int blocks, float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
     __shared__ Exchange<W> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = blocks > 1 ? cluster_rank() : 0;
-    if (blocks > 1)
-        cluster_sync(); // every block of the cluster runs before another writes into its memory
+    exchange_begin(ex, blocks);
     griddep_wait();
-    const Chain c     = chain_of((int64_t)(blockIdx.x / blocks) * 32 + lane, chains, steps, channels, lengths);
-    double state      = c.here && state0 ? (double)state0[c.index] : 0.0;
+    const Chain c      = chain_of((int64_t)(blockIdx.x / blocks) * 32 + lane, chains, steps, channels, lengths);
+    double state       = c.here && state0 ? (double)state0[c.index] : 0.0;
     const int64_t tile = (int64_t)blocks * W * S;
     int64_t t0         = ((int64_t)rank * W + warp) * S;
-    const float *pg = gate + c.first, *pv = value + c.first;
     float g[S], v[S];
+    // Steps that a chain does not have keep its state: a = 1, and nothing is added.
     auto fetch = [&](int64_t t) {
+        const float *pg = gate + c.first + t * channels, *pv = value + c.first + t * channels;
+        if (__all_sync(0xffffffffu, t + S <= c.steps)) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in = c.here && t + i < c.steps;
-            g[i]          = in ? __ldcs(pg + (t + i) * channels) : 0.0f;
-            v[i]          = in ? __ldcs(pv + (t + i) * channels) : 0.0f;
+            for (int i = 0; i < S; ++i)
+                g[i] = __ldcs(pg + (int64_t)i * channels), v[i] = __ldcs(pv + (int64_t)i * channels);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const bool in = t + i < c.steps;
+                g[i]          = in ? __ldcs(pg + (int64_t)i * channels) : INFINITY;
+                v[i]          = in ? __ldcs(pv + (int64_t)i * channels) : 0.0f;
+            }
         }
     };
     fetch(t0);
-    int turn = 0;
-    for (int64_t base = 0; base < steps; base += tile, t0 += tile, turn ^= 1) {
-        float side[S], val[S];
-        Piece mine = {0.0f, 0.0f};
-        float a    = 1.0f;
+    const int tiles = (int)((steps + tile - 1) / tile);
+    for (int i = 0; i < tiles; ++i, t0 += tile) {
+        float a[S], add[S];
+        Piece mine;
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in = t0 + i < c.steps;
-            side[i]       = in ? smaller_side(g[i]) : 0.0f;
-            val[i]        = v[i];
-            if (in) {
-                mine.b    = move(side[i], mine.b, val[i]);
-                mine.side = move(side[i], mine.side, 1.0f); // 1 - the product of all a
-                a         = times_a(side[i], a);
-            }
+        for (int j = 0; j < S; ++j) {
+            float rest;
+            sigmoids(g[j], a[j], rest);
+            add[j] = __fmul_rn(rest, v[j]);
+            mine.step(a[j], rest, add[j]);
         }
-        if (a < 0.5f)
-            mine.side = -a;
         fetch(t0 + tile);
-        float h = (float)exchange<W>(ex, turn, mine, state, warp, lane, blocks, rank);
-        if (out && c.here) {
+        float h = (float)exchange(ex, i, mine, state, warp, lane, blocks, rank);
+        if (out) {
+            float *to = out + c.first + t0 * channels;
+            if (__all_sync(0xffffffffu, t0 + S <= c.steps)) {
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool in = t0 + i < c.steps;
-                if (in)
-                    h = move(side[i], h, val[i]);
-                if (t0 + i < steps)
-                    __stcs(out + c.first + (t0 + i) * channels, in ? h : 0.0f);
+                for (int j = 0; j < S; ++j) {
+                    h = __fmaf_rn(a[j], h, add[j]);
+                    __stcs(to + (int64_t)j * channels, h);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < S; ++j) {
+                    h = __fmaf_rn(a[j], h, add[j]);
+                    if (c.here && t0 + j < steps)
+                        __stcs(to + (int64_t)j * channels, t0 + j < c.steps ? h : 0.0f);
+                }
             }
         }
     }
     if (state_out && warp == 0 && rank == 0 && c.here)
         state_out[c.index] = (float)state;
+    exchange_end(ex, blocks, flags);
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
-template <int W, int S>
-__global__ void __launch_bounds__(W * 32) gated_scan_grad_kernel(
+template <int W, int S, int FIT>
+__global__ void __launch_bounds__(W * 32, FIT) gated_scan_grad_kernel(
     const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths,
-    const float *__restrict__ out, const float *__restrict__ dout, const float *dstate, int64_t chains, int64_t steps, int64_t channels, int blocks,
-    float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0) {
+    const float *__restrict__ out, const float *__restrict__ dout, const float *dstate, int64_t chains, int64_t steps, int channels, int blocks,
+    float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
     __shared__ Exchange<W> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = blocks > 1 ? cluster_rank() : 0;
-    if (blocks > 1)
-        cluster_sync();
+    exchange_begin(ex, blocks);
     griddep_wait();
     const Chain c      = chain_of((int64_t)(blockIdx.x / blocks) * 32 + lane, chains, steps, channels, lengths);
     double state       = c.here && dstate ? (double)dstate[c.index] : 0.0; // c[t+1]
@@ -191,61 +221,57 @@ __global__ void __launch_bounds__(W * 32) gated_scan_grad_kernel(
     int64_t t1         = steps - 1 - ((int64_t)rank * W + warp) * S; // the piece's last step
     float g[S], v[S], d[S], h[S];
     auto fetch = [&](int64_t t) {
+        const int64_t at = c.first + t * channels;
+        if (__all_sync(0xffffffffu, t < c.steps && t >= S)) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in    = c.here && t - i >= 0 && t - i < c.steps;
-            const int64_t at = c.first + (t - i) * channels;
-            g[i]             = in ? __ldcs(gate + at) : 0.0f;
-            v[i]             = in ? __ldcs(value + at) : 0.0f;
-            d[i]             = in ? __ldcs(dout + at) : 0.0f;
-            h[i]             = in ? (t - i > 0 ? __ldcs(out + at - channels) : first) : 0.0f;
+            for (int i = 0; i < S; ++i) {
+                g[i] = __ldcs(gate + at - (int64_t)i * channels), v[i] = __ldcs(value + at - (int64_t)i * channels);
+                d[i] = __ldcs(dout + at - (int64_t)i * channels), h[i] = __ldcs(out + at - (int64_t)(i + 1) * channels);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const bool in = t - i >= 0 && t - i < c.steps;
+                g[i]          = in ? __ldcs(gate + at - (int64_t)i * channels) : INFINITY;
+                v[i]          = in ? __ldcs(value + at - (int64_t)i * channels) : 0.0f;
+                d[i]          = in ? __ldcs(dout + at - (int64_t)i * channels) : 0.0f;
+                h[i]          = in ? (t - i > 0 ? __ldcs(out + at - (int64_t)(i + 1) * channels) : first) : 0.0f;
+            }
         }
     };
     fetch(t1);
-    int turn = 0;
-    for (int64_t base = 0; base < steps; base += tile, t1 -= tile, turn ^= 1) {
-        float side[S], gap[S], dy[S];
-        Piece mine = {0.0f, 0.0f};
-        float a    = 1.0f;
+    const int tiles = (int)((steps + tile - 1) / tile);
+    for (int i = 0; i < tiles; ++i, t1 -= tile) {
+        float a[S], rest[S], gap[S], dy[S];
+        Piece mine;
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const bool in = t1 - i >= 0 && t1 - i < c.steps;
-            side[i]       = in ? smaller_side(g[i]) : 0.0f;
-            gap[i]        = __fsub_rn(h[i], v[i]);
-            dy[i]         = d[i];
-            if (in) {
-                mine.b    = times_a(side[i], __fadd_rn(dy[i], mine.b));
-                mine.side = move(side[i], mine.side, 1.0f);
-                a         = times_a(side[i], a);
-            }
+        for (int j = 0; j < S; ++j) {
+            sigmoids(g[j], a[j], rest[j]);
+            gap[j] = __fsub_rn(h[j], v[j]);
+            dy[j]  = d[j];
+            mine.step(a[j], rest[j], __fmul_rn(a[j], dy[j]));
         }
-        if (a < 0.5f)
-            mine.side = -a;
         fetch(t1 - tile);
-        float carry = (float)exchange<W>(ex, turn, mine, state, warp, lane, blocks, rank);
-        if (c.here) {
+        float carry = (float)exchange(ex, i, mine, state, warp, lane, blocks, rank);
+        const int64_t at = c.first + t1 * channels;
+        const bool whole = __all_sync(0xffffffffu, t1 < c.steps && t1 >= S - 1);
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool in    = t1 - i >= 0 && t1 - i < c.steps;
-                const int64_t at = c.first + (t1 - i) * channels;
-                float dv = 0.0f, dg = 0.0f;
-                if (in) {
-                    const float x = __fadd_rn(dy[i], carry), rest = one_minus_a(side[i]);
-                    carry = times_a(side[i], x);
-                    dv    = __fmul_rn(rest, x);
-                    dg    = __fmul_rn(__fmul_rn(rest, carry), gap[i]);
-                }
-                if (t1 - i >= 0) {
-                    if (dvalue)
-                        __stcs(dvalue + at, dv);
-                    if (dgate)
-                        __stcs(dgate + at, dg);
-                }
+        for (int j = 0; j < S; ++j) {
+            const float x = __fadd_rn(dy[j], carry);
+            carry         = __fmul_rn(a[j], x);
+            const float dv = __fmul_rn(rest[j], x), dg = __fmul_rn(__fmul_rn(rest[j], carry), gap[j]);
+            if (whole || (c.here && t1 - j >= 0)) {
+                const bool in = whole || t1 - j < c.steps;
+                if (dvalue)
+                    __stcs(dvalue + at - (int64_t)j * channels, in ? dv : 0.0f);
+                if (dgate)
+                    __stcs(dgate + at - (int64_t)j * channels, in ? dg : 0.0f);
             }
         }
     }
     if (dstate0 && warp == 0 && rank == 0 && c.here)
         dstate0[c.index] = (float)state;
+    exchange_end(ex, blocks, flags);
 }
 
 ct_status check_scan(const char *name, int64_t batch, int64_t steps, int64_t channels) {
@@ -290,8 +316,8 @@ ct_status ct_gated_scan(
     constexpr int W = 8, S = 16;
     const int64_t groups = (chains + 31) / 32;
     const int blocks     = scan_blocks(st, groups, steps, W * S);
-    CT_CUDA(launch_dependent_cluster(gated_scan_kernel<W, S>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
-                                     lengths, chains, steps, channels, blocks, out, state));
+    CT_CUDA(launch_dependent_cluster(gated_scan_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
+                                     lengths, chains, steps, (int)channels, blocks, out, state, st->flags_dev));
     CT_LAUNCH_CHECK("gated_scan");
     return CT_OK;
 }
@@ -312,8 +338,8 @@ ct_status ct_gated_scan_grad(
     constexpr int W = 8, S = 8;
     const int64_t groups = (chains + 31) / 32;
     const int blocks     = scan_blocks(st, groups, steps, W * S);
-    CT_CUDA(launch_dependent_cluster(gated_scan_grad_kernel<W, S>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
-                                     lengths, out, dout, dstate, chains, steps, channels, blocks, dgate, dvalue, dstate0));
+    CT_CUDA(launch_dependent_cluster(gated_scan_grad_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
+                                     lengths, out, dout, dstate, chains, steps, (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev));
     CT_LAUNCH_CHECK("gated_scan_grad");
     return CT_OK;
 }
