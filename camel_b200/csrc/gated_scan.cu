@@ -18,6 +18,8 @@
 #include "tc_ptx.cuh"
 
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
 
 namespace ct {
 namespace {
@@ -274,6 +276,120 @@ __global__ void __launch_bounds__(W * 32, FIT) gated_scan_grad_kernel(
     exchange_end(ex, blocks, flags);
 }
 
+// A few steps, S at most: a thread goes through those of V chains, all of which are on their way together.
+template <int V, int S>
+__global__ void __launch_bounds__(128) gated_steps_kernel(
+    const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int steps,
+    int channels, float *__restrict__ out, float *state_out) {
+    using Values = std::conditional_t<V == 4, float4, float>;
+    griddep_wait();
+    const Chain c = chain_of(((int64_t)blockIdx.x * 128 + threadIdx.x) * V, chains, steps, channels, lengths);
+    if (!c.here)
+        return;
+    alignas(16) float g[S][V], v[S][V], h[V];
+    auto load = [](const float *from, float (&to)[V]) { *reinterpret_cast<Values *>(to) = *reinterpret_cast<const Values *>(from); };
+    auto store = [](float *to, const float (&from)[V]) { *reinterpret_cast<Values *>(to) = *reinterpret_cast<const Values *>(from); };
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (j < c.steps) {
+            load(gate + c.first + (int64_t)j * channels, g[j]);
+            load(value + c.first + (int64_t)j * channels, v[j]);
+        }
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+        h[q] = 0.0f;
+    if (state0)
+        load(state0 + c.index, h);
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (j < steps) {
+            alignas(16) float to[V];
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                to[q] = 0.0f;
+                if (j < c.steps) {
+                    float a, rest;
+                    sigmoids(g[j][q], a, rest);
+                    to[q] = h[q] = __fmaf_rn(a, h[q], __fmul_rn(rest, v[j][q]));
+                }
+            }
+            if (out)
+                store(out + c.first + (int64_t)j * channels, to);
+        }
+    if (state_out)
+        store(state_out + c.index, h);
+}
+
+template <int V, int S>
+__global__ void __launch_bounds__(128) gated_steps_grad_kernel(
+    const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths,
+    const float *__restrict__ out, const float *__restrict__ dout, const float *dstate, int64_t chains, int steps, int channels,
+    float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0) {
+    using Values = std::conditional_t<V == 4, float4, float>;
+    griddep_wait();
+    const Chain c = chain_of(((int64_t)blockIdx.x * 128 + threadIdx.x) * V, chains, steps, channels, lengths);
+    if (!c.here)
+        return;
+    alignas(16) float g[S][V], v[S][V], d[S][V], h[S][V], last[V]; // h: before the step
+    auto load = [](const float *from, float (&to)[V]) { *reinterpret_cast<Values *>(to) = *reinterpret_cast<const Values *>(from); };
+    auto store = [](float *to, const float (&from)[V]) { *reinterpret_cast<Values *>(to) = *reinterpret_cast<const Values *>(from); };
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+        last[q] = h[0][q] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (j < c.steps) {
+            load(gate + c.first + (int64_t)j * channels, g[j]);
+            load(value + c.first + (int64_t)j * channels, v[j]);
+            load(dout + c.first + (int64_t)j * channels, d[j]);
+            if (j > 0)
+                load(out + c.first + (int64_t)(j - 1) * channels, h[j]);
+        }
+    if (state0)
+        load(state0 + c.index, h[0]);
+    if (dstate)
+        load(dstate + c.index, last);
+    double carry[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+        carry[q] = (double)last[q];
+#pragma unroll
+    for (int j = S - 1; j >= 0; --j)
+        if (j < steps) {
+            alignas(16) float dg[V], dv[V];
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                dg[q] = dv[q] = 0.0f;
+                if (j < c.steps) {
+                    float a, rest;
+                    sigmoids(g[j][q], a, rest);
+                    const double x = (double)d[j][q] + carry[q];
+                    carry[q]       = (rest <= 0.5f ? 1.0 - (double)rest : (double)a) * x;
+                    dv[q]          = __fmul_rn(rest, (float)x);
+                    dg[q]          = __fmul_rn(__fmul_rn(rest, (float)carry[q]), __fsub_rn(h[j][q], v[j][q]));
+                }
+            }
+            if (dvalue)
+                store(dvalue + c.first + (int64_t)j * channels, dv);
+            if (dgate)
+                store(dgate + c.first + (int64_t)j * channels, dg);
+        }
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+        last[q] = (float)carry[q];
+    if (dstate0)
+        store(dstate0 + c.index, last);
+}
+
+constexpr int kFewSteps = 16;
+
+bool aligned16(std::initializer_list<const void *> all) { // null is
+    for (const void *p : all)
+        if (reinterpret_cast<uintptr_t>(p) & 15u)
+            return false;
+    return true;
+}
+
 ct_status check_scan(const char *name, int64_t batch, int64_t steps, int64_t channels) {
     if (batch < 0 || steps < 0 || channels < 0)
         return fail(CT_ERR_INVALID, "%s: negative dimension", name);
@@ -314,6 +430,20 @@ ct_status ct_gated_scan(
         return fail(CT_ERR_INVALID, "gated_scan: null pointer");
     ProfScope prof("gated_scan");
     constexpr int W = 8, S = 16;
+    if (steps <= kFewSteps) {
+        const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, state});
+        auto launch     = [&](auto kernel, int v) -> ct_status {
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((chains / v + 127) / 128)), dim3(128), 0, stream(), gate, value, state0, lengths, chains, (int)steps,
+                                     (int)channels, out, state));
+            CT_LAUNCH_CHECK("gated_steps");
+            return CT_OK;
+        };
+        if (steps <= 1)
+            return four ? launch(gated_steps_kernel<4, 1>, 4) : launch(gated_steps_kernel<1, 1>, 1);
+        if (steps <= 4)
+            return four ? launch(gated_steps_kernel<4, 4>, 4) : launch(gated_steps_kernel<1, 4>, 1);
+        return launch(gated_steps_kernel<1, kFewSteps>, 1);
+    }
     const int64_t groups = (chains + 31) / 32;
     const int blocks     = scan_blocks(st, groups, steps, W * S);
     CT_CUDA(launch_dependent_cluster(gated_scan_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
@@ -336,6 +466,20 @@ ct_status ct_gated_scan_grad(
         return fail(CT_ERR_INVALID, "gated_scan_grad: null pointer");
     ProfScope prof("gated_scan_grad");
     constexpr int W = 8, S = 8;
+    if (steps <= kFewSteps) {
+        const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, dout, dstate, dgate, dvalue, dstate0});
+        auto launch     = [&](auto kernel, int v) -> ct_status {
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((chains / v + 127) / 128)), dim3(128), 0, stream(), gate, value, state0, lengths, out, dout, dstate,
+                                     chains, (int)steps, (int)channels, dgate, dvalue, dstate0));
+            CT_LAUNCH_CHECK("gated_steps_grad");
+            return CT_OK;
+        };
+        if (steps <= 1)
+            return four ? launch(gated_steps_grad_kernel<4, 1>, 4) : launch(gated_steps_grad_kernel<1, 1>, 1);
+        if (steps <= 4)
+            return four ? launch(gated_steps_grad_kernel<4, 4>, 4) : launch(gated_steps_grad_kernel<1, 4>, 1);
+        return launch(gated_steps_grad_kernel<1, kFewSteps>, 1);
+    }
     const int64_t groups = (chains + 31) / 32;
     const int blocks     = scan_blocks(st, groups, steps, W * S);
     CT_CUDA(launch_dependent_cluster(gated_scan_grad_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
