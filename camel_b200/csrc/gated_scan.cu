@@ -14,6 +14,7 @@
 // what they add, b, and their 1 - A is summed up by itself, S' = a S + (1 - a).  A is 1 - S in 64 bits, or, from where S has more than 1/2, the
 // product, which is then small and has its digits.  Between pieces states are in 64 bits.
 #include "common.cuh"
+#include "fastmath.cuh"
 #include "gate.cuh"
 #include "tc_ptx.cuh"
 
@@ -37,90 +38,147 @@ struct Piece {
     __device__ __forceinline__ double2 joined() const { return make_double2(lost <= 0.5f ? 1.0 - (double)lost : (double)a, (double)b); }
 };
 
-constexpr int kMostBlocks = 8; // of a cluster
+// a and 1 - a of two gates, in the machine's two-lane instructions: a scan is bound by their number as much as by memory.  With e = exp(-gate),
+// 2^t of the rounded t = -gate log2(e) and what that lacks, a is 1 / (1 + e), from a reciprocal and a Newton step, and 1 - a is e a: to 2 U and to 7 U of
+// themselves (U = 2^-24), and 2^-26 |gate| more of what the float32 log2(e) lacks.  Gates below -87.33654 count as that: 1 + e is not above 2^126, whose
+// reciprocal is the smallest number that ftz leaves.
+__device__ __forceinline__ void sigmoids2(float g0, float g1, f32x2 &a, f32x2 &rest) {
+    float t0, t1;
+    asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g0));
+    asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g1));
+    asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g0)); // 104: e is 0 there
+    asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g1));
+    const f32x2 g = pack2(g0, g1), t = mul2(g, dup2(0xBFB8AA3Bu)), r = fma2(g, dup2(0x3FB8AA3Bu), t); // minus what t lacks
+    unpack2(t, t0, t1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(t0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(t1));
+    f32x2 e = pack2(t0, t1);
+    e       = fma2(e, mul2(r, dup2(0xBF317218u)), e); // ln 2
+    const f32x2 minus_d = fma2(e, dup2(0xBF800000u), dup2(0xBF800000u));
+    unpack2(minus_d, t0, t1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(-t0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(-t1));
+    const f32x2 q = pack2(t0, t1);
+    a    = fma2(q, fma2(minus_d, q, dup2(0x3F800000u)), q);
+    rest = mul2(e, a);
+}
 
-// The state before each warp's steps, from what all pieces of the tile do; `state` goes on to the tile's end.  Pieces lie in the order of warps, and
-// of the cluster's blocks.  One tile after the other alternates between two places, so that a fast warp does not write over what a slow one reads.
-// Blocks send what their pieces do to one another by st.async, whose arrival a barrier counts: a cluster-wide barrier would wait until the last
-// tile's stores to global memory are done.
-template <int W> struct Exchange {
-    double2 pieces[2][W][32];
-    double2 blocks[2][kMostBlocks][32];
-    uint64_t arrived[2];
+constexpr int kMostBlocks = 16; // of a cluster
+
+// How the pieces of a tile meet.  A block's pieces lie in the order of its warps; what they do together goes to the other blocks of the cluster by
+// st.async, whose arrival a barrier counts (a cluster-wide barrier would wait until the last tile's stores to global memory are done).  Meanwhile the block
+// goes on with the next tile, so that a block may be three tiles behind another: there are four places for what blocks send, and two for pieces.
+template <int W, bool CLUSTER> struct Exchange {
+    double2 pieces[2][W][32]; // (a, b)
+};
+template <int W> struct Exchange<W, true> : Exchange<W, false> {
+    double2 blocks[4][kMostBlocks][32];
+    uint64_t arrived[4];
     int gave_up;
 };
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void send(uint32_t at, uint32_t barrier, double2 p) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(at), "d"(p.x), "d"(p.y), "r"(barrier)
                  : "memory");
 }
-template <int W>
-__device__ __forceinline__ double exchange(Exchange<W> &e, int tile, Piece mine, double &state, int warp, int lane, int blocks, uint32_t rank) {
-    const int turn             = tile & 1;
-    e.pieces[turn][warp][lane] = mine.joined();
-    __syncthreads();
-    double before = state;
-    if (blocks == 1) {
+
+// Walks the tiles: first(i, steps) takes tile i into `steps`, a lane's registers, and says what they do; second(i, steps, state) goes through them from
+// the state before them.  Returns the state behind all tiles.
+template <typename Steps, int W, typename First, typename Second>
+__device__ __forceinline__ double walk(Exchange<W, false> &e, int tiles, double state, int, First &&first, Second &&second) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Steps s;
+    for (int i = 0; i < tiles; ++i) {
+        e.pieces[i & 1][warp][lane] = first(i, s);
+        __syncthreads();
+        double before = state;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             before          = w == warp ? state : before;
-            const double2 p = e.pieces[turn][w][lane];
+            const double2 p = e.pieces[i & 1][w][lane];
             state           = fma(p.x, state, p.y);
         }
-        return before;
+        second(i, s, before);
     }
-    // what the warps before this one do, and the last warp's with it: the block's
-    double a = 1.0, b = 0.0;
-    const int upto = warp == W - 1 ? W : warp;
+    return state;
+}
+template <typename Steps, int W, typename First, typename Second>
+__device__ __forceinline__ double walk(Exchange<W, true> &e, int tiles, double state, int blocks, First &&first, Second &&second) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t rank = cluster_rank();
+    double a = 1.0, b = 0.0; // what the warps before this one do in the tile before
+    auto turn = [&](int i, Steps &now, Steps &past) {
+        double next_a = 1.0, next_b = 0.0;
+        if (i < tiles) {
+            e.pieces[i & 1][warp][lane] = first(i, now);
+            __syncthreads();
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < upto) {
-            const double2 p = e.pieces[turn][w][lane];
-            if (w == W - 1) {
-                const uint32_t at  = static_cast<uint32_t>(__cvta_generic_to_shared(&e.blocks[turn][rank][lane]));
-                const uint32_t bar = static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[turn]));
-                const double2 all  = make_double2(a * p.x, fma(p.x, b, p.y));
+            for (int w = 0; w < W - 1; ++w)
+                if (w < warp) {
+                    const double2 p = e.pieces[i & 1][w][lane];
+                    next_b          = fma(p.x, next_b, p.y);
+                    next_a *= p.x;
+                }
+            if (warp == W - 1) {
+                const double2 p    = e.pieces[i & 1][warp][lane];
+                const uint32_t at  = shared_address(&e.blocks[i & 3][rank][lane]);
+                const uint32_t bar = shared_address(&e.arrived[i & 3]);
                 if (lane == 0)
                     mbar_expect_tx(bar, blocks * 512);
                 for (int r = 0; r < blocks; ++r)
-                    send(mapa(at, r), mapa(bar, r), all);
-            } else {
-                b = fma(p.x, b, p.y);
-                a *= p.x;
+                    send(mapa(at, r), mapa(bar, r), make_double2(next_a * p.x, fma(p.x, next_b, p.y)));
             }
         }
-    // a wait that has run out is reported by the kernel's end; until then the block goes on, for the others' sake
-    if (!*(volatile int *)&e.gave_up)
-        mbar_wait<kClusterWritten>(static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[turn])), (tile >> 1) & 1, &e.gave_up);
-    for (int r = 0; r < blocks; ++r) {
-        const double2 p = e.blocks[turn][r][lane];
-        before          = r == (int)rank ? state : before;
-        state           = fma(p.x, state, p.y);
+        if (i > 0) {
+            const int j = i - 1;
+            // a wait that has run out is reported by the kernel's end; until then the block goes on, for the others' sake
+            if (!*(volatile int *)&e.gave_up)
+                mbar_wait<kClusterWritten>(shared_address(&e.arrived[j & 3]), (j >> 2) & 1, &e.gave_up);
+            auto pass = [&](int r) {
+                const double2 p = e.blocks[j & 3][r][lane];
+                state           = fma(p.x, state, p.y);
+            };
+            for (int r = 0; r < (int)rank; ++r)
+                pass(r);
+            const double before = state;
+            for (int r = rank; r < blocks; ++r)
+                pass(r);
+            second(j, past, fma(a, before, b));
+        }
+        a = next_a, b = next_b;
+    };
+    Steps even, odd;
+    for (int i = 0;; i += 2) {
+        turn(i, even, odd);
+        if (i == tiles)
+            break;
+        turn(i + 1, odd, even);
+        if (i + 1 == tiles)
+            break;
     }
-    return fma(a, before, b);
+    return state;
 }
-template <int W> __device__ __forceinline__ void exchange_begin(Exchange<W> &e, int blocks) {
-    if (blocks == 1)
-        return;
+template <int W> __device__ __forceinline__ void walk_begin(Exchange<W, false> &) {}
+template <int W> __device__ __forceinline__ void walk_begin(Exchange<W, true> &e) {
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i)
-            mbar_init(static_cast<uint32_t>(__cvta_generic_to_shared(&e.arrived[i])), 1);
+        for (int i = 0; i < 4; ++i)
+            mbar_init(shared_address(&e.arrived[i]), 1);
         e.gave_up = 0;
         mbar_fence_init();
     }
     cluster_sync();
 }
-template <int W> __device__ __forceinline__ void exchange_end(Exchange<W> &e, int blocks, uint32_t *flags) {
-    if (blocks == 1)
-        return;
+template <int W> __device__ __forceinline__ void walk_end(Exchange<W, false> &, uint32_t *) {}
+template <int W> __device__ __forceinline__ void walk_end(Exchange<W, true> &e, uint32_t *flags) {
     cluster_sync(); // nothing is on its way to a block that has ended
     if (threadIdx.x == 0 && e.gave_up)
-        atomicMax(&flags[FLAG_TIMEOUT], 1u + blockIdx.x);
+        atomicExch(&flags[FLAG_TIMEOUT], 1u + blockIdx.x);
 }
 
 struct Chain {
     int64_t first; // of its values, at step 0
     int64_t index; // of its state
-    int64_t steps; // that belong to the sequence
+    int64_t steps; // that belong to the sequence; none of a chain that is not there
     bool here;
 };
 __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t steps, int64_t channels, const int64_t *__restrict__ lengths) {
@@ -137,143 +195,223 @@ __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t
     return c;
 }
 
+// The values of a warp's pieces on their way to shared memory, [tile][array][step][lane], AHEAD tiles of them, a group of copies to a tile.
+// QUADS: 16 bytes at a time, which other lanes of the warp read; else each lane what it reads itself.
+template <int ARRAYS, int S> constexpr int kTileFloats = ARRAYS * S * 32;
+template <int BYTES> __device__ __forceinline__ void copy(uint32_t to, const float *from) {
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits for a tile behind which the copies of AHEAD - 1 more have begun.
+template <int AHEAD, bool QUADS> __device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+    if (QUADS)
+        __syncwarp();
+}
+
+// Rows that follow one another, from `from` on, `count` of them there: steps first, first + 4, ... of a piece.
+template <int S, bool QUADS> __device__ __forceinline__ void copy_rows(uint32_t to, const float *from, int stride, int count, int lane) {
+    const int first = QUADS ? lane >> 3 : 0;
+    from += (int64_t)first * stride;
+    to += (first * 32 + (QUADS ? (lane & 7) * 4 : lane)) * 4;
+#pragma unroll
+    for (int j = 0; j < (QUADS ? S / 4 : S); ++j)
+        if ((QUADS ? j * 4 : j) + first < count)
+            copy<QUADS ? 16 : 4>(to + j * (QUADS ? 512 : 128), from + (int64_t)(QUADS ? j * 4 : j) * stride);
+}
+__device__ __forceinline__ int clamped(int64_t steps) { return (int)max((int64_t)-1, min((int64_t)1 << 20, steps)); }
+
 // W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
-template <int W, int S, int FIT>
-__global__ void __launch_bounds__(W * 32, FIT) gated_scan_kernel(
+template <int W, int S, int AHEAD, bool QUADS, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_scan_kernel(
     const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths, int64_t chains,
     int64_t steps, int channels, int blocks, float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
-    __shared__ Exchange<W> ex;
+    extern __shared__ __align__(16) float ring[];
+    __shared__ Exchange<W, CLUSTER> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t rank = blocks > 1 ? cluster_rank() : 0;
-    exchange_begin(ex, blocks);
+    const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+    walk_begin(ex);
     griddep_wait();
-    const Chain c      = chain_of((int64_t)(blockIdx.x / blocks) * 32 + lane, chains, steps, channels, lengths);
-    double state       = c.here && state0 ? (double)state0[c.index] : 0.0;
-    const int64_t tile = (int64_t)blocks * W * S;
-    int64_t t0         = ((int64_t)rank * W + warp) * S;
-    float g[S], v[S];
-    // Steps that a chain does not have keep its state: a = 1, and nothing is added.
-    auto fetch = [&](int64_t t) {
-        const float *pg = gate + c.first + t * channels, *pv = value + c.first + t * channels;
-        if (__all_sync(0xffffffffu, t + S <= c.steps)) {
-#pragma unroll
-            for (int i = 0; i < S; ++i)
-                g[i] = __ldcs(pg + (int64_t)i * channels), v[i] = __ldcs(pv + (int64_t)i * channels);
-        } else {
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool in = t + i < c.steps;
-                g[i]          = in ? __ldcs(pg + (int64_t)i * channels) : INFINITY;
-                v[i]          = in ? __ldcs(pv + (int64_t)i * channels) : 0.0f;
-            }
-        }
+    const int64_t group = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * 32;
+    const Chain c       = chain_of(group + lane, chains, steps, channels, lengths);
+    const Chain source  = QUADS ? chain_of(group + (lane & 7) * 4, chains, steps, channels, lengths) : c;
+    const int64_t tile  = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = ((int64_t)rank * W + warp) * S;
+    float *mine         = ring + warp * AHEAD * kTileFloats<2, S>;
+    const uint32_t mine_at = shared_address(mine);
+    auto fetch             = [&](int i) {
+        const int64_t t   = t0 + i * tile, at = source.first + t * channels;
+        const uint32_t to = mine_at + (i % AHEAD) * kTileFloats<2, S> * 4;
+        const int count   = clamped(source.steps - t);
+        copy_rows<S, QUADS>(to, gate + at, channels, count, lane);
+        copy_rows<S, QUADS>(to + S * 128, value + at, channels, count, lane);
+        copies_end();
     };
-    fetch(t0);
-    const int tiles = (int)((steps + tile - 1) / tile);
-    for (int i = 0; i < tiles; ++i, t0 += tile) {
+    for (int i = 0; i < AHEAD; ++i)
+        fetch(i);
+    struct Steps {
         float a[S], add[S];
-        Piece mine;
+    };
+    const double state = walk<Steps>(
+        ex, (int)((steps + tile - 1) / tile), c.here && state0 ? (double)state0[c.index] : 0.0, blocks,
+        [&](int i, Steps &s) {
+            copies_wait<AHEAD, QUADS>();
+            const float *g  = mine + (i % AHEAD) * kTileFloats<2, S> + lane, *v = g + S * 32;
+            const int count = clamped(c.steps - (t0 + i * tile));
+            if (__all_sync(0xffffffffu, count >= S)) {
 #pragma unroll
-        for (int j = 0; j < S; ++j) {
-            float rest;
-            sigmoids(g[j], a[j], rest);
-            add[j] = __fmul_rn(rest, v[j]);
-            mine.step(a[j], rest, add[j]);
-        }
-        fetch(t0 + tile);
-        float h = (float)exchange(ex, i, mine, state, warp, lane, blocks, rank);
-        if (out) {
-            float *to = out + c.first + t0 * channels;
-            if (__all_sync(0xffffffffu, t0 + S <= c.steps)) {
-#pragma unroll
-                for (int j = 0; j < S; ++j) {
-                    h = __fmaf_rn(a[j], h, add[j]);
-                    __stcs(to + (int64_t)j * channels, h);
-                }
+                for (int j = 0; j < S; ++j)
+                    s.a[j] = g[j * 32], s.add[j] = v[j * 32];
             } else {
 #pragma unroll
+                for (int j = 0; j < S; ++j) // steps that a chain does not have keep its state: a = 1, and nothing is added
+                    s.a[j] = j < count ? g[j * 32] : INFINITY, s.add[j] = j < count ? v[j * 32] : 0.0f;
+            }
+            if (QUADS)
+                __syncwarp();
+            fetch(i + AHEAD);
+            Piece p;
+#pragma unroll
+            for (int j = 0; j < S; j += 2) {
+                f32x2 a, rest;
+                sigmoids2(s.a[j], s.a[j + 1], a, rest);
+                unpack2(mul2(rest, pack2(s.add[j], s.add[j + 1])), s.add[j], s.add[j + 1]);
+                unpack2(a, s.a[j], s.a[j + 1]);
+                float r0, r1;
+                unpack2(rest, r0, r1);
+                p.step(s.a[j], r0, s.add[j]);
+                p.step(s.a[j + 1], r1, s.add[j + 1]);
+            }
+            return p.joined();
+        },
+        [&](int i, const Steps &s, double before) {
+            if (!out)
+                return;
+            const int64_t t = t0 + i * tile;
+            const int count = clamped(c.steps - t);
+            float *to       = out + c.first + t * channels;
+            float h         = (float)before;
+            if (__all_sync(0xffffffffu, count >= S)) {
+#pragma unroll
                 for (int j = 0; j < S; ++j) {
-                    h = __fmaf_rn(a[j], h, add[j]);
-                    if (c.here && t0 + j < steps)
-                        __stcs(to + (int64_t)j * channels, t0 + j < c.steps ? h : 0.0f);
+                    h = __fmaf_rn(s.a[j], h, s.add[j]);
+                    __stcs(to + (int64_t)j * channels, h);
+                }
+            } else if (c.here) {
+#pragma unroll
+                for (int j = 0; j < S; ++j) {
+                    h = __fmaf_rn(s.a[j], h, s.add[j]);
+                    if (t + j < steps)
+                        __stcs(to + (int64_t)j * channels, j < count ? h : 0.0f);
                 }
             }
-        }
-    }
+        });
     if (state_out && warp == 0 && rank == 0 && c.here)
         state_out[c.index] = (float)state;
-    exchange_end(ex, blocks, flags);
+    walk_end(ex, flags);
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
-template <int W, int S, int FIT>
-__global__ void __launch_bounds__(W * 32, FIT) gated_scan_grad_kernel(
+template <int W, int S, int AHEAD, bool QUADS, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_scan_grad_kernel(
     const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths,
     const float *__restrict__ out, const float *__restrict__ dout, const float *dstate, int64_t chains, int64_t steps, int channels, int blocks,
     float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
-    __shared__ Exchange<W> ex;
+    extern __shared__ __align__(16) float ring[];
+    __shared__ Exchange<W, CLUSTER> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t rank = blocks > 1 ? cluster_rank() : 0;
-    exchange_begin(ex, blocks);
+    const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+    walk_begin(ex);
     griddep_wait();
-    const Chain c      = chain_of((int64_t)(blockIdx.x / blocks) * 32 + lane, chains, steps, channels, lengths);
-    double state       = c.here && dstate ? (double)dstate[c.index] : 0.0; // c[t+1]
-    const float first  = c.here && state0 ? state0[c.index] : 0.0f;
-    const int64_t tile = (int64_t)blocks * W * S;
-    int64_t t1         = steps - 1 - ((int64_t)rank * W + warp) * S; // the piece's last step
-    float g[S], v[S], d[S], h[S];
-    auto fetch = [&](int64_t t) {
-        const int64_t at = c.first + t * channels;
-        if (__all_sync(0xffffffffu, t < c.steps && t >= S)) {
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                g[i] = __ldcs(gate + at - (int64_t)i * channels), v[i] = __ldcs(value + at - (int64_t)i * channels);
-                d[i] = __ldcs(dout + at - (int64_t)i * channels), h[i] = __ldcs(out + at - (int64_t)(i + 1) * channels);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const bool in = t - i >= 0 && t - i < c.steps;
-                g[i]          = in ? __ldcs(gate + at - (int64_t)i * channels) : INFINITY;
-                v[i]          = in ? __ldcs(value + at - (int64_t)i * channels) : 0.0f;
-                d[i]          = in ? __ldcs(dout + at - (int64_t)i * channels) : 0.0f;
-                h[i]          = in ? (t - i > 0 ? __ldcs(out + at - (int64_t)(i + 1) * channels) : first) : 0.0f;
-            }
+    const int64_t group = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * 32;
+    const Chain c       = chain_of(group + lane, chains, steps, channels, lengths);
+    const Chain source  = QUADS ? chain_of(group + (lane & 7) * 4, chains, steps, channels, lengths) : c;
+    const float first   = c.here && state0 ? state0[c.index] : 0.0f;
+    // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
+    const int64_t tile  = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = steps - ((int64_t)rank * W + warp + 1) * S;
+    float *mine         = ring + warp * AHEAD * kTileFloats<4, S>;
+    const uint32_t mine_at = shared_address(mine);
+    auto fetch             = [&](int i) {
+        const int64_t t   = t0 - i * tile;
+        const uint32_t to = mine_at + (i % AHEAD) * kTileFloats<4, S> * 4;
+        const int skip    = t < 0 ? clamped(-t) : 0, count = clamped(source.steps - t);
+        const int64_t at  = source.first + (t + skip) * channels;
+        if (skip < S) {
+            const uint32_t from = to + skip * 128;
+            copy_rows<S, QUADS>(from, gate + at, channels, min(count, S) - skip, lane);
+            copy_rows<S, QUADS>(from + S * 128, value + at, channels, min(count, S) - skip, lane);
+            copy_rows<S, QUADS>(from + 2 * S * 128, dout + at, channels, min(count, S) - skip, lane);
+            const int begin = t + skip == 0; // the state before step 0 is none of out's
+            copy_rows<S, QUADS>(from + (3 * S + begin) * 128, out + at + (begin - 1) * (int64_t)channels, channels, min(count, S) - skip - begin, lane);
         }
+        copies_end();
     };
-    fetch(t1);
-    const int tiles = (int)((steps + tile - 1) / tile);
-    for (int i = 0; i < tiles; ++i, t1 -= tile) {
-        float a[S], rest[S], gap[S], dy[S];
-        Piece mine;
+    for (int i = 0; i < AHEAD; ++i)
+        fetch(i);
+    struct Steps {
+        float a[S], rest[S], gap[S], dy[S]; // gap: h[t-1] - value[t]
+    };
+    const double state = walk<Steps>( // c[t+1]
+        ex, (int)((steps + tile - 1) / tile), c.here && dstate ? (double)dstate[c.index] : 0.0, blocks,
+        [&](int i, Steps &s) {
+            copies_wait<AHEAD, QUADS>();
+            const float *g = mine + (i % AHEAD) * kTileFloats<4, S> + lane, *v = g + S * 32, *d = v + S * 32, *h = d + S * 32;
+            const int64_t t = t0 - i * tile;
+            const int begin = clamped(-t), count = clamped(c.steps - t); // steps begin .. count - 1 are there
+            if (__all_sync(0xffffffffu, t > 0 && count >= S)) {
 #pragma unroll
-        for (int j = 0; j < S; ++j) {
-            sigmoids(g[j], a[j], rest[j]);
-            gap[j] = __fsub_rn(h[j], v[j]);
-            dy[j]  = d[j];
-            mine.step(a[j], rest[j], __fmul_rn(a[j], dy[j]));
-        }
-        fetch(t1 - tile);
-        float carry = (float)exchange(ex, i, mine, state, warp, lane, blocks, rank);
-        const int64_t at = c.first + t1 * channels;
-        const bool whole = __all_sync(0xffffffffu, t1 < c.steps && t1 >= S - 1);
+                for (int j = 0; j < S; ++j)
+                    s.a[j] = g[j * 32], s.rest[j] = v[j * 32], s.dy[j] = d[j * 32], s.gap[j] = h[j * 32];
+            } else {
 #pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const float x = __fadd_rn(dy[j], carry);
-            carry         = __fmul_rn(a[j], x);
-            const float dv = __fmul_rn(rest[j], x), dg = __fmul_rn(__fmul_rn(rest[j], carry), gap[j]);
-            if (whole || (c.here && t1 - j >= 0)) {
-                const bool in = whole || t1 - j < c.steps;
-                if (dvalue)
-                    __stcs(dvalue + at - (int64_t)j * channels, in ? dv : 0.0f);
-                if (dgate)
-                    __stcs(dgate + at - (int64_t)j * channels, in ? dg : 0.0f);
+                for (int j = 0; j < S; ++j) {
+                    const bool in = j >= begin && j < count;
+                    s.a[j] = in ? g[j * 32] : INFINITY, s.rest[j] = in ? v[j * 32] : 0.0f, s.dy[j] = in ? d[j * 32] : 0.0f;
+                    s.gap[j] = in ? (t + j > 0 ? h[j * 32] : first) : 0.0f;
+                }
             }
-        }
-    }
+            if (QUADS)
+                __syncwarp();
+            fetch(i + AHEAD);
+            Piece p;
+#pragma unroll
+            for (int j = S - 2; j >= 0; j -= 2) {
+                f32x2 a, rest;
+                sigmoids2(s.a[j], s.a[j + 1], a, rest);
+                float add0, add1;
+                unpack2(mul2(a, pack2(s.dy[j], s.dy[j + 1])), add0, add1);
+                unpack2(fma2(pack2(s.rest[j], s.rest[j + 1]), dup2(0xBF800000u), pack2(s.gap[j], s.gap[j + 1])), s.gap[j], s.gap[j + 1]);
+                unpack2(a, s.a[j], s.a[j + 1]);
+                unpack2(rest, s.rest[j], s.rest[j + 1]);
+                p.step(s.a[j + 1], s.rest[j + 1], add1);
+                p.step(s.a[j], s.rest[j], add0);
+            }
+            return p.joined();
+        },
+        [&](int i, const Steps &s, double before) {
+            const int64_t t = t0 - i * tile, at = c.first + t * channels;
+            const int count = clamped(c.steps - t);
+            const bool all  = __all_sync(0xffffffffu, t >= 0 && count >= S);
+            float carry     = (float)before;
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j) {
+                const float x  = __fadd_rn(s.dy[j], carry);
+                carry          = __fmul_rn(s.a[j], x);
+                const float dv = __fmul_rn(s.rest[j], x), dg = __fmul_rn(__fmul_rn(s.rest[j], carry), s.gap[j]);
+                if (all || (c.here && t + j >= 0)) {
+                    const bool in = all || j < count;
+                    if (dvalue)
+                        __stcs(dvalue + at + (int64_t)j * channels, in ? dv : 0.0f);
+                    if (dgate)
+                        __stcs(dgate + at + (int64_t)j * channels, in ? dg : 0.0f);
+                }
+            }
+        });
     if (dstate0 && warp == 0 && rank == 0 && c.here)
         dstate0[c.index] = (float)state;
-    exchange_end(ex, blocks, flags);
+    walk_end(ex, flags);
 }
 
 // A few steps, S at most: a thread goes through those of V chains, all of which are on their way together.
@@ -401,12 +539,32 @@ ct_status check_scan(const char *name, int64_t batch, int64_t steps, int64_t cha
     return CT_OK;
 }
 
-// Blocks to a cluster: while the groups of 32 chains do not fill the machine, and a tile does not exceed the steps.
-int scan_blocks(const DeviceState *st, int64_t groups, int64_t steps, int piece) {
-    int blocks = 1;
-    while (blocks < 8 && groups * blocks * 2 <= st->sm_count * 2 && steps > (int64_t)blocks * piece)
-        blocks *= 2;
-    return blocks;
+// Blocks to a cluster: as many as let all groups of 32 chains run at once, and have a piece of the steps each.  (Clusters that wait for others' end cost a
+// second walk: 16 groups in clusters of 8, of which 15 fit beside one another, took twice the time.)
+template <typename Kernel> ct_status scan_blocks(const DeviceState *st, Kernel kernel, int threads, int smem, int64_t groups, int64_t pieces, int *blocks) {
+    static int fit[16][kMostBlocks + 1] = {}; // clusters at once, by device and size, and 1; under the entry points' lock
+    int *mine                           = fit[st->device & 15];
+    if (mine[1] == 0) {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (int size = 2; size <= kMostBlocks; ++size) {
+            cudaLaunchAttribute attr{};
+            attr.id               = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = (unsigned)size, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)size), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = (size_t)smem;
+            cfg.attrs = &attr, cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&mine[size], kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                mine[size] = 0;
+            }
+        }
+        mine[1] = 1;
+    }
+    *blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kMostBlocks, pieces));
+    while (*blocks > 1 && mine[*blocks] < groups)
+        --*blocks;
+    return CT_OK;
 }
 
 } // namespace
@@ -429,7 +587,7 @@ ct_status ct_gated_scan(
     if (steps > 0 && (!gate || !value))
         return fail(CT_ERR_INVALID, "gated_scan: null pointer");
     ProfScope prof("gated_scan");
-    constexpr int W = 8, S = 16;
+    constexpr int W = 8, S = 16, AHEAD = 2;
     if (steps <= kFewSteps) {
         const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, state});
         auto launch     = [&](auto kernel, int v) -> ct_status {
@@ -445,11 +603,21 @@ ct_status ct_gated_scan(
         return launch(gated_steps_kernel<1, kFewSteps>, 1);
     }
     const int64_t groups = (chains + 31) / 32;
-    const int blocks     = scan_blocks(st, groups, steps, W * S);
-    CT_CUDA(launch_dependent_cluster(gated_scan_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
-                                     lengths, chains, steps, (int)channels, blocks, out, state, st->flags_dev));
-    CT_LAUNCH_CHECK("gated_scan");
-    return CT_OK;
+    constexpr int smem   = W * AHEAD * kTileFloats<2, S> * 4;
+    const bool quads     = channels % 4 == 0 && aligned16({gate, value});
+    int blocks;
+    CT_TRY(scan_blocks(st, gated_scan_kernel<W, S, AHEAD, true, true>, W * 32, smem, groups, (steps + W * S - 1) / (W * S), &blocks));
+    auto launch = [&](auto kernel) -> ct_status {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (blocks > 8)
+            CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), smem, stream(), gate, value, state0, lengths, chains, steps, (int)channels, blocks, out, state, st->flags_dev));
+        CT_LAUNCH_CHECK("gated_scan");
+        return CT_OK;
+    };
+    if (blocks == 1)
+        return quads ? launch(gated_scan_kernel<W, S, AHEAD, true, false>) : launch(gated_scan_kernel<W, S, AHEAD, false, false>);
+    return quads ? launch(gated_scan_kernel<W, S, AHEAD, true, true>) : launch(gated_scan_kernel<W, S, AHEAD, false, true>);
 }
 
 ct_status ct_gated_scan_grad(
@@ -465,7 +633,7 @@ ct_status ct_gated_scan_grad(
     if (steps > 0 && (!gate || !value || !out || !dout))
         return fail(CT_ERR_INVALID, "gated_scan_grad: null pointer");
     ProfScope prof("gated_scan_grad");
-    constexpr int W = 8, S = 8;
+    constexpr int W = 8, S = 8, AHEAD = 2;
     if (steps <= kFewSteps) {
         const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, dout, dstate, dgate, dvalue, dstate0});
         auto launch     = [&](auto kernel, int v) -> ct_status {
@@ -481,11 +649,21 @@ ct_status ct_gated_scan_grad(
         return launch(gated_steps_grad_kernel<1, kFewSteps>, 1);
     }
     const int64_t groups = (chains + 31) / 32;
-    const int blocks     = scan_blocks(st, groups, steps, W * S);
-    CT_CUDA(launch_dependent_cluster(gated_scan_grad_kernel<W, S, 2>, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), 0, stream(), gate, value, state0,
-                                     lengths, out, dout, dstate, chains, steps, (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev));
-    CT_LAUNCH_CHECK("gated_scan_grad");
-    return CT_OK;
+    constexpr int smem   = W * AHEAD * kTileFloats<4, S> * 4;
+    const bool quads     = channels % 4 == 0 && aligned16({gate, value, out, dout});
+    int blocks;
+    CT_TRY(scan_blocks(st, gated_scan_grad_kernel<W, S, AHEAD, true, true>, W * 32, smem, groups, (steps + W * S - 1) / (W * S), &blocks));
+    auto launch = [&](auto kernel) -> ct_status {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (blocks > 8)
+            CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), smem, stream(), gate, value, state0, lengths, out, dout, dstate, chains, steps, (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev));
+        CT_LAUNCH_CHECK("gated_scan_grad");
+        return CT_OK;
+    };
+    if (blocks == 1)
+        return quads ? launch(gated_scan_grad_kernel<W, S, AHEAD, true, false>) : launch(gated_scan_grad_kernel<W, S, AHEAD, false, false>);
+    return quads ? launch(gated_scan_grad_kernel<W, S, AHEAD, true, true>) : launch(gated_scan_grad_kernel<W, S, AHEAD, false, true>);
 }
 
 } // extern "C"

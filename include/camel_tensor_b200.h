@@ -427,7 +427,7 @@ ct_status ct_embedding_grad(
  * there and state that of the last step before, whatever gate and value hold.  out or state may be null, and state may be state0 itself: with
  * steps = 1 a call moves the states of a batch that is being answered by one token.
  * The error of h is a few roundings of the largest |value| and |state0| so far, however long a gate near 1 remembers (a and 1 - a each have their own
- * digits, and states are carried between pieces of the steps in 64 bits; the smaller of the two is 0 below 2^-126, beyond gates of 87).  A state that is infinite or NaN leaves such values behind it. */
+ * digits, and states are carried between pieces of the steps in 64 bits; the smaller of the two ends at 2^-126, beyond gates of 87.3).  A state that is infinite or NaN leaves such values behind it. */
 ct_status ct_gated_scan(
     const float *gate_dev, const float *value_dev, const float *state0_dev, const int64_t *lengths_dev, int64_t batch, int64_t steps, int64_t channels,
     float *out_dev, float *state_dev);

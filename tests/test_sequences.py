@@ -16,7 +16,9 @@ from test_layers_calls import Buffer
 
 gpu = pytest.mark.gpu
 TINY = 2.0 ** -149
-FLUSHED = 2.0 ** -126
+# The smaller of a and 1 - a: 0 below 2^-126, or (a, of many steps) not below that of the gate -87.33654022, 4.53e-6 short of 126 ln 2: 2^-126 times
+# 1 + 4.53e-6, and 7 U of it.  Either way off by less than
+FLUSHED = 2.0 ** -126 * (1 + 2.0 ** -17)
 
 
 # ---- embedding ------------------------------------------------------------------------------------
@@ -198,8 +200,8 @@ def scan_grad64(gate, value, state0, lengths, out, dout, dstate):
         near[i % 16] = np.where(on, np.abs(dout[:, i]), 0.0)
         d = np.where(on, dout[:, i], 0.0).astype(np.float64)
         g, g_size = d + carry, np.abs(d) + size
-        # 16 steps of two roundings, the beginning's, what the state lacks.  The smaller of a and 1 - a is 0 below FLUSHED (as in the gated layer): it,
-        # and what it multiplies, is off by that much of its other factors
+        # 16 steps of two roundings, the beginning's, what the state lacks.  The smaller of a and 1 - a, and what it multiplies, is off by FLUSHED
+        # of its other factors
         e = off + 40 * U * g_size
         s, p = rest[:, i], a[:, i]
         dvalue[:, i], off_value[:, i] = np.where(on, s * g, 0.0), np.where(on, s * (e + 12 * U * g_size) + FLUSHED * g_size, 0.0)
