@@ -17,6 +17,7 @@
 #include "fastmath.cuh"
 #include "gate.cuh"
 #include "tc_ptx.cuh"
+#include "tmap.cuh"
 
 #include <algorithm>
 #include <initializer_list>
@@ -42,26 +43,46 @@ struct Piece {
 // 2^t of the rounded t = -gate log2(e) and what that lacks, a is 1 / (1 + e), from a reciprocal and a Newton step, and 1 - a is e a: to 2 U and to 7 U of
 // themselves (U = 2^-24), and 2^-26 |gate| more of what the float32 log2(e) lacks.  Gates below -87.33654 count as that: 1 + e is not above 2^126, whose
 // reciprocal is the smallest number that ftz leaves.
-__device__ __forceinline__ void sigmoids2(float g0, float g1, f32x2 &a, f32x2 &rest) {
-    float t0, t1;
-    asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g0));
-    asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g1));
-    asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g0)); // 104: e is 0 there
-    asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g1));
-    const f32x2 g = pack2(g0, g1), t = mul2(g, dup2(0xBFB8AA3Bu)), r = fma2(g, dup2(0x3FB8AA3Bu), t); // minus what t lacks
-    unpack2(t, t0, t1);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(t0));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(t1));
-    f32x2 e = pack2(t0, t1);
-    e       = fma2(e, mul2(r, dup2(0xBF317218u)), e); // ln 2
-    const f32x2 minus_d = fma2(e, dup2(0xBF800000u), dup2(0xBF800000u));
-    unpack2(minus_d, t0, t1);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(-t0));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(-t1));
-    const f32x2 q = pack2(t0, t1);
-    a    = fma2(q, fma2(minus_d, q, dup2(0x3F800000u)), q);
-    rest = mul2(e, a);
+// N pairs together, stage by stage: one after the other they wait for their exponentials and reciprocals (the pieces of a tile 2000 clocks).
+template <int N> __device__ __forceinline__ void sigmoids2(const float *g, f32x2 (&a)[N], f32x2 (&rest)[N]) {
+    f32x2 x[N], t[N], e[N];
+    auto each = [](auto &&stage) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            stage(i);
+    };
+    each([&](int i) {
+        float g0 = g[2 * i], g1 = g[2 * i + 1];
+        asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g0));
+        asm("max.NaN.f32 %0, %0, 0fC2AEAC4F;" : "+f"(g1));
+        asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g0)); // 104: e is 0 there
+        asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g1));
+        x[i] = pack2(g0, g1);
+    });
+    each([&](int i) { t[i] = mul2(x[i], dup2(0xBFB8AA3Bu)); });
+    each([&](int i) {
+        float t0, t1;
+        unpack2(t[i], t0, t1);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(t0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(t1));
+        e[i] = pack2(t0, t1);
+    });
+    each([&](int i) { x[i] = fma2(x[i], dup2(0x3FB8AA3Bu), t[i]); }); // minus what t lacks
+    each([&](int i) { x[i] = mul2(x[i], dup2(0xBF317218u)); });       // ln 2
+    each([&](int i) { e[i] = fma2(e[i], x[i], e[i]); });
+    each([&](int i) { t[i] = fma2(e[i], dup2(0xBF800000u), dup2(0xBF800000u)); }); // -(1 + e)
+    each([&](int i) {
+        float d0, d1;
+        unpack2(t[i], d0, d1);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d0) : "f"(-d0));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d1) : "f"(-d1));
+        x[i] = pack2(d0, d1);
+    });
+    each([&](int i) { t[i] = fma2(t[i], x[i], dup2(0x3F800000u)); });
+    each([&](int i) { a[i] = fma2(x[i], t[i], x[i]); });
+    each([&](int i) { rest[i] = mul2(e[i], a[i]); });
 }
+constexpr int kPairs = 4; // together
 
 constexpr int kMostBlocks = 16; // of a cluster
 
@@ -70,11 +91,11 @@ constexpr int kMostBlocks = 16; // of a cluster
 // goes on with the next tile, so that a block may be three tiles behind another: there are four places for what blocks send, and two for pieces.
 template <int W, bool CLUSTER> struct Exchange {
     double2 pieces[2][W][32]; // (a, b)
+    int gave_up;              // a wait has run out: it is reported at the end, and until then the block goes on, for the others' sake
 };
 template <int W> struct Exchange<W, true> : Exchange<W, false> {
     double2 blocks[4][kMostBlocks][32];
     uint64_t arrived[4];
-    int gave_up;
 };
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void send(uint32_t at, uint32_t barrier, double2 p) {
@@ -131,7 +152,6 @@ __device__ __forceinline__ double walk(Exchange<W, true> &e, int tiles, double s
         }
         if (i > 0) {
             const int j = i - 1;
-            // a wait that has run out is reported by the kernel's end; until then the block goes on, for the others' sake
             if (!*(volatile int *)&e.gave_up)
                 mbar_wait<kClusterWritten>(shared_address(&e.arrived[j & 3]), (j >> 2) & 1, &e.gave_up);
             auto pass = [&](int r) {
@@ -158,19 +178,25 @@ __device__ __forceinline__ double walk(Exchange<W, true> &e, int tiles, double s
     }
     return state;
 }
-template <int W> __device__ __forceinline__ void walk_begin(Exchange<W, false> &) {}
-template <int W> __device__ __forceinline__ void walk_begin(Exchange<W, true> &e) {
+template <int W, bool CLUSTER> __device__ __forceinline__ void walk_begin(Exchange<W, CLUSTER> &e) {
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4; ++i)
-            mbar_init(shared_address(&e.arrived[i]), 1);
         e.gave_up = 0;
-        mbar_fence_init();
+        if constexpr (CLUSTER) {
+            for (int i = 0; i < 4; ++i)
+                mbar_init(shared_address(&e.arrived[i]), 1);
+            mbar_fence_init();
+        }
     }
-    cluster_sync();
+    if (CLUSTER)
+        cluster_sync();
+    else
+        __syncthreads();
 }
-template <int W> __device__ __forceinline__ void walk_end(Exchange<W, false> &, uint32_t *) {}
-template <int W> __device__ __forceinline__ void walk_end(Exchange<W, true> &e, uint32_t *flags) {
-    cluster_sync(); // nothing is on its way to a block that has ended
+template <int W, bool CLUSTER> __device__ __forceinline__ void walk_end(Exchange<W, CLUSTER> &e, uint32_t *flags) {
+    if (CLUSTER)
+        cluster_sync(); // nothing is on its way to a block that has ended
+    else
+        __syncthreads();
     if (threadIdx.x == 0 && e.gave_up)
         atomicExch(&flags[FLAG_TIMEOUT], 1u + blockIdx.x);
 }
@@ -195,59 +221,106 @@ __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t
     return c;
 }
 
-// The values of a warp's pieces on their way to shared memory, [tile][array][step][lane], AHEAD tiles of them, a group of copies to a tile.
-// QUADS: 16 bytes at a time, which other lanes of the warp read; else each lane what it reads itself.
-template <int ARRAYS, int S> constexpr int kTileFloats = ARRAYS * S * 32;
-template <int BYTES> __device__ __forceinline__ void copy(uint32_t to, const float *from) {
-    if (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits for a tile behind which the copies of AHEAD - 1 more have begun.
-template <int AHEAD, bool QUADS> __device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
-    if (QUADS)
-        __syncwarp();
-}
-
-// Rows that follow one another, from `from` on, `count` of them there: steps first, first + 4, ... of a piece.
-template <int S, bool QUADS> __device__ __forceinline__ void copy_rows(uint32_t to, const float *from, int stride, int count, int lane) {
-    const int first = QUADS ? lane >> 3 : 0;
-    from += (int64_t)first * stride;
-    to += (first * 32 + (QUADS ? (lane & 7) * 4 : lane)) * 4;
-#pragma unroll
-    for (int j = 0; j < (QUADS ? S / 4 : S); ++j)
-        if ((QUADS ? j * 4 : j) + first < count)
-            copy<QUADS ? 16 : 4>(to + j * (QUADS ? 512 : 128), from + (int64_t)(QUADS ? j * 4 : j) * stride);
-}
 __device__ __forceinline__ int clamped(int64_t steps) { return (int)max((int64_t)-1, min((int64_t)1 << 20, steps)); }
 
+// How values come into a block's shared memory.
+//   TILES: a group is 32 channels of one sequence; a piece of an array is one box of a tensor map, whose bytes a barrier counts.  (By cp.async, 16 bytes to a
+//     lane, copies and their addresses took a third of the first walk; as a bulk copy to each row, 15 clocks a row.)
+//   SINGLE: a group is 32 chains that follow one another, of several sequences where they have few channels, at any address; each lane copies what it reads.
+enum Source { TILES, SINGLE };
+template <int ARRAYS> struct Arrays {
+    CUtensorMap map[ARRAYS]; // [batch][steps][channels], TILES
+    const float *base[ARRAYS];
+};
+template <Source FROM>
+__device__ __forceinline__ Chain chain_of_lane(
+    int64_t group, int lane, int64_t chains, int64_t steps, int channels, const int64_t *__restrict__ lengths) {
+    if (FROM == SINGLE)
+        return chain_of(group * 32 + lane, chains, steps, channels, lengths);
+    const int64_t per = (channels + 31) / 32, b = group / per, c = (group - b * per) * 32 + lane;
+    return chain_of(c < channels ? b * channels + c : chains, chains, steps, channels, lengths);
+}
+
+// A warp's part of the ring: AHEAD tiles of ARRAYS pieces of S rows.  The last array's rows may be those of the step before (SHIFTED).
+template <int ARRAYS, int S, int AHEAD, Source FROM, bool SHIFTED> struct Ring {
+    static constexpr int FLOATS = AHEAD * ARRAYS * S * 32;
+    float *memory;
+    uint64_t *arrived; // [AHEAD]
+    int *gave_up;
+    const Arrays<ARRAYS> *arrays;
+    int64_t first; // SINGLE: of the chain's values
+    int channels, c0, batch, lane;
+
+    __device__ __forceinline__ Ring(float *all, uint64_t *barriers, int *flag, const Arrays<ARRAYS> &from, int width)
+        : memory(all + (threadIdx.x >> 5) * FLOATS), arrived(barriers), gave_up(flag), arrays(&from), channels(width), lane(threadIdx.x & 31) {
+        if (FROM == TILES && lane == 0) {
+            for (int i = 0; i < AHEAD; ++i)
+                mbar_init(shared_address(arrived + i), 1);
+            mbar_fence_init();
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void at(const Chain &c, int64_t group) {
+        first             = c.first;
+        const int64_t per = (channels + 31) / 32, b = group / per;
+        batch = (int)b, c0 = (int)(group - b * per) * 32;
+    }
+    // The piece that begins at step t, which has the chain's steps first_row .. last_row - 1 as rows.
+    __device__ __forceinline__ void fetch(int i, int64_t t, int first_row, int last_row) {
+        float *slot = memory + (i % AHEAD) * ARRAYS * S * 32;
+        if (FROM == SINGLE) {
+#pragma unroll
+            for (int k = 0; k < ARRAYS; ++k) {
+                const int shift   = SHIFTED && k == ARRAYS - 1;
+                const float *from = arrays->base[k] + first + (t - shift) * channels;
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    if (j >= first_row && j < last_row && (!shift || t + j > 0))
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(slot + (k * S + j) * 32 + lane)),
+                                     "l"(from + (int64_t)j * channels)
+                                     : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        } else if (lane < ARRAYS) {
+            const uint32_t bar = shared_address(arrived + i % AHEAD);
+            if (lane == 0)
+                mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * 128 : 0);
+            if (last_row > 0) // rows outside the sequence are zeros
+                tma_load_3d(shared_address(slot + lane * S * 32), &arrays->map[lane], bar, c0, (int)t - (SHIFTED && lane == ARRAYS - 1), batch);
+        }
+    }
+    __device__ __forceinline__ void wait(int i) {
+        if (FROM == SINGLE)
+            asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        else if (!*(volatile int *)gave_up) // (see Exchange)
+            mbar_wait(shared_address(arrived + i % AHEAD), (i / AHEAD) & 1, gave_up);
+        __syncwarp();
+    }
+    __device__ __forceinline__ float read(int i, int k, int j) const { return memory[(((i % AHEAD) * ARRAYS + k) * S + j) * 32 + lane]; }
+};
+
 // W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
-template <int W, int S, int AHEAD, bool QUADS, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_scan_kernel(
-    const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths, int64_t chains,
-    int64_t steps, int channels, int blocks, float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
-    extern __shared__ __align__(16) float ring[];
+template <int W, int S, int AHEAD, Source FROM, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_scan_kernel(
+    const __grid_constant__ Arrays<2> arrays, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int64_t steps, int channels, int blocks,
+    float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
+    extern __shared__ __align__(128) float ring[];
     __shared__ Exchange<W, CLUSTER> ex;
+    __shared__ uint64_t arrived[W][AHEAD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+    const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
+    Ring<2, S, AHEAD, FROM, false> values(ring, arrived[warp], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
-    const int64_t group = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * 32;
-    const Chain c       = chain_of(group + lane, chains, steps, channels, lengths);
-    const Chain source  = QUADS ? chain_of(group + (lane & 7) * 4, chains, steps, channels, lengths) : c;
-    const int64_t tile  = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = ((int64_t)rank * W + warp) * S;
-    float *mine         = ring + warp * AHEAD * kTileFloats<2, S>;
-    const uint32_t mine_at = shared_address(mine);
-    auto fetch             = [&](int i) {
-        const int64_t t   = t0 + i * tile, at = source.first + t * channels;
-        const uint32_t to = mine_at + (i % AHEAD) * kTileFloats<2, S> * 4;
-        const int count   = clamped(source.steps - t);
-        copy_rows<S, QUADS>(to, gate + at, channels, count, lane);
-        copy_rows<S, QUADS>(to + S * 128, value + at, channels, count, lane);
-        copies_end();
+    const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
+    values.at(c, group);
+    const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = ((int64_t)rank * W + warp) * S;
+    // (of a group's chains one is there, and its sequence is the others': whether anything of a piece is fetched is the same to the warp)
+    const int64_t last = FROM == SINGLE ? c.steps : __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
+    auto fetch         = [&](int i) {
+        const int64_t t = t0 + i * tile;
+        values.fetch(i, t, 0, clamped(last - t));
     };
     for (int i = 0; i < AHEAD; ++i)
         fetch(i);
@@ -257,32 +330,35 @@ __global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_
     const double state = walk<Steps>(
         ex, (int)((steps + tile - 1) / tile), c.here && state0 ? (double)state0[c.index] : 0.0, blocks,
         [&](int i, Steps &s) {
-            copies_wait<AHEAD, QUADS>();
-            const float *g  = mine + (i % AHEAD) * kTileFloats<2, S> + lane, *v = g + S * 32;
-            const int count = clamped(c.steps - (t0 + i * tile));
-            if (__all_sync(0xffffffffu, count >= S)) {
+            const int64_t t = t0 + i * tile;
+            const int count = clamped(c.steps - t);
+            values.wait(i);
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                s.a[j] = values.read(i, 0, j), s.add[j] = values.read(i, 1, j);
+            if (!__all_sync(0xffffffffu, count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j)
-                    s.a[j] = g[j * 32], s.add[j] = v[j * 32];
-            } else {
-#pragma unroll
-                for (int j = 0; j < S; ++j) // steps that a chain does not have keep its state: a = 1, and nothing is added
-                    s.a[j] = j < count ? g[j * 32] : INFINITY, s.add[j] = j < count ? v[j * 32] : 0.0f;
+                    if (j >= count) // steps that a chain does not have keep its state: a = 1, and nothing is added
+                        s.a[j] = INFINITY, s.add[j] = 0.0f;
             }
-            if (QUADS)
-                __syncwarp();
+            __syncwarp();
             fetch(i + AHEAD);
             Piece p;
 #pragma unroll
-            for (int j = 0; j < S; j += 2) {
-                f32x2 a, rest;
-                sigmoids2(s.a[j], s.a[j + 1], a, rest);
-                unpack2(mul2(rest, pack2(s.add[j], s.add[j + 1])), s.add[j], s.add[j + 1]);
-                unpack2(a, s.a[j], s.a[j + 1]);
-                float r0, r1;
-                unpack2(rest, r0, r1);
-                p.step(s.a[j], r0, s.add[j]);
-                p.step(s.a[j + 1], r1, s.add[j + 1]);
+            for (int j0 = 0; j0 < S; j0 += 2 * kPairs) {
+                f32x2 a[kPairs], rest[kPairs];
+                sigmoids2(s.a + j0, a, rest);
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i) {
+                    const int j = j0 + 2 * i;
+                    unpack2(mul2(rest[i], pack2(s.add[j], s.add[j + 1])), s.add[j], s.add[j + 1]);
+                    unpack2(a[i], s.a[j], s.a[j + 1]);
+                    float r0, r1;
+                    unpack2(rest[i], r0, r1);
+                    p.step(s.a[j], r0, s.add[j]);
+                    p.step(s.a[j + 1], r1, s.add[j + 1]);
+                }
             }
             return p.joined();
         },
@@ -314,39 +390,29 @@ __global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
-template <int W, int S, int AHEAD, bool QUADS, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_scan_grad_kernel(
-    const float *__restrict__ gate, const float *__restrict__ value, const float *state0, const int64_t *__restrict__ lengths,
-    const float *__restrict__ out, const float *__restrict__ dout, const float *dstate, int64_t chains, int64_t steps, int channels, int blocks,
-    float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
-    extern __shared__ __align__(16) float ring[];
+template <int W, int S, int AHEAD, Source FROM, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_scan_grad_kernel(
+    const __grid_constant__ Arrays<4> arrays, const float *state0, const int64_t *__restrict__ lengths, const float *dstate, int64_t chains, int64_t steps,
+    int channels, int blocks, float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
+    extern __shared__ __align__(128) float ring[];
     __shared__ Exchange<W, CLUSTER> ex;
+    __shared__ uint64_t arrived[W][AHEAD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
+    const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
+    Ring<4, S, AHEAD, FROM, true> values(ring, arrived[warp], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
-    const int64_t group = (int64_t)(CLUSTER ? blockIdx.x / blocks : blockIdx.x) * 32;
-    const Chain c       = chain_of(group + lane, chains, steps, channels, lengths);
-    const Chain source  = QUADS ? chain_of(group + (lane & 7) * 4, chains, steps, channels, lengths) : c;
-    const float first   = c.here && state0 ? state0[c.index] : 0.0f;
+    const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
+    values.at(c, group);
+    const float first = c.here && state0 ? state0[c.index] : 0.0f;
     // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
-    const int64_t tile  = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = steps - ((int64_t)rank * W + warp + 1) * S;
-    float *mine         = ring + warp * AHEAD * kTileFloats<4, S>;
-    const uint32_t mine_at = shared_address(mine);
-    auto fetch             = [&](int i) {
-        const int64_t t   = t0 - i * tile;
-        const uint32_t to = mine_at + (i % AHEAD) * kTileFloats<4, S> * 4;
-        const int skip    = t < 0 ? clamped(-t) : 0, count = clamped(source.steps - t);
-        const int64_t at  = source.first + (t + skip) * channels;
-        if (skip < S) {
-            const uint32_t from = to + skip * 128;
-            copy_rows<S, QUADS>(from, gate + at, channels, min(count, S) - skip, lane);
-            copy_rows<S, QUADS>(from + S * 128, value + at, channels, min(count, S) - skip, lane);
-            copy_rows<S, QUADS>(from + 2 * S * 128, dout + at, channels, min(count, S) - skip, lane);
-            const int begin = t + skip == 0; // the state before step 0 is none of out's
-            copy_rows<S, QUADS>(from + (3 * S + begin) * 128, out + at + (begin - 1) * (int64_t)channels, channels, min(count, S) - skip - begin, lane);
-        }
-        copies_end();
+    const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = steps - ((int64_t)rank * W + warp + 1) * S;
+    const int64_t last = FROM == SINGLE ? c.steps : __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
+    auto rows_there    = [&](int64_t t) { return t > -S ? clamped(last - t) : 0; };
+    auto fetch         = [&](int i) {
+        const int64_t t = t0 - i * tile;
+        values.fetch(i, t, clamped(-t), rows_there(t));
     };
     for (int i = 0; i < AHEAD; ++i)
         fetch(i);
@@ -356,37 +422,41 @@ __global__ void __launch_bounds__(W * 32, CLUSTER ? (W <= 8 ? 2 : 1) : 1) gated_
     const double state = walk<Steps>( // c[t+1]
         ex, (int)((steps + tile - 1) / tile), c.here && dstate ? (double)dstate[c.index] : 0.0, blocks,
         [&](int i, Steps &s) {
-            copies_wait<AHEAD, QUADS>();
-            const float *g = mine + (i % AHEAD) * kTileFloats<4, S> + lane, *v = g + S * 32, *d = v + S * 32, *h = d + S * 32;
             const int64_t t = t0 - i * tile;
             const int begin = clamped(-t), count = clamped(c.steps - t); // steps begin .. count - 1 are there
-            if (__all_sync(0xffffffffu, t > 0 && count >= S)) {
+            values.wait(i);
 #pragma unroll
-                for (int j = 0; j < S; ++j)
-                    s.a[j] = g[j * 32], s.rest[j] = v[j * 32], s.dy[j] = d[j * 32], s.gap[j] = h[j * 32];
-            } else {
+            for (int j = 0; j < S; ++j) {
+                s.a[j] = values.read(i, 0, j), s.rest[j] = values.read(i, 1, j), s.dy[j] = values.read(i, 2, j);
+                s.gap[j] = values.read(i, 3, j);
+            }
+            if (!__all_sync(0xffffffffu, t > 0 && count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
-                    const bool in = j >= begin && j < count;
-                    s.a[j] = in ? g[j * 32] : INFINITY, s.rest[j] = in ? v[j * 32] : 0.0f, s.dy[j] = in ? d[j * 32] : 0.0f;
-                    s.gap[j] = in ? (t + j > 0 ? h[j * 32] : first) : 0.0f;
+                    if (t + j == 0)
+                        s.gap[j] = first;
+                    if (j < begin || j >= count)
+                        s.a[j] = INFINITY, s.rest[j] = s.dy[j] = s.gap[j] = 0.0f;
                 }
             }
-            if (QUADS)
-                __syncwarp();
+            __syncwarp();
             fetch(i + AHEAD);
             Piece p;
 #pragma unroll
-            for (int j = S - 2; j >= 0; j -= 2) {
-                f32x2 a, rest;
-                sigmoids2(s.a[j], s.a[j + 1], a, rest);
-                float add0, add1;
-                unpack2(mul2(a, pack2(s.dy[j], s.dy[j + 1])), add0, add1);
-                unpack2(fma2(pack2(s.rest[j], s.rest[j + 1]), dup2(0xBF800000u), pack2(s.gap[j], s.gap[j + 1])), s.gap[j], s.gap[j + 1]);
-                unpack2(a, s.a[j], s.a[j + 1]);
-                unpack2(rest, s.rest[j], s.rest[j + 1]);
-                p.step(s.a[j + 1], s.rest[j + 1], add1);
-                p.step(s.a[j], s.rest[j], add0);
+            for (int j0 = S - 2 * kPairs; j0 >= 0; j0 -= 2 * kPairs) {
+                f32x2 a[kPairs], rest[kPairs];
+                sigmoids2(s.a + j0, a, rest);
+#pragma unroll
+                for (int i = kPairs - 1; i >= 0; --i) {
+                    const int j = j0 + 2 * i;
+                    float add0, add1;
+                    unpack2(mul2(a[i], pack2(s.dy[j], s.dy[j + 1])), add0, add1);
+                    unpack2(fma2(pack2(s.rest[j], s.rest[j + 1]), dup2(0xBF800000u), pack2(s.gap[j], s.gap[j + 1])), s.gap[j], s.gap[j + 1]);
+                    unpack2(a[i], s.a[j], s.a[j + 1]);
+                    unpack2(rest[i], s.rest[j], s.rest[j + 1]);
+                    p.step(s.a[j + 1], s.rest[j + 1], add1);
+                    p.step(s.a[j], s.rest[j], add0);
+                }
             }
             return p.joined();
         },
@@ -541,12 +611,12 @@ ct_status check_scan(const char *name, int64_t batch, int64_t steps, int64_t cha
 
 // Blocks to a cluster: as many as let all groups of 32 chains run at once, and have a piece of the steps each.  (Clusters that wait for others' end cost a
 // second walk: 16 groups in clusters of 8, of which 15 fit beside one another, took twice the time.)
-template <typename Kernel> ct_status scan_blocks(const DeviceState *st, Kernel kernel, int threads, int smem, int64_t groups, int64_t pieces, int *blocks) {
-    static int fit[16][kMostBlocks + 1] = {}; // clusters at once, by device and size, and 1; under the entry points' lock
+template <auto KERNEL> ct_status scan_blocks(const DeviceState *st, int threads, int smem, int64_t groups, int64_t pieces, int *blocks) {
+    static int fit[16][kMostBlocks + 1] = {}; // clusters at once, by device and size; [1] 1 when they are known.  Under the entry points' lock
     int *mine                           = fit[st->device & 15];
     if (mine[1] == 0) {
-        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CT_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CT_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         for (int size = 2; size <= kMostBlocks; ++size) {
             cudaLaunchAttribute attr{};
             attr.id               = cudaLaunchAttributeClusterDimension;
@@ -554,7 +624,7 @@ template <typename Kernel> ct_status scan_blocks(const DeviceState *st, Kernel k
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3((unsigned)size), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = (size_t)smem;
             cfg.attrs = &attr, cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&mine[size], kernel, &cfg) != cudaSuccess) {
+            if (cudaOccupancyMaxActiveClusters(&mine[size], KERNEL, &cfg) != cudaSuccess) {
                 cudaGetLastError();
                 mine[size] = 0;
             }
@@ -566,6 +636,61 @@ template <typename Kernel> ct_status scan_blocks(const DeviceState *st, Kernel k
         --*blocks;
     return CT_OK;
 }
+
+template <int ARRAYS> ct_status encode_arrays(Arrays<ARRAYS> &arrays, int64_t batch, int64_t steps, int64_t channels, int rows) {
+    const uint64_t dims[3] = {(uint64_t)channels, (uint64_t)steps, (uint64_t)batch}, strides[2] = {(uint64_t)channels * 4, (uint64_t)(steps * channels) * 4};
+    const uint32_t box[3]  = {32, (uint32_t)rows, 1};
+    for (int k = 0; k < ARRAYS; ++k)
+        CT_TRY(encode_tiled_map_f32(&arrays.map[k], arrays.base[k], 3, dims, strides, box, 0));
+    return CT_OK;
+}
+
+#define CT_SCAN(NAME, KERNEL, W, S, AHEAD, FROM, RING, ...)                                                                                              \
+    [&]() -> ct_status {                                                                                                                                 \
+        constexpr int smem   = (W) * RING::FLOATS * 4;                                                                                                   \
+        const int64_t groups = (FROM) == SINGLE ? (chains + 31) / 32 : batch * ((channels + 31) / 32);                                                   \
+        int blocks;                                                                                                                                      \
+        CT_TRY((scan_blocks<KERNEL<W, S, AHEAD, FROM, true>>(st, (W) * 32, smem, groups, (steps + (W) * (S) - 1) / ((W) * (S)), &blocks)));              \
+        auto kernel = blocks > 1 ? KERNEL<W, S, AHEAD, FROM, true> : KERNEL<W, S, AHEAD, FROM, false>;                                                   \
+        if (blocks == 1)                                                                                                                                 \
+            CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                                    \
+        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3((W) * 32), smem, stream(), __VA_ARGS__));               \
+        CT_LAUNCH_CHECK(NAME);                                                                                                                           \
+        return CT_OK;                                                                                                                                    \
+    }()
+
+bool scan_is_short(const DeviceState *st, int64_t batch, int64_t steps, int64_t channels) {
+    static const int ov = getenv("CT_VAR") ? atoi(getenv("CT_VAR")) : 0;
+    (void)st, (void)batch, (void)channels;
+    return ov ? ov == 4 : steps <= 256;
+}
+template <int W, Source FROM>
+ct_status launch_scan(
+    const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, int64_t batch, int64_t steps, int64_t channels,
+    float *out, float *state) {
+    constexpr int S = 16, AHEAD = 2;
+    const int64_t chains = batch * channels;
+    using Values         = Ring<2, S, AHEAD, FROM, false>;
+    Arrays<2> arrays     = {{}, {gate, value}};
+    if (FROM == TILES)
+        CT_TRY(encode_arrays(arrays, batch, steps, channels, S));
+    return CT_SCAN("gated_scan", gated_scan_kernel, W, S, AHEAD, FROM, Values, arrays, state0, lengths, chains, steps, (int)channels, blocks, out, state,
+                   st->flags_dev);
+}
+template <int W, Source FROM>
+ct_status launch_scan_grad(
+    const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, const float *out, const float *dout,
+    const float *dstate, int64_t batch, int64_t steps, int64_t channels, float *dgate, float *dvalue, float *dstate0) {
+    constexpr int S = 8, AHEAD = 2;
+    const int64_t chains = batch * channels;
+    using Values         = Ring<4, S, AHEAD, FROM, true>;
+    Arrays<4> arrays     = {{}, {gate, value, dout, out}};
+    if (FROM == TILES)
+        CT_TRY(encode_arrays(arrays, batch, steps, channels, S));
+    return CT_SCAN("gated_scan_grad", gated_scan_grad_kernel, W, S, AHEAD, FROM, Values, arrays, state0, lengths, dstate, chains, steps,
+                   (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev);
+}
+#undef CT_SCAN
 
 } // namespace
 } // namespace ct
@@ -587,7 +712,6 @@ ct_status ct_gated_scan(
     if (steps > 0 && (!gate || !value))
         return fail(CT_ERR_INVALID, "gated_scan: null pointer");
     ProfScope prof("gated_scan");
-    constexpr int W = 8, S = 16, AHEAD = 2;
     if (steps <= kFewSteps) {
         const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, state});
         auto launch     = [&](auto kernel, int v) -> ct_status {
@@ -602,22 +726,14 @@ ct_status ct_gated_scan(
             return four ? launch(gated_steps_kernel<4, 4>, 4) : launch(gated_steps_kernel<1, 4>, 1);
         return launch(gated_steps_kernel<1, kFewSteps>, 1);
     }
-    const int64_t groups = (chains + 31) / 32;
-    constexpr int smem   = W * AHEAD * kTileFloats<2, S> * 4;
-    const bool quads     = channels % 4 == 0 && aligned16({gate, value});
-    int blocks;
-    CT_TRY(scan_blocks(st, gated_scan_kernel<W, S, AHEAD, true, true>, W * 32, smem, groups, (steps + W * S - 1) / (W * S), &blocks));
-    auto launch = [&](auto kernel) -> ct_status {
-        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        if (blocks > 8)
-            CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), smem, stream(), gate, value, state0, lengths, chains, steps, (int)channels, blocks, out, state, st->flags_dev));
-        CT_LAUNCH_CHECK("gated_scan");
-        return CT_OK;
+    // (groups of fewer channels would leave lanes without a chain; a tensor map has 40 bits for a stride)
+    const bool tiles = channels >= 32 && channels % 4 == 0 && aligned16({gate, value}) && steps * channels < (int64_t)1 << 37;
+    auto launch      = [&](auto warps) -> ct_status {
+        constexpr int W = decltype(warps)::value;
+        return tiles ? launch_scan<W, TILES>(st, gate, value, state0, lengths, batch, steps, channels, out, state)
+                     : launch_scan<W, SINGLE>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
     };
-    if (blocks == 1)
-        return quads ? launch(gated_scan_kernel<W, S, AHEAD, true, false>) : launch(gated_scan_kernel<W, S, AHEAD, false, false>);
-    return quads ? launch(gated_scan_kernel<W, S, AHEAD, true, true>) : launch(gated_scan_kernel<W, S, AHEAD, false, true>);
+    return scan_is_short(st, batch, steps, channels) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
 }
 
 ct_status ct_gated_scan_grad(
@@ -633,7 +749,6 @@ ct_status ct_gated_scan_grad(
     if (steps > 0 && (!gate || !value || !out || !dout))
         return fail(CT_ERR_INVALID, "gated_scan_grad: null pointer");
     ProfScope prof("gated_scan_grad");
-    constexpr int W = 8, S = 8, AHEAD = 2;
     if (steps <= kFewSteps) {
         const bool four = channels % 4 == 0 && aligned16({gate, value, state0, out, dout, dstate, dgate, dvalue, dstate0});
         auto launch     = [&](auto kernel, int v) -> ct_status {
@@ -648,22 +763,14 @@ ct_status ct_gated_scan_grad(
             return four ? launch(gated_steps_grad_kernel<4, 4>, 4) : launch(gated_steps_grad_kernel<1, 4>, 1);
         return launch(gated_steps_grad_kernel<1, kFewSteps>, 1);
     }
-    const int64_t groups = (chains + 31) / 32;
-    constexpr int smem   = W * AHEAD * kTileFloats<4, S> * 4;
-    const bool quads     = channels % 4 == 0 && aligned16({gate, value, out, dout});
-    int blocks;
-    CT_TRY(scan_blocks(st, gated_scan_grad_kernel<W, S, AHEAD, true, true>, W * 32, smem, groups, (steps + W * S - 1) / (W * S), &blocks));
-    auto launch = [&](auto kernel) -> ct_status {
-        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        if (blocks > 8)
-            CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3(W * 32), smem, stream(), gate, value, state0, lengths, out, dout, dstate, chains, steps, (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev));
-        CT_LAUNCH_CHECK("gated_scan_grad");
-        return CT_OK;
+    // (groups of fewer channels would leave lanes without a chain; a tensor map has 40 bits for a stride)
+    const bool tiles = channels >= 32 && channels % 4 == 0 && aligned16({gate, value, out, dout}) && steps * channels < (int64_t)1 << 37;
+    auto launch      = [&](auto warps) -> ct_status {
+        constexpr int W = decltype(warps)::value;
+        return tiles ? launch_scan_grad<W, TILES>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0)
+                     : launch_scan_grad<W, SINGLE>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
     };
-    if (blocks == 1)
-        return quads ? launch(gated_scan_grad_kernel<W, S, AHEAD, true, false>) : launch(gated_scan_grad_kernel<W, S, AHEAD, false, false>);
-    return quads ? launch(gated_scan_grad_kernel<W, S, AHEAD, true, true>) : launch(gated_scan_grad_kernel<W, S, AHEAD, false, true>);
+    return scan_is_short(st, batch, steps, channels) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
 }
 
 } // extern "C"
