@@ -84,7 +84,7 @@ template <int N> __device__ __forceinline__ void sigmoids2(const float *g, f32x2
 }
 constexpr int kPairs = 4; // together
 
-constexpr int kMostBlocks = 16; // of a cluster
+template <int W> constexpr int kMostBlocks = W == 8 ? 15 : 8; // of a cluster; their places are shared memory that other blocks cannot have
 
 // How the pieces of a tile meet.  A block's pieces lie in the order of its warps; what they do together goes to the other blocks of the cluster by
 // st.async, whose arrival a barrier counts (a cluster-wide barrier would wait until the last tile's stores to global memory are done).  Meanwhile the block
@@ -94,7 +94,7 @@ template <int W, bool CLUSTER> struct Exchange {
     int gave_up;              // a wait has run out: it is reported at the end, and until then the block goes on, for the others' sake
 };
 template <int W> struct Exchange<W, true> : Exchange<W, false> {
-    double2 blocks[4][kMostBlocks][32];
+    double2 blocks[4][kMostBlocks<W>][32];
     uint64_t arrived[4];
 };
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -226,10 +226,12 @@ __device__ __forceinline__ int clamped(int64_t steps) { return (int)max((int64_t
 // How values come into a block's shared memory.
 //   TILES: a group is 32 channels of one sequence; a piece of an array is one box of a tensor map, whose bytes a barrier counts.  (By cp.async, 16 bytes to a
 //     lane, copies and their addresses took a third of the first walk; as a bulk copy to each row, 15 clocks a row.)
+//   ROWS: the same where channels are no multiple of four, and rows begin anywhere.  Four rows together do begin on 16 bytes: the map's rows are these, and
+//     a piece is four boxes, of the rows 0, 4, .., those behind them, and so on, each from the multiple of four values before its first one.
 //   SINGLE: a group is 32 chains that follow one another, of several sequences where they have few channels, at any address; each lane copies what it reads.
-enum Source { TILES, SINGLE };
+enum Source { TILES, ROWS, SINGLE };
 template <int ARRAYS> struct Arrays {
-    CUtensorMap map[ARRAYS]; // [batch][steps][channels], TILES
+    CUtensorMap map[ARRAYS]; // TILES: [batch][steps][channels]; ROWS: [batch * steps / 4][4 channels]
     const float *base[ARRAYS];
 };
 template <Source FROM>
@@ -241,33 +243,37 @@ __device__ __forceinline__ Chain chain_of_lane(
     return chain_of(c < channels ? b * channels + c : chains, chains, steps, channels, lengths);
 }
 
-// A warp's part of the ring: AHEAD tiles of ARRAYS pieces of S rows.  The last array's rows may be those of the step before (SHIFTED).
-template <int ARRAYS, int S, int AHEAD, Source FROM, bool SHIFTED> struct Ring {
-    static constexpr int FLOATS = AHEAD * ARRAYS * S * 32;
+// A warp's ARRAYS pieces of S rows.  The next tile's are fetched when a tile's have been read, a quarter of a tile's time from its beginning, and arrive
+// meanwhile; a second place for them gained nothing and kept other blocks out (8 x 2048 x 2048 backward 152 us with it, 136 without).
+// The last array's rows may be those of the step before (SHIFTED).
+template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
+    static constexpr int BOXES = FROM == ROWS ? 4 : 1, ROW = FROM == ROWS ? 36 : 32; // values of a box's row
+    static constexpr int BOX = (S / BOXES * ROW + 31) & ~31, PIECE = BOXES * BOX, FLOATS = ARRAYS * PIECE; // a box begins on 128 bytes
     float *memory;
-    uint64_t *arrived; // [AHEAD]
+    uint64_t *arrived;
     int *gave_up;
     const Arrays<ARRAYS> *arrays;
-    int64_t first; // SINGLE: of the chain's values
+    int64_t first;     // SINGLE: of the chain's values; ROWS: of the sequence's rows
+    int64_t in_groups; // ROWS: rows that are in groups of four, all but the last three at most
     int channels, c0, batch, lane;
 
-    __device__ __forceinline__ Ring(float *all, uint64_t *barriers, int *flag, const Arrays<ARRAYS> &from, int width)
+    __device__ __forceinline__ Pieces(float *all, uint64_t *barriers, int *flag, const Arrays<ARRAYS> &from, int width)
         : memory(all + (threadIdx.x >> 5) * FLOATS), arrived(barriers), gave_up(flag), arrays(&from), channels(width), lane(threadIdx.x & 31) {
-        if (FROM == TILES && lane == 0) {
-            for (int i = 0; i < AHEAD; ++i)
-                mbar_init(shared_address(arrived + i), 1);
+        if (FROM != SINGLE && lane == 0) {
+            mbar_init(shared_address(arrived), 1);
             mbar_fence_init();
         }
         __syncwarp();
     }
-    __device__ __forceinline__ void at(const Chain &c, int64_t group) {
-        first             = c.first;
+    __device__ __forceinline__ void at(const Chain &c, int64_t group, int64_t chains, int64_t steps) {
         const int64_t per = (channels + 31) / 32, b = group / per;
         batch = (int)b, c0 = (int)(group - b * per) * 32;
+        first     = FROM == ROWS ? b * steps : c.first;
+        in_groups = chains / channels * steps & ~(int64_t)3;
+        t_end     = steps;
     }
     // The piece that begins at step t, which has the chain's steps first_row .. last_row - 1 as rows.
-    __device__ __forceinline__ void fetch(int i, int64_t t, int first_row, int last_row) {
-        float *slot = memory + (i % AHEAD) * ARRAYS * S * 32;
+    __device__ __forceinline__ void fetch(int64_t t, int first_row, int last_row) {
         if (FROM == SINGLE) {
 #pragma unroll
             for (int k = 0; k < ARRAYS; ++k) {
@@ -276,54 +282,87 @@ template <int ARRAYS, int S, int AHEAD, Source FROM, bool SHIFTED> struct Ring {
 #pragma unroll
                 for (int j = 0; j < S; ++j)
                     if (j >= first_row && j < last_row && (!shift || t + j > 0))
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(slot + (k * S + j) * 32 + lane)),
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(memory + k * PIECE + j * 32 + lane)),
                                      "l"(from + (int64_t)j * channels)
                                      : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-        } else if (lane < ARRAYS) {
-            const uint32_t bar = shared_address(arrived + i % AHEAD);
+            return;
+        }
+        if (lane < ARRAYS * BOXES) {
+            const uint32_t bar = shared_address(arrived);
+            const int k = lane / BOXES, box = lane % BOXES, shift = SHIFTED && k == ARRAYS - 1;
             if (lane == 0)
-                mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * 128 : 0);
-            if (last_row > 0) // rows outside the sequence are zeros
-                tma_load_3d(shared_address(slot + lane * S * 32), &arrays->map[lane], bar, c0, (int)t - (SHIFTED && lane == ARRAYS - 1), batch);
+                mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * ROW * 4 : 0);
+            if (last_row > 0) { // what a box has outside the array is zeros; rows of other sequences are not used
+                const uint32_t to = shared_address(memory + lane * BOX);
+                if (FROM == TILES) {
+                    tma_load_3d(to, &arrays->map[k], bar, c0, (int)t - shift, batch);
+                } else {
+                    const int64_t row = first + t - shift + box;
+                    tma_load_2d(to, &arrays->map[k], bar, ((int)(row & 3) * channels + c0) & ~3, (int)(row >> 2));
+                }
+            }
         }
     }
     __device__ __forceinline__ void wait(int i) {
         if (FROM == SINGLE)
-            asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         else if (!*(volatile int *)gave_up) // (see Exchange)
-            mbar_wait(shared_address(arrived + i % AHEAD), (i / AHEAD) & 1, gave_up);
+            mbar_wait(shared_address(arrived), i & 1, gave_up);
         __syncwarp();
     }
-    __device__ __forceinline__ float read(int i, int k, int j) const { return memory[(((i % AHEAD) * ARRAYS + k) * S + j) * 32 + lane]; }
+    // The lane's values in array k of the piece that begins at step t.
+    __device__ __forceinline__ void read(int k, int64_t t, float (&to)[S]) const {
+        const float *from = memory + k * PIECE + lane;
+        if (FROM == ROWS) {
+            const int64_t row = first + t - (SHIFTED && k == ARRAYS - 1);
+            int skew[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                skew[q] = (((int)(row + q) & 3) * channels + c0) & 3;
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                to[j] = from[(j & 3) * BOX + j / 4 * ROW + skew[j & 3]];
+            if (row + S > in_groups) { // the array's last rows
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    if (row + j >= in_groups && t + j < t_end && c0 + lane < channels)
+                        to[j] = arrays->base[k][(row + j) * channels + c0 + lane];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                to[j] = from[j * ROW];
+        }
+    }
+    int64_t t_end; // steps of the sequence, padding among them
 };
 
 // W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
-template <int W, int S, int AHEAD, Source FROM, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_scan_kernel(
+template <int W, int S, Source FROM, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated_scan_kernel(
     const __grid_constant__ Arrays<2> arrays, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int64_t steps, int channels, int blocks,
     float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
-    extern __shared__ __align__(128) float ring[];
+    extern __shared__ __align__(128) float pieces[];
     __shared__ Exchange<W, CLUSTER> ex;
-    __shared__ uint64_t arrived[W][AHEAD];
+    __shared__ uint64_t arrived[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
     const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
-    Ring<2, S, AHEAD, FROM, false> values(ring, arrived[warp], &ex.gave_up, arrays, channels);
+    Pieces<2, S, FROM, false> values(pieces, &arrived[warp], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
-    values.at(c, group);
+    values.at(c, group, chains, steps);
     const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = ((int64_t)rank * W + warp) * S;
     // (of a group's chains one is there, and its sequence is the others': whether anything of a piece is fetched is the same to the warp)
     const int64_t last = FROM == SINGLE ? c.steps : __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
     auto fetch         = [&](int i) {
         const int64_t t = t0 + i * tile;
-        values.fetch(i, t, 0, clamped(last - t));
+        values.fetch(t, 0, clamped(last - t));
     };
-    for (int i = 0; i < AHEAD; ++i)
-        fetch(i);
+    fetch(0);
     struct Steps {
         float a[S], add[S];
     };
@@ -333,9 +372,8 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
             const int64_t t = t0 + i * tile;
             const int count = clamped(c.steps - t);
             values.wait(i);
-#pragma unroll
-            for (int j = 0; j < S; ++j)
-                s.a[j] = values.read(i, 0, j), s.add[j] = values.read(i, 1, j);
+            values.read(0, t, s.a);
+            values.read(1, t, s.add);
             if (!__all_sync(0xffffffffu, count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j)
@@ -343,7 +381,7 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
                         s.a[j] = INFINITY, s.add[j] = 0.0f;
             }
             __syncwarp();
-            fetch(i + AHEAD);
+            fetch(i + 1);
             Piece p;
 #pragma unroll
             for (int j0 = 0; j0 < S; j0 += 2 * kPairs) {
@@ -390,21 +428,21 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
-template <int W, int S, int AHEAD, Source FROM, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_scan_grad_kernel(
+template <int W, int S, Source FROM, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated_scan_grad_kernel(
     const __grid_constant__ Arrays<4> arrays, const float *state0, const int64_t *__restrict__ lengths, const float *dstate, int64_t chains, int64_t steps,
     int channels, int blocks, float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
-    extern __shared__ __align__(128) float ring[];
+    extern __shared__ __align__(128) float pieces[];
     __shared__ Exchange<W, CLUSTER> ex;
-    __shared__ uint64_t arrived[W][AHEAD];
+    __shared__ uint64_t arrived[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
     const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
-    Ring<4, S, AHEAD, FROM, true> values(ring, arrived[warp], &ex.gave_up, arrays, channels);
+    Pieces<4, S, FROM, true> values(pieces, &arrived[warp], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
-    values.at(c, group);
+    values.at(c, group, chains, steps);
     const float first = c.here && state0 ? state0[c.index] : 0.0f;
     // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
     const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = steps - ((int64_t)rank * W + warp + 1) * S;
@@ -412,10 +450,9 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
     auto rows_there    = [&](int64_t t) { return t > -S ? clamped(last - t) : 0; };
     auto fetch         = [&](int i) {
         const int64_t t = t0 - i * tile;
-        values.fetch(i, t, clamped(-t), rows_there(t));
+        values.fetch(t, clamped(-t), rows_there(t));
     };
-    for (int i = 0; i < AHEAD; ++i)
-        fetch(i);
+    fetch(0);
     struct Steps {
         float a[S], rest[S], gap[S], dy[S]; // gap: h[t-1] - value[t]
     };
@@ -425,11 +462,10 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
             const int64_t t = t0 - i * tile;
             const int begin = clamped(-t), count = clamped(c.steps - t); // steps begin .. count - 1 are there
             values.wait(i);
-#pragma unroll
-            for (int j = 0; j < S; ++j) {
-                s.a[j] = values.read(i, 0, j), s.rest[j] = values.read(i, 1, j), s.dy[j] = values.read(i, 2, j);
-                s.gap[j] = values.read(i, 3, j);
-            }
+            values.read(0, t, s.a);
+            values.read(1, t, s.rest);
+            values.read(2, t, s.dy);
+            values.read(3, t, s.gap);
             if (!__all_sync(0xffffffffu, t > 0 && count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
@@ -440,7 +476,7 @@ __global__ void __launch_bounds__(W * 32, FROM == TILES ? 16 / W : 8 / W) gated_
                 }
             }
             __syncwarp();
-            fetch(i + AHEAD);
+            fetch(i + 1);
             Piece p;
 #pragma unroll
             for (int j0 = S - 2 * kPairs; j0 >= 0; j0 -= 2 * kPairs) {
@@ -611,18 +647,18 @@ ct_status check_scan(const char *name, int64_t batch, int64_t steps, int64_t cha
 
 // Blocks to a cluster: as many as let all groups of 32 chains run at once, and have a piece of the steps each.  (Clusters that wait for others' end cost a
 // second walk: 16 groups in clusters of 8, of which 15 fit beside one another, took twice the time.)
-template <auto KERNEL> ct_status scan_blocks(const DeviceState *st, int threads, int smem, int64_t groups, int64_t pieces, int *blocks) {
-    static int fit[16][kMostBlocks + 1] = {}; // clusters at once, by device and size; [1] 1 when they are known.  Under the entry points' lock
+template <auto KERNEL, int W> ct_status scan_blocks(const DeviceState *st, int smem, int64_t groups, int64_t pieces, int *blocks) {
+    static int fit[16][kMostBlocks<W> + 1] = {}; // clusters at once, by device and size; [1] 1 when they are known.  Under the entry points' lock
     int *mine                           = fit[st->device & 15];
     if (mine[1] == 0) {
         CT_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         CT_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        for (int size = 2; size <= kMostBlocks; ++size) {
+        for (int size = 2; size <= kMostBlocks<W>; ++size) {
             cudaLaunchAttribute attr{};
             attr.id               = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = (unsigned)size, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
             cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3((unsigned)size), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = (size_t)smem;
+            cfg.gridDim = dim3((unsigned)size), cfg.blockDim = dim3((unsigned)W * 32), cfg.dynamicSmemBytes = (size_t)smem;
             cfg.attrs = &attr, cfg.numAttrs = 1;
             if (cudaOccupancyMaxActiveClusters(&mine[size], KERNEL, &cfg) != cudaSuccess) {
                 cudaGetLastError();
@@ -631,27 +667,33 @@ template <auto KERNEL> ct_status scan_blocks(const DeviceState *st, int threads,
         }
         mine[1] = 1;
     }
-    *blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kMostBlocks, pieces));
+    *blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kMostBlocks<W>, pieces));
     while (*blocks > 1 && mine[*blocks] < groups)
         --*blocks;
     return CT_OK;
 }
 
-template <int ARRAYS> ct_status encode_arrays(Arrays<ARRAYS> &arrays, int64_t batch, int64_t steps, int64_t channels, int rows) {
-    const uint64_t dims[3] = {(uint64_t)channels, (uint64_t)steps, (uint64_t)batch}, strides[2] = {(uint64_t)channels * 4, (uint64_t)(steps * channels) * 4};
-    const uint32_t box[3]  = {32, (uint32_t)rows, 1};
+template <int ARRAYS> ct_status encode_arrays(Source from, Arrays<ARRAYS> &arrays, int64_t batch, int64_t steps, int64_t channels, int rows) {
+    const uint64_t c = (uint64_t)channels, t = (uint64_t)steps, b = (uint64_t)batch;
+    const uint64_t tiles[3] = {c, t, b}, tile_strides[2] = {c * 4, t * c * 4}, fours[2] = {4 * c, b * t / 4}, four_strides[1] = {16 * c};
+    const uint32_t tile_box[3] = {32, (uint32_t)rows, 1}, four_box[2] = {36, (uint32_t)rows / 4};
     for (int k = 0; k < ARRAYS; ++k)
-        CT_TRY(encode_tiled_map_f32(&arrays.map[k], arrays.base[k], 3, dims, strides, box, 0));
+        CT_TRY(from == TILES ? encode_tiled_map_f32(&arrays.map[k], arrays.base[k], 3, tiles, tile_strides, tile_box, 0)
+                             : encode_tiled_map_f32(&arrays.map[k], arrays.base[k], 2, fours, four_strides, four_box, 0));
     return CT_OK;
 }
 
-#define CT_SCAN(NAME, KERNEL, W, S, AHEAD, FROM, RING, ...)                                                                                              \
+int64_t scan_groups(Source from, int64_t batch, int64_t channels) {
+    return from == SINGLE ? (batch * channels + 31) / 32 : batch * ((channels + 31) / 32);
+}
+
+#define CT_SCAN(NAME, KERNEL, W, S, FROM, PIECES, ...)                                                                                              \
     [&]() -> ct_status {                                                                                                                                 \
-        constexpr int smem   = (W) * RING::FLOATS * 4;                                                                                                   \
-        const int64_t groups = (FROM) == SINGLE ? (chains + 31) / 32 : batch * ((channels + 31) / 32);                                                   \
+        constexpr int smem   = (W) * PIECES::FLOATS * 4;                                                                                                   \
+        const int64_t groups = scan_groups(FROM, batch, channels);                                                                                       \
         int blocks;                                                                                                                                      \
-        CT_TRY((scan_blocks<KERNEL<W, S, AHEAD, FROM, true>>(st, (W) * 32, smem, groups, (steps + (W) * (S) - 1) / ((W) * (S)), &blocks)));              \
-        auto kernel = blocks > 1 ? KERNEL<W, S, AHEAD, FROM, true> : KERNEL<W, S, AHEAD, FROM, false>;                                                   \
+        CT_TRY((scan_blocks<KERNEL<W, S, FROM, true>, W>(st, smem, groups, (steps + (W) * (S) - 1) / ((W) * (S)), &blocks)));              \
+        auto kernel = blocks > 1 ? KERNEL<W, S, FROM, true> : KERNEL<W, S, FROM, false>;                                                   \
         if (blocks == 1)                                                                                                                                 \
             CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                                    \
         CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3((W) * 32), smem, stream(), __VA_ARGS__));               \
@@ -659,35 +701,41 @@ template <int ARRAYS> ct_status encode_arrays(Arrays<ARRAYS> &arrays, int64_t ba
         return CT_OK;                                                                                                                                    \
     }()
 
-bool scan_is_short(const DeviceState *st, int64_t batch, int64_t steps, int64_t channels) {
-    static const int ov = getenv("CT_VAR") ? atoi(getenv("CT_VAR")) : 0;
-    (void)st, (void)batch, (void)channels;
-    return ov ? ov == 4 : steps <= 256;
+Source scan_source(int64_t batch, int64_t steps, int64_t channels, bool aligned) {
+    // groups of fewer channels would leave lanes without a chain; a tensor map has 31 bits for a row and 40 for a stride
+    if (channels < 32 || !aligned || steps * channels >= (int64_t)1 << 37 || batch * steps >= (int64_t)1 << 31)
+        return SINGLE;
+    return channels % 4 == 0 ? TILES : ROWS;
 }
+// Warps to a block, measured (us forward, backward; 2, 4 and 8 warps): 16 groups of chains, 65536 steps 195 and 104 (4, 8), 480 and 212; 32 groups, 2048
+// steps 19, 16, 14, 35, 25, 21; 64 groups 23, 19, 18, 39, 29, 31; 175 groups, 1537 steps 39, 37, 41, 72, 62, 76; 512 groups, 2048 steps 80, 72, 74, 156, 135,
+// 140; 16000 groups, 20 steps 45, 81, 156, 64, 76, 162.
+int scan_warps(const DeviceState *st, int64_t groups, int64_t steps) { return steps <= 32 ? 2 : groups * 3 <= st->sm_count ? 8 : 4; }
+
 template <int W, Source FROM>
 ct_status launch_scan(
     const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, int64_t batch, int64_t steps, int64_t channels,
     float *out, float *state) {
-    constexpr int S = 16, AHEAD = 2;
+    constexpr int S = 16;
     const int64_t chains = batch * channels;
-    using Values         = Ring<2, S, AHEAD, FROM, false>;
+    using Values         = Pieces<2, S, FROM, false>;
     Arrays<2> arrays     = {{}, {gate, value}};
-    if (FROM == TILES)
-        CT_TRY(encode_arrays(arrays, batch, steps, channels, S));
-    return CT_SCAN("gated_scan", gated_scan_kernel, W, S, AHEAD, FROM, Values, arrays, state0, lengths, chains, steps, (int)channels, blocks, out, state,
+    if (FROM != SINGLE)
+        CT_TRY(encode_arrays(FROM, arrays, batch, steps, channels, S));
+    return CT_SCAN("gated_scan", gated_scan_kernel, W, S, FROM, Values, arrays, state0, lengths, chains, steps, (int)channels, blocks, out, state,
                    st->flags_dev);
 }
 template <int W, Source FROM>
 ct_status launch_scan_grad(
     const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, const float *out, const float *dout,
     const float *dstate, int64_t batch, int64_t steps, int64_t channels, float *dgate, float *dvalue, float *dstate0) {
-    constexpr int S = 8, AHEAD = 2;
+    constexpr int S = 8;
     const int64_t chains = batch * channels;
-    using Values         = Ring<4, S, AHEAD, FROM, true>;
+    using Values         = Pieces<4, S, FROM, true>;
     Arrays<4> arrays     = {{}, {gate, value, dout, out}};
-    if (FROM == TILES)
-        CT_TRY(encode_arrays(arrays, batch, steps, channels, S));
-    return CT_SCAN("gated_scan_grad", gated_scan_grad_kernel, W, S, AHEAD, FROM, Values, arrays, state0, lengths, dstate, chains, steps,
+    if (FROM != SINGLE)
+        CT_TRY(encode_arrays(FROM, arrays, batch, steps, channels, S));
+    return CT_SCAN("gated_scan_grad", gated_scan_grad_kernel, W, S, FROM, Values, arrays, state0, lengths, dstate, chains, steps,
                    (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev);
 }
 #undef CT_SCAN
@@ -726,14 +774,26 @@ ct_status ct_gated_scan(
             return four ? launch(gated_steps_kernel<4, 4>, 4) : launch(gated_steps_kernel<1, 4>, 1);
         return launch(gated_steps_kernel<1, kFewSteps>, 1);
     }
-    // (groups of fewer channels would leave lanes without a chain; a tensor map has 40 bits for a stride)
-    const bool tiles = channels >= 32 && channels % 4 == 0 && aligned16({gate, value}) && steps * channels < (int64_t)1 << 37;
-    auto launch      = [&](auto warps) -> ct_status {
+    const Source from = scan_source(batch, steps, channels, aligned16({gate, value}));
+    auto launch       = [&](auto warps) -> ct_status {
         constexpr int W = decltype(warps)::value;
-        return tiles ? launch_scan<W, TILES>(st, gate, value, state0, lengths, batch, steps, channels, out, state)
-                     : launch_scan<W, SINGLE>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+        switch (from) {
+        case TILES:
+            return launch_scan<W, TILES>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+        case ROWS:
+            return launch_scan<W, ROWS>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+        default:
+            return launch_scan<W, SINGLE>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+        }
     };
-    return scan_is_short(st, batch, steps, channels) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
+    switch (scan_warps(st, scan_groups(from, batch, channels), steps)) {
+    case 2:
+        return launch(std::integral_constant<int, 2>{});
+    case 4:
+        return launch(std::integral_constant<int, 4>{});
+    default:
+        return launch(std::integral_constant<int, 8>{});
+    }
 }
 
 ct_status ct_gated_scan_grad(
@@ -763,14 +823,26 @@ ct_status ct_gated_scan_grad(
             return four ? launch(gated_steps_grad_kernel<4, 4>, 4) : launch(gated_steps_grad_kernel<1, 4>, 1);
         return launch(gated_steps_grad_kernel<1, kFewSteps>, 1);
     }
-    // (groups of fewer channels would leave lanes without a chain; a tensor map has 40 bits for a stride)
-    const bool tiles = channels >= 32 && channels % 4 == 0 && aligned16({gate, value, out, dout}) && steps * channels < (int64_t)1 << 37;
-    auto launch      = [&](auto warps) -> ct_status {
+    const Source from = scan_source(batch, steps, channels, aligned16({gate, value, out, dout}));
+    auto launch       = [&](auto warps) -> ct_status {
         constexpr int W = decltype(warps)::value;
-        return tiles ? launch_scan_grad<W, TILES>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0)
-                     : launch_scan_grad<W, SINGLE>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+        switch (from) {
+        case TILES:
+            return launch_scan_grad<W, TILES>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+        case ROWS:
+            return launch_scan_grad<W, ROWS>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+        default:
+            return launch_scan_grad<W, SINGLE>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+        }
     };
-    return scan_is_short(st, batch, steps, channels) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 8>{});
+    switch (scan_warps(st, scan_groups(from, batch, channels), steps)) {
+    case 2:
+        return launch(std::integral_constant<int, 2>{});
+    case 4:
+        return launch(std::integral_constant<int, 4>{});
+    default:
+        return launch(std::integral_constant<int, 8>{});
+    }
 }
 
 } // extern "C"

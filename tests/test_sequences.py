@@ -216,7 +216,8 @@ def scan_grad64(gate, value, state0, lengths, out, dout, dstate):
 
 
 SCAN_SHAPES = [(1, 1, 1), (3, 1, 70), (64, 1, 2048), (2, 2, 5), (2, 5, 33), (3, 17, 40), (1, 129, 32), (4, 300, 40), (1, 2000, 3), (2, 4100, 5), (7, 700, 77),
-               (1, 20000, 31), (70, 17, 100), (1, 1025, 513), (33, 130, 257)]
+               (1, 20000, 31), (70, 17, 100), (1, 1025, 513), (33, 130, 257),
+               (5, 23, 96), (3, 19, 33), (2, 50, 45), (1, 5000, 260), (3, 2500, 1001), (2, 31, 34), (60, 64, 36)]
 
 
 def scan_inputs(b, t, c, seed=0):
