@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(256) embedding_kernel(
 
 // One cluster sorts: each CTA has a range of the tokens, each of its warps a range of that.  A pass over `bits` bits of the ids counts each
 // warp's digits, adds up the counts in the order of warps and CTAs, and puts every token behind those of smaller digits and those before it.
-constexpr int kSortWarps = 32, kSortBits = 10, kSortCtas = 8;
+// ROUNDS: tokens of a lane, which stay in its registers from the count to the end of a pass; 0: any number, read twice.
+constexpr int kSortWarps = 32, kSortBits = 10;
 struct Sorted {
     uint32_t *ids[2], *at[2]; // two places each: a pass goes from one to the other
     uint32_t *counts;         // [0] tokens with an id of the table; [1] rows across slices (of the kernel behind)
@@ -85,8 +86,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr, uint32_t rank)
     return v;
 }
 
+template <int CTAS, int ROUNDS>
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
-    const int64_t *__restrict__ ids, uint32_t m, uint32_t n, int passes, int bits, Sorted s, uint32_t ctas) {
+    const int64_t *__restrict__ ids, uint32_t m, uint32_t n, int passes, int bits, Sorted s) {
     extern __shared__ uint32_t smem[];
     const int bins   = 1 << bits;
     uint32_t *counts = smem;                      // [warp][bin]
@@ -94,12 +96,14 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
     uint32_t *base   = totals + bins + 1;
     __shared__ uint32_t warp_sums[kSortWarps];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const uint32_t rank = cluster_rank();
-    const uint32_t each = ((m + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) & ~31u; // tokens of a warp
+    const uint32_t rank = CTAS > 1 ? cluster_rank() : 0;
+    const uint32_t each = ((m + CTAS * kSortWarps - 1) / (CTAS * kSortWarps) + 31) & ~31u; // tokens of a warp
     const uint64_t lo64 = (uint64_t)(rank * kSortWarps + warp) * each;
     const uint32_t lo = (uint32_t)min(lo64, (uint64_t)m), hi = (uint32_t)min(lo64 + each, (uint64_t)m);
     const uint32_t totals_at = static_cast<uint32_t>(__cvta_generic_to_shared(totals));
+    uint32_t *mine           = counts + warp * bins;
     griddep_wait();
+    griddep_launch_dependents(); // the sums' kernel reads what this one writes from L2
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * bits, from = pass & 1, to = from ^ 1;
         auto id_of      = [&](uint32_t i) -> uint32_t {
@@ -108,39 +112,93 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
             const int64_t id = ids[i];
             return id >= 0 && id < (int64_t)n ? (uint32_t)id : n;
         };
-        for (int i = t; i < kSortWarps * bins; i += kSortWarps * 32)
-            counts[i] = 0;
+        // Counts a round of the warp, and says how many tokens of its digit a lane's has before it.
+        auto count = [&](uint32_t id, bool here) -> uint32_t {
+            // lanes of the same digit, bit by bit (__match_any_sync takes 250 clocks, these 30)
+            const uint32_t d = (id >> shift) & (bins - 1);
+            uint32_t alike   = __ballot_sync(0xffffffffu, here);
+            for (int b = 0; b < bits; ++b) {
+                const uint32_t set = __ballot_sync(0xffffffffu, (d >> b) & 1);
+                alike &= (d >> b) & 1 ? set : ~set;
+            }
+            const uint32_t ahead = __popc(alike & ((1u << lane) - 1));
+            const uint32_t place = here ? mine[d] + ahead : 0;
+            __syncwarp();
+            if (here && ahead == 0)
+                mine[d] += __popc(alike);
+            __syncwarp();
+            return place;
+        };
+        uint32_t id[ROUNDS ? ROUNDS : 1], at[ROUNDS ? ROUNDS : 1], place[ROUNDS ? ROUNDS : 1];
+        if (ROUNDS) {
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r) {
+                const uint32_t i = lo + r * 32 + lane;
+                // (without conditions: each load would wait for the one before)
+                id[r] = id_of(min(i, m - 1)), at[r] = pass ? __ldcg(s.at[from] + min(i, m - 1)) : i;
+            }
+        }
+        for (int i = lane; i < bins; i += 32)
+            mine[i] = 0;
         if (t == 0)
             totals[bins] = 0;
         __syncthreads();
         uint32_t none = 0;
+        if (ROUNDS) {
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r) {
+                const bool here = lo + r * 32 + lane < hi;
+                none += here && id[r] == n;
+                place[r] = count(id[r], here);
+            }
+        } else {
 #pragma unroll 4
-        for (uint32_t i = lo + lane; i < hi; i += 32) {
-            const uint32_t id = id_of(i);
-            none += id == n;
-            atomicAdd(&counts[warp * bins + ((id >> shift) & (bins - 1))], 1u);
+            for (uint32_t i = lo + lane; i < hi; i += 32) {
+                const uint32_t v = id_of(i);
+                none += v == n;
+                atomicAdd(&mine[(v >> shift) & (bins - 1)], 1u);
+            }
         }
-        if (none)
+        none = __reduce_add_sync(0xffffffffu, none);
+        if (none && lane == 0)
             atomicAdd(&totals[bins], none);
         __syncthreads();
         for (int d = t; d < bins; d += kSortWarps * 32) {
-            uint32_t sum = 0;
+            uint32_t sum = 0, c[kSortWarps];
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w)
+                c[w] = counts[w * bins + d];
 #pragma unroll
             for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t c      = counts[w * bins + d];
-                counts[w * bins + d]  = sum;
-                sum                  += c;
+                counts[w * bins + d] = sum;
+                sum += c[w];
             }
             totals[d] = sum;
         }
-        cluster_sync();
+        if (CTAS > 1)
+            cluster_sync();
+        else
+            __syncthreads();
         uint32_t before = 0, all = 0; // of this thread's digit (bins <= threads)
-        if (t < bins)
-            for (uint32_t r = 0; r < ctas; ++r) {
-                const uint32_t c = ld_cluster_u32(totals_at + t * 4, r);
-                before += r < rank ? c : 0;
-                all += c;
+        if (t < bins) {
+            uint32_t c[CTAS];
+#pragma unroll
+            for (int r = 0; r < CTAS; ++r)
+                c[r] = CTAS > 1 ? ld_cluster_u32(totals_at + t * 4, r) : totals[t];
+#pragma unroll
+            for (int r = 0; r < CTAS; ++r) {
+                before += r < (int)rank ? c[r] : 0;
+                all += c[r];
             }
+        }
+        if (pass == 0 && rank == 0 && warp == kSortWarps - 1) {
+            const uint32_t none_of = lane < CTAS ? (CTAS > 1 ? ld_cluster_u32(totals_at + bins * 4, lane) : totals[bins]) : 0;
+            const uint32_t without = __reduce_add_sync(0xffffffffu, none_of);
+            if (lane == 0)
+                s.counts[0] = m - without, s.counts[1] = 0;
+        }
+        if (CTAS > 1)
+            cluster_arrive(); // this CTA has read the others' totals
         uint32_t upto = all; // over digits, this one included
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -149,67 +207,105 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
         }
         if (lane == 31)
             warp_sums[warp] = upto;
-        if (pass == 0 && rank == 0 && t == 0) {
-            uint32_t without = 0;
-            for (uint32_t r = 0; r < ctas; ++r)
-                without += ld_cluster_u32(totals_at + bins * 4, r);
-            s.counts[0] = m - without;
-            s.counts[1] = 0;
-        }
         __syncthreads();
-        uint32_t digits = 0;
-        for (int w = 0; w < warp; ++w)
-            digits += warp_sums[w];
+        const uint32_t digits = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
         if (t < bins)
             base[t] = digits + upto - all + before;
         __syncthreads();
-        for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
-            const uint32_t i  = i0 + lane;
-            const bool here   = i < hi;
-            const uint32_t id = here ? id_of(i) : 0, at = here ? (pass ? __ldcg(s.at[from] + i) : i) : 0;
-            const uint32_t d     = here ? (id >> shift) & (bins - 1) : 0xffffffffu;
-            const uint32_t alike = __match_any_sync(0xffffffffu, d);
-            const uint32_t ahead = __popc(alike & ((1u << lane) - 1));
-            uint32_t *count      = &counts[warp * bins + (here ? d : 0)];
-            const uint32_t place = here ? base[d] + *count + ahead : 0;
-            __syncwarp();
-            if (here && ahead == 0)
-                *count += __popc(alike);
-            __syncwarp();
-            if (here) {
-                s.ids[to][place] = id;
-                s.at[to][place]  = at;
+        auto put = [&](uint32_t id, uint32_t at, uint32_t place) {
+            s.ids[to][place] = id;
+            s.at[to][place]  = at;
+        };
+        if (ROUNDS) {
+#pragma unroll
+            for (int r = 0; r < ROUNDS; ++r) {
+                const uint32_t d = (id[r] >> shift) & (bins - 1);
+                if (lo + r * 32 + lane < hi)
+                    put(id[r], at[r], base[d] + mine[d] + place[r]);
+            }
+            // (mine holds the counts of the warps before: a lane's place is by its own warp's, taken before they were replaced)
+        } else {
+            for (uint32_t i0 = lo; i0 < hi; i0 += 32) {
+                const uint32_t i = i0 + lane;
+                const bool here  = i < hi;
+                const uint32_t v = here ? id_of(i) : 0, a = here && pass ? __ldcg(s.at[from] + i) : i;
+                const uint32_t p = count(v, here); // from the counts of the warps before on
+                if (here)
+                    put(v, a, base[(v >> shift) & (bins - 1)] + p);
             }
         }
-        cluster_sync(); // the next pass reads what the others wrote; their totals have been read
+        if (CTAS > 1) {
+            cluster_wait();
+            if (pass + 1 < passes)
+                cluster_sync(); // the next pass reads what the others wrote
+        } else {
+            __syncthreads();
+        }
     }
 }
 
 // ---- sums ---------------------------------------------------------------------------------------
 
-// How many tokens stand among the first d of the merged list: token i is number i + ids[i] of it.
-__device__ __forceinline__ uint32_t tokens_before(const uint32_t *__restrict__ ids, uint32_t tokens, uint32_t n, uint64_t d, int lane) {
-    uint32_t lo = d > n ? (uint32_t)(d - n) : 0, hi = (uint32_t)min(d, (uint64_t)tokens);
-    while (lo < hi) {
-        const uint32_t step = (hi - lo + 31) / 32, i = lo + lane * step;
-        const bool is_before = i < hi && (uint64_t)i + __ldcg(ids + i) < d;
-        const int before     = __popc(__ballot_sync(0xffffffffu, is_before));
-        if (before == 0)
-            break;
-        hi = min(hi, lo + before * step);
-        lo = lo + (before - 1) * step + 1;
+// Where a slice begins: its first token, and the row that that is in or before.
+struct Begin {
+    uint32_t token, row;
+};
+// Of two slices' beginnings, d[0] and d[1] places behind that of the merged list, in which token i is number i + ids[i].  A row that lies across, but by
+// fewer than about `near` tokens (a multiple of 32, 1024 at most), belongs to the slice before.
+__device__ __forceinline__ void beginnings(
+    const uint32_t *__restrict__ ids, uint32_t tokens, uint32_t n, uint32_t near, const uint64_t (&d)[2], int lane, Begin (&b)[2], bool (&goes_on)[2]) {
+    uint32_t lo[2], hi[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        lo[q] = d[q] > n ? (uint32_t)(d[q] - n) : 0, hi[q] = (uint32_t)min(d[q], (uint64_t)tokens);
+    while (lo[0] < hi[0] || lo[1] < hi[1]) {
+        uint32_t step[2], id[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            step[q]          = (hi[q] - lo[q] + 31) / 32;
+            const uint32_t i = lo[q] + lane * step[q];
+            id[q]            = __ldcg(ids + min(i, tokens - 1)); // (tokens > 0: there is something to look for)
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t i = lo[q] + lane * step[q];
+            const int before = __popc(__ballot_sync(0xffffffffu, i < hi[q] && (uint64_t)i + id[q] < d[q]));
+            if (before == 0)
+                hi[q] = lo[q];
+            else
+                hi[q] = min(hi[q], lo[q] + before * step[q]), lo[q] = lo[q] + (before - 1) * step[q] + 1;
+        }
     }
-    return lo;
+    // the row's tokens from there on, up to `near`: every step-th of them, and those behind the last one that is its
+    const uint32_t step = near / 32;
+    uint32_t last[2], next[2], more[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        last[q] = __ldcg(ids + max(lo[q], 1u) - 1), next[q] = __ldcg(ids + min(lo[q] + lane * step, max(tokens, 1u) - 1));
+        b[q]       = {lo[q], (uint32_t)(d[q] - lo[q])};
+        goes_on[q] = lo[q] > 0 && last[q] == b[q].row && d[q] < (uint64_t)n + tokens; // the row has tokens in slices before
+        hi[q]      = __popc(__ballot_sync(0xffffffffu, lo[q] + lane * step < tokens && next[q] == b[q].row));
+        lo[q] += hi[q] ? (hi[q] - 1) * step + 1 : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        more[q] = __ldcg(ids + min(lo[q] + lane, max(tokens, 1u) - 1));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int beyond = __popc(__ballot_sync(0xffffffffu, lo[q] + lane < tokens && lane < (int)step - 1 && more[q] == b[q].row));
+        if (goes_on[q] && hi[q] < 32)
+            b[q].token = lo[q] + (hi[q] ? beyond : 0), ++b[q].row, goes_on[q] = false;
+    }
 }
 
 enum SliceState : uint8_t { SLICE_THROUGH = 1 }; // all of it belongs to a row that began before and ends behind
 
 // A warp to a slice and 128 V columns.
-template <int V, bool VEC>
-__global__ void __launch_bounds__(256) embedding_grad_kernel(
+template <int V, int AT_ONCE, int FIT, bool VEC>
+__global__ void __launch_bounds__(256, FIT) embedding_grad_kernel(
     const uint32_t *__restrict__ ids, const uint32_t *__restrict__ at, uint32_t *__restrict__ counts, const float *__restrict__ dout, uint32_t n,
     int64_t k, float scale, uint32_t slices, uint32_t strips, float *__restrict__ dtable, double *__restrict__ head, double *__restrict__ tail,
-    uint8_t *__restrict__ states, uint32_t *__restrict__ across) {
+    uint8_t *__restrict__ states, uint2 *__restrict__ across) {
     griddep_wait();
     const int lane       = threadIdx.x & 31;
     const uint64_t unit  = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -219,12 +315,12 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(
     const int64_t c0 = (int64_t)strip * 128 * V;
     auto column      = [&](int j, int q) -> int64_t { return c0 + (VEC ? (j * 32 + lane) * 4 + q : (j * 4 + q) * 32 + lane); };
     const uint32_t tokens = __ldcg(counts);
-    const uint64_t total  = (uint64_t)n + tokens;
-    const uint64_t each   = (total + slices - 1) / slices;
-    const uint64_t d0 = min((uint64_t)slice * each, total), d1 = min(d0 + each, total);
-    const uint32_t i0 = tokens_before(ids, tokens, n, d0, lane), i1 = tokens_before(ids, tokens, n, d1, lane);
-    const uint32_t r0 = (uint32_t)(d0 - i0), r1 = (uint32_t)(d1 - i1);
-    const bool goes_on = d0 < d1 && i0 > 0 && __ldcg(ids + i0 - 1) == r0; // row r0 has tokens in slices before
+    const uint64_t total  = (uint64_t)n + tokens, each = (total + slices - 1) / slices;
+    const uint64_t d[2]   = {min((uint64_t)slice * each, total), min((uint64_t)(slice + 1) * each, total)};
+    Begin bounds[2];
+    bool goes_on[2];
+    beginnings(ids, tokens, n, (uint32_t)min(max(each / 2, (uint64_t)32), (uint64_t)1024) & ~31u, d, lane, bounds, goes_on);
+    const uint32_t i0 = bounds[0].token, i1 = bounds[1].token, r0 = bounds[0].row, r1 = bounds[1].row;
     double sum[4 * V];
 #pragma unroll
     for (int j = 0; j < 4 * V; ++j)
@@ -239,7 +335,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(
                     to[column(j, q)] = sum[4 * j + q];
     };
     auto finish = [&](uint32_t row) {
-        if (row == r0 && goes_on) {
+        if (row == r0 && goes_on[0]) {
             leave(head);
         } else {
             float *to = dtable + (int64_t)row * k;
@@ -262,35 +358,60 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(
         for (int j = 0; j < 4 * V; ++j)
             sum[j] = 0.0;
     };
+    // rows without a token
+    auto clear = [&](uint32_t first, uint32_t last) {
+        float *to = dtable + (int64_t)first * k;
+        for (uint32_t row = first; row < last; ++row, to += k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (VEC) {
+                    if (column(j, 0) < k)
+                        __stcs(reinterpret_cast<float4 *>(to + column(j, 0)), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (column(j, q) < k)
+                            __stcs(to + column(j, q), 0.0f);
+                }
+            }
+    };
     uint32_t row = r0;
-    constexpr int kAtOnce = 4;
+    bool open    = goes_on[0]; // whether the row has tokens
+    auto go_to   = [&](uint32_t next) {
+        if (row < next) {
+            if (open)
+                finish(row);
+            clear(row + open, next);
+            row = next, open = false;
+        }
+    };
+    constexpr int kAtOnce = AT_ONCE;
     for (uint32_t i = i0; i < i1; i += 32) {
-        const uint32_t mine = i + lane < i1 ? __ldcg(ids + i + lane) : 0, mine_at = i + lane < i1 ? __ldcg(at + i + lane) : 0;
+        const uint32_t mine = __ldcg(ids + min(i + lane, i1 - 1)), mine_at = __ldcg(at + min(i + lane, i1 - 1));
         const int count = min(32u, i1 - i);
         for (int g = 0; g < count; g += kAtOnce) {
             float v[kAtOnce][4 * V];
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
-                const float *src = dout + (int64_t)__shfl_sync(0xffffffffu, mine_at, (g + u) & 31) * k;
+                // without conditions, which would make each load wait for the one before: the last token or column again
+                const float *src = dout + (int64_t)__shfl_sync(0xffffffffu, mine_at, min(g + u, count - 1)) * k;
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     if (VEC) {
-                        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (g + u < count && column(j, 0) < k)
-                            f = __ldcs(reinterpret_cast<const float4 *>(src + column(j, 0)));
+                        const float4 f = __ldcs(reinterpret_cast<const float4 *>(src + min(column(j, 0), k - 4)));
                         v[u][4 * j] = f.x, v[u][4 * j + 1] = f.y, v[u][4 * j + 2] = f.z, v[u][4 * j + 3] = f.w;
                     } else {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            v[u][4 * j + q] = g + u < count && column(j, q) < k ? __ldcs(src + column(j, q)) : 0.0f;
+                            v[u][4 * j + q] = __ldcs(src + min(column(j, q), k - 1));
                     }
             }
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const uint32_t id = __shfl_sync(0xffffffffu, mine, (g + u) & 31);
                 if (g + u < count) {
-                    for (; row < id; ++row)
-                        finish(row);
+                    go_to(id);
+                    open = true;
 #pragma unroll
                     for (int j = 0; j < 4 * V; ++j)
                         sum[j] += (double)v[u][j];
@@ -298,36 +419,31 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(
             }
         }
     }
-    for (; row < r1; ++row)
-        finish(row);
-    const bool through = goes_on && r0 == r1;
-    if (through || (i1 > i0 && __ldcg(ids + i1 - 1) == r1)) // row r1 ends in a later slice
+    go_to(r1);
+    const bool through = goes_on[0] && r0 == r1;
+    if (goes_on[1]) // row r1 ends in a later slice
         leave(tail);
     if (strip == 0 && lane == 0) {
         states[slice] = through ? SLICE_THROUGH : 0;
-        if (goes_on && r0 < r1)
-            across[atomicAdd(counts + 1, 1u)] = slice; // in any order: each is a row of its own
+        if (goes_on[0] && r0 < r1)
+            across[atomicAdd(counts + 1, 1u)] = make_uint2(slice, r0); // in any order: each is a row of its own
     }
 }
 
 // The rows that lie across slices: what each slice left of it, the last one's first.  A block has 32 columns of a row, and eight parts of its slices.
 __global__ void __launch_bounds__(256) embedding_join_kernel(
-    const uint32_t *__restrict__ ids, const uint32_t *__restrict__ counts, uint32_t n, int64_t k, float scale, uint32_t slices, uint32_t column_blocks,
-    const double *__restrict__ head, const double *__restrict__ tail, const uint8_t *__restrict__ states, const uint32_t *__restrict__ across,
-    float *__restrict__ dtable) {
+    const uint32_t *__restrict__ counts, int64_t k, float scale, uint32_t column_blocks, const double *__restrict__ head, const double *__restrict__ tail,
+    const uint8_t *__restrict__ states, const uint2 *__restrict__ across, float *__restrict__ dtable) {
     __shared__ double part[8][32];
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t tokens = __ldcg(counts);
-    const uint64_t total = (uint64_t)n + tokens, each = (total + slices - 1) / slices, units = (uint64_t)__ldcg(counts + 1) * column_blocks;
+    const uint64_t units = (uint64_t)__ldcg(counts + 1) * column_blocks;
     for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t slice = __ldcg(across + u / column_blocks);
+        const uint2 last     = __ldcg(across + u / column_blocks); // the slice in which the row ends, and the row
         const int64_t c      = (int64_t)(u % column_blocks) * 32 + lane;
-        const uint64_t d     = (uint64_t)slice * each;
-        const uint32_t row   = (uint32_t)(d - tokens_before(ids, tokens, n, d, lane));
-        uint32_t first       = slice - 1; // the slice in which the row begins, 32 of them looked at together
+        uint32_t first       = last.x - 1; // the slice in which it begins, 32 of them looked at together
         for (;;) {
-            const bool through     = lane <= first && (__ldcg(states + first - lane) & SLICE_THROUGH);
+            const bool through    = lane <= first && (__ldcg(states + first - lane) & SLICE_THROUGH);
             const uint32_t beyond = __ballot_sync(0xffffffffu, !through);
             if (beyond) {
                 first -= __ffs(beyond) - 1;
@@ -336,17 +452,19 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(
             first -= 32;
         }
         double sum = 0.0;
-        if (c < k)
-            for (uint32_t s = first + warp; s < slice; s += 8)
+        if (c < k) {
+#pragma unroll 8
+            for (uint32_t s = first + warp; s < last.x; s += 8)
                 sum += __ldcg(tail + (int64_t)s * k + c);
+        }
         part[warp][lane] = sum;
         __syncthreads();
         if (warp == 0 && c < k) {
-            sum = __ldcg(head + (int64_t)slice * k + c);
+            sum = __ldcg(head + (int64_t)last.x * k + c);
 #pragma unroll
             for (int w = 0; w < 8; ++w)
                 sum += part[w][lane];
-            dtable[(int64_t)row * k + c] = (float)(sum * scale);
+            dtable[(int64_t)last.y * k + c] = (float)(sum * scale);
         }
         __syncthreads();
     }
@@ -415,34 +533,44 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     const bool vec = (k & 3) == 0 && aligned16(dout) && aligned16(dtable);
     const int v    = k <= 128 ? 1 : 2;
     const int64_t strips = (k + 128 * v - 1) / (128 * v);
-    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>((int64_t)st->sm_count * 32 / strips, (n + m + 7) / 8));
+    // Slices: as many as run at once, of 8 items at least; where that is more than 64 items each, four times as many, since their ends come apart
+    // (16384 x 50257 x 2048: 149 us with one for each warp that runs, 125 with four)
+    const int64_t wave = std::max<int64_t>(1, (int64_t)st->sm_count * 16 / strips), items = n + m;
+    const int64_t slices = items < wave * 64 ? std::max<int64_t>(1, std::min(wave, items / 8)) : std::min(wave * 4 + 1, items / 64);
 
     int bits = 1; // of the ids and of n, which stands for none
     while ((n >> bits) > 0)
         ++bits;
     const int passes = (bits + kSortBits - 1) / kSortBits;
     bits             = (bits + passes - 1) / passes;
-    int ctas         = 1;
-    while (ctas < kSortCtas && m > (int64_t)ctas * kSortWarps * 32)
-        ctas *= 2;
 
     auto up              = [](int64_t bytes) { return (bytes + 255) & ~(int64_t)255; };
     const int64_t words  = up(m * 4), partial = up(slices * k * 8);
     Scratch scratch;
-    CT_TRY(scratch.get((size_t)(4 * words + 2 * partial + 256 + up(slices) + up(slices * 4))));
+    CT_TRY(scratch.get((size_t)(4 * words + 2 * partial + 256 + up(slices) + up(slices * 8))));
     Sorted s;
     for (int i = 0; i < 2; ++i)
         s.ids[i] = scratch.as<uint32_t>(2 * i * words), s.at[i] = scratch.as<uint32_t>((2 * i + 1) * words);
     double *head = scratch.as<double>(4 * words), *tail = scratch.as<double>(4 * words + partial);
     s.counts        = scratch.as<uint32_t>(4 * words + 2 * partial);
-    uint32_t *across = scratch.as<uint32_t>(4 * words + 2 * partial + 256);
-    uint8_t *states  = scratch.as<uint8_t>(4 * words + 2 * partial + 256 + up(slices * 4));
+    uint2 *across   = scratch.as<uint2>(4 * words + 2 * partial + 256);
+    uint8_t *states = scratch.as<uint8_t>(4 * words + 2 * partial + 256 + up(slices * 8));
 
-    const size_t smem = ((size_t)(kSortWarps + 2) * (1 << bits) + 1) * 4;
-    CT_CUDA(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ((kSortWarps + 2) * (1 << kSortBits) + 1) * 4));
-    CT_CUDA(launch_dependent_cluster(embedding_sort_kernel, ctas, dim3((unsigned)ctas), dim3(kSortWarps * 32), smem, stream(), ids, (uint32_t)m, (uint32_t)n,
-                                     passes, bits, s, (uint32_t)ctas));
-    CT_LAUNCH_CHECK("embedding_sort");
+    auto sort = [&](auto kernel, int ctas) -> ct_status {
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ((kSortWarps + 2) * (1 << kSortBits) + 1) * 4));
+        CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CT_CUDA(launch_dependent_cluster(kernel, ctas, dim3((unsigned)ctas), dim3(kSortWarps * 32), ((size_t)(kSortWarps + 2) * (1 << bits) + 1) * 4, stream(), ids,
+                                         (uint32_t)m, (uint32_t)n, passes, bits, s));
+        CT_LAUNCH_CHECK("embedding_sort");
+        return CT_OK;
+    };
+    CT_TRY(m <= 1024        ? sort(embedding_sort_kernel<1, 1>, 1)
+           : m <= 8 * 1024  ? sort(embedding_sort_kernel<8, 1>, 8)
+           : m <= 16 * 1024 ? sort(embedding_sort_kernel<16, 1>, 16)
+           : m <= 32 * 1024 ? sort(embedding_sort_kernel<16, 2>, 16)
+           : m <= 64 * 1024 ? sort(embedding_sort_kernel<16, 4>, 16)
+           : m <= 128 * 1024 ? sort(embedding_sort_kernel<16, 8>, 16)
+                             : sort(embedding_sort_kernel<16, 0>, 16));
     const uint32_t *sorted_ids = s.ids[passes & 1], *sorted_at = s.at[passes & 1];
     auto launch = [&](auto kernel) -> ct_status {
         CT_CUDA(launch_dependent(kernel, dim3((unsigned)((slices * strips + 7) / 8)), dim3(256), 0, stream(), sorted_ids, sorted_at, s.counts, dout, (uint32_t)n,
@@ -451,14 +579,13 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
         return CT_OK;
     };
     if (v == 1)
-        CT_TRY(vec ? launch(embedding_grad_kernel<1, true>) : launch(embedding_grad_kernel<1, false>));
+        CT_TRY(vec ? launch(embedding_grad_kernel<1, 8, 3, true>) : launch(embedding_grad_kernel<1, 8, 3, false>));
     else
-        CT_TRY(vec ? launch(embedding_grad_kernel<2, true>) : launch(embedding_grad_kernel<2, false>));
+        CT_TRY(vec ? launch(embedding_grad_kernel<2, 4, 2, true>) : launch(embedding_grad_kernel<2, 4, 2, false>));
     if (slices > 1) {
-        CT_CUDA(launch_dependent(embedding_join_kernel, dim3((unsigned)(2 * st->sm_count)), dim3(256), 0, stream(), sorted_ids,
-                                 static_cast<const uint32_t *>(s.counts), (uint32_t)n, k, (float)scale, (uint32_t)slices, (uint32_t)((k + 31) / 32),
-                                 static_cast<const double *>(head), static_cast<const double *>(tail), static_cast<const uint8_t *>(states),
-                                 static_cast<const uint32_t *>(across), dtable));
+        CT_CUDA(launch_dependent(embedding_join_kernel, dim3((unsigned)(8 * st->sm_count)), dim3(256), 0, stream(), static_cast<const uint32_t *>(s.counts), k,
+                                 (float)scale, (uint32_t)((k + 31) / 32), static_cast<const double *>(head), static_cast<const double *>(tail),
+                                 static_cast<const uint8_t *>(states), static_cast<const uint2 *>(across), dtable));
         CT_LAUNCH_CHECK("embedding_join");
     }
     return CT_OK;
