@@ -69,56 +69,76 @@ template <int TPR> __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 
-// The entries' weights are p[j] = exp(teacher[j] / T - top) / sum.  entry(j, &u): whether entry j has a class, and its teacher logit.
+// The entries' weights are p[j] = exp((teacher[j] - top) / T) / sum.
 struct Weights {
     float top, sum;
     bool some; // whether there is any entry
 };
-template <int TPR, typename F> __device__ __forceinline__ Weights weights_of(int top, float inv_t, int t, F &&entry) {
-    float most = -INFINITY;
-    bool some  = false, bad = false;
-    for (int j = t; j < top; j += TPR) {
-        float u;
-        if (entry(j, u)) {
-            some = true;
-            bad |= u != u;
-            most = fmaxf(most, u);
-        }
-    }
-    most           = max_lanes<TPR>(most);
-    const float base = about(most);
-    float sum      = bad ? NAN : 0.0f;
-    for (int j = t; j < top; j += TPR) {
-        float u;
-        if (entry(j, u))
-            sum = __fadd_rn(sum, expf(__fmul_rn(__fsub_rn(u, base), inv_t)));
-    }
-    const unsigned group = TPR == 32 ? 0xffffffffu : ((1u << (TPR & 31)) - 1) << ((threadIdx.x & 31) / TPR * TPR);
-    return {base, sum_lanes<TPR>(sum), (__ballot_sync(0xffffffffu, some) & group) != 0};
-}
-// T^2 times the sum of p (log p - (z / T - lse)).  entry(j, &u, &z)
-template <int TPR, typename F>
-__device__ __forceinline__ float loss_of(const Weights &w, int top, float temperature, float inv_t, float lse, int t, F &&entry) {
-    const float log_sum = logf(w.sum), inv_sum = __fdiv_rn(1.0f, w.sum);
-    float loss = 0.0f;
-    for (int j = t; j < top; j += TPR) {
-        float u, z;
-        if (entry(j, u, z)) {
-            const float x = __fmul_rn(__fsub_rn(u, w.top), inv_t), p = __fmul_rn(expf(x), inv_sum);
-            if (p != 0.0f) // 0 log 0 is 0
-                loss = __fmaf_rn(p, __fsub_rn(__fsub_rn(x, log_sum), __fsub_rn(__fdiv_rn(z, temperature), lse)), loss);
-        }
-    }
-    loss = __fmul_rn(__fmul_rn(temperature, temperature), sum_lanes<TPR>(loss));
-    return w.some ? loss : 0.0f;
-}
-__device__ __forceinline__ float lse_of(Sum s, float temperature) { return __fadd_rn(__fdiv_rn(about(s.top), temperature), logf(s.sum)); }
-
 __device__ __forceinline__ bool class_of(int64_t id, int64_t n) { return id >= 0 && id < n; }
+__device__ __forceinline__ float lse_of(Sum s, float temperature) { return __fadd_rn(__fdiv_rn(about(s.top), temperature), logf(s.sum)); }
+// p (log p - (z / T - lse)) of an entry, x = (teacher - top) / T
+__device__ __forceinline__ float divergence(float x, const Weights &w, float log_sum, float inv_sum, float z, float temperature, float lse) {
+    const float p = __fmul_rn(expf(x), inv_sum);
+    return p == 0.0f ? 0.0f : __fmul_rn(p, __fsub_rn(__fsub_rn(x, log_sum), __fsub_rn(__fdiv_rn(z, temperature), lse))); // 0 log 0 is 0
+}
+// exp(z / T - lse) of a logit: 1 / T in two parts.  -infinity becomes a number, which neither part makes a NaN.
+__device__ __forceinline__ float probability(float z, float inv_t, float inv_t_rest, float lse) {
+    asm("max.NaN.f32 %0, %0, 0fFF7FFFFF;" : "+f"(z));
+    return ex2(__fmul_rn(__fmaf_rn(z, inv_t, __fmaf_rn(z, inv_t_rest, -lse)), kLog2e));
+}
+
+// A row's entries in the registers of its TPR threads, E each: entry e TPR + t; no class: -1.  All loads are on their way before one is looked at.
+template <int TPR, int E> struct Entries {
+    int id[E];
+    float u[E];
+    __device__ __forceinline__ Entries(const int64_t *__restrict__ ids, const float *__restrict__ teacher, int top, int64_t n, bool here, int t) {
+        int64_t wide[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = max(min(e * TPR + t, top - 1), 0);
+            wide[e]     = here && top > 0 ? ids[j] : -1;
+            u[e]        = here && top > 0 ? teacher[j] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            id[e] = e * TPR + t < top && class_of(wide[e], n) ? (int)wide[e] : -1;
+    }
+    __device__ __forceinline__ Weights weights(float inv_t) const {
+        float most = -INFINITY, sum = 0.0f;
+        bool some = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (id[e] >= 0) {
+                some = true;
+                most = fmaxf(most, u[e]);
+                sum  = u[e] != u[e] ? NAN : sum; // (fmaxf passes over it)
+            }
+        most             = max_lanes<TPR>(most);
+        const float base = about(most);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (id[e] >= 0)
+                sum = __fadd_rn(sum, expf(__fmul_rn(__fsub_rn(u[e], base), inv_t)));
+        const unsigned group = TPR == 32 ? 0xffffffffu : ((1u << (TPR & 31)) - 1) << ((threadIdx.x & 31) / TPR * TPR);
+        return {base, sum_lanes<TPR>(sum), (__ballot_sync(0xffffffffu, some) & group) != 0};
+    }
+};
+
+template <int TPR, int E>
+__device__ __forceinline__ float loss_of(const Entries<TPR, E> &entries, const Weights &w, const float (&z)[E], float temperature, float inv_t, float lse) {
+    const float log_sum = logf(w.sum), inv_sum = __fdiv_rn(1.0f, w.sum);
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (entries.id[e] >= 0)
+            sum = __fadd_rn(sum, divergence(__fmul_rn(__fsub_rn(entries.u[e], w.top), inv_t), w, log_sum, inv_sum, z[e], temperature, lse));
+    sum = __fmul_rn(__fmul_rn(temperature, temperature), sum_lanes<TPR>(sum));
+    return w.some ? sum : 0.0f;
+}
 
 // ---- rows of few classes: TPR threads to a row, V of its logits in each ---------------------------
 
-template <int TPR, int V>
+template <int TPR, int V, int E>
 __global__ void __launch_bounds__(256) distill_short_kernel(
     const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t m, int n, int top, float temperature,
     float inv_t, float *__restrict__ loss, float *__restrict__ lse) {
@@ -129,25 +149,25 @@ __global__ void __launch_bounds__(256) distill_short_kernel(
     const bool here   = row < m; // the others go along
     const float c     = __fmul_rn(inv_t, kLog2e);
     const float *src  = logits + (here ? row * n : 0);
+    const Entries<TPR, E> entries(ids + (here ? row * top : 0), teacher + (here ? row * top : 0), loss ? top : 0, n, here, t);
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        z[i] = here && i * TPR + t < n ? src[i * TPR + t] : -INFINITY;
-    Sum s = {-INFINITY, 0.0f};
+        z[i] = here ? src[min(i * TPR + t, n - 1)] : 0.0f;
+    float at[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        at[e] = entries.id[e] >= 0 ? src[entries.id[e]] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        z[i] = i * TPR + t < n ? z[i] : -INFINITY;
+    const Weights w = entries.weights(inv_t);
+    Sum s           = {-INFINITY, 0.0f};
     take(s, z, c);
     s             = join_lanes<TPR>(s, c);
     const float l = lse_of(s, temperature);
     if (loss) {
-        const int count       = here ? top : 0;
-        const int64_t *row_id = ids + (here ? row * top : 0);
-        const float *row_u    = teacher + (here ? row * top : 0);
-        const Weights w       = weights_of<TPR>(count, inv_t, t, [&](int j, float &u) { return u = row_u[j], class_of(row_id[j], n); });
-        const float value     = loss_of<TPR>(w, count, temperature, inv_t, l, t, [&](int j, float &u, float &zj) {
-            const int64_t id = row_id[j];
-            const bool has   = class_of(id, n);
-            u = row_u[j], zj = has ? src[id] : 0.0f;
-            return has;
-        });
+        const float value = loss_of(entries, w, at, temperature, inv_t, l);
         if (here && t == 0)
             loss[row] = value;
     }
@@ -155,81 +175,228 @@ __global__ void __launch_bounds__(256) distill_short_kernel(
         lse[row] = l;
 }
 
-// exp(z / T - lse) of a logit: 1 / T in two parts.  -infinity becomes a number, which neither part makes a NaN.
-__device__ __forceinline__ float probability(float z, float inv_t, float inv_t_rest, float lse) {
-    asm("max.NaN.f32 %0, %0, 0fFF7FFFFF;" : "+f"(z));
-    return ex2(__fmul_rn(__fmaf_rn(z, inv_t, __fmaf_rn(z, inv_t_rest, -lse)), kLog2e));
-}
-
-// The entries of a row, in shared or global memory: from where the row has been written, each class takes its weights off once.
-template <int TPR, typename F, typename G>
-__device__ __forceinline__ void take_off(const Weights &w, int top, float inv_t, float scale, int t, float *row, int64_t c0, int64_t c1, F &&id_of, G &&u_of) {
-    const float by = __fdiv_rn(scale, w.sum);
-    for (int j = t; j < top; j += TPR) {
-        const int64_t id = id_of(j);
-        if (id < c0 || id >= c1)
-            continue;
-        bool first = true;
-        float p    = 0.0f;
-        for (int i = 0; i < top; ++i)
-            if (id_of(i) == id) { // a class may stand in several entries
-                first &= i >= j;
-                p = __fadd_rn(p, expf(__fmul_rn(__fsub_rn(u_of(i), w.top), inv_t)));
-            }
+// Takes the entries' weights off a row that the TPR threads have written, memory that they share: TPR entries after another, of which the first of a class
+// takes off the weights of all.
+template <int TPR, int E>
+__device__ __forceinline__ void take_off(const Entries<TPR, E> &entries, const Weights &w, float inv_t, float by, int top, int t, float *row) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (e * TPR >= top)
+            break;
+        const float p = expf(__fmul_rn(__fsub_rn(entries.u[e], w.top), inv_t));
+        float total   = 0.0f;
+        bool first    = entries.id[e] >= 0;
+        for (int o = 0; o < min(TPR, top - e * TPR); ++o) {
+            const int id    = __shfl_sync(0xffffffffu, entries.id[e], o, TPR);
+            const float one = __shfl_sync(0xffffffffu, p, o, TPR);
+            if (id == entries.id[e])
+                total = __fadd_rn(total, one), first &= o >= t;
+        }
         if (first)
-            row[id] = __fmaf_rn(-p, by, row[id]);
+            row[entries.id[e]] = __fmaf_rn(-total, by, row[entries.id[e]]);
+        __syncwarp();
     }
 }
 
-template <int TPR, int V>
+// Rows lie in shared memory while their entries' weights are taken off.
+template <int TPR, int V, int E>
 __global__ void __launch_bounds__(256) distill_grad_short_kernel(
     const float *logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, const float *__restrict__ lse,
     const float *__restrict__ dloss, int64_t m, int n, int top, float temperature, float inv_t, float inv_t_rest, float *dlogits) {
+    __shared__ float rows[256 / TPR][TPR * V];
     griddep_wait();
     const int t       = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const bool here   = row < m;
     const float *src  = logits + (here ? row * n : 0);
     float *dst        = dlogits + (here ? row * n : 0);
+    float *mine       = rows[threadIdx.x / TPR];
+    const Entries<TPR, E> entries(ids + (here ? row * top : 0), teacher + (here ? row * top : 0), top, n, here, t);
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        z[i] = here && i * TPR + t < n ? src[i * TPR + t] : 0.0f;
-    const int count       = here ? top : 0;
-    const int64_t *row_id = ids + (here ? row * top : 0);
-    const float *row_u    = teacher + (here ? row * top : 0);
-    const Weights w       = weights_of<TPR>(count, inv_t, t, [&](int j, float &u) { return u = row_u[j], class_of(row_id[j], n); });
-    const float l = here ? lse[row] : 0.0f, scale = here ? __fmul_rn(dloss ? dloss[row] : 1.0f, temperature) : 0.0f;
+        z[i] = here ? src[min(i * TPR + t, n - 1)] : 0.0f;
+    const float l = here ? lse[row] : 0.0f, given = here && dloss ? dloss[row] : 1.0f, scale = __fmul_rn(given, temperature);
+    const Weights w = entries.weights(inv_t);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        mine[i * TPR + t] = w.some ? __fmul_rn(probability(z[i], inv_t, inv_t_rest, l), scale) : 0.0f;
+    __syncwarp();
+    take_off(entries, w, inv_t, __fdiv_rn(scale, w.sum), top, t, mine);
 #pragma unroll
     for (int i = 0; i < V; ++i)
         if (here && i * TPR + t < n)
-            dst[i * TPR + t] = w.some ? __fmul_rn(probability(z[i], inv_t, inv_t_rest, l), scale) : 0.0f;
-    __syncwarp();
-    if (w.some)
-        take_off<TPR>(w, count, inv_t, scale, t, dst, 0, n, [&](int j) { return row_id[j]; }, [&](int j) { return row_u[j]; });
+            dst[i * TPR + t] = mine[i * TPR + t];
 }
 
 // ---- longer rows: a block to a row, or to a part of one -------------------------------------------
 
-// 16-byte pieces of a stretch of floats at any address: `head` values before the first, and `tail` behind the last.
+// 16-byte pieces of a stretch of floats at any address, from a multiple of 128 bytes on: `head` values before the first, and `tail` behind the last.
 struct Stretch {
     int64_t head, pieces, tail;
 };
 __device__ __forceinline__ Stretch stretch_of(const float *p, int64_t count) {
     Stretch s;
-    s.head   = min((int64_t)((4 - ((reinterpret_cast<uintptr_t>(p) >> 2) & 3)) & 3), count);
+    s.head   = min((int64_t)((32 - ((reinterpret_cast<uintptr_t>(p) >> 2) & 31)) & 31), count);
     s.pieces = (count - s.head) / 4;
     s.tail   = count - s.head - 4 * s.pieces;
     return s;
 }
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kAtOnce = 4; // pieces of a thread that are on their way together
+
+// Loads without conditions (with them each would wait for the one before): the last piece again.
+template <int THREADS> __device__ __forceinline__ void load_pieces(float4 (&z)[kAtOnce], const float4 *from, int64_t i, int64_t pieces) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+        z[u] = from[min(i + u * THREADS, pieces - 1)];
+}
+// The sum of a stretch by THREADS threads; z: its first pieces, on their way.
+template <int THREADS>
+__device__ __forceinline__ Sum sum_stretch(const float *src, const Stretch &st, float4 (&f)[kAtOnce], float c, int t) {
+    const float *body = src + st.head;
+    Sum s             = {-INFINITY, 0.0f};
+    for (int i = t; i < st.head + st.tail; i += THREADS) {
+        const float z[1] = {i < st.head ? src[i] : body[4 * st.pieces + i - st.head]};
+        take(s, z, c);
+    }
+    for (int64_t i = t; i < st.pieces;) {
+        float z[4 * kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const bool in = i + u * THREADS < st.pieces;
+            z[4 * u] = in ? f[u].x : -INFINITY, z[4 * u + 1] = in ? f[u].y : -INFINITY;
+            z[4 * u + 2] = in ? f[u].z : -INFINITY, z[4 * u + 3] = in ? f[u].w : -INFINITY;
+        }
+        i += THREADS * kAtOnce;
+        if (i < st.pieces)
+            load_pieces<THREADS>(f, reinterpret_cast<const float4 *>(body), i, st.pieces);
+        take(s, z, c);
+    }
+    return s;
+}
+// f(z) of each logit of a stretch, written to a row that lies as far from 16 bytes (VEC), or at any address.
+template <int THREADS, bool VEC, typename F>
+__device__ __forceinline__ void map_stretch(const float *src, float *dst, int64_t count, const Stretch &st, float4 (&z)[kAtOnce], int t, F &&f) {
+    if (VEC) {
+        for (int q = t; q < st.head + st.tail; q += THREADS) {
+            const int64_t i = q < st.head ? q : st.pieces * 4 + q;
+            dst[i]          = f(src[i]);
+        }
+        const float4 *from = reinterpret_cast<const float4 *>(src + st.head);
+        float4 *to         = reinterpret_cast<float4 *>(dst + st.head);
+        for (int64_t i = t; i < st.pieces;) {
+            float4 d[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                d[u] = make_float4(f(z[u].x), f(z[u].y), f(z[u].z), f(z[u].w));
+            const int64_t now = i;
+            i += THREADS * kAtOnce;
+            if (i < st.pieces)
+                load_pieces<THREADS>(z, from, i, st.pieces);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (now + u * THREADS < st.pieces)
+                    to[now + u * THREADS] = d[u];
+        }
+    } else {
+        for (int64_t i = t; i < count; i += THREADS * kAtOnce) {
+            float v[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                v[u] = src[min(i + u * THREADS, count - 1)];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (i + u * THREADS < count)
+                    dst[i + u * THREADS] = f(v[u]);
+        }
+    }
+}
+
+// Many rows: a warp to each.
+constexpr int kWarpEntries = 128;
+__global__ void __launch_bounds__(kThreads) distill_warp_kernel(
+    const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t m, int64_t n, int top, float temperature,
+    float inv_t, float *__restrict__ loss, float *__restrict__ lse) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane    = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (row >= m)
+        return;
+    const float c    = __fmul_rn(inv_t, kLog2e);
+    const float *src = logits + row * n;
+    const Stretch st = stretch_of(src, n);
+    float4 f[kAtOnce];
+    if (lane < st.pieces)
+        load_pieces<32>(f, reinterpret_cast<const float4 *>(src + st.head), lane, st.pieces);
+    constexpr int E = kWarpEntries / 32;
+    const Entries<32, E> entries(ids + row * top, teacher + row * top, loss ? top : 0, n, true, lane);
+    float at[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        at[e] = entries.id[e] >= 0 ? src[entries.id[e]] : 0.0f;
+    const float l = lse_of(join_lanes<32>(sum_stretch<32>(src, st, f, c, lane), c), temperature);
+    if (loss) {
+        const float value = loss_of(entries, entries.weights(inv_t), at, temperature, inv_t, l);
+        if (lane == 0)
+            loss[row] = value;
+    }
+    if (lse && lane == 0)
+        lse[row] = l;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) distill_grad_warp_kernel(
+    const float *logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, const float *__restrict__ lse,
+    const float *__restrict__ dloss, int64_t m, int64_t n, int top, float temperature, float inv_t, float inv_t_rest, float *dlogits) {
+    griddep_wait();
+    const int lane    = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (row >= m)
+        return;
+    const float *src = logits + row * n;
+    float *dst       = dlogits + row * n;
+    const Stretch st = VEC ? stretch_of(src, n) : Stretch{0, 0, 0};
+    float4 z[kAtOnce];
+    if (lane < st.pieces)
+        load_pieces<32>(z, reinterpret_cast<const float4 *>(src + st.head), lane, st.pieces);
+    const Entries<32, kWarpEntries / 32> entries(ids + row * top, teacher + row * top, top, n, true, lane);
+    const float l = lse[row], scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
+    const Weights w = entries.weights(inv_t);
+    map_stretch<32, VEC>(src, dst, n, st, z, lane, [&](float v) { return w.some ? __fmul_rn(probability(v, inv_t, inv_t_rest, l), scale) : 0.0f; });
+    __syncwarp();
+    if (w.some)
+        take_off(entries, w, inv_t, __fdiv_rn(scale, w.sum), top, lane, dst);
+}
+
+// The entries of a row in shared memory; the sum of weights is left to one warp.
+struct SharedEntries {
+    float u[kMostEntries];
+    int id[kMostEntries]; // no class: -1
+};
+__device__ __forceinline__ Weights weights_of(const SharedEntries &s, int top, float inv_t, int lane) {
+    float most = -INFINITY, sum = 0.0f;
+    bool some = false;
+    for (int j = lane; j < top; j += 32)
+        if (s.id[j] >= 0) {
+            some = true;
+            most = fmaxf(most, s.u[j]);
+            sum  = s.u[j] != s.u[j] ? NAN : sum;
+        }
+    most             = max_lanes<32>(most);
+    const float base = about(most);
+    for (int j = lane; j < top; j += 32)
+        if (s.id[j] >= 0)
+            sum = __fadd_rn(sum, expf(__fmul_rn(__fsub_rn(s.u[j], base), inv_t)));
+    return {base, sum_lanes<32>(sum), __any_sync(0xffffffffu, some) != 0};
+}
 
 __global__ void __launch_bounds__(kThreads) distill_kernel(
     const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t n, int top, float temperature,
     float inv_t, int parts, int64_t part, float *__restrict__ loss, float *__restrict__ lse) {
-    __shared__ float entry_u[kMostEntries], entry_z[kMostEntries];
-    __shared__ bool entry_has[kMostEntries];
+    __shared__ SharedEntries entries;
+    __shared__ float entry_z[kMostEntries];
     __shared__ Sum warps[kThreads / 32], blocks[8];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t rank = parts > 1 ? cluster_rank() : 0;
@@ -240,33 +407,19 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
     const int64_t row = blockIdx.x / parts;
     const float c     = __fmul_rn(inv_t, kLog2e);
     const float *src  = logits + row * n;
+    const int64_t c0 = min(rank * part, n), count = min(part, n - c0);
+    const Stretch st  = stretch_of(src + c0, count);
+    float4 f[kAtOnce];
+    if (t < st.pieces)
+        load_pieces<kThreads>(f, reinterpret_cast<const float4 *>(src + c0 + st.head), t, st.pieces); // on its way while the entries are fetched
     if (rank == 0 && loss)
         for (int j = t; j < top; j += kThreads) {
             const int64_t id = ids[row * top + j];
-            entry_has[j]     = class_of(id, n);
-            entry_u[j]       = teacher[row * top + j];
+            entries.u[j]     = teacher[row * top + j];
+            entries.id[j]    = class_of(id, n) ? (int)id : -1;
             entry_z[j]       = class_of(id, n) ? src[id] : 0.0f;
         }
-    const int64_t c0 = min(rank * part, n), count = min(part, n - c0);
-    const Stretch st = stretch_of(src + c0, count);
-    const float *body = src + c0 + st.head;
-    Sum s = {-INFINITY, 0.0f};
-    if (t < st.head + st.tail) {
-        const float z[1] = {t < st.head ? src[c0 + t] : body[4 * st.pieces + t - st.head]};
-        take(s, z, c);
-    }
-    constexpr int kAtOnce = 4;
-    for (int64_t i = t; i < st.pieces; i += kThreads * kAtOnce) {
-        float z[4 * kAtOnce];
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (i + u * kThreads < st.pieces)
-                f = __ldcs(reinterpret_cast<const float4 *>(body) + i + u * kThreads);
-            z[4 * u] = f.x, z[4 * u + 1] = f.y, z[4 * u + 2] = f.z, z[4 * u + 3] = f.w;
-        }
-        take(s, z, c);
-    }
+    Sum s = sum_stretch<kThreads>(src + c0, st, f, c, t);
     s = join_lanes<32>(s, c);
     if (lane == 0)
         warps[warp] = s;
@@ -289,11 +442,15 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
     if (rank == 0 && warp == 0) {
         const float l = lse_of(s, temperature);
         if (loss) {
-            const Weights w   = weights_of<32>(top, inv_t, lane, [&](int j, float &u) { return u = entry_u[j], entry_has[j]; });
-            const float value = loss_of<32>(w, top, temperature, inv_t, l, lane,
-                                            [&](int j, float &u, float &z) { return u = entry_u[j], z = entry_z[j], entry_has[j]; });
+            const Weights w     = weights_of(entries, top, inv_t, lane);
+            const float log_sum = logf(w.sum), inv_sum = __fdiv_rn(1.0f, w.sum);
+            float sum = 0.0f;
+            for (int j = lane; j < top; j += 32)
+                if (entries.id[j] >= 0)
+                    sum = __fadd_rn(sum, divergence(__fmul_rn(__fsub_rn(entries.u[j], w.top), inv_t), w, log_sum, inv_sum, entry_z[j], temperature, l));
+            sum = __fmul_rn(__fmul_rn(temperature, temperature), sum_lanes<32>(sum));
             if (lane == 0)
-                loss[row] = value;
+                loss[row] = w.some ? sum : 0.0f;
         }
         if (lse && lane == 0)
             lse[row] = l;
@@ -304,59 +461,52 @@ template <bool VEC>
 __global__ void __launch_bounds__(kThreads) distill_grad_kernel(
     const float *logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, const float *__restrict__ lse,
     const float *__restrict__ dloss, int64_t n, int top, float temperature, float inv_t, float inv_t_rest, int parts, int64_t part, float *dlogits) {
-    __shared__ int64_t entry_id[kMostEntries];
-    __shared__ float entry_u[kMostEntries];
+    __shared__ SharedEntries entries;
     griddep_wait();
     const int t       = threadIdx.x;
     const int64_t row = blockIdx.x / parts, c0 = min((int64_t)(blockIdx.x % parts) * part, n), count = min(part, n - c0);
     const float *src  = logits + row * n + c0;
     float *dst        = dlogits + row * n + c0;
-    bool mine         = false;
+    const Stretch st  = VEC ? stretch_of(src, count) : Stretch{0, 0, 0};
+    float4 z[kAtOnce];
+    if (t < st.pieces)
+        load_pieces<kThreads>(z, reinterpret_cast<const float4 *>(src + st.head), t, st.pieces);
+    bool mine = false;
     for (int j = t; j < top; j += kThreads) {
         const int64_t id = ids[row * top + j];
-        entry_id[j]      = class_of(id, n) ? id : -1;
-        entry_u[j]       = teacher[row * top + j];
+        entries.u[j]     = teacher[row * top + j];
+        entries.id[j]    = class_of(id, n) ? (int)id : -1;
         mine |= class_of(id, n);
     }
     const float l = lse[row], scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
     const bool some = __syncthreads_or(mine);
-    auto slope      = [&](float z) { return some ? __fmul_rn(probability(z, inv_t, inv_t_rest, l), scale) : 0.0f; };
-    constexpr int kAtOnce = 4;
-    if (VEC) {
-        const Stretch st = stretch_of(src, count);
-        if (t < st.head + st.tail) {
-            const int64_t i = t < st.head ? t : st.pieces * 4 + t;
-            dst[i]          = slope(src[i]);
-        }
-        const float4 *from = reinterpret_cast<const float4 *>(src + st.head);
-        float4 *to         = reinterpret_cast<float4 *>(dst + st.head);
-        for (int64_t i = t; i < st.pieces; i += kThreads * kAtOnce) {
-            float4 z[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                z[u] = i + u * kThreads < st.pieces ? __ldcs(from + i + u * kThreads) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                if (i + u * kThreads < st.pieces)
-                    __stcs(to + i + u * kThreads, make_float4(slope(z[u].x), slope(z[u].y), slope(z[u].z), slope(z[u].w)));
-        }
-    } else {
-        for (int64_t i = t; i < count; i += kThreads * kAtOnce) {
-            float z[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                z[u] = i + u * kThreads < count ? __ldcs(src + i + u * kThreads) : 0.0f;
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                if (i + u * kThreads < count)
-                    __stcs(dst + i + u * kThreads, slope(z[u]));
-        }
+    map_stretch<kThreads, VEC>(src, dst, count, st, z, t, [&](float v) { return some ? __fmul_rn(probability(v, inv_t, inv_t_rest, l), scale) : 0.0f; });
+    if (!some)
+        return;
+    const Weights w = weights_of(entries, top, inv_t, t & 31);
+    const float by  = __fdiv_rn(scale, w.sum);
+    __syncthreads(); // the row has been written: each class takes its entries' weights off, by the first of them
+    for (int j = t; j < top; j += kThreads) {
+        const int id = entries.id[j];
+        if (id < c0 || id >= c0 + count)
+            continue;
+        bool first = true;
+        float p    = 0.0f;
+        for (int i = 0; i < top; ++i)
+            if (entries.id[i] == id) {
+                first &= i >= j;
+                p = __fadd_rn(p, expf(__fmul_rn(__fsub_rn(entries.u[i], w.top), inv_t)));
+            }
+        if (first)
+            dst[id - c0] = __fmaf_rn(-p, by, dst[id - c0]);
     }
-    __syncthreads();
-    if (some) {
-        const Weights w = weights_of<32>(top, inv_t, t & 31, [&](int j, float &u) { return u = entry_u[j], entry_id[j] >= 0; });
-        take_off<kThreads>(w, top, inv_t, scale, t, dlogits + row * n, c0, c0 + count, [&](int j) { return entry_id[j]; }, [&](int j) { return entry_u[j]; });
-    }
+}
+
+// Whether a warp takes a row, or a block; measured (us, blocks and warps; forward, then backward): 1000 x 600 13 and 9, 12 and 9; 2000 x 1000 16 and 11,
+// 17 and 10; 1000 x 4000 14 and 15, 14 and 17; 4700 x 4000 29 and 23, 37 and 35; 60000 x 1500 250 and 88, 324 and 147; 20000 x 8000 150 and 127, 252 and 261;
+// 20000 x 16000 232 and 239, 447 and 502.
+bool distill_by_warps(const DeviceState *st, int64_t m, int64_t n, int64_t top) {
+    return top <= kWarpEntries && (n <= 1024 || (n <= 6000 && m >= st->sm_count * 16));
 }
 
 ct_status check_distill(const char *name, int64_t m, int64_t n, int64_t top, double temperature) {
@@ -392,15 +542,19 @@ ct_status ct_distill(
         return fail(CT_ERR_INVALID, "distill: null pointer");
     ProfScope prof("distill");
     const float warm = (float)temperature, inv_t = (float)(1.0 / (double)warm);
-    if (n <= 512) {
-        auto launch = [&](auto kernel, int tpr) -> ct_status {
-            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, m, (int)n, (int)top,
-                                     warm, inv_t, loss, lse));
-            CT_LAUNCH_CHECK("distill_short");
-            return CT_OK;
-        };
-        return n <= 32 ? launch(distill_short_kernel<8, 4>, 8) : launch(distill_short_kernel<32, 16>, 32);
-    }
+    auto short_rows = [&](auto kernel, int tpr) -> ct_status {
+        CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, m, n, (int)top, warm, inv_t, loss, lse));
+        CT_LAUNCH_CHECK("distill_short");
+        return CT_OK;
+    };
+    if (n <= 32 && top <= 16)
+        return short_rows(distill_short_kernel<8, 4, 2>, 8);
+    if (n <= 128 && top <= 32)
+        return short_rows(distill_short_kernel<8, 16, 4>, 8);
+    if (n <= 512 && top <= 64)
+        return short_rows(distill_short_kernel<16, 32, 4>, 16);
+    if (distill_by_warps(st, m, n, top))
+        return short_rows(distill_warp_kernel, 32);
     int parts = 1;
     while (parts < 8 && m * parts * 2 <= st->sm_count * 4 && n > (int64_t)parts * kThreads * 16)
         parts *= 2;
@@ -424,15 +578,20 @@ ct_status ct_distill_grad(
         return fail(CT_ERR_INVALID, "distill_grad: null pointer");
     ProfScope prof("distill_grad");
     const float warm = (float)temperature, inv_t = (float)(1.0 / (double)warm), rest = (float)(1.0 / (double)warm - (double)inv_t);
-    if (n <= 512) {
-        auto launch = [&](auto kernel, int tpr) -> ct_status {
-            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, lse, dloss, m,
-                                     (int)n, (int)top, warm, inv_t, rest, dlogits));
-            CT_LAUNCH_CHECK("distill_grad_short");
-            return CT_OK;
-        };
-        return n <= 32 ? launch(distill_grad_short_kernel<8, 4>, 8) : launch(distill_grad_short_kernel<32, 16>, 32);
-    }
+    auto short_rows = [&](auto kernel, int tpr) -> ct_status {
+        CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, lse, dloss, m, n, (int)top, warm, inv_t, rest, dlogits));
+        CT_LAUNCH_CHECK("distill_grad_short");
+        return CT_OK;
+    };
+    if (n <= 32 && top <= 16)
+        return short_rows(distill_grad_short_kernel<8, 4, 2>, 8);
+    if (n <= 128 && top <= 32)
+        return short_rows(distill_grad_short_kernel<8, 16, 4>, 8);
+    if (n <= 512 && top <= 64)
+        return short_rows(distill_grad_short_kernel<16, 32, 4>, 16);
+    const bool alike = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15u) == 0; // 16 bytes of one are 16 of the other
+    if (distill_by_warps(st, m, n, top))
+        return alike ? short_rows(distill_grad_warp_kernel<true>, 32) : short_rows(distill_grad_warp_kernel<false>, 32);
     int parts = 1;
     while (m * parts < st->sm_count * 8 && n > (int64_t)parts * kThreads * 16)
         parts *= 2;
@@ -443,7 +602,6 @@ ct_status ct_distill_grad(
         CT_LAUNCH_CHECK("distill_grad");
         return CT_OK;
     };
-    const bool alike = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15u) == 0;
     return alike ? launch(distill_grad_kernel<true>) : launch(distill_grad_kernel<false>);
 }
 

@@ -398,12 +398,12 @@ __global__ void __launch_bounds__(256, FIT) embedding_grad_kernel(
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     if (VEC) {
-                        const float4 f = __ldcs(reinterpret_cast<const float4 *>(src + min(column(j, 0), k - 4)));
+                        const float4 f = *reinterpret_cast<const float4 *>(src + min(column(j, 0), k - 4));
                         v[u][4 * j] = f.x, v[u][4 * j + 1] = f.y, v[u][4 * j + 2] = f.z, v[u][4 * j + 3] = f.w;
                     } else {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            v[u][4 * j + q] = __ldcs(src + min(column(j, q), k - 1));
+                            v[u][4 * j + q] = src[min(column(j, q), k - 1)];
                     }
             }
 #pragma unroll

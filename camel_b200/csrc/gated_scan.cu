@@ -411,14 +411,14 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
                     h = __fmaf_rn(s.a[j], h, s.add[j]);
-                    __stcs(to + (int64_t)j * channels, h);
+                    to[(int64_t)j * channels] = h;
                 }
             } else if (c.here) {
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
                     h = __fmaf_rn(s.a[j], h, s.add[j]);
                     if (t + j < steps)
-                        __stcs(to + (int64_t)j * channels, j < count ? h : 0.0f);
+                        to[(int64_t)j * channels] = j < count ? h : 0.0f;
                 }
             }
         });
@@ -509,9 +509,9 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
                 if (all || (c.here && t + j >= 0)) {
                     const bool in = all || j < count;
                     if (dvalue)
-                        __stcs(dvalue + at + (int64_t)j * channels, in ? dv : 0.0f);
+                        dvalue[at + (int64_t)j * channels] = in ? dv : 0.0f;
                     if (dgate)
-                        __stcs(dgate + at + (int64_t)j * channels, in ? dg : 0.0f);
+                        dgate[at + (int64_t)j * channels] = in ? dg : 0.0f;
                 }
             }
         });
