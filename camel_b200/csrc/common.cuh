@@ -204,6 +204,13 @@ inline int64_t blocks_for(int64_t turns, int64_t at_once, int64_t chain) {
     return turns < blocks ? turns : blocks;
 }
 
+// Whether no 128-byte line holds values of both: else what a kernel's loads of one bring into a first-level cache of the other is stale for a successor that
+// was launched before them (see launch_dependent).
+inline bool lines_apart(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a) & ~(uintptr_t)127, b0 = reinterpret_cast<uintptr_t>(b) & ~(uintptr_t)127;
+    return !a || !b || reinterpret_cast<uintptr_t>(a) + a_bytes <= b0 || reinterpret_cast<uintptr_t>(b) + b_bytes <= a0;
+}
+
 inline size_t dtype_size(int dt) { return dt == CT_F32 ? 4 : (dt == CT_I64 ? 8 : 1); }
 inline bool valid_dtype(int dt) { return dt == CT_F32 || dt == CT_I64 || dt == CT_BOOL; }
 

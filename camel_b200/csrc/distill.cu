@@ -10,7 +10,7 @@
 #include "tc_ptx.cuh"
 
 #include <algorithm>
-#include <cfloat>
+#include <initializer_list>
 
 namespace ct {
 namespace {
@@ -141,9 +141,10 @@ __device__ __forceinline__ float loss_of(const Entries<TPR, E> &entries, const W
 template <int TPR, int V, int E>
 __global__ void __launch_bounds__(256) distill_short_kernel(
     const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t m, int n, int top, float temperature,
-    float inv_t, float *__restrict__ loss, float *__restrict__ lse) {
+    float inv_t, float *__restrict__ loss, float *__restrict__ lse, int early) {
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int t       = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const bool here   = row < m; // the others go along
@@ -317,9 +318,10 @@ __device__ __forceinline__ void map_stretch(const float *src, float *dst, int64_
 constexpr int kWarpEntries = 128;
 __global__ void __launch_bounds__(kThreads) distill_warp_kernel(
     const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t m, int64_t n, int top, float temperature,
-    float inv_t, float *__restrict__ loss, float *__restrict__ lse) {
+    float inv_t, float *__restrict__ loss, float *__restrict__ lse, int early) {
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int lane    = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     if (row >= m)
@@ -394,7 +396,7 @@ __device__ __forceinline__ Weights weights_of(const SharedEntries &s, int top, f
 
 __global__ void __launch_bounds__(kThreads) distill_kernel(
     const float *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int64_t n, int top, float temperature,
-    float inv_t, int parts, int64_t part, float *__restrict__ loss, float *__restrict__ lse) {
+    float inv_t, int parts, int64_t part, float *__restrict__ loss, float *__restrict__ lse, int early) {
     __shared__ SharedEntries entries;
     __shared__ float entry_z[kMostEntries];
     __shared__ Sum warps[kThreads / 32], blocks[8];
@@ -403,7 +405,8 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
     if (parts > 1)
         cluster_sync(); // every block of the cluster runs before another writes into its memory
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int64_t row = blockIdx.x / parts;
     const float c     = __fmul_rn(inv_t, kLog2e);
     const float *src  = logits + row * n;
@@ -542,11 +545,16 @@ ct_status ct_distill(
         return fail(CT_ERR_INVALID, "distill: null pointer");
     ProfScope prof("distill");
     const float warm = (float)temperature, inv_t = (float)(1.0 / (double)warm);
+    int early        = 1;
+    for (const float *to : {loss, lse})
+        early &= lines_apart(to, m * 4, logits, m * n * 4) && lines_apart(to, m * 4, ids, m * top * 8) && lines_apart(to, m * 4, teacher, m * top * 4);
     auto short_rows = [&](auto kernel, int tpr) -> ct_status {
-        CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, m, n, (int)top, warm, inv_t, loss, lse));
+        CT_CUDA(launch_dependent(kernel, dim3((unsigned)((m + 256 / tpr - 1) / (256 / tpr))), dim3(256), 0, stream(), logits, ids, teacher, m, n, (int)top, warm, inv_t, loss, lse, early));
         CT_LAUNCH_CHECK("distill_short");
         return CT_OK;
     };
+    // (us, 60000 rows; 8 threads with 4 values each, 8 with 16, 16 with 32, a warp; forward, then backward: 10 classes 12, 18, 39, 53, 12, 18, 45, 41; 128 classes
+    // -, 18, 39, 55, -, 25, 47, 45; 512 -, -, 43, 57, -, -, 51, 53)
     if (n <= 32 && top <= 16)
         return short_rows(distill_short_kernel<8, 4, 2>, 8);
     if (n <= 128 && top <= 32)
@@ -556,11 +564,12 @@ ct_status ct_distill(
     if (distill_by_warps(st, m, n, top))
         return short_rows(distill_warp_kernel, 32);
     int parts = 1;
-    while (parts < 8 && m * parts * 2 <= st->sm_count * 4 && n > (int64_t)parts * kThreads * 16)
+    // 131072 classes, 1, 2, 4 and 8 blocks to a row: 31, 19, 14, 10 us (1 row), 33, 22, 17, 16 (64), 37, 28, 25, 28 (148), 47, 40, 44, 47 (300), 70, 71, 76, 76 (600)
+    while (parts < 8 && m * parts * 2 <= st->sm_count * 5 && n > (int64_t)parts * kThreads * 16)
         parts *= 2;
     const int64_t part = ((n + parts - 1) / parts + 3) & ~(int64_t)3;
     CT_CUDA(launch_dependent_cluster(distill_kernel, parts, dim3((unsigned)(m * parts)), dim3(kThreads), 0, stream(), logits, ids, teacher, n, (int)top, warm,
-                                     inv_t, parts, part, loss, lse));
+                                     inv_t, parts, part, loss, lse, early));
     CT_LAUNCH_CHECK("distill");
     return CT_OK;
 }
@@ -592,7 +601,9 @@ ct_status ct_distill_grad(
     const bool alike = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15u) == 0; // 16 bytes of one are 16 of the other
     if (distill_by_warps(st, m, n, top))
         return alike ? short_rows(distill_grad_warp_kernel<true>, 32) : short_rows(distill_grad_warp_kernel<false>, 32);
-    int parts = 1;
+    // Parts of about 16384 classes, or of less where rows are few; measured with 1, 2, 3, 4 and 8: 4096 x 50257 279, 266, 258, 264, 301 us; 4096 x 131072 689, 675,
+    // 677, 659, 641; 1500 x 32003 78, 72, 74, 74, 82; 8000 x 16000 168, 173, 215, 201, 344; 1 x 131072 33 with one, 8 with 16 and 32
+    int parts = (int)std::max<int64_t>(1, (n + 8192) / 16384);
     while (m * parts < st->sm_count * 8 && n > (int64_t)parts * kThreads * 16)
         parts *= 2;
     const int64_t part = ((n + parts - 1) / parts + 3) & ~(int64_t)3;

@@ -28,9 +28,10 @@ constexpr int kLookupValues = 16;
 template <int TPR, bool VEC>
 __global__ void __launch_bounds__(256) embedding_kernel(
     const float *__restrict__ table, const int64_t *__restrict__ ids, int64_t m, int64_t n, int64_t k, int64_t pieces, float scale,
-    float *__restrict__ out) {
+    float *__restrict__ out, int early) {
     griddep_wait();
-    griddep_launch_dependents();
+    if (early)
+        griddep_launch_dependents();
     const int t = threadIdx.x % TPR;
     const int64_t units = m * pieces;
     for (int64_t u = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; u < units; u += (int64_t)gridDim.x * (256 / TPR)) {
@@ -251,7 +252,7 @@ struct Begin {
     uint32_t token, row;
 };
 // Of two slices' beginnings, d[0] and d[1] places behind that of the merged list, in which token i is number i + ids[i].  A row that lies across, but by
-// fewer than about `near` tokens (a multiple of 32, 1024 at most), belongs to the slice before.
+// fewer than about `near` tokens (32 at most, or a multiple of 32), belongs to the slice before.
 __device__ __forceinline__ void beginnings(
     const uint32_t *__restrict__ ids, uint32_t tokens, uint32_t n, uint32_t near, const uint64_t (&d)[2], int lane, Begin (&b)[2], bool (&goes_on)[2]) {
     uint32_t lo[2], hi[2];
@@ -277,14 +278,14 @@ __device__ __forceinline__ void beginnings(
         }
     }
     // the row's tokens from there on, up to `near`: every step-th of them, and those behind the last one that is its
-    const uint32_t step = near / 32;
+    const uint32_t step = max(near / 32, 1u), probes = min(near, 32u);
     uint32_t last[2], next[2], more[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         last[q] = __ldcg(ids + max(lo[q], 1u) - 1), next[q] = __ldcg(ids + min(lo[q] + lane * step, max(tokens, 1u) - 1));
         b[q]       = {lo[q], (uint32_t)(d[q] - lo[q])};
         goes_on[q] = lo[q] > 0 && last[q] == b[q].row && d[q] < (uint64_t)n + tokens; // the row has tokens in slices before
-        hi[q]      = __popc(__ballot_sync(0xffffffffu, lo[q] + lane * step < tokens && next[q] == b[q].row));
+        hi[q]      = __popc(__ballot_sync(0xffffffffu, lane < probes && lo[q] + lane * step < tokens && next[q] == b[q].row));
         lo[q] += hi[q] ? (hi[q] - 1) * step + 1 : 0;
     }
 #pragma unroll
@@ -293,7 +294,7 @@ __device__ __forceinline__ void beginnings(
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int beyond = __popc(__ballot_sync(0xffffffffu, lo[q] + lane < tokens && lane < (int)step - 1 && more[q] == b[q].row));
-        if (goes_on[q] && hi[q] < 32)
+        if (goes_on[q] && hi[q] < probes)
             b[q].token = lo[q] + (hi[q] ? beyond : 0), ++b[q].row, goes_on[q] = false;
     }
 }
@@ -317,9 +318,11 @@ __global__ void __launch_bounds__(256, FIT) embedding_grad_kernel(
     const uint32_t tokens = __ldcg(counts);
     const uint64_t total  = (uint64_t)n + tokens, each = (total + slices - 1) / slices;
     const uint64_t d[2]   = {min((uint64_t)slice * each, total), min((uint64_t)(slice + 1) * each, total)};
+    // half a slice, at least 8
+    const uint32_t near = each >= 64 ? (uint32_t)min(each / 2, (uint64_t)1024) & ~31u : max((uint32_t)each / 2, 8u);
     Begin bounds[2];
     bool goes_on[2];
-    beginnings(ids, tokens, n, (uint32_t)min(max(each / 2, (uint64_t)32), (uint64_t)1024) & ~31u, d, lane, bounds, goes_on);
+    beginnings(ids, tokens, n, near, d, lane, bounds, goes_on);
     const uint32_t i0 = bounds[0].token, i1 = bounds[1].token, r0 = bounds[0].row, r1 = bounds[1].row;
     double sum[4 * V];
 #pragma unroll
@@ -500,17 +503,22 @@ ct_status ct_embedding(const float *table, const int64_t *ids, int64_t m, int64_
         return fail(CT_ERR_INVALID, "embedding: null pointer");
     ProfScope prof("embedding");
     const bool vec = (k & 3) == 0 && aligned16(table) && aligned16(out);
-    auto launch    = [&](auto kernel, int tpr) -> ct_status {
+    const int early = lines_apart(out, m * k * 4, table, n * k * 4) && lines_apart(out, m * k * 4, ids, m * 8);
+    auto launch     = [&](auto kernel, int tpr) -> ct_status {
         const int64_t pieces = (k + tpr * kLookupValues - 1) / (tpr * kLookupValues), per_block = 256 / tpr;
         const int64_t blocks = std::min<int64_t>((m * pieces + per_block - 1) / per_block, INT32_MAX);
-        CT_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), table, ids, m, n, k, pieces, (float)scale, out));
+        CT_CUDA(launch_dependent(kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), table, ids, m, n, k, pieces, (float)scale, out, early));
         CT_LAUNCH_CHECK("embedding");
         return CT_OK;
     };
 #define CT_LOOKUP(TPR) return vec ? launch(embedding_kernel<TPR, true>, TPR) : launch(embedding_kernel<TPR, false>, TPR)
-    if (k <= 4 * kLookupValues)
+    // measured (us, 65536 rows of 50000; 4, 8, 16 and 32 threads): 16 columns 8, 10, 12, 18; 64 12, 10, 14, 18; 128 16, 14, 14, 20; 256 23, 21, 21, 23;
+    // 512 37, 35, 35, 33; 2048 125, 117, 121, 117
+    if (k <= 32)
         CT_LOOKUP(4);
-    if (k <= 16 * kLookupValues)
+    if (k <= 128)
+        CT_LOOKUP(8);
+    if (k <= 256)
         CT_LOOKUP(16);
     CT_LOOKUP(32);
 #undef CT_LOOKUP
@@ -531,12 +539,14 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     }
     ProfScope prof("embedding_grad");
     const bool vec = (k & 3) == 0 && aligned16(dout) && aligned16(dtable);
-    const int v    = k <= 128 ? 1 : 2;
+    const int v    = k <= 64 ? 1 : 2; // 16384 x 50000 x 32 33 us by 128 columns, 38 by 256; 64 36 and 39; 128 42 and 40; 256 46 and 44
     const int64_t strips = (k + 128 * v - 1) / (128 * v);
     // Slices: as many as run at once, of 8 items at least; where that is more than 64 items each, four times as many, since their ends come apart
     // (16384 x 50257 x 2048: 149 us with one for each warp that runs, 125 with four)
     const int64_t wave = std::max<int64_t>(1, (int64_t)st->sm_count * 16 / strips), items = n + m;
-    const int64_t slices = items < wave * 64 ? std::max<int64_t>(1, std::min(wave, items / 8)) : std::min(wave * 4 + 1, items / 64);
+    const int64_t slices = wave == 1           ? 1 // of rows so long, whose partial sums would take more memory than they save time
+                           : items < wave * 64 ? std::max<int64_t>(1, std::min(wave, items / 8))
+                                               : std::min(wave * 4 + 1, items / 64);
 
     int bits = 1; // of the ids and of n, which stands for none
     while ((n >> bits) > 0)
@@ -564,7 +574,9 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
         CT_LAUNCH_CHECK("embedding_sort");
         return CT_OK;
     };
+    // (4000 tokens: 4 rounds of one CTA 26 us in all, one of eight 21; 2000: 19 and 20)
     CT_TRY(m <= 1024        ? sort(embedding_sort_kernel<1, 1>, 1)
+           : m <= 2048      ? sort(embedding_sort_kernel<1, 2>, 1)
            : m <= 8 * 1024  ? sort(embedding_sort_kernel<8, 1>, 8)
            : m <= 16 * 1024 ? sort(embedding_sort_kernel<16, 1>, 16)
            : m <= 32 * 1024 ? sort(embedding_sort_kernel<16, 2>, 16)

@@ -68,7 +68,9 @@ def test_embedding(m, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", EMBEDDING_SHAPES + [(5000, 300, 5), (9000, 70000, 24), (40000, 1000, 8), (3000, 1, 40), (100, 1500000, 2), (70000, 131072, 3)])
+@pytest.mark.parametrize("m,n,k", EMBEDDING_SHAPES + [(5000, 300, 5), (9000, 70000, 24), (40000, 1000, 8), (3000, 1, 40), (100, 1500000, 2), (70000, 131072, 3),
+                                                     (1025, 500, 6), (2049, 500, 70), (8193, 60, 4), (17000, 40, 4), (33000, 300, 3), (140000, 2000, 2), (300000, 70, 1),
+                                                     (65, 129, 65), (700, 60, 100), (3000, 200, 60)])
 def test_embedding_grad(m, n, k):
     ids, _, dout = embedding_inputs(m, n, k, 1)
     want, size = embedding_grad64(ids, dout, n, 3.7)
@@ -478,7 +480,8 @@ def distill_grad64(z, ids, p, lse, dloss, temperature):
 
 
 DISTILL_SHAPES = [(1, 1, 1), (3, 2, 1), (5, 10, 5), (40, 10, 3), (9, 32, 32), (7, 33, 4), (70, 130, 20), (6, 512, 64), (6, 513, 64), (5, 2050, 7), (300, 1025, 1),
-                  (2, 32003, 20), (64, 5000, 40), (1, 131072, 64), (3, 50257, 128), (2, 700, 1024), (2, 9, 100), (700, 4099, 9), (1500, 6000, 3)]
+                  (2, 32003, 20), (64, 5000, 40), (1, 131072, 64), (3, 50257, 128), (2, 700, 1024), (2, 9, 100), (700, 4099, 9), (1500, 6000, 3),
+                  (33, 20, 30), (31, 100, 50), (30, 300, 100), (3, 200, 200), (2500, 1500, 20), (2500, 5000, 33), (600, 9000, 40), (3, 25000, 5), (4000, 33, 2)]
 
 
 @gpu
