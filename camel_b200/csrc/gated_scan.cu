@@ -204,7 +204,7 @@ template <int W, bool CLUSTER> __device__ __forceinline__ void walk_end(Exchange
 struct Chain {
     int64_t first; // of its values, at step 0
     int64_t index; // of its state
-    int64_t steps; // that belong to the sequence; none of a chain that is not there
+    int steps;     // that belong to the sequence; none of a chain that is not there
     bool here;
 };
 __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t steps, int64_t channels, const int64_t *__restrict__ lengths) {
@@ -213,15 +213,13 @@ __device__ __forceinline__ Chain chain_of(int64_t index, int64_t chains, int64_t
     c.index         = c.here ? index : 0;
     const int64_t b = c.index / channels;
     c.first         = b * steps * channels + (c.index - b * channels);
-    c.steps         = c.here ? steps : 0;
+    c.steps         = c.here ? (int)steps : 0;
     if (c.here && lengths) {
         const int64_t length = lengths[b];
-        c.steps              = length < 0 ? 0 : (length < steps ? length : steps);
+        c.steps              = length < 0 ? 0 : (int)(length < steps ? length : steps);
     }
     return c;
 }
-
-__device__ __forceinline__ int clamped(int64_t steps) { return (int)max((int64_t)-1, min((int64_t)1 << 20, steps)); }
 
 // How values come into a block's shared memory.
 //   TILES: a group is 32 channels of one sequence; a piece of an array is one box of a tensor map, whose bytes a barrier counts.  (By cp.async, 16 bytes to a
@@ -253,9 +251,11 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
     uint64_t *arrived;
     int *gave_up;
     const Arrays<ARRAYS> *arrays;
-    int64_t first;     // SINGLE: of the chain's values; ROWS: of the sequence's rows
-    int64_t in_groups; // ROWS: rows that are in groups of four, all but the last three at most
+    int64_t first; // SINGLE: of the chain's values
     int channels, c0, batch, lane;
+    int row0, in_fours; // ROWS: the sequence's first row, and how many rows are in groups of four (all but the last three at most)
+    int steps;          // of the sequence, padding among them
+    int skew[4];        // ROWS: how far the group lies from a multiple of four values in the rows 0, 1, 2 and 3 of any piece
 
     __device__ __forceinline__ Pieces(float *all, uint64_t *barriers, int *flag, const Arrays<ARRAYS> &from, int width)
         : memory(all + (threadIdx.x >> 5) * FLOATS), arrived(barriers), gave_up(flag), arrays(&from), channels(width), lane(threadIdx.x & 31) {
@@ -265,20 +265,25 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
         }
         __syncwarp();
     }
-    __device__ __forceinline__ void at(const Chain &c, int64_t group, int64_t chains, int64_t steps) {
+    // t: where one of the warp's pieces begins; the others do a multiple of S, and so of four, steps from there
+    __device__ __forceinline__ void at(const Chain &c, int64_t group, int64_t chains, int64_t all_steps, int t) {
         const int64_t per = (channels + 31) / 32, b = group / per;
-        batch = (int)b, c0 = (int)(group - b * per) * 32;
-        first     = FROM == ROWS ? b * steps : c.first;
-        in_groups = chains / channels * steps & ~(int64_t)3;
-        t_end     = steps;
+        first = c.first, steps = (int)all_steps, batch = (int)b, c0 = (int)(group - b * per) * 32;
+        if (FROM == ROWS) {
+            row0     = batch * steps;
+            in_fours = (int)(chains / channels * all_steps) & ~3;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                skew[q] = (((row0 + t + q) & 3) * channels + c0) & 3;
+        }
     }
     // The piece that begins at step t, which has the chain's steps first_row .. last_row - 1 as rows.
-    __device__ __forceinline__ void fetch(int64_t t, int first_row, int last_row) {
+    __device__ __forceinline__ void fetch(int t, int first_row, int last_row) {
         if (FROM == SINGLE) {
 #pragma unroll
             for (int k = 0; k < ARRAYS; ++k) {
                 const int shift   = SHIFTED && k == ARRAYS - 1;
-                const float *from = arrays->base[k] + first + (t - shift) * channels;
+                const float *from = arrays->base[k] + first + (int64_t)(t - shift) * channels;
 #pragma unroll
                 for (int j = 0; j < S; ++j)
                     if (j >= first_row && j < last_row && (!shift || t + j > 0))
@@ -297,10 +302,10 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
             if (last_row > 0) { // what a box has outside the array is zeros; rows of other sequences are not used
                 const uint32_t to = shared_address(memory + lane * BOX);
                 if (FROM == TILES) {
-                    tma_load_3d(to, &arrays->map[k], bar, c0, (int)t - shift, batch);
+                    tma_load_3d(to, &arrays->map[k], bar, c0, t - shift, batch);
                 } else {
-                    const int64_t row = first + t - shift + box;
-                    tma_load_2d(to, &arrays->map[k], bar, ((int)(row & 3) * channels + c0) & ~3, (int)(row >> 2));
+                    const int row = row0 + t - shift + box;
+                    tma_load_2d(to, &arrays->map[k], bar, ((row & 3) * channels + c0) & ~3, row >> 2);
                 }
             }
         }
@@ -313,22 +318,20 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
         __syncwarp();
     }
     // The lane's values in array k of the piece that begins at step t.
-    __device__ __forceinline__ void read(int k, int64_t t, float (&to)[S]) const {
+    __device__ __forceinline__ void read(int k, int t, float (&to)[S]) const {
         const float *from = memory + k * PIECE + lane;
         if (FROM == ROWS) {
-            const int64_t row = first + t - (SHIFTED && k == ARRAYS - 1);
-            int skew[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                skew[q] = (((int)(row + q) & 3) * channels + c0) & 3;
+            constexpr int SHIFT = SHIFTED ? 1 : 0;
+            const bool shift    = SHIFT && k == ARRAYS - 1;
 #pragma unroll
             for (int j = 0; j < S; ++j)
-                to[j] = from[(j & 3) * BOX + j / 4 * ROW + skew[j & 3]];
-            if (row + S > in_groups) { // the array's last rows
+                to[j] = from[(j & 3) * BOX + j / 4 * ROW + skew[shift ? (j + 3) & 3 : j & 3]];
+            const int row = row0 + t - shift;
+            if (row + S > in_fours) { // the array's last rows
 #pragma unroll
                 for (int j = 0; j < S; ++j)
-                    if (row + j >= in_groups && t + j < t_end && c0 + lane < channels)
-                        to[j] = arrays->base[k][(row + j) * channels + c0 + lane];
+                    if (row + j >= in_fours && t + j < steps && c0 + lane < channels)
+                        to[j] = arrays->base[k][(int64_t)(row + j) * channels + c0 + lane];
             }
         } else {
 #pragma unroll
@@ -336,7 +339,6 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
                 to[j] = from[j * ROW];
         }
     }
-    int64_t t_end; // steps of the sequence, padding among them
 };
 
 // W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
@@ -354,13 +356,12 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
-    values.at(c, group, chains, steps);
-    const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = ((int64_t)rank * W + warp) * S;
-    // (of a group's chains one is there, and its sequence is the others': whether anything of a piece is fetched is the same to the warp)
-    const int64_t last = FROM == SINGLE ? c.steps : __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
-    auto fetch         = [&](int i) {
-        const int64_t t = t0 + i * tile;
-        values.fetch(t, 0, clamped(last - t));
+    const int tile = (CLUSTER ? blocks : 1) * W * S, t0 = (rank * W + warp) * S;
+    values.at(c, group, chains, steps, t0);
+    const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
+    auto fetch     = [&](int i) {
+        const int t = t0 + i * tile;
+        values.fetch(t, 0, (FROM == SINGLE ? c.steps : last) - t);
     };
     fetch(0);
     struct Steps {
@@ -369,8 +370,12 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
     const double state = walk<Steps>(
         ex, (int)((steps + tile - 1) / tile), c.here && state0 ? (double)state0[c.index] : 0.0, blocks,
         [&](int i, Steps &s) {
-            const int64_t t = t0 + i * tile;
-            const int count = clamped(c.steps - t);
+            const int t = t0 + i * tile, count = c.steps - t;
+            Piece p;
+            if (t >= last) {
+                fetch(i + 1);
+                return p.joined();
+            }
             values.wait(i);
             values.read(0, t, s.a);
             values.read(1, t, s.add);
@@ -382,7 +387,6 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
             }
             __syncwarp();
             fetch(i + 1);
-            Piece p;
 #pragma unroll
             for (int j0 = 0; j0 < S; j0 += 2 * kPairs) {
                 f32x2 a[kPairs], rest[kPairs];
@@ -403,11 +407,16 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
         [&](int i, const Steps &s, double before) {
             if (!out)
                 return;
-            const int64_t t = t0 + i * tile;
-            const int count = clamped(c.steps - t);
-            float *to       = out + c.first + t * channels;
-            float h         = (float)before;
-            if (__all_sync(0xffffffffu, count >= S)) {
+            const int t = t0 + i * tile, count = c.steps - t;
+            float *to   = out + c.first + (int64_t)t * channels;
+            float h     = (float)before;
+            if (t >= last) {
+                if (c.here)
+#pragma unroll
+                    for (int j = 0; j < S; ++j)
+                        if (t + j < steps)
+                            to[(int64_t)j * channels] = 0.0f;
+            } else if (__all_sync(0xffffffffu, count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
                     h = __fmaf_rn(s.a[j], h, s.add[j]);
@@ -442,15 +451,14 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
-    values.at(c, group, chains, steps);
     const float first = c.here && state0 ? state0[c.index] : 0.0f;
     // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
-    const int64_t tile = (int64_t)(CLUSTER ? blocks : 1) * W * S, t0 = steps - ((int64_t)rank * W + warp + 1) * S;
-    const int64_t last = FROM == SINGLE ? c.steps : __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
-    auto rows_there    = [&](int64_t t) { return t > -S ? clamped(last - t) : 0; };
-    auto fetch         = [&](int i) {
-        const int64_t t = t0 - i * tile;
-        values.fetch(t, clamped(-t), rows_there(t));
+    const int tile = (CLUSTER ? blocks : 1) * W * S, t0 = (int)steps - (int)(rank * W + warp + 1) * S;
+    values.at(c, group, chains, steps, t0);
+    const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
+    auto fetch     = [&](int i) {
+        const int t = t0 - i * tile;
+        values.fetch(t, -t, t > -S ? (FROM == SINGLE ? c.steps : last) - t : 0);
     };
     fetch(0);
     struct Steps {
@@ -459,8 +467,12 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
     const double state = walk<Steps>( // c[t+1]
         ex, (int)((steps + tile - 1) / tile), c.here && dstate ? (double)dstate[c.index] : 0.0, blocks,
         [&](int i, Steps &s) {
-            const int64_t t = t0 - i * tile;
-            const int begin = clamped(-t), count = clamped(c.steps - t); // steps begin .. count - 1 are there
+            const int t = t0 - i * tile, begin = -t, count = c.steps - t; // steps begin .. count - 1 are there
+            Piece p;
+            if (t >= last || t <= -S) {
+                fetch(i + 1);
+                return p.joined();
+            }
             values.wait(i);
             values.read(0, t, s.a);
             values.read(1, t, s.rest);
@@ -477,7 +489,6 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
             }
             __syncwarp();
             fetch(i + 1);
-            Piece p;
 #pragma unroll
             for (int j0 = S - 2 * kPairs; j0 >= 0; j0 -= 2 * kPairs) {
                 f32x2 a[kPairs], rest[kPairs];
@@ -497,21 +508,41 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
             return p.joined();
         },
         [&](int i, const Steps &s, double before) {
-            const int64_t t = t0 - i * tile, at = c.first + t * channels;
-            const int count = clamped(c.steps - t);
-            const bool all  = __all_sync(0xffffffffu, t >= 0 && count >= S);
-            float carry     = (float)before;
+            const int t = t0 - i * tile, count = c.steps - t;
+            const int64_t at = c.first + (int64_t)t * channels;
+            float *dg = dgate + at, *dv = dvalue + at;
+            float carry = (float)before;
+            auto slopes = [&](int j, float &g, float &v) {
+                const float x = __fadd_rn(s.dy[j], carry);
+                carry         = __fmul_rn(s.a[j], x);
+                v             = __fmul_rn(s.rest[j], x);
+                g             = __fmul_rn(__fmul_rn(s.rest[j], carry), s.gap[j]);
+            };
+            if (t >= last) {
+                if (c.here)
 #pragma unroll
-            for (int j = S - 1; j >= 0; --j) {
-                const float x  = __fadd_rn(s.dy[j], carry);
-                carry          = __fmul_rn(s.a[j], x);
-                const float dv = __fmul_rn(s.rest[j], x), dg = __fmul_rn(__fmul_rn(s.rest[j], carry), s.gap[j]);
-                if (all || (c.here && t + j >= 0)) {
-                    const bool in = all || j < count;
-                    if (dvalue)
-                        dvalue[at + (int64_t)j * channels] = in ? dv : 0.0f;
-                    if (dgate)
-                        dgate[at + (int64_t)j * channels] = in ? dg : 0.0f;
+                    for (int j = 0; j < S; ++j)
+                        if (t + j >= 0) {
+                            if (dvalue)
+                                dv[(int64_t)j * channels] = 0.0f;
+                            if (dgate)
+                                dg[(int64_t)j * channels] = 0.0f;
+                        }
+            } else if (dgate && dvalue && __all_sync(0xffffffffu, t >= 0 && count >= S)) {
+#pragma unroll
+                for (int j = S - 1; j >= 0; --j)
+                    slopes(j, dg[(int64_t)j * channels], dv[(int64_t)j * channels]);
+            } else if (c.here && t > -S) {
+#pragma unroll
+                for (int j = S - 1; j >= 0; --j) {
+                    float g, v;
+                    slopes(j, g, v);
+                    if (t + j >= 0) {
+                        if (dvalue)
+                            dv[(int64_t)j * channels] = j < count ? v : 0.0f;
+                        if (dgate)
+                            dg[(int64_t)j * channels] = j < count ? g : 0.0f;
+                    }
                 }
             }
         });
