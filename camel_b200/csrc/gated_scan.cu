@@ -294,20 +294,22 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
             asm volatile("cp.async.commit_group;" ::: "memory");
             return;
         }
-        if (lane < ARRAYS * BOXES) {
-            const uint32_t bar = shared_address(arrived);
-            const int k = lane / BOXES, box = lane % BOXES, shift = SHIFTED && k == ARRAYS - 1;
+        // what a box has outside the array is zeros; rows of other sequences are not used
+        const uint32_t bar = shared_address(arrived), to = shared_address(memory);
+        if (FROM == TILES) {
+            if (lane == 0) { // (by a lane to each array they would be issued one lane after the other)
+                mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * ROW * 4 : 0);
+                if (last_row > 0)
+#pragma unroll
+                    for (int k = 0; k < ARRAYS; ++k)
+                        tma_load_3d(to + k * PIECE * 4, &arrays->map[k], bar, c0, t - (SHIFTED && k == ARRAYS - 1), batch);
+            }
+        } else if (lane < ARRAYS * BOXES) { // 16 of them are issued sooner so than by one lane (7 x 1537 x 771 backward 55 us and 59)
+            const int k = lane / BOXES, row = row0 + t - (SHIFTED && k == ARRAYS - 1) + lane % BOXES;
             if (lane == 0)
                 mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * ROW * 4 : 0);
-            if (last_row > 0) { // what a box has outside the array is zeros; rows of other sequences are not used
-                const uint32_t to = shared_address(memory + lane * BOX);
-                if (FROM == TILES) {
-                    tma_load_3d(to, &arrays->map[k], bar, c0, t - shift, batch);
-                } else {
-                    const int row = row0 + t - shift + box;
-                    tma_load_2d(to, &arrays->map[k], bar, ((row & 3) * channels + c0) & ~3, row >> 2);
-                }
-            }
+            if (last_row > 0)
+                tma_load_2d(to + lane * BOX * 4, &arrays->map[k], bar, ((row & 3) * channels + c0) & ~3, row >> 2);
         }
     }
     __device__ __forceinline__ void wait(int i) {
