@@ -280,17 +280,23 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
     // The piece that begins at step t, which has the chain's steps first_row .. last_row - 1 as rows.
     __device__ __forceinline__ void fetch(int t, int first_row, int last_row) {
         if (FROM == SINGLE) {
+            auto copy_rows = [&](auto all) {
 #pragma unroll
-            for (int k = 0; k < ARRAYS; ++k) {
-                const int shift   = SHIFTED && k == ARRAYS - 1;
-                const float *from = arrays->base[k] + first + (int64_t)(t - shift) * channels;
+                for (int k = 0; k < ARRAYS; ++k) {
+                    const int shift   = SHIFTED && k == ARRAYS - 1;
+                    const float *from = arrays->base[k] + first + (int64_t)(t - shift) * channels;
 #pragma unroll
-                for (int j = 0; j < S; ++j)
-                    if (j >= first_row && j < last_row && (!shift || t + j > 0))
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(memory + k * PIECE + j * 32 + lane)),
-                                     "l"(from + (int64_t)j * channels)
-                                     : "memory");
-            }
+                    for (int j = 0; j < S; ++j)
+                        if (decltype(all)::value || (j >= first_row && j < last_row && (!shift || t + j > 0)))
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(memory + k * PIECE + j * 32 + lane)),
+                                         "l"(from + (int64_t)j * channels)
+                                         : "memory");
+                }
+            };
+            if (__all_sync(0xffffffffu, first_row < 0 && last_row >= S))
+                copy_rows(std::true_type{});
+            else
+                copy_rows(std::false_type{});
             asm volatile("cp.async.commit_group;" ::: "memory");
             return;
         }
@@ -345,7 +351,7 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
 
 // W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
 template <int W, int S, Source FROM, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated_scan_kernel(
+__global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     const __grid_constant__ Arrays<2> arrays, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int64_t steps, int channels, int blocks,
     float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
     const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
     auto fetch     = [&](int i) {
         const int t = t0 + i * tile;
-        values.fetch(t, 0, (FROM == SINGLE ? c.steps : last) - t);
+        values.fetch(t, -1, (FROM == SINGLE ? c.steps : last) - t);
     };
     fetch(0);
     struct Steps {
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
 template <int W, int S, Source FROM, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, FROM != SINGLE ? 16 / W : 8 / W) gated_scan_grad_kernel(
+__global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     const __grid_constant__ Arrays<4> arrays, const float *state0, const int64_t *__restrict__ lengths, const float *dstate, int64_t chains, int64_t steps,
     int channels, int blocks, float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
