@@ -86,16 +86,19 @@ constexpr int kPairs = 4; // together
 
 template <int W> constexpr int kMostBlocks = W == 8 ? 15 : 8; // of a cluster; their places are shared memory that other blocks cannot have
 
-// How the pieces of a tile meet.  A block's pieces lie in the order of its warps; what they do together goes to the other blocks of the cluster by
-// st.async, whose arrival a barrier counts (a cluster-wide barrier would wait until the last tile's stores to global memory are done).  Meanwhile the block
-// goes on with the next tile, so that a block may be three tiles behind another: there are four places for what blocks send, and two for pieces.
+// How the pieces of a tile meet.  Without a cluster every warp goes through the pieces of all.  In a cluster a warp of its own does, the joining one: it sends what
+// the block's pieces do together to the other blocks by st.async, whose arrival a barrier counts (a cluster-wide barrier would wait until the last tile's stores to
+// global memory are done), and hands each warp the state before its steps.  Meanwhile the warps work out the next tile's pieces: the state comes a tile late.
+// A warp has the state of tile i - 1 when it leaves the piece of tile i + 1, so there are two places for pieces and states; a block may send tile j while another
+// reads what came of tile j - 2, and four places for that.
 template <int W, bool CLUSTER> struct Exchange {
     double2 pieces[2][W][32]; // (a, b)
     int gave_up;              // a wait has run out: it is reported at the end, and until then the block goes on, for the others' sake
 };
 template <int W> struct Exchange<W, true> : Exchange<W, false> {
-    double2 blocks[4][kMostBlocks<W>][32];
-    uint64_t arrived[4];
+    float before[2][W][32];
+    double2 blocks[4][kMostBlocks<W + 1>][32];
+    uint64_t published[2], ready[2], arrived[4];
 };
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void send(uint32_t at, uint32_t barrier, double2 p) {
@@ -119,53 +122,70 @@ __device__ __forceinline__ double walk(Exchange<W, false> &e, int tiles, double 
             const double2 p = e.pieces[i & 1][w][lane];
             state           = fma(p.x, state, p.y);
         }
-        second(i, s, before);
+        second(i, s, (float)before);
     }
     return state;
+}
+template <int W> __device__ __forceinline__ void wait_for(Exchange<W, true> &e, const uint64_t &barrier, int phase, bool of_cluster = false) {
+    if (*(volatile int *)&e.gave_up)
+        return;
+    if (of_cluster)
+        mbar_wait<kClusterWritten>(shared_address(&barrier), phase & 1, &e.gave_up);
+    else
+        mbar_wait(shared_address(&barrier), phase & 1, &e.gave_up);
 }
 template <typename Steps, int W, typename First, typename Second>
 __device__ __forceinline__ double walk(Exchange<W, true> &e, int tiles, double state, int blocks, First &&first, Second &&second) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t rank = cluster_rank();
-    double a = 1.0, b = 0.0; // what the warps before this one do in the tile before
+    if (warp == W) {
+        const int rank = (int)cluster_rank();
+        for (int i = 0; i < tiles; ++i) {
+            wait_for(e, e.published[i & 1], i >> 1);
+            double2 p[W], all = make_double2(1.0, 0.0);
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                p[w] = e.pieces[i & 1][w][lane];
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                all = make_double2(all.x * p[w].x, fma(p[w].x, all.y, p[w].y));
+            const uint32_t at = shared_address(&e.blocks[i & 3][rank][lane]), bar = shared_address(&e.arrived[i & 3]);
+            if (lane == 0)
+                mbar_expect_tx(bar, blocks * 512);
+            for (int r = 0; r < blocks; ++r)
+                send(mapa(at, r), mapa(bar, r), all);
+            wait_for(e, e.arrived[i & 3], i >> 2, true);
+            auto pass = [&](int r) {
+                const double2 q = e.blocks[i & 3][r][lane];
+                state           = fma(q.x, state, q.y);
+            };
+            for (int r = 0; r < rank; ++r)
+                pass(r);
+            double before = state;
+            for (int r = rank; r < blocks; ++r)
+                pass(r);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                e.before[i & 1][w][lane] = (float)before;
+                before                   = fma(p[w].x, before, p[w].y);
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(shared_address(&e.ready[i & 1]));
+        }
+        return state;
+    }
     auto turn = [&](int i, Steps &now, Steps &past) {
-        double next_a = 1.0, next_b = 0.0;
         if (i < tiles) {
             e.pieces[i & 1][warp][lane] = first(i, now);
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < W - 1; ++w)
-                if (w < warp) {
-                    const double2 p = e.pieces[i & 1][w][lane];
-                    next_b          = fma(p.x, next_b, p.y);
-                    next_a *= p.x;
-                }
-            if (warp == W - 1) {
-                const double2 p    = e.pieces[i & 1][warp][lane];
-                const uint32_t at  = shared_address(&e.blocks[i & 3][rank][lane]);
-                const uint32_t bar = shared_address(&e.arrived[i & 3]);
-                if (lane == 0)
-                    mbar_expect_tx(bar, blocks * 512);
-                for (int r = 0; r < blocks; ++r)
-                    send(mapa(at, r), mapa(bar, r), make_double2(next_a * p.x, fma(p.x, next_b, p.y)));
-            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(shared_address(&e.published[i & 1]));
         }
         if (i > 0) {
             const int j = i - 1;
-            if (!*(volatile int *)&e.gave_up)
-                mbar_wait<kClusterWritten>(shared_address(&e.arrived[j & 3]), (j >> 2) & 1, &e.gave_up);
-            auto pass = [&](int r) {
-                const double2 p = e.blocks[j & 3][r][lane];
-                state           = fma(p.x, state, p.y);
-            };
-            for (int r = 0; r < (int)rank; ++r)
-                pass(r);
-            const double before = state;
-            for (int r = rank; r < blocks; ++r)
-                pass(r);
-            second(j, past, fma(a, before, b));
+            wait_for(e, e.ready[j & 1], j >> 1);
+            second(j, past, e.before[j & 1][warp][lane]);
         }
-        a = next_a, b = next_b;
     };
     Steps even, odd;
     for (int i = 0;; i += 2) {
@@ -184,6 +204,8 @@ template <int W, bool CLUSTER> __device__ __forceinline__ void walk_begin(Exchan
         if constexpr (CLUSTER) {
             for (int i = 0; i < 4; ++i)
                 mbar_init(shared_address(&e.arrived[i]), 1);
+            for (int i = 0; i < 2; ++i)
+                mbar_init(shared_address(&e.published[i]), W), mbar_init(shared_address(&e.ready[i]), 1);
             mbar_fence_init();
         }
     }
@@ -349,13 +371,14 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
     }
 };
 
-// W warps to a block, S steps to a lane; the blocks of a cluster have the same 32 chains.
+// W warps to a block, one of them the joining one in a cluster, S steps to a lane; the blocks of a cluster have the same 32 chains.
 template <int W, int S, Source FROM, bool CLUSTER>
 __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     const __grid_constant__ Arrays<2> arrays, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int64_t steps, int channels, int blocks,
     float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
-    __shared__ Exchange<W, CLUSTER> ex;
+    constexpr int WALK = W - CLUSTER; // warps that have pieces
+    __shared__ Exchange<WALK, CLUSTER> ex;
     __shared__ uint64_t arrived[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
@@ -364,14 +387,15 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
-    const int tile = (CLUSTER ? blocks : 1) * W * S, t0 = (rank * W + warp) * S;
+    const int tile = (CLUSTER ? blocks : 1) * WALK * S, t0 = (rank * WALK + warp) * S;
     values.at(c, group, chains, steps, t0);
     const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
     auto fetch     = [&](int i) {
         const int t = t0 + i * tile;
         values.fetch(t, -1, (FROM == SINGLE ? c.steps : last) - t);
     };
-    fetch(0);
+    if (warp < WALK)
+        fetch(0);
     struct Steps {
         float a[S], add[S];
     };
@@ -412,12 +436,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
             }
             return p.joined();
         },
-        [&](int i, const Steps &s, double before) {
+        [&](int i, const Steps &s, float before) {
             if (!out)
                 return;
             const int t = t0 + i * tile, count = c.steps - t;
             float *to   = out + c.first + (int64_t)t * channels;
-            float h     = (float)before;
+            float h     = before;
             if (t >= last) {
                 if (c.here)
 #pragma unroll
@@ -439,7 +463,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
                 }
             }
         });
-    if (state_out && warp == 0 && rank == 0 && c.here)
+    if (state_out && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here)
         state_out[c.index] = (float)state;
     walk_end(ex, flags);
 }
@@ -450,7 +474,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     const __grid_constant__ Arrays<4> arrays, const float *state0, const int64_t *__restrict__ lengths, const float *dstate, int64_t chains, int64_t steps,
     int channels, int blocks, float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
-    __shared__ Exchange<W, CLUSTER> ex;
+    constexpr int WALK = W - CLUSTER; // warps that have pieces
+    __shared__ Exchange<WALK, CLUSTER> ex;
     __shared__ uint64_t arrived[W];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
@@ -461,14 +486,15 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
     const float first = c.here && state0 ? state0[c.index] : 0.0f;
     // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
-    const int tile = (CLUSTER ? blocks : 1) * W * S, t0 = (int)steps - (int)(rank * W + warp + 1) * S;
+    const int tile = (CLUSTER ? blocks : 1) * WALK * S, t0 = (int)steps - (int)(rank * WALK + warp + 1) * S;
     values.at(c, group, chains, steps, t0);
     const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
     auto fetch     = [&](int i) {
         const int t = t0 - i * tile;
         values.fetch(t, -t, t > -S ? (FROM == SINGLE ? c.steps : last) - t : 0);
     };
-    fetch(0);
+    if (warp < WALK)
+        fetch(0);
     struct Steps {
         float a[S], rest[S], gap[S], dy[S]; // gap: h[t-1] - value[t]
     };
@@ -515,11 +541,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
             }
             return p.joined();
         },
-        [&](int i, const Steps &s, double before) {
+        [&](int i, const Steps &s, float before) {
             const int t = t0 - i * tile, count = c.steps - t;
             const int64_t at = c.first + (int64_t)t * channels;
             float *dg = dgate + at, *dv = dvalue + at;
-            float carry = (float)before;
+            float carry = before;
             auto slopes = [&](int j, float &g, float &v) {
                 const float x = __fadd_rn(s.dy[j], carry);
                 carry         = __fmul_rn(s.a[j], x);
@@ -554,7 +580,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
                 }
             }
         });
-    if (dstate0 && warp == 0 && rank == 0 && c.here)
+    if (dstate0 && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here)
         dstate0[c.index] = (float)state;
     walk_end(ex, flags);
 }
@@ -733,7 +759,7 @@ int64_t scan_groups(Source from, int64_t batch, int64_t channels) {
         constexpr int smem   = (W) * PIECES::FLOATS * 4;                                                                                                   \
         const int64_t groups = scan_groups(FROM, batch, channels);                                                                                       \
         int blocks;                                                                                                                                      \
-        CT_TRY((scan_blocks<KERNEL<W, S, FROM, true>, W>(st, smem, groups, (steps + (W) * (S) - 1) / ((W) * (S)), &blocks)));              \
+        CT_TRY((scan_blocks<KERNEL<W, S, FROM, true>, W>(st, smem, groups, (steps + ((W)-1) * (S)-1) / (((W)-1) * (S)), &blocks)));              \
         auto kernel = blocks > 1 ? KERNEL<W, S, FROM, true> : KERNEL<W, S, FROM, false>;                                                   \
         if (blocks == 1)                                                                                                                                 \
             CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                                    \
@@ -748,10 +774,14 @@ Source scan_source(int64_t batch, int64_t steps, int64_t channels, bool aligned)
         return SINGLE;
     return channels % 4 == 0 ? TILES : ROWS;
 }
-// Warps to a block, measured (us forward, backward; 2, 4 and 8 warps): 16 groups of chains, 65536 steps 195 and 104 (4, 8), 480 and 212; 32 groups, 2048
-// steps 19, 16, 14, 35, 25, 21; 64 groups 23, 19, 18, 39, 29, 31; 175 groups, 1537 steps 39, 37, 41, 72, 62, 76; 512 groups, 2048 steps 80, 72, 74, 156, 135,
-// 140; 16000 groups, 20 steps 45, 81, 156, 64, 76, 162.
-int scan_warps(const DeviceState *st, int64_t groups, int64_t steps) { return steps <= 32 ? 2 : groups * 3 <= st->sm_count ? 8 : 4; }
+// Warps to a block: 8, two such blocks to an SM, where clusters of them fill most of the machine; else 4, four to an SM.  Measured (us forward, backward; 4 and 8
+// warps): 64 groups of chains, 2048 steps 21 and 19, 31 and 29; 128 groups, 4000 steps 47 and 45, 82 and 76; 175 groups, 1537 steps (59 %) 33 and 33, 55 and 64;
+// 192 groups, 2048 steps (65 %) 45 and 39, 76 and 66; 256 groups, 1500 steps 39 and 33, 66 and 57; 320 groups, 1500 steps 47 and 49, 83 and 86; 512 groups,
+// 2048 steps 72 and 74, 134 and 137.  2 for few steps: 16000 groups, 20 steps 45, by 4 81.
+int scan_warps(const DeviceState *st, int64_t groups, int64_t steps) {
+    const int64_t blocks = 2 * st->sm_count;
+    return steps <= 32 ? 2 : blocks / groups * groups * 8 >= blocks * 5 ? 8 : 4;
+}
 
 template <int W, Source FROM>
 ct_status launch_scan(
