@@ -6,7 +6,7 @@
 // Gradient: the tokens are sorted by id (stable, so that sums have one order), then warps walk the tokens and the rows together.  Rows
 // without a token are as many as there are stores of zeros, rows with thousands as many as there are loads, so what is cut into equal slices is
 // the merged list of both: each token, and behind its last token the end of each row.  A row that lies across slices leaves a partial
-// sum in each, which a third kernel adds up.  Sums are kept in 64 bits and rounded once.
+// sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
@@ -473,6 +473,155 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(
     }
 }
 
+// ---- few tokens -----------------------------------------------------------------------------------
+
+// A block to a range of rows and 128 columns.  It looks through all ids for those of its rows, ranks them by row as the sorting kernel does, in shared memory, and adds
+// up: a warp to a row, or all of them, each a part of its tokens, to a row of more than kAloneTokens.
+constexpr int kAloneTokens = 48, kFewRows = 512; // (1537 x 2050 x 771 24 us with 48, 41 with 16, which the rows above it take in turn)
+template <int TOKENS, bool VEC>
+__global__ void __launch_bounds__(256) embedding_grad_few_kernel(
+    const int64_t *__restrict__ ids, const float *__restrict__ dout, int m, int64_t n, int64_t k, int rows, float scale, float *__restrict__ dtable) {
+    constexpr int TURNS = TOKENS / 256, AT_ONCE = 8;
+    __shared__ uint32_t counts[8][kFewRows], begins[kFewRows + 1], warp_sums[8];
+    __shared__ uint16_t order[TOKENS], many[kFewRows];
+    __shared__ double part[8][128];
+    __shared__ int many_count;
+    griddep_wait();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int64_t row0 = (int64_t)blockIdx.x * rows, c0 = (int64_t)blockIdx.y * 128;
+    const int here     = (int)min((int64_t)rows, n - row0);
+    int row[TURNS], rank[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) { // (without conditions: each load would wait for the one before)
+        const uint64_t id = (uint64_t)ids[min((warp * TURNS + i) * 32 + lane, m - 1)] - (uint64_t)row0;
+        row[i]            = (warp * TURNS + i) * 32 + lane < m && id < (uint64_t)here ? (int)id : -1;
+    }
+    for (int r = t; r < rows; r += 256)
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            counts[w][r] = 0;
+    if (t == 0)
+        many_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        uint32_t alike = __ballot_sync(0xffffffffu, row[i] >= 0);
+        if (alike) {
+            for (int b = 0; (rows - 1) >> b; ++b) {
+                const uint32_t set = __ballot_sync(0xffffffffu, (row[i] >> b) & 1);
+                alike &= (row[i] >> b) & 1 ? set : ~set;
+            }
+            const int ahead = __popc(alike & ((1u << lane) - 1));
+            rank[i]         = row[i] >= 0 ? counts[warp][row[i]] + ahead : 0;
+            __syncwarp();
+            if (row[i] >= 0 && ahead == 0)
+                counts[warp][row[i]] += __popc(alike);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    // where each row's tokens begin, and each warp's of it: two rows to a thread
+    uint32_t sum[2], upto;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        sum[q] = 0;
+        if (2 * t + q < rows) {
+            uint32_t c[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                c[w] = counts[w][2 * t + q];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                counts[w][2 * t + q] = sum[q];
+                sum[q] += c[w];
+            }
+        }
+    }
+    upto = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        upto += lane >= o ? v : 0;
+    }
+    if (lane == 31)
+        warp_sums[warp] = upto;
+    __syncthreads();
+    upto += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
+    begins[2 * t + 1] = upto - sum[1], begins[2 * t + 2] = upto;
+    if (t == 0)
+        begins[0] = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        if (sum[q] > kAloneTokens)
+            many[atomicAdd(&many_count, 1)] = (uint16_t)(2 * t + q); // in any order: each is a row of its own
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i)
+        if (row[i] >= 0)
+            order[begins[row[i]] + counts[warp][row[i]] + rank[i]] = (uint16_t)((warp * TURNS + i) * 32 + lane);
+    __syncthreads();
+    auto column = [&](int q) -> int64_t { return c0 + (VEC ? lane * 4 + q : q * 32 + lane); };
+    auto add    = [&](uint32_t first, uint32_t last, double (&to)[4]) {
+        for (uint32_t i = first; i < last; i += AT_ONCE) {
+            float v[AT_ONCE][4];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const float *src = dout + (int64_t)order[min(i + u, last - 1)] * k;
+                if (VEC) {
+                    const float4 f = *reinterpret_cast<const float4 *>(src + min(column(0), k - 4));
+                    v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        v[u][q] = src[min(column(q), k - 1)];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+                if (i + u < last)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        to[q] += (double)v[u][q];
+        }
+    };
+    for (int r = warp; r < here; r += 8) {
+        const uint32_t first = begins[r], last = begins[r + 1];
+        if (last - first > kAloneTokens)
+            continue;
+        double all[4] = {};
+        add(first, last, all);
+        float *to = dtable + (row0 + r) * k;
+        if (VEC) {
+            if (column(0) < k)
+                __stcs(reinterpret_cast<float4 *>(to + column(0)),
+                       make_float4((float)(all[0] * scale), (float)(all[1] * scale), (float)(all[2] * scale), (float)(all[3] * scale)));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (column(q) < k)
+                    __stcs(to + column(q), (float)(all[q] * scale));
+        }
+    }
+    for (int i = 0; i < many_count; ++i) {
+        const int r          = many[i];
+        const uint32_t first = begins[r], count = begins[r + 1] - first;
+        double all[4]        = {};
+        add(first + count * warp / 8, first + count * (warp + 1) / 8, all);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            part[warp][column(q) - c0] = all[q];
+        __syncthreads();
+        if (t < 128 && c0 + t < k) {
+            double whole = 0.0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                whole += part[w][t];
+            dtable[(row0 + r) * k + c0 + t] = (float)(whole * scale);
+        }
+        __syncthreads();
+    }
+}
+
 constexpr int64_t kMostTokens = 1 << 29;
 
 ct_status check_embedding(const char *name, int64_t m, int64_t n, int64_t k, double scale) {
@@ -539,6 +688,25 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     }
     ProfScope prof("embedding_grad");
     const bool vec = (k & 3) == 0 && aligned16(dout) && aligned16(dtable);
+    // In one launch, where that is sooner than sorting, adding up and joining in three (us in line, three launches and one; tokens x rows x columns):
+    // 8 x 131072 x 768 77 and 67, 500 x 50000 x 1000 58 and 47, 1000 x 5000 x 64 18 and 9, 1000 x 50000 x 1000 55 and 51 (behind other work 64 and 70, the
+    // only size with the order turned), 2000 x 10 x 2000 19 and 9, 4000 x 200 x 1000 22 and 18, 4000 x 50000 x 20 23 and 21; beyond the limits
+    // 1537 x 2050 x 771 21 and 24, 3000 x 3000 x 1000 23 and 31, 4000 x 50000 x 1000 57 and 81
+    if ((m <= 1024 || (m <= 4096 && n * k <= 1 << 20)) && k <= 65535 * 128) { // (of a grid's second size there are 65535)
+        const int64_t strips = (k + 127) / 128, blocks = st->sm_count * 12;
+        const int rows       = (int)std::min<int64_t>(kFewRows, (n * strips + blocks - 1) / blocks);
+        auto few             = [&](auto kernel) -> ct_status {
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((n + rows - 1) / rows), (unsigned)strips), dim3(256), 0, stream(), ids, dout, (int)m, n, k, rows,
+                                     (float)scale, dtable));
+            CT_LAUNCH_CHECK("embedding_grad_few");
+            return CT_OK;
+        };
+        if (m <= 1024)
+            return vec ? few(embedding_grad_few_kernel<1024, true>) : few(embedding_grad_few_kernel<1024, false>);
+        if (m <= 2048)
+            return vec ? few(embedding_grad_few_kernel<2048, true>) : few(embedding_grad_few_kernel<2048, false>);
+        return vec ? few(embedding_grad_few_kernel<4096, true>) : few(embedding_grad_few_kernel<4096, false>);
+    }
     const int v    = k <= 64 ? 1 : 2; // 16384 x 50000 x 32 33 us by 128 columns, 38 by 256; 64 36 and 39; 128 42 and 40; 256 46 and 44
     const int64_t strips = (k + 128 * v - 1) / (128 * v);
     // Slices: as many as run at once, of 8 items at least; where that is more than 64 items each, four times as many, since their ends come apart
@@ -575,8 +743,7 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
         return CT_OK;
     };
     // (4000 tokens: 4 rounds of one CTA 26 us in all, one of eight 21; 2000: 19 and 20)
-    CT_TRY(m <= 1024        ? sort(embedding_sort_kernel<1, 1>, 1)
-           : m <= 2048      ? sort(embedding_sort_kernel<1, 2>, 1)
+    CT_TRY(m <= 2048        ? sort(embedding_sort_kernel<1, 2>, 1)
            : m <= 8 * 1024  ? sort(embedding_sort_kernel<8, 1>, 8)
            : m <= 16 * 1024 ? sort(embedding_sort_kernel<16, 1>, 16)
            : m <= 32 * 1024 ? sort(embedding_sort_kernel<16, 2>, 16)

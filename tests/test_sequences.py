@@ -70,7 +70,8 @@ def test_embedding(m, n, k):
 @gpu
 @pytest.mark.parametrize("m,n,k", EMBEDDING_SHAPES + [(5000, 300, 5), (9000, 70000, 24), (40000, 1000, 8), (3000, 1, 40), (100, 1500000, 2), (70000, 131072, 3),
                                                      (1025, 500, 6), (2049, 500, 70), (8193, 60, 4), (17000, 40, 4), (33000, 300, 3), (140000, 2000, 2), (300000, 70, 1),
-                                                     (65, 129, 65), (700, 60, 100), (3000, 200, 60)])
+                                                     (65, 129, 65), (700, 60, 100), (3000, 200, 60), (1024, 700, 1030), (900, 200000, 12), (2048, 512, 512), (4096, 513, 300),
+                                                     (4096, 3, 1000), (1030, 4000, 700), (5, 2, 8388737)])
 def test_embedding_grad(m, n, k):
     ids, _, dout = embedding_inputs(m, n, k, 1)
     want, size = embedding_grad64(ids, dout, n, 3.7)
@@ -80,7 +81,7 @@ def test_embedding_grad(m, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(1, 50, 8), (4000, 50, 8), (20000, 5000, 300), (3000, 4, 2050)])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 8), (4000, 50, 8), (20000, 5000, 300), (3000, 4, 2050), (5000, 4, 2050)])
 @pytest.mark.parametrize("which", ["one", "last", "two", "none", "all", "descending"])
 def test_embedding_grad_of_uneven_tokens(m, n, k, which):
     """All tokens one row (it lies across every slice), two rows by turns, none of the table's, every row as often, in the other order."""
@@ -95,13 +96,14 @@ def test_embedding_grad_of_uneven_tokens(m, n, k, which):
 
 
 @gpu
-def test_embedding_grad_meets_64_bits():
+@pytest.mark.parametrize("m", [3001, 9001])
+def test_embedding_grad_meets_64_bits(m):
     """Terms that cancel: 2^20 and its negative around small ones, which a float32 sum would lose."""
-    m, n, k = 3001, 7, 33
+    n, k = 7, 33
     rng = np.random.default_rng(5)
     dout = rng.normal(0, 1, (m, k)).astype(np.float32)
     dout[::3], dout[1::3] = 2.0 ** 20, -2.0 ** 20
-    dout[3000] = 0.25
+    dout[m - 1] = 0.25
     ids = np.zeros(m, np.int64) + 3
     want, size = embedding_grad64(ids, dout, n, 1.0)
     within(T.embedding_grad(dev(ids), dev(dout), n).numpy(), want, embedding_grad_off(want, size, m), "dtable")
@@ -109,7 +111,7 @@ def test_embedding_grad_meets_64_bits():
 
 @gpu
 @pytest.mark.parametrize("shift", [0, 1, 2, 3])
-@pytest.mark.parametrize("m,n,k", [(9, 20, 7), (70, 33, 64), (300, 40, 260), (40, 9, 771), (5, 300, 2048)])
+@pytest.mark.parametrize("m,n,k", [(9, 20, 7), (70, 33, 64), (300, 40, 260), (40, 9, 771), (5, 300, 2048), (5000, 40, 771), (2000, 2000, 772), (6000, 300, 64)])
 def test_embedding_at_any_address(m, n, k, shift):
     ids, table, dout = embedding_inputs(m, n, k, 2)
     bt, bi, out = Buffer(table.shape, table, shift), Buffer(ids.shape, ids, 1, np.int64), Buffer((m, k), None, (shift * 3) % 4)

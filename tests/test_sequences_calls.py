@@ -20,17 +20,18 @@ def all_operators(seed, m=900, n=300, k=70, b=3, t=200, c=45, classes=1500, top=
     gate, value, state0, lengths, dy, dstate = [dev(a) for a in scan_inputs(b, t, c, seed)]
     z, entries, teacher, dloss = [dev(a) for a in distill_inputs(m, classes, top, seed)]
     small = [dev(a) for a in distill_inputs(m, 40, 5, seed)]
+    more_ids, _, more = [dev(a) for a in embedding_inputs(9 * m, n, 30, seed)]
     step_gate, step_value = [dev(a[:, :1]) for a in scan_inputs(b, t, c, seed)[:2]]
 
     def run():
         out, last = T.gated_scan(gate, value, state0, lengths)
         loss, lse = T.distill(z, entries, teacher, 2.0)
         loss2, lse2 = T.distill(*small[:3], 2.0)
-        return [T.embedding(table, ids, 3.0), T.embedding_grad(ids, dout, n, 3.0), out, last,
+        return [T.embedding(table, ids, 3.0), T.embedding_grad(ids, dout, n, 3.0), T.embedding_grad(more_ids, more, n), out, last,
                 *T.gated_scan_grad(gate, value, out, dy, state0, lengths, dstate), *T.gated_scan(step_gate, step_value, last),
                 loss, lse, T.distill_grad(z, entries, teacher, lse, 2.0, dloss), loss2, lse2, T.distill_grad(*small[:3], lse2, 2.0)]
 
-    return run, (ids, table, dout, gate, value, state0, lengths, dy, dstate, z, entries, teacher, dloss, small, step_gate, step_value)
+    return run, (ids, table, dout, gate, value, state0, lengths, dy, dstate, z, entries, teacher, dloss, small, more_ids, more, step_gate, step_value)
 
 
 def bytes_of(tensors):
@@ -124,7 +125,7 @@ def rewritten(rng, m, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(1, 300, 40), (2, 40, 64), (16, 2000, 512), (300, 77, 33), (700, 3000, 128)])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 40), (2, 40, 64), (16, 2000, 512), (300, 77, 33), (700, 3000, 128), (6000, 700, 24)])
 @pytest.mark.parametrize("name", ["embedding", "embedding_grad", "gated_scan", "gated_scan_in_place", "gated_scan_grad", "distill", "distill_grad",
                                   "distill_grad_in_place"])
 def test_operator_on_rewritten_inputs(name, m, n, k):
@@ -158,7 +159,7 @@ def any_call(rng, buffers, ids):
     at = lambda b, part=0: buffers[b].ptr + part * PART * 4  # noqa: E731
     log = lambda most: max(1, int(round(np.exp(rng.uniform(0, np.log(most))))))  # noqa: E731
     while True:
-        m, n, k, b, t = log(3000), log(3000), log(600), log(20), log(600)
+        m, n, k, b, t = log(20000), log(3000), log(600), log(20), log(600)
         top = log(40)
         if max(m * k, n * k, m * n, b * t * k) <= PART and m * top <= ids.numel:
             break
