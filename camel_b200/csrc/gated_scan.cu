@@ -106,6 +106,13 @@ __device__ __forceinline__ void send(uint32_t at, uint32_t barrier, double2 p) {
                  : "memory");
 }
 
+// After a wait has run out: what is on its way to this block's memory lands before the block ends, or is waited for once more.
+template <WaitFor FOR = kCta> __device__ __forceinline__ void land(const uint64_t &barrier, int phase) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait<FOR>(shared_address(&barrier), phase & 1) && globaltimer_ns() - t0 < kWaitBudgetNs) {
+    }
+}
+
 // Walks the tiles: first(i, steps) takes tile i into `steps`, a lane's registers, and says what they do; second(i, steps, state) goes through them from
 // the state before them.  Returns the state behind all tiles.
 template <typename Steps, int W, typename First, typename Second>
@@ -172,6 +179,9 @@ __device__ __forceinline__ double walk(Exchange<W, true> &e, int tiles, double s
             if (lane == 0)
                 mbar_arrive(shared_address(&e.ready[i & 1]));
         }
+        if (*(volatile int *)&e.gave_up)
+            for (int i = max(tiles - 4, 0); i < tiles; ++i)
+                land<kClusterWritten>(e.arrived[i & 3], i >> 2);
         return state;
     }
     auto turn = [&](int i, Steps &now, Steps &past) {
@@ -340,11 +350,14 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
                 tma_load_2d(to + lane * BOX * 4, &arrays->map[k], bar, ((row & 3) * channels + c0) & ~3, row >> 2);
         }
     }
-    __device__ __forceinline__ void wait(int i) {
+    // When the wait has run out `last` becomes a step before all: the warp fetches nothing more and waits for nothing more.
+    __device__ __forceinline__ void wait(int i, int &last) {
         if (FROM == SINGLE)
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-        else if (!*(volatile int *)gave_up) // (see Exchange)
-            mbar_wait(shared_address(arrived), i & 1, gave_up);
+        else if (!__all_sync(0xffffffffu, mbar_wait(shared_address(arrived), i & 1, gave_up))) {
+            land(*arrived, i);
+            last = -(1 << 30);
+        }
         __syncwarp();
     }
     // The lane's values in array k of the piece that begins at step t.
@@ -389,7 +402,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
     const int tile = (CLUSTER ? blocks : 1) * WALK * S, t0 = (rank * WALK + warp) * S;
     values.at(c, group, chains, steps, t0);
-    const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
+    int last       = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
     auto fetch     = [&](int i) {
         const int t = t0 + i * tile;
         values.fetch(t, -1, (FROM == SINGLE ? c.steps : last) - t);
@@ -408,7 +421,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
                 fetch(i + 1);
                 return p.joined();
             }
-            values.wait(i);
+            values.wait(i, last);
             values.read(0, t, s.a);
             values.read(1, t, s.add);
             if (!__all_sync(0xffffffffu, count >= S)) {
@@ -463,9 +476,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
                 }
             }
         });
-    if (state_out && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here)
-        state_out[c.index] = (float)state;
     walk_end(ex, flags);
+    if (state_out && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here) // (behind the other blocks' loads of state0, which it may be)
+        state_out[c.index] = (float)state;
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     // a piece has S steps in their own order, the walk goes through them backwards; t0: the first piece's first step, which may be below 0
     const int tile = (CLUSTER ? blocks : 1) * WALK * S, t0 = (int)steps - (int)(rank * WALK + warp + 1) * S;
     values.at(c, group, chains, steps, t0);
-    const int last = __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
+    int last       = __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
     auto fetch     = [&](int i) {
         const int t = t0 - i * tile;
         values.fetch(t, -t, t > -S ? (FROM == SINGLE ? c.steps : last) - t : 0);
@@ -507,7 +520,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
                 fetch(i + 1);
                 return p.joined();
             }
-            values.wait(i);
+            values.wait(i, last);
             values.read(0, t, s.a);
             values.read(1, t, s.rest);
             values.read(2, t, s.dy);
@@ -580,9 +593,9 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
                 }
             }
         });
-    if (dstate0 && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here)
-        dstate0[c.index] = (float)state;
     walk_end(ex, flags);
+    if (dstate0 && warp == (CLUSTER ? WALK : 0) && rank == 0 && c.here) // (behind the other blocks' loads of dstate, which it may be)
+        dstate0[c.index] = (float)state;
 }
 
 // A few steps, S at most: a thread goes through those of V chains, all of which are on their way together.
