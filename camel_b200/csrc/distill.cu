@@ -6,6 +6,8 @@
 // Both are bound by memory: the logits are read once (4 bytes each), and on the way back written once (8).  Forward, a thread keeps the
 // maximum of its logits and the sum of exponentials about it, which meet at the end; a row of a small batch is shared by the blocks of a cluster.
 // Backward, lse is given: a row is q times a factor, from which its block takes the entries' p where it has written them.
+// Measured (L2 flushed): 4096 x 131072 with 64 entries 311 to 341 us (2.15 GB, 0.96 to 1.06 of a copy), 64 x 32003 5.6 us; gradient 4096 x 50257 256 to 278 us
+// (1.65 GB, 0.91 to 0.98), 60000 x 10 6.9 us (9 MB: a launch, and the loads one after the other).
 #include "common.cuh"
 #include "tc_ptx.cuh"
 

@@ -7,6 +7,8 @@
 // without a token are as many as there are stores of zeros, rows with thousands as many as there are loads, so what is cut into equal slices is
 // the merged list of both: each token, and behind its last token the end of each row.  A row that lies across slices leaves a partial
 // sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once.
+// Measured (L2 flushed): 32768 rows of 50257 x 2048 59 to 61 us (348 MB, 0.88 to 0.90 of a copy); gradient of 16384 tokens in the same table 111 us (546 MB,
+// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 23 us (three launches), of one token in a small table 5.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
@@ -689,11 +691,12 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     ProfScope prof("embedding_grad");
     const bool vec = (k & 3) == 0 && aligned16(dout) && aligned16(dtable);
     // In one launch, where that is sooner than sorting, adding up and joining in three (us in line, three launches and one; tokens x rows x columns):
-    // 8 x 131072 x 768 77 and 67, 500 x 50000 x 1000 58 and 47, 1000 x 5000 x 64 18 and 9, 1000 x 50000 x 1000 55 and 51 (behind other work 64 and 70, the
-    // only size with the order turned), 2000 x 10 x 2000 19 and 9, 4000 x 200 x 1000 22 and 18, 4000 x 50000 x 20 23 and 21; beyond the limits
-    // 1537 x 2050 x 771 21 and 24, 3000 x 3000 x 1000 23 and 31, 4000 x 50000 x 1000 57 and 81
+    // 8 x 131072 x 768 77 and 63, 500 x 50000 x 1000 58 and 42, 1000 x 5000 x 64 18 and 9, 1000 x 50000 x 1000 55 and 44,
+    // 2000 x 10 x 2000 19 and 9, 4000 x 200 x 1000 22 and 18, 4000 x 50000 x 20 23 and 21; beyond the limits 1537 x 2050 x 771 21 and 24, 3000 x 3000 x 1000 23 and 31, 4000 x 50000 x 1000 57 and 81
     if ((m <= 1024 || (m <= 4096 && n * k <= 1 << 20)) && k <= 65535 * 128) { // (of a grid's second size there are 65535)
-        const int64_t strips = (k + 127) / 128, blocks = st->sm_count * 12;
+        // 12 blocks for each SM, of large tables 36 (us with 12, 24, 36 and 48; 500 x 50000 x 1000 47, 44, 42, 43; 8 x 131072 x 768 67, 64, 63, 62;
+        // 16 x 32003 x 1024 23, 24, 27, 30; 1000 x 20000 x 400 15, 17, 20, 22)
+        const int64_t strips = (k + 127) / 128, blocks = st->sm_count * (n * k > 1 << 25 ? 36 : 12);
         const int rows       = (int)std::min<int64_t>(kFewRows, (n * strips + blocks - 1) / blocks);
         auto few             = [&](auto kernel) -> ct_status {
             CT_CUDA(launch_dependent(kernel, dim3((unsigned)((n + rows - 1) / rows), (unsigned)strips), dim3(256), 0, stream(), ids, dout, (int)m, n, k, rows,

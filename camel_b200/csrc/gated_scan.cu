@@ -13,6 +13,10 @@
 // of its digits, and a state that remembers 1 / (1 - a) steps would add that up.  A lane's steps therefore do to a state h what is a product A and
 // what they add, b, and their 1 - A is summed up by itself, S' = a S + (1 - a).  A is 1 - S in 64 bits, or, from where S has more than 1/2, the
 // product, which is then small and has its digits.  Between pieces states are in 64 bits.
+//
+// Measured (L2 flushed): one sequence of 65536 steps and 512 channels 79 to 86 us forward (403 MB, 0.71 to 0.78 of a copy; a tile waits for what the blocks before
+// send) and 162 backward; 8 of 2048 steps and 2048 channels 64 to 72 and 126 to 137 us (805 MB, 0.90 to 0.98); 7 of up to 1537 steps and 771
+// channels backward 48 to 56 us (166 MB, 0.45 to 0.53: the boxes of odd rows, 16 to a piece, take half of the instructions); one step of 64 x 2048 5 us.
 #include "common.cuh"
 #include "fastmath.cuh"
 #include "gate.cuh"
