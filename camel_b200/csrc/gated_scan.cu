@@ -277,10 +277,12 @@ __device__ __forceinline__ Chain chain_of_lane(
     return chain_of(c < channels ? b * channels + c : chains, chains, steps, channels, lengths);
 }
 
-// A warp's ARRAYS pieces of S rows.  The next tile's are fetched when a tile's have been read, a quarter of a tile's time from its beginning, and arrive
-// meanwhile; a second place for them gained nothing and kept other blocks out (8 x 2048 x 2048 backward 152 us with it, 136 without).
+// A warp's ARRAYS pieces of S rows, in DEPTH places.  Tile i + DEPTH's are fetched when tile i's have been read, a quarter of a tile's time from its beginning,
+// and arrive meanwhile.  Two places are for the blocks of clusters, which do not fill the machine, from whole boxes (us in line with one and with two: 16384 steps of 16, 24 and 32 groups
+// 23 and 23, 31 and 29, 37 and 35, backward 42 and 39, 56 and 53, 70 and 76: there up to as many groups as a sixth of the SMs; blocks of 4 warps, 168
+// groups of 1537 steps 27 and 25, 41 and 36).  Elsewhere the second place keeps other blocks out (8 x 2048 x 2048 backward 136 and 152; 1537 steps of 175 groups by rows 27 and 35).
 // The last array's rows may be those of the step before (SHIFTED).
-template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
+template <int ARRAYS, int S, Source FROM, bool SHIFTED, int DEPTH> struct Pieces {
     static constexpr int BOXES = FROM == ROWS ? 4 : 1, ROW = FROM == ROWS ? 36 : 32; // values of a box's row
     static constexpr int BOX = (S / BOXES * ROW + 31) & ~31, PIECE = BOXES * BOX, FLOATS = ARRAYS * PIECE; // a box begins on 128 bytes
     float *memory;
@@ -294,9 +296,10 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
     int skew[4];        // ROWS: how far the group lies from a multiple of four values in the rows 0, 1, 2 and 3 of any piece
 
     __device__ __forceinline__ Pieces(float *all, uint64_t *barriers, int *flag, const Arrays<ARRAYS> &from, int width)
-        : memory(all + (threadIdx.x >> 5) * FLOATS), arrived(barriers), gave_up(flag), arrays(&from), channels(width), lane(threadIdx.x & 31) {
+        : memory(all + (threadIdx.x >> 5) * FLOATS * DEPTH), arrived(barriers), gave_up(flag), arrays(&from), channels(width), lane(threadIdx.x & 31) {
         if (FROM != SINGLE && lane == 0) {
-            mbar_init(shared_address(arrived), 1);
+            for (int d = 0; d < DEPTH; ++d)
+                mbar_init(shared_address(arrived + d), 1);
             mbar_fence_init();
         }
         __syncwarp();
@@ -313,8 +316,9 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
                 skew[q] = (((row0 + t + q) & 3) * channels + c0) & 3;
         }
     }
-    // The piece that begins at step t, which has the chain's steps first_row .. last_row - 1 as rows.
-    __device__ __forceinline__ void fetch(int t, int first_row, int last_row) {
+    // The warp's piece i, which begins at step t and has the chain's steps first_row .. last_row - 1 as rows.
+    __device__ __forceinline__ void fetch(int i, int t, int first_row, int last_row) {
+        float *place = memory + i % DEPTH * FLOATS;
         if (FROM == SINGLE) {
             auto copy_rows = [&](auto all) {
 #pragma unroll
@@ -324,7 +328,7 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
 #pragma unroll
                     for (int j = 0; j < S; ++j)
                         if (decltype(all)::value || (j >= first_row && j < last_row && (!shift || t + j > 0)))
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(memory + k * PIECE + j * 32 + lane)),
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(place + k * PIECE + j * 32 + lane)),
                                          "l"(from + (int64_t)j * channels)
                                          : "memory");
                 }
@@ -337,7 +341,7 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
             return;
         }
         // what a box has outside the array is zeros; rows of other sequences are not used
-        const uint32_t bar = shared_address(arrived), to = shared_address(memory);
+        const uint32_t bar = shared_address(arrived + i % DEPTH), to = shared_address(place);
         if (FROM == TILES) {
             if (lane == 0) { // (by a lane to each array they would be issued one lane after the other)
                 mbar_expect_tx(bar, last_row > 0 ? ARRAYS * S * ROW * 4 : 0);
@@ -357,16 +361,17 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
     // When the wait has run out `last` becomes a step before all: the warp fetches nothing more and waits for nothing more.
     __device__ __forceinline__ void wait(int i, int &last) {
         if (FROM == SINGLE)
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        else if (!__all_sync(0xffffffffu, mbar_wait(shared_address(arrived), i & 1, gave_up))) {
-            land(*arrived, i);
+            asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+        else if (!__all_sync(0xffffffffu, mbar_wait(shared_address(arrived + i % DEPTH), i / DEPTH & 1, gave_up))) {
+            for (int d = 0; d < DEPTH; ++d)
+                land(arrived[(i + d) % DEPTH], (i + d) / DEPTH);
             last = -(1 << 30);
         }
         __syncwarp();
     }
     // The lane's values in array k of the piece that begins at step t.
-    __device__ __forceinline__ void read(int k, int t, float (&to)[S]) const {
-        const float *from = memory + k * PIECE + lane;
+    __device__ __forceinline__ void read(int i, int k, int t, float (&to)[S]) const {
+        const float *from = memory + i % DEPTH * FLOATS + k * PIECE + lane;
         if (FROM == ROWS) {
             constexpr int SHIFT = SHIFTED ? 1 : 0;
             const bool shift    = SHIFT && k == ARRAYS - 1;
@@ -389,18 +394,18 @@ template <int ARRAYS, int S, Source FROM, bool SHIFTED> struct Pieces {
 };
 
 // W warps to a block, one of them the joining one in a cluster, S steps to a lane; the blocks of a cluster have the same 32 chains.
-template <int W, int S, Source FROM, bool CLUSTER>
+template <int W, int S, Source FROM, bool CLUSTER, int DEPTH>
 __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     const __grid_constant__ Arrays<2> arrays, const float *state0, const int64_t *__restrict__ lengths, int64_t chains, int64_t steps, int channels, int blocks,
     float *__restrict__ out, float *state_out, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
     constexpr int WALK = W - CLUSTER; // warps that have pieces
     __shared__ Exchange<WALK, CLUSTER> ex;
-    __shared__ uint64_t arrived[W];
+    __shared__ uint64_t arrived[W * DEPTH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
     const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
-    Pieces<2, S, FROM, false> values(pieces, &arrived[warp], &ex.gave_up, arrays, channels);
+    Pieces<2, S, FROM, false, DEPTH> values(pieces, &arrived[warp * DEPTH], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
@@ -409,10 +414,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
     int last       = __reduce_max_sync(0xffffffffu, (unsigned)c.steps); // behind it the warp has nothing but zeros to write
     auto fetch     = [&](int i) {
         const int t = t0 + i * tile;
-        values.fetch(t, -1, (FROM == SINGLE ? c.steps : last) - t);
+        values.fetch(i, t, -1, (FROM == SINGLE ? c.steps : last) - t);
     };
     if (warp < WALK)
-        fetch(0);
+        for (int i = 0; i < DEPTH; ++i)
+            fetch(i);
     struct Steps {
         float a[S], add[S];
     };
@@ -422,12 +428,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
             const int t = t0 + i * tile, count = c.steps - t;
             Piece p;
             if (t >= last) {
-                fetch(i + 1);
+                fetch(i + DEPTH);
                 return p.joined();
             }
             values.wait(i, last);
-            values.read(0, t, s.a);
-            values.read(1, t, s.add);
+            values.read(i, 0, t, s.a);
+            values.read(i, 1, t, s.add);
             if (!__all_sync(0xffffffffu, count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j)
@@ -435,7 +441,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
                         s.a[j] = INFINITY, s.add[j] = 0.0f;
             }
             __syncwarp();
-            fetch(i + 1);
+            fetch(i + DEPTH);
 #pragma unroll
             for (int j0 = 0; j0 < S; j0 += 2 * kPairs) {
                 f32x2 a[kPairs], rest[kPairs];
@@ -486,18 +492,18 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_kernel(
 }
 
 // The same along the reversed axis: piece u of a tile ends u S steps before the tile's end.
-template <int W, int S, Source FROM, bool CLUSTER>
+template <int W, int S, Source FROM, bool CLUSTER, int DEPTH>
 __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     const __grid_constant__ Arrays<4> arrays, const float *state0, const int64_t *__restrict__ lengths, const float *dstate, int64_t chains, int64_t steps,
     int channels, int blocks, float *__restrict__ dgate, float *__restrict__ dvalue, float *dstate0, uint32_t *__restrict__ flags) {
     extern __shared__ __align__(128) float pieces[];
     constexpr int WALK = W - CLUSTER; // warps that have pieces
     __shared__ Exchange<WALK, CLUSTER> ex;
-    __shared__ uint64_t arrived[W];
+    __shared__ uint64_t arrived[W * DEPTH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = CLUSTER ? cluster_rank() : 0;
     const int64_t group = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
-    Pieces<4, S, FROM, true> values(pieces, &arrived[warp], &ex.gave_up, arrays, channels);
+    Pieces<4, S, FROM, true, DEPTH> values(pieces, &arrived[warp * DEPTH], &ex.gave_up, arrays, channels);
     walk_begin(ex);
     griddep_wait();
     const Chain c = chain_of_lane<FROM>(group, lane, chains, steps, channels, lengths);
@@ -508,10 +514,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
     int last       = __reduce_max_sync(0xffffffffu, (unsigned)c.steps);
     auto fetch     = [&](int i) {
         const int t = t0 - i * tile;
-        values.fetch(t, -t, t > -S ? (FROM == SINGLE ? c.steps : last) - t : 0);
+        values.fetch(i, t, -t, t > -S ? (FROM == SINGLE ? c.steps : last) - t : 0);
     };
     if (warp < WALK)
-        fetch(0);
+        for (int i = 0; i < DEPTH; ++i)
+            fetch(i);
     struct Steps {
         float a[S], rest[S], gap[S], dy[S]; // gap: h[t-1] - value[t]
     };
@@ -521,14 +528,14 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
             const int t = t0 - i * tile, begin = -t, count = c.steps - t; // steps begin .. count - 1 are there
             Piece p;
             if (t >= last || t <= -S) {
-                fetch(i + 1);
+                fetch(i + DEPTH);
                 return p.joined();
             }
             values.wait(i, last);
-            values.read(0, t, s.a);
-            values.read(1, t, s.rest);
-            values.read(2, t, s.dy);
-            values.read(3, t, s.gap);
+            values.read(i, 0, t, s.a);
+            values.read(i, 1, t, s.rest);
+            values.read(i, 2, t, s.dy);
+            values.read(i, 3, t, s.gap);
             if (!__all_sync(0xffffffffu, t > 0 && count >= S)) {
 #pragma unroll
                 for (int j = 0; j < S; ++j) {
@@ -539,7 +546,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) gated_scan_grad_kernel(
                 }
             }
             __syncwarp();
-            fetch(i + 1);
+            fetch(i + DEPTH);
 #pragma unroll
             for (int j0 = S - 2 * kPairs; j0 >= 0; j0 -= 2 * kPairs) {
                 f32x2 a[kPairs], rest[kPairs];
@@ -771,16 +778,16 @@ int64_t scan_groups(Source from, int64_t batch, int64_t channels) {
     return from == SINGLE ? (batch * channels + 31) / 32 : batch * ((channels + 31) / 32);
 }
 
-#define CT_SCAN(NAME, KERNEL, W, S, FROM, PIECES, ...)                                                                                              \
+#define CT_SCAN(NAME, KERNEL, W, S, FROM, DEPTH, PIECES, ...)                                                                                              \
     [&]() -> ct_status {                                                                                                                                 \
         constexpr int smem   = (W) * PIECES::FLOATS * 4;                                                                                                   \
         const int64_t groups = scan_groups(FROM, batch, channels);                                                                                       \
         int blocks;                                                                                                                                      \
-        CT_TRY((scan_blocks<KERNEL<W, S, FROM, true>, W>(st, smem, groups, (steps + ((W)-1) * (S)-1) / (((W)-1) * (S)), &blocks)));              \
-        auto kernel = blocks > 1 ? KERNEL<W, S, FROM, true> : KERNEL<W, S, FROM, false>;                                                   \
+        CT_TRY((scan_blocks<KERNEL<W, S, FROM, true, DEPTH>, W>(st, smem * (DEPTH), groups, (steps + ((W)-1) * (S)-1) / (((W)-1) * (S)), &blocks)));              \
+        auto kernel = blocks > 1 ? KERNEL<W, S, FROM, true, DEPTH> : KERNEL<W, S, FROM, false, 1>;                                                   \
         if (blocks == 1)                                                                                                                                 \
             CT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                                    \
-        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3((W) * 32), smem, stream(), __VA_ARGS__));               \
+        CT_CUDA(launch_dependent_cluster(kernel, blocks, dim3((unsigned)(groups * blocks)), dim3((W) * 32), blocks > 1 ? smem * (DEPTH) : smem, stream(), __VA_ARGS__));               \
         CT_LAUNCH_CHECK(NAME);                                                                                                                           \
         return CT_OK;                                                                                                                                    \
     }()
@@ -800,30 +807,30 @@ int scan_warps(const DeviceState *st, int64_t groups, int64_t steps) {
     return steps <= 32 ? 2 : blocks / groups * groups * 8 >= blocks * 5 ? 8 : 4;
 }
 
-template <int W, Source FROM>
+template <int W, Source FROM, int DEPTH>
 ct_status launch_scan(
     const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, int64_t batch, int64_t steps, int64_t channels,
     float *out, float *state) {
     constexpr int S = 16;
     const int64_t chains = batch * channels;
-    using Values         = Pieces<2, S, FROM, false>;
+    using Values         = Pieces<2, S, FROM, false, 1>;
     Arrays<2> arrays     = {{}, {gate, value}};
     if (FROM != SINGLE)
         CT_TRY(encode_arrays(FROM, arrays, batch, steps, channels, S));
-    return CT_SCAN("gated_scan", gated_scan_kernel, W, S, FROM, Values, arrays, state0, lengths, chains, steps, (int)channels, blocks, out, state,
+    return CT_SCAN("gated_scan", gated_scan_kernel, W, S, FROM, DEPTH, Values, arrays, state0, lengths, chains, steps, (int)channels, blocks, out, state,
                    st->flags_dev);
 }
-template <int W, Source FROM>
+template <int W, Source FROM, int DEPTH>
 ct_status launch_scan_grad(
     const DeviceState *st, const float *gate, const float *value, const float *state0, const int64_t *lengths, const float *out, const float *dout,
     const float *dstate, int64_t batch, int64_t steps, int64_t channels, float *dgate, float *dvalue, float *dstate0) {
     constexpr int S = 8;
     const int64_t chains = batch * channels;
-    using Values         = Pieces<4, S, FROM, true>;
+    using Values         = Pieces<4, S, FROM, true, 1>;
     Arrays<4> arrays     = {{}, {gate, value, dout, out}};
     if (FROM != SINGLE)
         CT_TRY(encode_arrays(FROM, arrays, batch, steps, channels, S));
-    return CT_SCAN("gated_scan_grad", gated_scan_grad_kernel, W, S, FROM, Values, arrays, state0, lengths, dstate, chains, steps,
+    return CT_SCAN("gated_scan_grad", gated_scan_grad_kernel, W, S, FROM, DEPTH, Values, arrays, state0, lengths, dstate, chains, steps,
                    (int)channels, blocks, dgate, dvalue, dstate0, st->flags_dev);
 }
 #undef CT_SCAN
@@ -867,11 +874,11 @@ ct_status ct_gated_scan(
         constexpr int W = decltype(warps)::value;
         switch (from) {
         case TILES:
-            return launch_scan<W, TILES>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+            return launch_scan<W, TILES, W == 2 ? 1 : 2>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
         case ROWS:
-            return launch_scan<W, ROWS>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+            return launch_scan<W, ROWS, 1>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
         default:
-            return launch_scan<W, SINGLE>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
+            return launch_scan<W, SINGLE, 1>(st, gate, value, state0, lengths, batch, steps, channels, out, state);
         }
     };
     switch (scan_warps(st, scan_groups(from, batch, channels), steps)) {
@@ -914,11 +921,13 @@ ct_status ct_gated_scan_grad(
         constexpr int W = decltype(warps)::value;
         switch (from) {
         case TILES:
-            return launch_scan_grad<W, TILES>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+            if (W == 8 && scan_groups(from, batch, channels) * 6 > st->sm_count) // (see Pieces)
+                return launch_scan_grad<W, TILES, W == 4 ? 2 : 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+            return launch_scan_grad<W, TILES, W == 2 ? 1 : 2>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
         case ROWS:
-            return launch_scan_grad<W, ROWS>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+            return launch_scan_grad<W, ROWS, 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
         default:
-            return launch_scan_grad<W, SINGLE>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+            return launch_scan_grad<W, SINGLE, 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
         }
     };
     switch (scan_warps(st, scan_groups(from, batch, channels), steps)) {
