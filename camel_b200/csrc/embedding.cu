@@ -8,7 +8,7 @@
 // the merged list of both: each token, and behind its last token the end of each row.  A row that lies across slices leaves a partial
 // sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once.
 // Measured (L2 flushed): 32768 rows of 50257 x 2048 59 to 61 us (348 MB, 0.88 to 0.90 of a copy); gradient of 16384 tokens in the same table 111 us (546 MB,
-// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 23 us (three launches), of 1000 in 100 x 64 8.
+// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 13 to 20 us in one (11 MB; each block's chain of loads), of 1000 in 100 x 64 8.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
     uint32_t *base   = totals + bins + 1;
     __shared__ uint32_t warp_sums[kSortWarps];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const uint32_t rank = CTAS > 1 ? cluster_rank() : 0;
+    const uint32_t rank = cluster_rank();
     const uint32_t each = ((m + CTAS * kSortWarps - 1) / (CTAS * kSortWarps) + 31) & ~31u; // tokens of a warp
     const uint64_t lo64 = (uint64_t)(rank * kSortWarps + warp) * each;
     const uint32_t lo = (uint32_t)min(lo64, (uint64_t)m), hi = (uint32_t)min(lo64 + each, (uint64_t)m);
@@ -178,16 +178,13 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
             }
             totals[d] = sum;
         }
-        if (CTAS > 1)
-            cluster_sync();
-        else
-            __syncthreads();
+        cluster_sync();
         uint32_t before = 0, all = 0; // of this thread's digit (bins <= threads)
         if (t < bins) {
             uint32_t c[CTAS];
 #pragma unroll
             for (int r = 0; r < CTAS; ++r)
-                c[r] = CTAS > 1 ? ld_cluster_u32(totals_at + t * 4, r) : totals[t];
+                c[r] = ld_cluster_u32(totals_at + t * 4, r);
 #pragma unroll
             for (int r = 0; r < CTAS; ++r) {
                 before += r < (int)rank ? c[r] : 0;
@@ -195,13 +192,12 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
             }
         }
         if (pass == 0 && rank == 0 && warp == kSortWarps - 1) {
-            const uint32_t none_of = lane < CTAS ? (CTAS > 1 ? ld_cluster_u32(totals_at + bins * 4, lane) : totals[bins]) : 0;
+            const uint32_t none_of = lane < CTAS ? ld_cluster_u32(totals_at + bins * 4, lane) : 0;
             const uint32_t without = __reduce_add_sync(0xffffffffu, none_of);
             if (lane == 0)
                 s.counts[0] = m - without, s.counts[1] = 0;
         }
-        if (CTAS > 1)
-            cluster_arrive(); // this CTA has read the others' totals
+        cluster_arrive(); // this CTA has read the others' totals
         uint32_t upto = all; // over digits, this one included
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -237,13 +233,9 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(
                     put(v, a, base[(v >> shift) & (bins - 1)] + p);
             }
         }
-        if (CTAS > 1) {
-            cluster_wait();
-            if (pass + 1 < passes)
-                cluster_sync(); // the next pass reads what the others wrote
-        } else {
-            __syncthreads();
-        }
+        cluster_wait();
+        if (pass + 1 < passes)
+            cluster_sync(); // the next pass reads what the others wrote
     }
 }
 
@@ -477,12 +469,15 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(
 
 // ---- few tokens -----------------------------------------------------------------------------------
 
-// A block to a range of rows and 128 columns.  It looks through all ids for those of its rows, ranks them by row as the sorting kernel does, in shared memory, and adds
-// up: a warp to a row, or all of them, each a part of its tokens, to a row of more than kAloneTokens.
-constexpr int kAloneTokens = 48, kFewRows = 512; // (1537 x 2050 x 771 24 us with 48, 41 with 16, which the rows above it take in turn)
+// A block has 128 columns of every apart-th row, since those that follow one another may be the words that come most often (1000 x 3000 x 1000 15 us with rows that do,
+// 8 so).  It looks through all ids for those of its rows, ranks them by row as the sorting kernel does, in shared memory, and adds up: a warp to a row, or all of
+// them, each a part of its tokens, to a row of more than kAloneTokens.
+constexpr uint32_t kNoRow  = 0xffffffffu;
+constexpr int kAloneTokens = 48, kFewRows = 512; // (with 16 more rows are taken one after the other)
 template <int TOKENS, bool VEC>
 __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
-    const int64_t *__restrict__ ids, const float *__restrict__ dout, int m, int64_t n, int64_t k, int rows, float scale, float *__restrict__ dtable) {
+    const int64_t *__restrict__ ids, const float *__restrict__ dout, int m, int64_t n, int64_t k, int rows, uint32_t apart, int strips, float scale,
+    float *__restrict__ dtable) {
     constexpr int TURNS = TOKENS / 256, AT_ONCE = 8;
     __shared__ uint32_t counts[8][kFewRows], begins[kFewRows + 1], warp_sums[8];
     __shared__ uint16_t order[TOKENS], many[kFewRows];
@@ -490,13 +485,16 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
     __shared__ int many_count;
     griddep_wait();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t row0 = (int64_t)blockIdx.x * rows, c0 = (int64_t)blockIdx.y * 128;
-    const int here     = (int)min((int64_t)rows, n - row0);
-    int row[TURNS], rank[TURNS];
+    const uint32_t range = blockIdx.x / strips;
+    const int64_t c0     = (int64_t)(blockIdx.x - range * strips) * 128, c1 = c0;
+    const int here = (int)((n - 1 - range) / apart) + 1; // row range + r apart is its row r
+    uint32_t place[TURNS]; // the token's row of the block, and behind the 16th bit its place among the warp's tokens of that row
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) { // (without conditions: each load would wait for the one before)
-        const uint64_t id = (uint64_t)ids[min((warp * TURNS + i) * 32 + lane, m - 1)] - (uint64_t)row0;
-        row[i]            = (warp * TURNS + i) * 32 + lane < m && id < (uint64_t)here ? (int)id : -1;
+        const int64_t id = ids[min((warp * TURNS + i) * 32 + lane, m - 1)];
+        const bool is    = (warp * TURNS + i) * 32 + lane < m && id >= 0 && id < n;
+        const uint32_t r = (uint32_t)id / apart;
+        place[i]         = is && (uint32_t)id - r * apart == range ? r : kNoRow;
     }
     for (int r = t; r < rows; r += 256)
 #pragma unroll
@@ -507,17 +505,19 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-        uint32_t alike = __ballot_sync(0xffffffffu, row[i] >= 0);
+        const uint32_t row = place[i];
+        uint32_t alike     = __ballot_sync(0xffffffffu, row != kNoRow);
         if (alike) {
             for (int b = 0; (rows - 1) >> b; ++b) {
-                const uint32_t set = __ballot_sync(0xffffffffu, (row[i] >> b) & 1);
-                alike &= (row[i] >> b) & 1 ? set : ~set;
+                const uint32_t set = __ballot_sync(0xffffffffu, (row >> b) & 1);
+                alike &= (row >> b) & 1 ? set : ~set;
             }
             const int ahead = __popc(alike & ((1u << lane) - 1));
-            rank[i]         = row[i] >= 0 ? counts[warp][row[i]] + ahead : 0;
+            if (row != kNoRow)
+                place[i] |= (counts[warp][row] + ahead) << 16;
             __syncwarp();
-            if (row[i] >= 0 && ahead == 0)
-                counts[warp][row[i]] += __popc(alike);
+            if (row != kNoRow && ahead == 0)
+                counts[warp][row] += __popc(alike);
             __syncwarp();
         }
     }
@@ -559,23 +559,23 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TURNS; ++i)
-        if (row[i] >= 0)
-            order[begins[row[i]] + counts[warp][row[i]] + rank[i]] = (uint16_t)((warp * TURNS + i) * 32 + lane);
+        if (place[i] != kNoRow)
+            order[begins[place[i] & 0xffff] + counts[warp][place[i] & 0xffff] + (place[i] >> 16)] = (uint16_t)((warp * TURNS + i) * 32 + lane);
     __syncthreads();
-    auto column = [&](int q) -> int64_t { return c0 + (VEC ? lane * 4 + q : q * 32 + lane); };
-    auto add    = [&](uint32_t first, uint32_t last, double (&to)[4]) {
+    auto in_strip = [&](int q) { return VEC ? lane * 4 + q : q * 32 + lane; };
+    auto add      = [&](uint32_t first, uint32_t last, int64_t c1, double (&to)[4]) {
         for (uint32_t i = first; i < last; i += AT_ONCE) {
             float v[AT_ONCE][4];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
                 const float *src = dout + (int64_t)order[min(i + u, last - 1)] * k;
                 if (VEC) {
-                    const float4 f = *reinterpret_cast<const float4 *>(src + min(column(0), k - 4));
+                    const float4 f = *reinterpret_cast<const float4 *>(src + min(c1 + in_strip(0), k - 4));
                     v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        v[u][q] = src[min(column(q), k - 1)];
+                        v[u][q] = src[min(c1 + in_strip(q), k - 1)];
                 }
             }
 #pragma unroll
@@ -590,35 +590,47 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
         const uint32_t first = begins[r], last = begins[r + 1];
         if (last - first > kAloneTokens)
             continue;
+        float *to = dtable + (range + (int64_t)r * apart) * k + c1;
+        if (first == last) {
+            if (VEC) {
+                if (c1 + in_strip(0) < k)
+                    __stcs(reinterpret_cast<float4 *>(to + in_strip(0)), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (c1 + in_strip(q) < k)
+                        __stcs(to + in_strip(q), 0.0f);
+            }
+            continue;
+        }
         double all[4] = {};
-        add(first, last, all);
-        float *to = dtable + (row0 + r) * k;
+        add(first, last, c1, all);
         if (VEC) {
-            if (column(0) < k)
-                __stcs(reinterpret_cast<float4 *>(to + column(0)),
+            if (c1 + in_strip(0) < k)
+                __stcs(reinterpret_cast<float4 *>(to + in_strip(0)),
                        make_float4((float)(all[0] * scale), (float)(all[1] * scale), (float)(all[2] * scale), (float)(all[3] * scale)));
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (column(q) < k)
-                    __stcs(to + column(q), (float)(all[q] * scale));
+                if (c1 + in_strip(q) < k)
+                    __stcs(to + in_strip(q), (float)(all[q] * scale));
         }
     }
     for (int i = 0; i < many_count; ++i) {
         const int r          = many[i];
         const uint32_t first = begins[r], count = begins[r + 1] - first;
         double all[4]        = {};
-        add(first + count * warp / 8, first + count * (warp + 1) / 8, all);
+        add(first + count * warp / 8, first + count * (warp + 1) / 8, c1, all);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            part[warp][column(q) - c0] = all[q];
+            part[warp][in_strip(q)] = all[q];
         __syncthreads();
-        if (t < 128 && c0 + t < k) {
+        if (t < 128 && c1 + t < k) {
             double whole = 0.0;
 #pragma unroll
             for (int w = 0; w < 8; ++w)
                 whole += part[w][t];
-            dtable[(row0 + r) * k + c0 + t] = (float)(whole * scale);
+            dtable[(range + (int64_t)r * apart) * k + c1 + t] = (float)(whole * scale);
         }
         __syncthreads();
     }
@@ -691,16 +703,20 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     ProfScope prof("embedding_grad");
     const bool vec = (k & 3) == 0 && aligned16(dout) && aligned16(dtable);
     // In one launch, where that is sooner than sorting, adding up and joining in three (us in line, three launches and one; tokens x rows x columns):
-    // 8 x 131072 x 768 77 and 63, 500 x 50000 x 1000 58 and 42, 1000 x 5000 x 64 18 and 9, 1000 x 50000 x 1000 55 and 44,
-    // 2000 x 10 x 2000 19 and 9, 4000 x 200 x 1000 22 and 18, 4000 x 50000 x 20 23 and 21; beyond the limits 1537 x 2050 x 771 21 and 24, 3000 x 3000 x 1000 23 and 31, 4000 x 50000 x 1000 57 and 81
-    if ((m <= 1024 || (m <= 4096 && n * k <= 1 << 20)) && k <= 65535 * 128) { // (of a grid's second size there are 65535)
-        // 12 blocks for each SM, of large tables 36 (us with 12, 24, 36 and 48; 500 x 50000 x 1000 47, 44, 42, 43; 8 x 131072 x 768 67, 64, 63, 62;
-        // 16 x 32003 x 1024 23, 24, 27, 30; 1000 x 20000 x 400 15, 17, 20, 22)
-        const int64_t strips = (k + 127) / 128, blocks = st->sm_count * (n * k > 1 << 25 ? 36 : 12);
-        const int rows       = (int)std::min<int64_t>(kFewRows, (n * strips + blocks - 1) / blocks);
-        auto few             = [&](auto kernel) -> ct_status {
-            CT_CUDA(launch_dependent(kernel, dim3((unsigned)((n + rows - 1) / rows), (unsigned)strips), dim3(256), 0, stream(), ids, dout, (int)m, n, k, rows,
-                                     (float)scale, dtable));
+    // 1000 x 3000 x 1000 22 and 8, 1000 x 50000 x 1000 56 and 37, 8 x 131072 x 768 77 and 65, 1537 x 2050 x 771 21 and 13, 4000 x 4000 x 100 20 and 12,
+    // 4000 x 50000 x 300 32 and 26, 4000 x 50000 x 1000 58 and 52; but 8000 x 58000 x 266 39 and 52, 8000 x 20000 x 1000 39 and 52.  Rows of many tokens keep one
+    // block busy, for words of a text the first with every second to fifth token of few rows: 2000 x 10 x 2000 18 and 10, 4000 x 10 x 2000 19 and 17 (behind other work
+    // 29 and 35), 4000 x 3 x 64 17 and 22, 4000 x 1 x 500 22 and 39
+    const int64_t columns = (k + 127) / 128;
+    // 4 blocks to an SM run at once; large tables take 12 (us with 4 and 12; 500 x 50000 x 1000 46 and 37, 16 x 32003 x 1024 24 and 23, 1000 x 20000 x 400 13 and 14,
+    // 1537 x 2050 x 771 13 and 18)
+    const int64_t blocks = st->sm_count * (n * k > 1 << 24 ? 12 : 4);
+    const int rows       = (int)std::max<int64_t>(1, std::min<int64_t>(kFewRows, (n * columns + blocks - 1) / blocks));
+    const int64_t apart  = (n + rows - 1) / rows;
+    if ((m <= 1024 || (m <= 4096 && m <= 256 * n)) && apart * columns <= INT32_MAX) {
+        auto few = [&](auto kernel) -> ct_status {
+            CT_CUDA(launch_dependent(kernel, dim3((unsigned)(apart * columns)), dim3(256), 0, stream(), ids, dout, (int)m, n, k, rows,
+                                     (uint32_t)apart, (int)columns, (float)scale, dtable));
             CT_LAUNCH_CHECK("embedding_grad_few");
             return CT_OK;
         };
@@ -745,9 +761,7 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
         CT_LAUNCH_CHECK("embedding_sort");
         return CT_OK;
     };
-    // (4000 tokens: 4 rounds of one CTA 26 us in all, one of eight 21; 2000: 19 and 20)
-    CT_TRY(m <= 2048        ? sort(embedding_sort_kernel<1, 2>, 1)
-           : m <= 8 * 1024  ? sort(embedding_sort_kernel<8, 1>, 8)
+    CT_TRY(m <= 8 * 1024    ? sort(embedding_sort_kernel<8, 1>, 8)
            : m <= 16 * 1024 ? sort(embedding_sort_kernel<16, 1>, 16)
            : m <= 32 * 1024 ? sort(embedding_sort_kernel<16, 2>, 16)
            : m <= 64 * 1024 ? sort(embedding_sort_kernel<16, 4>, 16)

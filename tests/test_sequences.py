@@ -71,7 +71,8 @@ def test_embedding(m, n, k):
 @pytest.mark.parametrize("m,n,k", EMBEDDING_SHAPES + [(5000, 300, 5), (9000, 70000, 24), (40000, 1000, 8), (3000, 1, 40), (100, 1500000, 2), (70000, 131072, 3),
                                                      (1025, 500, 6), (2049, 500, 70), (8193, 60, 4), (17000, 40, 4), (33000, 300, 3), (140000, 2000, 2), (300000, 70, 1),
                                                      (65, 129, 65), (700, 60, 100), (3000, 200, 60), (1024, 700, 1030), (900, 200000, 12), (2048, 512, 512), (4096, 513, 300),
-                                                     (4096, 3, 1000), (1030, 4000, 700), (5, 2, 8388737)])
+                                                     (4096, 3, 1000), (1030, 4000, 700), (5, 2, 8388737), (4097, 40, 100), (1025, 4, 300), (1025, 5, 300), (1024, 1, 130),
+                                                     (3000, 149 * 4, 129), (2000, 13000, 1300), (60, 600000, 3), (8192, 300, 40)])
 def test_embedding_grad(m, n, k):
     ids, _, dout = embedding_inputs(m, n, k, 1)
     want, size = embedding_grad64(ids, dout, n, 3.7)
@@ -81,7 +82,7 @@ def test_embedding_grad(m, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(1, 50, 8), (4000, 50, 8), (20000, 5000, 300), (3000, 4, 2050), (5000, 4, 2050)])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 8), (4000, 50, 8), (20000, 5000, 300), (3000, 4, 2050), (3000, 13, 2050), (5000, 4, 2050)])
 @pytest.mark.parametrize("which", ["one", "last", "two", "none", "all", "descending"])
 def test_embedding_grad_of_uneven_tokens(m, n, k, which):
     """All tokens one row (it lies across every slice), two rows by turns, none of the table's, every row as often, in the other order."""
