@@ -355,22 +355,33 @@ __global__ void __launch_bounds__(256, FIT) embedding_grad_kernel(
         for (int j = 0; j < 4 * V; ++j)
             sum[j] = 0.0;
     };
-    // rows without a token
+    // Rows without a token.  Those that begin anywhere are cleared as what they are together, a stretch of which each strip has a part (16384 x 50257 x 2047 120 us
+    // so, 125 row by row).
     auto clear = [&](uint32_t first, uint32_t last) {
         float *to = dtable + (int64_t)first * k;
-        for (uint32_t row = first; row < last; ++row, to += k)
+        if (VEC) {
+            for (uint32_t row = first; row < last; ++row, to += k)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (VEC) {
+                for (int j = 0; j < V; ++j)
                     if (column(j, 0) < k)
                         __stcs(reinterpret_cast<float4 *>(to + column(j, 0)), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (column(j, q) < k)
-                            __stcs(to + column(j, q), 0.0f);
-                }
-            }
+            return;
+        }
+        int64_t count = (int64_t)(last - first) * k;
+        if (strips > 1) {
+            const int64_t part = count < (int64_t)1 << 32 ? (uint32_t)count / strips + 1 : count / strips + 1, begin = min(part * strip, count);
+            count              = min(part, count - begin);
+            to += begin;
+        }
+        const int ahead      = (int)min((int64_t)(-(reinterpret_cast<uintptr_t>(to) >> 2) & 3), count);
+        const int64_t pieces = (count - ahead) / 4;
+        if (lane < ahead)
+            to[lane] = 0.0f;
+        to += ahead;
+        for (int64_t i = lane; i < pieces; i += 32)
+            __stcs(reinterpret_cast<float4 *>(to) + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        if (lane < count - ahead - 4 * pieces)
+            to[4 * pieces + lane] = 0.0f;
     };
     uint32_t row = r0;
     bool open    = goes_on[0]; // whether the row has tokens
@@ -729,11 +740,14 @@ ct_status ct_embedding_grad(const int64_t *ids, const float *dout, int64_t m, in
     const int v    = k <= 64 ? 1 : 2; // 16384 x 50000 x 32 33 us by 128 columns, 38 by 256; 64 36 and 39; 128 42 and 40; 256 46 and 44
     const int64_t strips = (k + 128 * v - 1) / (128 * v);
     // Slices: as many as run at once, of 8 items at least; where that is more than 64 items each, four times as many, since their ends come apart
-    // (16384 x 50257 x 2048: 149 us with one for each warp that runs, 125 with four)
+    // (16384 x 50257 x 2048: 149 us with one for each warp that runs, 125 with four);
+    // up to twice as many of rows without tokens, which take less time than those with (6913 x 58582 x 266 40 and 34, 8666 x 575 x 2393 41 and 50)
     const int64_t wave = std::max<int64_t>(1, (int64_t)st->sm_count * 16 / strips), items = n + m;
+    const int64_t once = std::max<int64_t>(1, std::min(wave, items / 8));
     const int64_t slices = wave == 1           ? 1 // of rows so long, whose partial sums would take more memory than they save time
-                           : items < wave * 64 ? std::max<int64_t>(1, std::min(wave, items / 8))
-                                               : std::min(wave * 4 + 1, items / 64);
+                           : items >= wave * 64 ? std::min(wave * 4 + 1, items / 64)
+                           : n > 2 * m          ? std::max(once, std::min(wave * 2, items / 32))
+                                                : once;
 
     int bits = 1; // of the ids and of n, which stands for none
     while ((n >> bits) > 0)
