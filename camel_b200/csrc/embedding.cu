@@ -8,7 +8,7 @@
 // the merged list of both: each token, and behind its last token the end of each row.  A row that lies across slices leaves a partial
 // sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once.
 // Measured (L2 flushed): 32768 rows of 50257 x 2048 59 to 61 us (348 MB, 0.88 to 0.90 of a copy); gradient of 16384 tokens in the same table 111 us (546 MB,
-// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 13 to 20 us in one (11 MB; each block's chain of loads), of 1000 in 100 x 64 8.
+// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 12 us in one (11 MB; each block's chain of loads), of 1000 in 100 x 64 8.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 
