@@ -78,10 +78,60 @@ struct Weights {
 };
 __device__ __forceinline__ bool class_of(int64_t id, int64_t n) { return id >= 0 && id < n; }
 __device__ __forceinline__ float lse_of(Sum s, float temperature) { return __fadd_rn(__fdiv_rn(about(s.top), temperature), logf(s.sum)); }
-// p (log p - (z / T - lse)) of an entry, x = (teacher - top) / T
-__device__ __forceinline__ float divergence(float x, const Weights &w, float log_sum, float inv_sum, float z, float temperature, float lse) {
-    const float p = __fmul_rn(expf(x), inv_sum);
-    return p == 0.0f ? 0.0f : __fmul_rn(p, __fsub_rn(__fsub_rn(x, log_sum), __fsub_rn(__fdiv_rn(z, temperature), lse))); // 0 log 0 is 0
+// The loss over T^2, sum p (log p - log q), cancels where p is near q, and T^2 is large just where the cancelling is worst: both distributions are flat then.
+// So log p - log q of an entry is x - y + log(the classes' sum / the weights'), x = (teacher - its top) / T and y = (z - top) / T, in which
+// logits' common offsets are gone (z / T - lse would round them), and rows whose sum is below kSmall at temperatures above kWarm are taken again in 64 bits.  What is
+// left is off by T^2 times some 2^-20 (both sums' exponentials, 2^-22 each, and their arguments), 2^-16 at kWarm, and 2^-16 of a sum above kSmall.  (60000 rows of 10
+// classes, all of them entries, T = 8: 17 us in line so, 9 in 32 bits; 300 of 1000 14 and 11.)
+constexpr float kWarm = 4.0f, kSmall = 1.0f / 16.0f;
+struct Ratio {
+    float inv_sum, log; // 1 / the weights' sum; the logarithm of the classes' sum over it
+};
+__device__ __forceinline__ Ratio ratio_of(const Weights &w, const Sum &s) { return {__fdiv_rn(1.0f, w.sum), logf(__fdiv_rn(s.sum, w.sum))}; }
+__device__ __forceinline__ float divergence(float u, float z, const Weights &w, const Sum &s, const Ratio &r, float inv_t) {
+    const float x = __fsub_rn(u, w.top), p = __fmul_rn(expf(__fmul_rn(x, inv_t)), r.inv_sum);
+    return p == 0.0f ? 0.0f : __fmul_rn(p, __fadd_rn(__fmul_rn(__fsub_rn(x, __fsub_rn(z, about(s.top))), inv_t), r.log)); // 0 log 0 is 0
+}
+__device__ __forceinline__ bool again_wide(float sum, float temperature) { return temperature > kWarm && sum < kSmall; }
+__device__ __forceinline__ float loss_from(float sum, float temperature) { return __fmul_rn(__fmul_rn(temperature, temperature), sum); }
+
+// In 64 bits: of the classes' exponentials, of the weights, and of these times x - y; one thread's part of those of `threads`.
+struct Wide {
+    double classes, weights, cross;
+    __device__ __forceinline__ void add(const Wide &o) { classes += o.classes, weights += o.weights, cross += o.cross; }
+    template <int TPR> __device__ __forceinline__ void add_lanes() {
+#pragma unroll
+        for (int o = TPR / 2; o; o >>= 1) {
+            Wide b;
+            b.classes = __shfl_xor_sync(0xffffffffu, classes, o), b.weights = __shfl_xor_sync(0xffffffffu, weights, o);
+            b.cross = __shfl_xor_sync(0xffffffffu, cross, o);
+            add(b);
+        }
+    }
+    __device__ __forceinline__ float loss(float temperature) const {
+        return (float)((double)temperature * (double)temperature * (cross / weights + log(classes / weights)));
+    }
+};
+__device__ __forceinline__ Wide wide_sums(
+    const float *src, int64_t n, float z_top, const int64_t *__restrict__ ids, const float *__restrict__ teacher, int top, float u_top, float temperature, int t,
+    int threads) {
+    const double inv_t = 1.0 / (double)temperature;
+    Wide s = {0.0, 0.0, 0.0};
+#pragma unroll 1
+    for (int64_t i = t; i < n; i += threads)
+        s.classes += exp(((double)src[i] - (double)z_top) * inv_t);
+#pragma unroll 1
+    for (int j = t; j < top; j += threads) {
+        const int64_t id = ids[j];
+        if (!class_of(id, n))
+            continue;
+        const double x = ((double)teacher[j] - (double)u_top) * inv_t, e = exp(x);
+        if ((float)e > 0.0f) { // as in 32 bits, an entry of no weight adds nothing
+            s.weights += e;
+            s.cross += e * (x - ((double)src[id] - (double)z_top) * inv_t);
+        }
+    }
+    return s;
 }
 // exp(z / T - lse) of a logit: 1 / T in two parts.  -infinity becomes a number, which neither part makes a NaN.
 __device__ __forceinline__ float probability(float z, float inv_t, float inv_t_rest, float lse) {
@@ -126,16 +176,29 @@ template <int TPR, int E> struct Entries {
     }
 };
 
+// src, ids and teacher are those of the row; lanes whose row is not `here` go along.
 template <int TPR, int E>
-__device__ __forceinline__ float loss_of(const Entries<TPR, E> &entries, const Weights &w, const float (&z)[E], float temperature, float inv_t, float lse) {
-    const float log_sum = logf(w.sum), inv_sum = __fdiv_rn(1.0f, w.sum);
+__device__ __forceinline__ float loss_of(
+    const Entries<TPR, E> &entries, const float (&z)[E], const Sum &s, const float *src, int64_t n, const int64_t *__restrict__ ids,
+    const float *__restrict__ teacher, int top, float temperature, float inv_t, bool here, int t) {
+    const Weights w = entries.weights(inv_t);
+    const Ratio r   = ratio_of(w, s);
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (entries.id[e] >= 0)
-            sum = __fadd_rn(sum, divergence(__fmul_rn(__fsub_rn(entries.u[e], w.top), inv_t), w, log_sum, inv_sum, z[e], temperature, lse));
-    sum = __fmul_rn(__fmul_rn(temperature, temperature), sum_lanes<TPR>(sum));
-    return w.some ? sum : 0.0f;
+            sum = __fadd_rn(sum, divergence(entries.u[e], z[e], w, s, r, inv_t));
+    sum              = sum_lanes<TPR>(sum);
+    float loss       = loss_from(sum, temperature);
+    const bool again = here && w.some && again_wide(sum, temperature);
+    if (__any_sync(0xffffffffu, again)) {
+        Wide wide = {0.0, 0.0, 0.0};
+        if (again)
+            wide = wide_sums(src, n, s.top, ids, teacher, top, w.top, temperature, t, TPR);
+        wide.add_lanes<TPR>();
+        loss = again ? wide.loss(temperature) : loss;
+    }
+    return w.some ? loss : 0.0f;
 }
 
 // ---- rows of few classes: TPR threads to a row, V of its logits in each ---------------------------
@@ -164,18 +227,16 @@ __global__ void __launch_bounds__(256) distill_short_kernel(
 #pragma unroll
     for (int i = 0; i < V; ++i)
         z[i] = i * TPR + t < n ? z[i] : -INFINITY;
-    const Weights w = entries.weights(inv_t);
-    Sum s           = {-INFINITY, 0.0f};
+    Sum s = {-INFINITY, 0.0f};
     take(s, z, c);
-    s             = join_lanes<TPR>(s, c);
-    const float l = lse_of(s, temperature);
+    s = join_lanes<TPR>(s, c);
     if (loss) {
-        const float value = loss_of(entries, w, at, temperature, inv_t, l);
+        const float value = loss_of(entries, at, s, src, n, ids + (here ? row * top : 0), teacher + (here ? row * top : 0), top, temperature, inv_t, here, t);
         if (here && t == 0)
             loss[row] = value;
     }
     if (lse && here && t == 0)
-        lse[row] = l;
+        lse[row] = lse_of(s, temperature);
 }
 
 // Takes the entries' weights off a row that the TPR threads have written, memory that they share: TPR entries after another, of which the first of a class
@@ -340,14 +401,14 @@ __global__ void __launch_bounds__(kThreads) distill_warp_kernel(
 #pragma unroll
     for (int e = 0; e < E; ++e)
         at[e] = entries.id[e] >= 0 ? src[entries.id[e]] : 0.0f;
-    const float l = lse_of(join_lanes<32>(sum_stretch<32>(src, st, f, c, lane), c), temperature);
+    const Sum s = join_lanes<32>(sum_stretch<32>(src, st, f, c, lane), c);
     if (loss) {
-        const float value = loss_of(entries, entries.weights(inv_t), at, temperature, inv_t, l);
+        const float value = loss_of(entries, at, s, src, n, ids + row * top, teacher + row * top, top, temperature, inv_t, true, lane);
         if (lane == 0)
             loss[row] = value;
     }
     if (lse && lane == 0)
-        lse[row] = l;
+        lse[row] = lse_of(s, temperature);
 }
 
 template <bool VEC>
@@ -402,6 +463,9 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
     __shared__ SharedEntries entries;
     __shared__ float entry_z[kMostEntries];
     __shared__ Sum warps[kThreads / 32], blocks[8];
+    __shared__ Wide wide[kThreads / 32];
+    __shared__ float z_top, u_top;
+    __shared__ bool again;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t rank = parts > 1 ? cluster_rank() : 0;
     if (parts > 1)
@@ -444,21 +508,39 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
             s = join_lanes<32>(s, c);
         }
     }
-    if (rank == 0 && warp == 0) {
-        const float l = lse_of(s, temperature);
+    if (rank != 0)
+        return;
+    if (warp == 0) {
         if (loss) {
-            const Weights w     = weights_of(entries, top, inv_t, lane);
-            const float log_sum = logf(w.sum), inv_sum = __fdiv_rn(1.0f, w.sum);
+            const Weights w = weights_of(entries, top, inv_t, lane);
+            const Ratio r   = ratio_of(w, s);
             float sum = 0.0f;
             for (int j = lane; j < top; j += 32)
                 if (entries.id[j] >= 0)
-                    sum = __fadd_rn(sum, divergence(__fmul_rn(__fsub_rn(entries.u[j], w.top), inv_t), w, log_sum, inv_sum, entry_z[j], temperature, l));
-            sum = __fmul_rn(__fmul_rn(temperature, temperature), sum_lanes<32>(sum));
-            if (lane == 0)
-                loss[row] = w.some ? sum : 0.0f;
+                    sum = __fadd_rn(sum, divergence(entries.u[j], entry_z[j], w, s, r, inv_t));
+            sum = sum_lanes<32>(sum);
+            if (lane == 0) {
+                loss[row] = w.some ? loss_from(sum, temperature) : 0.0f;
+                z_top = s.top, u_top = w.top, again = w.some && again_wide(sum, temperature);
+            }
         }
         if (lse && lane == 0)
-            lse[row] = l;
+            lse[row] = lse_of(s, temperature);
+    }
+    if (!loss || !(temperature > kWarm))
+        return;
+    __syncthreads();
+    if (!again)
+        return;
+    Wide sums = wide_sums(src, n, z_top, ids + row * top, teacher + row * top, top, u_top, temperature, t, kThreads);
+    sums.add_lanes<32>();
+    if (lane == 0)
+        wide[warp] = sums;
+    __syncthreads();
+    if (t == 0) {
+        for (int w = 1; w < kThreads / 32; ++w)
+            sums.add(wide[w]);
+        loss[row] = sums.loss(temperature);
     }
 }
 

@@ -444,13 +444,16 @@ ct_status ct_gated_scan_grad(
  *   loss[i] = T^2 * (sum over entries of p * (log p - log q[class])),   lse[i] = log(sum over classes of exp(z / T))
  * An id outside 0 .. n-1 is no entry (a row may have fewer than top); a row without entries is padding: its loss is 0, whatever its logits hold.  Entries of
  * the same class count each.  An entry of weight 0 (teacher -infinity) adds nothing; otherwise infinities and NaN as for ct_dense_cross_entropy.  T is the
- * temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null. */
+ * temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null.
+ * The loss is off by about 2^-16 of the larger of 1 and itself, at any temperature and however far from zero the logits are (from T = 10^5 on by T^2 2^-49, which
+ * is more): where T is above 4 and the divergence below 1/16, as it is when the entries are all classes, a row is summed in 64 bits. */
 ct_status ct_distill(
     const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, int64_t m, int64_t n, int64_t top, double temperature, float *loss_dev,
     float *lse_dev);
 /* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
  *   dlogits[i][c] = dloss[i] * T * (exp(z[c] / T - lse[i]) - (sum of p over the row's entries of class c)), zeros in rows without entries.
- * dlogits may be logits itself. */
+ * The exponential q is off by some 2^-22 (1 + |z / T - lse|) of itself (0 below 2^-126), and as lse is rounded to float32 by 2^-24 |lse| more; dlogits by T times that.
+ * Where p is near q a difference of 1 in the logits is a difference of about q in dlogits / dloss: at T = 10^4 that is off by 1 % or so, at 10^6 it is lost.  dlogits may be logits itself. */
 ct_status ct_distill_grad(
     const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, const float *lse_dev, const float *dloss_dev, int64_t m, int64_t n,
     int64_t top, double temperature, float *dlogits_dev);

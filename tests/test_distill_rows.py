@@ -1,0 +1,80 @@
+"""Distillation where its rows are hard: any temperature that is accepted, logits far from zero, classes and entries that are masked."""
+import numpy as np
+import pytest
+
+from camel_b200 import tensor as T
+from test_layers import U, dev, within
+from test_sequences import distill_grad64
+
+gpu = pytest.mark.gpu
+
+
+def exact(z, ids, teacher, temperature):
+    """loss, lse and p from the definition, in 80 bits: at a temperature of 10^6 a sum of 64 bits is off by 10^12 2^-53 in the loss."""
+    w = np.longdouble(np.float32(temperature))
+    z, ids, teacher = np.atleast_2d(z), np.atleast_2d(ids), np.atleast_2d(teacher)
+    has = (ids >= 0) & (ids < z.shape[1])
+    with np.errstate(invalid="ignore"):
+        x, u = z.astype(np.longdouble) / w, np.where(has, teacher.astype(np.longdouble) / w, -np.inf)
+        x_top, u_top = x.max(1, keepdims=True), u.max(1, keepdims=True)
+        log_sum = np.log(np.exp(x - x_top).sum(1, keepdims=True))
+        log_p = u - u_top - np.log(np.exp(u - u_top).sum(1, keepdims=True))
+        log_q = np.take_along_axis(x, np.where(has, ids, 0), 1) - x_top - log_sum
+        p = np.exp(log_p)
+        loss = w * w * np.where(p > 0, p * (log_p - log_q), 0).sum(1)
+    return loss, (x_top + log_sum)[:, 0], p.astype(np.float64)
+
+
+def loss_off(loss, temperature):
+    """In 32 bits the divergence is off by some 16 U = 2^-20: 4 U (2^-22) of each of two exponentials, their sums' and logarithm's roundings, and 3 U of
+    the mean argument, which is around 1.  That counts T^2 times, 2^-16 at T = 4; above, a divergence below 1/16 is taken in 64 bits, off by a few 2^-52, and a
+    larger one is off by 16 of 2^-20 of itself."""
+    return 2.0 ** -16 * np.maximum(1, np.abs(loss.astype(np.float64))) + 2.0 ** -49 * temperature ** 2
+
+
+# a row's entries are all its classes: 8 and 16 threads to a row, a warp, a block
+COVERED = [(41, 10), (5, 2), (9, 16), (19, 32), (7, 60), (6, 128), (5, 700), (3, 1024)]
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-6, 0.01, 1.0, 4.0, 4.001, 20.0, 100.0, 1e3, 1e4, 1e6])
+@pytest.mark.parametrize("m,n", COVERED)
+def test_loss_of_all_classes_at_any_temperature(m, n, temperature):
+    rng = np.random.default_rng(n)
+    for offset in (0, 1000, -70000):
+        z = (rng.normal(0, 2, (m, n)) + offset).astype(np.float32)
+        ids = np.argsort(rng.uniform(0, 1, (m, n)), 1)
+        near = rng.choice([0.0, 0.01, 2.0], (m, 1))  # the teacher's answer itself, one near it, another one
+        teacher = (np.take_along_axis(z, ids, 1) + near * rng.normal(0, 1, (m, n)) - offset / 3).astype(np.float32)
+        want, want_lse, p = exact(z, ids, teacher, temperature)
+        loss, lse = T.distill(dev(z), dev(ids), dev(teacher), temperature)
+        within(loss.numpy(), want.astype(np.float64), loss_off(want, temperature), "loss")
+        # lse = top / T + log(sum), three roundings, and 2^-20 of the sum as above
+        within(lse.numpy(), want_lse.astype(np.float64), U * (3 * np.abs(want_lse.astype(np.float64)) + 16 + 3 * np.log(n)), "lse")
+        if temperature >= 0.01:
+            grad = T.distill_grad(dev(z), dev(ids), dev(teacher), lse, temperature)
+            want, off = distill_grad64(z, ids, p, lse.numpy(), np.ones(m), temperature)
+            # q is 0 below 2^-126, the smallest that ex2.approx.ftz gives: off by less than that times T
+            within(grad.numpy(), want, off + temperature * 2.0 ** -126, "dlogits")
+
+
+# rows of which a mask leaves `left` classes, all of them entries: a warp, a block, two and four blocks to a row
+MASKED = [(3, 1000, 40), (2400, 1030, 9), (4, 6001, 300), (50, 30000, 20), (2, 32003, 1000)]
+
+
+@gpu
+@pytest.mark.parametrize("mask", [-np.inf, np.finfo(np.float32).min, -1e9])
+@pytest.mark.parametrize("temperature", [2.0, 20.0, 1e3])
+@pytest.mark.parametrize("m,n,left", MASKED)
+def test_loss_of_masked_classes(m, n, left, temperature, mask):
+    rng = np.random.default_rng(n + left)
+    z = np.full((m, n), mask, np.float32)
+    ids = np.stack([rng.choice(n, left, False) for _ in range(m)])
+    some = rng.normal(0, 2, (m, left)).astype(np.float32)
+    np.put_along_axis(z, ids, some, 1)
+    teacher = (some + rng.choice([0.0, 0.01, 2.0], (m, 1)) * rng.normal(0, 1, (m, left))).astype(np.float32)
+    ids[::3, left // 2] = -1  # one of the classes is none of the row's entries
+    loss, lse = T.distill(dev(z), dev(ids), dev(teacher), temperature)
+    want, want_lse, p = exact(z, ids, teacher, temperature)
+    within(loss.numpy(), want.astype(np.float64), loss_off(want, temperature), "loss")
+    within(lse.numpy(), want_lse.astype(np.float64), U * (3 * np.abs(want_lse.astype(np.float64)) + 16 + 3 * np.log(n)), "lse")
