@@ -77,6 +77,8 @@ struct Weights {
     bool some; // whether there is any entry
 };
 __device__ __forceinline__ bool class_of(int64_t id, int64_t n) { return id >= 0 && id < n; }
+// An entry of weight 0 is none: a row of nothing else is one without entries.
+__device__ __forceinline__ bool entry_of(int64_t id, int64_t n, float teacher) { return class_of(id, n) && teacher != -INFINITY; }
 __device__ __forceinline__ float lse_of(Sum s, float temperature) { return __fadd_rn(__fdiv_rn(about(s.top), temperature), logf(s.sum)); }
 // The loss over T^2, sum p (log p - log q), cancels where p is near q, and T^2 is large just where the cancelling is worst: both distributions are flat then.
 // So log p - log q of an entry is x - y + log(the classes' sum / the weights'), x = (teacher - its top) / T and y = (z - top) / T, in which
@@ -139,7 +141,7 @@ __device__ __forceinline__ float probability(float z, float inv_t, float inv_t_r
     return ex2(__fmul_rn(__fmaf_rn(z, inv_t, __fmaf_rn(z, inv_t_rest, -lse)), kLog2e));
 }
 
-// A row's entries in the registers of its TPR threads, E each: entry e TPR + t; no class: -1.  All loads are on their way before one is looked at.
+// A row's entries in the registers of its TPR threads, E each: entry e TPR + t; none: -1.  All loads are on their way before one is looked at.
 template <int TPR, int E> struct Entries {
     int id[E];
     float u[E];
@@ -153,7 +155,7 @@ template <int TPR, int E> struct Entries {
         }
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            id[e] = e * TPR + t < top && class_of(wide[e], n) ? (int)wide[e] : -1;
+            id[e] = e * TPR + t < top && entry_of(wide[e], n, u[e]) ? (int)wide[e] : -1;
     }
     __device__ __forceinline__ Weights weights(float inv_t) const {
         float most = -INFINITY, sum = 0.0f;
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) distill_grad_warp_kernel(
 // The entries of a row in shared memory; the sum of weights is left to one warp.
 struct SharedEntries {
     float u[kMostEntries];
-    int id[kMostEntries]; // no class: -1
+    int id[kMostEntries]; // none: -1
 };
 __device__ __forceinline__ Weights weights_of(const SharedEntries &s, int top, float inv_t, int lane) {
     float most = -INFINITY, sum = 0.0f;
@@ -484,8 +486,9 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(
     if (rank == 0 && loss)
         for (int j = t; j < top; j += kThreads) {
             const int64_t id = ids[row * top + j];
-            entries.u[j]     = teacher[row * top + j];
-            entries.id[j]    = class_of(id, n) ? (int)id : -1;
+            const float u    = teacher[row * top + j];
+            entries.u[j]     = u;
+            entries.id[j]    = entry_of(id, n, u) ? (int)id : -1;
             entry_z[j]       = class_of(id, n) ? src[id] : 0.0f;
         }
     Sum s = sum_stretch<kThreads>(src + c0, st, f, c, t);
@@ -561,9 +564,10 @@ __global__ void __launch_bounds__(kThreads) distill_grad_kernel(
     bool mine = false;
     for (int j = t; j < top; j += kThreads) {
         const int64_t id = ids[row * top + j];
-        entries.u[j]     = teacher[row * top + j];
-        entries.id[j]    = class_of(id, n) ? (int)id : -1;
-        mine |= class_of(id, n);
+        const float u    = teacher[row * top + j];
+        entries.u[j]     = u;
+        entries.id[j]    = entry_of(id, n, u) ? (int)id : -1;
+        mine |= entry_of(id, n, u);
     }
     const float l = lse[row], scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
     const bool some = __syncthreads_or(mine);

@@ -791,7 +791,7 @@ def _distill_args(name: str, logits: Tensor, ids: Tensor, teacher: Tensor):
 
 def distill(logits: Tensor, ids: Tensor, teacher: Tensor, temperature: float = 1.0):
     """(loss, lse) of each row: T^2 times the divergence of softmax(logits / T) from softmax(teacher / T) over the row's entries, the classes ids with
-    the logits teacher of a larger network; an id outside the classes is no entry, and a row without entries has loss 0."""
+    the logits teacher of a larger network; an id outside the classes is no entry, nor is a teacher of -infinity, and a row without entries has loss 0."""
     m, n, top, pids = _distill_args("distill", logits, ids, teacher)
     loss, lse = Tensor(L.F32, (m,)), Tensor(L.F32, (m,))
     check(lib.ct_distill(logits.ptr, pids, teacher.ptr, m, n, top, float(temperature), loss.ptr, lse.ptr))

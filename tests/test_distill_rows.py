@@ -78,3 +78,35 @@ def test_loss_of_masked_classes(m, n, left, temperature, mask):
     want, want_lse, p = exact(z, ids, teacher, temperature)
     within(loss.numpy(), want.astype(np.float64), loss_off(want, temperature), "loss")
     within(lse.numpy(), want_lse.astype(np.float64), U * (3 * np.abs(want_lse.astype(np.float64)) + 16 + 3 * np.log(n)), "lse")
+
+
+PATHS = [(9, 10, 5), (9, 100, 20), (9, 400, 50), (9, 800, 100), (9, 5000, 200), (9, 40000, 7)]  # 8 and 16 threads to a row, a warp, a block, several
+
+
+@gpu
+@pytest.mark.parametrize("m,n,top", PATHS)
+def test_entries_masked_with_infinity(m, n, top):
+    """Entries whose teacher is -infinity are none: a row of nothing else has loss 0 and a gradient of zeros, whatever its logits hold."""
+    rng = np.random.default_rng(n)
+    z = rng.normal(0, 2, (m, n)).astype(np.float32)
+    ids = np.stack([rng.choice(n, top, False) for _ in range(m)])
+    teacher = rng.normal(0, 2, (m, top)).astype(np.float32)
+    teacher[0] = teacher[3] = -np.inf
+    ids[3, 1:] = -1
+    teacher[4, 1:] = -np.inf
+    teacher[5, :2] = -np.inf
+    teacher[6] = -np.inf
+    z[6] = np.nan
+    ids[7], teacher[7, 0] = -1, np.nan
+    rows = np.array([1, 2, 4, 5, 8])
+    for temperature in (2.0, 20.0):
+        loss, lse = T.distill(dev(z), dev(ids), dev(teacher), temperature)
+        grad = T.distill_grad(dev(z), dev(ids), dev(teacher), lse, temperature).numpy()
+        loss, lse = loss.numpy(), lse.numpy()
+        assert not loss[[0, 3, 6, 7]].any() and not grad[[0, 3, 6, 7]].any()
+        want, _, p = exact(z[rows], ids[rows], teacher[rows], temperature)
+        within(loss[rows], want.astype(np.float64), loss_off(want, temperature), "loss")
+        within(grad[rows], *distill_grad64(z[rows], ids[rows], p, lse[rows], np.ones(len(rows)), temperature), "dlogits")
+        some = np.where(np.isneginf(teacher), -1, ids)  # the same rows without these entries
+        other, _ = T.distill(dev(z), dev(some), dev(teacher), temperature)
+        assert other.numpy().tobytes() == loss.tobytes()
