@@ -135,6 +135,8 @@ __device__ __forceinline__ Wide wide_sums(
     }
     return s;
 }
+// The lse of a row; of one whose classes are all out, there is no distribution.
+__device__ __forceinline__ float lse_given(float lse) { return lse == -INFINITY ? NAN : lse; }
 // exp(z / T - lse) of a logit: 1 / T in two parts.  -infinity becomes a number, which neither part makes a NaN.
 __device__ __forceinline__ float probability(float z, float inv_t, float inv_t_rest, float lse) {
     asm("max.NaN.f32 %0, %0, 0fFF7FFFFF;" : "+f"(z));
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(256) distill_grad_short_kernel(
 #pragma unroll
     for (int i = 0; i < V; ++i)
         z[i] = here ? src[min(i * TPR + t, n - 1)] : 0.0f;
-    const float l = here ? lse[row] : 0.0f, given = here && dloss ? dloss[row] : 1.0f, scale = __fmul_rn(given, temperature);
+    const float l = here ? lse_given(lse[row]) : 0.0f, given = here && dloss ? dloss[row] : 1.0f, scale = __fmul_rn(given, temperature);
     const Weights w = entries.weights(inv_t);
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(kThreads) distill_grad_warp_kernel(
     if (lane < st.pieces)
         load_pieces<32>(z, reinterpret_cast<const float4 *>(src + st.head), lane, st.pieces);
     const Entries<32, kWarpEntries / 32> entries(ids + row * top, teacher + row * top, top, n, true, lane);
-    const float l = lse[row], scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
+    const float l = lse_given(lse[row]), scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
     const Weights w = entries.weights(inv_t);
     map_stretch<32, VEC>(src, dst, n, st, z, lane, [&](float v) { return w.some ? __fmul_rn(probability(v, inv_t, inv_t_rest, l), scale) : 0.0f; });
     __syncwarp();
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kThreads) distill_grad_kernel(
         entries.id[j]    = entry_of(id, n, u) ? (int)id : -1;
         mine |= entry_of(id, n, u);
     }
-    const float l = lse[row], scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
+    const float l = lse_given(lse[row]), scale = __fmul_rn(dloss ? dloss[row] : 1.0f, temperature);
     const bool some = __syncthreads_or(mine);
     map_stretch<kThreads, VEC>(src, dst, count, st, z, t, [&](float v) { return some ? __fmul_rn(probability(v, inv_t, inv_t_rest, l), scale) : 0.0f; });
     if (!some)

@@ -110,3 +110,21 @@ def test_entries_masked_with_infinity(m, n, top):
         some = np.where(np.isneginf(teacher), -1, ids)  # the same rows without these entries
         other, _ = T.distill(dev(z), dev(some), dev(teacher), temperature)
         assert other.numpy().tobytes() == loss.tobytes()
+
+
+@gpu
+@pytest.mark.parametrize("m,n,top", PATHS)
+def test_no_class_left(m, n, top):
+    """Logits that are all -infinity are no distribution: lse is -infinity, loss and gradient are NaN; 0 where the row has no entries."""
+    rng = np.random.default_rng(n)
+    z = np.full((m, n), -np.inf, np.float32)
+    z[1] = 0
+    ids = np.stack([rng.choice(n, top, False) for _ in range(m)])
+    ids[2] = -1
+    for temperature in (1e-3, 2.0, 20.0):
+        loss, lse = T.distill(dev(z), dev(ids), dev(rng.normal(0, 2, (m, top)).astype(np.float32)), temperature)
+        grad = T.distill_grad(dev(z), dev(ids), dev(np.zeros((m, top), np.float32)), lse, temperature).numpy()
+        loss = loss.numpy()
+        assert np.isneginf(np.delete(lse.numpy(), 1)).all() and np.isfinite(loss[1]) and np.isfinite(grad[1]).all()
+        assert loss[2] == 0 and not grad[2].any()
+        assert np.isnan(loss[[0, *range(3, m)]]).all() and np.isnan(grad[[0, *range(3, m)]]).all()
