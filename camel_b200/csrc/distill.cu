@@ -28,7 +28,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The largest of some logits and the sum of exp((z - top) / T); a NaN or +infinity among them shows in the sum.
+// A logit that is the largest of some or near it, and the sum of exp((z - top) / T) over them; a NaN or +infinity among them shows in the sum.
 struct Sum {
     float top, sum;
 };
@@ -38,6 +38,13 @@ __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
     // one of the two exponentials is 1; of an empty side 0
     return {top, __fadd_rn(__fmul_rn(a.sum, ex2(__fmul_rn(__fsub_rn(a.top, base), c))), __fmul_rn(b.sum, ex2(__fmul_rn(__fsub_rn(b.top, base), c))))};
 }
+template <int N> __device__ __forceinline__ float sum_about(const float (&z)[N], float base, float c) {
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        sum[i & 3] = __fadd_rn(sum[i & 3], ex2(__fmul_rn(__fsub_rn(z[i], base), c)));
+    return __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3]));
+}
 // N more logits
 template <int N> __device__ __forceinline__ void take(Sum &s, const float (&z)[N], float c) {
     float top = s.top;
@@ -45,12 +52,8 @@ template <int N> __device__ __forceinline__ void take(Sum &s, const float (&z)[N
     for (int i = 0; i < N; ++i)
         top = fmaxf(top, z[i]);
     const float base = about(top);
-    float sum[4]     = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        sum[i & 3] = __fadd_rn(sum[i & 3], ex2(__fmul_rn(__fsub_rn(z[i], base), c)));
-    s.sum = __fmaf_rn(s.sum, ex2(__fmul_rn(__fsub_rn(s.top, base), c)), __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
-    s.top = top;
+    s.sum            = __fmaf_rn(s.sum, ex2(__fmul_rn(__fsub_rn(s.top, base), c)), sum_about(z, base, c));
+    s.top            = top;
 }
 template <int TPR> __device__ __forceinline__ Sum join_lanes(Sum s, float c) {
 #pragma unroll
@@ -301,25 +304,27 @@ __global__ void __launch_bounds__(256) distill_grad_short_kernel(
 
 // 16-byte pieces of a stretch of floats at any address, from a multiple of 128 bytes on: `head` values before the first, and `tail` behind the last.
 struct Stretch {
-    int64_t head, pieces, tail;
+    int head, pieces, tail;
 };
 __device__ __forceinline__ Stretch stretch_of(const float *p, int64_t count) {
     Stretch s;
-    s.head   = min((int64_t)((32 - ((reinterpret_cast<uintptr_t>(p) >> 2) & 31)) & 31), count);
-    s.pieces = (count - s.head) / 4;
-    s.tail   = count - s.head - 4 * s.pieces;
+    s.head   = (int)min((int64_t)((32 - ((reinterpret_cast<uintptr_t>(p) >> 2) & 31)) & 31), count);
+    s.pieces = ((int)count - s.head) / 4;
+    s.tail   = (int)count - s.head - 4 * s.pieces;
     return s;
 }
 
 constexpr int kThreads = 256, kAtOnce = 4; // pieces of a thread that are on their way together
 
 // Loads without conditions (with them each would wait for the one before): the last piece again.
-template <int THREADS> __device__ __forceinline__ void load_pieces(float4 (&z)[kAtOnce], const float4 *from, int64_t i, int64_t pieces) {
+template <int THREADS> __device__ __forceinline__ void load_pieces(float4 (&z)[kAtOnce], const float4 *from, int i, int pieces) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
         z[u] = from[min(i + u * THREADS, pieces - 1)];
 }
-// The sum of a stretch by THREADS threads; z: its first pieces, on their way.
+// The sum of a stretch by THREADS threads; z: its first pieces, on their way.  A thread adds up its turns, of 16 logits, in 64 bits, about a logit that moves only
+// when one 256 times as likely comes: a move is off by 2^-22, and four of them leave nothing of what was before.  (In 32 bits and about the largest so far, lse of 2^27
+// logits that rise little by little was off by 6e-5, and now by a rounding.)
 template <int THREADS>
 __device__ __forceinline__ Sum sum_stretch(const float *src, const Stretch &st, float4 (&f)[kAtOnce], float c, int t) {
     const float *body = src + st.head;
@@ -328,7 +333,9 @@ __device__ __forceinline__ Sum sum_stretch(const float *src, const Stretch &st, 
         const float z[1] = {i < st.head ? src[i] : body[4 * st.pieces + i - st.head]};
         take(s, z, c);
     }
-    for (int64_t i = t; i < st.pieces;) {
+    const float reach = __fdiv_rn(8.0f, c);
+    double sum        = (double)s.sum;
+    for (int i = t; i < st.pieces;) {
         float z[4 * kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
@@ -339,8 +346,16 @@ __device__ __forceinline__ Sum sum_stretch(const float *src, const Stretch &st, 
         i += THREADS * kAtOnce;
         if (i < st.pieces)
             load_pieces<THREADS>(f, reinterpret_cast<const float4 *>(body), i, st.pieces);
-        take(s, z, c);
+        float top = z[0];
+#pragma unroll
+        for (int q = 1; q < 4 * kAtOnce; ++q)
+            top = fmaxf(top, z[q]);
+        top              = top > __fadd_rn(s.top, reach) ? top : s.top;
+        const float base = about(top), part = sum_about(z, base, c);
+        sum   = fma(sum, (double)ex2(__fmul_rn(__fsub_rn(s.top, base), c)), (double)part);
+        s.top = top;
     }
+    s.sum = (float)sum;
     return s;
 }
 // f(z) of each logit of a stretch, written to a row that lies as far from 16 bytes (VEC), or at any address.
@@ -348,17 +363,17 @@ template <int THREADS, bool VEC, typename F>
 __device__ __forceinline__ void map_stretch(const float *src, float *dst, int64_t count, const Stretch &st, float4 (&z)[kAtOnce], int t, F &&f) {
     if (VEC) {
         for (int q = t; q < st.head + st.tail; q += THREADS) {
-            const int64_t i = q < st.head ? q : st.pieces * 4 + q;
+            const int i = q < st.head ? q : st.pieces * 4 + q;
             dst[i]          = f(src[i]);
         }
         const float4 *from = reinterpret_cast<const float4 *>(src + st.head);
         float4 *to         = reinterpret_cast<float4 *>(dst + st.head);
-        for (int64_t i = t; i < st.pieces;) {
+        for (int i = t; i < st.pieces;) {
             float4 d[kAtOnce];
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u)
                 d[u] = make_float4(f(z[u].x), f(z[u].y), f(z[u].z), f(z[u].w));
-            const int64_t now = i;
+            const int now = i;
             i += THREADS * kAtOnce;
             if (i < st.pieces)
                 load_pieces<THREADS>(z, from, i, st.pieces);

@@ -445,8 +445,9 @@ ct_status ct_gated_scan_grad(
  * An id outside 0 .. n-1 is no entry (a row may have fewer than top); a row without entries is padding: its loss is 0, whatever its logits hold.  Entries of
  * the same class count each.  An entry of weight 0 (teacher -infinity) is none either: a row of nothing else is padding.  Otherwise infinities and NaN as for
  * ct_dense_cross_entropy (of a row with entries whose classes are all out, loss and gradient are NaN).  T is the temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null.
- * The loss is off by about 2^-16 of the larger of 1 and itself, at any temperature and however far from zero the logits are (from T = 10^5 on by T^2 2^-49, which
- * is more): where T is above 4 and the divergence below 1/16, as it is when the entries are all classes, a row is summed in 64 bits. */
+ * The sum in lse is off by some 2^-20 of itself, of any number of classes in any order.  The loss is off by about 2^-16 of the larger of 1 and itself, at any
+ * temperature and however far from zero the logits are (from T = 10^5 on by T^2 2^-49, which is more): where T is above 4 and the divergence below
+ * 1/16, as it is when the entries are all classes, a row is summed in 64 bits. */
 ct_status ct_distill(
     const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, int64_t m, int64_t n, int64_t top, double temperature, float *loss_dev,
     float *lse_dev);

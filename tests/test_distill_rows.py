@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import camel_b200._lib as L
 from camel_b200 import tensor as T
 from test_layers import U, dev, within
 from test_sequences import distill_grad64
@@ -128,3 +129,29 @@ def test_no_class_left(m, n, top):
         assert np.isneginf(np.delete(lse.numpy(), 1)).all() and np.isfinite(loss[1]) and np.isfinite(grad[1]).all()
         assert loss[2] == 0 and not grad[2].any()
         assert np.isnan(loss[[0, *range(3, m)]]).all() and np.isnan(grad[[0, *range(3, m)]]).all()
+
+
+@gpu
+@pytest.mark.parametrize("order", ["first", "last", "rising", "falling"])
+@pytest.mark.parametrize("m,n", [(1, 2 ** 27), (700, 2 ** 17), (3, 2 ** 22 + 3)])
+def test_sums_of_long_rows(m, n, order):
+    """lse does not depend on how many classes a row has, nor on where its likeliest one stands."""
+    import torch
+
+    z = torch.full((n,), -1.2345, device="cuda")
+    if order in ("rising", "falling"):
+        z = torch.linspace(-30, 0, n, device="cuda")
+    if order == "falling":
+        z = z.flip(0)
+    if order in ("first", "last"):
+        z[0 if order == "first" else -1] = 0
+    # in pieces: a sum of 2^27 doubles, as torch adds them up, is off by less than 2^-40
+    want = torch.logsumexp(torch.stack([torch.logsumexp(p.double(), 0) for p in z.split(2 ** 22)]), 0).item()
+    rows = z.expand(m, n).contiguous()
+    lse = torch.empty(m, device="cuda")
+    torch.cuda.synchronize()
+    L.check(L.lib.ct_distill(rows.data_ptr(), None, None, m, n, 0, 1.0, None, lse.data_ptr()))
+    T.check_async()
+    # an exponential 4 U, its argument's 3 U of up to 2 in the mean, 16 terms 6 U, four moves and eleven joins of 4 U and two roundings each; lse three roundings
+    off = U * (4 + 6 + 6 + 15 * 6 + 3 * abs(want))
+    within(lse.cpu().numpy(), np.full(m, want), off, "lse")
