@@ -18,11 +18,12 @@ namespace ct {
 // Device-side error words, read back by the entry points that must report them.
 //   words 0-1  data-dependent exceptions of one call: cleared by the entry point that checks them,
 //              read back (with a synchronisation) before it returns.
-//   word 2     sticky: written by a contraction kernel whose bounded wait ran out and by nothing
-//              else; only ct_check() (or a *_host entry point that reports it) clears it.  While it
-//              is set every later contraction kernel returns at once, so that a failed launch is
-//              not followed by products of its undefined output; no entry point clears it on the
-//              way in, and the failure is therefore still there when the host next looks.
+//   word 2     sticky: written by a contraction kernel or a gated scan whose bounded wait ran out
+//              and by nothing else; only ct_check() (or a *_host entry point that reports it) clears
+//              it.  While it is set every later contraction kernel returns at once, so that a failed
+//              launch is not followed by products of its undefined output (a scan, like the other
+//              operators, runs as ever); no entry point clears it on the way in, and the failure is
+//              therefore still there when the host next looks.
 enum FlagWord : int {
     FLAG_DIV_ZERO   = 0, // a divisor was 0 (reference: "Division by zero")
     FLAG_LOG_DOMAIN = 1, // an input of log was <= 0

@@ -220,6 +220,14 @@ __device__ __forceinline__ void tma_load_5d(
         : "memory");
 }
 
+// ---- copies of a thread of its own -------------------------------------------------------
+
+__device__ __forceinline__ void cp_async_4(uint32_t dst_smem, const float *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst_smem), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
 // ---- tensor memory ----------------------------------------------------------------------
 
 // Whole-warp instructions (.sync.aligned): call from all 32 lanes of one warp.
@@ -300,6 +308,11 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void st_cluster_f4(uint32_t cluster_addr, float4 v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+// 16 bytes on their way there, which the barrier (of that CTA too) counts when they are there.
+__device__ __forceinline__ void st_async_d2(uint32_t cluster_addr, uint32_t cluster_bar, double2 v) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr), "d"(v.x), "d"(v.y), "r"(cluster_bar)
                  : "memory");
 }
 // The address of the same shared-memory location in the leader.

@@ -102,8 +102,8 @@ ct_status ct_get_device(int *device_host);
 ct_status ct_set_stream(void *stream);
 ct_status ct_sync(void);
 /* Synchronises and reports errors that kernels of earlier asynchronous calls raised on the
- * device (CT_ERR_TIMEOUT: a bounded wait in a contraction kernel ran out; its output is then
- * undefined).  The record is sticky: no entry point clears it on the way in, contraction kernels
+ * device (CT_ERR_TIMEOUT: a bounded wait in a contraction kernel or a gated scan ran out; its output
+ * is then undefined).  The record is sticky: no entry point clears it on the way in, contraction kernels
  * launched after it return at once without writing, and it stays until ct_check (or a *_host
  * entry point) has reported it once - so a failure between two checks is never lost, however many
  * calls were enqueued after it.  ct_matmul_f32_static keeps its own status word (status_dev) and
