@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
     griddep_wait();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t range = blockIdx.x / strips;
-    const int64_t c0     = (int64_t)(blockIdx.x - range * strips) * 128, c1 = c0;
+    const int64_t c0     = (int64_t)(blockIdx.x - range * strips) * 128;
     const int here = (int)((n - 1 - range) / apart) + 1; // row range + r apart is its row r
     uint32_t place[TURNS]; // the token's row of the block, and behind the 16th bit its place among the warp's tokens of that row
 #pragma unroll
@@ -574,19 +574,19 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
             order[begins[place[i] & 0xffff] + counts[warp][place[i] & 0xffff] + (place[i] >> 16)] = (uint16_t)((warp * TURNS + i) * 32 + lane);
     __syncthreads();
     auto in_strip = [&](int q) { return VEC ? lane * 4 + q : q * 32 + lane; };
-    auto add      = [&](uint32_t first, uint32_t last, int64_t c1, double (&to)[4]) {
+    auto add      = [&](uint32_t first, uint32_t last, double (&to)[4]) {
         for (uint32_t i = first; i < last; i += AT_ONCE) {
             float v[AT_ONCE][4];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
                 const float *src = dout + (int64_t)order[min(i + u, last - 1)] * k;
                 if (VEC) {
-                    const float4 f = *reinterpret_cast<const float4 *>(src + min(c1 + in_strip(0), k - 4));
+                    const float4 f = *reinterpret_cast<const float4 *>(src + min(c0 + in_strip(0), k - 4));
                     v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        v[u][q] = src[min(c1 + in_strip(q), k - 1)];
+                        v[u][q] = src[min(c0 + in_strip(q), k - 1)];
                 }
             }
 #pragma unroll
@@ -601,29 +601,29 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
         const uint32_t first = begins[r], last = begins[r + 1];
         if (last - first > kAloneTokens)
             continue;
-        float *to = dtable + (range + (int64_t)r * apart) * k + c1;
+        float *to = dtable + (range + (int64_t)r * apart) * k + c0;
         if (first == last) {
             if (VEC) {
-                if (c1 + in_strip(0) < k)
+                if (c0 + in_strip(0) < k)
                     __stcs(reinterpret_cast<float4 *>(to + in_strip(0)), make_float4(0.0f, 0.0f, 0.0f, 0.0f));
             } else {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (c1 + in_strip(q) < k)
+                    if (c0 + in_strip(q) < k)
                         __stcs(to + in_strip(q), 0.0f);
             }
             continue;
         }
         double all[4] = {};
-        add(first, last, c1, all);
+        add(first, last, all);
         if (VEC) {
-            if (c1 + in_strip(0) < k)
+            if (c0 + in_strip(0) < k)
                 __stcs(reinterpret_cast<float4 *>(to + in_strip(0)),
                        make_float4((float)(all[0] * scale), (float)(all[1] * scale), (float)(all[2] * scale), (float)(all[3] * scale)));
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (c1 + in_strip(q) < k)
+                if (c0 + in_strip(q) < k)
                     __stcs(to + in_strip(q), (float)(all[q] * scale));
         }
     }
@@ -631,17 +631,17 @@ __global__ void __launch_bounds__(256) embedding_grad_few_kernel(
         const int r          = many[i];
         const uint32_t first = begins[r], count = begins[r + 1] - first;
         double all[4]        = {};
-        add(first + count * warp / 8, first + count * (warp + 1) / 8, c1, all);
+        add(first + count * warp / 8, first + count * (warp + 1) / 8, all);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             part[warp][in_strip(q)] = all[q];
         __syncthreads();
-        if (t < 128 && c1 + t < k) {
+        if (t < 128 && c0 + t < k) {
             double whole = 0.0;
 #pragma unroll
             for (int w = 0; w < 8; ++w)
                 whole += part[w][t];
-            dtable[(range + (int64_t)r * apart) * k + c1 + t] = (float)(whole * scale);
+            dtable[(range + (int64_t)r * apart) * k + c0 + t] = (float)(whole * scale);
         }
         __syncthreads();
     }

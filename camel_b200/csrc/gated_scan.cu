@@ -617,8 +617,9 @@ ct_status ct_gated_scan_grad(
         constexpr int W = decltype(warps)::value;
         switch (from) {
         case TILES:
-            if (W == 8 && scan_groups(from, batch, channels) * 6 > st->sm_count) // (see Pieces)
-                return launch_scan_grad<W, TILES, W == 4 ? 2 : 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
+            if constexpr (W == 8) // (see Pieces)
+                if (scan_groups(from, batch, channels) * 6 > st->sm_count)
+                    return launch_scan_grad<W, TILES, 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
             return launch_scan_grad<W, TILES, W == 2 ? 1 : 2>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
         case ROWS:
             return launch_scan_grad<W, ROWS, 1>(st, gate, value, state0, lengths, out, dout, dstate, batch, steps, channels, dgate, dvalue, dstate0);
