@@ -205,6 +205,12 @@ inline int64_t blocks_for(int64_t turns, int64_t at_once, int64_t chain) {
     return turns < blocks ? turns : blocks;
 }
 
+// Blocks that a cluster may have: 16 where the device has room for them, which it is asked for; CAMEL_TENSOR_PORTABLE_CLUSTERS=1: 8, which every device has.
+inline int cluster_limit() {
+    static const bool portable = getenv("CAMEL_TENSOR_PORTABLE_CLUSTERS") != nullptr;
+    return portable ? 8 : 16;
+}
+
 // Whether no 128-byte line holds values of both: else what a kernel's loads of one bring into a first-level cache of the other is stale for a successor that
 // was launched before them (see launch_dependent).
 inline bool lines_apart(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {

@@ -454,7 +454,7 @@ template <auto KERNEL, int W> ct_status scan_blocks(const DeviceState *st, int s
         }
         mine[1] = 1;
     }
-    *blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kMostBlocks<W>, pieces));
+    *blocks = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(kMostBlocks<W>, cluster_limit()), pieces));
     while (*blocks > 1 && mine[*blocks] < groups)
         --*blocks;
     return CT_OK;

@@ -32,6 +32,8 @@
  *    CAMEL_TENSOR_DEVICES = "2" or "0,1,2,3" (the process takes the entry at index LOCAL_RANK,
  *    else CAMEL_TENSOR_RANK, else 0, modulo the list's length); ct_set_precision / ct_set_device
  *    override them, a malformed value makes the first call fail with CT_ERR_INVALID.
+ *    CAMEL_TENSOR_PORTABLE_CLUSTERS=1: clusters of 8 blocks at most, as on a device (or a part of
+ *    one) that has no room for larger ones.
  */
 #ifndef CAMEL_TENSOR_B200_H
 #define CAMEL_TENSOR_B200_H
