@@ -610,11 +610,13 @@ __global__ void __launch_bounds__(kThreads) distill_grad_kernel(
     }
 }
 
-// Whether a warp takes a row, or a block; measured (us, blocks and warps; forward, then backward): 1000 x 600 13 and 9, 12 and 9; 2000 x 1000 16 and 11,
-// 17 and 10; 1000 x 4000 14 and 15, 14 and 17; 4700 x 4000 29 and 23, 37 and 35; 60000 x 1500 250 and 88, 324 and 147; 20000 x 8000 150 and 127, 252 and 261;
-// 20000 x 16000 232 and 239, 447 and 502.
-bool distill_by_warps(const DeviceState *st, int64_t m, int64_t n, int64_t top) {
-    return top <= kWarpEntries && (n <= 1024 || (n <= 6000 && m >= st->sm_count * 16));
+// Whether a warp takes a row, or a block; measured in line (us, 20 entries; a warp and a block, forward and backward): 1000 x 600 6.1 and 7.9, 5.6 and 8.7; 2000 x 1000
+// 5.6 and 11.8, 5.6 and 13.3; 300 x 4000 5.7 and 5.8, 6.0 and 5.1 (L2 flushed 13 and 10, 14 and 10); 1000 x 4000 5.6 and 7.9, 6.3 and 9.6 (14 and 13, 17 and 16);
+// 1500 x 4000 7.5 and 10.2, 8.4 and 11.0; 2000 x 6000 11.2 and 13.8, 15.2 and 19.4; 4700 x 4000 11.6 and 21.3, 25.7 and 33.5; 60000 x 1500 76 and 265, 117 and 317;
+// 20000 x 6000 82 and 125, 161 and 177.  Backward a block from there on, forward from twice that: 20000 x 8000 107 and 130, 213 and 200; 20000 x 12000 155 and 173,
+// 320 and 289; 20000 x 16000 210 and 212, 435 and 385; with few rows a block too: 2400 x 8000 18.5 and 16.5, 29.6 and 28.9, but 3000 x 12000 29 and 35, 52 and 50.
+bool distill_by_warps(const DeviceState *st, int64_t m, int64_t n, int64_t top, bool backward) {
+    return top <= kWarpEntries && (n <= 1024 || (n <= 6000 && m >= st->sm_count * 10) || (!backward && n <= 12000 && m >= st->sm_count * 20));
 }
 
 ct_status check_distill(const char *name, int64_t m, int64_t n, int64_t top, double temperature) {
@@ -658,15 +660,15 @@ ct_status ct_distill(
         CT_LAUNCH_CHECK("distill_short");
         return CT_OK;
     };
-    // (us, 60000 rows; 8 threads with 4 values each, 8 with 16, 16 with 32, a warp; forward, then backward: 10 classes 12, 18, 39, 53, 12, 18, 45, 41; 128 classes
-    // -, 18, 39, 55, -, 25, 47, 45; 512 -, -, 43, 57, -, -, 51, 53)
+    // (us in line, 60000 rows; 8 threads with 4 values each, 8 with 16, 16 with 32, a warp; forward, then backward: 10 classes, 5 entries 8.5, 13.9, 36, 40, 7.5, 14.2,
+    // 41, 33; 128 classes, 20 entries -, 14.8, 37, 43, -, 21, 47, 45; 512 classes, 64 entries -, -, 44, 49, -, -, 70, 83)
     if (n <= 32 && top <= 16)
         return short_rows(distill_short_kernel<8, 4, 2>, 8);
     if (n <= 128 && top <= 32)
         return short_rows(distill_short_kernel<8, 16, 4>, 8);
     if (n <= 512 && top <= 64)
         return short_rows(distill_short_kernel<16, 32, 4>, 16);
-    if (distill_by_warps(st, m, n, top))
+    if (distill_by_warps(st, m, n, top, false))
         return short_rows(distill_warp_kernel, 32);
     int parts = 1;
     // 131072 classes, 1, 2, 4 and 8 blocks to a row: 31, 19, 14, 10 us (1 row), 33, 22, 17, 16 (64), 37, 28, 25, 28 (148), 47, 40, 44, 47 (300), 70, 71, 76, 76 (600)
@@ -704,7 +706,7 @@ ct_status ct_distill_grad(
     if (n <= 512 && top <= 64)
         return short_rows(distill_grad_short_kernel<16, 32, 4>, 16);
     const bool alike = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15u) == 0; // 16 bytes of one are 16 of the other
-    if (distill_by_warps(st, m, n, top))
+    if (distill_by_warps(st, m, n, top, true))
         return alike ? short_rows(distill_grad_warp_kernel<true>, 32) : short_rows(distill_grad_warp_kernel<false>, 32);
     // Parts of about 16384 classes, or of less where rows are few; measured with 1, 2, 3, 4 and 8: 4096 x 50257 279, 266, 258, 264, 301 us; 4096 x 131072 689, 675,
     // 677, 659, 641; 1500 x 32003 78, 72, 74, 74, 82; 8000 x 16000 168, 173, 215, 201, 344; 1 x 131072 33 with one, 8 with 16 and 32

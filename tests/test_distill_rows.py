@@ -5,7 +5,7 @@ import pytest
 import camel_b200._lib as L
 from camel_b200 import tensor as T
 from test_layers import U, dev, within
-from test_sequences import distill_grad64
+from test_sequences import distill64, distill_grad64, distill_inputs
 
 gpu = pytest.mark.gpu
 
@@ -155,3 +155,16 @@ def test_sums_of_long_rows(m, n, order):
     # an exponential 4 U, its argument's 3 U of up to 2 in the mean, 16 terms 6 U, four moves and eleven joins of 4 U and two roundings each; lse three roundings
     off = U * (4 + 6 + 6 + 15 * 6 + 3 * abs(want))
     within(lse.cpu().numpy(), np.full(m, want), off, "lse")
+
+
+@gpu
+@pytest.mark.parametrize("m,n,top", [(1479, 3001, 5), (1480, 3001, 5), (1480, 6000, 128), (1480, 6001, 9), (2959, 7001, 20), (2960, 7001, 20), (2960, 12000, 3),
+                                     (2960, 12001, 3), (2960, 7000, 129)])
+def test_rows_where_warps_and_blocks_meet(m, n, top):
+    z, ids, teacher, dloss = distill_inputs(m, n, top, 4)
+    loss, lse = T.distill(dev(z), dev(ids), dev(teacher), 2.0)
+    p, want_lse, want, off_lse, off = distill64(z, ids, teacher, 2.0)
+    within(lse.numpy(), want_lse, off_lse, "lse")
+    within(loss.numpy(), want, off, "loss")
+    got = T.distill_grad(dev(z), dev(ids), dev(teacher), lse, 2.0, dev(dloss))
+    within(got.numpy(), *distill_grad64(z, ids, p, lse.numpy(), dloss, 2.0), "dlogits")
