@@ -3,11 +3,13 @@
 //   p = softmax(teacher / T) over a row's entries, q = softmax(z / T) over its classes
 //   loss = T^2 sum p (log p - log q),  dz[c] = dloss T (q[c] - the sum of p over the entries of class c)
 //
-// Both are bound by memory: the logits are read once (4 bytes each), and on the way back written once (8).  Forward, a thread keeps the
-// maximum of its logits and the sum of exponentials about it, which meet at the end; a row of a small batch is shared by the blocks of a cluster.
+// Both are bound by memory: the logits are read once (4 bytes each), and on the way back written once (8).  Forward, a thread keeps a
+// logit near the largest of its own and the sum of exponentials about it, which meet at the end; a row of a small batch is shared by the blocks of a cluster.
 // Backward, lse is given: a row is q times a factor, from which its block takes the entries' p where it has written them.
-// Measured (L2 flushed): 4096 x 131072 with 64 entries 311 to 341 us (2.15 GB, 0.96 to 1.06 of a copy), 64 x 32003 5.6 us; gradient 4096 x 50257 256 to 278 us
-// (1.65 GB, 0.91 to 0.98), 60000 x 10 6.9 us (9 MB: a launch, and the loads one after the other).
+// Measured (L2 flushed): 4096 x 131072 with 64 entries 318 us (2.15 GB, 1.03 of a copy), 64 x 32003 5.7 us; gradient 4096 x 50257 259 us (1.65 GB, 0.97),
+// 60000 x 10 6.9 us (9 MB: a launch and a round of loads).  Rows of 33 to 8000 classes are further from a copy: 60000 x 128 15 us in line (46 MB, 0.48), x 1500 76
+// (375 MB, 0.75), backward 21 (77 MB, 0.56) and 117 (735 MB, 0.96): a row's loads, its lanes' join and its entries come one after the other, and nothing of the next meanwhile.
+// Times at the rules below are of a lone call between two events, L2 flushed, with the events' own 4 us or so, unless in line is said: call behind call.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 

@@ -1,14 +1,16 @@
 // Embedding lookup, and the gradient of its table.
 //
-//   out[i] = scale table[ids[i]];   dtable[v] = scale (sum of dout[i] over the i with ids[i] = v), in an order that the ids decide
+//   out[i] = scale table[ids[i]];   dtable[v] = scale (sum of dout[i] over the i with ids[i] = v)
 //
 // Both are bound by memory: a lookup reads a row and writes one, the gradient reads dout once and writes every row of the table.
 // Gradient: the tokens are sorted by id (stable, so that sums have one order), then warps walk the tokens and the rows together.  Rows
 // without a token are as many as there are stores of zeros, rows with thousands as many as there are loads, so what is cut into equal slices is
 // the merged list of both: each token, and behind its last token the end of each row.  A row that lies across slices leaves a partial
-// sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once.
+// sum in each, which a third kernel adds up.  Few tokens are found by each block for its own rows, in one launch.  Sums are kept in 64 bits and rounded once; their
+// order follows from the ids, the sizes and the device, and not from when a block runs.
 // Measured (L2 flushed): 32768 rows of 50257 x 2048 59 to 61 us (348 MB, 0.88 to 0.90 of a copy); gradient of 16384 tokens in the same table 111 us (546 MB,
-// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 12 us in one (11 MB; each block's chain of loads), of 1000 in 100 x 64 8.
+// 0.75: sorting 15, sums 91, joining the rest), of 1537 in 2050 x 771 12 us in one (11 MB; each block's chain of loads), of 1000 in 100 x 64 5 in line.
+// Times at the rules below are of a lone call between two events, L2 flushed, with the events' own 4 us or so, unless in line is said: call behind call.
 #include "common.cuh"
 #include "tc_ptx.cuh"
 

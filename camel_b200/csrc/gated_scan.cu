@@ -14,9 +14,11 @@
 // what they add, b, and their 1 - A is summed up by itself, S' = a S + (1 - a).  A is 1 - S in 64 bits, or, from where S has more than 1/2, the
 // product, which is then small and has its digits.  Between pieces states are in 64 bits.
 //
-// Measured (L2 flushed): one sequence of 65536 steps and 512 channels 74 to 80 us forward (403 MB, 0.77 to 0.83 of a copy; a tile waits for what the blocks before
-// send) and 138 backward; 8 of 2048 steps and 2048 channels 64 to 72 and 126 to 137 us (805 MB, 0.90 to 0.98); 7 of up to 1537 steps and 771
-// channels backward 48 to 56 us (166 MB, 0.45 to 0.53: rows that begin anywhere lie in two lines of 128 bytes, 768 channels take 44); one step of 64 x 2048 5 us.
+// Measured (L2 flushed, and in line): one sequence of 65536 steps and 512 channels 78 to 81 us forward, in line 74 (403 MB, 0.76 to 0.83 of a copy; a tile waits for
+// what the blocks before send), and 138, 134 backward; 8 of 2048 steps and 2048 channels 72 and 63, backward 127 to 133 and 126 us (805 MB, 0.92 to 0.98); 7 of up to
+// 1537 steps and 771 channels backward 48 and 50 us (166 MB, 0.5: rows that begin anywhere lie in two lines of 128 bytes; in line 772 channels take 38, 768 32); one
+// step of 64 x 2048 5 us.
+// Times at the rules below are of a lone call between two events, L2 flushed, with the events' own 4 us or so, unless in line is said: call behind call.
 #include "common.cuh"
 #include "fastmath.cuh"
 #include "gate.cuh"

@@ -122,7 +122,8 @@ uint64_t ct_launch_count(void);
  * `kernel` ("gemm_tc", "gemm_prepass", "gemm_skinny", "gemm_splitk_reduce", "weights_pack",
  * "conv_prepass", "conv_small_c", "im2col", "elementwise", "reduce", "softmax", "transpose",
  * "concat", "maxpool", "layer_norm", "layer_norm_grad", "dense_gated", "dense_gated_grad", "cross_entropy",
- * "cross_entropy_grad"); NULL reads all. */
+ * "cross_entropy_grad", "embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "distill",
+ * "distill_grad"); NULL reads all. */
 ct_status ct_profile_enable(int on);
 ct_status ct_profile_read(const char *kernel, double *total_ms_host, uint64_t *launches_host);
 /* The tensor pipe's own ceiling, measured: every SM issues `mma_groups` x 4 tcgen05.mma of
@@ -417,8 +418,8 @@ ct_status ct_dense_cross_entropy_grad(
 ct_status ct_embedding(
     const float *table_dev, const int64_t *ids_dev, int64_t m, int64_t n, int64_t k, double scale, float *out_dev);
 /* The gradient of its table from the gradient dout [m][k] of its output: dtable[v] = scale * (sum of dout[i] over the i with ids[i] = v), every row
- * of dtable [n][k] written, zeros where no id is.  Rows of padding take no part, whatever dout holds there.  Sums are in 64 bits, in an order
- * that the ids alone decide, and rounded once: the same call gives the same bytes. */
+ * of dtable [n][k] written, zeros where no id is.  Rows of padding take no part, whatever dout holds there.  Sums are in 64 bits and rounded
+ * once, in an order that the ids, the sizes and the device decide: the same call on the same device gives the same bytes. */
 ct_status ct_embedding_grad(
     const int64_t *ids_dev, const float *dout_dev, int64_t m, int64_t n, int64_t k, double scale, float *dtable_dev);
 
@@ -445,8 +446,9 @@ ct_status ct_gated_scan_grad(
  * with the teacher's logits teacher[i][..].  With p = softmax(teacher / T) over the row's entries and q = softmax(z / T) over its classes
  *   loss[i] = T^2 * (sum over entries of p * (log p - log q[class])),   lse[i] = log(sum over classes of exp(z / T))
  * An id outside 0 .. n-1 is no entry (a row may have fewer than top); a row without entries is padding: its loss is 0, whatever its logits hold.  Entries of
- * the same class count each.  An entry of weight 0 (teacher -infinity) is none either: a row of nothing else is padding.  Otherwise infinities and NaN as for
- * ct_dense_cross_entropy (of a row with entries whose classes are all out, loss and gradient are NaN).  T is the temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null.
+ * the same class count each.  An entry of weight 0 (teacher -infinity) is none either: a row of nothing else is padding.  (One whose p rounds to 0 in
+ * float32 adds nothing.)  Otherwise infinities and NaN as for ct_dense_cross_entropy; in a row with entries whose classes are all out, loss and
+ * gradient are NaN.  T is the temperature, from 1e-6 to 1e6, rounded to float32; top is at most 1024; n >= 1.  loss or lse may be null.
  * The sum in lse is off by some 2^-20 of itself, of any number of classes in any order.  The loss is off by about 2^-16 of the larger of 1 and itself, at any
  * temperature and however far from zero the logits are (from T = 10^5 on by T^2 2^-49, which is more): where T is above 4 and the divergence below
  * 1/16, as it is when the entries are all classes, a row is summed in 64 bits. */
@@ -455,8 +457,9 @@ ct_status ct_distill(
     float *lse_dev);
 /* Its gradient, with lse as the forward call left it and the gradient dloss [m] of the losses (null: ones):
  *   dlogits[i][c] = dloss[i] * T * (exp(z[c] / T - lse[i]) - (sum of p over the row's entries of class c)), zeros in rows without entries.
- * The exponential q is off by some 2^-22 (1 + |z / T - lse|) of itself (0 below 2^-126), and as lse is rounded to float32 by 2^-24 |lse| more; dlogits by T times that.
- * Where p is near q a difference of 1 in the logits is a difference of about q in dlogits / dloss: at T = 10^4 that is off by 1 % or so, at 10^6 it is lost.  dlogits may be logits itself. */
+ * The exponential q is off by some 2^-22 (1 + |z / T - lse|) of itself (0 below 2^-126), and as lse is rounded to float32 by 2^-24 |lse| more;
+ * dlogits by T times that.  Where p is near q a difference of 1 in the logits is one of about q in dlogits / dloss: at T = 10^4 that is off by
+ * 1 % or so, at 10^6 it is lost.  dlogits may be logits itself. */
 ct_status ct_distill_grad(
     const float *logits_dev, const int64_t *ids_dev, const float *teacher_dev, const float *lse_dev, const float *dloss_dev, int64_t m, int64_t n,
     int64_t top, double temperature, float *dlogits_dev);
