@@ -22,7 +22,7 @@ int main(int argc, char **argv) {
     const int tiles        = argc > 1 ? atoi(argv[1]) : 40;
     const std::string what = argc > 2 ? argv[2] : "nothing";
     const int when         = argc > 3 ? atoi(argv[3]) : 6;
-    kWaitBudgetNs          = (what == "nothing" ? 20000 : 200) * 1000000ull;
+    kWaitBudgetNs          = (what == "nothing" ? 20000 : 400) * 1000000ull;
     std::vector<Memory> memory(kBlocks);
     uint32_t flags[kBlocks][4] = {};
     double states[kBlocks]     = {};
@@ -45,7 +45,7 @@ int main(int argc, char **argv) {
         values.at(Chain{0, 0, last, true}, 0, 32, last, t0);
         const bool mine = block == 1 && warp == 1;
         auto fetch      = [&](int i) {
-            arrays.map[1].after_ms = mine && i == when ? (what == "lost" ? -1 : what == "late" ? 320 : 0) : 0;
+            arrays.map[1].after_ms = mine && i == when ? (what == "lost" ? -1 : what == "late" ? 640 : 0) : 0;
             values.fetch(i, t0 + i * tile, -1, last - (t0 + i * tile), last);
         };
         if (warp < kWalk)
@@ -66,7 +66,7 @@ int main(int argc, char **argv) {
                 values.wait(i, last);
                 fetch(i + kDepth);
                 if (what == "slow" && mine && i == when)
-                    std::this_thread::sleep_for(std::chrono::milliseconds(2000));
+                    std::this_thread::sleep_for(std::chrono::milliseconds(2500));
                 return make_double2(0.5, value(i * kBlocks * kWalk + block * kWalk + warp));
             },
             [&](int i, const Steps &s, float) { right &= s.tile == i; });
